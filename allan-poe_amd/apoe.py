@@ -3,6 +3,9 @@
 Arrays may be numpy arrays (host) or torch tensors (host or the context's GPU); the
 library copies as needed. There is no CPU fallback: if the HIP library is missing or a
 call fails, an exception is raised.
+
+The operators that fit a query adapter (`softmax_loss`, `orthogonalize`, `gated_residual`) take torch tensors on the context's
+GPU, write torch tensors and return without waiting; their work is ordered with torch's current stream.
 """
 import ctypes as C
 import os
@@ -36,6 +39,14 @@ class SearchStats(C.Structure):
                 ("nnz_sparse", C.c_uint64), ("nnz_bm25", C.c_uint64), ("dense_rows", C.c_uint64), ("algo_bytes", C.c_uint64)]
 
 
+class SoftmaxLossArgs(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("n_queries", C.c_uint32), ("n_rows", C.c_uint32), ("dim", C.c_uint32),
+                ("q", C.c_void_p), ("rows", C.c_void_p), ("corpus", C.c_void_p),
+                ("q_stride", C.c_uint64), ("rows_stride", C.c_uint64), ("grad_q_stride", C.c_uint64), ("grad_rows_stride", C.c_uint64),
+                ("t_off", C.c_void_p), ("t_idx", C.c_void_p), ("t_val", C.c_void_p), ("live", C.c_void_p), ("weight", C.c_void_p),
+                ("scale", C.c_float), ("loss", C.c_void_p), ("lse", C.c_void_p), ("grad_q", C.c_void_p), ("grad_rows", C.c_void_p)]
+
+
 EXPORTS = [
     "apoe_last_error_string", "apoe_ctx_create", "apoe_ctx_destroy", "apoe_ctx_synchronize", "apoe_corpus_create", "apoe_corpus_create_without",
     "apoe_corpus_destroy", "apoe_corpus_info", "apoe_corpus_bytes", "apoe_corpus_pair_bytes", "apoe_corpus_make_half_rows", "apoe_queries_create", "apoe_queries_destroy",
@@ -44,6 +55,7 @@ EXPORTS = [
     "apoe_knn_download", "apoe_knn_upload", "apoe_knn_download_reverse", "apoe_knn_upload_reverse", "apoe_knn_set_prune_form", "apoe_prune", "apoe_prune_download", "apoe_finalize_graph",
     "apoe_knn_elapsed_ms", "apoe_knn_counters", "apoe_knn_read_counters", "apoe_graph_create", "apoe_graph_destroy", "apoe_graph_info", "apoe_graph_download",
     "apoe_search", "apoe_search_noalloc",
+    "apoe_ctx_create_on_stream", "apoe_ctx_stream", "apoe_softmax_loss",
 ]
 
 
@@ -99,13 +111,32 @@ def _ptr(a, dtype):
 
 
 class Context:
-    def __init__(self, device=0):
+    """stream: a torch stream (or the integer of a HIP stream) that the context's work is put on; by default it has a stream
+    of its own."""
+
+    def __init__(self, device=0, stream=None):
         self.h = C.c_void_p()
-        _check(lib().apoe_ctx_create(C.c_int(device), C.byref(self.h)))
+        if stream is None:
+            _check(lib().apoe_ctx_create(C.c_int(device), C.byref(self.h)))
+        else:
+            self._stream_kept = stream  # outlives the context
+            handle = int(getattr(stream, "cuda_stream", stream))
+            _check(lib().apoe_ctx_create_on_stream(C.c_int(device), C.c_void_p(handle), C.byref(self.h)))
+        out = C.c_void_p()
+        _check(lib().apoe_ctx_stream(self.h, C.byref(out)))
+        self.stream = out.value or 0
+        self._torch_stream = None
         self.device = device
 
     def synchronize(self):
         _check(lib().apoe_ctx_synchronize(self.h))
+
+    def torch_stream(self):
+        """The context's stream as torch sees it."""
+        if self._torch_stream is None:
+            import torch
+            self._torch_stream = torch.cuda.ExternalStream(self.stream, device=self.device) if self.stream else torch.cuda.default_stream(self.device)
+        return self._torch_stream
 
     def close(self):
         if self.h:
@@ -420,3 +451,120 @@ def search_noalloc(ctx, corpus, queries, graph, w3, cands, out_ids, out_dist, kg
     _check(lib().apoe_search_noalloc(ctx.h, corpus.h, queries.h, graph.h, kg.h if kg is not None else C.c_void_p(0), C.byref(p), ki[1], kd[1],
                                      C.byref(st) if want_stats else C.c_void_p(0)))
     return st
+
+
+# ---- fitting a query adapter ----
+
+_DTYPES = None
+
+
+def _dtype(t, name):
+    global _DTYPES
+    if _DTYPES is None:
+        import torch
+        _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ApoeError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
+    return code
+
+
+def _on_gpu(ctx, t, name):
+    if not (t.is_cuda and t.device.index == ctx.device):
+        raise ApoeError(f"{name} must be on GPU {ctx.device}, the context's")
+
+
+def _matrix(ctx, t, name, shape=None, dtype=None):
+    """Checks a matrix whose rows are contiguous; returns its row stride."""
+    _on_gpu(ctx, t, name)
+    if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ApoeError(f"{name} must be a matrix{'' if shape is None else f' of shape {tuple(shape)}'}, not {tuple(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise ApoeError(f"{name} must be {dtype}, not {t.dtype}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ApoeError(f"the rows of {name} must be contiguous")
+    if t.shape[0] <= 1:
+        return t.shape[1]
+    if t.stride(0) < t.shape[1]:
+        raise ApoeError(f"the rows of {name} overlap")
+    return t.stride(0)
+
+
+def _vector(ctx, t, name, n, dtypes):
+    _on_gpu(ctx, t, name)
+    if t.dtype not in dtypes or t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
+        raise ApoeError(f"{name} must be a contiguous vector of {' or '.join(str(d) for d in dtypes)}{'' if n is None else f' of length {n}'}")
+    return t.data_ptr()
+
+
+class _in_order:
+    """The context's stream waits for torch's current stream, and that for the context's afterwards (nothing where they are one)."""
+
+    def __init__(self, ctx):
+        import torch
+        self.theirs = torch.cuda.current_stream(ctx.device)
+        self.ours = None if self.theirs.cuda_stream == ctx.stream else ctx.torch_stream()
+
+    def __enter__(self):
+        if self.ours is not None:
+            self.ours.wait_stream(self.theirs)
+
+    def __exit__(self, *failure):
+        if self.ours is not None:
+            self.theirs.wait_stream(self.ours)
+
+
+def softmax_loss(ctx, queries, rows, t_off, t_idx, t_val=None, scale=1.0, weight=None, live=None, grad_queries=False, grad_rows=False):
+    """Softmax cross entropy of queries [m, d] over the rows [n, d] (a matrix, or a Corpus with half-precision rows), and the
+    gradients of sum(weight * loss). t_off, t_idx, t_val: CSR of each query's relevant rows and their weights (equal shares
+    without); live: int32 bit mask of the rows that take part; scale: of the inner products. grad_queries, grad_rows: True, or a
+    matrix to write to. Returns dict(loss [m], lse [m]) and the gradients asked for; the logits are never held."""
+    import torch
+    a = SoftmaxLossArgs()
+    a.dtype = _dtype(queries, "queries")
+    a.q_stride = _matrix(ctx, queries, "queries")
+    m, d = queries.shape
+    a.n_queries, a.dim = m, d
+    if isinstance(rows, Corpus):
+        a.n_rows, a.corpus = rows.n, rows.h
+        if d != rows.dim:
+            raise ApoeError(f"queries of {d} columns against a corpus of {rows.dim}")
+        if grad_rows is not False and grad_rows is not None:
+            raise ApoeError("the rows of a corpus stay as they are: no grad_rows")
+    else:
+        a.rows_stride = _matrix(ctx, rows, "rows", (rows.shape[0], d), queries.dtype)
+        a.n_rows, a.rows = rows.shape[0], rows.data_ptr()
+        if rows.shape[0] == 0:
+            raise ApoeError("rows is empty")
+    ints, floats = (torch.int32, torch.uint32), (torch.float32,)
+    a.t_off = _vector(ctx, t_off, "t_off", m + 1, ints)
+    a.t_idx = _vector(ctx, t_idx, "t_idx", None, ints)
+    if t_idx.numel() == 0:  # no target at all: no entry is read, but the pointer has to be one
+        a.t_idx = a.t_off
+    if t_val is not None:
+        a.t_val = _vector(ctx, t_val, "t_val", t_idx.shape[0], floats) if t_idx.numel() else None
+    if live is not None:
+        a.live = _vector(ctx, live, "live", (a.n_rows + 31) // 32, ints)
+    if weight is not None:
+        a.weight = _vector(ctx, weight, "weight", m, floats)
+    a.scale = scale
+    a.q = queries.data_ptr()
+    both = torch.empty((2, m), dtype=torch.float32, device=queries.device)
+    out = dict(loss=both[0], lse=both[1])
+    a.loss = both.data_ptr()
+    a.lse = a.loss + 4 * m if m else a.loss
+    if grad_queries is not False and grad_queries is not None:
+        g = torch.empty((m, d), dtype=queries.dtype, device=queries.device) if grad_queries is True else grad_queries
+        a.grad_q_stride = _matrix(ctx, g, "grad_queries", (m, d), queries.dtype)
+        out["grad_queries"], a.grad_q = g, g.data_ptr()
+    if grad_rows is not False and grad_rows is not None:
+        g = torch.empty((rows.shape[0], d), dtype=rows.dtype, device=rows.device) if grad_rows is True else grad_rows
+        a.grad_rows_stride = _matrix(ctx, g, "grad_rows", rows.shape, rows.dtype)
+        out["grad_rows"], a.grad_rows = g, g.data_ptr()
+    if m == 0:  # nothing to compute but a gradient of zeros
+        if "grad_rows" in out:
+            out["grad_rows"].zero_()
+        return out
+    with _in_order(ctx):
+        _check(lib().apoe_softmax_loss(ctx.h, C.byref(a)))
+    return out

@@ -91,6 +91,7 @@ inline uint32_t next_pow2(uint32_t v) {
 struct apoe_ctx {
     int device = 0;
     hipStream_t stream = nullptr;
+    bool own_stream = true; // destroyed with the context
     hipEvent_t ev0 = nullptr, ev1 = nullptr;
     int num_cus = 0;
     size_t lds_per_block = 0;
@@ -98,6 +99,7 @@ struct apoe_ctx {
     // request and is kept until the context is destroyed, so that repeated searches do not pay for
     // a device allocation each. One search at a time per context.
     apoe::DevBuf<char> search_ws;
+    apoe::DevBuf<char> adapt_ws; // the same for the operators that fit a query adapter
     char* static_ws = nullptr; // this GPU's copy of the static workspace of apoe_search_noalloc
     // Upload pipeline for large pageable host arrays: two pinned staging buffers that host threads fill while the
     // copy engine drains the other one (created on first use, kept until the context is destroyed).
@@ -106,6 +108,11 @@ struct apoe_ctx {
     int search_workspace(size_t bytes, char** out) {
         if (search_ws.n < bytes) APOE_TRY(search_ws.alloc(bytes));
         *out = search_ws.p;
+        return APOE_OK;
+    }
+    int adapt_workspace(size_t bytes, char** out) {
+        if (adapt_ws.n < bytes) APOE_TRY(adapt_ws.alloc(bytes));
+        *out = adapt_ws.p;
         return APOE_OK;
     }
 };
@@ -185,6 +192,7 @@ namespace apoe {
 // Copies between caller memory (host or device) and library device memory.
 int copy_in(apoe_ctx* ctx, void* dst_dev, const void* src_any, size_t bytes);
 int copy_out(apoe_ctx* ctx, void* dst_any, const void* src_dev, size_t bytes);
+bool is_device_ptr_of(const void* p, int device); // device memory of one particular GPU
 
 // Kernel launchers (one per .hip file).
 int launch_pack(apoe_ctx* ctx, uint32_t n, const float* dense, const uint32_t* s_off, const uint32_t* s_idx, const float* s_val,
@@ -213,6 +221,7 @@ bool gram_tiles_fit(const apoe_knn* g);
 int launch_nnd_merge_reverse(apoe_knn* g);
 int launch_prune(apoe_knn* g, uint32_t degree);
 int launch_final_graph(apoe_knn* g, uint32_t* rows_dev);
+int launch_softmax_loss(apoe_ctx* ctx, const apoe_softmax_loss_args* args); // strides filled in
 
 // Times `fn` (which enqueues work on ctx->stream) with HIP events; blocks until done.
 template <typename F>

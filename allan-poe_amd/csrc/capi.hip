@@ -34,7 +34,7 @@ static bool is_device_ptr(const void* p) {
 }
 
 // Device memory of one particular GPU.
-static bool is_device_ptr_of(const void* p, int device) {
+bool is_device_ptr_of(const void* p, int device) {
     hipPointerAttribute_t attr;
     if (hipPointerGetAttributes(&attr, p) != hipSuccess) {
         (void)hipGetLastError();
@@ -166,7 +166,7 @@ extern "C" {
 
 const char* apoe_last_error_string(void) { return g_error.c_str(); }
 
-int apoe_ctx_create(int device, apoe_ctx** out) {
+static int ctx_create(int device, bool own_stream, hipStream_t stream, apoe_ctx** out) {
     APOE_REQUIRE(out != nullptr, "out is null");
     *out = nullptr;
     int count = 0;
@@ -183,7 +183,9 @@ int apoe_ctx_create(int device, apoe_ctx** out) {
         delete ctx;
         return APOE_ERR_HIP;
     }
-    if (hipStreamCreate(&ctx->stream) != hipSuccess || hipEventCreate(&ctx->ev0) != hipSuccess || hipEventCreate(&ctx->ev1) != hipSuccess) {
+    ctx->own_stream = own_stream;
+    ctx->stream = stream;
+    if ((own_stream && hipStreamCreate(&ctx->stream) != hipSuccess) || hipEventCreate(&ctx->ev0) != hipSuccess || hipEventCreate(&ctx->ev1) != hipSuccess) {
         set_error("could not create the HIP stream/events: %s", hipGetErrorString(hipGetLastError()));
         apoe_ctx_destroy(ctx);
         return APOE_ERR_HIP;
@@ -192,22 +194,32 @@ int apoe_ctx_create(int device, apoe_ctx** out) {
     return APOE_OK;
 }
 
+int apoe_ctx_create(int device, apoe_ctx** out) { return ctx_create(device, true, nullptr, out); }
+
+int apoe_ctx_create_on_stream(int device, void* stream, apoe_ctx** out) { return ctx_create(device, false, static_cast<hipStream_t>(stream), out); }
+
 void apoe_ctx_destroy(apoe_ctx* ctx) {
     if (!ctx) return;
-    if (ctx->stream) (void)hipStreamSynchronize(ctx->stream);
+    if (ctx->stream || !ctx->own_stream) (void)hipStreamSynchronize(ctx->stream);
     if (ctx->ev0) (void)hipEventDestroy(ctx->ev0);
     if (ctx->ev1) (void)hipEventDestroy(ctx->ev1);
     for (int b = 0; b < 2; b++) {
         if (ctx->pinned_done[b]) (void)hipEventDestroy(ctx->pinned_done[b]);
         if (ctx->pinned[b]) (void)hipHostFree(ctx->pinned[b]);
     }
-    if (ctx->stream) (void)hipStreamDestroy(ctx->stream);
+    if (ctx->own_stream && ctx->stream) (void)hipStreamDestroy(ctx->stream);
     delete ctx;
 }
 
 int apoe_ctx_synchronize(apoe_ctx* ctx) {
     APOE_REQUIRE(ctx != nullptr, "ctx is null");
     APOE_HIP(hipStreamSynchronize(ctx->stream));
+    return APOE_OK;
+}
+
+int apoe_ctx_stream(const apoe_ctx* ctx, void** stream) {
+    APOE_REQUIRE(ctx && stream, "ctx/stream is null");
+    *stream = ctx->stream;
     return APOE_OK;
 }
 

@@ -1,0 +1,909 @@
+// Softmax cross entropy of queries over the rows of a table (documents, passages, terms), without the logits, and its gradients.
+//
+//   s_ij = scale <q_i, x_j> over the live rows j,  lse_i = log sum_j exp(s_ij),  W_i = sum_t w_it over query i's live targets
+//   loss_i = W_i lse_i - sum_t w_it s_it,   G_ij = weight_i scale (W_i exp(s_ij - lse_i) - w_ij),   grad q = G x,   grad x = G^T q
+//
+// The rows are taken in pieces. loss_tile multiplies rows with queries (rows on the M side, so that a lane holds one query and
+// its maximum and sum are taken in registers), and each 128 rows x query give a reference exponent and a sum: base 2, and the
+// reference is the maximum rounded up to a whole number, so that going over to another reference is exact. For gradients the
+// tile's exponentials are rounded to the rows' type and written as 32x32 blocks in the order that a lane has them, which is a
+// fragment of the next product; a piece of them is at most LOSS_PIECE_BYTES.
+//   grad q alone: one pass. A piece's exponentials (relative to their own references) are multiplied with the piece's rows at
+//     once; what the references lack to the common one goes into the exponents of the fragments on their way to the product.
+//   grad x: the normalised G of a piece is needed, so the logits are formed again once lse is known.
+// The targets' own terms are not left to the rounded blocks: their places are zeroed (or rewritten) and W p_t - w_t, which
+// nearly cancels for a query that is served well, is formed in 32 bits.
+#include "apoe_internal.h"
+#include "apoe_tile.h"
+
+namespace apoe {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr uint32_t LOSS_GROUP = 128;               // rows that share a reference
+constexpr size_t LOSS_PIECE_BYTES = 256u << 20;    // of exponentials (or of G) that exist at a time
+constexpr uint32_t LOSS_CHUNKS = 64;               // parts that the join of the sums is split into, at most
+
+template <typename T> __device__ inline float as_float(T v) { return (float)v; }
+
+// ---- blocks of 32 queries x 32 rows ----
+// Part p (16 bytes a lane) holds values 8 p .. 8 p + 7 (fp32: 4 p ..) of a lane's 16; half 1 is turned by four lanes, so that
+// the transposed read finds the halves in different banks.
+template <typename T> struct Block {
+    static constexpr int BYTES = 1024 * (int)sizeof(T), PARTS = BYTES / 1024, VALUES = 16 / (int)sizeof(T);
+    __device__ static int slot(int query, int half) { return half * 32 + (query ^ (half * 4)); }
+    __device__ static uint32_t place(int query, int row) { // byte offset of one value
+        const int half = (row >> 2) & 1, i = ((row >> 3) << 2) | (row & 3);
+        return (uint32_t)((i / VALUES) * 1024 + slot(query, half) * 16 + (i % VALUES) * (int)sizeof(T));
+    }
+};
+
+// Words that no kernel writes while one reads them, at a place that is the same in the wave: a scalar load, which does not wait
+// for the loads into LDS as a vector load's result would.
+using UniformWords = const __attribute__((address_space(4))) uint32_t*;
+
+// Live rows among 32 from `row` on, the same row in the whole wave.
+__device__ inline uint32_t live_word(const uint32_t* live, uint32_t row, uint32_t n) {
+    if (row >= n) return 0;
+    uint32_t w = live ? ((UniformWords)live)[row >> 5] : ~0u;
+    if (n - row < 32) w &= (1u << (n - row)) - 1u;
+    return w;
+}
+
+struct LossArgs {
+    const void* q;
+    const void* rows;
+    uint32_t q_pitch, r_pitch; // bytes
+    uint32_t nq, n, dim, qp;   // qp: queries rounded up to whole tiles
+    const uint32_t *t_off, *t_idx;
+    const float* t_val;
+    const uint32_t* live;
+    const float* weight;
+    float scale;
+    // one piece
+    uint32_t row0, row_tiles, q_tiles, row_blocks; // first row, tiles of either side, blocks of 32 rows (the pitch of `blocks`)
+    // workspace
+    float *ref, *sum;           // [n / LOSS_GROUP][qp]
+    float *chunk_ref, *chunk_sum; // [LOSS_CHUNKS][qp]
+    float2* lse_w;              // [qp]: lse in base 2, weight W (to be multiplied with exp(s - lse))
+    uint32_t* top_coef;         // largest |weight| (|W| + sum |w|), as bits
+    char* blocks;
+    float* part;                // [splits][qp][dim]
+    float* part_ref[2];         // [splits][qp]
+    float *loss, *lse;
+    void *grad_q, *grad_x;
+    uint32_t gq_pitch, gx_pitch;
+    uint32_t groups, chunks, splits;
+};
+
+// fp16 holds 30 binades of normal numbers, half of them above one: the largest exponential of a group is brought up to 2^14, so
+// that 28 binades stay below it. A query that is served well needs them: its target is the largest, and the gradient is what the
+// others, far below, leave.
+template <typename T> constexpr float HEADROOM = __is_same(T, _Float16) ? 14.f : 0.f;
+
+enum { TILE_SUMS = 0, TILE_EXP = 1, TILE_GRAD = 2 };
+
+// Power of two that brings the largest coefficient near 2^13: G fits fp16 with room below.
+__device__ inline float grad_scale_of(const uint32_t* top) {
+    const float t = __uint_as_float(*top);
+    return t > 0.f && t < 1e30f && t > 1e-30f ? exp2f(13.f - ceilf(log2f(t))) : 1.f;
+}
+
+template <typename T> __device__ inline i32x4 pack(const float* p) {
+    if constexpr (sizeof(T) == 4) {
+        return i32x4{__float_as_int(p[0]), __float_as_int(p[1]), __float_as_int(p[2]), __float_as_int(p[3])};
+    } else {
+        typedef T t8 __attribute__((ext_vector_type(8)));
+        t8 v;
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = (T)p[i];
+        return __builtin_bit_cast(i32x4, v);
+    }
+}
+
+template <typename T, int NT, int WM, int WN, int SF, int ST, int MODE>
+__global__ __launch_bounds__(64 * WM * WN, 2) void loss_tile(LossArgs a) {
+    constexpr int NW = WM * WN, BM = WM * 128, BN = WN * NT * 32;
+    using ATile = RowTile<T, BM, SF, NW>;
+    using BTile = RowTile<T, BN, SF, NW>;
+    constexpr int STAGE = ATile::BYTES + BTile::BYTES, PER = ATile::LOADS + BTile::LOADS;
+    __shared__ __align__(1024) char lds[ST * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    // consecutive workgroups go to the eight XCDs in turn: those of one XCD share a tile of rows, one after the other
+    uint32_t rt = blockIdx.x / a.q_tiles, qt = blockIdx.x % a.q_tiles;
+    const uint32_t whole = a.row_tiles / 8 * 8;
+    if (blockIdx.x < whole * a.q_tiles) {
+        const uint32_t i = blockIdx.x >> 3;
+        rt = (i / a.q_tiles) * 8 + (blockIdx.x & 7);
+        qt = i % a.q_tiles;
+    }
+    const uint32_t row = a.row0 + rt * BM, query = qt * BN;
+    ATile ta;
+    BTile tb;
+    ta.init(reinterpret_cast<const T*>((const char*)a.rows + (uint64_t)row * a.r_pitch), a.r_pitch, (int)min((uint32_t)BM, a.n - row), wave, lane);
+    tb.init(reinterpret_cast<const T*>((const char*)a.q + (uint64_t)query * a.q_pitch), a.q_pitch, (int)min((uint32_t)BN, a.nq - query), wave, lane);
+    const int bytes = (int)(a.dim * sizeof(T)), stages = (bytes + SF * 32 - 1) / (SF * 32);
+    const uint32_t base = lds_address(lds);
+    int left = bytes;
+    uint32_t into = 0;
+    auto issue = [&]() {
+        ta.load(base + into, left, wave);
+        tb.load(base + into + ATile::BYTES, left, wave);
+        ta.next();
+        tb.next();
+        left -= SF * 32;
+        into = into + STAGE == ST * STAGE ? 0 : into + STAGE;
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; s++) issue();
+    f32x16 acc[4][NT] = {};
+    uint32_t from = 0;
+    for (int s = 0; s < stages; s++) {
+        tile_wait<(ST - 2) * PER>();
+        issue();
+        const char* A = lds + from;
+        const char* B = A + ATile::BYTES;
+#pragma unroll
+        for (int f = 0; f < SF; f++) {
+            i32x4 x[4], y[NT];
+#pragma unroll
+            for (int m = 0; m < 4; m++) x[m] = ATile::read(A, wm * 4 + m, f, lane);
+#pragma unroll
+            for (int t = 0; t < NT; t++) y[t] = BTile::read(B, wn * NT + t, f, lane);
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) acc[m][t] = mfma_step<T>(x[m], y[t], acc[m][t]);
+        }
+        from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
+    }
+    // epilogue: one query a lane (and its other half), 128 rows a wave
+    const int h = lane >> 5;
+    const float c = a.scale * LOG2E;
+    const uint32_t wrow = row + wm * LOSS_GROUP;
+    uint32_t words[4];
+#pragma unroll
+    for (int m = 0; m < 4; m++) words[m] = live_word(a.live, wrow + m * 32, a.n);
+    const bool all = (words[0] & words[1] & words[2] & words[3]) == ~0u;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const uint32_t qi = query + (wn * NT + t) * 32 + (lane & 31);
+        if (!all) {
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                const uint32_t w = words[m] >> (4 * h);
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (!((w >> (8 * (i >> 2) + (i & 3))) & 1)) acc[m][t][i] = -INFINITY;
+            }
+        }
+        float p[16];
+        char* out = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((wrow - a.row0) >> 5)) * Block<T>::BYTES + Block<T>::slot(lane & 31, h) * 16;
+        if constexpr (MODE == TILE_GRAD) {
+            const float2 lw = a.lse_w[qi];
+            const float g = lw.y * grad_scale_of(a.top_coef);
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float z = acc[m][t][i];
+                    // a query that counts nothing, and a row that is left out, give zero whatever the logit is
+                    p[i] = g == 0.f || z == -INFINITY ? 0.f : g * __builtin_amdgcn_exp2f(__builtin_fmaf(z, c, -lw.x));
+                }
+#pragma unroll
+                for (int k = 0; k < Block<T>::PARTS; k++) *reinterpret_cast<i32x4*>(out + m * Block<T>::BYTES + k * 1024) = pack<T>(p + k * Block<T>::VALUES);
+            }
+        } else {
+            float top = -INFINITY;
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) top = fmaxf(top, acc[m][t][i]);
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float ref = top == -INFINITY ? -INFINITY : ceilf(top * c) - HEADROOM<T>;
+            const float less = top == -INFINITY ? 0.f : -ref;
+            float sum = 0.f;
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float z = acc[m][t][i];
+                    p[i] = z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(z, c, less));
+                    sum += p[i];
+                }
+                if constexpr (MODE == TILE_EXP) {
+#pragma unroll
+                    for (int k = 0; k < Block<T>::PARTS; k++) *reinterpret_cast<i32x4*>(out + m * Block<T>::BYTES + k * 1024) = pack<T>(p + k * Block<T>::VALUES);
+                }
+            }
+            sum += __shfl_xor(sum, 32);
+            if (h == 0) {
+                const size_t at = (size_t)(wrow / LOSS_GROUP) * a.qp + qi;
+                a.ref[at] = ref;
+                a.sum[at] = sum;
+            }
+        }
+    }
+    tile_wait<0>(); // the stages beyond the last have landed before the LDS goes to another workgroup
+}
+
+// (reference, sum) of two parts joined.
+__device__ inline void join_sums(float& ref, float& sum, float r, float s) {
+    const float top = fmaxf(ref, r);
+    if (top == -INFINITY) {
+        sum += s; // zeros, or NaN
+        return;
+    }
+    sum = sum * __builtin_amdgcn_exp2f(ref - top) + s * __builtin_amdgcn_exp2f(r - top);
+    ref = top;
+}
+
+// The groups' sums of 32 queries joined, chunk by chunk: grid (qp / 32, chunks). ZERO: the targets' places in this piece's
+// exponentials are zeroed as well, by chunk 0.
+template <typename T, bool ZERO> __global__ __launch_bounds__(256) void loss_join(LossArgs a, uint32_t group0, uint32_t groups, uint32_t chunk0) {
+    __shared__ float sr[8][32], ss[8][32];
+    const uint32_t ql = threadIdx.x & 31, gl = threadIdx.x >> 5, qi = blockIdx.x * 32 + ql;
+    const uint32_t per = (groups + gridDim.y - 1) / gridDim.y, g0 = blockIdx.y * per, g1 = min(g0 + per, groups);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.top_coef = 0;
+    float ref = -INFINITY, sum = 0.f;
+    for (uint32_t g = g0 + gl; g < g1; g += 8) {
+        const size_t at = (size_t)(group0 + g) * a.qp + qi;
+        join_sums(ref, sum, a.ref[at], a.sum[at]);
+    }
+    sr[gl][ql] = ref;
+    ss[gl][ql] = sum;
+    __syncthreads();
+    if (gl == 0) {
+        for (int k = 1; k < 8; k++) join_sums(ref, sum, sr[k][ql], ss[k][ql]);
+        a.chunk_ref[(chunk0 + blockIdx.y) * (size_t)a.qp + qi] = ref;
+        a.chunk_sum[(chunk0 + blockIdx.y) * (size_t)a.qp + qi] = sum;
+    }
+    if constexpr (ZERO) {
+        if (blockIdx.y == 0 && qi < a.nq && a.t_off) {
+            const uint32_t end = min(a.row0 + a.row_blocks * 32, a.n);
+            for (uint32_t e = a.t_off[qi] + gl; e < a.t_off[qi + 1]; e += 8) {
+                const uint32_t t = a.t_idx[e];
+                if (t < a.row0 || t >= end) continue;
+                char* block = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((t - a.row0) >> 5)) * Block<T>::BYTES;
+                *reinterpret_cast<T*>(block + Block<T>::place(ql, (t - a.row0) & 31)) = (T)0.f;
+            }
+        }
+    }
+}
+
+__device__ inline bool is_live(const LossArgs& a, uint32_t t) { return t < a.n && (!a.live || ((a.live[t >> 5] >> (t & 31)) & 1)); }
+__device__ inline float target_weight(const LossArgs& a, uint32_t e, uint32_t e0, uint32_t e1) { return a.t_val ? a.t_val[e] : 1.f / (float)(e1 - e0); }
+
+// lse (base 2) of a query from the chunks, by one wave.
+__device__ inline float join_chunks(const LossArgs& a, uint32_t qi, int lane) {
+    float ref = -INFINITY, sum = 0.f;
+    for (uint32_t k = lane; k < a.chunks; k += 64) join_sums(ref, sum, a.chunk_ref[(size_t)k * a.qp + qi], a.chunk_sum[(size_t)k * a.qp + qi]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        const float r = __shfl_xor(ref, d), s = __shfl_xor(sum, d);
+        join_sums(ref, sum, r, s);
+    }
+    if (ref == -INFINITY) return sum == 0.f ? -INFINITY : sum; // no live row (or NaN)
+    return ref + log2f(sum);
+}
+
+// What the second pass needs of a query, one wave each: lse, and weight W.
+__global__ __launch_bounds__(64) void loss_coefs(LossArgs a) {
+    const uint32_t qi = blockIdx.x;
+    const int lane = threadIdx.x;
+    if (qi >= a.nq) {
+        if (lane == 0) a.lse_w[qi] = make_float2(0.f, 0.f);
+        return;
+    }
+    const float lse = join_chunks(a, qi, lane);
+    const uint32_t e0 = a.t_off[qi], e1 = a.t_off[qi + 1];
+    float W = 0.f, A = 0.f;
+    for (uint32_t e = e0 + lane; e < e1; e += 64) {
+        const float w = is_live(a, a.t_idx[e]) ? target_weight(a, e, e0, e1) : 0.f;
+        W += w;
+        A += fabsf(w);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) {
+        W += __shfl_xor(W, d);
+        A += __shfl_xor(A, d);
+    }
+    if (lane == 0) {
+        const float c = a.weight ? a.weight[qi] : 1.f;
+        a.lse_w[qi] = make_float2(lse, c * W);
+        atomicMax(a.top_coef, __float_as_uint(fabsf(c) * (fabsf(W) + A))); // a maximum does not depend on the order
+    }
+}
+
+template <typename T> __device__ inline float dot16(const char* x, const char* y) { // of 16 bytes each
+    typedef T tv __attribute__((ext_vector_type(16 / sizeof(T))));
+    const tv u = *reinterpret_cast<const tv*>(x), v = *reinterpret_cast<const tv*>(y);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); i++) s = __builtin_fmaf((float)u[i], (float)v[i], s);
+    return s;
+}
+
+// Second pass: the targets' places in this piece's G, formed in 32 bits; one wave a query.
+template <typename T> __global__ __launch_bounds__(64) void loss_targets(LossArgs a) {
+    const uint32_t qi = blockIdx.x, end = min(a.row0 + a.row_blocks * 32, a.n);
+    const int lane = threadIdx.x;
+    const uint32_t e0 = a.t_off[qi], e1 = a.t_off[qi + 1];
+    const float2 lw = a.lse_w[qi];
+    const float gs = grad_scale_of(a.top_coef), cw = a.weight ? a.weight[qi] : 1.f;
+    for (uint32_t e = e0; e < e1; e++) {
+        const uint32_t t = a.t_idx[e];
+        if (t < a.row0 || t >= end || !is_live(a, t)) continue;
+        // a row that is named twice: its first entry takes the weights of all
+        float w = 0.f;
+        bool first = true;
+        for (uint32_t k = e0 + lane; k < e1; k += 64) {
+            if (a.t_idx[k] != t) continue;
+            w += target_weight(a, k, e0, e1);
+            if (k < e) first = false;
+        }
+        if (__any(!first)) continue;
+        float dot = 0.f;
+        const char* x = (const char*)a.rows + (uint64_t)t * a.r_pitch;
+        const char* q = (const char*)a.q + (uint64_t)qi * a.q_pitch;
+        for (uint32_t b = lane * 16; b < a.dim * sizeof(T); b += 1024) dot += dot16<T>(q + b, x + b);
+#pragma unroll
+        for (int d = 32; d; d >>= 1) {
+            dot += __shfl_xor(dot, d);
+            w += __shfl_xor(w, d);
+        }
+        if (lane == 0) {
+            const float p = exp2f(__builtin_fmaf(dot, a.scale * LOG2E, -lw.x));
+            const float g = cw == 0.f ? 0.f : gs * (lw.y * p - cw * w);
+            char* block = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((t - a.row0) >> 5)) * Block<T>::BYTES;
+            *reinterpret_cast<T*>(block + Block<T>::place(qi & 31, (t - a.row0) & 31)) = (T)g;
+        }
+    }
+}
+
+// A fragment's values times 2^-less, less >= 0. They are not negative, so bf16 needs one saturating subtraction on the exponent of
+// two at a time: what falls below the smallest normal number becomes zero or stays below it.
+template <typename T> __device__ inline i32x4 scale_down(i32x4 v, float less) {
+    if constexpr (sizeof(T) == 4) {
+        const float f = __builtin_amdgcn_exp2f(-less);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = __float_as_int(__int_as_float(v[i]) * f);
+    } else if constexpr (__is_same(T, _Float16)) {
+        // in two steps: a factor below 2^-24 is no fp16 number, but 2^14 times it may be
+        const float some = fminf(less, 14.f);
+        const _Float16 f = (_Float16)__builtin_amdgcn_exp2f(-some), g = (_Float16)__builtin_amdgcn_exp2f(some - less);
+        const f16x8 x = __builtin_bit_cast(f16x8, v) * f * g;
+        v = __builtin_bit_cast(i32x4, x);
+    } else {
+        const unsigned short k = (unsigned short)((int)fminf(less, 255.f) << 7);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int two = v[i]; // a bit cast of a vector's element takes the vector's first
+            v[i] = __builtin_bit_cast(int, __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, two), u16x2{k, k}));
+        }
+    }
+    return v;
+}
+
+// grad q: a split's rows x its queries' blocks. M side: queries (blocks), N side: columns of the rows. EXP: fragments are brought
+// to the largest reference of the split, and a split's sum to the largest so far.
+template <typename T, int MT, int NT, int WM, int WN, int ST, bool EXP>
+__global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint32_t n_tiles, uint32_t groups_per_split, uint32_t piece_groups, int turn, int first) {
+    constexpr int NW = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, SF = sizeof(T) == 4 ? 4 : 2;
+    using BTile = ColTile<T, BN, SF, NW, ORDER_BLOCKS>;
+    static_assert(BTile::KE == 32, "a block a stage");
+    constexpr int ABYTES = BM / 32 * Block<T>::BYTES, AINS = ABYTES / 1024, ALOADS = (AINS + NW - 1) / NW;
+    constexpr int RBYTES = NW * 256; // references: 64 queries a wave
+    static_assert(NW * 64 >= BM, "a reference a query");
+    constexpr int STAGE = ABYTES + BTile::BYTES + (EXP ? RBYTES : 0), PER = ALOADS + BTile::LOADS + (EXP ? 1 : 0);
+    __shared__ __align__(1024) char lds[ST * STAGE];
+    __shared__ float factor[2][BM];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    const uint32_t per_split = a.q_tiles * n_tiles;
+    uint32_t split = blockIdx.x / per_split, rest = blockIdx.x % per_split;
+    if (a.splits % 8 == 0) { // the workgroups of one split, which read the same rows, on one XCD
+        const uint32_t i = blockIdx.x >> 3;
+        split = (i / per_split) * 8 + (blockIdx.x & 7);
+        rest = i % per_split;
+    }
+    const uint32_t query = rest / n_tiles * BM, col = rest % n_tiles * BN;
+    const uint32_t g0 = min(split * groups_per_split, piece_groups), g1 = min(g0 + groups_per_split, piece_groups);
+    const uint32_t group0 = a.row0 / LOSS_GROUP;
+    float top = -INFINITY; // of query `query + threadIdx.x` (the first BM threads)
+    if constexpr (EXP) {
+        if (threadIdx.x < BM) {
+            const uint32_t qi = query + threadIdx.x;
+            const bool real = qi < a.qp;
+            for (uint32_t g = g0; g < g1; g++) top = fmaxf(top, real ? a.ref[(size_t)(group0 + g) * a.qp + qi] : -INFINITY);
+            factor[0][threadIdx.x] = top;
+        }
+        __syncthreads();
+    }
+    float mine[MT]; // the split's reference of the query whose blocks' lane this is
+#pragma unroll
+    for (int m = 0; m < MT; m++) mine[m] = EXP ? factor[0][(wm * MT + m) * 32 + (lane & 31)] : 0.f;
+
+    // queries: whole blocks, one 32 rows after the other
+    uint32_t aoff[ALOADS], adst[ALOADS];
+    const uint32_t q_blocks = a.qp / 32;
+#pragma unroll
+    for (int i = 0; i < ALOADS; i++) {
+        const int ins = (i * NW + wave) % AINS, b = ins / Block<T>::PARTS, k = ins % Block<T>::PARTS; // a wave without one of its own repeats another's
+        adst[i] = ins * 1024;
+        aoff[i] = query / 32 + b < q_blocks ? (uint32_t)b * (a.row_blocks * (uint32_t)Block<T>::BYTES) + k * 1024 + lane * 16 : TILE_MASKED;
+    }
+    uint64_t abase = uniform64((uint64_t)a.blocks + ((uint64_t)(query / 32) * a.row_blocks + g0 * (LOSS_GROUP / 32)) * Block<T>::BYTES);
+    uint64_t rbase = uniform64((uint64_t)(a.ref + (size_t)(group0 + g0) * a.qp + query));
+    BTile tb;
+    const uint32_t first_row = a.row0 + g0 * LOSS_GROUP;
+    tb.init(reinterpret_cast<const T*>((const char*)a.rows + (uint64_t)first_row * a.r_pitch) + col, a.r_pitch, (int)min((uint32_t)BN, a.dim - col), wave, lane);
+    const uint32_t roff = query + wave * 64 + lane < a.qp ? (wave * 64 + lane) * 4 : TILE_MASKED;
+
+    const int stages = (int)(g1 - g0) * (LOSS_GROUP / 32);
+    const uint32_t base = lds_address(lds);
+    uint32_t into = 0, issued = 0;
+    uint32_t word = stages ? live_word(a.live, first_row, a.n) : 0u;
+    auto issue = [&]() {
+        const bool in = (int)issued < stages;
+        const i32x4 ab = buffer_of(abase);
+#pragma unroll
+        for (int i = 0; i < ALOADS; i++) load_to_lds16(ab, in ? aoff[i] : TILE_MASKED, base + into + adst[i]);
+        tb.load(base + into + ABYTES, in ? word : 0u, wave, lane);
+        if constexpr (EXP) {
+            load_to_lds4(buffer_of(uniform64(rbase)), in ? roff : TILE_MASKED, base + into + ABYTES + BTile::BYTES + wave * 256);
+        }
+        abase += Block<T>::BYTES;
+        tb.next();
+        issued++;
+        if (issued % (LOSS_GROUP / 32) == 0) rbase += a.qp * 4;
+        word = (int)issued < stages ? live_word(a.live, first_row + issued * 32, a.n) : 0u;
+        into = into + STAGE == ST * STAGE ? 0 : into + STAGE;
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; s++) issue();
+    f32x16 acc[MT][NT] = {};
+    uint32_t from = 0;
+    for (int s = 0; s < stages; s++) {
+        tile_wait<(ST - 2) * PER>();
+        issue();
+        const char* A = lds + from;
+        const char* B = A + ABYTES;
+        float less[MT];
+        if constexpr (EXP) {
+            const float* r = reinterpret_cast<const float*>(B + BTile::BYTES);
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                const float own = r[(wm * MT + m) * 32 + (lane & 31)];
+                less[m] = own == -INFINITY ? 0.f : mine[m] - own; // a group without live rows holds zeros
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < SF; f++) {
+            i32x4 x[MT], y[NT];
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                x[m] = *reinterpret_cast<const i32x4*>(A + (wm * MT + m) * Block<T>::BYTES + f * 1024 + Block<T>::slot(lane & 31, lane >> 5) * 16);
+                if constexpr (EXP) x[m] = scale_down<T>(x[m], less[m]);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++) y[t] = BTile::read(B, wn * NT + t, f, lane);
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) acc[m][t] = mfma_step<T>(x[m], y[t], acc[m][t]);
+        }
+        from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
+    }
+    tile_wait<0>();
+    if constexpr (EXP) {
+        if (threadIdx.x < BM) {
+            const uint32_t qi = query + threadIdx.x;
+            const size_t at = (size_t)split * a.qp + qi;
+            const float old = first || qi >= a.qp ? -INFINITY : a.part_ref[turn ^ 1][at];
+            const float both = fmaxf(old, top);
+            factor[0][threadIdx.x] = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - both);
+            factor[1][threadIdx.x] = old == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(old - both);
+            if (col == 0 && qi < a.qp) a.part_ref[turn][at] = both;
+        }
+        __syncthreads();
+    }
+    const int h = lane >> 5;
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int r = (wm * MT + m) * 32 + result_row(i, h);
+            if (query + r >= a.nq) continue;
+            float* out = a.part + ((size_t)split * a.qp + query + r) * a.dim;
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const uint32_t d = col + (wn * NT + t) * 32 + (lane & 31);
+                if (d >= a.dim) continue;
+                float v = acc[m][t][i];
+                if constexpr (EXP) v *= factor[0][r];
+                if (!first) v += EXP ? out[d] * factor[1][r] : out[d];
+                out[d] = v;
+            }
+        }
+}
+
+// grad x of a piece: rows (blocks read transposed) x queries. Each row's gradient is whole here: all queries are in.
+template <typename T, int MT, int NT, int WM, int WN, int ST>
+__global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint32_t n_tiles, const uint32_t* q_on_words) {
+    constexpr int NW = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, SF = sizeof(T) == 4 ? 4 : 2;
+    using BTile = ColTile<T, BN, SF, NW, ORDER_ROWS>;
+    constexpr int ABYTES = BM / 32 * Block<T>::BYTES, ALOADS = ABYTES / (1024 * NW);
+    constexpr int STAGE = ABYTES + BTile::BYTES, PER = ALOADS + BTile::LOADS;
+    __shared__ __align__(1024) char lds[ST * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    const uint32_t rt = blockIdx.x / n_tiles, col = blockIdx.x % n_tiles * BN, block0 = rt * (BM / 32);
+    uint32_t aoff[ALOADS];
+#pragma unroll
+    for (int i = 0; i < ALOADS; i++) {
+        const int ins = i * NW + wave;
+        aoff[i] = block0 + ins / Block<T>::PARTS < a.row_blocks ? ins * 1024 + lane * 16 : TILE_MASKED;
+    }
+    uint64_t abase = uniform64((uint64_t)a.blocks + (uint64_t)block0 * Block<T>::BYTES);
+    const uint64_t astep = (uint64_t)a.row_blocks * Block<T>::BYTES;
+    BTile tb;
+    tb.init(reinterpret_cast<const T*>(a.q) + col, a.q_pitch, (int)min((uint32_t)BN, a.dim - col), wave, lane);
+    const UniformWords q_on = (UniformWords)q_on_words;
+    const int stages = (int)((a.nq + 31) / 32);
+    const uint32_t base = lds_address(lds);
+    uint32_t into = 0, issued = 0;
+    auto issue = [&]() {
+        const bool in = (int)issued < stages;
+        const i32x4 ab = buffer_of(abase);
+#pragma unroll
+        for (int i = 0; i < ALOADS; i++) load_to_lds16(ab, in ? aoff[i] : TILE_MASKED, base + into + (i * NW + wave) * 1024);
+        tb.load(base + into + ABYTES, in ? q_on[issued] : 0u, wave, lane);
+        abase += astep;
+        tb.next();
+        issued++;
+        into = into + STAGE == ST * STAGE ? 0 : into + STAGE;
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; s++) issue();
+    f32x16 acc[MT][NT] = {};
+    uint32_t from = 0;
+    for (int s = 0; s < stages; s++) {
+        tile_wait<(ST - 2) * PER>();
+        issue();
+        const char* A = lds + from;
+        const char* B = A + ABYTES;
+#pragma unroll
+        for (int f = 0; f < SF; f++) {
+            i32x4 x[MT], y[NT];
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+                const char* block = A + (wm * MT + m) * Block<T>::BYTES;
+                const int h = lane >> 5;
+                if constexpr (sizeof(T) == 2) {
+                    const int i = lane & 15, g = (lane >> 4) & 1;
+                    i32x2 part[2];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int q = f * 16 + 8 * h + 4 * j + (i >> 2);
+                        const char* p = block + g * 1024 + Block<T>::slot(q, i & 1) * 16 + ((i & 3) >> 1) * 8;
+                        part[j] = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+                    }
+                    x[m] = i32x4{part[0][0], part[0][1], part[1][0], part[1][1]};
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) x[m][j] = *reinterpret_cast<const int*>(block + Block<T>::place(f * 8 + 4 * h + j, lane & 31));
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++) y[t] = BTile::read(B, wn * NT + t, f, lane);
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) acc[m][t] = mfma_step<T>(x[m], y[t], acc[m][t]);
+        }
+        from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
+    }
+    tile_wait<0>();
+    const float back = a.scale / grad_scale_of(a.top_coef);
+    const int h = lane >> 5;
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+        const uint32_t row = a.row0 + rt * BM + (wm * MT + m) * 32;
+        const uint32_t word = live_word(a.live, row, a.n);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const uint32_t r = row + result_row(i, h);
+            if (r >= a.n) continue;
+            const bool on = (word >> result_row(i, h)) & 1;
+            T* out = reinterpret_cast<T*>((char*)a.grad_x + (uint64_t)r * a.gx_pitch);
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const uint32_t d = col + (wn * NT + t) * 32 + (lane & 31);
+                if (d < a.dim) out[d] = (T)(on ? acc[m][t][i] * back : 0.f);
+            }
+        }
+    }
+}
+
+// Queries that count something, as bits (what the other queries hold is not multiplied).
+__global__ __launch_bounds__(64) void loss_q_on(LossArgs a, uint32_t* __restrict__ out) {
+    const uint32_t qi = blockIdx.x * 64 + threadIdx.x;
+    bool on = false;
+    if (qi < a.nq && (!a.weight || a.weight[qi] != 0.f)) {
+        const uint32_t e0 = a.t_off[qi], e1 = a.t_off[qi + 1];
+        for (uint32_t e = e0; e < e1 && !on; e++) on = is_live(a, a.t_idx[e]) && target_weight(a, e, e0, e1) != 0.f;
+    }
+    const unsigned long long b = __ballot(on);
+    if ((threadIdx.x & 31) == 0) out[qi >> 5] = (uint32_t)(b >> (threadIdx.x & 32));
+}
+
+__device__ inline float block_sum(float v, float* buf) { // of 256 threads, the same for all
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (buf[0] + buf[1]) + (buf[2] + buf[3]);
+}
+
+// One workgroup a query: lse, loss, and the query's gradient from its splits. EXP: the splits are sums of exponentials relative
+// to their references without the targets, whose terms are added here; otherwise they are sums of scaled G.
+template <typename T, bool GRAD, bool EXP> __global__ __launch_bounds__(256) void loss_finish(LossArgs a, int turn) {
+    constexpr int V = 16 / (int)sizeof(T), C = APOE_LOSS_MAX_DIM / (256 * V);
+    __shared__ float buf[4], lse_of;
+    const uint32_t qi = blockIdx.x, tid = threadIdx.x;
+    if (tid < 64) {
+        const float l = join_chunks(a, qi, tid);
+        if (tid == 0) lse_of = l;
+    }
+    const uint32_t e0 = a.t_off ? a.t_off[qi] : 0, e1 = a.t_off ? a.t_off[qi + 1] : 0;
+    float W = 0.f;
+    bool any = false;
+    for (uint32_t e = e0 + tid; e < e1; e += 256) {
+        const float w = is_live(a, a.t_idx[e]) ? target_weight(a, e, e0, e1) : 0.f;
+        W += w;
+        any |= w != 0.f;
+    }
+    W = block_sum(W, buf);
+    const bool on = __syncthreads_or(any);
+    const float lse = lse_of, cw = a.weight ? a.weight[qi] : 1.f;
+    float acc[C][V] = {};
+    if constexpr (GRAD) {
+        const float gs = EXP ? 1.f : 1.f / grad_scale_of(a.top_coef);
+        if (on && cw != 0.f)
+            for (uint32_t s = 0; s < a.splits; s++) {
+                const float r = EXP ? a.part_ref[turn][(size_t)s * a.qp + qi] : 0.f;
+                if (EXP && r == -INFINITY) continue;
+                const float f = EXP ? W * __builtin_amdgcn_exp2f(r - lse) : gs;
+                const float* p = a.part + ((size_t)s * a.qp + qi) * a.dim;
+#pragma unroll
+                for (int k = 0; k < C; k++) {
+                    const uint32_t d = (k * 256 + tid) * V;
+                    if (d >= a.dim) continue;
+#pragma unroll
+                    for (int v = 0; v < V; v += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(p + d + v);
+                        acc[k][v] = __builtin_fmaf(f, x.x, acc[k][v]);
+                        acc[k][v + 1] = __builtin_fmaf(f, x.y, acc[k][v + 1]);
+                        acc[k][v + 2] = __builtin_fmaf(f, x.z, acc[k][v + 2]);
+                        acc[k][v + 3] = __builtin_fmaf(f, x.w, acc[k][v + 3]);
+                    }
+                }
+            }
+    }
+    // targets: s_t in 32 bits, in the order of the list
+    typedef T tv __attribute__((ext_vector_type(V)));
+    const char* q = (const char*)a.q + (uint64_t)qi * a.q_pitch;
+    float at = 0.f;
+    for (uint32_t e = e0; e < e1; e++) {
+        const uint32_t t = a.t_idx[e];
+        const float w = is_live(a, t) ? target_weight(a, e, e0, e1) : 0.f;
+        if (w == 0.f && !(GRAD && EXP)) continue;
+        if (!is_live(a, t)) continue;
+        const char* x = (const char*)a.rows + (uint64_t)t * a.r_pitch;
+        float dot = 0.f;
+        tv xs[C];
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            const uint32_t d = (k * 256 + tid) * V;
+            if (d >= a.dim) continue;
+            xs[k] = *reinterpret_cast<const tv*>(x + d * sizeof(T));
+            const tv u = *reinterpret_cast<const tv*>(q + d * sizeof(T));
+#pragma unroll
+            for (int v = 0; v < V; v++) dot = __builtin_fmaf((float)u[v], (float)xs[k][v], dot);
+        }
+        dot = block_sum(dot, buf);
+        if (w != 0.f) at = __builtin_fmaf(w, dot * a.scale, at);
+        if constexpr (GRAD && EXP) {
+            bool again = false; // its exponential was taken out once
+            for (uint32_t k = e0 + tid; k < e; k += 256) again |= a.t_idx[k] == t;
+            again = __syncthreads_or(again);
+            const float f = (again ? 0.f : W * exp2f(__builtin_fmaf(dot, a.scale * LOG2E, -lse))) - w;
+            if (on && cw != 0.f) {
+#pragma unroll
+                for (int k = 0; k < C; k++)
+                    if ((k * 256 + tid) * V < a.dim) {
+#pragma unroll
+                        for (int v = 0; v < V; v++) acc[k][v] = __builtin_fmaf(f, (float)xs[k][v], acc[k][v]);
+                    }
+            }
+        }
+    }
+    if (tid == 0) {
+        if (a.lse) a.lse[qi] = lse * LN2;
+        if (a.loss) a.loss[qi] = W == 0.f ? (on ? -at : 0.f) : __builtin_fmaf(W, lse * LN2, -at);
+    }
+    if constexpr (GRAD) {
+        const float f = EXP ? cw * a.scale : a.scale;
+        char* out = (char*)a.grad_q + (uint64_t)qi * a.gq_pitch;
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            const uint32_t d = (k * 256 + tid) * V;
+            if (d >= a.dim) continue;
+            tv o;
+#pragma unroll
+            for (int v = 0; v < V; v++) o[v] = (T)(on && cw != 0.f ? f * acc[k][v] : 0.f);
+            *reinterpret_cast<tv*>(out + d * sizeof(T)) = o;
+        }
+    }
+}
+
+// ---- launches ----
+
+static uint32_t up(uint64_t v, uint64_t to) { return (uint32_t)((v + to - 1) / to * to); }
+
+template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss_args* p) {
+    LossArgs a{};
+    const bool gq = p->grad_q != nullptr, gx = p->grad_rows != nullptr, two_pass = gx;
+    a.q = p->q;
+    a.rows = p->rows;
+    a.q_pitch = (uint32_t)(p->q_stride * sizeof(T));
+    a.r_pitch = (uint32_t)(p->rows_stride * sizeof(T));
+    a.gq_pitch = (uint32_t)(p->grad_q_stride * sizeof(T));
+    a.gx_pitch = (uint32_t)(p->grad_rows_stride * sizeof(T));
+    a.nq = p->n_queries;
+    a.n = p->n_rows;
+    a.dim = p->dim;
+    a.t_off = p->t_off;
+    a.t_idx = p->t_idx;
+    a.t_val = p->t_val;
+    a.live = p->live;
+    a.weight = p->weight;
+    a.scale = p->scale;
+    a.loss = p->loss;
+    a.lse = p->lse;
+    a.grad_q = p->grad_q;
+    a.grad_x = p->grad_rows;
+    // tiles: 256 rows x 128 queries, or 512 x 64 or 32 for few queries
+    const int form = a.nq <= 32 ? 2 : a.nq <= 64 ? 1 : 0;
+    const uint32_t bm = form ? 512 : 256, bn = form == 2 ? 32 : form == 1 ? 64 : 128;
+    a.qp = up(a.nq, bn);
+    a.q_tiles = a.qp / bn;
+    const uint32_t rows_up = up(a.n, bm);
+    uint64_t piece = rows_up; // rows of a piece: whole tiles
+    if (gq || gx) {
+        const uint64_t most = std::max<uint64_t>(bm, LOSS_PIECE_BYTES / ((uint64_t)a.qp * sizeof(T)) / bm * bm);
+        const uint64_t pieces = (rows_up + most - 1) / most;
+        piece = up((rows_up + pieces - 1) / pieces, bm);
+    }
+    const uint32_t pieces = (uint32_t)((rows_up + piece - 1) / piece);
+    a.groups = rows_up / LOSS_GROUP;
+    const uint32_t chunks_per_piece = std::min<uint32_t>(std::max<uint32_t>(1, LOSS_CHUNKS / pieces), (uint32_t)((piece / LOSS_GROUP + 31) / 32));
+    a.chunks = chunks_per_piece * pieces;
+    // grad q: tiles of 128 x 256 (fp32: 128 x 128), or 32 queries; enough splits of the rows to fill the GPU twice over
+    const uint32_t qm = form == 2 ? 32 : 128, qn = sizeof(T) == 4 ? 128 : 256;
+    const uint32_t gq_q_tiles = (a.qp + qm - 1) / qm, gq_n_tiles = (a.dim + qn - 1) / qn;
+    const uint32_t piece_groups = (uint32_t)(piece / LOSS_GROUP);
+    uint32_t splits = std::max<uint32_t>(1, (uint32_t)(2 * ctx->num_cus) / (gq_q_tiles * gq_n_tiles));
+    if (splits >= 8) splits = splits / 8 * 8;
+    splits = std::min(splits, piece_groups);
+    const uint32_t per_split = (piece_groups + splits - 1) / splits;
+    splits = (piece_groups + per_split - 1) / per_split;
+    a.splits = splits;
+
+    // workspace
+    size_t bytes = 0;
+    auto take = [&](size_t b) {
+        const size_t at = bytes;
+        bytes += (b + 1023) / 1024 * 1024;
+        return at;
+    };
+    const size_t o_ref = take((size_t)a.groups * a.qp * 4), o_sum = take((size_t)a.groups * a.qp * 4);
+    const size_t o_cr = take((size_t)a.chunks * a.qp * 4), o_cs = take((size_t)a.chunks * a.qp * 4);
+    const size_t o_lw = take((size_t)a.qp * 8), o_top = take(4), o_on = take(a.qp / 8 + 8);
+    const size_t o_blocks = take(gq || gx ? (size_t)a.qp * piece * sizeof(T) : 0);
+    const size_t o_part = take(gq ? (size_t)splits * a.qp * a.dim * 4 : 0);
+    const size_t o_pr0 = take((size_t)splits * a.qp * 4), o_pr1 = take((size_t)splits * a.qp * 4);
+    char* ws = nullptr;
+    APOE_TRY(ctx->adapt_workspace(bytes, &ws));
+    a.ref = (float*)(ws + o_ref);
+    a.sum = (float*)(ws + o_sum);
+    a.chunk_ref = (float*)(ws + o_cr);
+    a.chunk_sum = (float*)(ws + o_cs);
+    a.lse_w = (float2*)(ws + o_lw);
+    a.top_coef = (uint32_t*)(ws + o_top);
+    a.blocks = ws + o_blocks;
+    a.part = (float*)(ws + o_part);
+    a.part_ref[0] = (float*)(ws + o_pr0);
+    a.part_ref[1] = (float*)(ws + o_pr1);
+    uint32_t* q_on = (uint32_t*)(ws + o_on);
+    hipStream_t s = ctx->stream;
+
+    auto set_piece = [&](uint32_t i) {
+        a.row0 = (uint32_t)(i * piece);
+        const uint32_t rows = (uint32_t)std::min<uint64_t>(piece, rows_up - a.row0);
+        a.row_tiles = rows / bm;
+        a.row_blocks = rows / 32;
+        return rows / LOSS_GROUP;
+    };
+    auto tiles = [&](auto mode) {
+        constexpr int M = decltype(mode)::value;
+        const dim3 grid(a.row_tiles * a.q_tiles);
+        if (form == 0) loss_tile<T, 2, 2, 2, 2, 3, M><<<grid, 256, 0, s>>>(a);
+        else if (form == 1) loss_tile<T, 2, 4, 1, 2, 2, M><<<grid, 256, 0, s>>>(a);
+        else loss_tile<T, 1, 4, 1, 4, 2, M><<<grid, 256, 0, s>>>(a);
+    };
+    auto grad_q = [&](auto exp, uint32_t groups, int turn, int first) {
+        constexpr bool E = decltype(exp)::value;
+        const uint32_t keep = a.q_tiles;
+        a.q_tiles = gq_q_tiles;
+        const dim3 grid(gq_q_tiles * gq_n_tiles * splits);
+        if constexpr (sizeof(T) == 4) {
+            if (form == 2) loss_grad_q<T, 1, 1, 1, 4, 2, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
+            else loss_grad_q<T, 2, 2, 2, 2, 2, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
+        } else {
+            if (form == 2) loss_grad_q<T, 1, 2, 1, 4, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
+            else loss_grad_q<T, 2, 4, 2, 2, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
+        }
+        a.q_tiles = keep;
+    };
+    using Sums = std::integral_constant<int, TILE_SUMS>;
+    using Exp = std::integral_constant<int, TILE_EXP>;
+    using Grad = std::integral_constant<int, TILE_GRAD>;
+    const uint32_t join_q = a.qp / 32;
+    if (!two_pass) {
+        for (uint32_t i = 0; i < pieces; i++) {
+            const uint32_t groups = set_piece(i);
+            if (gq) tiles(Exp{});
+            else tiles(Sums{});
+            const dim3 grid(join_q, chunks_per_piece);
+            if (gq) loss_join<T, true><<<grid, 256, 0, s>>>(a, a.row0 / LOSS_GROUP, groups, i * chunks_per_piece);
+            else loss_join<T, false><<<grid, 256, 0, s>>>(a, a.row0 / LOSS_GROUP, groups, i * chunks_per_piece);
+            if (gq) grad_q(std::true_type{}, groups, (int)(i & 1), i == 0);
+        }
+        const int turn = (int)((pieces - 1) & 1);
+        if (gq) loss_finish<T, true, true><<<a.nq, 256, 0, s>>>(a, turn);
+        else loss_finish<T, false, false><<<a.nq, 256, 0, s>>>(a, turn);
+        APOE_HIP(hipGetLastError());
+        return APOE_OK;
+    }
+    for (uint32_t i = 0; i < pieces; i++) {
+        const uint32_t groups = set_piece(i);
+        tiles(Sums{});
+        loss_join<T, false><<<dim3(join_q, chunks_per_piece), 256, 0, s>>>(a, a.row0 / LOSS_GROUP, groups, i * chunks_per_piece);
+    }
+    loss_coefs<<<a.qp, 64, 0, s>>>(a);
+    loss_q_on<<<(a.qp + 63) / 64, 64, 0, s>>>(a, q_on);
+    const uint32_t xn = sizeof(T) == 4 ? 64 : 128, x_tiles = (a.dim + xn - 1) / xn;
+    for (uint32_t i = 0; i < pieces; i++) {
+        const uint32_t groups = set_piece(i);
+        tiles(Grad{});
+        loss_targets<T><<<a.nq, 64, 0, s>>>(a);
+        if (gq) grad_q(std::false_type{}, groups, 0, i == 0);
+        const dim3 grid((a.row_blocks + 7) / 8 * x_tiles);
+        if constexpr (sizeof(T) == 4) loss_grad_x<T, 4, 1, 2, 2, 2><<<grid, 256, 0, s>>>(a, x_tiles, q_on);
+        else loss_grad_x<T, 4, 2, 2, 2, 3><<<grid, 256, 0, s>>>(a, x_tiles, q_on);
+    }
+    if (gq) loss_finish<T, true, false><<<a.nq, 256, 0, s>>>(a, 0);
+    else loss_finish<T, false, false><<<a.nq, 256, 0, s>>>(a, 0);
+    APOE_HIP(hipGetLastError());
+    return APOE_OK;
+}
+
+int launch_softmax_loss(apoe_ctx* ctx, const apoe_softmax_loss_args* p) {
+    switch (p->dtype) {
+    case APOE_F32: return run_loss<float>(ctx, p);
+    case APOE_F16: return run_loss<_Float16>(ctx, p);
+    default: return run_loss<__bf16>(ctx, p);
+    }
+}
+
+} // namespace apoe

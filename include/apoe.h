@@ -49,8 +49,12 @@ const char* apoe_last_error_string(void);
 
 /* Replaces the implicit "device 0, default stream" of the reference. */
 int apoe_ctx_create(int device, apoe_ctx** out);
+/* A context whose work runs on a stream of the caller's (a hipStream_t; NULL: the default stream), in order with what else the caller
+ * puts there. The stream must outlive the context. */
+int apoe_ctx_create_on_stream(int device, void* stream, apoe_ctx** out);
 void apoe_ctx_destroy(apoe_ctx* ctx);
 int apoe_ctx_synchronize(apoe_ctx* ctx);
+int apoe_ctx_stream(const apoe_ctx* ctx, void** stream); /* the hipStream_t that the context's work runs on */
 
 /*
  * Corpus upload. Replaces the cudaMalloc/cudaMemcpy block of build_index_impl
@@ -290,6 +294,50 @@ int apoe_search(apoe_ctx* ctx, const apoe_corpus* c, const apoe_queries* q, cons
 int apoe_search_noalloc(apoe_ctx* ctx, const apoe_corpus* c, const apoe_queries* q, const apoe_graph* g,
                         const apoe_kg* kg, const apoe_search_params* p, uint32_t* out_ids, float* out_dist,
                         apoe_search_stats* stats);
+
+/*
+ * Fitting a query adapter to a stored index. New path weights need no rebuild, because weights are folded into the query;
+ * in the same way a learned map of the dense queries changes what is found while the rows and their graph stay. The three
+ * operators below are what a training step of such a map (or of the encoders themselves) needs beside plain matrix products:
+ * a loss over the rows, the frame of the map's block, and the step of its matrices. No counterpart in the reference.
+ *
+ * All three enqueue on the context's stream and return without waiting. Every pointer is device memory of the context's GPU,
+ * 16-byte aligned where it is a matrix; strides are in elements, from one row to the next, and 0 means dense. Inputs and
+ * outputs must not overlap unless a comment says so. Workspace is kept by the context and grows to the largest request (a
+ * call that grows it waits for the GPU and cannot be captured into a graph; a call of the same sizes after it can).
+ */
+#define APOE_F32 0u
+#define APOE_F16 1u
+#define APOE_BF16 2u
+#define APOE_LOSS_MAX_DIM 4096u /* columns that apoe_softmax_loss takes */
+
+typedef struct {
+    uint32_t dtype;             /* of q, rows, grad_q, grad_rows; sums, statistics and the loss are float */
+    uint32_t n_queries, n_rows; /* n_rows < 2^30 */
+    uint32_t dim;               /* at most APOE_LOSS_MAX_DIM, a multiple of 8 (APOE_F32: 4) */
+    const void* q;              /* [n_queries][dim] */
+    const void* rows;           /* [n_rows][dim]; NULL: the half-precision rows of `corpus` */
+    const apoe_corpus* corpus;  /* with rows == NULL: apoe_corpus_make_half_rows has run, dtype is APOE_F16 */
+    uint64_t q_stride, rows_stride, grad_q_stride, grad_rows_stride; /* multiples of 8 (APOE_F32: 4), at most 2^18 */
+    const uint32_t *t_off, *t_idx; /* CSR: the rows that are relevant to each query (entries at or above n_rows count nothing); t_off
+                                      may be NULL without gradients (lse alone) */
+    const float* t_val;         /* their weights; NULL: equal shares that sum to one */
+    const uint32_t* live;       /* bit i % 32 of word i / 32: row i takes part (NULL: all do). What other rows hold is not looked at */
+    const float* weight;        /* [n_queries] of the queries in the sum that is differentiated; NULL: 1. With APOE_F16 it is also the
+                                   place for a loss scale: gradients below 6e-5 lose bits in that type */
+    float scale;                /* of the inner products (one over the temperature), positive */
+    float *loss, *lse;          /* [n_queries], either may be NULL */
+    void *grad_q, *grad_rows;   /* like q and rows; either may be NULL */
+} apoe_softmax_loss_args;
+
+/*
+ * Softmax cross entropy of every query over the live rows, and the gradient of sum_i weight_i loss_i:
+ *   s_ij = scale <q_i, x_j>, lse_i = log sum_j exp(s_ij), W_i = sum_t w_it, loss_i = W_i lse_i - sum_t w_it s_it.
+ * Without live rows lse is -inf; without live targets loss and gradient are zero, whatever the query holds; a dead row's
+ * gradient is zero. The logits are never in memory as a whole: the workspace is bounded (256 MiB of exponentials, and
+ * 8 bytes for every 128 logits).
+ */
+int apoe_softmax_loss(apoe_ctx* ctx, const apoe_softmax_loss_args* args);
 
 #ifdef __cplusplus
 }
