@@ -8,6 +8,8 @@ using namespace apoe;
 
 namespace {
 
+constexpr uint32_t ORTHO_MAX_SIDE = 65536; // 128 rows of a working matrix stay within a 31-bit offset
+
 size_t size_of(uint32_t dtype) { return dtype == APOE_F32 ? 4 : 2; }
 
 // Device memory of the context's GPU, aligned.
@@ -66,6 +68,32 @@ int apoe_softmax_loss(apoe_ctx* ctx, const apoe_softmax_loss_args* args) {
     APOE_REQUIRE(a.n_queries >= 1, "grad_rows without queries");
     APOE_HIP(hipSetDevice(ctx->device));
     return launch_softmax_loss(ctx, &a);
+}
+
+int apoe_orthogonalize(apoe_ctx* ctx, const apoe_orthogonalize_args* args) {
+    APOE_REQUIRE(ctx && args, "ctx/args is null");
+    apoe_orthogonalize_args a = *args;
+    APOE_REQUIRE(a.in_dtype <= APOE_BF16 && a.out_dtype <= APOE_BF16, "unknown dtype %u or %u", a.in_dtype, a.out_dtype);
+    APOE_REQUIRE(a.products == APOE_F16 || a.products == APOE_F32, "products must be APOE_F16 or APOE_F32, got %u", a.products);
+    APOE_REQUIRE(a.rows <= ORTHO_MAX_SIDE && a.cols <= ORTHO_MAX_SIDE, "a side of %u x %u is beyond %u", a.rows, a.cols, ORTHO_MAX_SIDE);
+    APOE_REQUIRE(a.batch <= 65535, "batch of %u is beyond 65535", a.batch);
+    APOE_REQUIRE(a.steps >= 1 && a.steps <= 64, "steps must be in 1..64, got %u", a.steps);
+    APOE_REQUIRE(std::isfinite(a.a) && std::isfinite(a.b) && std::isfinite(a.c) && std::isfinite(a.alpha) && std::isfinite(a.beta), "a coefficient is not finite");
+    if (a.batch == 0 || a.rows == 0 || a.cols == 0) return APOE_OK;
+    if (a.in_stride == 0) a.in_stride = a.cols;
+    if (a.out_stride == 0) a.out_stride = a.cols;
+    APOE_REQUIRE(a.in_stride >= a.cols && a.out_stride >= a.cols, "rows overlap: strides %llu, %llu for %u columns", (unsigned long long)a.in_stride,
+                 (unsigned long long)a.out_stride, a.cols);
+    const uint64_t in_matrix = (uint64_t)(a.rows - 1) * a.in_stride + a.cols, out_matrix = (uint64_t)(a.rows - 1) * a.out_stride + a.cols;
+    if (a.in_batch_stride == 0) a.in_batch_stride = a.rows * a.in_stride;
+    if (a.out_batch_stride == 0) a.out_batch_stride = a.rows * a.out_stride;
+    APOE_REQUIRE(a.batch == 1 || (a.in_batch_stride >= in_matrix && a.out_batch_stride >= out_matrix), "matrices overlap: strides %llu, %llu",
+                 (unsigned long long)a.in_batch_stride, (unsigned long long)a.out_batch_stride);
+    APOE_REQUIRE(a.in && a.out, "in/out is null");
+    APOE_POINTER(a.in, size_of(a.in_dtype), "in");
+    APOE_POINTER(a.out, size_of(a.out_dtype), "out");
+    APOE_HIP(hipSetDevice(ctx->device));
+    return launch_orthogonalize(ctx, &a);
 }
 
 } // extern "C"

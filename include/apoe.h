@@ -339,6 +339,27 @@ typedef struct {
  */
 int apoe_softmax_loss(apoe_ctx* ctx, const apoe_softmax_loss_args* args);
 
+typedef struct {
+    uint32_t in_dtype, out_dtype;
+    uint32_t products;        /* APOE_F16: fp16 products on an fp32 iterate (off by 1e-4 to 6e-4 of the result; for bfloat16 results);
+                                 APOE_F32: products of 22 bits and more (1e-6 to 2e-5, as fp32 products have), at about twice the time */
+    uint32_t batch, rows, cols;
+    uint64_t in_stride, out_stride; /* from row to row */
+    uint64_t in_batch_stride, out_batch_stride; /* from matrix to matrix; 0: rows * stride */
+    const void* in;
+    void* out;                /* may be `in` itself when types and strides are equal */
+    uint32_t steps;           /* 1 .. 64 */
+    float a, b, c;            /* of the quintic a x + b x^3 + c x^5 */
+    float alpha, beta;        /* out = alpha X + beta out; out is not read when beta is 0 */
+} apoe_orthogonalize_args;
+
+/*
+ * Newton-Schulz: X = in / |in| (Frobenius; a zero matrix stays zero), then `steps` times X = a X + (b A + c A A) X with A = X X^T,
+ * on the short side, which drives the singular values towards one. Coefficients under which an entry of X passes 15 are beyond it
+ * (the result is then not finite). Any sizes and alignments of rows are taken.
+ */
+int apoe_orthogonalize(apoe_ctx* ctx, const apoe_orthogonalize_args* args);
+
 #ifdef __cplusplus
 }
 #endif
