@@ -55,6 +55,16 @@ class OrthogonalizeArgs(C.Structure):
                 ("a", C.c_float), ("b", C.c_float), ("c", C.c_float), ("alpha", C.c_float), ("beta", C.c_float)]
 
 
+class GatedResidualArgs(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("rows", C.c_uint32), ("dim", C.c_uint32), ("gate_kind", C.c_uint32),
+                ("x_stride", C.c_uint64), ("h_stride", C.c_uint64), ("gate_stride", C.c_uint64), ("y_stride", C.c_uint64), ("u_stride", C.c_uint64),
+                ("x", C.c_void_p), ("h", C.c_void_p), ("gate", C.c_void_p), ("scale", C.c_void_p), ("w_post", C.c_void_p), ("w_next", C.c_void_p),
+                ("eps", C.c_float), ("y", C.c_void_p), ("u", C.c_void_p),
+                ("grad_y_stride", C.c_uint64), ("grad_u_stride", C.c_uint64), ("grad_x_stride", C.c_uint64), ("grad_h_stride", C.c_uint64), ("grad_gate_stride", C.c_uint64),
+                ("grad_y", C.c_void_p), ("grad_u", C.c_void_p), ("grad_x", C.c_void_p), ("grad_h", C.c_void_p), ("grad_gate", C.c_void_p),
+                ("grad_scale", C.c_void_p), ("grad_w_post", C.c_void_p), ("grad_w_next", C.c_void_p)]
+
+
 EXPORTS = [
     "apoe_last_error_string", "apoe_ctx_create", "apoe_ctx_destroy", "apoe_ctx_synchronize", "apoe_corpus_create", "apoe_corpus_create_without",
     "apoe_corpus_destroy", "apoe_corpus_info", "apoe_corpus_bytes", "apoe_corpus_pair_bytes", "apoe_corpus_make_half_rows", "apoe_queries_create", "apoe_queries_destroy",
@@ -63,7 +73,7 @@ EXPORTS = [
     "apoe_knn_download", "apoe_knn_upload", "apoe_knn_download_reverse", "apoe_knn_upload_reverse", "apoe_knn_set_prune_form", "apoe_prune", "apoe_prune_download", "apoe_finalize_graph",
     "apoe_knn_elapsed_ms", "apoe_knn_counters", "apoe_knn_read_counters", "apoe_graph_create", "apoe_graph_destroy", "apoe_graph_info", "apoe_graph_download",
     "apoe_search", "apoe_search_noalloc",
-    "apoe_ctx_create_on_stream", "apoe_ctx_stream", "apoe_softmax_loss", "apoe_orthogonalize",
+    "apoe_ctx_create_on_stream", "apoe_ctx_stream", "apoe_softmax_loss", "apoe_orthogonalize", "apoe_gated_residual", "apoe_gated_residual_grad",
 ]
 
 
@@ -610,4 +620,73 @@ def orthogonalize(ctx, x, out=None, steps=5, coefs=COEFS, alpha=1.0, beta=0.0, p
     a.alpha, a.beta = alpha, beta
     with _in_order(ctx):
         _check(lib().apoe_orthogonalize(ctx.h, C.byref(a)))
+    return out
+
+
+def _residual_args(ctx, x, h, gate, scale, w_post, w_next, eps):
+    import torch
+    a = GatedResidualArgs()
+    a.dtype = _dtype(x, "x")
+    a.x_stride = _matrix(ctx, x, "x")
+    n, d = x.shape
+    a.rows, a.dim, a.eps, a.x = n, d, eps, x.data_ptr()
+    if h is not None:
+        a.h_stride, a.h = _matrix(ctx, h, "h", (n, d), x.dtype), h.data_ptr()
+    elif gate is not None or scale is not None or w_post is not None:
+        raise ApoeError("gate, scale and w_post belong to a block: h is None")
+    if gate is not None:
+        if gate.dim() == 1:
+            a.gate_kind, a.gate = 2, _vector(ctx, gate, "gate", d, (x.dtype,))
+        else:
+            a.gate_kind, a.gate_stride, a.gate = 1, _matrix(ctx, gate, "gate", (n, d), x.dtype), gate.data_ptr()
+    for t, name in ((scale, "scale"), (w_post, "w_post"), (w_next, "w_next")):
+        if t is not None:
+            setattr(a, name, _vector(ctx, t, name, d, (torch.float32,)))
+    return a
+
+
+def gated_residual(ctx, x, h=None, gate=None, scale=None, w_post=None, w_next=None, eps=1e-6, want_u=True):
+    """(y, u): y = x + scale * sigmoid(gate) * w_post * h / rms(h) and u = w_next * y / rms(y). gate: [n, d] or [d]; without h,
+    y is x itself and u its norm."""
+    import torch
+    a = _residual_args(ctx, x, h, gate, scale, w_post, w_next, eps)
+    y = x if h is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    u = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_u else None
+    if x.numel() == 0:
+        return y, u
+    a.y = None if h is None else y.data_ptr()
+    a.u = None if u is None else u.data_ptr()
+    with _in_order(ctx):
+        _check(lib().apoe_gated_residual(ctx.h, C.byref(a)))
+    return y, u
+
+
+def gated_residual_grad(ctx, x, h=None, gate=None, scale=None, w_post=None, w_next=None, eps=1e-6, grad_y=None, grad_u=None):
+    """Gradients of gated_residual from those of y and u (either may be None): a dict of grad_x, and of grad_h, grad_gate,
+    grad_scale, grad_w_post, grad_w_next for the inputs that are not None."""
+    import torch
+    a = _residual_args(ctx, x, h, gate, scale, w_post, w_next, eps)
+    n, d = x.shape
+    if grad_y is None and grad_u is None:
+        raise ApoeError("neither grad_y nor grad_u")
+    for t, name in ((grad_y, "grad_y"), (grad_u, "grad_u")):
+        if t is not None:
+            setattr(a, name + "_stride", _matrix(ctx, t, name, (n, d), x.dtype))
+            setattr(a, name, t.data_ptr())
+    out = dict(grad_x=torch.empty((n, d), dtype=x.dtype, device=x.device))
+    if h is not None:
+        out["grad_h"] = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    if gate is not None:
+        out["grad_gate"] = torch.empty(gate.shape, dtype=x.dtype, device=x.device)
+    for t, name in ((scale, "grad_scale"), (w_post, "grad_w_post"), (w_next, "grad_w_next")):
+        if t is not None:
+            out[name] = torch.empty(d, dtype=torch.float32, device=x.device)
+    if x.numel() == 0:
+        for v in out.values():
+            v.zero_()
+        return out
+    for name, t in out.items():
+        setattr(a, name, t.data_ptr())
+    with _in_order(ctx):
+        _check(lib().apoe_gated_residual_grad(ctx.h, C.byref(a)))
     return out

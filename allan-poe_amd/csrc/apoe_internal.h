@@ -223,6 +223,7 @@ int launch_prune(apoe_knn* g, uint32_t degree);
 int launch_final_graph(apoe_knn* g, uint32_t* rows_dev);
 int launch_softmax_loss(apoe_ctx* ctx, const apoe_softmax_loss_args* args); // strides filled in
 int launch_orthogonalize(apoe_ctx* ctx, const apoe_orthogonalize_args* args);
+int launch_gated_residual(apoe_ctx* ctx, const apoe_gated_residual_args* args, bool grad);
 
 // Times `fn` (which enqueues work on ctx->stream) with HIP events; blocks until done.
 template <typename F>

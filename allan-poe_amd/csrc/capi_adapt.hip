@@ -96,4 +96,57 @@ int apoe_orthogonalize(apoe_ctx* ctx, const apoe_orthogonalize_args* args) {
     return launch_orthogonalize(ctx, &a);
 }
 
+static int gated_residual(apoe_ctx* ctx, const apoe_gated_residual_args* args, bool grad) {
+    APOE_REQUIRE(ctx && args, "ctx/args is null");
+    apoe_gated_residual_args a = *args;
+    APOE_REQUIRE(a.dtype <= APOE_BF16, "unknown dtype %u", a.dtype);
+    APOE_REQUIRE(a.dim >= 1 && a.dim <= APOE_RESIDUAL_MAX_DIM, "dim must be in 1..%u, got %u", APOE_RESIDUAL_MAX_DIM, a.dim);
+    APOE_REQUIRE(a.gate_kind <= APOE_GATE_CHANNEL, "unknown kind of gate %u", a.gate_kind);
+    APOE_REQUIRE((a.gate_kind == APOE_GATE_NONE) == (a.gate == nullptr), "gate and gate_kind disagree");
+    APOE_REQUIRE(a.h || (!a.gate && !a.scale && !a.w_post && !a.grad_h && !a.grad_gate && !a.grad_scale && !a.grad_w_post), "gate, scale and w_post belong to a block: h is null");
+    APOE_REQUIRE(std::isfinite(a.eps) && a.eps >= 0.f, "eps must not be negative, got %g", a.eps);
+    uint64_t* strides[] = {&a.x_stride, &a.h_stride, &a.gate_stride, &a.y_stride, &a.u_stride, &a.grad_y_stride, &a.grad_u_stride, &a.grad_x_stride, &a.grad_h_stride,
+                           &a.grad_gate_stride};
+    for (uint64_t* s : strides) {
+        if (*s == 0) *s = a.dim;
+        APOE_REQUIRE(*s >= a.dim, "rows overlap: stride %llu for %u columns", (unsigned long long)*s, a.dim);
+    }
+    if (grad) {
+        APOE_REQUIRE(a.grad_y || a.grad_u, "neither grad_y nor grad_u");
+        APOE_REQUIRE(a.gate_kind != APOE_GATE_NONE || !a.grad_gate, "grad_gate without a gate");
+        APOE_REQUIRE(a.grad_x || a.grad_h || a.grad_gate || a.grad_scale || a.grad_w_post || a.grad_w_next, "nothing to compute");
+        APOE_REQUIRE(a.grad_u || !a.grad_w_next, "grad_w_next needs grad_u");
+    } else {
+        APOE_REQUIRE((a.h && a.y) || a.u, "nothing to compute");
+    }
+    if (a.rows == 0 && !(grad && (a.grad_scale || a.grad_w_post || a.grad_w_next || (a.grad_gate && a.gate_kind == APOE_GATE_CHANNEL)))) return APOE_OK;
+    APOE_REQUIRE(a.x || a.rows == 0, "x is null");
+    const size_t e = size_of(a.dtype);
+    APOE_POINTER(a.x, e, "x");
+    APOE_POINTER(a.h, e, "h");
+    APOE_POINTER(a.gate, e, "gate");
+    APOE_POINTER(a.scale, 4, "scale");
+    APOE_POINTER(a.w_post, 4, "w_post");
+    APOE_POINTER(a.w_next, 4, "w_next");
+    if (grad) {
+        APOE_POINTER(a.grad_y, e, "grad_y");
+        APOE_POINTER(a.grad_u, e, "grad_u");
+        APOE_POINTER(a.grad_x, e, "grad_x");
+        APOE_POINTER(a.grad_h, e, "grad_h");
+        APOE_POINTER(a.grad_gate, e, "grad_gate");
+        APOE_POINTER(a.grad_scale, 4, "grad_scale");
+        APOE_POINTER(a.grad_w_post, 4, "grad_w_post");
+        APOE_POINTER(a.grad_w_next, 4, "grad_w_next");
+    } else {
+        APOE_POINTER(a.y, e, "y");
+        APOE_POINTER(a.u, e, "u");
+    }
+    APOE_HIP(hipSetDevice(ctx->device));
+    return launch_gated_residual(ctx, &a, grad);
+}
+
+int apoe_gated_residual(apoe_ctx* ctx, const apoe_gated_residual_args* args) { return gated_residual(ctx, args, false); }
+
+int apoe_gated_residual_grad(apoe_ctx* ctx, const apoe_gated_residual_args* args) { return gated_residual(ctx, args, true); }
+
 } // extern "C"

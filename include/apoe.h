@@ -310,6 +310,7 @@ int apoe_search_noalloc(apoe_ctx* ctx, const apoe_corpus* c, const apoe_queries*
 #define APOE_F16 1u
 #define APOE_BF16 2u
 #define APOE_LOSS_MAX_DIM 4096u /* columns that apoe_softmax_loss takes */
+#define APOE_RESIDUAL_MAX_DIM 8192u /* columns that apoe_gated_residual takes */
 
 typedef struct {
     uint32_t dtype;             /* of q, rows, grad_q, grad_rows; sums, statistics and the loss are float */
@@ -359,6 +360,35 @@ typedef struct {
  * (the result is then not finite). Any sizes and alignments of rows are taken.
  */
 int apoe_orthogonalize(apoe_ctx* ctx, const apoe_orthogonalize_args* args);
+
+#define APOE_GATE_NONE 0u
+#define APOE_GATE_ELEMENT 1u /* gate is [rows][dim] */
+#define APOE_GATE_CHANNEL 2u /* gate is [dim], the same for every row */
+
+typedef struct {
+    uint32_t dtype;          /* of x, h, gate, y, u and their gradients; vectors are float */
+    uint32_t rows, dim;      /* dim at most APOE_RESIDUAL_MAX_DIM; rows == 0 is fine */
+    uint32_t gate_kind;
+    uint64_t x_stride, h_stride, gate_stride, y_stride, u_stride;
+    const void *x, *h, *gate;  /* h == NULL: no block yet, y = x (and y is not written) */
+    const float *scale, *w_post, *w_next; /* [dim]; NULL: ones */
+    float eps;
+    void *y, *u;             /* u may be NULL */
+    /* the gradient: what comes in (either may be NULL, not both) and what goes out (each may be NULL) */
+    uint64_t grad_y_stride, grad_u_stride, grad_x_stride, grad_h_stride, grad_gate_stride;
+    const void *grad_y, *grad_u;
+    void *grad_x, *grad_h, *grad_gate;
+    float *grad_scale, *grad_w_post, *grad_w_next;
+} apoe_gated_residual_args;
+
+/*
+ * A block's output h on its way back into the stream of rows x, and the norm in front of the next block:
+ *   y = x + scale * sigmoid(gate) * w_post * h / rms(h),  u = w_next * y / rms(y),  rms(v) = sqrt(mean v^2 + eps)
+ * (u is of unit length with eps = 0 and w_next = 1 / sqrt(dim): what the index searches with.) apoe_gated_residual_grad forms
+ * the gradients from x, h and gate alone: nothing is kept from the forward call. y and u may be NULL there.
+ */
+int apoe_gated_residual(apoe_ctx* ctx, const apoe_gated_residual_args* args);
+int apoe_gated_residual_grad(apoe_ctx* ctx, const apoe_gated_residual_args* args);
 
 #ifdef __cplusplus
 }
