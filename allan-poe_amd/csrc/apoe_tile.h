@@ -78,19 +78,35 @@ template <int YOUNGER> __device__ inline void tile_wait() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(YOUNGER) : "memory");
 }
 
+// The order of a stage's instructions: the first fragments' READS, then with the MFMAS of each fragment the next one's reads, so that
+// no product waits for a read that was just sent off. The code around it reads fragment f + 1 before it multiplies f.
+template <int READS, int MFMAS, int SF> __device__ inline void interleave() {
+    constexpr int READ = 0x100, MFMA = 0x008;
+    __builtin_amdgcn_sched_group_barrier(READ, READS, 0);
+#pragma unroll
+    for (int f = 0; f + 1 < SF; f++) {
+#pragma unroll
+        for (int i = 0; i < MFMAS; i++) {
+            __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+            if (i < READS) __builtin_amdgcn_sched_group_barrier(READ, (READS + MFMAS - 1) / MFMAS, 0);
+        }
+    }
+    __builtin_amdgcn_sched_group_barrier(MFMA, MFMAS, 0);
+}
+
 // ROWS rows of a matrix whose inner dimension is contiguous; SF fragments a stage. 16-byte pieces of a row lie in LDS at a place
-// that the row's number turns (xor), so that 8 consecutive rows' equal pieces are in different banks.
+// that the row's number turns (xor), so that 16 consecutive rows' equal pieces, which one cycle reads, are in different banks.
 template <typename T, int ROWS, int SF, int NW> struct RowTile {
     static constexpr int BYTES = ROWS * SF * 32, LOADS = BYTES / (1024 * NW), PIECES = SF * 2;
     static constexpr int KE = SF * 32 / (int)sizeof(T); // inner indices of a stage
-    static_assert(BYTES % (1024 * NW) == 0 && (SF == 2 || SF == 4), "whole loads");
+    static_assert(BYTES % (1024 * NW) == 0 && (SF == 2 || SF == 4) && NW % 2 == 0, "whole loads");
     uint32_t offset[LOADS], piece;
     uint64_t base;
-    __device__ static int turn(int row) { return SF == 2 ? (row >> 1) & 3 : row & 7; }
+    __device__ static int turn(int row) { return SF == 2 ? (row >> 2) & 3 : (row >> 1) & 7; }
     // row0: the tile's first row; rows: how many of the tile's rows exist
     __device__ void init(const T* row0, uint32_t pitch_bytes, int rows, int wave, int lane) {
         base = uniform64((uint64_t)row0);
-        piece = (uint32_t)((lane % PIECES) ^ turn(lane / PIECES));
+        piece = (uint32_t)((lane % PIECES) ^ turn(wave * (64 / PIECES) + lane / PIECES)); // loads of a wave are 16 rows apart or a multiple
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
             const int row = (i * NW + wave) * (64 / PIECES) + lane / PIECES;

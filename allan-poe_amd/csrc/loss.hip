@@ -26,14 +26,14 @@ constexpr uint32_t LOSS_CHUNKS = 64;               // parts that the join of the
 template <typename T> __device__ inline float as_float(T v) { return (float)v; }
 
 // ---- blocks of 32 queries x 32 rows ----
-// Part p (16 bytes a lane) holds values 8 p .. 8 p + 7 (fp32: 4 p ..) of a lane's 16; half 1 is turned by four lanes, so that
-// the transposed read finds the halves in different banks.
+// Part p (16 bytes a lane) holds values 8 p .. 8 p + 7 (fp32: 4 p ..) of a lane's 16; half 1 is turned by four lanes and odd parts
+// by eight, so that the transposed read finds halves and parts in different banks.
 template <typename T> struct Block {
     static constexpr int BYTES = 1024 * (int)sizeof(T), PARTS = BYTES / 1024, VALUES = 16 / (int)sizeof(T);
-    __device__ static int slot(int query, int half) { return half * 32 + (query ^ (half * 4)); }
+    __device__ static int slot(int query, int half, int part) { return half * 32 + (query ^ (half * 4) ^ ((part & 1) * 8)); }
     __device__ static uint32_t place(int query, int row) { // byte offset of one value
         const int half = (row >> 2) & 1, i = ((row >> 3) << 2) | (row & 3);
-        return (uint32_t)((i / VALUES) * 1024 + slot(query, half) * 16 + (i % VALUES) * (int)sizeof(T));
+        return (uint32_t)((i / VALUES) * 1024 + slot(query, half, i / VALUES) * 16 + (i % VALUES) * (int)sizeof(T));
     }
 };
 
@@ -65,7 +65,8 @@ struct LossArgs {
     float *ref, *sum;           // [n / LOSS_GROUP][qp]
     float *chunk_ref, *chunk_sum; // [LOSS_CHUNKS][qp]
     float2* lse_w;              // [qp]: lse in base 2, weight W (to be multiplied with exp(s - lse))
-    uint32_t* top_coef;         // largest |weight| (|W| + sum |w|), as bits
+    float* coef;                // [qp]: |weight| (|W| + sum |w|)
+    uint32_t *top_coef, *q_on;  // the largest of them, as bits; those that are not zero, as a bit mask
     char* blocks;
     float* part;                // [splits][qp][dim]
     float* part_ref[2];         // [splits][qp]
@@ -101,7 +102,7 @@ template <typename T> __device__ inline i32x4 pack(const float* p) {
 }
 
 template <typename T, int NT, int WM, int WN, int SF, int ST, int MODE>
-__global__ __launch_bounds__(64 * WM * WN, 2) void loss_tile(LossArgs a) {
+__global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossArgs a) {
     constexpr int NW = WM * WN, BM = WM * 128, BN = WN * NT * 32;
     using ATile = RowTile<T, BM, SF, NW>;
     using BTile = RowTile<T, BN, SF, NW>;
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_tile(LossArgs a) {
     const uint32_t row = a.row0 + rt * BM, query = qt * BN;
     ATile ta;
     BTile tb;
-    ta.init(reinterpret_cast<const T*>((const char*)a.rows + (uint64_t)row * a.r_pitch), a.r_pitch, (int)min((uint32_t)BM, a.n - row), wave, lane);
+    ta.init(reinterpret_cast<const T*>((const char*)a.rows + (uint64_t)row * a.r_pitch), a.r_pitch, (int)(row < a.n ? min((uint32_t)BM, a.n - row) : 0u), wave, lane);
     tb.init(reinterpret_cast<const T*>((const char*)a.q + (uint64_t)query * a.q_pitch), a.q_pitch, (int)min((uint32_t)BN, a.nq - query), wave, lane);
     const int bytes = (int)(a.dim * sizeof(T)), stages = (bytes + SF * 32 - 1) / (SF * 32);
     const uint32_t base = lds_address(lds);
@@ -142,18 +143,23 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_tile(LossArgs a) {
         issue();
         const char* A = lds + from;
         const char* B = A + ATile::BYTES;
+        i32x4 x[2][4], y[2][NT];
+        auto read = [&](int f) {
+#pragma unroll
+            for (int m = 0; m < 4; m++) x[f & 1][m] = ATile::read(A, wm * 4 + m, f, lane);
+#pragma unroll
+            for (int t = 0; t < NT; t++) y[f & 1][t] = BTile::read(B, wn * NT + t, f, lane);
+        };
+        read(0);
 #pragma unroll
         for (int f = 0; f < SF; f++) {
-            i32x4 x[4], y[NT];
-#pragma unroll
-            for (int m = 0; m < 4; m++) x[m] = ATile::read(A, wm * 4 + m, f, lane);
-#pragma unroll
-            for (int t = 0; t < NT; t++) y[t] = BTile::read(B, wn * NT + t, f, lane);
+            if (f + 1 < SF) read(f + 1);
 #pragma unroll
             for (int m = 0; m < 4; m++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) acc[m][t] = mfma_step<T>(x[m], y[t], acc[m][t]);
+                for (int t = 0; t < NT; t++) acc[m][t] = mfma_step<T>(x[f & 1][m], y[f & 1][t], acc[m][t]);
         }
+        if constexpr (sizeof(T) == 2) interleave<4 + NT, 4 * NT, SF>();
         from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
     }
     // epilogue: one query a lane (and its other half), 128 rows a wave
@@ -177,7 +183,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_tile(LossArgs a) {
             }
         }
         float p[16];
-        char* out = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((wrow - a.row0) >> 5)) * Block<T>::BYTES + Block<T>::slot(lane & 31, h) * 16;
+        char* out = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((wrow - a.row0) >> 5)) * Block<T>::BYTES;
         if constexpr (MODE == TILE_GRAD) {
             const float2 lw = a.lse_w[qi];
             const float g = lw.y * grad_scale_of(a.top_coef);
@@ -190,7 +196,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_tile(LossArgs a) {
                     p[i] = g == 0.f || z == -INFINITY ? 0.f : g * __builtin_amdgcn_exp2f(__builtin_fmaf(z, c, -lw.x));
                 }
 #pragma unroll
-                for (int k = 0; k < Block<T>::PARTS; k++) *reinterpret_cast<i32x4*>(out + m * Block<T>::BYTES + k * 1024) = pack<T>(p + k * Block<T>::VALUES);
+                for (int k = 0; k < Block<T>::PARTS; k++) *reinterpret_cast<i32x4*>(out + m * Block<T>::BYTES + k * 1024 + Block<T>::slot(lane & 31, h, k) * 16) = pack<T>(p + k * Block<T>::VALUES);
             }
         } else {
             float top = -INFINITY;
@@ -212,7 +218,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_tile(LossArgs a) {
                 }
                 if constexpr (MODE == TILE_EXP) {
 #pragma unroll
-                    for (int k = 0; k < Block<T>::PARTS; k++) *reinterpret_cast<i32x4*>(out + m * Block<T>::BYTES + k * 1024) = pack<T>(p + k * Block<T>::VALUES);
+                    for (int k = 0; k < Block<T>::PARTS; k++) *reinterpret_cast<i32x4*>(out + m * Block<T>::BYTES + k * 1024 + Block<T>::slot(lane & 31, h, k) * 16) = pack<T>(p + k * Block<T>::VALUES);
                 }
             }
             sum += __shfl_xor(sum, 32);
@@ -243,7 +249,6 @@ template <typename T, bool ZERO> __global__ __launch_bounds__(256) void loss_joi
     __shared__ float sr[8][32], ss[8][32];
     const uint32_t ql = threadIdx.x & 31, gl = threadIdx.x >> 5, qi = blockIdx.x * 32 + ql;
     const uint32_t per = (groups + gridDim.y - 1) / gridDim.y, g0 = blockIdx.y * per, g1 = min(g0 + per, groups);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *a.top_coef = 0;
     float ref = -INFINITY, sum = 0.f;
     for (uint32_t g = g0 + gl; g < g1; g += 8) {
         const size_t at = (size_t)(group0 + g) * a.qp + qi;
@@ -310,7 +315,28 @@ __global__ __launch_bounds__(64) void loss_coefs(LossArgs a) {
     if (lane == 0) {
         const float c = a.weight ? a.weight[qi] : 1.f;
         a.lse_w[qi] = make_float2(lse, c * W);
-        atomicMax(a.top_coef, __float_as_uint(fabsf(c) * (fabsf(W) + A))); // a maximum does not depend on the order
+        a.coef[qi] = fabsf(c) * (fabsf(W) + A);
+    }
+}
+
+// The largest coefficient, and which queries count something (what the others hold is not multiplied), as bits: one workgroup.
+__global__ __launch_bounds__(1024) void loss_queries(LossArgs a) {
+    __shared__ uint32_t top[16];
+    uint32_t most = 0; // of floats that are not negative, as bits
+    for (uint32_t q0 = 0; q0 < a.qp; q0 += 1024) {
+        const uint32_t qi = q0 + threadIdx.x;
+        const uint32_t c = qi < a.nq ? __float_as_uint(a.coef[qi]) : 0;
+        most = max(most, c);
+        const unsigned long long b = __ballot(c != 0);
+        if ((threadIdx.x & 31) == 0 && qi < a.qp) a.q_on[qi >> 5] = (uint32_t)(b >> (threadIdx.x & 32));
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
+    if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < 16; k++) most = max(most, top[k]);
+        *a.top_coef = most;
     }
 }
 
@@ -481,7 +507,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
             i32x4 x[MT], y[NT];
 #pragma unroll
             for (int m = 0; m < MT; m++) {
-                x[m] = *reinterpret_cast<const i32x4*>(A + (wm * MT + m) * Block<T>::BYTES + f * 1024 + Block<T>::slot(lane & 31, lane >> 5) * 16);
+                x[m] = *reinterpret_cast<const i32x4*>(A + (wm * MT + m) * Block<T>::BYTES + f * 1024 + Block<T>::slot(lane & 31, lane >> 5, f) * 16);
                 if constexpr (EXP) x[m] = scale_down<T>(x[m], less[m]);
             }
 #pragma unroll
@@ -528,14 +554,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
 
 // grad x of a piece: rows (blocks read transposed) x queries. Each row's gradient is whole here: all queries are in.
 template <typename T, int MT, int NT, int WM, int WN, int ST>
-__global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint32_t n_tiles, const uint32_t* q_on_words) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint32_t n_tiles) {
     constexpr int NW = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, SF = sizeof(T) == 4 ? 4 : 2;
     using BTile = ColTile<T, BN, SF, NW, ORDER_ROWS>;
     constexpr int ABYTES = BM / 32 * Block<T>::BYTES, ALOADS = ABYTES / (1024 * NW);
     constexpr int STAGE = ABYTES + BTile::BYTES, PER = ALOADS + BTile::LOADS;
     __shared__ __align__(1024) char lds[ST * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
-    const uint32_t rt = blockIdx.x / n_tiles, col = blockIdx.x % n_tiles * BN, block0 = rt * (BM / 32);
+    uint32_t rt = blockIdx.x / n_tiles, col = blockIdx.x % n_tiles * BN;
+    const uint32_t whole = gridDim.x / n_tiles / 8 * 8;
+    if (blockIdx.x < whole * n_tiles) { // the column tiles of one tile of rows, which read the same blocks, on one XCD
+        const uint32_t i = blockIdx.x >> 3;
+        rt = (i / n_tiles) * 8 + (blockIdx.x & 7);
+        col = i % n_tiles * BN;
+    }
+    const uint32_t block0 = rt * (BM / 32);
     uint32_t aoff[ALOADS];
 #pragma unroll
     for (int i = 0; i < ALOADS; i++) {
@@ -546,7 +579,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint3
     const uint64_t astep = (uint64_t)a.row_blocks * Block<T>::BYTES;
     BTile tb;
     tb.init(reinterpret_cast<const T*>(a.q) + col, a.q_pitch, (int)min((uint32_t)BN, a.dim - col), wave, lane);
-    const UniformWords q_on = (UniformWords)q_on_words;
+    const UniformWords q_on = (UniformWords)a.q_on;
     const int stages = (int)((a.nq + 31) / 32);
     const uint32_t base = lds_address(lds);
     uint32_t into = 0, issued = 0;
@@ -583,7 +616,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint3
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         const int q = f * 16 + 8 * h + 4 * j + (i >> 2);
-                        const char* p = block + g * 1024 + Block<T>::slot(q, i & 1) * 16 + ((i & 3) >> 1) * 8;
+                        const char* p = block + g * 1024 + Block<T>::slot(q, i & 1, g) * 16 + ((i & 3) >> 1) * 8;
                         part[j] = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
                     }
                     x[m] = i32x4{part[0][0], part[0][1], part[1][0], part[1][1]};
@@ -621,18 +654,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint3
             }
         }
     }
-}
-
-// Queries that count something, as bits (what the other queries hold is not multiplied).
-__global__ __launch_bounds__(64) void loss_q_on(LossArgs a, uint32_t* __restrict__ out) {
-    const uint32_t qi = blockIdx.x * 64 + threadIdx.x;
-    bool on = false;
-    if (qi < a.nq && (!a.weight || a.weight[qi] != 0.f)) {
-        const uint32_t e0 = a.t_off[qi], e1 = a.t_off[qi + 1];
-        for (uint32_t e = e0; e < e1 && !on; e++) on = is_live(a, a.t_idx[e]) && target_weight(a, e, e0, e1) != 0.f;
-    }
-    const unsigned long long b = __ballot(on);
-    if ((threadIdx.x & 31) == 0) out[qi >> 5] = (uint32_t)(b >> (threadIdx.x & 32));
 }
 
 __device__ inline float block_sum(float v, float* buf) { // of 256 threads, the same for all
@@ -772,9 +793,12 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.lse = p->lse;
     a.grad_q = p->grad_q;
     a.grad_x = p->grad_rows;
-    // tiles: 256 rows x 128 queries, or 512 x 64 or 32 for few queries
-    const int form = a.nq <= 32 ? 2 : a.nq <= 64 ? 1 : 0;
-    const uint32_t bm = form ? 512 : 256, bn = form == 2 ? 32 : form == 1 ? 64 : 128;
+    // Tiles: 256 rows x 256 queries where that pads no more queries than 128 would (or few) and fills the GPU, 16-bit types
+    // (1024 x 65 536 of 1024 columns: 1040 TFLOP/s, which is what the library's product of these shapes reaches; 256 x 128: 900), else 256 x 128, or 512 x 64 or 32 for few queries.
+    const uint32_t wide_tiles = (a.n + 255) / 256 * ((a.nq + 255) / 256);
+    const bool wide = sizeof(T) == 2 && wide_tiles >= (uint32_t)ctx->num_cus && (up(a.nq, 256) == up(a.nq, 128) || a.nq > 1024);
+    const int form = a.nq <= 32 ? 2 : a.nq <= 64 ? 1 : wide ? 3 : 0;
+    const uint32_t bm = form == 1 || form == 2 ? 512 : 256, bn = form == 2 ? 32 : form == 1 ? 64 : form == 3 ? 256 : 128;
     a.qp = up(a.nq, bn);
     a.q_tiles = a.qp / bn;
     const uint32_t rows_up = up(a.n, bm);
@@ -808,7 +832,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     };
     const size_t o_ref = take((size_t)a.groups * a.qp * 4), o_sum = take((size_t)a.groups * a.qp * 4);
     const size_t o_cr = take((size_t)a.chunks * a.qp * 4), o_cs = take((size_t)a.chunks * a.qp * 4);
-    const size_t o_lw = take((size_t)a.qp * 8), o_top = take(4), o_on = take(a.qp / 8 + 8);
+    const size_t o_lw = take((size_t)a.qp * 8), o_top = take(4), o_on = take(a.qp / 8), o_coef = take((size_t)a.qp * 4);
     const size_t o_blocks = take(gq || gx ? (size_t)a.qp * piece * sizeof(T) : 0);
     const size_t o_part = take(gq ? (size_t)splits * a.qp * a.dim * 4 : 0);
     const size_t o_pr0 = take((size_t)splits * a.qp * 4), o_pr1 = take((size_t)splits * a.qp * 4);
@@ -824,7 +848,8 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.part = (float*)(ws + o_part);
     a.part_ref[0] = (float*)(ws + o_pr0);
     a.part_ref[1] = (float*)(ws + o_pr1);
-    uint32_t* q_on = (uint32_t*)(ws + o_on);
+    a.q_on = (uint32_t*)(ws + o_on);
+    a.coef = (float*)(ws + o_coef);
     hipStream_t s = ctx->stream;
 
     auto set_piece = [&](uint32_t i) {
@@ -837,6 +862,12 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     auto tiles = [&](auto mode) {
         constexpr int M = decltype(mode)::value;
         const dim3 grid(a.row_tiles * a.q_tiles);
+        if constexpr (sizeof(T) == 2) {
+            if (form == 3) {
+                loss_tile<T, 2, 2, 4, 4, 2, M><<<grid, 512, 0, s>>>(a);
+                return;
+            }
+        }
         if (form == 0) loss_tile<T, 2, 2, 2, 2, 3, M><<<grid, 256, 0, s>>>(a);
         else if (form == 1) loss_tile<T, 2, 4, 1, 2, 2, M><<<grid, 256, 0, s>>>(a);
         else loss_tile<T, 1, 4, 1, 4, 2, M><<<grid, 256, 0, s>>>(a);
@@ -881,7 +912,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         loss_join<T, false><<<dim3(join_q, chunks_per_piece), 256, 0, s>>>(a, a.row0 / LOSS_GROUP, groups, i * chunks_per_piece);
     }
     loss_coefs<<<a.qp, 64, 0, s>>>(a);
-    loss_q_on<<<(a.qp + 63) / 64, 64, 0, s>>>(a, q_on);
+    loss_queries<<<1, 1024, 0, s>>>(a);
     const uint32_t xn = sizeof(T) == 4 ? 64 : 128, x_tiles = (a.dim + xn - 1) / xn;
     for (uint32_t i = 0; i < pieces; i++) {
         const uint32_t groups = set_piece(i);
@@ -889,8 +920,8 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         loss_targets<T><<<a.nq, 64, 0, s>>>(a);
         if (gq) grad_q(std::false_type{}, groups, 0, i == 0);
         const dim3 grid((a.row_blocks + 7) / 8 * x_tiles);
-        if constexpr (sizeof(T) == 4) loss_grad_x<T, 4, 1, 2, 2, 2><<<grid, 256, 0, s>>>(a, x_tiles, q_on);
-        else loss_grad_x<T, 4, 2, 2, 2, 3><<<grid, 256, 0, s>>>(a, x_tiles, q_on);
+        if constexpr (sizeof(T) == 4) loss_grad_x<T, 4, 1, 2, 2, 2><<<grid, 256, 0, s>>>(a, x_tiles);
+        else loss_grad_x<T, 4, 2, 2, 2, 3><<<grid, 256, 0, s>>>(a, x_tiles);
     }
     if (gq) loss_finish<T, true, false><<<a.nq, 256, 0, s>>>(a, 0);
     else loss_finish<T, false, false><<<a.nq, 256, 0, s>>>(a, 0);
