@@ -10,7 +10,8 @@
 // fragment of the next product; a piece of them is at most LOSS_PIECE_BYTES.
 //   grad q alone: one pass. A piece's exponentials (relative to their own references) are multiplied with the piece's rows at
 //     once; what the references lack to the common one goes into the exponents of the fragments on their way to the product.
-//   grad x: the normalised G of a piece is needed, so the logits are formed again once lse is known.
+//   grad x: the normalised G is needed. Where one piece holds everything its exponentials are brought to G in place (a pass over
+//     memory: 38 us for 2048 x 30 522, forming the logits again 150 us); otherwise the logits are formed again once lse is known.
 // The targets' own terms are not left to the rounded blocks: their places are zeroed (or rewritten) and W p_t - w_t, which
 // nearly cancels for a query that is served well, is formed in 32 bits.
 #include "apoe_internal.h"
@@ -20,7 +21,9 @@ namespace apoe {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr uint32_t LOSS_GROUP = 128;               // rows that share a reference
-constexpr size_t LOSS_PIECE_BYTES = 256u << 20;    // of exponentials (or of G) that exist at a time
+// Of exponentials (or of G) that exist at a time. Each piece reads and writes the queries' partial sums once more: 1024 queries x 1 M
+// rows take 5.17 ms with pieces of 256 MiB, 4.82 ms with 1 GiB.
+constexpr size_t LOSS_PIECE_BYTES = 1u << 30;
 constexpr uint32_t LOSS_CHUNKS = 64;               // parts that the join of the sums is split into, at most
 
 template <typename T> __device__ inline float as_float(T v) { return (float)v; }
@@ -340,6 +343,37 @@ __global__ __launch_bounds__(1024) void loss_queries(LossArgs a) {
     }
 }
 
+// Exponentials to G in place, one wave a group of rows and 32 queries.
+template <typename T> __global__ __launch_bounds__(256) void loss_normalise(LossArgs a, uint32_t groups) {
+    const uint32_t wave = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t g = wave % groups, qb = wave / groups;
+    if (qb >= a.qp / 32) return;
+    char* block = a.blocks + ((size_t)qb * a.row_blocks + g * (LOSS_GROUP / 32)) * Block<T>::BYTES;
+    constexpr int LOADS = LOSS_GROUP / 32 * Block<T>::PARTS;
+    float f[2]; // of odd parts another lane's query
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint32_t qi = qb * 32 + (uint32_t)((int)(lane & 31) ^ ((int)(lane >> 5) * 4) ^ (k * 8)); // slot() is its own inverse within a half
+        const float ref = a.ref[(size_t)(a.row0 / LOSS_GROUP + g) * a.qp + qi];
+        const float2 lw = a.lse_w[qi];
+        const float c = lw.y * grad_scale_of(a.top_coef);
+        f[k] = c == 0.f || ref == -INFINITY ? 0.f : c * __builtin_amdgcn_exp2f(ref - lw.x);
+    }
+    i32x4 v[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) v[i] = *reinterpret_cast<const i32x4*>(block + i * 1024 + lane * 16);
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+        typedef T tv __attribute__((ext_vector_type(Block<T>::VALUES)));
+        const tv x = __builtin_bit_cast(tv, v[i]);
+        float p[Block<T>::VALUES];
+        const float c = f[i & 1]; // PARTS is even
+#pragma unroll
+        for (int k = 0; k < Block<T>::VALUES; k++) p[k] = c == 0.f ? 0.f : (float)x[k] * c;
+        *reinterpret_cast<i32x4*>(block + i * 1024 + lane * 16) = pack<T>(p);
+    }
+}
+
 template <typename T> __device__ inline float dot16(const char* x, const char* y) { // of 16 bytes each
     typedef T tv __attribute__((ext_vector_type(16 / sizeof(T))));
     const tv u = *reinterpret_cast<const tv*>(x), v = *reinterpret_cast<const tv*>(y);
@@ -502,21 +536,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
                 less[m] = own == -INFINITY ? 0.f : mine[m] - own; // a group without live rows holds zeros
             }
         }
+        i32x4 x[2][MT], y[2][NT];
+        auto read = [&](int f) {
+#pragma unroll
+            for (int m = 0; m < MT; m++) x[f & 1][m] = *reinterpret_cast<const i32x4*>(A + (wm * MT + m) * Block<T>::BYTES + f * 1024 + Block<T>::slot(lane & 31, lane >> 5, f) * 16);
+#pragma unroll
+            for (int t = 0; t < NT; t++) y[f & 1][t] = BTile::read(B, wn * NT + t, f, lane);
+        };
+        read(0);
 #pragma unroll
         for (int f = 0; f < SF; f++) {
-            i32x4 x[MT], y[NT];
+            if (f + 1 < SF) read(f + 1);
+            if constexpr (EXP) {
 #pragma unroll
-            for (int m = 0; m < MT; m++) {
-                x[m] = *reinterpret_cast<const i32x4*>(A + (wm * MT + m) * Block<T>::BYTES + f * 1024 + Block<T>::slot(lane & 31, lane >> 5, f) * 16);
-                if constexpr (EXP) x[m] = scale_down<T>(x[m], less[m]);
+                for (int m = 0; m < MT; m++) x[f & 1][m] = scale_down<T>(x[f & 1][m], less[m]);
             }
-#pragma unroll
-            for (int t = 0; t < NT; t++) y[t] = BTile::read(B, wn * NT + t, f, lane);
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) acc[m][t] = mfma_step<T>(x[m], y[t], acc[m][t]);
+                for (int t = 0; t < NT; t++) acc[m][t] = mfma_step<T>(x[f & 1][m], y[f & 1][t], acc[m][t]);
         }
+        if constexpr (sizeof(T) == 2) interleave<MT + 2 * NT, MT * NT, SF>();
         from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
     }
     tile_wait<0>();
@@ -603,9 +643,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint3
         issue();
         const char* A = lds + from;
         const char* B = A + ABYTES;
-#pragma unroll
-        for (int f = 0; f < SF; f++) {
-            i32x4 x[MT], y[NT];
+        i32x4 x[2][MT], y[2][NT];
+        auto read = [&](int f) {
 #pragma unroll
             for (int m = 0; m < MT; m++) {
                 const char* block = A + (wm * MT + m) * Block<T>::BYTES;
@@ -619,19 +658,25 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint3
                         const char* p = block + g * 1024 + Block<T>::slot(q, i & 1, g) * 16 + ((i & 3) >> 1) * 8;
                         part[j] = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
                     }
-                    x[m] = i32x4{part[0][0], part[0][1], part[1][0], part[1][1]};
+                    x[f & 1][m] = i32x4{part[0][0], part[0][1], part[1][0], part[1][1]};
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) x[m][j] = *reinterpret_cast<const int*>(block + Block<T>::place(f * 8 + 4 * h + j, lane & 31));
+                    for (int j = 0; j < 4; j++) x[f & 1][m][j] = *reinterpret_cast<const int*>(block + Block<T>::place(f * 8 + 4 * h + j, lane & 31));
                 }
             }
 #pragma unroll
-            for (int t = 0; t < NT; t++) y[t] = BTile::read(B, wn * NT + t, f, lane);
+            for (int t = 0; t < NT; t++) y[f & 1][t] = BTile::read(B, wn * NT + t, f, lane);
+        };
+        read(0);
+#pragma unroll
+        for (int f = 0; f < SF; f++) {
+            if (f + 1 < SF) read(f + 1);
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) acc[m][t] = mfma_step<T>(x[m], y[t], acc[m][t]);
+                for (int t = 0; t < NT; t++) acc[m][t] = mfma_step<T>(x[f & 1][m], y[f & 1][t], acc[m][t]);
         }
+        if constexpr (sizeof(T) == 2) interleave<2 * MT + 2 * NT, MT * NT, SF>();
         from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
     }
     tile_wait<0>();
@@ -812,11 +857,12 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.groups = rows_up / LOSS_GROUP;
     const uint32_t chunks_per_piece = std::min<uint32_t>(std::max<uint32_t>(1, LOSS_CHUNKS / pieces), (uint32_t)((piece / LOSS_GROUP + 31) / 32));
     a.chunks = chunks_per_piece * pieces;
-    // grad q: tiles of 128 x 256 (fp32: 128 x 128), or 32 queries; enough splits of the rows to fill the GPU twice over
-    const uint32_t qm = form == 2 ? 32 : 128, qn = sizeof(T) == 4 ? 128 : 256;
+    // grad q: tiles of 256 x 256, of 128 x 256 (fp32: 128 x 128), or of 32 queries; enough splits of the rows to fill the GPU (twice over
+    // where a CU holds two workgroups)
+    const uint32_t qm = form == 2 ? 32 : form == 3 ? 256 : 128, qn = sizeof(T) == 4 ? 128 : 256;
     const uint32_t gq_q_tiles = (a.qp + qm - 1) / qm, gq_n_tiles = (a.dim + qn - 1) / qn;
     const uint32_t piece_groups = (uint32_t)(piece / LOSS_GROUP);
-    uint32_t splits = std::max<uint32_t>(1, (uint32_t)(2 * ctx->num_cus) / (gq_q_tiles * gq_n_tiles));
+    uint32_t splits = std::max<uint32_t>(1, (uint32_t)((form == 3 ? 1 : 2) * ctx->num_cus) / (gq_q_tiles * gq_n_tiles));
     if (splits >= 8) splits = splits / 8 * 8;
     splits = std::min(splits, piece_groups);
     const uint32_t per_split = (piece_groups + splits - 1) / splits;
@@ -882,6 +928,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
             else loss_grad_q<T, 2, 2, 2, 2, 2, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
         } else {
             if (form == 2) loss_grad_q<T, 1, 2, 1, 4, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
+            else if (form == 3) loss_grad_q<T, 4, 2, 2, 4, 4, E><<<grid, 512, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
             else loss_grad_q<T, 2, 4, 2, 2, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
         }
         a.q_tiles = keep;
@@ -908,20 +955,25 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     }
     for (uint32_t i = 0; i < pieces; i++) {
         const uint32_t groups = set_piece(i);
-        tiles(Sums{});
+        if (pieces == 1) tiles(Exp{});
+        else tiles(Sums{});
         loss_join<T, false><<<dim3(join_q, chunks_per_piece), 256, 0, s>>>(a, a.row0 / LOSS_GROUP, groups, i * chunks_per_piece);
     }
     loss_coefs<<<a.qp, 64, 0, s>>>(a);
     loss_queries<<<1, 1024, 0, s>>>(a);
-    const uint32_t xn = sizeof(T) == 4 ? 64 : 128, x_tiles = (a.dim + xn - 1) / xn;
+    // grad x: tiles of 256 rows x 256 columns, or of 128 x 128 where those do not fill the GPU (fp32: 256 x 64)
+    const bool x_wide = sizeof(T) == 2 && (uint64_t)((piece + 255) / 256) * ((a.dim + 255) / 256) >= (uint32_t)ctx->num_cus;
+    const uint32_t xm = sizeof(T) == 4 || x_wide ? 256 : 128, xn = sizeof(T) == 4 ? 64 : x_wide ? 256 : 128, x_tiles = (a.dim + xn - 1) / xn;
     for (uint32_t i = 0; i < pieces; i++) {
         const uint32_t groups = set_piece(i);
-        tiles(Grad{});
+        if (pieces == 1) loss_normalise<T><<<(uint32_t)(((uint64_t)groups * (a.qp / 32) + 3) / 4), 256, 0, s>>>(a, groups);
+        else tiles(Grad{});
         loss_targets<T><<<a.nq, 64, 0, s>>>(a);
         if (gq) grad_q(std::false_type{}, groups, 0, i == 0);
-        const dim3 grid((a.row_blocks + 7) / 8 * x_tiles);
+        const dim3 grid((a.row_blocks * 32 + xm - 1) / xm * x_tiles);
         if constexpr (sizeof(T) == 4) loss_grad_x<T, 4, 1, 2, 2, 2><<<grid, 256, 0, s>>>(a, x_tiles);
-        else loss_grad_x<T, 4, 2, 2, 2, 3><<<grid, 256, 0, s>>>(a, x_tiles);
+        else if (x_wide) loss_grad_x<T, 4, 2, 2, 4, 4><<<grid, 512, 0, s>>>(a, x_tiles);
+        else loss_grad_x<T, 2, 2, 2, 2, 3><<<grid, 256, 0, s>>>(a, x_tiles);
     }
     if (gq) loss_finish<T, true, false><<<a.nq, 256, 0, s>>>(a, 0);
     else loss_finish<T, false, false><<<a.nq, 256, 0, s>>>(a, 0);

@@ -183,27 +183,32 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ortho_tile(OrthoArgs a) {
         issue();
         const char* A = lds + from;
         const char* B = A + ATile::BYTES;
-#pragma unroll
-        for (int f = 0; f < SF; f++) {
-            i32x4 x[PLANES][MT], y[PLANES][NT];
+        i32x4 x[2][PLANES][MT], y[2][PLANES][NT];
+        auto read = [&](int f) {
 #pragma unroll
             for (int p = 0; p < PLANES; p++) {
 #pragma unroll
-                for (int m = 0; m < MT; m++) x[p][m] = ATile::read(A + p * PLANE, wm * MT + m, f, lane);
+                for (int m = 0; m < MT; m++) x[f & 1][p][m] = ATile::read(A + p * PLANE, wm * MT + m, f, lane);
 #pragma unroll
-                for (int t = 0; t < NT; t++) y[p][t] = BTile::read(B + p * PLANE, wn * NT + t, f, lane);
+                for (int t = 0; t < NT; t++) y[f & 1][p][t] = BTile::read(B + p * PLANE, wn * NT + t, f, lane);
             }
+        };
+        read(0);
+#pragma unroll
+        for (int f = 0; f < SF; f++) {
+            if (f + 1 < SF) read(f + 1);
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     if constexpr (SPLIT) {
-                        acc[m][t] = mfma_step<T>(x[1][m], y[0][t], acc[m][t]);
-                        acc[m][t] = mfma_step<T>(x[0][m], y[1][t], acc[m][t]);
+                        acc[m][t] = mfma_step<T>(x[f & 1][1][m], y[f & 1][0][t], acc[m][t]);
+                        acc[m][t] = mfma_step<T>(x[f & 1][0][m], y[f & 1][1][t], acc[m][t]);
                     }
-                    acc[m][t] = mfma_step<T>(x[0][m], y[0][t], acc[m][t]);
+                    acc[m][t] = mfma_step<T>(x[f & 1][0][m], y[f & 1][0][t], acc[m][t]);
                 }
         }
+        interleave<PLANES * (MT + (SYM ? 1 : 2) * NT), (SPLIT ? 3 : 1) * MT * NT, SF>();
         from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
     }
     tile_wait<0>();

@@ -335,8 +335,8 @@ typedef struct {
  * Softmax cross entropy of every query over the live rows, and the gradient of sum_i weight_i loss_i:
  *   s_ij = scale <q_i, x_j>, lse_i = log sum_j exp(s_ij), W_i = sum_t w_it, loss_i = W_i lse_i - sum_t w_it s_it.
  * Without live rows lse is -inf; without live targets loss and gradient are zero, whatever the query holds; a dead row's
- * gradient is zero. The logits are never in memory as a whole: the workspace is bounded (256 MiB of exponentials, and
- * 8 bytes for every 128 logits).
+ * gradient is zero. The logits are never in memory as a whole: the workspace holds at most 1 GiB of exponentials at a time,
+ * 8 bytes for every 128 logits, and partial sums of grad_q.
  */
 int apoe_softmax_loss(apoe_ctx* ctx, const apoe_softmax_loss_args* args);
 

@@ -274,6 +274,61 @@ def test_more_than_one_piece(gpu_ctx, dtype, grad_rows):
         assert err < 2 * U[dtype] + 6e-5, err
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("grad_rows", [False, True])
+def test_pieces_of_a_gibibyte(gpu_ctx, dtype, grad_rows):
+    """8192 queries over rows whose exponentials pass 1 GiB, ragged, a tenth of them dead and holding NaN; one query in 64 names no row, the others
+    up to three, some of them dead. The formula in blocks on the GPU."""
+    import torch
+    import apoe
+    m, n, d = 8192, 35_005 if dtype == "float32" else 70_003, 16
+    g = torch.Generator(device="cuda").manual_seed(2)
+    dt = getattr(torch, dtype)
+    q = torch.randn(m, d, generator=g, device="cuda").to(dt)
+    x = torch.randn(n, d, generator=g, device="cuda").to(dt)
+    on = torch.rand(n, generator=g, device="cuda") < 0.9
+    X = torch.where(on[:, None], x.double(), torch.zeros((), dtype=torch.float64, device="cuda"))
+    x[~on] = float("nan")
+    count = torch.arange(m, device="cuda") % 4
+    t_off = torch.zeros(m + 1, dtype=torch.int32, device="cuda")
+    t_off[1:] = torch.cumsum(count, 0)
+    t_idx = torch.randint(0, n, (int(t_off[-1]),), generator=g, device="cuda", dtype=torch.int32)
+    t_val = torch.rand(t_idx.shape[0], generator=g, device="cuda") + 0.5
+    weight = torch.rand(m, generator=g, device="cuda") + 0.5
+    scale = 0.5
+    got = apoe.softmax_loss(gpu_ctx, q, x, t_off, t_idx, t_val, scale=scale, weight=weight, live=pack_bits(on.cpu()).cuda(), grad_queries=True, grad_rows=grad_rows)
+    gx = torch.zeros(n, d, dtype=torch.float64, device="cuda")
+    u, tiny = U[dtype], 2.0 ** -24 if dtype == "float16" else 0.0
+    for r in range(0, m, 512):
+        Q = q[r:r + 512].double()
+        z = scale * Q @ X.T
+        z[:, ~on] = -float("inf")
+        lse = torch.logsumexp(z, 1)
+        e0, e1 = int(t_off[r]), int(t_off[r + 512])
+        t, k = t_idx[e0:e1].long(), torch.repeat_interleave(torch.arange(512, device="cuda"), count[r:r + 512])
+        w = torch.zeros(512, n, dtype=torch.float64, device="cuda").index_put_((k, t), t_val[e0:e1].double(), accumulate=True)
+        w[:, ~on] = 0
+        W = w.sum(1)
+        loss = W * lse - (w * torch.where(on, z, torch.zeros_like(z))).sum(1)
+        p = torch.exp(z - lse[:, None])
+        c = scale * weight[r:r + 512, None].double()
+        mass = c * (W[:, None] * p + w)
+        G = c * (W[:, None] * p - w)
+        # |logit| < 50 or so: off by 0.5 * 20 * 2^-24 * 50 = 3e-5, p by twice that
+        off = 2 * u + 6e-5 + (n + m) * 2.0 ** -24
+        assert bool(((got["loss"][r:r + 512] - loss).abs() <= W * (6e-5 + 2.0 ** -20 * lse.abs()) + 6e-5 + 2.0 ** -20 * loss.abs()).all())
+        assert bool(((got["lse"][r:r + 512] - lse).abs() <= 3e-5 + 2.0 ** -20 * lse.abs()).all())
+        gq = G @ X
+        tol = off * (mass @ X.abs()) + u * gq.abs() + 2.0 ** -24 * (dtype == "float16") + tiny * 2 * c * (W[:, None] + 3) * p.max(1, keepdim=True).values * X.abs().sum(0)
+        assert bool(((got["grad_queries"][r:r + 512].double() - gq).abs() <= tol).all())
+        gx += G.T.contiguous() @ Q
+        del z, p, w, mass, G
+    if grad_rows:
+        assert not bool(got["grad_rows"][~on].any())
+        err = float((got["grad_rows"].double() - gx).norm() / gx.norm())
+        assert err < 2 * u + 6e-5, err
+
+
 def test_gradients_against_differences(gpu_ctx):
     """Central differences of the kernel's own loss along random directions, float32. Truncation: the third derivative along a unit
     direction is at most (2 scale)^3 |W| a query; rounding: the losses' own error over the step."""
