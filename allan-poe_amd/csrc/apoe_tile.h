@@ -64,6 +64,12 @@ __device__ inline uint64_t uniform64(uint64_t v) {
 
 __device__ inline i32x4 buffer_of(uint64_t base) { return i32x4{(int)(uint32_t)base, (int)(uint32_t)(base >> 32), (int)TILE_RANGE, 0x00020000}; }
 
+// Workgroups go to the eight XCDs in turn, each of which has an L2 of its own. The number that gives each XCD a run of consecutive tiles.
+__device__ inline uint32_t xcd_run(uint32_t id, uint32_t total) {
+    const uint32_t per = total / 8;
+    return id < per * 8 ? (id & 7) * per + (id >> 3) : id;
+}
+
 // 16 bytes a lane from base + offset to LDS at lds + 16 lane. lds and the descriptor are the same in the wave.
 __device__ inline void load_to_lds16(i32x4 buffer, uint32_t offset, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(buffer) : "memory");

@@ -26,7 +26,7 @@ struct OrthoArgs {
     void* out;
     uint64_t in_stride, out_stride, in_batch, out_batch; // elements
     uint32_t in_dtype, out_dtype, m, n, mp, np, parts;   // m <= n: the sides; mp, np: rounded up
-    bool tall;
+    bool tall, whole_out; // worked on transposed; rows of `out` are multiples of 16 bytes
     float a, b, c, alpha, beta;
     double* part;  // [batch][ORTHO_PARTS]
     float* x;      // [batch][m][np] the iterate
@@ -55,31 +55,98 @@ __device__ inline void store_from_float(void* p, uint64_t i, uint32_t dtype, flo
     else ((__bf16*)p)[i] = (__bf16)v;
 }
 
-// Sums of squares, in 64 bits (no input over- or underflows): grid (parts, batch), a part takes every parts-th row.
-__global__ __launch_bounds__(256) void ortho_squares(OrthoArgs a) {
+// Sums of squares, in 64 bits (no input over- or underflows): grid (parts, batch), a wave a row. WHOLE: rows are multiples of 16 bytes.
+template <bool WHOLE> __global__ __launch_bounds__(256) void ortho_squares(OrthoArgs a) {
     __shared__ double buf[4];
-    const uint32_t rows = a.tall ? a.n : a.m, cols = a.tall ? a.m : a.n;
+    const uint32_t rows = a.tall ? a.n : a.m, cols = a.tall ? a.m : a.n, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double s = 0;
-    for (uint32_t r = blockIdx.x; r < rows; r += gridDim.x)
-        for (uint32_t c = threadIdx.x; c < cols; c += 256) {
-            const double v = load_as_float(a.in, blockIdx.y * a.in_batch + r * a.in_stride + c, a.in_dtype);
-            s += v * v;
+    for (uint32_t r = blockIdx.x * 4 + wave; r < rows; r += gridDim.x * 4) {
+        const uint64_t at = blockIdx.y * a.in_batch + r * a.in_stride;
+        if constexpr (WHOLE) {
+            const uint32_t v = a.in_dtype == APOE_F32 ? 4 : 8;
+#pragma unroll 4
+            for (uint32_t c = lane * v; c < cols; c += 64 * v) {
+                if (a.in_dtype == APOE_F32) {
+                    const f32x4 x = *reinterpret_cast<const f32x4*>((const float*)a.in + at + c);
+                    for (int k = 0; k < 4; k++) s += (double)x[k] * (double)x[k];
+                } else if (a.in_dtype == APOE_F16) {
+                    const f16x8 x = *reinterpret_cast<const f16x8*>((const _Float16*)a.in + at + c);
+                    for (int k = 0; k < 8; k++) s += (double)((float)x[k] * (float)x[k]); // a square of 11 bits is exact in fp32
+                } else {
+                    const bf16x8 x = *reinterpret_cast<const bf16x8*>((const __bf16*)a.in + at + c);
+                    for (int k = 0; k < 8; k++) s += (double)(float)x[k] * (double)(float)x[k];
+                }
+            }
+        } else {
+            for (uint32_t c = lane; c < cols; c += 64) {
+                const double v = load_as_float(a.in, at + c, a.in_dtype);
+                s += v * v;
+            }
         }
+    }
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+    if (lane == 0) buf[wave] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) a.part[blockIdx.y * ORTHO_PARTS + blockIdx.x] = (buf[0] + buf[1]) + (buf[2] + buf[3]);
+}
+
+// One over the norm, from the parts; the same for all 256 threads.
+__device__ inline double ortho_inverse(const OrthoArgs& a, uint32_t batch, double* buf) {
+    double s = threadIdx.x < a.parts ? a.part[batch * ORTHO_PARTS + threadIdx.x] : 0.;
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
     if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) a.part[blockIdx.y * ORTHO_PARTS + blockIdx.x] = (buf[0] + buf[1]) + (buf[2] + buf[3]);
+    const double norm = sqrt((buf[0] + buf[1]) + (buf[2] + buf[3]));
+    return norm == 0. ? 0. : 1. / norm;
+}
+
+// X and its operand copy from rows that are multiples of 16 bytes (and not turned), eight values a thread: grid (.., batch).
+template <bool SPLIT> __global__ __launch_bounds__(256) void ortho_first_whole(OrthoArgs a) {
+    __shared__ double buf[4];
+    const double inv = ortho_inverse(a, blockIdx.y, buf);
+    const uint32_t per = a.np / 8, rows_at_once = gridDim.x * 256 / per;
+    const uint32_t at0 = blockIdx.x * 256 + threadIdx.x;
+    if (at0 >= rows_at_once * per) return;
+    const uint32_t j = at0 % per * 8;
+    for (uint32_t i = at0 / per; i < a.m; i += rows_at_once) {
+        const uint64_t from = blockIdx.y * a.in_batch + i * a.in_stride + j;
+        float v[8] = {};
+        if (j < a.n) {
+            if (a.in_dtype == APOE_F32) {
+#pragma unroll
+                for (int k = 0; k < 8; k += 4)
+                    if (j + k < a.n) {
+                        const f32x4 x = *reinterpret_cast<const f32x4*>((const float*)a.in + from + k);
+                        for (int l = 0; l < 4; l++) v[k + l] = x[l];
+                    }
+            } else if (a.in_dtype == APOE_F16) {
+                const f16x8 x = *reinterpret_cast<const f16x8*>((const _Float16*)a.in + from);
+                for (int k = 0; k < 8; k++) v[k] = (float)x[k];
+            } else {
+                const bf16x8 x = *reinterpret_cast<const bf16x8*>((const __bf16*)a.in + from);
+                for (int k = 0; k < 8; k++) v[k] = (float)x[k];
+            }
+        }
+        const uint64_t at = ((uint64_t)blockIdx.y * a.m + i) * a.np + j;
+        f16x8 hi, lo;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            v[k] = (float)(v[k] * inv);
+            hi[k] = (_Float16)(v[k] * ORTHO_UP);
+            lo[k] = (_Float16)(v[k] * ORTHO_UP - (float)hi[k]);
+        }
+        *reinterpret_cast<f32x4*>(a.x + at) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(a.x + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        *reinterpret_cast<f16x8*>(a.h + at) = hi;
+        if constexpr (SPLIT) *reinterpret_cast<f16x8*>(a.h + a.h_low + at) = lo;
+    }
 }
 
 // X and its operand copy, 64 x 64 at a time (through LDS where the matrix is turned): grid (np / 64, m / 64 up, batch).
 template <bool SPLIT> __global__ __launch_bounds__(256) void ortho_first(OrthoArgs a) {
     __shared__ double buf[4];
     __shared__ float tile[64][65];
-    double s = threadIdx.x < a.parts ? a.part[blockIdx.z * ORTHO_PARTS + threadIdx.x] : 0.;
-    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = s;
-    __syncthreads();
-    const double norm = sqrt((buf[0] + buf[1]) + (buf[2] + buf[3])), inv = norm == 0. ? 0. : 1. / norm;
+    const double inv = ortho_inverse(a, blockIdx.z, buf);
     const uint32_t i0 = blockIdx.y * 64, j0 = blockIdx.x * 64, tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
     const uint64_t in0 = blockIdx.z * a.in_batch;
     if (a.tall) {
@@ -100,6 +167,47 @@ template <bool SPLIT> __global__ __launch_bounds__(256) void ortho_first(OrthoAr
     }
 }
 
+template <bool SPLIT> __device__ inline void put8(_Float16* at, uint64_t low, const float* v) {
+    f16x8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        hi[k] = (_Float16)(v[k] * ORTHO_UP);
+        lo[k] = (_Float16)(v[k] * ORTHO_UP - (float)hi[k]);
+    }
+    *reinterpret_cast<f16x8*>(at) = hi;
+    if constexpr (SPLIT) *reinterpret_cast<f16x8*>(at + low) = lo;
+}
+
+// v = b A + c v, for eight values of A at `gram`.
+template <bool SPLIT> __device__ inline void ortho_poly(const OrthoArgs& a, const _Float16* gram, float* v) {
+    const f16x8 hi = *reinterpret_cast<const f16x8*>(gram);
+    f16x8 lo = {};
+    if constexpr (SPLIT) lo = *reinterpret_cast<const f16x8*>(gram + a.g_low);
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = __builtin_fmaf(a.c, v[k], a.b * ORTHO_DOWN * ((float)hi[k] + (float)lo[k]));
+}
+
+// Eight values into `out`, whose rows are multiples of 16 bytes (and of eight values).
+__device__ inline void add_row8(const OrthoArgs& a, uint64_t at, float* v) {
+    if (a.beta != 0.f)
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = __builtin_fmaf(a.beta, load_as_float(a.out, at + k, a.out_dtype), v[k]);
+    if (a.out_dtype == APOE_F32) {
+        *reinterpret_cast<f32x4*>((float*)a.out + at) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>((float*)a.out + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    } else if (a.out_dtype == APOE_F16) {
+        f16x8 x;
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = (_Float16)v[k];
+        *reinterpret_cast<f16x8*>((_Float16*)a.out + at) = x;
+    } else {
+        bf16x8 x;
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = (__bf16)v[k];
+        *reinterpret_cast<bf16x8*>((__bf16*)a.out + at) = x;
+    }
+}
+
 enum { ORTHO_GRAM = 0, ORTHO_POLY = 1, ORTHO_STEP = 2, ORTHO_LAST = 3 };
 
 // One product of a step. GRAM: A = X X^T; POLY: B = b A + c A A, whose diagonal goes to `diag`; both symmetric, so the tiles on and
@@ -115,20 +223,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ortho_tile(OrthoArgs a) {
     constexpr int PLANE = ATile::BYTES + BTile::BYTES, STAGE = PLANES * PLANE, PER = PLANES * (ATile::LOADS + BTile::LOADS), KE = ATile::KE;
     __shared__ __align__(1024) char lds[ST * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    const uint32_t id = xcd_run(blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y), tile = id % gridDim.x, batch = id / gridDim.x;
     uint32_t ti, tj;
     if constexpr (SYM) {
-        ti = (uint32_t)((sqrtf(8.f * blockIdx.x + 1.f) - 1.f) * 0.5f);
-        while (ti * (ti + 1) / 2 > blockIdx.x) ti--;
-        while ((ti + 1) * (ti + 2) / 2 <= blockIdx.x) ti++;
-        tj = blockIdx.x - ti * (ti + 1) / 2;
+        ti = (uint32_t)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
+        while (ti * (ti + 1) / 2 > tile) ti--;
+        while ((ti + 1) * (ti + 2) / 2 <= tile) ti++;
+        tj = tile - ti * (ti + 1) / 2;
         ti = __builtin_amdgcn_readfirstlane(ti);
         tj = __builtin_amdgcn_readfirstlane(tj);
     } else {
         const uint32_t nt = (a.n + BN - 1) / BN;
-        ti = blockIdx.x / nt;
-        tj = blockIdx.x % nt;
+        ti = tile / nt;
+        tj = tile % nt;
     }
-    const uint32_t row = ti * BM, col = tj * BN, batch = blockIdx.y;
+    const uint32_t row = ti * BM, col = tj * BN;
     const uint64_t xo = (uint64_t)batch * a.m * a.np, go = (uint64_t)batch * a.m * a.mp;
     const T* h = a.h + xo;
     const T* gram = a.gram + go;
@@ -212,71 +321,291 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ortho_tile(OrthoArgs a) {
         from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
     }
     tile_wait<0>();
+    // 64 rows at a time through LDS: then a thread has eight values of a row, of the tile and of the mirrored one
+    constexpr int PITCH = BN + 1, ITEMS = 64 * BN / 8 / (64 * NW), OWN = 64 / 32; // OWN: blocks of 32 rows of a wave in a chunk
+    static_assert(64 * PITCH * 4 <= ST * STAGE && MT % OWN == 0, "the sum fits the stages");
+    float* sum = reinterpret_cast<float*>(lds);
     const int half = lane >> 5;
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int chunk = 0; chunk < BM / 64; chunk++) {
+        const uint32_t crow = row + chunk * 64;
+        if (crow >= a.m) break;
+        if (wm == chunk / (MT / OWN)) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const uint32_t j = col + (wn * NT + t) * 32 + (lane & 31);
+            for (int o = 0; o < OWN; o++)
 #pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const uint32_t i0 = row + (wm * MT + m) * 32 + 8 * g + 4 * half;
-                float v[4];
+                for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) v[k] = acc[m][t][4 * g + k] * (ORTHO_DOWN * ORTHO_DOWN);
-                if constexpr (SYM) {
-                    if (j >= a.mp) continue;
-                    T* to = (KIND == ORTHO_GRAM ? a.gram : a.poly) + go;
+                    for (int k = 0; k < 16; k++)
+                        sum[(o * 32 + result_row(k, half)) * PITCH + (wn * NT + t) * 32 + (lane & 31)] = acc[chunk % (MT / OWN) * OWN + o][t][k] * (ORTHO_DOWN * ORTHO_DOWN);
+        }
+        __syncthreads();
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t i = i0 + k;
-                        if (i >= a.m) continue;
-                        const uint64_t at = (uint64_t)i * a.mp + j;
+        for (int item = 0; item < ITEMS; item++) {
+            const uint32_t at = item * 64 * NW + threadIdx.x;
+            if constexpr (SYM || KIND == ORTHO_STEP) {
+                const uint32_t r = at / (BN / 8), c = at % (BN / 8) * 8, i = crow + r, j = col + c;
+                if (i < a.m && j < (SYM ? a.mp : a.np)) {
+                    float v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) v[k] = sum[r * PITCH + c + k];
+                    if constexpr (SYM) {
                         if constexpr (KIND == ORTHO_POLY) {
-                            float own = (float)gram[at];
-                            if constexpr (SPLIT) own += (float)gram[at + a.g_low];
-                            v[k] = j < a.m ? __builtin_fmaf(a.c, v[k], a.b * ORTHO_DOWN * own) : 0.f;
-                            if (i == j) {
-                                a.diag[(uint64_t)batch * a.mp + i] = v[k];
-                                v[k] = 0.f;
-                            }
-                        }
-                        put<SPLIT>(to + at, a.g_low, v[k]);
-                    }
-                    if (ti != tj && j < a.m && i0 < a.mp) {
-                        // four values of a row at once; beyond m they are the zeros that the pad holds
-                        typedef T t4 __attribute__((ext_vector_type(4)));
-                        t4 hi, lo;
+                            ortho_poly<SPLIT>(a, gram + (uint64_t)i * a.mp + j, v);
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            hi[k] = (T)(v[k] * ORTHO_UP);
-                            lo[k] = (T)(v[k] * ORTHO_UP - (float)hi[k]);
+                            for (int k = 0; k < 8; k++)
+                                if (i == j + k) {
+                                    a.diag[(uint64_t)batch * a.mp + i] = v[k];
+                                    v[k] = 0.f;
+                                }
                         }
-                        T* at = to + (uint64_t)j * a.mp + i0;
-                        *reinterpret_cast<t4*>(at) = hi;
-                        if constexpr (SPLIT) *reinterpret_cast<t4*>(at + a.g_low) = lo;
-                    }
-                } else {
-                    if (j >= a.np) continue;
+                        put8<SPLIT>((KIND == ORTHO_GRAM ? a.gram : a.poly) + go + (uint64_t)i * a.mp + j, a.g_low, v);
+                    } else {
+                        const uint64_t o = xo + (uint64_t)i * a.np + j;
+                        const float d = a.a + a.diag[(uint64_t)batch * a.mp + i];
+                        const f32x4 x0 = *reinterpret_cast<const f32x4*>(a.x + o), x1 = *reinterpret_cast<const f32x4*>(a.x + o + 4);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t i = i0 + k;
-                        if (i >= a.m) continue;
-                        const uint64_t at = xo + (uint64_t)i * a.np + j;
-                        v[k] = __builtin_fmaf(a.a + a.diag[(uint64_t)batch * a.mp + i], a.x[at], v[k]);
-                        if constexpr (KIND == ORTHO_STEP) {
-                            a.x[at] = v[k];
-                            put<SPLIT>(a.h2 + at, a.h_low, v[k]);
-                        } else if (j < a.n) {
-                            const uint64_t o = batch * a.out_batch + (a.tall ? (uint64_t)j * a.out_stride + i : (uint64_t)i * a.out_stride + j);
-                            float r = a.alpha * v[k];
-                            if (a.beta != 0.f) r = __builtin_fmaf(a.beta, load_as_float(a.out, o, a.out_dtype), r);
-                            store_from_float(a.out, o, a.out_dtype, r);
-                        }
+                        for (int k = 0; k < 8; k++) v[k] = __builtin_fmaf(d, k < 4 ? x0[k] : x1[k - 4], v[k]);
+                        *reinterpret_cast<f32x4*>(a.x + o) = f32x4{v[0], v[1], v[2], v[3]};
+                        *reinterpret_cast<f32x4*>(a.x + o + 4) = f32x4{v[4], v[5], v[6], v[7]};
+                        put8<SPLIT>(a.h2 + o, a.h_low, v);
                     }
+                }
+                if constexpr (SYM) {
+                    const uint32_t mr = at / 8, mc = at % 8 * 8, mj = col + mr, mi = crow + mc;
+                    if (ti != tj && mj < a.m && mi < a.mp) {
+                        float v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) v[k] = sum[(mc + k) * PITCH + mr];
+                        if constexpr (KIND == ORTHO_POLY) ortho_poly<SPLIT>(a, gram + (uint64_t)mj * a.mp + mi, v);
+                        put8<SPLIT>((KIND == ORTHO_GRAM ? a.gram : a.poly) + go + (uint64_t)mj * a.mp + mi, a.g_low, v);
+                    }
+                }
+            } else if (a.whole_out) {
+                const uint32_t r = at / (BN / 8), c = at % (BN / 8) * 8, i = crow + r, j = col + c;
+                if (i < a.m && j < a.n) {
+                    const uint64_t o = xo + (uint64_t)i * a.np + j, to = batch * a.out_batch + (uint64_t)i * a.out_stride + j;
+                    const float d = a.a + a.diag[(uint64_t)batch * a.mp + i];
+                    const f32x4 x0 = *reinterpret_cast<const f32x4*>(a.x + o), x1 = *reinterpret_cast<const f32x4*>(a.x + o + 4);
+                    float v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) v[k] = a.alpha * __builtin_fmaf(d, k < 4 ? x0[k] : x1[k - 4], sum[r * PITCH + c + k]);
+                    add_row8(a, to, v);
+                }
+            } else {
+                // consecutive threads along a row of `out`
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const uint32_t e = (item * 8 + k) * 64 * NW + threadIdx.x;
+                    const uint32_t r = a.tall ? e % 64 : e / BN, c = a.tall ? e / 64 : e % BN, i = crow + r, j = col + c;
+                    if (i >= a.m || j >= a.n) continue;
+                    const uint64_t o = batch * a.out_batch + (a.tall ? (uint64_t)j * a.out_stride + i : (uint64_t)i * a.out_stride + j);
+                    float v = a.alpha * __builtin_fmaf(a.a + a.diag[(uint64_t)batch * a.mp + i], a.x[xo + (uint64_t)i * a.np + j], sum[r * PITCH + c]);
+                    if (a.beta != 0.f) v = __builtin_fmaf(a.beta, load_as_float(a.out, o, a.out_dtype), v);
+                    store_from_float(a.out, o, a.out_dtype, v);
                 }
             }
         }
+        __syncthreads();
+    }
+}
+
+// The same on tiles of 64 x 64 for matrices that larger tiles do not fill the GPU with. What counts then is the time of one tile:
+// eight waves, of which four take the even and four the odd half of a stage's fragments; what the epilogue needs of memory is
+// asked for before the first stage; and the sum goes through LDS, so that rows are written (and mirrored) 16 bytes a thread.
+template <bool SPLIT, int KIND> __global__ __launch_bounds__(512, 2) void ortho_small(OrthoArgs a) {
+    using T = _Float16;
+    constexpr int NW = 8, B = 64, SF = 4, ST = 3, PLANES = SPLIT ? 2 : 1, PITCH = 65;
+    constexpr bool SYM = KIND == ORTHO_GRAM || KIND == ORTHO_POLY;
+    using ATile = RowTile<T, B, SF, NW>;
+    using BTile = std::conditional_t<SYM, RowTile<T, B, SF, NW>, ColTile<T, B, SF, NW, ORDER_ROWS>>;
+    constexpr int PLANE = ATile::BYTES + BTile::BYTES, STAGE = PLANES * PLANE, PER = PLANES * (ATile::LOADS + BTile::LOADS), KE = ATile::KE;
+    static_assert(B * PITCH * 4 <= ST * STAGE, "the sum fits the stages");
+    __shared__ __align__(1024) char lds[ST * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = wave >> 2, wm = (wave >> 1) & 1, wn = wave & 1;
+    const uint32_t tile = blockIdx.x, batch = blockIdx.y;
+    uint32_t ti, tj;
+    if constexpr (SYM) {
+        ti = (uint32_t)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
+        while (ti * (ti + 1) / 2 > tile) ti--;
+        while ((ti + 1) * (ti + 2) / 2 <= tile) ti++;
+        tj = tile - ti * (ti + 1) / 2;
+        ti = __builtin_amdgcn_readfirstlane(ti);
+        tj = __builtin_amdgcn_readfirstlane(tj);
+    } else {
+        const uint32_t nt = (a.n + B - 1) / B;
+        ti = tile / nt;
+        tj = tile % nt;
+    }
+    const uint32_t row = ti * B, col = tj * B;
+    const uint64_t xo = (uint64_t)batch * a.m * a.np, go = (uint64_t)batch * a.m * a.mp;
+    const T* h = a.h + xo;
+    const T* gram = a.gram + go;
+    const T* poly = a.poly + go;
+    ATile ta[PLANES];
+    BTile tb[PLANES];
+    const uint32_t xp = a.np * (uint32_t)sizeof(T), gp = a.mp * (uint32_t)sizeof(T);
+    const int mrows = (int)min((uint32_t)B, a.m - row);
+#pragma unroll
+    for (int p = 0; p < PLANES; p++) {
+        const uint64_t hl = p * a.h_low, gl = p * a.g_low;
+        if constexpr (KIND == ORTHO_GRAM) {
+            ta[p].init(h + hl + (uint64_t)row * a.np, xp, mrows, wave, lane);
+            tb[p].init(h + hl + (uint64_t)col * a.np, xp, (int)min((uint32_t)B, a.m - col), wave, lane);
+        } else if constexpr (KIND == ORTHO_POLY) {
+            ta[p].init(gram + gl + (uint64_t)row * a.mp, gp, mrows, wave, lane);
+            tb[p].init(gram + gl + (uint64_t)col * a.mp, gp, (int)min((uint32_t)B, a.m - col), wave, lane);
+        } else {
+            ta[p].init(poly + gl + (uint64_t)row * a.mp, gp, mrows, wave, lane);
+            tb[p].init(h + hl + col, xp, (int)min((uint32_t)B, a.np - col), wave, lane);
+        }
+    }
+    // the epilogue's place: eight columns of a row (GRAM, POLY, STEP); eight values down a column or along a row (LAST)
+    const uint32_t er = threadIdx.x >> 3, ec = (threadIdx.x & 7) * 8, i = row + er, j = col + ec;
+    const uint32_t mi = row + ec, mj = col + er; // of the mirrored tile
+    f16x8 own = {}, own_low = {}, mir = {}, mir_low = {};
+    f32x4 x0 = {}, x1 = {};
+    float diag = 0.f, xl[8] = {}, dl[8] = {};
+    const bool turned = KIND == ORTHO_LAST && a.tall;
+    const uint32_t lc = threadIdx.x & 63, lr = threadIdx.x >> 6; // LAST: lc along the row of `out`
+    if constexpr (KIND == ORTHO_POLY) {
+        if (i < a.m) {
+            own = *reinterpret_cast<const f16x8*>(gram + (uint64_t)i * a.mp + j);
+            if constexpr (SPLIT) own_low = *reinterpret_cast<const f16x8*>(gram + a.g_low + (uint64_t)i * a.mp + j);
+        }
+        if (ti != tj && mj < a.m) {
+            mir = *reinterpret_cast<const f16x8*>(gram + (uint64_t)mj * a.mp + mi);
+            if constexpr (SPLIT) mir_low = *reinterpret_cast<const f16x8*>(gram + a.g_low + (uint64_t)mj * a.mp + mi);
+        }
+    } else if constexpr (KIND == ORTHO_STEP) {
+        if (i < a.m) {
+            diag = a.diag[(uint64_t)batch * a.mp + i];
+            x0 = *reinterpret_cast<const f32x4*>(a.x + xo + (uint64_t)i * a.np + j);
+            x1 = *reinterpret_cast<const f32x4*>(a.x + xo + (uint64_t)i * a.np + j + 4);
+        }
+    } else if constexpr (KIND == ORTHO_LAST) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const uint32_t r = row + (turned ? lc : lr + 8 * k), c = col + (turned ? lr + 8 * k : lc);
+            if (r < a.m) {
+                dl[k] = a.diag[(uint64_t)batch * a.mp + r];
+                xl[k] = a.x[xo + (uint64_t)r * a.np + c];
+            }
+        }
+    }
+    const int inner = (int)(KIND == ORTHO_GRAM ? a.np : a.mp);
+    const int stages = (inner + KE - 1) / KE;
+    const uint32_t base = lds_address(lds);
+    int left = inner;
+    uint32_t into = 0;
+    auto issue = [&]() {
+#pragma unroll
+        for (int p = 0; p < PLANES; p++) {
+            const uint32_t at = base + into + p * PLANE;
+            ta[p].load(at, left * (int)sizeof(T), wave);
+            if constexpr (SYM) {
+                tb[p].load(at + ATile::BYTES, left * (int)sizeof(T), wave);
+            } else {
+                using Mask = typename BTile::Mask;
+                const int rows = left - (int)(a.mp - a.m); // of X
+                tb[p].load(at + ATile::BYTES, rows >= KE ? BTile::ALL : rows > 0 ? (Mask)(((Mask)1 << rows) - 1) : (Mask)0, wave, lane);
+            }
+            ta[p].next();
+            tb[p].next();
+        }
+        left -= KE;
+        into = into + STAGE == ST * STAGE ? 0 : into + STAGE;
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; s++) issue();
+    f32x16 acc[2] = {}; // even and odd fragments: two chains
+    uint32_t from = 0;
+    for (int s = 0; s < stages; s++) {
+        tile_wait<(ST - 2) * PER>();
+        issue();
+        const char* A = lds + from;
+        const char* Bt = A + ATile::BYTES;
+        i32x4 x[2][PLANES], y[2][PLANES];
+#pragma unroll
+        for (int f = 0; f < 2; f++)
+#pragma unroll
+            for (int p = 0; p < PLANES; p++) {
+                x[f][p] = ATile::read(A + p * PLANE, wm, group * 2 + f, lane);
+                y[f][p] = BTile::read(Bt + p * PLANE, wn, group * 2 + f, lane);
+            }
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+            if constexpr (SPLIT) {
+                acc[f] = mfma_step<T>(x[f][1], y[f][0], acc[f]);
+                acc[f] = mfma_step<T>(x[f][0], y[f][1], acc[f]);
+            }
+            acc[f] = mfma_step<T>(x[f][0], y[f][0], acc[f]);
+        }
+        from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
+    }
+    tile_wait<0>();
+    float* sum = reinterpret_cast<float*>(lds);
+    const int half = lane >> 5;
+#pragma unroll
+    for (int g = 1; g >= 0; g--) {
+        if (group == g) {
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                float* at = sum + (wm * 32 + result_row(k, half)) * PITCH + wn * 32 + (lane & 31);
+                const float v = acc[0][k] + acc[1][k];
+                *at = g ? v : (*at + v) * (ORTHO_DOWN * ORTHO_DOWN);
+            }
+        }
+        __syncthreads();
+    }
+    if constexpr (SYM) {
+        T* to = (KIND == ORTHO_GRAM ? a.gram : a.poly) + go;
+        if (i < a.m) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                v[k] = sum[er * PITCH + ec + k];
+                if constexpr (KIND == ORTHO_POLY) {
+                    v[k] = __builtin_fmaf(a.c, v[k], a.b * ORTHO_DOWN * ((float)own[k] + (float)own_low[k]));
+                    if (i == j + k) {
+                        a.diag[(uint64_t)batch * a.mp + i] = v[k];
+                        v[k] = 0.f;
+                    }
+                }
+            }
+            put8<SPLIT>(to + (uint64_t)i * a.mp + j, a.g_low, v);
+        }
+        if (ti != tj && mj < a.m) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                v[k] = sum[(ec + k) * PITCH + er];
+                if constexpr (KIND == ORTHO_POLY) v[k] = __builtin_fmaf(a.c, v[k], a.b * ORTHO_DOWN * ((float)mir[k] + (float)mir_low[k]));
+            }
+            put8<SPLIT>(to + (uint64_t)mj * a.mp + mi, a.g_low, v);
+        }
+    } else if constexpr (KIND == ORTHO_STEP) {
+        if (i < a.m) {
+            float v[8];
+            const float d = a.a + diag;
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = __builtin_fmaf(d, k < 4 ? x0[k] : x1[k - 4], sum[er * PITCH + ec + k]);
+            const uint64_t at = xo + (uint64_t)i * a.np + j;
+            *reinterpret_cast<f32x4*>(a.x + at) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4*>(a.x + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+            put8<SPLIT>(a.h2 + at, a.h_low, v);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const uint32_t r = turned ? lc : lr + 8 * k, c = turned ? lr + 8 * k : lc;
+            if (row + r >= a.m || col + c >= a.n) continue;
+            const uint64_t o = batch * a.out_batch + (turned ? (uint64_t)(col + c) * a.out_stride + row + r : (uint64_t)(row + r) * a.out_stride + col + c);
+            float v = a.alpha * __builtin_fmaf(a.a + dl[k], xl[k], sum[r * PITCH + c]);
+            if (a.beta != 0.f) v = __builtin_fmaf(a.beta, load_as_float(a.out, o, a.out_dtype), v);
+            store_from_float(a.out, o, a.out_dtype, v);
+        }
+    }
 }
 
 template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonalize_args* p) {
@@ -299,7 +628,7 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
     a.c = p->c;
     a.alpha = p->alpha;
     a.beta = p->beta;
-    a.parts = std::min<uint32_t>(ORTHO_PARTS, p->rows);
+    a.parts = std::min<uint32_t>(ORTHO_PARTS, (p->rows + 3) / 4);
     const uint32_t batch = p->batch;
     size_t bytes = 0;
     auto take = [&](size_t b) {
@@ -323,22 +652,43 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
     a.gram = (_Float16*)(ws + o_gram);
     a.poly = (_Float16*)(ws + o_poly);
     hipStream_t s = ctx->stream;
-    ortho_squares<<<dim3(a.parts, batch), 256, 0, s>>>(a);
-    ortho_first<SPLIT><<<dim3(a.np / 64, (a.m + 63) / 64, batch), 256, 0, s>>>(a);
+    const uint32_t v = p->in_dtype == APOE_F32 ? 4 : 8;
+    const bool whole = p->cols % v == 0 && a.in_stride % v == 0 && (batch == 1 || a.in_batch % v == 0) && ((uintptr_t)a.in & 15) == 0;
+    a.whole_out = !a.tall && p->cols % 8 == 0 && a.out_stride % 8 == 0 && (batch == 1 || a.out_batch % 8 == 0) && ((uintptr_t)a.out & 15) == 0;
+    if (whole) ortho_squares<true><<<dim3(a.parts, batch), 256, 0, s>>>(a);
+    else ortho_squares<false><<<dim3(a.parts, batch), 256, 0, s>>>(a);
+    if (whole && !a.tall) {
+        const uint32_t per = a.np / 8; // at least one row at once, at most all of them
+        const uint32_t blocks = std::max((per + 255) / 256, std::min((uint32_t)(((uint64_t)a.m * per + 255) / 256), std::max(1u, 2048 / batch)));
+        ortho_first_whole<SPLIT><<<dim3(blocks, batch), 256, 0, s>>>(a);
+    } else {
+        ortho_first<SPLIT><<<dim3(a.np / 64, (a.m + 63) / 64, batch), 256, 0, s>>>(a);
+    }
+    // Tiles, by how many there are for the CUs (times of one product, 256 CUs, fp16):
+    //  256: symmetric products from half as many tiles as CUs on (4096 x 4096: X X^T 96 us; 128: 107)
+    //  128: from as many tiles as CUs on; for X X^T from half as many, where the rows are long (4 x 1024 x 4096: 40 us; 64: 53)
+    //  64: below (1024 x 1024: X X^T 9 us; 128: 12)
+    const uint32_t cus = (uint32_t)ctx->num_cus;
+    auto tiles = [](uint32_t side, uint32_t t) { return (side + t - 1) / t; };
     auto triangle = [](uint32_t t) { return t * (t + 1) / 2; };
-    // tiles of 128 x 128 where they fill the GPU, else of 64 x 64
-    const uint32_t t128 = (a.m + 127) / 128, t64 = (a.m + 63) / 64, n128 = (a.n + 127) / 128, n64 = (a.n + 63) / 64;
-    const bool wide_sym = (uint64_t)triangle(t128) * batch >= (uint32_t)ctx->num_cus;
-    const bool wide_step = (uint64_t)t128 * n128 * batch >= (uint32_t)ctx->num_cus;
+    const uint64_t s256 = (uint64_t)triangle(tiles(a.m, 256)) * batch, s128 = (uint64_t)triangle(tiles(a.m, 128)) * batch, x128 = (uint64_t)tiles(a.m, 128) * tiles(a.n, 128) * batch;
     auto sym = [&](auto kind) {
         constexpr int K = decltype(kind)::value;
-        if (wide_sym) ortho_tile<SPLIT, 2, 2, 2, 2, 2, SPLIT ? 2 : 3, K><<<dim3(triangle(t128), batch), 256, 0, s>>>(a);
-        else ortho_tile<SPLIT, 1, 1, 2, 2, SPLIT ? 2 : 4, 3, K><<<dim3(triangle(t64), batch), 256, 0, s>>>(a);
+        const uint32_t inner = K == ORTHO_GRAM ? a.n : a.m;
+        if constexpr (!SPLIT) {
+            if (s256 >= cus / 2) {
+                ortho_tile<SPLIT, 4, 2, 2, 4, 4, 2, K><<<dim3(triangle(tiles(a.m, 256)), batch), 512, 0, s>>>(a);
+                return;
+            }
+        }
+        if (s128 < cus && s128 >= cus / 2 && inner >= 4096) ortho_tile<SPLIT, 2, 1, 2, 4, SPLIT ? 2 : 4, 4, K><<<dim3(triangle(tiles(a.m, 128)), batch), 512, 0, s>>>(a);
+        else if (s128 >= cus) ortho_tile<SPLIT, 2, 1, 2, 4, 4, 2, K><<<dim3(triangle(tiles(a.m, 128)), batch), 512, 0, s>>>(a);
+        else ortho_small<SPLIT, K><<<dim3(triangle(tiles(a.m, 64)), batch), 512, 0, s>>>(a);
     };
     auto step = [&](auto kind) {
         constexpr int K = decltype(kind)::value;
-        if (wide_step) ortho_tile<SPLIT, 2, 2, 2, 2, 2, SPLIT ? 2 : 3, K><<<dim3(t128 * n128, batch), 256, 0, s>>>(a);
-        else ortho_tile<SPLIT, 1, 1, 2, 2, SPLIT ? 2 : 4, 3, K><<<dim3(t64 * n64, batch), 256, 0, s>>>(a);
+        if (x128 >= cus) ortho_tile<SPLIT, 2, 1, 2, 4, 4, 2, K><<<dim3(tiles(a.m, 128) * tiles(a.n, 128), batch), 512, 0, s>>>(a);
+        else ortho_small<SPLIT, K><<<dim3(tiles(a.m, 64) * tiles(a.n, 64), batch), 512, 0, s>>>(a);
     };
     for (uint32_t i = 0; i < p->steps; i++) {
         sym(std::integral_constant<int, ORTHO_GRAM>{});
