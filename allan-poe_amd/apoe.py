@@ -474,14 +474,20 @@ def search_noalloc(ctx, corpus, queries, graph, w3, cands, out_ids, out_dist, kg
 # ---- fitting a query adapter ----
 
 COEFS = (3.4445, -4.7750, 2.0315)  # quintic of five steps that bring singular values from 1e-3 on to between 0.7 and 1.2
-_DTYPES = None
+_torch = _DTYPES = _INTS = _FLOATS = None
+
+
+def _load_torch():
+    global _torch, _DTYPES, _INTS, _FLOATS
+    import torch
+    _torch = torch
+    _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    _INTS, _FLOATS = (torch.int32, torch.uint32), (torch.float32,)
 
 
 def _dtype(t, name):
-    global _DTYPES
-    if _DTYPES is None:
-        import torch
-        _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    if _torch is None:
+        _load_torch()
     code = _DTYPES.get(t.dtype)
     if code is None:
         raise ApoeError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
@@ -489,24 +495,28 @@ def _dtype(t, name):
 
 
 def _on_gpu(ctx, t, name):
-    if not (t.is_cuda and t.device.index == ctx.device):
+    if t.get_device() != ctx.device:
         raise ApoeError(f"{name} must be on GPU {ctx.device}, the context's")
 
 
 def _matrix(ctx, t, name, shape=None, dtype=None):
     """Checks a matrix whose rows are contiguous; returns its row stride."""
-    _on_gpu(ctx, t, name)
-    if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise ApoeError(f"{name} must be a matrix{'' if shape is None else f' of shape {tuple(shape)}'}, not {tuple(t.shape)}")
-    if dtype is not None and t.dtype != dtype:
+    have = t.shape
+    if t.get_device() != ctx.device:
+        raise ApoeError(f"{name} must be on GPU {ctx.device}, the context's")
+    if len(have) != 2 or (shape is not None and have != shape):
+        raise ApoeError(f"{name} must be a matrix{'' if shape is None else f' of shape {tuple(shape)}'}, not {tuple(have)}")
+    if dtype is not None and t.dtype is not dtype:
         raise ApoeError(f"{name} must be {dtype}, not {t.dtype}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    n, d = have
+    row, col = t.stride()
+    if col != 1 and d > 1:
         raise ApoeError(f"the rows of {name} must be contiguous")
-    if t.shape[0] <= 1:
-        return t.shape[1]
-    if t.stride(0) < t.shape[1]:
+    if n <= 1:
+        return d
+    if row < d:
         raise ApoeError(f"the rows of {name} overlap")
-    return t.stride(0)
+    return row
 
 
 def _vector(ctx, t, name, n, dtypes):
@@ -516,21 +526,18 @@ def _vector(ctx, t, name, n, dtypes):
     return t.data_ptr()
 
 
-class _in_order:
-    """The context's stream waits for torch's current stream, and that for the context's afterwards (nothing where they are one)."""
-
-    def __init__(self, ctx):
-        import torch
-        self.theirs = torch.cuda.current_stream(ctx.device)
-        self.ours = None if self.theirs.cuda_stream == ctx.stream else ctx.torch_stream()
-
-    def __enter__(self):
-        if self.ours is not None:
-            self.ours.wait_stream(self.theirs)
-
-    def __exit__(self, *failure):
-        if self.ours is not None:
-            self.theirs.wait_stream(self.ours)
+def _call(ctx, function, args):
+    """Calls `function`; the context's stream waits for torch's current stream, and that for the context's afterwards (nothing where
+    they are one)."""
+    theirs = _torch.cuda.current_stream(ctx.device)
+    if theirs.cuda_stream == ctx.stream:
+        _check(function(ctx.h, C.byref(args)))
+        return
+    ours = ctx.torch_stream()
+    ours.wait_stream(theirs)
+    status = function(ctx.h, C.byref(args))
+    theirs.wait_stream(ours)
+    _check(status)
 
 
 def softmax_loss(ctx, queries, rows, t_off, t_idx, t_val=None, scale=1.0, weight=None, live=None, grad_queries=False, grad_rows=False):
@@ -538,7 +545,6 @@ def softmax_loss(ctx, queries, rows, t_off, t_idx, t_val=None, scale=1.0, weight
     gradients of sum(weight * loss). t_off, t_idx, t_val: CSR of each query's relevant rows and their weights (equal shares
     without); live: int32 bit mask of the rows that take part; scale: of the inner products. grad_queries, grad_rows: True, or a
     matrix to write to. Returns dict(loss [m], lse [m]) and the gradients asked for; the logits are never held."""
-    import torch
     a = SoftmaxLossArgs()
     a.dtype = _dtype(queries, "queries")
     a.q_stride = _matrix(ctx, queries, "queries")
@@ -551,58 +557,56 @@ def softmax_loss(ctx, queries, rows, t_off, t_idx, t_val=None, scale=1.0, weight
         if grad_rows is not False and grad_rows is not None:
             raise ApoeError("the rows of a corpus stay as they are: no grad_rows")
     else:
-        a.rows_stride = _matrix(ctx, rows, "rows", (rows.shape[0], d), queries.dtype)
+        a.rows_stride = _matrix(ctx, rows, "rows", (len(rows), d), queries.dtype)
         a.n_rows, a.rows = rows.shape[0], rows.data_ptr()
         if rows.shape[0] == 0:
             raise ApoeError("rows is empty")
-    ints, floats = (torch.int32, torch.uint32), (torch.float32,)
-    a.t_off = _vector(ctx, t_off, "t_off", m + 1, ints)
-    a.t_idx = _vector(ctx, t_idx, "t_idx", None, ints)
+    a.t_off = _vector(ctx, t_off, "t_off", m + 1, _INTS)
+    a.t_idx = _vector(ctx, t_idx, "t_idx", None, _INTS)
     if t_idx.numel() == 0:  # no target at all: no entry is read, but the pointer has to be one
         a.t_idx = a.t_off
     if t_val is not None:
-        a.t_val = _vector(ctx, t_val, "t_val", t_idx.shape[0], floats) if t_idx.numel() else None
+        a.t_val = _vector(ctx, t_val, "t_val", t_idx.shape[0], _FLOATS) if t_idx.numel() else None
     if live is not None:
-        a.live = _vector(ctx, live, "live", (a.n_rows + 31) // 32, ints)
+        a.live = _vector(ctx, live, "live", (a.n_rows + 31) // 32, _INTS)
     if weight is not None:
-        a.weight = _vector(ctx, weight, "weight", m, floats)
+        a.weight = _vector(ctx, weight, "weight", m, _FLOATS)
     a.scale = scale
     a.q = queries.data_ptr()
-    both = torch.empty((2, m), dtype=torch.float32, device=queries.device)
+    both = _torch.empty((2, m), dtype=_torch.float32, device=queries.device)
     out = dict(loss=both[0], lse=both[1])
     a.loss = both.data_ptr()
     a.lse = a.loss + 4 * m if m else a.loss
     if grad_queries is not False and grad_queries is not None:
-        g = torch.empty((m, d), dtype=queries.dtype, device=queries.device) if grad_queries is True else grad_queries
+        g = _torch.empty((m, d), dtype=queries.dtype, device=queries.device) if grad_queries is True else grad_queries
         a.grad_q_stride = _matrix(ctx, g, "grad_queries", (m, d), queries.dtype)
         out["grad_queries"], a.grad_q = g, g.data_ptr()
     if grad_rows is not False and grad_rows is not None:
-        g = torch.empty((rows.shape[0], d), dtype=rows.dtype, device=rows.device) if grad_rows is True else grad_rows
+        g = _torch.empty((rows.shape[0], d), dtype=rows.dtype, device=rows.device) if grad_rows is True else grad_rows
         a.grad_rows_stride = _matrix(ctx, g, "grad_rows", rows.shape, rows.dtype)
         out["grad_rows"], a.grad_rows = g, g.data_ptr()
     if m == 0:  # nothing to compute but a gradient of zeros
         if "grad_rows" in out:
             out["grad_rows"].zero_()
         return out
-    with _in_order(ctx):
-        _check(lib().apoe_softmax_loss(ctx.h, C.byref(a)))
+    _call(ctx, lib().apoe_softmax_loss, a)
     return out
 
 
 def orthogonalize(ctx, x, out=None, steps=5, coefs=COEFS, alpha=1.0, beta=0.0, products=None):
     """out = alpha NS(x) + beta out for a matrix or a batch of matrices: the Newton-Schulz steps that bring x's singular values to
     about one. products: "f16" (on an fp32 iterate: 1e-4 to 6e-4 of the result) or "f32"; by default "f16" where out is bfloat16."""
-    import torch
     if x.dim() not in (2, 3):
         raise ApoeError(f"x must be a matrix or a batch of matrices, not {tuple(x.shape)}")
+    in_dtype = _dtype(x, "x")
     if out is None:
         if beta != 0.0:
             raise ApoeError("beta without out")
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if out.shape != x.shape:
         raise ApoeError(f"out must be of shape {tuple(x.shape)}, not {tuple(out.shape)}")
     a = OrthogonalizeArgs()
-    a.in_dtype, a.out_dtype = _dtype(x, "x"), _dtype(out, "out")
+    a.in_dtype, a.out_dtype = in_dtype, _dtype(out, "out")
     if products is None:
         products = "f16" if a.out_dtype == 2 else "f32"
     if products not in ("f16", "f32"):
@@ -618,13 +622,11 @@ def orthogonalize(ctx, x, out=None, steps=5, coefs=COEFS, alpha=1.0, beta=0.0, p
     a.in_, a.out, a.steps = x.data_ptr(), out.data_ptr(), steps
     a.a, a.b, a.c = coefs
     a.alpha, a.beta = alpha, beta
-    with _in_order(ctx):
-        _check(lib().apoe_orthogonalize(ctx.h, C.byref(a)))
+    _call(ctx, lib().apoe_orthogonalize, a)
     return out
 
 
 def _residual_args(ctx, x, h, gate, scale, w_post, w_next, eps):
-    import torch
     a = GatedResidualArgs()
     a.dtype = _dtype(x, "x")
     a.x_stride = _matrix(ctx, x, "x")
@@ -641,30 +643,27 @@ def _residual_args(ctx, x, h, gate, scale, w_post, w_next, eps):
             a.gate_kind, a.gate_stride, a.gate = 1, _matrix(ctx, gate, "gate", (n, d), x.dtype), gate.data_ptr()
     for t, name in ((scale, "scale"), (w_post, "w_post"), (w_next, "w_next")):
         if t is not None:
-            setattr(a, name, _vector(ctx, t, name, d, (torch.float32,)))
+            setattr(a, name, _vector(ctx, t, name, d, _FLOATS))
     return a
 
 
 def gated_residual(ctx, x, h=None, gate=None, scale=None, w_post=None, w_next=None, eps=1e-6, want_u=True):
     """(y, u): y = x + scale * sigmoid(gate) * w_post * h / rms(h) and u = w_next * y / rms(y). gate: [n, d] or [d]; without h,
     y is x itself and u its norm."""
-    import torch
     a = _residual_args(ctx, x, h, gate, scale, w_post, w_next, eps)
-    y = x if h is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    u = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_u else None
+    y = x if h is None else _torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    u = _torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_u else None
     if x.numel() == 0:
         return y, u
     a.y = None if h is None else y.data_ptr()
     a.u = None if u is None else u.data_ptr()
-    with _in_order(ctx):
-        _check(lib().apoe_gated_residual(ctx.h, C.byref(a)))
+    _call(ctx, lib().apoe_gated_residual, a)
     return y, u
 
 
 def gated_residual_grad(ctx, x, h=None, gate=None, scale=None, w_post=None, w_next=None, eps=1e-6, grad_y=None, grad_u=None):
     """Gradients of gated_residual from those of y and u (either may be None): a dict of grad_x, and of grad_h, grad_gate,
     grad_scale, grad_w_post, grad_w_next for the inputs that are not None."""
-    import torch
     a = _residual_args(ctx, x, h, gate, scale, w_post, w_next, eps)
     n, d = x.shape
     if grad_y is None and grad_u is None:
@@ -673,20 +672,19 @@ def gated_residual_grad(ctx, x, h=None, gate=None, scale=None, w_post=None, w_ne
         if t is not None:
             setattr(a, name + "_stride", _matrix(ctx, t, name, (n, d), x.dtype))
             setattr(a, name, t.data_ptr())
-    out = dict(grad_x=torch.empty((n, d), dtype=x.dtype, device=x.device))
+    out = dict(grad_x=_torch.empty((n, d), dtype=x.dtype, device=x.device))
     if h is not None:
-        out["grad_h"] = torch.empty((n, d), dtype=x.dtype, device=x.device)
+        out["grad_h"] = _torch.empty((n, d), dtype=x.dtype, device=x.device)
     if gate is not None:
-        out["grad_gate"] = torch.empty(gate.shape, dtype=x.dtype, device=x.device)
+        out["grad_gate"] = _torch.empty(gate.shape, dtype=x.dtype, device=x.device)
     for t, name in ((scale, "grad_scale"), (w_post, "grad_w_post"), (w_next, "grad_w_next")):
         if t is not None:
-            out[name] = torch.empty(d, dtype=torch.float32, device=x.device)
+            out[name] = _torch.empty(d, dtype=_torch.float32, device=x.device)
     if x.numel() == 0:
         for v in out.values():
             v.zero_()
         return out
     for name, t in out.items():
         setattr(a, name, t.data_ptr())
-    with _in_order(ctx):
-        _check(lib().apoe_gated_residual_grad(ctx.h, C.byref(a)))
+    _call(ctx, lib().apoe_gated_residual_grad, a)
     return out

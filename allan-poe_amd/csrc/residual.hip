@@ -261,23 +261,31 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
     }
 }
 
-// Columns' sums over the workgroups, and from them the vectors' gradients: 64 columns x 4 a workgroup.
-template <typename T> __global__ __launch_bounds__(256) void residual_vectors(ResArgs a) {
-    __shared__ float q[4][64], r[4][64];
+// Columns' sums over the workgroups, and from them the vectors' gradients: 16 columns a workgroup, 64 threads each (512 rows of
+// partial sums are eight loads a thread; four threads a column took 42 us at 1024 columns, these 6).
+template <typename T> __global__ __launch_bounds__(1024) void residual_vectors(ResArgs a) {
+    __shared__ float q[64][17], r[64][17];
     const apoe_gated_residual_args& p = a.p;
-    const uint32_t c = threadIdx.x & 63, l = threadIdx.x >> 6, d = blockIdx.x * 64 + c;
+    const uint32_t c = threadIdx.x & 15, l = threadIdx.x >> 4, d = blockIdx.x * 16 + c;
     float Q = 0.f, R = 0.f;
     if (d < p.dim)
-        for (uint32_t b = l; b < a.blocks; b += 4) {
+#pragma unroll 4
+        for (uint32_t b = l; b < a.blocks; b += 64) {
             Q += a.part[(size_t)b * 2 * p.dim + d];
             R += a.part[((size_t)b * 2 + 1) * p.dim + d];
         }
     q[l][c] = Q;
     r[l][c] = R;
-    __syncthreads();
+    for (uint32_t n = 32; n; n >>= 1) {
+        __syncthreads();
+        if (l < n) {
+            q[l][c] += q[l + n][c];
+            r[l][c] += r[l + n][c];
+        }
+    }
     if (l || d >= p.dim) return;
-    Q = (q[0][c] + q[1][c]) + (q[2][c] + q[3][c]);
-    R = (r[0][c] + r[1][c]) + (r[2][c] + r[3][c]);
+    Q = q[0][c];
+    R = r[0][c];
     const float s = p.scale ? p.scale[d] : 1.f, w = p.w_post ? p.w_post[d] : 1.f;
     if (p.grad_scale) p.grad_scale[d] = Q * w;
     if (p.grad_w_post) p.grad_w_post[d] = Q * s;
@@ -304,7 +312,7 @@ template <typename T, int V> static int run_residual(apoe_ctx* ctx, const apoe_g
             a.part = (float*)ws;
         }
         residual_backward<T, V, G><<<a.blocks, THREADS, 0, s>>>(a);
-        if (vectors) residual_vectors<T><<<(p->dim + 63) / 64, 256, 0, s>>>(a);
+        if (vectors) residual_vectors<T><<<(p->dim + 15) / 16, 1024, 0, s>>>(a);
         return APOE_OK;
     };
     int st;
