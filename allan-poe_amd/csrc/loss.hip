@@ -812,9 +812,240 @@ template <typename T, bool GRAD, bool EXP> __global__ __launch_bounds__(256) voi
     }
 }
 
+// ---- few queries ----
+// Up to four queries of up to 1024 columns: every row is read once, by one wave, which keeps the queries, its running sums and the
+// rows on their way in registers (a tile of 32 queries would be mostly empty, and its rows would be read twice). A wave takes four
+// rows at a time and asks for the next four before it works on these; four inner products are summed over the lanes together.
+// Exponentials are relative to a whole exponent that moves only when a logit passes it by 2^60: sums in 32 bits bear that.
+constexpr int FEW_E = 16; // values of a row that a lane holds
+constexpr uint32_t FEW_MAX_DIM = 64 * FEW_E, FEW_BLOCKS = 512;
+template <typename T> constexpr uint32_t FEW_QUERIES = sizeof(T) == 2 ? 4 : 2; // what the registers hold beside the rows on their way
+
+template <typename T, int NQ, bool GRAD> __global__ __launch_bounds__(256, 2) void loss_few(LossArgs a) {
+    constexpr int V = 16 / (int)sizeof(T), C = FEW_E / V;
+    typedef T tv __attribute__((ext_vector_type(V)));
+    __shared__ float refs[NQ][4], sums[NQ][4];
+    __shared__ float part[GRAD ? 4 : 1][GRAD ? NQ * FEW_MAX_DIM : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t fours = (a.n + 3) / 4, step = gridDim.x * 4;
+    const float c = a.scale * LOG2E;
+    float q[NQ][FEW_E], acc[NQ][FEW_E] = {}, ref[NQ], sum[NQ] = {};
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        ref[n] = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            const uint32_t d = (k * 64 + lane) * V;
+            tv x = {};
+            if (n < (int)a.nq && d < a.dim) x = *reinterpret_cast<const tv*>((const char*)a.q + (uint64_t)n * a.q_pitch + d * sizeof(T));
+#pragma unroll
+            for (int v = 0; v < V; v++) q[n][k * V + v] = (float)x[v];
+        }
+    }
+    auto live_four = [&](uint32_t four) { return four < fours ? (live_word(a.live, four * 4 & ~31u, a.n) >> (four * 4 & 31)) & 15u : 0u; };
+    auto load = [&](tv (&x)[4][C], uint32_t four, uint32_t on) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int k = 0; k < C; k++) {
+                const uint32_t d = (k * 64 + lane) * V;
+                x[r][k] = tv{};
+                if (((on >> r) & 1) && d < a.dim) x[r][k] = *reinterpret_cast<const tv*>((const char*)a.rows + (uint64_t)(four * 4 + r) * a.r_pitch + d * sizeof(T));
+            }
+    };
+    uint32_t four = blockIdx.x * 4 + wave, on = live_four(four);
+    tv next[4][C];
+    load(next, four, on);
+    while (four < fours) {
+        tv raw[4][C];
+        const uint32_t now = on;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int k = 0; k < C; k++) raw[r][k] = next[r][k];
+        four += step;
+        on = live_four(four);
+        load(next, four, on);
+        if (!now) continue;
+        float x[4][FEW_E];
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int k = 0; k < C; k++)
+#pragma unroll
+                for (int v = 0; v < V; v++) x[r][k * V + v] = (float)raw[r][k][v];
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            float z[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                z[r] = 0.f;
+#pragma unroll
+                for (int e = 0; e < FEW_E; e++) z[r] = __builtin_fmaf(q[n][e], x[r][e], z[r]);
+            }
+            // four sums over 64 lanes in seven exchanges: each halves what a lane carries, or the lanes that differ
+            const bool hi = lane & 32, mid = lane & 16;
+            float u = (hi ? z[1] : z[0]) + __shfl_xor(hi ? z[0] : z[1], 32);
+            float w = (hi ? z[3] : z[2]) + __shfl_xor(hi ? z[2] : z[3], 32);
+            u = (mid ? w : u) + __shfl_xor(mid ? u : w, 16);
+#pragma unroll
+            for (int d = 8; d; d >>= 1) u += __shfl_xor(u, d);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                if (!((now >> r) & 1)) continue;
+                const float y = c * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(u), (r & 1) * 32 + (r >> 1) * 16));
+                if (y > ref[n] + 60.f) {
+                    const float to = ceilf(y), f = __builtin_amdgcn_exp2f(ref[n] - to);
+                    ref[n] = to;
+                    sum[n] *= f;
+                    if constexpr (GRAD) {
+#pragma unroll
+                        for (int e = 0; e < FEW_E; e++) acc[n][e] *= f;
+                    }
+                }
+                const float p = y == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(y - ref[n]);
+                sum[n] += p;
+                if constexpr (GRAD) {
+#pragma unroll
+                    for (int e = 0; e < FEW_E; e++) acc[n][e] = __builtin_fmaf(p, x[r][e], acc[n][e]);
+                }
+            }
+        }
+    }
+    // the four waves joined
+    if (lane == 0)
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            refs[n][wave] = ref[n];
+            sums[n][wave] = sum[n];
+        }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NQ; n++) {
+        const float top = fmaxf(fmaxf(refs[n][0], refs[n][1]), fmaxf(refs[n][2], refs[n][3]));
+        if (threadIdx.x == 0) {
+            float t = 0.f, r = -INFINITY;
+            for (int k = 0; k < 4; k++) join_sums(r, t, refs[n][k], sums[n][k]);
+            const size_t at = (size_t)blockIdx.x * a.qp + n;
+            a.chunk_ref[at] = r;
+            a.chunk_sum[at] = t;
+            if constexpr (GRAD) a.part_ref[0][at] = top;
+        }
+        if constexpr (GRAD) {
+            const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ref[n] - top); // without live rows: zeros (or NaN)
+#pragma unroll
+            for (int k = 0; k < C; k++)
+#pragma unroll
+                for (int v = 0; v < V; v++) part[wave][n * FEW_MAX_DIM + (k * 64 + lane) * V + v] = acc[n][k * V + v] * f;
+        }
+    }
+    if constexpr (GRAD) {
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NQ; n++)
+            for (uint32_t d = threadIdx.x; d < a.dim; d += 256) {
+                const uint32_t at = n * FEW_MAX_DIM + d;
+                a.part[((size_t)blockIdx.x * a.qp + n) * a.dim + d] = (part[0][at] + part[1][at]) + (part[2][at] + part[3][at]);
+            }
+    }
+}
+
+// One workgroup a query, a thread a column.
+template <typename T, bool GRAD> __global__ __launch_bounds__(1024) void loss_few_finish(LossArgs a) {
+    __shared__ float lse_of, buf[16], scale_of[FEW_BLOCKS];
+    __shared__ f32x4 quarter[GRAD ? 4 : 1][GRAD ? 256 : 1];
+    const uint32_t qi = blockIdx.x, tid = threadIdx.x;
+    if (tid < 64) {
+        const float l = join_chunks(a, qi, tid);
+        if (tid == 0) lse_of = l;
+    }
+    auto all_sum = [&](float v) {
+#pragma unroll
+        for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+        __syncthreads();
+        if ((tid & 63) == 0) buf[tid >> 6] = v;
+        __syncthreads();
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; k++) s += buf[k];
+        return s;
+    };
+    const uint32_t e0 = a.t_off ? a.t_off[qi] : 0, e1 = a.t_off ? a.t_off[qi + 1] : 0;
+    float W = 0.f;
+    bool any = false;
+    for (uint32_t e = e0 + tid; e < e1; e += 1024) {
+        const float w = is_live(a, a.t_idx[e]) ? target_weight(a, e, e0, e1) : 0.f;
+        W += w;
+        any |= w != 0.f;
+    }
+    W = all_sum(W);
+    const bool on = __syncthreads_or(any);
+    const float lse = lse_of, cw = a.weight ? a.weight[qi] : 1.f;
+    const bool counts = on && cw != 0.f;
+    float g = 0.f;
+    if constexpr (GRAD) {
+        for (uint32_t s = tid; s < a.splits; s += 1024) {
+            const float r = a.part_ref[0][(size_t)s * a.qp + qi];
+            scale_of[s] = r == -INFINITY ? 0.f : W * __builtin_amdgcn_exp2f(r - lse);
+        }
+        __syncthreads();
+        const uint32_t d4 = (tid & 255) * 4;
+        f32x4 v = {};
+        if (counts && d4 < a.dim)
+#pragma unroll 8
+            for (uint32_t s = tid >> 8; s < a.splits; s += 4) v += scale_of[s] * *reinterpret_cast<const f32x4*>(a.part + ((size_t)s * a.qp + qi) * a.dim + d4);
+        quarter[tid >> 8][tid & 255] = v;
+        __syncthreads();
+        const float* p = reinterpret_cast<const float*>(quarter);
+        g = (p[tid] + p[1024 + tid]) + (p[2048 + tid] + p[3072 + tid]);
+    }
+    const float qd = tid < a.dim ? (float)reinterpret_cast<const T*>((const char*)a.q + (uint64_t)qi * a.q_pitch)[tid] : 0.f;
+    float at = 0.f;
+    for (uint32_t e = e0; e < e1; e++) {
+        const uint32_t t = a.t_idx[e];
+        const float w = is_live(a, t) ? target_weight(a, e, e0, e1) : 0.f;
+        if (w == 0.f) continue;
+        const float xd = tid < a.dim ? (float)reinterpret_cast<const T*>((const char*)a.rows + (uint64_t)t * a.r_pitch)[tid] : 0.f;
+        at = __builtin_fmaf(w, all_sum(qd * xd) * a.scale, at);
+        if (GRAD && counts) g = __builtin_fmaf(-w, xd, g);
+    }
+    if (tid == 0) {
+        if (a.lse) a.lse[qi] = lse * LN2;
+        if (a.loss) a.loss[qi] = W == 0.f ? (on ? -at : 0.f) : __builtin_fmaf(W, lse * LN2, -at);
+    }
+    if (GRAD && tid < a.dim) reinterpret_cast<T*>((char*)a.grad_q + (uint64_t)qi * a.gq_pitch)[tid] = (T)(counts ? cw * a.scale * g : 0.f);
+}
+
 // ---- launches ----
 
 static uint32_t up(uint64_t v, uint64_t to) { return (uint32_t)((v + to - 1) / to * to); }
+
+template <typename T> static int run_few(apoe_ctx* ctx, LossArgs& a, bool grad) {
+    // a wave has two turns of four rows at least, a CU two workgroups at most
+    const uint32_t blocks = std::max(1u, std::min((a.n + 31) / 32, std::min(FEW_BLOCKS, 2 * (uint32_t)ctx->num_cus)));
+    a.qp = next_pow2(a.nq); // as many as the kernel carries
+    a.chunks = a.splits = blocks;
+    const size_t sums = (size_t)blocks * a.qp * 4, up16 = (sums + 15) / 16 * 16;
+    char* ws = nullptr;
+    APOE_TRY(ctx->adapt_workspace(3 * up16 + (grad ? (size_t)blocks * a.qp * a.dim * 4 : 0), &ws));
+    a.chunk_ref = (float*)ws;
+    a.chunk_sum = (float*)(ws + up16);
+    a.part_ref[0] = (float*)(ws + 2 * up16);
+    a.part = (float*)(ws + 3 * up16);
+    hipStream_t s = ctx->stream;
+    auto go = [&](auto n) {
+        constexpr int NQ = decltype(n)::value;
+        if (grad) loss_few<T, NQ, true><<<blocks, 256, 0, s>>>(a);
+        else loss_few<T, NQ, false><<<blocks, 256, 0, s>>>(a);
+    };
+    if (a.nq == 1) go(std::integral_constant<int, 1>{});
+    else if (a.nq == 2) go(std::integral_constant<int, 2>{});
+    else if constexpr (FEW_QUERIES<T> == 4) go(std::integral_constant<int, 4>{});
+    if (grad) loss_few_finish<T, true><<<a.nq, 1024, 0, s>>>(a);
+    else loss_few_finish<T, false><<<a.nq, 1024, 0, s>>>(a);
+    APOE_HIP(hipGetLastError());
+    return APOE_OK;
+}
 
 template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss_args* p) {
     LossArgs a{};
@@ -838,6 +1069,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.lse = p->lse;
     a.grad_q = p->grad_q;
     a.grad_x = p->grad_rows;
+    if (a.nq <= FEW_QUERIES<T> && a.dim <= FEW_MAX_DIM && !gx) return run_few<T>(ctx, a, gq);
     // Tiles: 256 rows x 256 queries where that pads no more queries than 128 would (or few) and fills the GPU, 16-bit types
     // (1024 x 65 536 of 1024 columns: 1040 TFLOP/s, which is what the library's product of these shapes reaches; 256 x 128: 900), else 256 x 128, or 512 x 64 or 32 for few queries.
     const uint32_t wide_tiles = (a.n + 255) / 256 * ((a.nq + 255) / 256);

@@ -128,6 +128,28 @@ def test_sizes_and_types(gpu_ctx, m, n, d, dtype):
     check(gpu_ctx, a, False, False)
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5])
+def test_few_queries(gpu_ctx, m, dtype):
+    """Queries that are carried in registers (up to four of 16 bits, two of float32, rows of up to 1024 columns), and the sizes around."""
+    for n, d, live in ((1, 8, None), (3, 1024, None), (4, 520, None), (5, 1000, 0.5), (33, 16, 0.0), (130, 1032, 0.8), (2500, 1024, 0.3), (70_001, 24, 0.9)):
+        a = make(m, n, d, dtype, seed=m + n, live=live, targets=3, scale=12.0, pad=8 if d < 1000 else 0)
+        check(gpu_ctx, a, True, False)
+        check(gpu_ctx, a, False, False)
+
+
+def test_few_queries_whose_logits_climb(gpu_ctx):
+    """Each row above the last by more than the running exponent bears, in both orders, and below it by hundreds."""
+    import torch
+    for order in (1, -1):
+        a = make(2, 40, 32, "bfloat16", seed=3, scale=100.0)
+        x = torch.zeros(40, 32)
+        x[:, 0] = torch.arange(40.0) / 8 - 2
+        a["rows"] = (x if order == 1 else x.flip(0)).to(torch.bfloat16).contiguous().cuda()
+        a["queries"] = torch.eye(2, 32).to(torch.bfloat16).cuda()
+        check(gpu_ctx, a, True, False)
+
+
 @pytest.mark.parametrize("dtype,d", [("float16", 4096), ("bfloat16", 2056), ("float32", 4092), ("float32", 4)])
 def test_long_and_short_rows(gpu_ctx, dtype, d):
     check(gpu_ctx, make(70, 300, d, dtype, seed=d), True, True)
