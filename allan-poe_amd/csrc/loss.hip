@@ -446,7 +446,8 @@ template <typename T> __device__ inline i32x4 scale_down(i32x4 v, float less) {
 
 // grad q: a split's rows x its queries' blocks. M side: queries (blocks), N side: columns of the rows. EXP: fragments are brought
 // to the largest reference of the split, and a split's sum to the largest so far.
-template <typename T, int MT, int NT, int WM, int WN, int ST, bool EXP>
+// DIRECT: the only split of the only piece, whose sum is the gradient.
+template <typename T, int MT, int NT, int WM, int WN, int ST, bool EXP, bool DIRECT = false>
 __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint32_t n_tiles, uint32_t groups_per_split, uint32_t piece_groups, int turn, int first) {
     constexpr int NW = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, SF = sizeof(T) == 4 ? 4 : 2;
     using BTile = ColTile<T, BN, SF, NW, ORDER_BLOCKS>;
@@ -573,12 +574,23 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
         __syncthreads();
     }
     const int h = lane >> 5;
+    const float back = DIRECT ? a.scale / grad_scale_of(a.top_coef) : 1.f;
 #pragma unroll
     for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const int r = (wm * MT + m) * 32 + result_row(i, h);
             if (query + r >= a.nq) continue;
+            if constexpr (DIRECT) {
+                const bool on = (a.q_on[(query + r) >> 5] >> (r & 31)) & 1;
+                T* to = reinterpret_cast<T*>((char*)a.grad_q + (uint64_t)(query + r) * a.gq_pitch);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const uint32_t d = col + (wn * NT + t) * 32 + (lane & 31);
+                    if (d < a.dim) to[d] = (T)(on ? acc[m][t][i] * back : 0.f);
+                }
+                continue;
+            }
             float* out = a.part + ((size_t)split * a.qp + query + r) * a.dim;
 #pragma unroll
             for (int t = 0; t < NT; t++) {
@@ -701,21 +713,47 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint3
     }
 }
 
-__device__ inline float block_sum(float v, float* buf) { // of 256 threads, the same for all
+template <int THREADS> __device__ inline float block_sum(float v, float* buf) { // the same for all threads
 #pragma unroll
     for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (buf[0] + buf[1]) + (buf[2] + buf[3]);
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < THREADS / 64; k++) s += buf[k];
+    return s;
 }
 
+constexpr uint32_t LOSS_SPLITS = 512; // of the rows under one partial sum of grad q, at most
+
 // One workgroup a query: lse, loss, and the query's gradient from its splits. EXP: the splits are sums of exponentials relative
-// to their references without the targets, whose terms are added here; otherwise they are sums of scaled G.
-template <typename T, bool GRAD, bool EXP> __global__ __launch_bounds__(256) void loss_finish(LossArgs a, int turn) {
-    constexpr int V = 16 / (int)sizeof(T), C = APOE_LOSS_MAX_DIM / (256 * V);
-    __shared__ float buf[4], lse_of;
+// to their references without the targets, whose terms are added here; otherwise they are sums of scaled G. A thread holds four
+// columns (and their next 4 THREADS); where a row has fewer than 4 THREADS columns the threads share the splits.
+template <typename T, bool GRAD, bool EXP, int THREADS> __global__ __launch_bounds__(THREADS) void loss_finish(LossArgs a, int turn) {
+    constexpr int C = APOE_LOSS_MAX_DIM / (THREADS * 4);
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    __shared__ float buf[THREADS / 64], lse_of, factor[GRAD ? LOSS_SPLITS : 1];
+    __shared__ f32x4 share[GRAD ? THREADS : 1];
     const uint32_t qi = blockIdx.x, tid = threadIdx.x;
+    f32x4 acc[C] = {};
+    uint32_t lanes = THREADS;
+    while (lanes * 2 >= a.dim && lanes > 64) lanes /= 2; // threads along a row
+    const uint32_t groups = THREADS / lanes, g = tid / lanes, d0 = tid % lanes * 4;
+    auto add_splits = [&]() {
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            const uint32_t d = d0 + k * THREADS * 4;
+            if (d >= a.dim || (k && groups > 1)) continue;
+            const float* p = a.part + (size_t)qi * a.dim + d;
+#pragma unroll 4
+            for (uint32_t s = g; s < a.splits; s += groups) {
+                const f32x4 x = *reinterpret_cast<const f32x4*>(p + (size_t)s * a.qp * a.dim);
+                acc[k] += EXP ? factor[s] * x : x;
+            }
+        }
+    };
+    if constexpr (GRAD && !EXP) add_splits(); // on their way while the sums are joined
     if (tid < 64) {
         const float l = join_chunks(a, qi, tid);
         if (tid == 0) lse_of = l;
@@ -723,72 +761,70 @@ template <typename T, bool GRAD, bool EXP> __global__ __launch_bounds__(256) voi
     const uint32_t e0 = a.t_off ? a.t_off[qi] : 0, e1 = a.t_off ? a.t_off[qi + 1] : 0;
     float W = 0.f;
     bool any = false;
-    for (uint32_t e = e0 + tid; e < e1; e += 256) {
+    for (uint32_t e = e0 + tid; e < e1; e += THREADS) {
         const float w = is_live(a, a.t_idx[e]) ? target_weight(a, e, e0, e1) : 0.f;
         W += w;
         any |= w != 0.f;
     }
-    W = block_sum(W, buf);
+    W = block_sum<THREADS>(W, buf);
     const bool on = __syncthreads_or(any);
     const float lse = lse_of, cw = a.weight ? a.weight[qi] : 1.f;
-    float acc[C][V] = {};
+    const bool counts = on && cw != 0.f;
     if constexpr (GRAD) {
-        const float gs = EXP ? 1.f : 1.f / grad_scale_of(a.top_coef);
-        if (on && cw != 0.f)
-            for (uint32_t s = 0; s < a.splits; s++) {
-                const float r = EXP ? a.part_ref[turn][(size_t)s * a.qp + qi] : 0.f;
-                if (EXP && r == -INFINITY) continue;
-                const float f = EXP ? W * __builtin_amdgcn_exp2f(r - lse) : gs;
-                const float* p = a.part + ((size_t)s * a.qp + qi) * a.dim;
-#pragma unroll
-                for (int k = 0; k < C; k++) {
-                    const uint32_t d = (k * 256 + tid) * V;
-                    if (d >= a.dim) continue;
-#pragma unroll
-                    for (int v = 0; v < V; v += 4) {
-                        const float4 x = *reinterpret_cast<const float4*>(p + d + v);
-                        acc[k][v] = __builtin_fmaf(f, x.x, acc[k][v]);
-                        acc[k][v + 1] = __builtin_fmaf(f, x.y, acc[k][v + 1]);
-                        acc[k][v + 2] = __builtin_fmaf(f, x.z, acc[k][v + 2]);
-                        acc[k][v + 3] = __builtin_fmaf(f, x.w, acc[k][v + 3]);
-                    }
-                }
+        if constexpr (EXP) {
+            for (uint32_t s = tid; s < a.splits; s += THREADS) {
+                const float r = a.part_ref[turn][(size_t)s * a.qp + qi];
+                factor[s] = r == -INFINITY ? 0.f : W * __builtin_amdgcn_exp2f(r - lse);
             }
+            __syncthreads();
+            if (counts) add_splits();
+        }
+        if (groups > 1) {
+            share[tid] = acc[0];
+            __syncthreads();
+            if (g == 0)
+                for (uint32_t k = 1; k < groups; k++) acc[0] += share[k * lanes + tid];
+            if (g) acc[0] = f32x4{};
+        }
+        if constexpr (!EXP) {
+            const float gs = 1.f / grad_scale_of(a.top_coef);
+#pragma unroll
+            for (int k = 0; k < C; k++) acc[k] *= gs;
+        }
     }
     // targets: s_t in 32 bits, in the order of the list
-    typedef T tv __attribute__((ext_vector_type(V)));
     const char* q = (const char*)a.q + (uint64_t)qi * a.q_pitch;
     float at = 0.f;
     for (uint32_t e = e0; e < e1; e++) {
         const uint32_t t = a.t_idx[e];
-        const float w = is_live(a, t) ? target_weight(a, e, e0, e1) : 0.f;
-        if (w == 0.f && !(GRAD && EXP)) continue;
         if (!is_live(a, t)) continue;
+        const float w = target_weight(a, e, e0, e1);
+        if (w == 0.f && !(GRAD && EXP)) continue;
         const char* x = (const char*)a.rows + (uint64_t)t * a.r_pitch;
         float dot = 0.f;
-        tv xs[C];
+        t4 xs[C];
 #pragma unroll
         for (int k = 0; k < C; k++) {
-            const uint32_t d = (k * 256 + tid) * V;
+            const uint32_t d = (k * THREADS + tid) * 4;
             if (d >= a.dim) continue;
-            xs[k] = *reinterpret_cast<const tv*>(x + d * sizeof(T));
-            const tv u = *reinterpret_cast<const tv*>(q + d * sizeof(T));
+            xs[k] = *reinterpret_cast<const t4*>(x + d * sizeof(T));
+            const t4 u = *reinterpret_cast<const t4*>(q + d * sizeof(T));
 #pragma unroll
-            for (int v = 0; v < V; v++) dot = __builtin_fmaf((float)u[v], (float)xs[k][v], dot);
+            for (int v = 0; v < 4; v++) dot = __builtin_fmaf((float)u[v], (float)xs[k][v], dot);
         }
-        dot = block_sum(dot, buf);
+        dot = block_sum<THREADS>(dot, buf);
         if (w != 0.f) at = __builtin_fmaf(w, dot * a.scale, at);
         if constexpr (GRAD && EXP) {
             bool again = false; // its exponential was taken out once
-            for (uint32_t k = e0 + tid; k < e; k += 256) again |= a.t_idx[k] == t;
+            for (uint32_t k = e0 + tid; k < e; k += THREADS) again |= a.t_idx[k] == t;
             again = __syncthreads_or(again);
             const float f = (again ? 0.f : W * exp2f(__builtin_fmaf(dot, a.scale * LOG2E, -lse))) - w;
-            if (on && cw != 0.f) {
+            if (counts) {
 #pragma unroll
                 for (int k = 0; k < C; k++)
-                    if ((k * 256 + tid) * V < a.dim) {
+                    if ((k * THREADS + tid) * 4 < a.dim) {
 #pragma unroll
-                        for (int v = 0; v < V; v++) acc[k][v] = __builtin_fmaf(f, (float)xs[k][v], acc[k][v]);
+                        for (int v = 0; v < 4; v++) acc[k][v] = __builtin_fmaf(f, (float)xs[k][v], acc[k][v]);
                     }
             }
         }
@@ -802,12 +838,12 @@ template <typename T, bool GRAD, bool EXP> __global__ __launch_bounds__(256) voi
         char* out = (char*)a.grad_q + (uint64_t)qi * a.gq_pitch;
 #pragma unroll
         for (int k = 0; k < C; k++) {
-            const uint32_t d = (k * 256 + tid) * V;
+            const uint32_t d = (k * THREADS + tid) * 4;
             if (d >= a.dim) continue;
-            tv o;
+            t4 o;
 #pragma unroll
-            for (int v = 0; v < V; v++) o[v] = (T)(on && cw != 0.f ? f * acc[k][v] : 0.f);
-            *reinterpret_cast<tv*>(out + d * sizeof(T)) = o;
+            for (int v = 0; v < 4; v++) o[v] = (T)(counts ? f * acc[k][v] : 0.f);
+            *reinterpret_cast<t4*>(out + d * sizeof(T)) = o;
         }
     }
 }
@@ -1070,12 +1106,23 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.grad_q = p->grad_q;
     a.grad_x = p->grad_rows;
     if (a.nq <= FEW_QUERIES<T> && a.dim <= FEW_MAX_DIM && !gx) return run_few<T>(ctx, a, gq);
-    // Tiles: 256 rows x 256 queries where that pads no more queries than 128 would (or few) and fills the GPU, 16-bit types
-    // (1024 x 65 536 of 1024 columns: 1040 TFLOP/s, which is what the library's product of these shapes reaches; 256 x 128: 900), else 256 x 128, or 512 x 64 or 32 for few queries.
-    const uint32_t wide_tiles = (a.n + 255) / 256 * ((a.nq + 255) / 256);
-    const bool wide = sizeof(T) == 2 && wide_tiles >= (uint32_t)ctx->num_cus && (up(a.nq, 256) == up(a.nq, 128) || a.nq > 1024);
-    const int form = a.nq <= 32 ? 2 : a.nq <= 64 ? 1 : wide ? 3 : 0;
-    const uint32_t bm = form == 1 || form == 2 ? 512 : 256, bn = form == 2 ? 32 : form == 1 ? 64 : form == 3 ? 256 : 128;
+    // Tiles of rows x queries (times at 1024 columns, fp16, with the exponentials written):
+    //   256 x 256  where they fill the GPU and pad no more queries than 128 would, or hardly (1024 x 65 536: 130 us, 256 x 128: 150)
+    //   256 x 128  where those fill it (128 x 131 072: 56 us; 128 x 128: 66)
+    //   128 x 128  for fewer rows (1024 x 4000: 16.5 us; 256 x 128: 20)
+    //   128 x 64   up to 64 queries (64 x 30 000: 15.5 us; 128 x 128: 17), 512 x 32 for up to 32 where those fill it (32 x 131 072: 44 us; 48)
+    // and for fp32, whose products are 16 times as long, 256 x 128 and 512 x 64 or 32.
+    enum { T256, T256_128, T128, T128_64, T512_32, F256_128, F512_64, F512_32 } form;
+    const uint32_t cus = (uint32_t)ctx->num_cus;
+    auto count = [&](uint32_t rows, uint32_t queries) { return (uint64_t)((a.n + rows - 1) / rows) * ((a.nq + queries - 1) / queries); };
+    if (sizeof(T) == 4) form = a.nq <= 32 ? F512_32 : a.nq <= 64 ? F512_64 : F256_128;
+    else if (a.nq <= 32 && count(512, 32) >= cus) form = T512_32;
+    else if (a.nq <= 64) form = T128_64;
+    else if (count(256, 256) >= cus && (up(a.nq, 256) == up(a.nq, 128) || a.nq > 1024)) form = T256;
+    else if (count(256, 128) >= cus) form = T256_128;
+    else form = T128;
+    const uint32_t bm = form == T512_32 || form == F512_32 || form == F512_64 ? 512 : form == T128 || form == T128_64 ? 128 : 256;
+    const uint32_t bn = form == T256 ? 256 : form == T128_64 || form == F512_64 ? 64 : form == T512_32 || form == F512_32 ? 32 : 128;
     a.qp = up(a.nq, bn);
     a.q_tiles = a.qp / bn;
     const uint32_t rows_up = up(a.n, bm);
@@ -1089,12 +1136,14 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.groups = rows_up / LOSS_GROUP;
     const uint32_t chunks_per_piece = std::min<uint32_t>(std::max<uint32_t>(1, LOSS_CHUNKS / pieces), (uint32_t)((piece / LOSS_GROUP + 31) / 32));
     a.chunks = chunks_per_piece * pieces;
-    // grad q: tiles of 256 x 256, of 128 x 256 (fp32: 128 x 128), or of 32 queries; enough splits of the rows to fill the GPU (twice over
-    // where a CU holds two workgroups)
-    const uint32_t qm = form == 2 ? 32 : form == 3 ? 256 : 128, qn = sizeof(T) == 4 ? 128 : 256;
+    // grad q: tiles of 256 x 256, of 128 or 64 x 256 (fp32: 128 or 32 x 128); enough splits of the rows to fill the GPU (twice
+    // over where a CU holds two workgroups)
+    const uint32_t qm = form == T256 ? 256 : a.nq > 64 ? 128 : sizeof(T) == 2 ? 64 : a.nq > 32 ? 128 : 32, qn = sizeof(T) == 4 ? 128 : 256;
     const uint32_t gq_q_tiles = (a.qp + qm - 1) / qm, gq_n_tiles = (a.dim + qn - 1) / qn;
     const uint32_t piece_groups = (uint32_t)(piece / LOSS_GROUP);
-    uint32_t splits = std::max<uint32_t>(1, (uint32_t)((form == 3 ? 1 : 2) * ctx->num_cus) / (gq_q_tiles * gq_n_tiles));
+    // With G whole in one piece, tiles of 128 x 128 that fill the GPU need no splits: 4096 x 4096 takes 15 us less.
+    const bool direct = sizeof(T) == 2 && gq && two_pass && pieces == 1 && (uint64_t)((a.qp + 127) / 128) * ((a.dim + 127) / 128) >= cus * 9 / 10;
+    uint32_t splits = std::min(LOSS_SPLITS, std::max<uint32_t>(1, (form == T256 ? 1 : 2) * cus / (gq_q_tiles * gq_n_tiles)));
     if (splits >= 8) splits = splits / 8 * 8;
     splits = std::min(splits, piece_groups);
     const uint32_t per_split = (piece_groups + splits - 1) / splits;
@@ -1112,7 +1161,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     const size_t o_cr = take((size_t)a.chunks * a.qp * 4), o_cs = take((size_t)a.chunks * a.qp * 4);
     const size_t o_lw = take((size_t)a.qp * 8), o_top = take(4), o_on = take(a.qp / 8), o_coef = take((size_t)a.qp * 4);
     const size_t o_blocks = take(gq || gx ? (size_t)a.qp * piece * sizeof(T) : 0);
-    const size_t o_part = take(gq ? (size_t)splits * a.qp * a.dim * 4 : 0);
+    const size_t o_part = take(gq && !direct ? (size_t)splits * a.qp * a.dim * 4 : 0);
     const size_t o_pr0 = take((size_t)splits * a.qp * 4), o_pr1 = take((size_t)splits * a.qp * 4);
     char* ws = nullptr;
     APOE_TRY(ctx->adapt_workspace(bytes, &ws));
@@ -1141,14 +1190,16 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         constexpr int M = decltype(mode)::value;
         const dim3 grid(a.row_tiles * a.q_tiles);
         if constexpr (sizeof(T) == 2) {
-            if (form == 3) {
-                loss_tile<T, 2, 2, 4, 4, 2, M><<<grid, 512, 0, s>>>(a);
-                return;
-            }
+            if (form == T256) loss_tile<T, 2, 2, 4, 4, 2, M><<<grid, 512, 0, s>>>(a);
+            else if (form == T256_128) loss_tile<T, 1, 2, 4, 4, 3, M><<<grid, 512, 0, s>>>(a);
+            else if (form == T128) loss_tile<T, 1, 1, 4, 4, 2, M><<<grid, 256, 0, s>>>(a);
+            else if (form == T128_64) loss_tile<T, 1, 1, 2, 4, 3, M><<<grid, 128, 0, s>>>(a);
+            else loss_tile<T, 1, 4, 1, 4, 2, M><<<grid, 256, 0, s>>>(a);
+        } else {
+            if (form == F256_128) loss_tile<T, 2, 2, 2, 2, 3, M><<<grid, 256, 0, s>>>(a);
+            else if (form == F512_64) loss_tile<T, 2, 4, 1, 2, 2, M><<<grid, 256, 0, s>>>(a);
+            else loss_tile<T, 1, 4, 1, 4, 2, M><<<grid, 256, 0, s>>>(a);
         }
-        if (form == 0) loss_tile<T, 2, 2, 2, 2, 3, M><<<grid, 256, 0, s>>>(a);
-        else if (form == 1) loss_tile<T, 2, 4, 1, 2, 2, M><<<grid, 256, 0, s>>>(a);
-        else loss_tile<T, 1, 4, 1, 4, 2, M><<<grid, 256, 0, s>>>(a);
     };
     auto grad_q = [&](auto exp, uint32_t groups, int turn, int first) {
         constexpr bool E = decltype(exp)::value;
@@ -1156,11 +1207,11 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         a.q_tiles = gq_q_tiles;
         const dim3 grid(gq_q_tiles * gq_n_tiles * splits);
         if constexpr (sizeof(T) == 4) {
-            if (form == 2) loss_grad_q<T, 1, 1, 1, 4, 2, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
+            if (qm == 32) loss_grad_q<T, 1, 1, 1, 4, 2, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
             else loss_grad_q<T, 2, 2, 2, 2, 2, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
         } else {
-            if (form == 2) loss_grad_q<T, 1, 2, 1, 4, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
-            else if (form == 3) loss_grad_q<T, 4, 2, 2, 4, 4, E><<<grid, 512, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
+            if (qm == 64) loss_grad_q<T, 2, 2, 1, 4, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
+            else if (qm == 256) loss_grad_q<T, 4, 2, 2, 4, 4, E><<<grid, 512, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
             else loss_grad_q<T, 2, 4, 2, 2, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
         }
         a.q_tiles = keep;
@@ -1169,6 +1220,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     using Exp = std::integral_constant<int, TILE_EXP>;
     using Grad = std::integral_constant<int, TILE_GRAD>;
     const uint32_t join_q = a.qp / 32;
+    const bool many = splits > 16; // of which one workgroup adds up a query's: with 16 waves
     if (!two_pass) {
         for (uint32_t i = 0; i < pieces; i++) {
             const uint32_t groups = set_piece(i);
@@ -1180,8 +1232,9 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
             if (gq) grad_q(std::true_type{}, groups, (int)(i & 1), i == 0);
         }
         const int turn = (int)((pieces - 1) & 1);
-        if (gq) loss_finish<T, true, true><<<a.nq, 256, 0, s>>>(a, turn);
-        else loss_finish<T, false, false><<<a.nq, 256, 0, s>>>(a, turn);
+        if (!gq) loss_finish<T, false, false, 256><<<a.nq, 256, 0, s>>>(a, turn);
+        else if (many) loss_finish<T, true, true, 1024><<<a.nq, 1024, 0, s>>>(a, turn);
+        else loss_finish<T, true, true, 256><<<a.nq, 256, 0, s>>>(a, turn);
         APOE_HIP(hipGetLastError());
         return APOE_OK;
     }
@@ -1201,14 +1254,24 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         if (pieces == 1) loss_normalise<T><<<(uint32_t)(((uint64_t)groups * (a.qp / 32) + 3) / 4), 256, 0, s>>>(a, groups);
         else tiles(Grad{});
         loss_targets<T><<<a.nq, 64, 0, s>>>(a);
-        if (gq) grad_q(std::false_type{}, groups, 0, i == 0);
+        if constexpr (sizeof(T) == 2) {
+            if (direct) {
+                LossArgs d = a;
+                d.q_tiles = (a.qp + 127) / 128;
+                d.splits = 1;
+                const uint32_t nt = (a.dim + 127) / 128;
+                loss_grad_q<T, 2, 2, 2, 2, 3, false, true><<<d.q_tiles * nt, 256, 0, s>>>(d, nt, groups, groups, 0, 1);
+            }
+        }
+        if (gq && !direct) grad_q(std::false_type{}, groups, 0, i == 0);
         const dim3 grid((a.row_blocks * 32 + xm - 1) / xm * x_tiles);
         if constexpr (sizeof(T) == 4) loss_grad_x<T, 4, 1, 2, 2, 2><<<grid, 256, 0, s>>>(a, x_tiles);
         else if (x_wide) loss_grad_x<T, 4, 2, 2, 4, 4><<<grid, 512, 0, s>>>(a, x_tiles);
         else loss_grad_x<T, 2, 2, 2, 2, 3><<<grid, 256, 0, s>>>(a, x_tiles);
     }
-    if (gq) loss_finish<T, true, false><<<a.nq, 256, 0, s>>>(a, 0);
-    else loss_finish<T, false, false><<<a.nq, 256, 0, s>>>(a, 0);
+    if (!gq || direct) loss_finish<T, false, false, 256><<<a.nq, 256, 0, s>>>(a, 0);
+    else if (many) loss_finish<T, true, false, 1024><<<a.nq, 1024, 0, s>>>(a, 0);
+    else loss_finish<T, true, false, 256><<<a.nq, 256, 0, s>>>(a, 0);
     APOE_HIP(hipGetLastError());
     return APOE_OK;
 }

@@ -257,6 +257,12 @@ def test_a_query_that_is_served_well_keeps_its_small_gradient(gpu_ctx):
             assert err < 2 * u + 4 * 23 * 2.0 ** -24 / 1.2e-4, err
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_a_batch_that_fills_the_gpu_without_splits(gpu_ctx, dtype):
+    """4003 queries against 70 rows of 1024 columns, both gradients: the queries' one is written by its product itself."""
+    check(gpu_ctx, make(4003, 70, 1024, dtype, seed=5, live=0.8), True, True)
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("grad_rows", [False, True])
 def test_more_than_one_piece(gpu_ctx, dtype, grad_rows):
