@@ -68,7 +68,7 @@ struct LossArgs {
     float *ref, *sum;           // [n / LOSS_GROUP][qp]
     float *chunk_ref, *chunk_sum; // [LOSS_CHUNKS][qp]
     float2* lse_w;              // [qp]: lse in base 2, weight W (to be multiplied with exp(s - lse))
-    float* coef;                // [qp]: |weight| (|W| + sum |w|)
+    float *coef, *total;        // [qp]: |weight| (|W| + sum |w|); W
     uint32_t *top_coef, *q_on;  // the largest of them, as bits; those that are not zero, as a bit mask
     char* blocks;
     float* part;                // [splits][qp][dim]
@@ -319,6 +319,7 @@ __global__ __launch_bounds__(64) void loss_coefs(LossArgs a) {
         const float c = a.weight ? a.weight[qi] : 1.f;
         a.lse_w[qi] = make_float2(lse, c * W);
         a.coef[qi] = fabsf(c) * (fabsf(W) + A);
+        a.total[qi] = W;
     }
 }
 
@@ -383,13 +384,15 @@ template <typename T> __device__ inline float dot16(const char* x, const char* y
     return s;
 }
 
-// Second pass: the targets' places in this piece's G, formed in 32 bits; one wave a query.
-template <typename T> __global__ __launch_bounds__(64) void loss_targets(LossArgs a) {
+// Second pass: the targets' places in this piece's G, formed in 32 bits; one wave a query. ALL: the piece holds all rows and no
+// kernel behind this one adds anything, so it writes the loss.
+template <typename T, bool ALL> __global__ __launch_bounds__(64) void loss_targets(LossArgs a) {
     const uint32_t qi = blockIdx.x, end = min(a.row0 + a.row_blocks * 32, a.n);
     const int lane = threadIdx.x;
     const uint32_t e0 = a.t_off[qi], e1 = a.t_off[qi + 1];
     const float2 lw = a.lse_w[qi];
     const float gs = grad_scale_of(a.top_coef), cw = a.weight ? a.weight[qi] : 1.f;
+    float at = 0.f;
     for (uint32_t e = e0; e < e1; e++) {
         const uint32_t t = a.t_idx[e];
         if (t < a.row0 || t >= end || !is_live(a, t)) continue;
@@ -411,12 +414,18 @@ template <typename T> __global__ __launch_bounds__(64) void loss_targets(LossArg
             dot += __shfl_xor(dot, d);
             w += __shfl_xor(w, d);
         }
+        if (w != 0.f) at = __builtin_fmaf(w, dot * a.scale, at);
         if (lane == 0) {
             const float p = exp2f(__builtin_fmaf(dot, a.scale * LOG2E, -lw.x));
             const float g = cw == 0.f ? 0.f : gs * (lw.y * p - cw * w);
             char* block = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((t - a.row0) >> 5)) * Block<T>::BYTES;
             *reinterpret_cast<T*>(block + Block<T>::place(qi & 31, (t - a.row0) & 31)) = (T)g;
         }
+    }
+    if (ALL && lane == 0) {
+        const float W = a.total[qi], lse = lw.x * LN2;
+        if (a.lse) a.lse[qi] = lse;
+        if (a.loss) a.loss[qi] = W == 0.f ? 0.f - at : __builtin_fmaf(W, lse, -at);
     }
 }
 
@@ -1159,7 +1168,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     };
     const size_t o_ref = take((size_t)a.groups * a.qp * 4), o_sum = take((size_t)a.groups * a.qp * 4);
     const size_t o_cr = take((size_t)a.chunks * a.qp * 4), o_cs = take((size_t)a.chunks * a.qp * 4);
-    const size_t o_lw = take((size_t)a.qp * 8), o_top = take(4), o_on = take(a.qp / 8), o_coef = take((size_t)a.qp * 4);
+    const size_t o_lw = take((size_t)a.qp * 8), o_top = take(4), o_on = take(a.qp / 8), o_coef = take((size_t)a.qp * 4), o_total = take((size_t)a.qp * 4);
     const size_t o_blocks = take(gq || gx ? (size_t)a.qp * piece * sizeof(T) : 0);
     const size_t o_part = take(gq && !direct ? (size_t)splits * a.qp * a.dim * 4 : 0);
     const size_t o_pr0 = take((size_t)splits * a.qp * 4), o_pr1 = take((size_t)splits * a.qp * 4);
@@ -1177,6 +1186,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.part_ref[1] = (float*)(ws + o_pr1);
     a.q_on = (uint32_t*)(ws + o_on);
     a.coef = (float*)(ws + o_coef);
+    a.total = (float*)(ws + o_total);
     hipStream_t s = ctx->stream;
 
     auto set_piece = [&](uint32_t i) {
@@ -1238,11 +1248,17 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         APOE_HIP(hipGetLastError());
         return APOE_OK;
     }
+    const bool whole = pieces == 1 && (!gq || direct); // nothing is left to a last kernel
     for (uint32_t i = 0; i < pieces; i++) {
         const uint32_t groups = set_piece(i);
         if (pieces == 1) tiles(Exp{});
         else tiles(Sums{});
-        loss_join<T, false><<<dim3(join_q, chunks_per_piece), 256, 0, s>>>(a, a.row0 / LOSS_GROUP, groups, i * chunks_per_piece);
+        if (a.groups > LOSS_CHUNKS) loss_join<T, false><<<dim3(join_q, chunks_per_piece), 256, 0, s>>>(a, a.row0 / LOSS_GROUP, groups, i * chunks_per_piece);
+    }
+    if (a.groups <= LOSS_CHUNKS) { // few enough for one wave as they are
+        a.chunk_ref = a.ref;
+        a.chunk_sum = a.sum;
+        a.chunks = a.groups;
     }
     loss_coefs<<<a.qp, 64, 0, s>>>(a);
     loss_queries<<<1, 1024, 0, s>>>(a);
@@ -1253,7 +1269,8 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         const uint32_t groups = set_piece(i);
         if (pieces == 1) loss_normalise<T><<<(uint32_t)(((uint64_t)groups * (a.qp / 32) + 3) / 4), 256, 0, s>>>(a, groups);
         else tiles(Grad{});
-        loss_targets<T><<<a.nq, 64, 0, s>>>(a);
+        if (whole) loss_targets<T, true><<<a.nq, 64, 0, s>>>(a);
+        else loss_targets<T, false><<<a.nq, 64, 0, s>>>(a);
         if constexpr (sizeof(T) == 2) {
             if (direct) {
                 LossArgs d = a;
@@ -1269,7 +1286,8 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         else if (x_wide) loss_grad_x<T, 4, 2, 2, 4, 4><<<grid, 512, 0, s>>>(a, x_tiles);
         else loss_grad_x<T, 2, 2, 2, 2, 3><<<grid, 256, 0, s>>>(a, x_tiles);
     }
-    if (!gq || direct) loss_finish<T, false, false, 256><<<a.nq, 256, 0, s>>>(a, 0);
+    if (whole) {
+    } else if (!gq) loss_finish<T, false, false, 256><<<a.nq, 256, 0, s>>>(a, 0);
     else if (many) loss_finish<T, true, false, 1024><<<a.nq, 1024, 0, s>>>(a, 0);
     else loss_finish<T, true, false, 256><<<a.nq, 256, 0, s>>>(a, 0);
     APOE_HIP(hipGetLastError());
