@@ -1,10 +1,10 @@
 // Tiles of a matrix product on the matrix cores, shared by the operators that fit a query adapter (loss.hip, ortho.hip).
 //
 // A workgroup of NW waves multiplies a tile of A (M side) with a tile of B (N side), both staged through LDS in steps of the
-// inner dimension. The unit of the inner dimension is a fragment: 16 bytes a lane, 32 bytes of a row, which is 16 values of
-// 16 bits (one 32x32x16 product) or 8 floats (four 32x32x2 products; fp32 stays fp32). What the two sides have to agree on is
-// which inner index a lane's j-th value holds, so a fragment may permute them; two orders occur:
-//   ROWS    lane half h holds 8 (fp32: 4) consecutive indices, half 0 first, as 16 bytes of a row come;
+// inner dimension. Values have 16 bits (float matrices come as two or three planes of such). The unit of the inner dimension is a
+// fragment: 16 bytes a lane, 16 values of a row, one 32x32x16 product. What the two sides have to agree on is which inner index
+// a lane's j-th value holds, so a fragment may permute them; two orders occur:
+//   ROWS    lane half h holds 8 consecutive indices, half 0 first, as 16 bytes of a row come;
 //   BLOCKS  value j of half h is index 8 (j / 4) + 4 h + j % 4: what a lane has of a 32x32 result, so a result turns into
 //           the next product's operand without a move between lanes.
 //
@@ -45,13 +45,6 @@ template <> __device__ inline f32x16 mfma_step<_Float16>(i32x4 a, i32x4 b, f32x1
 template <> __device__ inline f32x16 mfma_step<__bf16>(i32x4 a, i32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-template <> __device__ inline f32x16 mfma_step<float>(i32x4 a, i32x4 b, f32x16 c) {
-    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-    for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
-    return c;
-}
-
 // Row of a 32x32 result that value i of a lane in half h holds (its column is lane % 32).
 __device__ inline int result_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
@@ -104,7 +97,8 @@ template <int READS, int MFMAS, int SF> __device__ inline void interleave() {
 // that the row's number turns (xor), so that 16 consecutive rows' equal pieces, which one cycle reads, are in different banks.
 template <typename T, int ROWS, int SF, int NW> struct RowTile {
     static constexpr int BYTES = ROWS * SF * 32, LOADS = BYTES / (1024 * NW), PIECES = SF * 2;
-    static constexpr int KE = SF * 32 / (int)sizeof(T); // inner indices of a stage
+    static constexpr int KE = SF * 16; // inner indices of a stage
+    static_assert(sizeof(T) == 2, "values of 16 bits");
     static_assert(BYTES % (1024 * NW) == 0 && (SF == 2 || SF == 4) && NW % 2 == 0, "whole loads");
     uint32_t offset[LOADS], piece;
     uint64_t base;
@@ -142,8 +136,8 @@ template <typename T, int ROWS, int SF, int NW> struct RowTile {
 // COLS columns of a matrix whose inner dimension goes down the rows: rows of a stage as they come, read transposed. The pieces'
 // places turn with the row's last two bits: the four rows that sixteen lanes read together are in different banks.
 template <typename T, int COLS, int SF, int NW, int ORDER> struct ColTile {
-    static constexpr int KE = SF * 32 / (int)sizeof(T), ROWB = COLS * (int)sizeof(T), BYTES = KE * ROWB, LOADS = BYTES / (1024 * NW), PIECES = ROWB / 16;
-    static constexpr int TURN = sizeof(T) == 2 ? (PIECES >= 16 ? 12 : PIECES - 4) : 0;
+    static constexpr int KE = SF * 16, ROWB = COLS * 2, BYTES = KE * ROWB, LOADS = BYTES / (1024 * NW), PIECES = ROWB / 16;
+    static constexpr int TURN = PIECES >= 16 ? 12 : PIECES - 4;
     static_assert(BYTES % (1024 * NW) == 0 && PIECES >= 8, "whole loads");
     using Mask = std::conditional_t<(KE > 32), uint64_t, uint32_t>;
     static_assert(KE <= 64, "one word of rows");
@@ -158,7 +152,7 @@ template <typename T, int COLS, int SF, int NW, int ORDER> struct ColTile {
 #pragma unroll
         for (int i = 0; i < LOADS; i++) {
             const int l = (i * NW + wave) * 64 + lane, row = l / PIECES, piece = (l % PIECES) ^ ((4 * row) & TURN);
-            offset[i] = piece * (16 / (int)sizeof(T)) < cols ? (uint32_t)row * pitch_bytes + piece * 16 : TILE_MASKED;
+            offset[i] = piece * 8 < cols ? (uint32_t)row * pitch_bytes + piece * 16 : TILE_MASKED;
         }
     }
     // bit r of `rows` (KE of them): row r of the stage counts
@@ -175,23 +169,15 @@ template <typename T, int COLS, int SF, int NW, int ORDER> struct ColTile {
     __device__ void next() { base += step; }
     // fragment f of the 32 columns of block cb
     __device__ static i32x4 read(const char* lds, int cb, int f, int lane) {
-        const int h = lane >> 5;
-        if constexpr (sizeof(T) == 2) {
-            const int i = lane & 15, col = ((lane >> 4) & 1) * 16 + 4 * (i & 3), sub = (col & 7) * 2;
-            i32x2 part[2];
+        const int h = lane >> 5, i = lane & 15, col = ((lane >> 4) & 1) * 16 + 4 * (i & 3), sub = (col & 7) * 2;
+        i32x2 part[2];
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int row = f * 16 + (ORDER == ORDER_ROWS ? 8 * h + 4 * j : 4 * h + 8 * j) + (i >> 2);
-                const char* p = lds + row * ROWB + (((cb * 4 + (col >> 3)) ^ ((4 * row) & TURN)) * 16) + sub;
-                part[j] = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
-            }
-            return i32x4{part[0][0], part[0][1], part[1][0], part[1][1]};
-        } else {
-            i32x4 v;
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = *reinterpret_cast<const int*>(lds + (f * 8 + 4 * h + j) * ROWB + (cb * 32 + (lane & 31)) * 4);
-            return v;
+        for (int j = 0; j < 2; j++) {
+            const int row = f * 16 + (ORDER == ORDER_ROWS ? 8 * h + 4 * j : 4 * h + 8 * j) + (i >> 2);
+            const char* p = lds + row * ROWB + (((cb * 4 + (col >> 3)) ^ ((4 * row) & TURN)) * 16) + sub;
+            part[j] = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
         }
+        return i32x4{part[0][0], part[0][1], part[1][0], part[1][1]};
     }
 };
 

@@ -8,10 +8,10 @@
 // reference is the maximum rounded up to a whole number, so that going over to another reference is exact. For gradients the
 // tile's exponentials are rounded to the rows' type and written as 32x32 blocks in the order that a lane has them, which is a
 // fragment of the next product; a piece of them is at most LOSS_PIECE_BYTES.
-//   grad q alone: one pass. A piece's exponentials (relative to their own references) are multiplied with the piece's rows at
+//   grad q (for 16 bits: alone): one pass. A piece's exponentials (relative to their own references) are multiplied with the piece's rows at
 //     once; what the references lack to the common one goes into the exponents of the fragments on their way to the product.
-//   grad x: the normalised G is needed. Where one piece holds everything its exponentials are brought to G in place (a pass over
-//     memory: 38 us for 2048 x 30 522, forming the logits again 150 us); otherwise the logits are formed again once lse is known.
+//   grad x: the normalised G is needed. Where one piece holds everything its 16-bit exponentials are brought to G in place (a pass
+//     over memory: 38 us for 2048 x 30 522, forming the logits again 150 us); otherwise the logits are formed again once lse is known.
 // The targets' own terms are not left to the rounded blocks: their places are zeroed (or rewritten) and W p_t - w_t, which
 // nearly cancels for a query that is served well, is formed in 32 bits.
 #include "apoe_internal.h"
@@ -26,19 +26,34 @@ constexpr uint32_t LOSS_GROUP = 128;               // rows that share a referenc
 constexpr size_t LOSS_PIECE_BYTES = 1u << 30;
 constexpr uint32_t LOSS_CHUNKS = 64;               // parts that the join of the sums is split into, at most
 
-template <typename T> __device__ inline float as_float(T v) { return (float)v; }
+// What the tiles are made of: the type itself, or for float two fp16 planes, a value (times a power of two) rounded and what that
+// left: 22 bits, and a product is three, high x high, high x low, low x high (fp32 products on the matrix cores are 16 times as long).
+template <typename T> struct Tiles {
+    using S = T;
+    static constexpr int PLANES = 1;
+};
+template <> struct Tiles<float> {
+    using S = _Float16;
+    static constexpr int PLANES = 2;
+};
+// G and the queries that it is multiplied with for grad x. fp16 planes hold what is within 2^-38 of the largest of their group, which
+// a sum over rows does not miss; a row of grad x has a sum of its own, however small, so float takes three bf16 planes: 24 bits at any
+// size, and a product is six.
+template <typename T> struct GradTiles : Tiles<T> {};
+template <> struct GradTiles<float> {
+    using S = __bf16;
+    static constexpr int PLANES = 3;
+};
 
 // ---- blocks of 32 queries x 32 rows ----
-// Part p (16 bytes a lane) holds values 8 p .. 8 p + 7 (fp32: 4 p ..) of a lane's 16; half 1 is turned by four lanes and odd parts
-// by eight, so that the transposed read finds halves and parts in different banks.
-template <typename T> struct Block {
-    static constexpr int BYTES = 1024 * (int)sizeof(T), PARTS = BYTES / 1024, VALUES = 16 / (int)sizeof(T);
-    __device__ static int slot(int query, int half, int part) { return half * 32 + (query ^ (half * 4) ^ ((part & 1) * 8)); }
-    __device__ static uint32_t place(int query, int row) { // byte offset of one value
-        const int half = (row >> 2) & 1, i = ((row >> 3) << 2) | (row & 3);
-        return (uint32_t)((i / VALUES) * 1024 + slot(query, half, i / VALUES) * 16 + (i % VALUES) * (int)sizeof(T));
-    }
-};
+// Part p (16 bytes a lane) holds values 8 p .. 8 p + 7 of a lane's 16; half 1 is turned by four lanes and odd parts by eight, so that
+// the transposed read finds halves and parts in different banks.
+constexpr int BLOCK_BYTES = 2048, BLOCK_PARTS = 2;
+__device__ inline int block_slot(int query, int half, int part) { return half * 32 + (query ^ (half * 4) ^ (part * 8)); }
+__device__ inline uint32_t block_place(int query, int row) { // byte offset of one value
+    const int half = (row >> 2) & 1, i = ((row >> 3) << 2) | (row & 3);
+    return (uint32_t)((i >> 3) * 1024 + block_slot(query, half, i >> 3) * 16 + (i & 7) * 2);
+}
 
 // Words that no kernel writes while one reads them, at a place that is the same in the wave: a scalar load, which does not wait
 // for the loads into LDS as a vector load's result would.
@@ -66,6 +81,14 @@ struct LossArgs {
     uint32_t row0, row_tiles, q_tiles, row_blocks; // first row, tiles of either side, blocks of 32 rows (the pitch of `blocks`)
     // workspace
     float *ref, *sum;           // [n / LOSS_GROUP][qp]
+    float* block_ref;           // the same for the blocks: `ref` itself, or with planes less the smallest exponent of the group's rows
+    // the tiles' operands: rows and q themselves, or (float) planes of this piece's rows and of q, whose low parts lie *_low bytes behind
+    const char *tile_rows, *tile_q;
+    uint32_t tile_row0, tile_r_pitch, tile_q_pitch, tile_dim; // the first row at tile_rows; bytes; columns with the pad
+    uint64_t tile_r_low, tile_q_low, block_low;
+    const char* grad_tile_q;    // q as grad x takes it; (float) the planes lie tile_q_low bytes apart
+    float *row_exp, *q_exp;     // planes: exponents of each 32 rows [n / 32]; of q (one)
+    float* q_max;               // [Q_PARTS] largest values of parts of q
     float *chunk_ref, *chunk_sum; // [LOSS_CHUNKS][qp]
     float2* lse_w;              // [qp]: lse in base 2, weight W (to be multiplied with exp(s - lse))
     float *coef, *total;        // [qp]: |weight| (|W| + sum |w|); W
@@ -82,7 +105,7 @@ struct LossArgs {
 // fp16 holds 30 binades of normal numbers, half of them above one: the largest exponential of a group is brought up to 2^14, so
 // that 28 binades stay below it. A query that is served well needs them: its target is the largest, and the gradient is what the
 // others, far below, leave.
-template <typename T> constexpr float HEADROOM = __is_same(T, _Float16) ? 14.f : 0.f;
+template <typename T> constexpr float HEADROOM = __is_same(T, __bf16) ? 0.f : 14.f;
 
 enum { TILE_SUMS = 0, TILE_EXP = 1, TILE_GRAD = 2 };
 
@@ -92,24 +115,161 @@ __device__ inline float grad_scale_of(const uint32_t* top) {
     return t > 0.f && t < 1e30f && t > 1e-30f ? exp2f(13.f - ceilf(log2f(t))) : 1.f;
 }
 
-template <typename T> __device__ inline i32x4 pack(const float* p) {
-    if constexpr (sizeof(T) == 4) {
-        return i32x4{__float_as_int(p[0]), __float_as_int(p[1]), __float_as_int(p[2]), __float_as_int(p[3])};
-    } else {
-        typedef T t8 __attribute__((ext_vector_type(8)));
-        t8 v;
+// A value as a sum of P values of type S.
+template <typename S, int P> __device__ inline void split(float v, S* out) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = (T)p[i];
-        return __builtin_bit_cast(i32x4, v);
+    for (int p = 0; p < P; p++) {
+        out[p] = (S)v;
+        v -= (float)out[p];
+    }
+}
+
+// Eight values of a block (16 bytes of a lane's), and one; the planes lie `low` bytes apart. W: Tiles or GradTiles.
+template <typename W> __device__ inline void put_block(char* at, uint64_t low, const float* v) {
+    using S = typename W::S;
+    typedef S s8 __attribute__((ext_vector_type(8)));
+    s8 planes[W::PLANES];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        S x[W::PLANES];
+        split<S, W::PLANES>(v[i], x);
+#pragma unroll
+        for (int p = 0; p < W::PLANES; p++) planes[p][i] = x[p];
+    }
+#pragma unroll
+    for (int p = 0; p < W::PLANES; p++) *reinterpret_cast<s8*>(at + p * low) = planes[p];
+}
+template <typename W> __device__ inline void put_value(char* at, uint64_t low, float v) {
+    typename W::S x[W::PLANES];
+    split<typename W::S, W::PLANES>(v, x);
+#pragma unroll
+    for (int p = 0; p < W::PLANES; p++) *reinterpret_cast<typename W::S*>(at + p * low) = x[p];
+}
+
+// The product of two fragments of one, two or three planes: the terms that the planes' bits reach, small ones first.
+template <typename W> __device__ inline f32x16 multiply(const i32x4* x, const i32x4* y, f32x16 c) {
+    using S = typename W::S;
+#pragma unroll
+    for (int order = W::PLANES - 1; order >= 0; order--)
+#pragma unroll
+        for (int p = 0; p <= order; p++) c = mfma_step<S>(x[p], y[order - p], c);
+    return c;
+}
+template <typename W> constexpr int PRODUCTS = W::PLANES * (W::PLANES + 1) / 2;
+
+// ---- planes of float matrices ----
+constexpr int Q_PARTS = 256;
+// The power of two that brings `top` to 2^14 .. 2^15.
+__device__ inline int plane_exp(float top) {
+    int e = 0;
+    if (top > 0.f) (void)frexpf(top, &e);
+    return top > 0.f ? 15 - e : 0;
+}
+__device__ inline float finite_abs(float v) {
+    v = fabsf(v);
+    return v <= 3.402823466e38f ? v : 0.f; // not a number: zero
+}
+__device__ inline float block_max(float v, float* buf) { // of 256 threads
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(buf[0], buf[1]), fmaxf(buf[2], buf[3]));
+}
+template <typename S, int P> __device__ inline void put_planes(char* at, uint64_t low, f32x4 x, int k) {
+    typedef S s4 __attribute__((ext_vector_type(4)));
+    s4 planes[P];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        S v[P];
+        split<S, P>(ldexpf(x[i], k), v);
+#pragma unroll
+        for (int p = 0; p < P; p++) planes[p][i] = v[p];
+    }
+#pragma unroll
+    for (int p = 0; p < P; p++) *reinterpret_cast<s4*>(at + p * low) = planes[p];
+}
+
+// 32 rows, which share an exponent: up to 1024 columns they are held in registers between their largest value and the planes (read
+// twice, 100 000 rows took 250 us). Rows that are left out are zeros, and 32 of them have an exponent that no others have.
+constexpr int EMPTY_EXP = 1000;
+__global__ __launch_bounds__(512) void loss_split_rows(LossArgs a) {
+    constexpr int HELD = 16;
+    __shared__ float buf[8];
+    const uint32_t row0 = a.row0 + blockIdx.x * 32, d4 = a.tile_dim / 4, total = 32 * d4;
+    uint32_t on = 0;
+    if (row0 < a.n) {
+        on = a.live ? a.live[row0 >> 5] : ~0u;
+        if (a.n - row0 < 32) on &= (1u << (a.n - row0)) - 1u;
+    }
+    auto fetch = [&](uint32_t at) {
+        const uint32_t r = at / d4, d = at % d4 * 4;
+        f32x4 x = {};
+        if (((on >> r) & 1) && d < a.dim) x = *reinterpret_cast<const f32x4*>((const char*)a.rows + (uint64_t)(row0 + r) * a.r_pitch + d * 4);
+        return x;
+    };
+    auto largest = [](f32x4 x) { return fmaxf(fmaxf(finite_abs(x[0]), finite_abs(x[1])), fmaxf(finite_abs(x[2]), finite_abs(x[3]))); };
+    f32x4 held[HELD];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        const uint32_t at = i * 512 + threadIdx.x;
+        held[i] = at < total ? fetch(at) : f32x4{};
+    }
+#pragma unroll
+    for (int i = 0; i < HELD; i++) top = fmaxf(top, largest(held[i]));
+    for (uint32_t at = HELD * 512 + threadIdx.x; at < total; at += 512) top = fmaxf(top, largest(fetch(at)));
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; w++) top = fmaxf(top, buf[w]);
+    const int k = plane_exp(top);
+    if (threadIdx.x == 0) a.row_exp[row0 / 32] = (float)(on ? k : EMPTY_EXP);
+    auto put = [&](uint32_t at, f32x4 x) {
+        const uint32_t r = at / d4, d = at % d4 * 4;
+        put_planes<_Float16, 2>((char*)a.tile_rows + (uint64_t)(row0 + r - a.tile_row0) * a.tile_r_pitch + d * 2, a.tile_r_low, x, k);
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        const uint32_t at = i * 512 + threadIdx.x;
+        if (at < total) put(at, held[i]);
+    }
+    for (uint32_t at = HELD * 512 + threadIdx.x; at < total; at += 512) put(at, fetch(at));
+}
+__global__ __launch_bounds__(256) void loss_max_q(LossArgs a) {
+    __shared__ float buf[4];
+    float top = 0.f;
+    for (uint32_t r = blockIdx.x; r < a.nq; r += Q_PARTS)
+        for (uint32_t d = threadIdx.x * 4; d < a.dim; d += 1024) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>((const char*)a.q + (uint64_t)r * a.q_pitch + d * 4);
+            top = fmaxf(fmaxf(fmaxf(top, finite_abs(x[0])), fmaxf(finite_abs(x[1]), finite_abs(x[2]))), finite_abs(x[3]));
+        }
+    top = block_max(top, buf);
+    if (threadIdx.x == 0) a.q_max[blockIdx.x] = top;
+}
+__global__ __launch_bounds__(256) void loss_split_q(LossArgs a) {
+    __shared__ float buf[4];
+    const int k = plane_exp(block_max(a.q_max[threadIdx.x], buf));
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.q_exp[0] = (float)k;
+    for (uint32_t d = threadIdx.x * 4; d < a.tile_dim; d += 1024) {
+        f32x4 x = {};
+        if (d < a.dim) x = *reinterpret_cast<const f32x4*>((const char*)a.q + (uint64_t)blockIdx.x * a.q_pitch + d * 4);
+        const uint64_t at = (uint64_t)blockIdx.x * a.tile_q_pitch + d * 2;
+        put_planes<_Float16, 2>((char*)a.tile_q + at, a.tile_q_low, x, k);
+        if (a.grad_x) put_planes<__bf16, 3>((char*)a.grad_tile_q + at, a.tile_q_low, x, 0);
     }
 }
 
 template <typename T, int NT, int WM, int WN, int SF, int ST, int MODE>
 __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossArgs a) {
-    constexpr int NW = WM * WN, BM = WM * 128, BN = WN * NT * 32;
-    using ATile = RowTile<T, BM, SF, NW>;
-    using BTile = RowTile<T, BN, SF, NW>;
-    constexpr int STAGE = ATile::BYTES + BTile::BYTES, PER = ATile::LOADS + BTile::LOADS;
+    using S = typename Tiles<T>::S;
+    constexpr int NW = WM * WN, BM = WM * 128, BN = WN * NT * 32, P = Tiles<T>::PLANES;
+    using ATile = RowTile<S, BM, SF, NW>;
+    using BTile = RowTile<S, BN, SF, NW>;
+    constexpr int PLANE = ATile::BYTES + BTile::BYTES, STAGE = P * PLANE, PER = P * (ATile::LOADS + BTile::LOADS);
     __shared__ __align__(1024) char lds[ST * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
     // consecutive workgroups go to the eight XCDs in turn: those of one XCD share a tile of rows, one after the other
@@ -121,19 +281,25 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
         qt = i % a.q_tiles;
     }
     const uint32_t row = a.row0 + rt * BM, query = qt * BN;
-    ATile ta;
-    BTile tb;
-    ta.init(reinterpret_cast<const T*>((const char*)a.rows + (uint64_t)row * a.r_pitch), a.r_pitch, (int)(row < a.n ? min((uint32_t)BM, a.n - row) : 0u), wave, lane);
-    tb.init(reinterpret_cast<const T*>((const char*)a.q + (uint64_t)query * a.q_pitch), a.q_pitch, (int)min((uint32_t)BN, a.nq - query), wave, lane);
-    const int bytes = (int)(a.dim * sizeof(T)), stages = (bytes + SF * 32 - 1) / (SF * 32);
+    ATile ta[P];
+    BTile tb[P];
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+        ta[p].init(reinterpret_cast<const S*>(a.tile_rows + p * a.tile_r_low + (uint64_t)(row - a.tile_row0) * a.tile_r_pitch), a.tile_r_pitch, (int)(row < a.n ? min((uint32_t)BM, a.n - row) : 0u), wave, lane);
+        tb[p].init(reinterpret_cast<const S*>(a.tile_q + p * a.tile_q_low + (uint64_t)query * a.tile_q_pitch), a.tile_q_pitch, (int)min((uint32_t)BN, a.nq - query), wave, lane);
+    }
+    const int bytes = (int)(a.tile_dim * 2), stages = (bytes + SF * 32 - 1) / (SF * 32);
     const uint32_t base = lds_address(lds);
     int left = bytes;
     uint32_t into = 0;
     auto issue = [&]() {
-        ta.load(base + into, left, wave);
-        tb.load(base + into + ATile::BYTES, left, wave);
-        ta.next();
-        tb.next();
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            ta[p].load(base + into + p * PLANE, left, wave);
+            tb[p].load(base + into + p * PLANE + ATile::BYTES, left, wave);
+            ta[p].next();
+            tb[p].next();
+        }
         left -= SF * 32;
         into = into + STAGE == ST * STAGE ? 0 : into + STAGE;
     };
@@ -146,12 +312,15 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
         issue();
         const char* A = lds + from;
         const char* B = A + ATile::BYTES;
-        i32x4 x[2][4], y[2][NT];
+        i32x4 x[2][4][P], y[2][NT][P];
         auto read = [&](int f) {
 #pragma unroll
-            for (int m = 0; m < 4; m++) x[f & 1][m] = ATile::read(A, wm * 4 + m, f, lane);
+            for (int p = 0; p < P; p++) {
 #pragma unroll
-            for (int t = 0; t < NT; t++) y[f & 1][t] = BTile::read(B, wn * NT + t, f, lane);
+                for (int m = 0; m < 4; m++) x[f & 1][m][p] = ATile::read(A + p * PLANE, wm * 4 + m, f, lane);
+#pragma unroll
+                for (int t = 0; t < NT; t++) y[f & 1][t][p] = BTile::read(B + p * PLANE, wn * NT + t, f, lane);
+            }
         };
         read(0);
 #pragma unroll
@@ -160,15 +329,32 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
 #pragma unroll
             for (int m = 0; m < 4; m++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) acc[m][t] = mfma_step<T>(x[f & 1][m], y[f & 1][t], acc[m][t]);
+                for (int t = 0; t < NT; t++) acc[m][t] = multiply<Tiles<T>>(x[f & 1][m], y[f & 1][t], acc[m][t]);
         }
-        if constexpr (sizeof(T) == 2) interleave<4 + NT, 4 * NT, SF>();
+        interleave<P * (4 + NT), PRODUCTS<Tiles<T>> * 4 * NT, SF>();
         from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
     }
     // epilogue: one query a lane (and its other half), 128 rows a wave
     const int h = lane >> 5;
-    const float c = a.scale * LOG2E;
     const uint32_t wrow = row + wm * LOSS_GROUP;
+    float c[4], down[4], row_exp = 0.f; // of each 32 rows: from sums to logits in base 2; what brings their exponentials to the group's exponent
+    if constexpr (P == 2) {
+        float e[4];
+#pragma unroll
+        for (int m = 0; m < 4; m++) e[m] = a.row_exp[wrow / 32 + m];
+        row_exp = fminf(fminf(e[0], e[1]), fminf(e[2], e[3]));
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            c[m] = ldexpf(a.scale * LOG2E, -(int)(e[m] + a.q_exp[0]));
+            down[m] = __builtin_amdgcn_exp2f(row_exp - e[m]);
+        }
+    } else {
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            c[m] = a.scale * LOG2E;
+            down[m] = 1.f;
+        }
+    }
     uint32_t words[4];
 #pragma unroll
     for (int m = 0; m < 4; m++) words[m] = live_word(a.live, wrow + m * 32, a.n);
@@ -186,7 +372,7 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
             }
         }
         float p[16];
-        char* out = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((wrow - a.row0) >> 5)) * Block<T>::BYTES;
+        char* out = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((wrow - a.row0) >> 5)) * BLOCK_BYTES;
         if constexpr (MODE == TILE_GRAD) {
             const float2 lw = a.lse_w[qi];
             const float g = lw.y * grad_scale_of(a.top_coef);
@@ -196,19 +382,22 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
                 for (int i = 0; i < 16; i++) {
                     const float z = acc[m][t][i];
                     // a query that counts nothing, and a row that is left out, give zero whatever the logit is
-                    p[i] = g == 0.f || z == -INFINITY ? 0.f : g * __builtin_amdgcn_exp2f(__builtin_fmaf(z, c, -lw.x));
+                    p[i] = g == 0.f || z == -INFINITY ? 0.f : g * __builtin_amdgcn_exp2f(__builtin_fmaf(z, c[m], -lw.x));
                 }
 #pragma unroll
-                for (int k = 0; k < Block<T>::PARTS; k++) *reinterpret_cast<i32x4*>(out + m * Block<T>::BYTES + k * 1024 + Block<T>::slot(lane & 31, h, k) * 16) = pack<T>(p + k * Block<T>::VALUES);
+                for (int k = 0; k < BLOCK_PARTS; k++) put_block<GradTiles<T>>(out + m * BLOCK_BYTES + k * 1024 + block_slot(lane & 31, h, k) * 16, a.block_low, p + k * 8);
             }
         } else {
             float top = -INFINITY;
 #pragma unroll
-            for (int m = 0; m < 4; m++)
+            for (int m = 0; m < 4; m++) {
+                float most = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 16; i++) top = fmaxf(top, acc[m][t][i]);
+                for (int i = 0; i < 16; i++) most = fmaxf(most, acc[m][t][i]);
+                if (most != -INFINITY) top = fmaxf(top, most * c[m]); // -inf: all left out (and c may be zero)
+            }
             top = fmaxf(top, __shfl_xor(top, 32));
-            const float ref = top == -INFINITY ? -INFINITY : ceilf(top * c) - HEADROOM<T>;
+            const float ref = top == -INFINITY ? -INFINITY : ceilf(top) - HEADROOM<T>;
             const float less = top == -INFINITY ? 0.f : -ref;
             float sum = 0.f;
 #pragma unroll
@@ -216,12 +405,13 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const float z = acc[m][t][i];
-                    p[i] = z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(z, c, less));
+                    p[i] = z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(z, c[m], less));
                     sum += p[i];
+                    if (P == 2 && MODE == TILE_EXP) p[i] *= down[m];
                 }
                 if constexpr (MODE == TILE_EXP) {
 #pragma unroll
-                    for (int k = 0; k < Block<T>::PARTS; k++) *reinterpret_cast<i32x4*>(out + m * Block<T>::BYTES + k * 1024 + Block<T>::slot(lane & 31, h, k) * 16) = pack<T>(p + k * Block<T>::VALUES);
+                    for (int k = 0; k < BLOCK_PARTS; k++) put_block<Tiles<T>>(out + m * BLOCK_BYTES + k * 1024 + block_slot(lane & 31, h, k) * 16, a.block_low, p + k * 8);
                 }
             }
             sum += __shfl_xor(sum, 32);
@@ -229,6 +419,7 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
                 const size_t at = (size_t)(wrow / LOSS_GROUP) * a.qp + qi;
                 a.ref[at] = ref;
                 a.sum[at] = sum;
+                if (P == 2 && MODE == TILE_EXP) a.block_ref[at] = ref - row_exp;
             }
         }
     }
@@ -271,8 +462,8 @@ template <typename T, bool ZERO> __global__ __launch_bounds__(256) void loss_joi
             for (uint32_t e = a.t_off[qi] + gl; e < a.t_off[qi + 1]; e += 8) {
                 const uint32_t t = a.t_idx[e];
                 if (t < a.row0 || t >= end) continue;
-                char* block = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((t - a.row0) >> 5)) * Block<T>::BYTES;
-                *reinterpret_cast<T*>(block + Block<T>::place(ql, (t - a.row0) & 31)) = (T)0.f;
+                char* block = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((t - a.row0) >> 5)) * BLOCK_BYTES;
+                put_value<Tiles<T>>(block + block_place(ql, (t - a.row0) & 31), a.block_low, 0.f);
             }
         }
     }
@@ -349,29 +540,28 @@ template <typename T> __global__ __launch_bounds__(256) void loss_normalise(Loss
     const uint32_t wave = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t g = wave % groups, qb = wave / groups;
     if (qb >= a.qp / 32) return;
-    char* block = a.blocks + ((size_t)qb * a.row_blocks + g * (LOSS_GROUP / 32)) * Block<T>::BYTES;
-    constexpr int LOADS = LOSS_GROUP / 32 * Block<T>::PARTS;
+    char* block = a.blocks + ((size_t)qb * a.row_blocks + g * (LOSS_GROUP / 32)) * BLOCK_BYTES + lane * 16;
+    constexpr int LOADS = LOSS_GROUP / 32 * BLOCK_PARTS;
     float f[2]; // of odd parts another lane's query
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        const uint32_t qi = qb * 32 + (uint32_t)((int)(lane & 31) ^ ((int)(lane >> 5) * 4) ^ (k * 8)); // slot() is its own inverse within a half
+        const uint32_t qi = qb * 32 + (uint32_t)((int)(lane & 31) ^ ((int)(lane >> 5) * 4) ^ (k * 8)); // a slot is its own inverse within a half
         const float ref = a.ref[(size_t)(a.row0 / LOSS_GROUP + g) * a.qp + qi];
         const float2 lw = a.lse_w[qi];
         const float c = lw.y * grad_scale_of(a.top_coef);
         f[k] = c == 0.f || ref == -INFINITY ? 0.f : c * __builtin_amdgcn_exp2f(ref - lw.x);
     }
-    i32x4 v[LOADS];
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    t8 v[LOADS];
 #pragma unroll
-    for (int i = 0; i < LOADS; i++) v[i] = *reinterpret_cast<const i32x4*>(block + i * 1024 + lane * 16);
+    for (int i = 0; i < LOADS; i++) v[i] = *reinterpret_cast<const t8*>(block + i * 1024);
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
-        typedef T tv __attribute__((ext_vector_type(Block<T>::VALUES)));
-        const tv x = __builtin_bit_cast(tv, v[i]);
-        float p[Block<T>::VALUES];
-        const float c = f[i & 1]; // PARTS is even
+        float p[8];
+        const float c = f[i & 1];
 #pragma unroll
-        for (int k = 0; k < Block<T>::VALUES; k++) p[k] = c == 0.f ? 0.f : (float)x[k] * c;
-        *reinterpret_cast<i32x4*>(block + i * 1024 + lane * 16) = pack<T>(p);
+        for (int k = 0; k < 8; k++) p[k] = c == 0.f ? 0.f : (float)v[i][k] * c;
+        put_block<Tiles<T>>(block + i * 1024, 0, p);
     }
 }
 
@@ -418,8 +608,8 @@ template <typename T, bool ALL> __global__ __launch_bounds__(64) void loss_targe
         if (lane == 0) {
             const float p = exp2f(__builtin_fmaf(dot, a.scale * LOG2E, -lw.x));
             const float g = cw == 0.f ? 0.f : gs * (lw.y * p - cw * w);
-            char* block = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((t - a.row0) >> 5)) * Block<T>::BYTES;
-            *reinterpret_cast<T*>(block + Block<T>::place(qi & 31, (t - a.row0) & 31)) = (T)g;
+            char* block = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((t - a.row0) >> 5)) * BLOCK_BYTES;
+            put_value<GradTiles<T>>(block + block_place(qi & 31, (t - a.row0) & 31), a.block_low, g);
         }
     }
     if (ALL && lane == 0) {
@@ -429,14 +619,10 @@ template <typename T, bool ALL> __global__ __launch_bounds__(64) void loss_targe
     }
 }
 
-// A fragment's values times 2^-less, less >= 0. They are not negative, so bf16 needs one saturating subtraction on the exponent of
+// A fragment's values times 2^-less, less >= 0. bf16 exponentials are not negative and need one saturating subtraction on the exponent of
 // two at a time: what falls below the smallest normal number becomes zero or stays below it.
 template <typename T> __device__ inline i32x4 scale_down(i32x4 v, float less) {
-    if constexpr (sizeof(T) == 4) {
-        const float f = __builtin_amdgcn_exp2f(-less);
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = __float_as_int(__int_as_float(v[i]) * f);
-    } else if constexpr (__is_same(T, _Float16)) {
+    if constexpr (__is_same(T, _Float16)) {
         // in two steps: a factor below 2^-24 is no fp16 number, but 2^14 times it may be
         const float some = fminf(less, 14.f);
         const _Float16 f = (_Float16)__builtin_amdgcn_exp2f(-some), g = (_Float16)__builtin_amdgcn_exp2f(some - less);
@@ -458,13 +644,14 @@ template <typename T> __device__ inline i32x4 scale_down(i32x4 v, float less) {
 // DIRECT: the only split of the only piece, whose sum is the gradient.
 template <typename T, int MT, int NT, int WM, int WN, int ST, bool EXP, bool DIRECT = false>
 __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint32_t n_tiles, uint32_t groups_per_split, uint32_t piece_groups, int turn, int first) {
-    constexpr int NW = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, SF = sizeof(T) == 4 ? 4 : 2;
-    using BTile = ColTile<T, BN, SF, NW, ORDER_BLOCKS>;
+    using S = typename Tiles<T>::S;
+    constexpr int NW = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, SF = 2, P = Tiles<T>::PLANES;
+    using BTile = ColTile<S, BN, SF, NW, ORDER_BLOCKS>;
     static_assert(BTile::KE == 32, "a block a stage");
-    constexpr int ABYTES = BM / 32 * Block<T>::BYTES, AINS = ABYTES / 1024, ALOADS = (AINS + NW - 1) / NW;
+    constexpr int ABYTES = BM / 32 * BLOCK_BYTES, AINS = ABYTES / 1024, ALOADS = (AINS + NW - 1) / NW, PLANE = ABYTES + BTile::BYTES;
     constexpr int RBYTES = NW * 256; // references: 64 queries a wave
     static_assert(NW * 64 >= BM, "a reference a query");
-    constexpr int STAGE = ABYTES + BTile::BYTES + (EXP ? RBYTES : 0), PER = ALOADS + BTile::LOADS + (EXP ? 1 : 0);
+    constexpr int STAGE = P * PLANE + (EXP ? RBYTES : 0), PER = P * (ALOADS + BTile::LOADS) + (EXP ? 1 : 0);
     __shared__ __align__(1024) char lds[ST * STAGE];
     __shared__ float factor[2][BM];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
@@ -483,7 +670,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
         if (threadIdx.x < BM) {
             const uint32_t qi = query + threadIdx.x;
             const bool real = qi < a.qp;
-            for (uint32_t g = g0; g < g1; g++) top = fmaxf(top, real ? a.ref[(size_t)(group0 + g) * a.qp + qi] : -INFINITY);
+            for (uint32_t g = g0; g < g1; g++) top = fmaxf(top, real ? a.block_ref[(size_t)(group0 + g) * a.qp + qi] : -INFINITY);
             factor[0][threadIdx.x] = top;
         }
         __syncthreads();
@@ -497,15 +684,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
     const uint32_t q_blocks = a.qp / 32;
 #pragma unroll
     for (int i = 0; i < ALOADS; i++) {
-        const int ins = (i * NW + wave) % AINS, b = ins / Block<T>::PARTS, k = ins % Block<T>::PARTS; // a wave without one of its own repeats another's
+        const int ins = (i * NW + wave) % AINS, b = ins / BLOCK_PARTS, k = ins % BLOCK_PARTS; // a wave without one of its own repeats another's
         adst[i] = ins * 1024;
-        aoff[i] = query / 32 + b < q_blocks ? (uint32_t)b * (a.row_blocks * (uint32_t)Block<T>::BYTES) + k * 1024 + lane * 16 : TILE_MASKED;
+        aoff[i] = query / 32 + b < q_blocks ? (uint32_t)b * (a.row_blocks * (uint32_t)BLOCK_BYTES) + k * 1024 + lane * 16 : TILE_MASKED;
     }
-    uint64_t abase = uniform64((uint64_t)a.blocks + ((uint64_t)(query / 32) * a.row_blocks + g0 * (LOSS_GROUP / 32)) * Block<T>::BYTES);
-    uint64_t rbase = uniform64((uint64_t)(a.ref + (size_t)(group0 + g0) * a.qp + query));
-    BTile tb;
+    uint64_t abase = uniform64((uint64_t)a.blocks + ((uint64_t)(query / 32) * a.row_blocks + g0 * (LOSS_GROUP / 32)) * BLOCK_BYTES);
+    uint64_t rbase = uniform64((uint64_t)(a.block_ref + (size_t)(group0 + g0) * a.qp + query));
+    BTile tb[P];
     const uint32_t first_row = a.row0 + g0 * LOSS_GROUP;
-    tb.init(reinterpret_cast<const T*>((const char*)a.rows + (uint64_t)first_row * a.r_pitch) + col, a.r_pitch, (int)min((uint32_t)BN, a.dim - col), wave, lane);
+#pragma unroll
+    for (int p = 0; p < P; p++)
+        tb[p].init(reinterpret_cast<const S*>(a.tile_rows + p * a.tile_r_low + (uint64_t)(first_row - a.tile_row0) * a.tile_r_pitch) + col, a.tile_r_pitch, (int)min((uint32_t)BN, a.tile_dim - col), wave, lane);
     const uint32_t roff = query + wave * 64 + lane < a.qp ? (wave * 64 + lane) * 4 : TILE_MASKED;
 
     const int stages = (int)(g1 - g0) * (LOSS_GROUP / 32);
@@ -514,15 +703,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
     uint32_t word = stages ? live_word(a.live, first_row, a.n) : 0u;
     auto issue = [&]() {
         const bool in = (int)issued < stages;
-        const i32x4 ab = buffer_of(abase);
 #pragma unroll
-        for (int i = 0; i < ALOADS; i++) load_to_lds16(ab, in ? aoff[i] : TILE_MASKED, base + into + adst[i]);
-        tb.load(base + into + ABYTES, in ? word : 0u, wave, lane);
-        if constexpr (EXP) {
-            load_to_lds4(buffer_of(uniform64(rbase)), in ? roff : TILE_MASKED, base + into + ABYTES + BTile::BYTES + wave * 256);
+        for (int p = 0; p < P; p++) {
+            const i32x4 ab = buffer_of(abase + p * a.block_low);
+#pragma unroll
+            for (int i = 0; i < ALOADS; i++) load_to_lds16(ab, in ? aoff[i] : TILE_MASKED, base + into + p * PLANE + adst[i]);
+            tb[p].load(base + into + p * PLANE + ABYTES, in ? word : 0u, wave, lane);
+            tb[p].next();
         }
-        abase += Block<T>::BYTES;
-        tb.next();
+        if constexpr (EXP) load_to_lds4(buffer_of(uniform64(rbase)), in ? roff : TILE_MASKED, base + into + P * PLANE + wave * 256);
+        abase += BLOCK_BYTES;
         issued++;
         if (issued % (LOSS_GROUP / 32) == 0) rbase += a.qp * 4;
         word = (int)issued < stages ? live_word(a.live, first_row + issued * 32, a.n) : 0u;
@@ -539,19 +729,23 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
         const char* B = A + ABYTES;
         float less[MT];
         if constexpr (EXP) {
-            const float* r = reinterpret_cast<const float*>(B + BTile::BYTES);
+            const float* r = reinterpret_cast<const float*>(A + P * PLANE);
 #pragma unroll
             for (int m = 0; m < MT; m++) {
                 const float own = r[(wm * MT + m) * 32 + (lane & 31)];
                 less[m] = own == -INFINITY ? 0.f : mine[m] - own; // a group without live rows holds zeros
             }
         }
-        i32x4 x[2][MT], y[2][NT];
+        i32x4 x[2][MT][P], y[2][NT][P];
         auto read = [&](int f) {
 #pragma unroll
-            for (int m = 0; m < MT; m++) x[f & 1][m] = *reinterpret_cast<const i32x4*>(A + (wm * MT + m) * Block<T>::BYTES + f * 1024 + Block<T>::slot(lane & 31, lane >> 5, f) * 16);
+            for (int p = 0; p < P; p++) {
 #pragma unroll
-            for (int t = 0; t < NT; t++) y[f & 1][t] = BTile::read(B, wn * NT + t, f, lane);
+                for (int m = 0; m < MT; m++)
+                    x[f & 1][m][p] = *reinterpret_cast<const i32x4*>(A + p * PLANE + (wm * MT + m) * BLOCK_BYTES + f * 1024 + block_slot(lane & 31, lane >> 5, f) * 16);
+#pragma unroll
+                for (int t = 0; t < NT; t++) y[f & 1][t][p] = BTile::read(B + p * PLANE, wn * NT + t, f, lane);
+            }
         };
         read(0);
 #pragma unroll
@@ -559,14 +753,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
             if (f + 1 < SF) read(f + 1);
             if constexpr (EXP) {
 #pragma unroll
-                for (int m = 0; m < MT; m++) x[f & 1][m] = scale_down<T>(x[f & 1][m], less[m]);
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int p = 0; p < P; p++) x[f & 1][m][p] = scale_down<S>(x[f & 1][m][p], less[m]);
             }
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) acc[m][t] = mfma_step<T>(x[f & 1][m], y[f & 1][t], acc[m][t]);
+                for (int t = 0; t < NT; t++) acc[m][t] = multiply<Tiles<T>>(x[f & 1][m], y[f & 1][t], acc[m][t]);
         }
-        if constexpr (sizeof(T) == 2) interleave<MT + 2 * NT, MT * NT, SF>();
+        interleave<P * (MT + 2 * NT), PRODUCTS<Tiles<T>> * MT * NT, SF>();
         from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
     }
     tile_wait<0>();
@@ -616,10 +812,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
 // grad x of a piece: rows (blocks read transposed) x queries. Each row's gradient is whole here: all queries are in.
 template <typename T, int MT, int NT, int WM, int WN, int ST>
 __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint32_t n_tiles) {
-    constexpr int NW = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, SF = sizeof(T) == 4 ? 4 : 2;
-    using BTile = ColTile<T, BN, SF, NW, ORDER_ROWS>;
-    constexpr int ABYTES = BM / 32 * Block<T>::BYTES, ALOADS = ABYTES / (1024 * NW);
-    constexpr int STAGE = ABYTES + BTile::BYTES, PER = ALOADS + BTile::LOADS;
+    using S = typename GradTiles<T>::S;
+    constexpr int NW = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, SF = 2, P = GradTiles<T>::PLANES;
+    using BTile = ColTile<S, BN, SF, NW, ORDER_ROWS>;
+    constexpr int ABYTES = BM / 32 * BLOCK_BYTES, ALOADS = ABYTES / (1024 * NW), PLANE = ABYTES + BTile::BYTES;
+    constexpr int STAGE = P * PLANE, PER = P * (ALOADS + BTile::LOADS);
     __shared__ __align__(1024) char lds[ST * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
     uint32_t rt = blockIdx.x / n_tiles, col = blockIdx.x % n_tiles * BN;
@@ -634,24 +831,29 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint3
 #pragma unroll
     for (int i = 0; i < ALOADS; i++) {
         const int ins = i * NW + wave;
-        aoff[i] = block0 + ins / Block<T>::PARTS < a.row_blocks ? ins * 1024 + lane * 16 : TILE_MASKED;
+        aoff[i] = block0 + ins / BLOCK_PARTS < a.row_blocks ? ins * 1024 + lane * 16 : TILE_MASKED;
     }
-    uint64_t abase = uniform64((uint64_t)a.blocks + (uint64_t)block0 * Block<T>::BYTES);
-    const uint64_t astep = (uint64_t)a.row_blocks * Block<T>::BYTES;
-    BTile tb;
-    tb.init(reinterpret_cast<const T*>(a.q) + col, a.q_pitch, (int)min((uint32_t)BN, a.dim - col), wave, lane);
+    uint64_t abase = uniform64((uint64_t)a.blocks + (uint64_t)block0 * BLOCK_BYTES);
+    const uint64_t astep = (uint64_t)a.row_blocks * BLOCK_BYTES;
+    BTile tb[P];
+#pragma unroll
+    for (int p = 0; p < P; p++) tb[p].init(reinterpret_cast<const S*>(a.grad_tile_q + p * a.tile_q_low) + col, a.tile_q_pitch, (int)min((uint32_t)BN, a.tile_dim - col), wave, lane);
     const UniformWords q_on = (UniformWords)a.q_on;
     const int stages = (int)((a.nq + 31) / 32);
     const uint32_t base = lds_address(lds);
     uint32_t into = 0, issued = 0;
     auto issue = [&]() {
         const bool in = (int)issued < stages;
-        const i32x4 ab = buffer_of(abase);
+        const uint32_t on = in ? q_on[issued] : 0u;
 #pragma unroll
-        for (int i = 0; i < ALOADS; i++) load_to_lds16(ab, in ? aoff[i] : TILE_MASKED, base + into + (i * NW + wave) * 1024);
-        tb.load(base + into + ABYTES, in ? q_on[issued] : 0u, wave, lane);
+        for (int p = 0; p < P; p++) {
+            const i32x4 ab = buffer_of(abase + p * a.block_low);
+#pragma unroll
+            for (int i = 0; i < ALOADS; i++) load_to_lds16(ab, in ? aoff[i] : TILE_MASKED, base + into + p * PLANE + (i * NW + wave) * 1024);
+            tb[p].load(base + into + p * PLANE + ABYTES, on, wave, lane);
+            tb[p].next();
+        }
         abase += astep;
-        tb.next();
         issued++;
         into = into + STAGE == ST * STAGE ? 0 : into + STAGE;
     };
@@ -664,29 +866,26 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint3
         issue();
         const char* A = lds + from;
         const char* B = A + ABYTES;
-        i32x4 x[2][MT], y[2][NT];
+        i32x4 x[2][MT][P], y[2][NT][P];
         auto read = [&](int f) {
+            const int h = lane >> 5, i = lane & 15, g = (lane >> 4) & 1;
 #pragma unroll
-            for (int m = 0; m < MT; m++) {
-                const char* block = A + (wm * MT + m) * Block<T>::BYTES;
-                const int h = lane >> 5;
-                if constexpr (sizeof(T) == 2) {
-                    const int i = lane & 15, g = (lane >> 4) & 1;
+            for (int p = 0; p < P; p++) {
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    const char* block = A + p * PLANE + (wm * MT + m) * BLOCK_BYTES;
                     i32x2 part[2];
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         const int q = f * 16 + 8 * h + 4 * j + (i >> 2);
-                        const char* p = block + g * 1024 + Block<T>::slot(q, i & 1, g) * 16 + ((i & 3) >> 1) * 8;
-                        part[j] = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+                        const char* at = block + g * 1024 + block_slot(q, i & 1, g) * 16 + ((i & 3) >> 1) * 8;
+                        part[j] = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at));
                     }
-                    x[f & 1][m] = i32x4{part[0][0], part[0][1], part[1][0], part[1][1]};
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) x[f & 1][m][j] = *reinterpret_cast<const int*>(block + Block<T>::place(f * 8 + 4 * h + j, lane & 31));
+                    x[f & 1][m][p] = i32x4{part[0][0], part[0][1], part[1][0], part[1][1]};
                 }
-            }
 #pragma unroll
-            for (int t = 0; t < NT; t++) y[f & 1][t] = BTile::read(B, wn * NT + t, f, lane);
+                for (int t = 0; t < NT; t++) y[f & 1][t][p] = BTile::read(B + p * PLANE, wn * NT + t, f, lane);
+            }
         };
         read(0);
 #pragma unroll
@@ -695,9 +894,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint3
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) acc[m][t] = mfma_step<T>(x[f & 1][m], y[f & 1][t], acc[m][t]);
+                for (int t = 0; t < NT; t++) acc[m][t] = multiply<GradTiles<T>>(x[f & 1][m], y[f & 1][t], acc[m][t]);
         }
-        if constexpr (sizeof(T) == 2) interleave<2 * MT + 2 * NT, MT * NT, SF>();
+        interleave<P * (2 * MT + 2 * NT), PRODUCTS<GradTiles<T>> * MT * NT, SF>();
         from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
     }
     tile_wait<0>();
@@ -858,21 +1057,25 @@ template <typename T, bool GRAD, bool EXP, int THREADS> __global__ __launch_boun
 }
 
 // ---- few queries ----
-// Up to four queries of up to 1024 columns: every row is read once, by one wave, which keeps the queries, its running sums and the
+// Up to four queries (float: eight) of up to 1024 columns: every row is read once from memory, by one wave, which keeps the queries, its running sums and the
 // rows on their way in registers (a tile of 32 queries would be mostly empty, and its rows would be read twice). A wave takes four
 // rows at a time and asks for the next four before it works on these; four inner products are summed over the lanes together.
 // Exponentials are relative to a whole exponent that moves only when a logit passes it by 2^60: sums in 32 bits bear that.
 constexpr int FEW_E = 16; // values of a row that a lane holds
 constexpr uint32_t FEW_MAX_DIM = 64 * FEW_E, FEW_BLOCKS = 512;
-template <typename T> constexpr uint32_t FEW_QUERIES = sizeof(T) == 2 ? 4 : 2; // what the registers hold beside the rows on their way
+// What the registers hold beside the rows on their way, and up to how many queries: pairs of float queries are worked on side by side,
+// by workgroups that read the same rows at the same time (8 queries x 1 M rows: 2.48 ms; by tiles, whose planes are written first: 3.34).
+template <typename T> constexpr uint32_t FEW_HELD = sizeof(T) == 2 ? 4 : 2;
+template <typename T> constexpr uint32_t FEW_QUERIES = sizeof(T) == 2 ? 4 : 8;
 
-template <typename T, int NQ, bool GRAD> __global__ __launch_bounds__(256, 2) void loss_few(LossArgs a) {
+template <typename T, int NQ, bool GRAD> __global__ __launch_bounds__(256, 2) void loss_few(LossArgs a, uint32_t sets) {
     constexpr int V = 16 / (int)sizeof(T), C = FEW_E / V;
     typedef T tv __attribute__((ext_vector_type(V)));
     __shared__ float refs[NQ][4], sums[NQ][4];
     __shared__ float part[GRAD ? 4 : 1][GRAD ? NQ * FEW_MAX_DIM : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t fours = (a.n + 3) / 4, step = gridDim.x * 4;
+    const uint32_t split = blockIdx.x / sets, q0 = blockIdx.x % sets * NQ; // the sets of one split side by side
+    const uint32_t fours = (a.n + 3) / 4, step = gridDim.x / sets * 4;
     const float c = a.scale * LOG2E;
     float q[NQ][FEW_E], acc[NQ][FEW_E] = {}, ref[NQ], sum[NQ] = {};
 #pragma unroll
@@ -882,7 +1085,7 @@ template <typename T, int NQ, bool GRAD> __global__ __launch_bounds__(256, 2) vo
         for (int k = 0; k < C; k++) {
             const uint32_t d = (k * 64 + lane) * V;
             tv x = {};
-            if (n < (int)a.nq && d < a.dim) x = *reinterpret_cast<const tv*>((const char*)a.q + (uint64_t)n * a.q_pitch + d * sizeof(T));
+            if (q0 + n < a.nq && d < a.dim) x = *reinterpret_cast<const tv*>((const char*)a.q + (uint64_t)(q0 + n) * a.q_pitch + d * sizeof(T));
 #pragma unroll
             for (int v = 0; v < V; v++) q[n][k * V + v] = (float)x[v];
         }
@@ -898,7 +1101,7 @@ template <typename T, int NQ, bool GRAD> __global__ __launch_bounds__(256, 2) vo
                 if (((on >> r) & 1) && d < a.dim) x[r][k] = *reinterpret_cast<const tv*>((const char*)a.rows + (uint64_t)(four * 4 + r) * a.r_pitch + d * sizeof(T));
             }
     };
-    uint32_t four = blockIdx.x * 4 + wave, on = live_four(four);
+    uint32_t four = split * 4 + wave, on = live_four(four);
     tv next[4][C];
     load(next, four, on);
     while (four < fours) {
@@ -971,7 +1174,7 @@ template <typename T, int NQ, bool GRAD> __global__ __launch_bounds__(256, 2) vo
         if (threadIdx.x == 0) {
             float t = 0.f, r = -INFINITY;
             for (int k = 0; k < 4; k++) join_sums(r, t, refs[n][k], sums[n][k]);
-            const size_t at = (size_t)blockIdx.x * a.qp + n;
+            const size_t at = (size_t)split * a.qp + q0 + n;
             a.chunk_ref[at] = r;
             a.chunk_sum[at] = t;
             if constexpr (GRAD) a.part_ref[0][at] = top;
@@ -990,7 +1193,7 @@ template <typename T, int NQ, bool GRAD> __global__ __launch_bounds__(256, 2) vo
         for (int n = 0; n < NQ; n++)
             for (uint32_t d = threadIdx.x; d < a.dim; d += 256) {
                 const uint32_t at = n * FEW_MAX_DIM + d;
-                a.part[((size_t)blockIdx.x * a.qp + n) * a.dim + d] = (part[0][at] + part[1][at]) + (part[2][at] + part[3][at]);
+                a.part[((size_t)split * a.qp + q0 + n) * a.dim + d] = (part[0][at] + part[1][at]) + (part[2][at] + part[3][at]);
             }
     }
 }
@@ -1067,8 +1270,9 @@ static uint32_t up(uint64_t v, uint64_t to) { return (uint32_t)((v + to - 1) / t
 
 template <typename T> static int run_few(apoe_ctx* ctx, LossArgs& a, bool grad) {
     // a wave has two turns of four rows at least, a CU two workgroups at most
-    const uint32_t blocks = std::max(1u, std::min((a.n + 31) / 32, std::min(FEW_BLOCKS, 2 * (uint32_t)ctx->num_cus)));
-    a.qp = next_pow2(a.nq); // as many as the kernel carries
+    const uint32_t held = std::min(FEW_HELD<T>, next_pow2(a.nq)), sets = (a.nq + held - 1) / held;
+    const uint32_t blocks = std::max(1u, std::min((a.n + 31) / 32, std::min(FEW_BLOCKS, 2 * (uint32_t)ctx->num_cus) / sets));
+    a.qp = sets * held;
     a.chunks = a.splits = blocks;
     const size_t sums = (size_t)blocks * a.qp * 4, up16 = (sums + 15) / 16 * 16;
     char* ws = nullptr;
@@ -1080,12 +1284,12 @@ template <typename T> static int run_few(apoe_ctx* ctx, LossArgs& a, bool grad) 
     hipStream_t s = ctx->stream;
     auto go = [&](auto n) {
         constexpr int NQ = decltype(n)::value;
-        if (grad) loss_few<T, NQ, true><<<blocks, 256, 0, s>>>(a);
-        else loss_few<T, NQ, false><<<blocks, 256, 0, s>>>(a);
+        if (grad) loss_few<T, NQ, true><<<blocks * sets, 256, 0, s>>>(a, sets);
+        else loss_few<T, NQ, false><<<blocks * sets, 256, 0, s>>>(a, sets);
     };
-    if (a.nq == 1) go(std::integral_constant<int, 1>{});
-    else if (a.nq == 2) go(std::integral_constant<int, 2>{});
-    else if constexpr (FEW_QUERIES<T> == 4) go(std::integral_constant<int, 4>{});
+    if (held == 1) go(std::integral_constant<int, 1>{});
+    else if (held == 2) go(std::integral_constant<int, 2>{});
+    else if constexpr (FEW_HELD<T> == 4) go(std::integral_constant<int, 4>{});
     if (grad) loss_few_finish<T, true><<<a.nq, 1024, 0, s>>>(a);
     else loss_few_finish<T, false><<<a.nq, 1024, 0, s>>>(a);
     APOE_HIP(hipGetLastError());
@@ -1094,7 +1298,7 @@ template <typename T> static int run_few(apoe_ctx* ctx, LossArgs& a, bool grad) 
 
 template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss_args* p) {
     LossArgs a{};
-    const bool gq = p->grad_q != nullptr, gx = p->grad_rows != nullptr, two_pass = gx;
+    const bool gq = p->grad_q != nullptr, gx = p->grad_rows != nullptr;
     a.q = p->q;
     a.rows = p->rows;
     a.q_pitch = (uint32_t)(p->q_stride * sizeof(T));
@@ -1120,39 +1324,41 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     //   256 x 128  where those fill it (128 x 131 072: 56 us; 128 x 128: 66)
     //   128 x 128  for fewer rows (1024 x 4000: 16.5 us; 256 x 128: 20)
     //   128 x 64   up to 64 queries (64 x 30 000: 15.5 us; 128 x 128: 17), 512 x 32 for up to 32 where those fill it (32 x 131 072: 44 us; 48)
-    // and for fp32, whose products are 16 times as long, 256 x 128 and 512 x 64 or 32.
-    enum { T256, T256_128, T128, T128_64, T512_32, F256_128, F512_64, F512_32 } form;
+    // For float, whose planes are twice the bytes, 256 x 256, 128 x 128 or 128 x 64.
+    enum { T256, T256_128, T128, T128_64, T512_32 } form;
+    constexpr int PLANES = Tiles<T>::PLANES;
     const uint32_t cus = (uint32_t)ctx->num_cus;
     auto count = [&](uint32_t rows, uint32_t queries) { return (uint64_t)((a.n + rows - 1) / rows) * ((a.nq + queries - 1) / queries); };
-    if (sizeof(T) == 4) form = a.nq <= 32 ? F512_32 : a.nq <= 64 ? F512_64 : F256_128;
-    else if (a.nq <= 32 && count(512, 32) >= cus) form = T512_32;
+    if (PLANES == 1 && a.nq <= 32 && count(512, 32) >= cus) form = T512_32;
     else if (a.nq <= 64) form = T128_64;
     else if (count(256, 256) >= cus && (up(a.nq, 256) == up(a.nq, 128) || a.nq > 1024)) form = T256;
-    else if (count(256, 128) >= cus) form = T256_128;
+    else if (PLANES == 1 && count(256, 128) >= cus) form = T256_128;
     else form = T128;
-    const uint32_t bm = form == T512_32 || form == F512_32 || form == F512_64 ? 512 : form == T128 || form == T128_64 ? 128 : 256;
-    const uint32_t bn = form == T256 ? 256 : form == T128_64 || form == F512_64 ? 64 : form == T512_32 || form == F512_32 ? 32 : 128;
+    const uint32_t bm = form == T512_32 ? 512 : form == T128 || form == T128_64 ? 128 : 256;
+    const uint32_t bn = form == T256 ? 256 : form == T128_64 ? 64 : form == T512_32 ? 32 : 128;
     a.qp = up(a.nq, bn);
     a.q_tiles = a.qp / bn;
     const uint32_t rows_up = up(a.n, bm);
-    uint64_t piece = rows_up; // rows of a piece: whole tiles
-    if (gq || gx) {
-        const uint64_t most = std::max<uint64_t>(bm, LOSS_PIECE_BYTES / ((uint64_t)a.qp * sizeof(T)) / bm * bm);
-        const uint64_t pieces = (rows_up + most - 1) / most;
-        piece = up((rows_up + pieces - 1) / pieces, bm);
-    }
+    a.tile_dim = up(a.dim, 8);
+    // rows of a piece, whole tiles: bounded by the exponentials, by the planes, and by what a launch may count
+    uint64_t most = (uint64_t)bm * std::max<uint32_t>(1, (1u << 22) / a.q_tiles);
+    if (gq || gx) most = std::min(most, LOSS_PIECE_BYTES / ((uint64_t)a.qp * 2 * (gx ? GradTiles<T>::PLANES : PLANES)) / bm * bm);
+    if (PLANES == 2) most = std::min(most, LOSS_PIECE_BYTES / ((uint64_t)a.tile_dim * 4) / bm * bm);
+    most = std::max<uint64_t>(bm, most);
+    const uint64_t even = (rows_up + most - 1) / most;
+    const uint64_t piece = up((rows_up + even - 1) / even, bm);
     const uint32_t pieces = (uint32_t)((rows_up + piece - 1) / piece);
     a.groups = rows_up / LOSS_GROUP;
     const uint32_t chunks_per_piece = std::min<uint32_t>(std::max<uint32_t>(1, LOSS_CHUNKS / pieces), (uint32_t)((piece / LOSS_GROUP + 31) / 32));
     a.chunks = chunks_per_piece * pieces;
-    // grad q: tiles of 256 x 256, of 128 or 64 x 256 (fp32: 128 or 32 x 128); enough splits of the rows to fill the GPU (twice
+    // grad q: tiles of 256 x 256, of 128 or 64 x 256 (float: 128 or 64 x 128); enough splits of the rows to fill the GPU (twice
     // over where a CU holds two workgroups)
-    const uint32_t qm = form == T256 ? 256 : a.nq > 64 ? 128 : sizeof(T) == 2 ? 64 : a.nq > 32 ? 128 : 32, qn = sizeof(T) == 4 ? 128 : 256;
+    const uint32_t qm = a.nq <= 64 ? 64 : form == T256 && PLANES == 1 ? 256 : 128, qn = PLANES == 2 ? 128 : 256;
     const uint32_t gq_q_tiles = (a.qp + qm - 1) / qm, gq_n_tiles = (a.dim + qn - 1) / qn;
     const uint32_t piece_groups = (uint32_t)(piece / LOSS_GROUP);
     // With G whole in one piece, tiles of 128 x 128 that fill the GPU need no splits: 4096 x 4096 takes 15 us less.
-    const bool direct = sizeof(T) == 2 && gq && two_pass && pieces == 1 && (uint64_t)((a.qp + 127) / 128) * ((a.dim + 127) / 128) >= cus * 9 / 10;
-    uint32_t splits = std::min(LOSS_SPLITS, std::max<uint32_t>(1, (form == T256 ? 1 : 2) * cus / (gq_q_tiles * gq_n_tiles)));
+    const bool direct = PLANES == 1 && gq && gx && pieces == 1 && (uint64_t)((a.qp + 127) / 128) * ((a.dim + 127) / 128) >= cus * 9 / 10;
+    uint32_t splits = std::min(LOSS_SPLITS, std::max<uint32_t>(1, (qm == 256 || PLANES == 2 ? 1 : 2) * cus / (gq_q_tiles * gq_n_tiles)));
     if (splits >= 8) splits = splits / 8 * 8;
     splits = std::min(splits, piece_groups);
     const uint32_t per_split = (piece_groups + splits - 1) / splits;
@@ -1169,7 +1375,12 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     const size_t o_ref = take((size_t)a.groups * a.qp * 4), o_sum = take((size_t)a.groups * a.qp * 4);
     const size_t o_cr = take((size_t)a.chunks * a.qp * 4), o_cs = take((size_t)a.chunks * a.qp * 4);
     const size_t o_lw = take((size_t)a.qp * 8), o_top = take(4), o_on = take(a.qp / 8), o_coef = take((size_t)a.qp * 4), o_total = take((size_t)a.qp * 4);
-    const size_t o_blocks = take(gq || gx ? (size_t)a.qp * piece * sizeof(T) : 0);
+    a.block_low = (size_t)a.qp * piece * 2;
+    const size_t o_blocks = take(gx ? GradTiles<T>::PLANES * a.block_low : gq ? PLANES * a.block_low : 0);
+    a.tile_r_low = PLANES == 2 ? piece * a.tile_dim * 2 : 0;
+    a.tile_q_low = PLANES == 2 ? (uint64_t)a.qp * a.tile_dim * 2 : 0;
+    const size_t o_rows = take(2 * a.tile_r_low), o_q = take(2 * a.tile_q_low), o_gq = take(gx ? 3 * a.tile_q_low : 0), o_bref = take(PLANES == 2 && gq ? (size_t)a.groups * a.qp * 4 : 0);
+    const size_t o_rexp = take((size_t)a.groups * 16), o_qexp = take(4), o_qmax = take(Q_PARTS * 4);
     const size_t o_part = take(gq && !direct ? (size_t)splits * a.qp * a.dim * 4 : 0);
     const size_t o_pr0 = take((size_t)splits * a.qp * 4), o_pr1 = take((size_t)splits * a.qp * 4);
     char* ws = nullptr;
@@ -1187,27 +1398,46 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.q_on = (uint32_t*)(ws + o_on);
     a.coef = (float*)(ws + o_coef);
     a.total = (float*)(ws + o_total);
+    a.row_exp = (float*)(ws + o_rexp);
+    a.q_exp = (float*)(ws + o_qexp);
+    a.q_max = (float*)(ws + o_qmax);
+    a.block_ref = PLANES == 2 ? (float*)(ws + o_bref) : a.ref;
+    a.tile_rows = PLANES == 2 ? ws + o_rows : (const char*)a.rows;
+    a.tile_q = PLANES == 2 ? ws + o_q : (const char*)a.q;
+    a.grad_tile_q = PLANES == 2 ? ws + o_gq : a.tile_q;
+    a.tile_r_pitch = PLANES == 2 ? a.tile_dim * 2 : a.r_pitch;
+    a.tile_q_pitch = PLANES == 2 ? a.tile_dim * 2 : a.q_pitch;
     hipStream_t s = ctx->stream;
+    if constexpr (PLANES == 2) {
+        loss_max_q<<<Q_PARTS, 256, 0, s>>>(a);
+        loss_split_q<<<a.nq, 256, 0, s>>>(a);
+    }
 
+    uint32_t split_piece = ~0u;
     auto set_piece = [&](uint32_t i) {
         a.row0 = (uint32_t)(i * piece);
         const uint32_t rows = (uint32_t)std::min<uint64_t>(piece, rows_up - a.row0);
         a.row_tiles = rows / bm;
         a.row_blocks = rows / 32;
+        if constexpr (PLANES == 2) {
+            a.tile_row0 = a.row0;
+            if (i != split_piece) loss_split_rows<<<rows / 32, 512, 0, s>>>(a); // unless the planes are of this piece already
+            split_piece = i;
+        }
         return rows / LOSS_GROUP;
     };
     auto tiles = [&](auto mode) {
         constexpr int M = decltype(mode)::value;
         const dim3 grid(a.row_tiles * a.q_tiles);
-        if constexpr (sizeof(T) == 2) {
+        if constexpr (PLANES == 2) {
+            if (form == T256) loss_tile<T, 2, 2, 4, 2, 2, M><<<grid, 512, 0, s>>>(a);
+            else if (form == T128) loss_tile<T, 1, 1, 4, 2, 3, M><<<grid, 256, 0, s>>>(a);
+            else loss_tile<T, 1, 1, 2, 2, 3, M><<<grid, 128, 0, s>>>(a);
+        } else {
             if (form == T256) loss_tile<T, 2, 2, 4, 4, 2, M><<<grid, 512, 0, s>>>(a);
             else if (form == T256_128) loss_tile<T, 1, 2, 4, 4, 3, M><<<grid, 512, 0, s>>>(a);
             else if (form == T128) loss_tile<T, 1, 1, 4, 4, 2, M><<<grid, 256, 0, s>>>(a);
             else if (form == T128_64) loss_tile<T, 1, 1, 2, 4, 3, M><<<grid, 128, 0, s>>>(a);
-            else loss_tile<T, 1, 4, 1, 4, 2, M><<<grid, 256, 0, s>>>(a);
-        } else {
-            if (form == F256_128) loss_tile<T, 2, 2, 2, 2, 3, M><<<grid, 256, 0, s>>>(a);
-            else if (form == F512_64) loss_tile<T, 2, 4, 1, 2, 2, M><<<grid, 256, 0, s>>>(a);
             else loss_tile<T, 1, 4, 1, 4, 2, M><<<grid, 256, 0, s>>>(a);
         }
     };
@@ -1216,9 +1446,9 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         const uint32_t keep = a.q_tiles;
         a.q_tiles = gq_q_tiles;
         const dim3 grid(gq_q_tiles * gq_n_tiles * splits);
-        if constexpr (sizeof(T) == 4) {
-            if (qm == 32) loss_grad_q<T, 1, 1, 1, 4, 2, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
-            else loss_grad_q<T, 2, 2, 2, 2, 2, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
+        if constexpr (PLANES == 2) {
+            if (qm == 64) loss_grad_q<T, 2, 1, 1, 4, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
+            else loss_grad_q<T, 2, 2, 2, 2, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
         } else {
             if (qm == 64) loss_grad_q<T, 2, 2, 1, 4, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
             else if (qm == 256) loss_grad_q<T, 4, 2, 2, 4, 4, E><<<grid, 512, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
@@ -1229,67 +1459,84 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     using Sums = std::integral_constant<int, TILE_SUMS>;
     using Exp = std::integral_constant<int, TILE_EXP>;
     using Grad = std::integral_constant<int, TILE_GRAD>;
-    const uint32_t join_q = a.qp / 32;
     const bool many = splits > 16; // of which one workgroup adds up a query's: with 16 waves
-    if (!two_pass) {
+    const dim3 join(a.qp / 32, chunks_per_piece);
+    auto join_piece = [&](uint32_t i, uint32_t groups, auto zero) {
+        loss_join<T, decltype(zero)::value><<<join, 256, 0, s>>>(a, a.row0 / LOSS_GROUP, groups, i * chunks_per_piece);
+    };
+    auto finish = [&](auto grad, auto exp, int turn) {
+        constexpr bool G = decltype(grad)::value, E = decltype(exp)::value;
+        if (G && many) loss_finish<T, G, E, 1024><<<a.nq, 1024, 0, s>>>(a, turn);
+        else loss_finish<T, G, E, 256><<<a.nq, 256, 0, s>>>(a, turn);
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    // One pass, for what needs no G: everything without grad x, and for float the loss and grad q beside it too.
+    const bool one_pass = !gx || PLANES == 2;
+    if (one_pass) {
         for (uint32_t i = 0; i < pieces; i++) {
             const uint32_t groups = set_piece(i);
-            if (gq) tiles(Exp{});
-            else tiles(Sums{});
-            const dim3 grid(join_q, chunks_per_piece);
-            if (gq) loss_join<T, true><<<grid, 256, 0, s>>>(a, a.row0 / LOSS_GROUP, groups, i * chunks_per_piece);
-            else loss_join<T, false><<<grid, 256, 0, s>>>(a, a.row0 / LOSS_GROUP, groups, i * chunks_per_piece);
-            if (gq) grad_q(std::true_type{}, groups, (int)(i & 1), i == 0);
-        }
-        const int turn = (int)((pieces - 1) & 1);
-        if (!gq) loss_finish<T, false, false, 256><<<a.nq, 256, 0, s>>>(a, turn);
-        else if (many) loss_finish<T, true, true, 1024><<<a.nq, 1024, 0, s>>>(a, turn);
-        else loss_finish<T, true, true, 256><<<a.nq, 256, 0, s>>>(a, turn);
-        APOE_HIP(hipGetLastError());
-        return APOE_OK;
-    }
-    const bool whole = pieces == 1 && (!gq || direct); // nothing is left to a last kernel
-    for (uint32_t i = 0; i < pieces; i++) {
-        const uint32_t groups = set_piece(i);
-        if (pieces == 1) tiles(Exp{});
-        else tiles(Sums{});
-        if (a.groups > LOSS_CHUNKS) loss_join<T, false><<<dim3(join_q, chunks_per_piece), 256, 0, s>>>(a, a.row0 / LOSS_GROUP, groups, i * chunks_per_piece);
-    }
-    if (a.groups <= LOSS_CHUNKS) { // few enough for one wave as they are
-        a.chunk_ref = a.ref;
-        a.chunk_sum = a.sum;
-        a.chunks = a.groups;
-    }
-    loss_coefs<<<a.qp, 64, 0, s>>>(a);
-    loss_queries<<<1, 1024, 0, s>>>(a);
-    // grad x: tiles of 256 rows x 256 columns, or of 128 x 128 where those do not fill the GPU (fp32: 256 x 64)
-    const bool x_wide = sizeof(T) == 2 && (uint64_t)((piece + 255) / 256) * ((a.dim + 255) / 256) >= (uint32_t)ctx->num_cus;
-    const uint32_t xm = sizeof(T) == 4 || x_wide ? 256 : 128, xn = sizeof(T) == 4 ? 64 : x_wide ? 256 : 128, x_tiles = (a.dim + xn - 1) / xn;
-    for (uint32_t i = 0; i < pieces; i++) {
-        const uint32_t groups = set_piece(i);
-        if (pieces == 1) loss_normalise<T><<<(uint32_t)(((uint64_t)groups * (a.qp / 32) + 3) / 4), 256, 0, s>>>(a, groups);
-        else tiles(Grad{});
-        if (whole) loss_targets<T, true><<<a.nq, 64, 0, s>>>(a);
-        else loss_targets<T, false><<<a.nq, 64, 0, s>>>(a);
-        if constexpr (sizeof(T) == 2) {
-            if (direct) {
-                LossArgs d = a;
-                d.q_tiles = (a.qp + 127) / 128;
-                d.splits = 1;
-                const uint32_t nt = (a.dim + 127) / 128;
-                loss_grad_q<T, 2, 2, 2, 2, 3, false, true><<<d.q_tiles * nt, 256, 0, s>>>(d, nt, groups, groups, 0, 1);
+            if (gq) {
+                tiles(Exp{});
+                join_piece(i, groups, Yes{});
+                grad_q(Yes{}, groups, (int)(i & 1), i == 0);
+            } else {
+                tiles(Sums{});
+                join_piece(i, groups, No{});
             }
         }
-        if (gq && !direct) grad_q(std::false_type{}, groups, 0, i == 0);
-        const dim3 grid((a.row_blocks * 32 + xm - 1) / xm * x_tiles);
-        if constexpr (sizeof(T) == 4) loss_grad_x<T, 4, 1, 2, 2, 2><<<grid, 256, 0, s>>>(a, x_tiles);
-        else if (x_wide) loss_grad_x<T, 4, 2, 2, 4, 4><<<grid, 512, 0, s>>>(a, x_tiles);
-        else loss_grad_x<T, 2, 2, 2, 2, 3><<<grid, 256, 0, s>>>(a, x_tiles);
+        if (gq) finish(Yes{}, Yes{}, (int)((pieces - 1) & 1));
+        else finish(No{}, No{}, 0);
+    } else {
+        for (uint32_t i = 0; i < pieces; i++) {
+            const uint32_t groups = set_piece(i);
+            if (pieces == 1) tiles(Exp{});
+            else tiles(Sums{});
+            if (a.groups > LOSS_CHUNKS) join_piece(i, groups, No{});
+        }
+        if (a.groups <= LOSS_CHUNKS) { // few enough for one wave as they are
+            a.chunk_ref = a.ref;
+            a.chunk_sum = a.sum;
+            a.chunks = a.groups;
+        }
     }
-    if (whole) {
-    } else if (!gq) loss_finish<T, false, false, 256><<<a.nq, 256, 0, s>>>(a, 0);
-    else if (many) loss_finish<T, true, false, 1024><<<a.nq, 1024, 0, s>>>(a, 0);
-    else loss_finish<T, true, false, 256><<<a.nq, 256, 0, s>>>(a, 0);
+    if (gx) {
+        loss_coefs<<<a.qp, 64, 0, s>>>(a);
+        loss_queries<<<1, 1024, 0, s>>>(a);
+        // grad x: tiles of 256 rows x 256 columns, or of 128 x 128 where those do not fill the GPU, and for float
+        const bool x_wide = PLANES == 1 && (uint64_t)((piece + 255) / 256) * ((a.dim + 255) / 256) >= cus;
+        const uint32_t xm = x_wide ? 256 : 128, x_tiles = (a.dim + xm - 1) / xm;
+        const bool whole = !one_pass && pieces == 1 && (!gq || direct); // nothing is left to a last kernel
+        for (uint32_t i = 0; i < pieces; i++) {
+            const uint32_t groups = set_piece(i);
+            if constexpr (PLANES == 1) {
+                if (pieces == 1) loss_normalise<T><<<(uint32_t)(((uint64_t)groups * (a.qp / 32) + 3) / 4), 256, 0, s>>>(a, groups);
+                else tiles(Grad{});
+            } else {
+                tiles(Grad{});
+            }
+            if (whole) loss_targets<T, true><<<a.nq, 64, 0, s>>>(a);
+            else loss_targets<T, false><<<a.nq, 64, 0, s>>>(a);
+            const dim3 grid((a.row_blocks * 32 + xm - 1) / xm * x_tiles);
+            if constexpr (PLANES == 1) {
+                if (direct) {
+                    LossArgs d = a;
+                    d.q_tiles = (a.qp + 127) / 128;
+                    d.splits = 1;
+                    const uint32_t nt = (a.dim + 127) / 128;
+                    loss_grad_q<T, 2, 2, 2, 2, 3, false, true><<<d.q_tiles * nt, 256, 0, s>>>(d, nt, groups, groups, 0, 1);
+                } else if (gq) {
+                    grad_q(No{}, groups, 0, i == 0);
+                }
+                if (x_wide) loss_grad_x<T, 4, 2, 2, 4, 4><<<grid, 512, 0, s>>>(a, x_tiles);
+            }
+            if (!x_wide) loss_grad_x<T, 2, 2, 2, 2, 3><<<grid, 256, 0, s>>>(a, x_tiles);
+        }
+        if (!one_pass && !whole) {
+            if (gq) finish(Yes{}, No{}, 0);
+            else finish(No{}, No{}, 0);
+        }
+    }
     APOE_HIP(hipGetLastError());
     return APOE_OK;
 }
