@@ -181,4 +181,26 @@ template <typename T, int COLS, int SF, int NW, int ORDER> struct ColTile {
     }
 };
 
+// Two groups of waves have summed up every other stage each (KG = 2): they exchange halves, and each has the whole sums of its half of the blocks.
+template <int MT, int NT, int WAVES> __device__ inline void exchange_halves(f32x16 (&acc)[MT][NT], char* lds, int group, int wave, int lane) {
+    static_assert(MT % 2 == 0, "halves");
+    float* buf = reinterpret_cast<float*>(lds) + lane;
+    const auto at = [&](int g, int m, int t, int k) { return (((g * WAVES + wave) * (MT / 2) + m % (MT / 2)) * NT + t) * 1024 + k * 64; };
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+        if (m / (MT / 2) != group)
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) buf[at(group, m, t, k)] = acc[m][t][k];
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+        if (m / (MT / 2) == group)
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) acc[m][t][k] += buf[at(group ^ 1, m, t, k)];
+}
+
 } // namespace apoe

@@ -642,10 +642,12 @@ template <typename T> __device__ inline i32x4 scale_down(i32x4 v, float less) {
 // grad q: a split's rows x its queries' blocks. M side: queries (blocks), N side: columns of the rows. EXP: fragments are brought
 // to the largest reference of the split, and a split's sum to the largest so far.
 // DIRECT: the only split of the only piece, whose sum is the gradient.
-template <typename T, int MT, int NT, int WM, int WN, int ST, bool EXP, bool DIRECT = false>
-__global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint32_t n_tiles, uint32_t groups_per_split, uint32_t piece_groups, int turn, int first) {
+// KG: groups of waves that take every KG-th stage, where one workgroup has a CU to itself: two waves a SIMD, each with a whole wave's
+// piece of the tile (4096 x 4096 x 1024, direct: 47 us; one group 53, the same on eight waves of half the piece 52; grad x 42, 48.6).
+template <typename T, int MT, int NT, int WM, int WN, int ST, bool EXP, bool DIRECT = false, int KG = 1>
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void loss_grad_q(LossArgs a, uint32_t n_tiles, uint32_t groups_per_split, uint32_t piece_groups, int turn, int first) {
     using S = typename Tiles<T>::S;
-    constexpr int NW = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, SF = 2, P = Tiles<T>::PLANES;
+    constexpr int NW = WM * WN * KG, BM = WM * MT * 32, BN = WN * NT * 32, SF = 2, P = Tiles<T>::PLANES;
     using BTile = ColTile<S, BN, SF, NW, ORDER_BLOCKS>;
     static_assert(BTile::KE == 32, "a block a stage");
     constexpr int ABYTES = BM / 32 * BLOCK_BYTES, AINS = ABYTES / 1024, ALOADS = (AINS + NW - 1) / NW, PLANE = ABYTES + BTile::BYTES;
@@ -654,7 +656,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
     constexpr int STAGE = P * PLANE + (EXP ? RBYTES : 0), PER = P * (ALOADS + BTile::LOADS) + (EXP ? 1 : 0);
     __shared__ __align__(1024) char lds[ST * STAGE];
     __shared__ float factor[2][BM];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / (WM * WN), wm = wave % (WM * WN) / WN, wn = wave % WN;
     const uint32_t per_split = a.q_tiles * n_tiles;
     uint32_t split = blockIdx.x / per_split, rest = blockIdx.x % per_split;
     if (a.splits % 8 == 0) { // the workgroups of one split, which read the same rows, on one XCD
@@ -662,6 +664,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
         split = (i / per_split) * 8 + (blockIdx.x & 7);
         rest = i % per_split;
     }
+    if constexpr (DIRECT) rest = xcd_run(blockIdx.x, gridDim.x); // and the column tiles of one tile of queries, which read the same blocks
     const uint32_t query = rest / n_tiles * BM, col = rest % n_tiles * BN;
     const uint32_t g0 = min(split * groups_per_split, piece_groups), g1 = min(g0 + groups_per_split, piece_groups);
     const uint32_t group0 = a.row0 / LOSS_GROUP;
@@ -719,13 +722,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
         into = into + STAGE == ST * STAGE ? 0 : into + STAGE;
     };
 #pragma unroll
-    for (int s = 0; s < ST - 1; s++) issue();
+    for (int s = 0; s < ST - KG; s++) issue();
     f32x16 acc[MT][NT] = {};
     uint32_t from = 0;
-    for (int s = 0; s < stages; s++) {
-        tile_wait<(ST - 2) * PER>();
-        issue();
-        const char* A = lds + from;
+    for (int s = 0; s < stages; s += KG) {
+        tile_wait<(ST - 2 * KG) * PER>();
+        const char* A = lds + from + kg * STAGE;
         const char* B = A + ABYTES;
         float less[MT];
         if constexpr (EXP) {
@@ -749,6 +751,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
         };
         read(0);
 #pragma unroll
+        for (int k = 0; k < KG; k++) issue();
+#pragma unroll
         for (int f = 0; f < SF; f++) {
             if (f + 1 < SF) read(f + 1);
             if constexpr (EXP) {
@@ -763,9 +767,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
                 for (int t = 0; t < NT; t++) acc[m][t] = multiply<Tiles<T>>(x[f & 1][m], y[f & 1][t], acc[m][t]);
         }
         interleave<P * (MT + 2 * NT), PRODUCTS<Tiles<T>> * MT * NT, SF>();
-        from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
+        from = from + KG * STAGE == ST * STAGE ? 0 : from + KG * STAGE;
     }
     tile_wait<0>();
+    if constexpr (KG == 2) {
+        static_assert(BM * BN * 4 <= ST * STAGE, "the sums fit the stages");
+        exchange_halves<MT, NT, WM * WN>(acc, lds, kg, wave % (WM * WN), lane);
+    }
     if constexpr (EXP) {
         if (threadIdx.x < BM) {
             const uint32_t qi = query + threadIdx.x;
@@ -781,7 +789,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
     const int h = lane >> 5;
     const float back = DIRECT ? a.scale / grad_scale_of(a.top_coef) : 1.f;
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int m = 0; m < MT; m++) {
+        if (KG == 2 && m / (MT / 2) != kg) continue;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             const int r = (wm * MT + m) * 32 + result_row(i, h);
@@ -807,18 +816,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_q(LossArgs a, uint3
                 out[d] = v;
             }
         }
+    }
 }
 
 // grad x of a piece: rows (blocks read transposed) x queries. Each row's gradient is whole here: all queries are in.
-template <typename T, int MT, int NT, int WM, int WN, int ST>
-__global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint32_t n_tiles) {
+template <typename T, int MT, int NT, int WM, int WN, int ST, int KG = 1>
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void loss_grad_x(LossArgs a, uint32_t n_tiles) {
     using S = typename GradTiles<T>::S;
-    constexpr int NW = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, SF = 2, P = GradTiles<T>::PLANES;
+    constexpr int NW = WM * WN * KG, BM = WM * MT * 32, BN = WN * NT * 32, SF = 2, P = GradTiles<T>::PLANES;
     using BTile = ColTile<S, BN, SF, NW, ORDER_ROWS>;
     constexpr int ABYTES = BM / 32 * BLOCK_BYTES, ALOADS = ABYTES / (1024 * NW), PLANE = ABYTES + BTile::BYTES;
     constexpr int STAGE = P * PLANE, PER = P * (ALOADS + BTile::LOADS);
     __shared__ __align__(1024) char lds[ST * STAGE];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / (WM * WN), wm = wave % (WM * WN) / WN, wn = wave % WN;
     uint32_t rt = blockIdx.x / n_tiles, col = blockIdx.x % n_tiles * BN;
     const uint32_t whole = gridDim.x / n_tiles / 8 * 8;
     if (blockIdx.x < whole * n_tiles) { // the column tiles of one tile of rows, which read the same blocks, on one XCD
@@ -858,13 +868,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint3
         into = into + STAGE == ST * STAGE ? 0 : into + STAGE;
     };
 #pragma unroll
-    for (int s = 0; s < ST - 1; s++) issue();
+    for (int s = 0; s < ST - KG; s++) issue();
     f32x16 acc[MT][NT] = {};
     uint32_t from = 0;
-    for (int s = 0; s < stages; s++) {
-        tile_wait<(ST - 2) * PER>();
-        issue();
-        const char* A = lds + from;
+    for (int s = 0; s < stages; s += KG) {
+        tile_wait<(ST - 2 * KG) * PER>();
+        const char* A = lds + from + kg * STAGE;
         const char* B = A + ABYTES;
         i32x4 x[2][MT][P], y[2][NT][P];
         auto read = [&](int f) {
@@ -889,6 +898,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint3
         };
         read(0);
 #pragma unroll
+        for (int k = 0; k < KG; k++) issue();
+#pragma unroll
         for (int f = 0; f < SF; f++) {
             if (f + 1 < SF) read(f + 1);
 #pragma unroll
@@ -897,13 +908,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void loss_grad_x(LossArgs a, uint3
                 for (int t = 0; t < NT; t++) acc[m][t] = multiply<GradTiles<T>>(x[f & 1][m], y[f & 1][t], acc[m][t]);
         }
         interleave<P * (2 * MT + 2 * NT), PRODUCTS<GradTiles<T>> * MT * NT, SF>();
-        from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
+        from = from + KG * STAGE == ST * STAGE ? 0 : from + KG * STAGE;
     }
     tile_wait<0>();
+    if constexpr (KG == 2) {
+        static_assert(BM * BN * 4 <= ST * STAGE, "the sums fit the stages");
+        exchange_halves<MT, NT, WM * WN>(acc, lds, kg, wave % (WM * WN), lane);
+    }
     const float back = a.scale / grad_scale_of(a.top_coef);
     const int h = lane >> 5;
 #pragma unroll
     for (int m = 0; m < MT; m++) {
+        if (KG == 2 && m / (MT / 2) != kg) continue;
         const uint32_t row = a.row0 + rt * BM + (wm * MT + m) * 32;
         const uint32_t word = live_word(a.live, row, a.n);
 #pragma unroll
@@ -1524,13 +1540,16 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
                     d.q_tiles = (a.qp + 127) / 128;
                     d.splits = 1;
                     const uint32_t nt = (a.dim + 127) / 128;
-                    loss_grad_q<T, 2, 2, 2, 2, 3, false, true><<<d.q_tiles * nt, 256, 0, s>>>(d, nt, groups, groups, 0, 1);
+                    loss_grad_q<T, 2, 2, 2, 2, 6, false, true, 2><<<d.q_tiles * nt, 512, 0, s>>>(d, nt, groups, groups, 0, 1);
                 } else if (gq) {
                     grad_q(No{}, groups, 0, i == 0);
                 }
                 if (x_wide) loss_grad_x<T, 4, 2, 2, 4, 4><<<grid, 512, 0, s>>>(a, x_tiles);
             }
-            if (!x_wide) loss_grad_x<T, 2, 2, 2, 2, 3><<<grid, 256, 0, s>>>(a, x_tiles);
+            if (!x_wide) {
+                if constexpr (PLANES == 1) loss_grad_x<T, 2, 2, 2, 2, 6, 2><<<grid, 512, 0, s>>>(a, x_tiles);
+                else loss_grad_x<T, 2, 2, 2, 2, 3><<<grid, 256, 0, s>>>(a, x_tiles);
+            }
         }
         if (!one_pass && !whole) {
             if (gq) finish(Yes{}, No{}, 0);

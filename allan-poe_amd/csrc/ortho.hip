@@ -187,11 +187,31 @@ template <bool SPLIT> __device__ inline void ortho_poly(const OrthoArgs& a, cons
     for (int k = 0; k < 8; k++) v[k] = __builtin_fmaf(a.c, v[k], a.b * ORTHO_DOWN * ((float)hi[k] + (float)lo[k]));
 }
 
+// Eight values from rows that are multiples of 16 bytes.
+__device__ inline void load8(const void* p, uint64_t at, uint32_t dtype, float* v) {
+    if (dtype == APOE_F32) {
+        const f32x4 x0 = *reinterpret_cast<const f32x4*>((const float*)p + at), x1 = *reinterpret_cast<const f32x4*>((const float*)p + at + 4);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = k < 4 ? x0[k] : x1[k - 4];
+    } else if (dtype == APOE_F16) {
+        const f16x8 x = *reinterpret_cast<const f16x8*>((const _Float16*)p + at);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = (float)x[k];
+    } else {
+        const bf16x8 x = *reinterpret_cast<const bf16x8*>((const __bf16*)p + at);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = (float)x[k];
+    }
+}
+
 // Eight values into `out`, whose rows are multiples of 16 bytes (and of eight values).
 __device__ inline void add_row8(const OrthoArgs& a, uint64_t at, float* v) {
-    if (a.beta != 0.f)
+    if (a.beta != 0.f) {
+        float old[8];
+        load8(a.out, at, a.out_dtype, old);
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = __builtin_fmaf(a.beta, load_as_float(a.out, at + k, a.out_dtype), v[k]);
+        for (int k = 0; k < 8; k++) v[k] = __builtin_fmaf(a.beta, old[k], v[k]);
+    }
     if (a.out_dtype == APOE_F32) {
         *reinterpret_cast<f32x4*>((float*)a.out + at) = f32x4{v[0], v[1], v[2], v[3]};
         *reinterpret_cast<f32x4*>((float*)a.out + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
@@ -211,18 +231,18 @@ __device__ inline void add_row8(const OrthoArgs& a, uint64_t at, float* v) {
 enum { ORTHO_GRAM = 0, ORTHO_POLY = 1, ORTHO_STEP = 2, ORTHO_LAST = 3 };
 
 // One product of a step. GRAM: A = X X^T; POLY: B = b A + c A A, whose diagonal goes to `diag`; both symmetric, so the tiles on and
-// below the diagonal are computed and written twice. STEP: X = (a + diag) X + B X; LAST: the same into `out`.
-template <bool SPLIT, int MT, int NT, int WM, int WN, int SF, int ST, int KIND>
-__global__ __launch_bounds__(64 * WM * WN, 2) void ortho_tile(OrthoArgs a) {
+// below the diagonal are computed and written twice. KG groups of waves share a stage's inner indices. STEP: X = (a + diag) X + B X; LAST: the same into `out`.
+template <bool SPLIT, int MT, int NT, int WM, int WN, int KG, int SF, int ST, int KIND>
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void ortho_tile(OrthoArgs a) {
     using T = _Float16;
-    constexpr int NW = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, PLANES = SPLIT ? 2 : 1;
+    constexpr int NW = WM * WN * KG, FS = SF / KG, BM = WM * MT * 32, BN = WN * NT * 32, PLANES = SPLIT ? 2 : 1;
     constexpr bool SYM = KIND == ORTHO_GRAM || KIND == ORTHO_POLY;
     using ATile = RowTile<T, BM, SF, NW>;
     using BTile = std::conditional_t<SYM, RowTile<T, BN, SF, NW>, ColTile<T, BN, SF, NW, ORDER_ROWS>>;
     static_assert(!SYM || BM == BN, "square tiles");
     constexpr int PLANE = ATile::BYTES + BTile::BYTES, STAGE = PLANES * PLANE, PER = PLANES * (ATile::LOADS + BTile::LOADS), KE = ATile::KE;
     __shared__ __align__(1024) char lds[ST * STAGE];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / (WM * WN), wm = wave % (WM * WN) / WN, wn = wave % WN;
     const uint32_t id = xcd_run(blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y), tile = id % gridDim.x, batch = id / gridDim.x;
     uint32_t ti, tj;
     if constexpr (SYM) {
@@ -289,7 +309,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ortho_tile(OrthoArgs a) {
     uint32_t from = 0;
     for (int s = 0; s < stages; s++) {
         tile_wait<(ST - 2) * PER>();
-        issue();
         const char* A = lds + from;
         const char* B = A + ATile::BYTES;
         i32x4 x[2][PLANES][MT], y[2][PLANES][NT];
@@ -297,15 +316,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ortho_tile(OrthoArgs a) {
 #pragma unroll
             for (int p = 0; p < PLANES; p++) {
 #pragma unroll
-                for (int m = 0; m < MT; m++) x[f & 1][p][m] = ATile::read(A + p * PLANE, wm * MT + m, f, lane);
+                for (int m = 0; m < MT; m++) x[f & 1][p][m] = ATile::read(A + p * PLANE, wm * MT + m, kg * FS + f, lane);
 #pragma unroll
-                for (int t = 0; t < NT; t++) y[f & 1][p][t] = BTile::read(B + p * PLANE, wn * NT + t, f, lane);
+                for (int t = 0; t < NT; t++) y[f & 1][p][t] = BTile::read(B + p * PLANE, wn * NT + t, kg * FS + f, lane);
             }
         };
         read(0);
+        issue();
 #pragma unroll
-        for (int f = 0; f < SF; f++) {
-            if (f + 1 < SF) read(f + 1);
+        for (int f = 0; f < FS; f++) {
+            if (f + 1 < FS) read(f + 1);
 #pragma unroll
             for (int m = 0; m < MT; m++)
 #pragma unroll
@@ -317,10 +337,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ortho_tile(OrthoArgs a) {
                     acc[m][t] = mfma_step<T>(x[f & 1][0][m], y[f & 1][0][t], acc[m][t]);
                 }
         }
-        interleave<PLANES * (MT + (SYM ? 1 : 2) * NT), (SPLIT ? 3 : 1) * MT * NT, SF>();
+        interleave<PLANES * (MT + (SYM ? 1 : 2) * NT), (SPLIT ? 3 : 1) * MT * NT, FS>();
         from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
     }
     tile_wait<0>();
+    if constexpr (KG == 2) {
+        static_assert(BM * BN * 4 <= ST * STAGE, "the sums fit the stages");
+        exchange_halves<MT, NT, WM * WN>(acc, lds, kg, wave % (WM * WN), lane);
+        __syncthreads();
+    }
     // 64 rows at a time through LDS: then a thread has eight values of a row, of the tile and of the mirrored one
     constexpr int PITCH = BN + 1, ITEMS = 64 * BN / 8 / (64 * NW), OWN = 64 / 32; // OWN: blocks of 32 rows of a wave in a chunk
     static_assert(64 * PITCH * 4 <= ST * STAGE && MT % OWN == 0, "the sum fits the stages");
@@ -332,15 +357,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void ortho_tile(OrthoArgs a) {
         if (crow >= a.m) break;
         if (wm == chunk / (MT / OWN)) {
 #pragma unroll
-            for (int o = 0; o < OWN; o++)
+            for (int o = 0; o < OWN; o++) {
+                if (KG == 2 && (chunk % (MT / OWN) * OWN + o) / (MT / 2) != kg) continue;
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int k = 0; k < 16; k++)
                         sum[(o * 32 + result_row(k, half)) * PITCH + (wn * NT + t) * 32 + (lane & 31)] = acc[chunk % (MT / OWN) * OWN + o][t][k] * (ORTHO_DOWN * ORTHO_DOWN);
+            }
         }
         __syncthreads();
-#pragma unroll
+#pragma unroll(KIND == ORTHO_LAST && MT > 2 ? 1 : ITEMS) // the last kind's three ways out would not fit beside the largest sums
         for (int item = 0; item < ITEMS; item++) {
             const uint32_t at = item * 64 * NW + threadIdx.x;
             if constexpr (SYM || KIND == ORTHO_STEP) {
@@ -664,30 +691,43 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
     } else {
         ortho_first<SPLIT><<<dim3(a.np / 64, (a.m + 63) / 64, batch), 256, 0, s>>>(a);
     }
-    // Tiles, by how many there are for the CUs (times of one product, 256 CUs, fp16):
-    //  256: symmetric products from half as many tiles as CUs on (4096 x 4096: X X^T 96 us; 128: 107)
-    //  128: from as many tiles as CUs on; for X X^T from half as many, where the rows are long (4 x 1024 x 4096: 40 us; 64: 53)
+    // Tiles, by how many there are for the CUs (times of one product or of the whole, 256 CUs, fp16):
+    //  symmetric products from half as many tiles of 256 as CUs on: 256, or 192 on twelve waves where the rounds over the CUs times a
+    //    tile's size (and a seventh, which the smaller one is slower by) are less (4096 x 4096: 253 tiles of 192 for 136 of 256, X X^T 84 us
+    //    for 106, the whole 1.53 ms for 1.80; 4608: 300 for 171, 2.86 ms for 2.62)
+    //  128: from as many tiles as CUs on; for X X^T from half as many, where the rows are long (4 x 1024 x 4096: 40 us; 64: 53), there
+    //    with the waves in two groups that take half of a stage each: larger pieces a wave, fewer reads (45 us in the run of the whole, 51)
     //  64: below (1024 x 1024: X X^T 9 us; 128: 12)
+    //  B X: 256 where those fill the GPU and the inner side is long enough to hide the end of a tile, whose traffic the next one does not
+    //    overlap (the whole: 4096 x 8192 2.62 ms for 2.98, 8192 x 8192 11.0 for 12.4; 4 x 1024 x 4096 0.575 for 0.541), 128, 64
     const uint32_t cus = (uint32_t)ctx->num_cus;
     auto tiles = [](uint32_t side, uint32_t t) { return (side + t - 1) / t; };
     auto triangle = [](uint32_t t) { return t * (t + 1) / 2; };
-    const uint64_t s256 = (uint64_t)triangle(tiles(a.m, 256)) * batch, s128 = (uint64_t)triangle(tiles(a.m, 128)) * batch, x128 = (uint64_t)tiles(a.m, 128) * tiles(a.n, 128) * batch;
+    const uint64_t s256 = (uint64_t)triangle(tiles(a.m, 256)) * batch, s192 = (uint64_t)triangle(tiles(a.m, 192)) * batch, s128 = (uint64_t)triangle(tiles(a.m, 128)) * batch, x256 = (uint64_t)tiles(a.m, 256) * tiles(a.n, 256) * batch, x128 = (uint64_t)tiles(a.m, 128) * tiles(a.n, 128) * batch;
+    auto rounds = [&](uint64_t t) { return (t + cus - 1) / cus; };
     auto sym = [&](auto kind) {
         constexpr int K = decltype(kind)::value;
         const uint32_t inner = K == ORTHO_GRAM ? a.n : a.m;
         if constexpr (!SPLIT) {
             if (s256 >= cus / 2) {
-                ortho_tile<SPLIT, 4, 2, 2, 4, 4, 2, K><<<dim3(triangle(tiles(a.m, 256)), batch), 512, 0, s>>>(a);
+                if (rounds(s192) * 36864 * 23 / 20 < rounds(s256) * 65536) ortho_tile<SPLIT, 2, 3, 3, 2, 2, 4, 3, K><<<dim3(triangle(tiles(a.m, 192)), batch), 768, 0, s>>>(a);
+                else ortho_tile<SPLIT, 4, 2, 2, 4, 1, 4, 2, K><<<dim3(triangle(tiles(a.m, 256)), batch), 512, 0, s>>>(a);
                 return;
             }
         }
-        if (s128 < cus && s128 >= cus / 2 && inner >= 4096) ortho_tile<SPLIT, 2, 1, 2, 4, SPLIT ? 2 : 4, 4, K><<<dim3(triangle(tiles(a.m, 128)), batch), 512, 0, s>>>(a);
-        else if (s128 >= cus) ortho_tile<SPLIT, 2, 1, 2, 4, 4, 2, K><<<dim3(triangle(tiles(a.m, 128)), batch), 512, 0, s>>>(a);
+        if (s128 < cus && s128 >= cus / 2 && inner >= 4096) ortho_tile<SPLIT, 2, 2, 2, 2, 2, SPLIT ? 2 : 4, 4, K><<<dim3(triangle(tiles(a.m, 128)), batch), 512, 0, s>>>(a);
+        else if (s128 >= cus) ortho_tile<SPLIT, 2, 1, 2, 4, 1, 4, 2, K><<<dim3(triangle(tiles(a.m, 128)), batch), 512, 0, s>>>(a);
         else ortho_small<SPLIT, K><<<dim3(triangle(tiles(a.m, 64)), batch), 512, 0, s>>>(a);
     };
     auto step = [&](auto kind) {
         constexpr int K = decltype(kind)::value;
-        if (x128 >= cus) ortho_tile<SPLIT, 2, 1, 2, 4, 4, 2, K><<<dim3(tiles(a.m, 128) * tiles(a.n, 128), batch), 512, 0, s>>>(a);
+        if constexpr (!SPLIT) {
+            if (x256 >= cus * 4 / 5 && a.m >= 2048) {
+                ortho_tile<SPLIT, 4, 2, 2, 4, 1, 4, 2, K><<<dim3(tiles(a.m, 256) * tiles(a.n, 256), batch), 512, 0, s>>>(a);
+                return;
+            }
+        }
+        if (x128 >= cus) ortho_tile<SPLIT, 2, 1, 2, 4, 1, 4, 2, K><<<dim3(tiles(a.m, 128) * tiles(a.n, 128), batch), 512, 0, s>>>(a);
         else ortho_small<SPLIT, K><<<dim3(tiles(a.m, 64) * tiles(a.n, 64), batch), 512, 0, s>>>(a);
     };
     for (uint32_t i = 0; i < p->steps; i++) {

@@ -74,6 +74,17 @@ def test_tiles_of_the_large_form(gpu_ctx):
             assert error(got[i], reference(x[i])) < limit("bfloat16", "f16")
 
 
+@pytest.mark.parametrize("batch,rows,cols", [(130, 130, 136), (130, 136, 100), (129, 193, 200), (128, 200, 260), (1, 2048, 7000), (14, 300, 4100)])
+def test_tiles_by_the_rounds_they_take(gpu_ctx, batch, rows, cols):
+    """Batches whose symmetric products take tiles of 192 or of 256, an inner side long enough for 256 in the last product, and long rows
+    on tiles of 128."""
+    import apoe
+    x = matrix(rows, cols, "float32", 4, batch=batch, pad=1)
+    got = apoe.orthogonalize(gpu_ctx, x, products="f16")
+    for i in {0, batch // 2, batch - 1}:
+        assert error(got[i], reference(x[i])) < limit("float32", "f16")
+
+
 def test_a_low_floor_keeps_its_directions(gpu_ctx):
     """Strong directions 250 times over the floor: an iterate in 16 bits would lose the floor in their rounding (1 % and more)."""
     import apoe
