@@ -5,12 +5,14 @@
 // raise the floor by up to a^steps (485 for the usual five). Rounding X itself to 16 bits plants noise of the strong directions'
 // size in the floor, which is raised with it (fp16: 1.6 % of the result at 1024 x 1024, bf16: 13 %). Rounding A and B = b A + c A A
 // does not: they multiply X, so their errors are relative to what they multiply, and B is near zero on the floor. So X is kept
-// in 32 bits and the products take fp16 copies of X, A and B (times 2^12: X and A are about one at most, their small values stay
-// clear of the subnormal numbers); B's diagonal, which is its largest part when all singular values are alike, stays in 32
-// bits and scales X's rows outside the product. That leaves 1e-4 to 6e-4 (fp16 rounds its result by 2e-4, bf16 by 17e-4), less the
-// longer the sides are, over which the roundings average.
-// SPLIT, for results in 32 bits, for fp16 ones and for short sides, where nothing averages: every operand is two fp16 matrices, its
-// rounded value and what that left (22 bits together), and a product is three: high x high, high x low, low x high.
+// as two fp16 matrices, its rounded value and what that left (22 bits together; kept in fp32 beside an fp16 copy, the errors below are
+// the same in two digits, and the traffic of B X half as much again: 4 x 1024 x 4096 625 us for 595), and the products take fp16
+// copies of X (the high part), A and B, all times 2^12: X and A are about one at most, their small values stay clear of the subnormal
+// numbers; B's diagonal, which is its largest part when all singular values are alike, stays in 32 bits and scales X's rows outside
+// the product. That leaves 1e-4 to 6e-4 (fp16 rounds its result by 2e-4, bf16 by 17e-4), less the longer the sides are, over which
+// the roundings average.
+// SPLIT, for results in 32 bits, for fp16 ones and (ortho_narrow) for short sides, where nothing averages: X in fp32, every operand two fp16 matrices,
+// and a product is three: high x high, high x low, low x high.
 #include <type_traits>
 
 #include "apoe_internal.h"
@@ -29,21 +31,23 @@ struct OrthoArgs {
     bool tall, whole_out; // worked on transposed; rows of `out` are multiples of 16 bytes
     float a, b, c, alpha, beta;
     double* part;  // [batch][ORTHO_PARTS]
-    float* x;      // [batch][m][np] the iterate
-    _Float16 *h, *h2;      // [batch][m][np] operand of the products, now and next; SPLIT: the low parts lie h_low values behind
+    float* x;      // [batch][m][np] the iterate, SPLIT only
+    _Float16 *h, *h2;      // [batch][m][np] the iterate, now and next: high parts, operand of the products; the low parts lie h_low values behind
     _Float16 *gram, *poly; // [batch][m][mp]; SPLIT: g_low values behind
     uint64_t h_low, g_low;
     float* diag;   // [batch][mp]
+    float* cut;    // [batch][tiles][cuts][64 x 64]: X X^T of parts of the inner side
+    uint32_t cuts, cut_stages; // 1: none
 };
 
 constexpr float ORTHO_UP = 4096.f, ORTHO_DOWN = 1.f / 4096.f; // of the fp16 copies
 
 // v times 2^12 as fp16, and what that leaves.
-template <bool SPLIT> __device__ inline void put(_Float16* at, uint64_t low, float v) {
+__device__ inline void put(_Float16* at, uint64_t low, float v) {
     v *= ORTHO_UP;
     const _Float16 hi = (_Float16)v;
     *at = hi;
-    if constexpr (SPLIT) at[low] = (_Float16)(v - (float)hi);
+    at[low] = (_Float16)(v - (float)hi);
 }
 
 __device__ inline float load_as_float(const void* p, uint64_t i, uint32_t dtype) {
@@ -135,10 +139,12 @@ template <bool SPLIT> __global__ __launch_bounds__(256) void ortho_first_whole(O
             hi[k] = (_Float16)(v[k] * ORTHO_UP);
             lo[k] = (_Float16)(v[k] * ORTHO_UP - (float)hi[k]);
         }
-        *reinterpret_cast<f32x4*>(a.x + at) = f32x4{v[0], v[1], v[2], v[3]};
-        *reinterpret_cast<f32x4*>(a.x + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        if constexpr (SPLIT) {
+            *reinterpret_cast<f32x4*>(a.x + at) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4*>(a.x + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        }
         *reinterpret_cast<f16x8*>(a.h + at) = hi;
-        if constexpr (SPLIT) *reinterpret_cast<f16x8*>(a.h + a.h_low + at) = lo;
+        *reinterpret_cast<f16x8*>(a.h + a.h_low + at) = lo;
     }
 }
 
@@ -162,8 +168,8 @@ template <bool SPLIT> __global__ __launch_bounds__(256) void ortho_first(OrthoAr
         if (j < a.n) v = a.tall ? tile[r][tx] : load_as_float(a.in, in0 + (uint64_t)i * a.in_stride + j, a.in_dtype);
         v = (float)(v * inv);
         const uint64_t at = ((uint64_t)blockIdx.z * a.m + i) * a.np + j;
-        a.x[at] = v;
-        put<SPLIT>(a.h + at, a.h_low, v);
+        if constexpr (SPLIT) a.x[at] = v;
+        put(a.h + at, a.h_low, v);
     }
 }
 
@@ -176,6 +182,35 @@ template <bool SPLIT> __device__ inline void put8(_Float16* at, uint64_t low, co
     }
     *reinterpret_cast<f16x8*>(at) = hi;
     if constexpr (SPLIT) *reinterpret_cast<f16x8*>(at + low) = lo;
+}
+
+// Eight values of the iterate, as they come (two times f32x4, or high and low parts), and as numbers.
+template <bool SPLIT> struct Iterate8 {
+    f32x4 x0 = {}, x1 = {};
+    __device__ void load(const OrthoArgs& a, uint64_t at) {
+        x0 = *reinterpret_cast<const f32x4*>(a.x + at);
+        x1 = *reinterpret_cast<const f32x4*>(a.x + at + 4);
+    }
+    __device__ float operator[](int k) const { return k < 4 ? x0[k] : x1[k - 4]; }
+};
+template <> struct Iterate8<false> {
+    f16x8 hi = {}, lo = {};
+    __device__ void load(const OrthoArgs& a, uint64_t at) {
+        hi = *reinterpret_cast<const f16x8*>(a.h + at);
+        lo = *reinterpret_cast<const f16x8*>(a.h + a.h_low + at);
+    }
+    __device__ float operator[](int k) const { return ((float)hi[k] + (float)lo[k]) * ORTHO_DOWN; }
+};
+template <bool SPLIT> __device__ inline float iterate1(const OrthoArgs& a, uint64_t at) {
+    if constexpr (SPLIT) return a.x[at];
+    else return ((float)a.h[at] + (float)a.h[a.h_low + at]) * ORTHO_DOWN;
+}
+template <bool SPLIT> __device__ inline void put_iterate8(const OrthoArgs& a, uint64_t at, const float* v) {
+    if constexpr (SPLIT) {
+        *reinterpret_cast<f32x4*>(a.x + at) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(a.x + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    }
+    put8<true>(a.h2 + at, a.h_low, v);
 }
 
 // v = b A + c v, for eight values of A at `gram`.
@@ -228,6 +263,16 @@ __device__ inline void add_row8(const OrthoArgs& a, uint64_t at, float* v) {
     }
 }
 
+// The tiles on and below the diagonal, row by row.
+__device__ inline void tile_of(uint32_t tile, uint32_t& ti, uint32_t& tj) {
+    ti = (uint32_t)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
+    while (ti * (ti + 1) / 2 > tile) ti--;
+    while ((ti + 1) * (ti + 2) / 2 <= tile) ti++;
+    tj = tile - ti * (ti + 1) / 2;
+    ti = __builtin_amdgcn_readfirstlane(ti);
+    tj = __builtin_amdgcn_readfirstlane(tj);
+}
+
 enum { ORTHO_GRAM = 0, ORTHO_POLY = 1, ORTHO_STEP = 2, ORTHO_LAST = 3 };
 
 // One product of a step. GRAM: A = X X^T; POLY: B = b A + c A A, whose diagonal goes to `diag`; both symmetric, so the tiles on and
@@ -246,12 +291,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void ortho_tile(OrthoArgs a) 
     const uint32_t id = xcd_run(blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y), tile = id % gridDim.x, batch = id / gridDim.x;
     uint32_t ti, tj;
     if constexpr (SYM) {
-        ti = (uint32_t)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
-        while (ti * (ti + 1) / 2 > tile) ti--;
-        while ((ti + 1) * (ti + 2) / 2 <= tile) ti++;
-        tj = tile - ti * (ti + 1) / 2;
-        ti = __builtin_amdgcn_readfirstlane(ti);
-        tj = __builtin_amdgcn_readfirstlane(tj);
+        tile_of(tile, ti, tj);
     } else {
         const uint32_t nt = (a.n + BN - 1) / BN;
         ti = tile / nt;
@@ -390,12 +430,11 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void ortho_tile(OrthoArgs a) 
                     } else {
                         const uint64_t o = xo + (uint64_t)i * a.np + j;
                         const float d = a.a + a.diag[(uint64_t)batch * a.mp + i];
-                        const f32x4 x0 = *reinterpret_cast<const f32x4*>(a.x + o), x1 = *reinterpret_cast<const f32x4*>(a.x + o + 4);
+                        Iterate8<SPLIT> x;
+                        x.load(a, o);
 #pragma unroll
-                        for (int k = 0; k < 8; k++) v[k] = __builtin_fmaf(d, k < 4 ? x0[k] : x1[k - 4], v[k]);
-                        *reinterpret_cast<f32x4*>(a.x + o) = f32x4{v[0], v[1], v[2], v[3]};
-                        *reinterpret_cast<f32x4*>(a.x + o + 4) = f32x4{v[4], v[5], v[6], v[7]};
-                        put8<SPLIT>(a.h2 + o, a.h_low, v);
+                        for (int k = 0; k < 8; k++) v[k] = __builtin_fmaf(d, x[k], v[k]);
+                        put_iterate8<SPLIT>(a, o, v);
                     }
                 }
                 if constexpr (SYM) {
@@ -413,10 +452,11 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void ortho_tile(OrthoArgs a) 
                 if (i < a.m && j < a.n) {
                     const uint64_t o = xo + (uint64_t)i * a.np + j, to = batch * a.out_batch + (uint64_t)i * a.out_stride + j;
                     const float d = a.a + a.diag[(uint64_t)batch * a.mp + i];
-                    const f32x4 x0 = *reinterpret_cast<const f32x4*>(a.x + o), x1 = *reinterpret_cast<const f32x4*>(a.x + o + 4);
+                    Iterate8<SPLIT> x;
+                    x.load(a, o);
                     float v[8];
 #pragma unroll
-                    for (int k = 0; k < 8; k++) v[k] = a.alpha * __builtin_fmaf(d, k < 4 ? x0[k] : x1[k - 4], sum[r * PITCH + c + k]);
+                    for (int k = 0; k < 8; k++) v[k] = a.alpha * __builtin_fmaf(d, x[k], sum[r * PITCH + c + k]);
                     add_row8(a, to, v);
                 }
             } else {
@@ -427,7 +467,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void ortho_tile(OrthoArgs a) 
                     const uint32_t r = a.tall ? e % 64 : e / BN, c = a.tall ? e / 64 : e % BN, i = crow + r, j = col + c;
                     if (i >= a.m || j >= a.n) continue;
                     const uint64_t o = batch * a.out_batch + (a.tall ? (uint64_t)j * a.out_stride + i : (uint64_t)i * a.out_stride + j);
-                    float v = a.alpha * __builtin_fmaf(a.a + a.diag[(uint64_t)batch * a.mp + i], a.x[xo + (uint64_t)i * a.np + j], sum[r * PITCH + c]);
+                    float v = a.alpha * __builtin_fmaf(a.a + a.diag[(uint64_t)batch * a.mp + i], iterate1<SPLIT>(a, xo + (uint64_t)i * a.np + j), sum[r * PITCH + c]);
                     if (a.beta != 0.f) v = __builtin_fmaf(a.beta, load_as_float(a.out, o, a.out_dtype), v);
                     store_from_float(a.out, o, a.out_dtype, v);
                 }
@@ -450,15 +490,10 @@ template <bool SPLIT, int KIND> __global__ __launch_bounds__(512, 2) void ortho_
     static_assert(B * PITCH * 4 <= ST * STAGE, "the sum fits the stages");
     __shared__ __align__(1024) char lds[ST * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = wave >> 2, wm = (wave >> 1) & 1, wn = wave & 1;
-    const uint32_t tile = blockIdx.x, batch = blockIdx.y;
+    const uint32_t batch = blockIdx.y, tile = KIND == ORTHO_GRAM ? blockIdx.x / a.cuts : blockIdx.x, cut = KIND == ORTHO_GRAM ? blockIdx.x % a.cuts : 0;
     uint32_t ti, tj;
     if constexpr (SYM) {
-        ti = (uint32_t)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
-        while (ti * (ti + 1) / 2 > tile) ti--;
-        while ((ti + 1) * (ti + 2) / 2 <= tile) ti++;
-        tj = tile - ti * (ti + 1) / 2;
-        ti = __builtin_amdgcn_readfirstlane(ti);
-        tj = __builtin_amdgcn_readfirstlane(tj);
+        tile_of(tile, ti, tj);
     } else {
         const uint32_t nt = (a.n + B - 1) / B;
         ti = tile / nt;
@@ -477,8 +512,8 @@ template <bool SPLIT, int KIND> __global__ __launch_bounds__(512, 2) void ortho_
     for (int p = 0; p < PLANES; p++) {
         const uint64_t hl = p * a.h_low, gl = p * a.g_low;
         if constexpr (KIND == ORTHO_GRAM) {
-            ta[p].init(h + hl + (uint64_t)row * a.np, xp, mrows, wave, lane);
-            tb[p].init(h + hl + (uint64_t)col * a.np, xp, (int)min((uint32_t)B, a.m - col), wave, lane);
+            ta[p].init(h + hl + (uint64_t)row * a.np + cut * a.cut_stages * KE, xp, mrows, wave, lane);
+            tb[p].init(h + hl + (uint64_t)col * a.np + cut * a.cut_stages * KE, xp, (int)min((uint32_t)B, a.m - col), wave, lane);
         } else if constexpr (KIND == ORTHO_POLY) {
             ta[p].init(gram + gl + (uint64_t)row * a.mp, gp, mrows, wave, lane);
             tb[p].init(gram + gl + (uint64_t)col * a.mp, gp, (int)min((uint32_t)B, a.m - col), wave, lane);
@@ -491,7 +526,7 @@ template <bool SPLIT, int KIND> __global__ __launch_bounds__(512, 2) void ortho_
     const uint32_t er = threadIdx.x >> 3, ec = (threadIdx.x & 7) * 8, i = row + er, j = col + ec;
     const uint32_t mi = row + ec, mj = col + er; // of the mirrored tile
     f16x8 own = {}, own_low = {}, mir = {}, mir_low = {};
-    f32x4 x0 = {}, x1 = {};
+    Iterate8<SPLIT> x_own;
     float diag = 0.f, xl[8] = {}, dl[8] = {};
     const bool turned = KIND == ORTHO_LAST && a.tall;
     const uint32_t lc = threadIdx.x & 63, lr = threadIdx.x >> 6; // LAST: lc along the row of `out`
@@ -507,8 +542,7 @@ template <bool SPLIT, int KIND> __global__ __launch_bounds__(512, 2) void ortho_
     } else if constexpr (KIND == ORTHO_STEP) {
         if (i < a.m) {
             diag = a.diag[(uint64_t)batch * a.mp + i];
-            x0 = *reinterpret_cast<const f32x4*>(a.x + xo + (uint64_t)i * a.np + j);
-            x1 = *reinterpret_cast<const f32x4*>(a.x + xo + (uint64_t)i * a.np + j + 4);
+            x_own.load(a, xo + (uint64_t)i * a.np + j);
         }
     } else if constexpr (KIND == ORTHO_LAST) {
 #pragma unroll
@@ -516,14 +550,14 @@ template <bool SPLIT, int KIND> __global__ __launch_bounds__(512, 2) void ortho_
             const uint32_t r = row + (turned ? lc : lr + 8 * k), c = col + (turned ? lr + 8 * k : lc);
             if (r < a.m) {
                 dl[k] = a.diag[(uint64_t)batch * a.mp + r];
-                xl[k] = a.x[xo + (uint64_t)r * a.np + c];
+                xl[k] = iterate1<SPLIT>(a, xo + (uint64_t)r * a.np + c);
             }
         }
     }
     const int inner = (int)(KIND == ORTHO_GRAM ? a.np : a.mp);
-    const int stages = (inner + KE - 1) / KE;
+    const int all = (inner + KE - 1) / KE, stage0 = (int)(cut * a.cut_stages), stages = KIND == ORTHO_GRAM ? min(all - stage0, (int)a.cut_stages) : all;
     const uint32_t base = lds_address(lds);
-    int left = inner;
+    int left = min(inner - stage0 * KE, stages * KE); // of this part
     uint32_t into = 0;
     auto issue = [&]() {
 #pragma unroll
@@ -585,6 +619,17 @@ template <bool SPLIT, int KIND> __global__ __launch_bounds__(512, 2) void ortho_
         }
         __syncthreads();
     }
+    if constexpr (KIND == ORTHO_GRAM) {
+        if (a.cuts > 1) {
+            float* to = a.cut + (((uint64_t)batch * gridDim.x + blockIdx.x) * B + er) * B + ec;
+            f32x4 v[2];
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k >> 2][k & 3] = sum[er * PITCH + ec + k];
+            *reinterpret_cast<f32x4*>(to) = v[0];
+            *reinterpret_cast<f32x4*>(to + 4) = v[1];
+            return;
+        }
+    }
     if constexpr (SYM) {
         T* to = (KIND == ORTHO_GRAM ? a.gram : a.poly) + go;
         if (i < a.m) {
@@ -616,11 +661,8 @@ template <bool SPLIT, int KIND> __global__ __launch_bounds__(512, 2) void ortho_
             float v[8];
             const float d = a.a + diag;
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = __builtin_fmaf(d, k < 4 ? x0[k] : x1[k - 4], sum[er * PITCH + ec + k]);
-            const uint64_t at = xo + (uint64_t)i * a.np + j;
-            *reinterpret_cast<f32x4*>(a.x + at) = f32x4{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<f32x4*>(a.x + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
-            put8<SPLIT>(a.h2 + at, a.h_low, v);
+            for (int k = 0; k < 8; k++) v[k] = __builtin_fmaf(d, x_own[k], sum[er * PITCH + ec + k]);
+            put_iterate8<SPLIT>(a, xo + (uint64_t)i * a.np + j, v);
         }
     } else {
 #pragma unroll
@@ -635,7 +677,314 @@ template <bool SPLIT, int KIND> __global__ __launch_bounds__(512, 2) void ortho_
     }
 }
 
-template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonalize_args* p) {
+// A from the parts that its inner side was cut into: grid (tiles, batch).
+template <bool SPLIT> __global__ __launch_bounds__(512) void ortho_join(OrthoArgs a) {
+    constexpr int B = 64, PITCH = 65;
+    __shared__ float sum[B * PITCH];
+    uint32_t ti, tj;
+    tile_of(blockIdx.x, ti, tj);
+    const uint32_t er = threadIdx.x >> 3, ec = (threadIdx.x & 7) * 8, row = ti * B, col = tj * B, i = row + er, mi = row + ec, mj = col + er;
+    const float* from = a.cut + (((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.cuts * B + er) * B + ec;
+    f32x4 lo = {}, hi = {};
+#pragma unroll 4
+    for (uint32_t c = 0; c < a.cuts; c++) {
+        lo += *reinterpret_cast<const f32x4*>(from + (uint64_t)c * B * B);
+        hi += *reinterpret_cast<const f32x4*>(from + (uint64_t)c * B * B + 4);
+    }
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) sum[er * PITCH + ec + k] = v[k] = k < 4 ? lo[k] : hi[k - 4];
+    _Float16* to = a.gram + (uint64_t)blockIdx.y * a.m * a.mp;
+    if (i < a.m) put8<SPLIT>(to + (uint64_t)i * a.mp + col + ec, a.g_low, v);
+    __syncthreads();
+    if (ti != tj && mj < a.m) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = sum[(ec + k) * PITCH + er];
+        put8<SPLIT>(to + (uint64_t)mj * a.mp + mi, a.g_low, v);
+    }
+}
+
+// ---- a side of at most 64 ----
+// All of A fits a workgroup, so a step needs no kernel of its own for A and B: a workgroup has 256 columns of X in registers (a wave 32,
+// as a 32x32 result lies in its lanes, which is a fragment of the next product too), every workgroup forms the same A from the sums of
+// all of them, and B from it, then its columns of (a + diag) X + B X and what they add to the next A. 256 columns and less are one
+// workgroup and one launch; otherwise a launch a step, X and the sums in memory between them.
+// What it costs is launches and waiting, about 3.5 us a step where one workgroup has everything, 8 us a launch otherwise (five steps, by the
+// kernels above and by these: 64 x 64 68 and 27 us, 64 x 1024 95 and 55, 64 x 4096 200 and 70, 64 x 65 536 2.27 and 0.14 ms, 512 of 16 x 64
+// 121 and 53 us). More than NARROW_PARTS sums of 64 x 64 are joined by a launch of their own, fewer by each workgroup (64 x 4096, sixteen: 73 us).
+constexpr uint32_t NARROW = 64, NARROW_COLS = 256, NARROW_PARTS = 8;
+
+struct NarrowArgs {
+    float* x;       // [batch][slabs][8 waves][32 values][64 lanes]
+    float* sums[2]; // [batch][slabs][64 x 64], of the launch before and of this one
+    float* joined;  // [batch][64 x 64]: those of the launch before added up, where there are more than NARROW_PARTS
+    uint32_t slabs, steps;
+};
+
+// Planes of a 64 x 64 matrix that is symmetric, or of columns of X: 64 values of a column, and what keeps sixteen lanes in different banks.
+constexpr int NARROW_PITCH = 72;
+// Of values that a 32x32 result's lane holds (rows from `at` on): four at a time, times 2^12, as high and low part.
+template <int SIZE> __device__ inline void narrow_put(_Float16 (*planes)[SIZE], int at, const float* v) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        f16x4 hi, lo;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float x = v[4 * q + k] * ORTHO_UP;
+            hi[k] = (_Float16)x;
+            lo[k] = (_Float16)(x - (float)hi[k]);
+        }
+        *reinterpret_cast<f16x4*>(planes[0] + at + 8 * q) = hi;
+        *reinterpret_cast<f16x4*>(planes[1] + at + 8 * q) = lo;
+    }
+}
+// Fragments. Of a symmetric matrix, a row: 8 values in order, or as ORDER_BLOCKS has them.
+__device__ inline i32x4 narrow_row(const _Float16* plane, int row, int f, int half) { return *reinterpret_cast<const i32x4*>(plane + row * NARROW_PITCH + f * 16 + 8 * half); }
+__device__ inline i32x4 narrow_row_blocks(const _Float16* plane, int row, int f, int half) {
+    const i32x2 a = *reinterpret_cast<const i32x2*>(plane + row * NARROW_PITCH + f * 16 + 4 * half);
+    const i32x2 b = *reinterpret_cast<const i32x2*>(plane + row * NARROW_PITCH + f * 16 + 8 + 4 * half);
+    return i32x4{a[0], a[1], b[0], b[1]};
+}
+// Of X: 32 rows from `row` on, 16 columns, read transposed.
+__device__ inline i32x4 narrow_columns(const _Float16* plane, int row, int f, int lane) {
+    i32x2 part[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const _Float16* p = plane + (f * 16 + 8 * (lane >> 5) + 4 * j + ((lane & 15) >> 2)) * NARROW_PITCH + row + ((lane >> 4) & 1) * 16 + 4 * (lane & 3);
+        part[j] = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+    }
+    return i32x4{part[0][0], part[0][1], part[1][0], part[1][1]};
+}
+
+// A thread's 32 of the 64 x 256 values of `in` or `out` from column j0 on, consecutive threads along the rows as they lie in memory:
+// every second row, or where the matrix lies the other way every eighth column.
+struct NarrowPlaces {
+    uint32_t row, j, first, by, end; // of the first value; `first` counts on by `by`, up to `end`, from one value to the next
+    bool tall, any;
+    __device__ NarrowPlaces(const OrthoArgs& a, uint32_t j0, uint32_t thread) {
+        tall = a.tall;
+        row = tall ? thread % NARROW : thread / NARROW_COLS;
+        j = tall ? thread / NARROW : thread % NARROW_COLS;
+        first = tall ? j0 + j : row;
+        by = tall ? 512 / NARROW : 512 / NARROW_COLS;
+        end = tall ? a.n : a.m;
+        any = tall ? row < a.m : j0 + j < a.n;
+    }
+    __device__ uint64_t offset(uint32_t j0, uint64_t stride) const { return tall ? (uint64_t)(j0 + j) * stride + row : (uint64_t)row * stride + j0 + j; }
+    __device__ bool in(int k) const { return any && first + k * by < end; }
+};
+template <typename F> __device__ inline void narrow_read(const NarrowPlaces& p, const F* from, uint64_t at, uint64_t stride, float (&v)[32]) {
+    const uint64_t step = p.by * stride;
+#pragma unroll
+    for (int k = 0; k < 32; k++) {
+        const float x = (float)from[p.in(k) ? at : 0]; // no branch, so that all are on their way together
+        v[k] = p.in(k) ? x : 0.f;
+        at += step;
+    }
+}
+__device__ inline void narrow_read(const NarrowPlaces& p, const void* from, uint64_t first, uint64_t at, uint64_t stride, uint32_t dtype, float (&v)[32]) {
+    if (dtype == APOE_F32) narrow_read(p, (const float*)from + first, at, stride, v);
+    else if (dtype == APOE_F16) narrow_read(p, (const _Float16*)from + first, at, stride, v);
+    else narrow_read(p, (const __bf16*)from + first, at, stride, v);
+}
+template <typename F> __device__ inline void narrow_write(const NarrowPlaces& p, F* to, uint64_t at, uint64_t stride, const float (&v)[32]) {
+    const uint64_t step = p.by * stride;
+#pragma unroll
+    for (int k = 0; k < 32; k++) {
+        if (p.in(k)) to[at] = (F)v[k];
+        at += step;
+    }
+}
+
+// FIRST: from `in`, else a step on X in memory. ONE: the only workgroup of its matrix, all steps. Grid (slabs, batch).
+// The three products of a fragment have sums of their own, added at the end: a third of the chain.
+template <bool FIRST, bool ONE> __global__ __launch_bounds__(512) void ortho_narrow(OrthoArgs a, NarrowArgs w, bool last) {
+    constexpr int STP = NARROW_COLS + 1;
+    __shared__ __align__(16) _Float16 ap[2][NARROW * NARROW_PITCH], bp[2][NARROW * NARROW_PITCH], xp[2][NARROW_COLS * NARROW_PITCH];
+    __shared__ float other[4 * 16 * 64];
+    __shared__ __align__(16) float diag[NARROW];
+    __shared__ double buf[8];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
+    const uint32_t batch = blockIdx.y, slab0 = blockIdx.x * NARROW_COLS;
+    const uint64_t slab = (uint64_t)batch * w.slabs + blockIdx.x;
+    float* kept = w.x + (slab * 8 + wave) * 32 * 64 + lane;
+    float x[2][16];
+    const int bi = (wave & 1) * 32, bj = ((wave >> 1) & 1) * 32; // a wave's block of the 64 x 64
+    auto multiply = [&](f32x16 (&acc)[3], const i32x4* l, const i32x4* r) {
+        acc[0] = mfma_step<_Float16>(l[1], r[0], acc[0]);
+        acc[1] = mfma_step<_Float16>(l[0], r[1], acc[1]);
+        acc[2] = mfma_step<_Float16>(l[0], r[0], acc[2]);
+    };
+    auto total = [&](const f32x16 (&acc)[3], int k) { return (acc[0][k] + acc[1][k]) + acc[2][k]; };
+    // A = X X^T over this workgroup's columns: the first four waves have it, 32 x 32 each, in `mine`
+    float mine[16];
+    auto gram = [&]() {
+#pragma unroll
+        for (int b = 0; b < 2; b++) narrow_put(xp, (wave * 32 + (lane & 31)) * NARROW_PITCH + b * 32 + 4 * half, x[b]);
+        __syncthreads();
+        const int frags = (int)(min(NARROW_COLS, a.n - slab0) + 15) / 16, end = min(frags, (wave >> 2) * 8 + 8);
+        f32x16 acc[3] = {};
+#pragma unroll 2
+        for (int f = (wave >> 2) * 8; f < end; f++) {
+            const i32x4 l[2] = {narrow_columns(xp[0], bi, f, lane), narrow_columns(xp[1], bi, f, lane)};
+            const i32x4 r[2] = {narrow_columns(xp[0], bj, f, lane), narrow_columns(xp[1], bj, f, lane)};
+            multiply(acc, l, r);
+        }
+        float* at = other + (wave & 3) * 16 * 64 + lane;
+        if (frags > 8) {
+            if (wave >> 2)
+#pragma unroll
+                for (int k = 0; k < 16; k++) at[k * 64] = total(acc, k);
+            __syncthreads();
+        }
+        if (wave < 4)
+#pragma unroll
+            for (int k = 0; k < 16; k++) mine[k] = (total(acc, k) + (frags > 8 ? at[k * 64] : 0.f)) * (ORTHO_DOWN * ORTHO_DOWN);
+    };
+    auto step = [&]() { // B from A, and X
+        if (wave < 4) narrow_put(ap, (bj + (lane & 31)) * NARROW_PITCH + bi + 4 * half, mine);
+        __syncthreads();
+        if (wave < 4) {
+            f32x16 acc[3] = {};
+#pragma unroll
+            for (int f = 0; f < 4; f++) {
+                const i32x4 l[2] = {narrow_row(ap[0], bi + (lane & 31), f, half), narrow_row(ap[1], bi + (lane & 31), f, half)};
+                const i32x4 r[2] = {narrow_row(ap[0], bj + (lane & 31), f, half), narrow_row(ap[1], bj + (lane & 31), f, half)};
+                multiply(acc, l, r);
+            }
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                mine[k] = __builtin_fmaf(a.c, total(acc, k) * (ORTHO_DOWN * ORTHO_DOWN), a.b * mine[k]);
+                if (bi + result_row(k, half) == bj + (lane & 31)) {
+                    diag[bj + (lane & 31)] = mine[k];
+                    mine[k] = 0.f;
+                }
+            }
+            narrow_put(bp, (bj + (lane & 31)) * NARROW_PITCH + bi + 4 * half, mine);
+        }
+        __syncthreads();
+        f32x16 acc[2][3] = {};
+#pragma unroll
+        for (int f = 0; f < 4; f++) {
+            f16x8 hi, lo; // X's fragment is eight of the lane's own values
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float v = x[f / 2][f % 2 * 8 + j] * ORTHO_UP;
+                hi[j] = (_Float16)v;
+                lo[j] = (_Float16)(v - (float)hi[j]);
+            }
+            const i32x4 r[2] = {__builtin_bit_cast(i32x4, hi), __builtin_bit_cast(i32x4, lo)};
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const i32x4 l[2] = {narrow_row_blocks(bp[0], b * 32 + (lane & 31), f, half), narrow_row_blocks(bp[1], b * 32 + (lane & 31), f, half)};
+                multiply(acc[b], l, r);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[b][i] = __builtin_fmaf(a.a + diag[b * 32 + result_row(i, half)], x[b][i], total(acc[b], i) * (ORTHO_DOWN * ORTHO_DOWN));
+    };
+    // 256 columns of `in` or `out` pass through LDS, so that consecutive threads are along their rows whichever way they lie
+    float* stage = reinterpret_cast<float*>(&xp[0][0]);
+    static_assert(NARROW * STP * 4 <= sizeof(xp), "fp32 in the planes' place");
+    auto staged = [&](int b, int i) -> float& { return stage[(b * 32 + result_row(i, half)) * STP + wave * 32 + (lane & 31)]; };
+    auto stage_at = [&](const NarrowPlaces& p, int k) -> float& { return stage[p.row * STP + p.j + k * (p.tall ? 512 / NARROW : 512 / NARROW_COLS * STP)]; };
+    float v[32];
+    if constexpr (FIRST) {
+        const NarrowPlaces places(a, slab0, threadIdx.x);
+        narrow_read(places, a.in, batch * a.in_batch, places.offset(slab0, a.in_stride), a.in_stride, a.in_dtype, v);
+        double s = 0;
+#pragma unroll
+        for (int k = 0; k < 32; k++) {
+            stage_at(places, k) = v[k];
+            if constexpr (ONE) s += (double)v[k] * (double)v[k];
+        }
+        double inv;
+        if constexpr (ONE) {
+            for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+            if (lane == 0) buf[wave] = s;
+            __syncthreads();
+            const double norm = sqrt(((buf[0] + buf[1]) + (buf[2] + buf[3])) + ((buf[4] + buf[5]) + (buf[6] + buf[7])));
+            inv = norm == 0. ? 0. : 1. / norm;
+        } else {
+            inv = ortho_inverse(a, batch, buf); // which waits for all threads
+        }
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[b][i] = (float)(staged(b, i) * inv);
+        __syncthreads();
+        if constexpr (ONE)
+            for (uint32_t k = 0; k < w.steps; k++) {
+                gram();
+                step();
+            }
+    } else {
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[b][i] = kept[(b * 16 + i) * 64];
+        const uint32_t parts = w.slabs > NARROW_PARTS ? 1 : w.slabs;
+        const float* from = (parts == 1 ? w.joined : w.sums[0]) + (uint64_t)batch * parts * NARROW * NARROW;
+        if (wave < 4) {
+#pragma unroll
+            for (int k = 0; k < 16; k++) mine[k] = 0.f;
+#pragma unroll 2
+            for (uint32_t g = 0; g < parts; g++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) mine[k] += from[(uint64_t)g * NARROW * NARROW + (bi + result_row(k, half)) * NARROW + bj + (lane & 31)];
+        }
+        step();
+    }
+    if constexpr (!ONE) {
+        if (!last) {
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) kept[(b * 16 + i) * 64] = x[b][i];
+            gram();
+            if (wave < 4)
+#pragma unroll
+                for (int k = 0; k < 16; k++) w.sums[1][slab * NARROW * NARROW + (bi + result_row(k, half)) * NARROW + bj + (lane & 31)] = mine[k];
+            return;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) staged(b, i) = a.alpha * x[b][i];
+    __syncthreads();
+    uint32_t thread = threadIdx.x;
+    asm volatile("" : "+v"(thread)); // places are worked out anew: kept since the reading, they would not leave room for the steps
+    const NarrowPlaces places(a, slab0, thread);
+    const uint64_t first = batch * a.out_batch, to = places.offset(slab0, a.out_stride);
+    if (a.beta != 0.f) narrow_read(places, a.out, first, to, a.out_stride, a.out_dtype, v);
+#pragma unroll
+    for (int k = 0; k < 32; k++) {
+        const float own = stage_at(places, k);
+        v[k] = a.beta != 0.f ? __builtin_fmaf(a.beta, v[k], own) : own;
+    }
+    if (a.out_dtype == APOE_F32) narrow_write(places, (float*)a.out + first, to, a.out_stride, v);
+    else if (a.out_dtype == APOE_F16) narrow_write(places, (_Float16*)a.out + first, to, a.out_stride, v);
+    else narrow_write(places, (__bf16*)a.out + first, to, a.out_stride, v);
+}
+
+// The sums of many workgroups, added up: grid (16, batch), four groups of waves that take every fourth of 256 values' sums.
+__global__ __launch_bounds__(1024) void ortho_narrow_join(NarrowArgs w) {
+    __shared__ float part[4][256];
+    const uint32_t value = threadIdx.x & 255, group = threadIdx.x >> 8, at = blockIdx.x * 256 + value;
+    const float* from = w.sums[0] + (uint64_t)blockIdx.y * w.slabs * NARROW * NARROW + at;
+    float v = 0.f;
+#pragma unroll 8
+    for (uint32_t g = group; g < w.slabs; g += 4) v += from[(uint64_t)g * NARROW * NARROW];
+    part[group][value] = v;
+    __syncthreads();
+    if (group == 0) w.joined[blockIdx.y * NARROW * NARROW + at] = (part[0][value] + part[1][value]) + (part[2][value] + part[3][value]);
+}
+
+static OrthoArgs ortho_args(const apoe_orthogonalize_args* p) {
     OrthoArgs a{};
     a.in = p->in;
     a.out = p->out;
@@ -656,6 +1005,50 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
     a.alpha = p->alpha;
     a.beta = p->beta;
     a.parts = std::min<uint32_t>(ORTHO_PARTS, (p->rows + 3) / 4);
+    return a;
+}
+
+// Rows of `in` are multiples of 16 bytes.
+static bool whole_rows(const apoe_orthogonalize_args* p, const OrthoArgs& a) {
+    const uint32_t v = p->in_dtype == APOE_F32 ? 4 : 8;
+    return p->cols % v == 0 && a.in_stride % v == 0 && (p->batch == 1 || a.in_batch % v == 0) && ((uintptr_t)a.in & 15) == 0;
+}
+
+// A short side of up to 64.
+static int run_narrow(apoe_ctx* ctx, const apoe_orthogonalize_args* p) {
+    OrthoArgs a = ortho_args(p);
+    NarrowArgs w{};
+    w.slabs = (a.n + NARROW_COLS - 1) / NARROW_COLS;
+    w.steps = p->steps;
+    const dim3 grid(w.slabs, p->batch);
+    hipStream_t s = ctx->stream;
+    if (w.slabs == 1) {
+        ortho_narrow<true, true><<<grid, 512, 0, s>>>(a, w, true);
+        APOE_HIP(hipGetLastError());
+        return APOE_OK;
+    }
+    const size_t part = (size_t)p->batch * ORTHO_PARTS * 8, x = (size_t)p->batch * w.slabs * NARROW * NARROW_COLS * 4, sums = (size_t)p->batch * w.slabs * NARROW * NARROW * 4;
+    char* ws = nullptr;
+    APOE_TRY(ctx->adapt_workspace(part + x + 2 * sums + (size_t)p->batch * NARROW * NARROW * 4, &ws));
+    a.part = (double*)ws;
+    w.x = (float*)(ws + part);
+    w.sums[0] = (float*)(ws + part + x + sums);
+    w.sums[1] = (float*)(ws + part + x);
+    w.joined = (float*)(ws + part + x + 2 * sums);
+    if (whole_rows(p, a)) ortho_squares<true><<<dim3(a.parts, p->batch), 256, 0, s>>>(a);
+    else ortho_squares<false><<<dim3(a.parts, p->batch), 256, 0, s>>>(a);
+    ortho_narrow<true, false><<<grid, 512, 0, s>>>(a, w, false);
+    for (uint32_t i = 0; i < p->steps; i++) {
+        std::swap(w.sums[0], w.sums[1]);
+        if (w.slabs > NARROW_PARTS) ortho_narrow_join<<<dim3(NARROW * NARROW / 256, p->batch), 1024, 0, s>>>(w);
+        ortho_narrow<false, false><<<grid, 512, 0, s>>>(a, w, i + 1 == p->steps);
+    }
+    APOE_HIP(hipGetLastError());
+    return APOE_OK;
+}
+
+template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonalize_args* p) {
+    OrthoArgs a = ortho_args(p);
     const uint32_t batch = p->batch;
     size_t bytes = 0;
     auto take = [&](size_t b) {
@@ -664,11 +1057,22 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
         return at;
     };
     const size_t xs = (size_t)batch * a.m * a.np, gs = (size_t)batch * a.m * a.mp;
-    const size_t o_part = take((size_t)batch * ORTHO_PARTS * 8), o_diag = take((size_t)batch * a.mp * 4), o_x = take(xs * 4);
+    const size_t o_part = take((size_t)batch * ORTHO_PARTS * 8), o_diag = take((size_t)batch * a.mp * 4), o_x = take(SPLIT ? xs * 4 : 0);
     constexpr int PLANES = SPLIT ? 2 : 1;
     a.h_low = (xs + 511) / 512 * 512;
     a.g_low = (gs + 511) / 512 * 512;
-    const size_t o_h = take(PLANES * a.h_low * 2), o_h2 = take(PLANES * a.h_low * 2), o_gram = take(PLANES * a.g_low * 2), o_poly = take(PLANES * a.g_low * 2);
+    const uint32_t cus = (uint32_t)ctx->num_cus;
+    auto tiles = [](uint32_t side, uint32_t t) { return (side + t - 1) / t; };
+    auto triangle = [](uint32_t t) { return t * (t + 1) / 2; };
+    // X X^T on tiles of 64 that leave CUs idle: its inner side is cut, and what the cuts give is joined by a launch of its own. 1024 values
+    // a cut at least, no more workgroups than CUs (the whole, fp16: 128 x 4096 103 us for 141, 128 x 16 384 136 for 382, 512 x 4096 142 for
+    // 173; twice the CUs: 4 x 512 x 4096 263 for 245).
+    const uint32_t g64 = triangle(tiles(a.m, 64)) * batch, stages = a.np / 64;
+    a.cuts = std::max(1u, std::min(cus / g64, stages / 16));
+    a.cut_stages = (stages + a.cuts - 1) / a.cuts;
+    a.cuts = (stages + a.cut_stages - 1) / a.cut_stages;
+    const size_t o_cut = take(a.cuts > 1 ? (size_t)g64 * a.cuts * 64 * 64 * 4 : 0);
+    const size_t o_h = take(2 * a.h_low * 2), o_h2 = take(2 * a.h_low * 2), o_gram = take(PLANES * a.g_low * 2), o_poly = take(PLANES * a.g_low * 2);
     char* ws = nullptr;
     APOE_TRY(ctx->adapt_workspace(bytes, &ws));
     a.part = (double*)(ws + o_part);
@@ -678,9 +1082,9 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
     a.h2 = (_Float16*)(ws + o_h2);
     a.gram = (_Float16*)(ws + o_gram);
     a.poly = (_Float16*)(ws + o_poly);
+    a.cut = (float*)(ws + o_cut);
     hipStream_t s = ctx->stream;
-    const uint32_t v = p->in_dtype == APOE_F32 ? 4 : 8;
-    const bool whole = p->cols % v == 0 && a.in_stride % v == 0 && (batch == 1 || a.in_batch % v == 0) && ((uintptr_t)a.in & 15) == 0;
+    const bool whole = whole_rows(p, a);
     a.whole_out = !a.tall && p->cols % 8 == 0 && a.out_stride % 8 == 0 && (batch == 1 || a.out_batch % 8 == 0) && ((uintptr_t)a.out & 15) == 0;
     if (whole) ortho_squares<true><<<dim3(a.parts, batch), 256, 0, s>>>(a);
     else ortho_squares<false><<<dim3(a.parts, batch), 256, 0, s>>>(a);
@@ -700,9 +1104,6 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
     //  64: below (1024 x 1024: X X^T 9 us; 128: 12)
     //  B X: 256 where those fill the GPU and the inner side is long enough to hide the end of a tile, whose traffic the next one does not
     //    overlap (the whole: 4096 x 8192 2.62 ms for 2.98, 8192 x 8192 11.0 for 12.4; 4 x 1024 x 4096 0.575 for 0.541), 128, 64
-    const uint32_t cus = (uint32_t)ctx->num_cus;
-    auto tiles = [](uint32_t side, uint32_t t) { return (side + t - 1) / t; };
-    auto triangle = [](uint32_t t) { return t * (t + 1) / 2; };
     const uint64_t s256 = (uint64_t)triangle(tiles(a.m, 256)) * batch, s192 = (uint64_t)triangle(tiles(a.m, 192)) * batch, s128 = (uint64_t)triangle(tiles(a.m, 128)) * batch, x256 = (uint64_t)tiles(a.m, 256) * tiles(a.n, 256) * batch, x128 = (uint64_t)tiles(a.m, 128) * tiles(a.n, 128) * batch;
     auto rounds = [&](uint64_t t) { return (t + cus - 1) / cus; };
     auto sym = [&](auto kind) {
@@ -717,7 +1118,12 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
         }
         if (s128 < cus && s128 >= cus / 2 && inner >= 4096) ortho_tile<SPLIT, 2, 2, 2, 2, 2, SPLIT ? 2 : 4, 4, K><<<dim3(triangle(tiles(a.m, 128)), batch), 512, 0, s>>>(a);
         else if (s128 >= cus) ortho_tile<SPLIT, 2, 1, 2, 4, 1, 4, 2, K><<<dim3(triangle(tiles(a.m, 128)), batch), 512, 0, s>>>(a);
-        else ortho_small<SPLIT, K><<<dim3(triangle(tiles(a.m, 64)), batch), 512, 0, s>>>(a);
+        else if (K == ORTHO_GRAM && a.cuts > 1) {
+            ortho_small<SPLIT, K><<<dim3(triangle(tiles(a.m, 64)) * a.cuts, batch), 512, 0, s>>>(a);
+            ortho_join<SPLIT><<<dim3(triangle(tiles(a.m, 64)), batch), 512, 0, s>>>(a);
+        } else {
+            ortho_small<SPLIT, K><<<dim3(triangle(tiles(a.m, 64)), batch), 512, 0, s>>>(a);
+        }
     };
     auto step = [&](auto kind) {
         constexpr int K = decltype(kind)::value;
@@ -742,8 +1148,8 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
 }
 
 int launch_orthogonalize(apoe_ctx* ctx, const apoe_orthogonalize_args* p) {
-    // a side of one tile: the roundings do not average (2 x 3: 0.8 % off in fp16 products); 87 us for 74 at 64 x 64, 143 for 97 at 64 x 1024
-    const bool split = p->products == APOE_F32 || std::min(p->rows, p->cols) <= 64;
+    if (std::min(p->rows, p->cols) <= NARROW) return run_narrow(ctx, p); // in fp16 products the roundings would not average (2 x 3: 0.8 % off)
+    const bool split = p->products == APOE_F32;
     return split ? run_ortho<true>(ctx, p) : run_ortho<false>(ctx, p);
 }
 

@@ -64,6 +64,34 @@ def test_sizes_and_types(gpu_ctx, rows, cols, dtype):
         assert error(got, reference(x)) < limit(dtype, products), (products, error(got, reference(x)))
 
 
+@pytest.mark.parametrize("batch,short,long", [(1, 64, 256), (3, 64, 257), (2, 33, 300), (1, 31, 1025), (5, 17, 4095), (1, 64, 4097), (2, 9, 9001), (70, 64, 129), (1, 1, 5000)])
+def test_one_short_side(gpu_ctx, batch, short, long):
+    """One workgroup a matrix, several, and so many that their sums are joined first; wide and tall, summed into what is there."""
+    import torch
+    import apoe
+    for rows, cols in ((short, long), (long, short)):
+        x = matrix(rows, cols, "float32", short + long, batch=batch, pad=3)
+        w = torch.randn(batch, rows, cols + 1, device="cuda")[..., :cols]
+        want = w.double().cpu()
+        got = apoe.orthogonalize(gpu_ctx, x, out=w, alpha=2.0, beta=-1.0)
+        for i in {0, batch // 2, batch - 1}:
+            r = reference(x[i])
+            assert float(torch.linalg.matrix_norm(got[i].double().cpu() - (2 * r - want[i]))) < 2 * 2e-5 * float(torch.linalg.matrix_norm(r)) + 2.0 ** -23 * float(torch.linalg.matrix_norm(want[i]))
+        again = apoe.orthogonalize(gpu_ctx, x, alpha=2.0)
+        assert bool((again == apoe.orthogonalize(gpu_ctx, x, alpha=2.0)).all())  # sums in a fixed order
+
+
+@pytest.mark.parametrize("batch,rows,cols", [(1, 100, 4100), (1, 2100, 300), (3, 65, 9000), (1, 129, 3000)])
+def test_few_tiles_and_a_long_side(gpu_ctx, batch, rows, cols):
+    """Products of few tiles, whose inner side is cut into parts (the last one shorter)."""
+    import apoe
+    x = matrix(rows, cols, "float32", 8, batch=batch, pad=1)
+    for products in ("f16", "f32"):
+        got = apoe.orthogonalize(gpu_ctx, x, products=products)
+        for i in {0, batch - 1}:
+            assert error(got[i], reference(x[i])) < limit("float32", products)
+
+
 def test_tiles_of_the_large_form(gpu_ctx):
     """Sides at which 128 x 128 tiles are taken (they fill the GPU), beyond whole tiles, wide and tall, one and several."""
     import apoe
