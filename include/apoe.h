@@ -335,14 +335,15 @@ typedef struct {
  * Softmax cross entropy of every query over the live rows, and the gradient of sum_i weight_i loss_i:
  *   s_ij = scale <q_i, x_j>, lse_i = log sum_j exp(s_ij), W_i = sum_t w_it, loss_i = W_i lse_i - sum_t w_it s_it.
  * Without live rows lse is -inf; without live targets loss and gradient are zero, whatever the query holds; a dead row's
- * gradient is zero. The logits are never in memory as a whole: the workspace holds at most 1 GiB of exponentials at a time,
- * 8 bytes for every 128 logits, and partial sums of grad_q.
+ * gradient is zero. The logits are never in memory as a whole: the workspace holds at most 1 GiB of exponentials at a time (one
+ * tile's rows at least), 8 bytes for every 128 logits, partial sums of grad_q, and for APOE_F32 at most 1 GiB of rows in the form
+ * that the products take.
  */
 int apoe_softmax_loss(apoe_ctx* ctx, const apoe_softmax_loss_args* args);
 
 typedef struct {
     uint32_t in_dtype, out_dtype;
-    uint32_t products;        /* APOE_F16: fp16 products on an fp32 iterate (off by 1e-4 to 6e-4 of the result; for bfloat16 results);
+    uint32_t products;        /* APOE_F16: fp16 products, the iterate in two fp16 parts (off by 1e-4 to 6e-4 of the result; for bfloat16 results);
                                  APOE_F32: products of 22 bits and more (1e-6 to 2e-5, as fp32 products have), at about twice the time */
     uint32_t batch, rows, cols;
     uint64_t in_stride, out_stride; /* from row to row */
