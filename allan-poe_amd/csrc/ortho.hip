@@ -480,9 +480,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void ortho_tile(OrthoArgs a) 
 // The same on tiles of 64 x 64 for matrices that larger tiles do not fill the GPU with. What counts then is the time of one tile:
 // eight waves, of which four take the even and four the odd half of a stage's fragments; what the epilogue needs of memory is
 // asked for before the first stage; and the sum goes through LDS, so that rows are written (and mirrored) 16 bytes a thread.
-template <bool SPLIT, int KIND> __global__ __launch_bounds__(512, 2) void ortho_small(OrthoArgs a) {
+template <bool SPLIT, int KIND, bool DEEP> __global__ __launch_bounds__(512, 2) void ortho_small(OrthoArgs a) {
     using T = _Float16;
-    constexpr int NW = 8, B = 64, SF = 4, ST = 3, PLANES = SPLIT ? 2 : 1, PITCH = 65;
+    constexpr int NW = 8, B = 64, SF = 4, AT_ONCE = DEEP ? 2 : 1, ST = DEEP ? 6 : 3, PLANES = SPLIT ? 2 : 1, PITCH = 65;
     constexpr bool SYM = KIND == ORTHO_GRAM || KIND == ORTHO_POLY;
     using ATile = RowTile<T, B, SF, NW>;
     using BTile = std::conditional_t<SYM, RowTile<T, B, SF, NW>, ColTile<T, B, SF, NW, ORDER_ROWS>>;
@@ -578,31 +578,37 @@ template <bool SPLIT, int KIND> __global__ __launch_bounds__(512, 2) void ortho_
         into = into + STAGE == ST * STAGE ? 0 : into + STAGE;
     };
 #pragma unroll
-    for (int s = 0; s < ST - 1; s++) issue();
+    for (int s = 0; s < ST - AT_ONCE; s++) issue();
     f32x16 acc[2] = {}; // even and odd fragments: two chains
     uint32_t from = 0;
-    for (int s = 0; s < stages; s++) {
-        tile_wait<(ST - 2) * PER>();
-        issue();
-        const char* A = lds + from;
-        const char* Bt = A + ATile::BYTES;
-        i32x4 x[2][PLANES], y[2][PLANES];
+    for (int s = 0; s < stages; s += AT_ONCE) {
+        tile_wait<(ST - 2 * AT_ONCE) * PER>();
+        i32x4 x[AT_ONCE][2][PLANES], y[AT_ONCE][2][PLANES];
 #pragma unroll
-        for (int f = 0; f < 2; f++)
+        for (int u = 0; u < AT_ONCE; u++) {
+            const char* A = lds + from + u * STAGE;
+            const char* Bt = A + ATile::BYTES;
 #pragma unroll
-            for (int p = 0; p < PLANES; p++) {
-                x[f][p] = ATile::read(A + p * PLANE, wm, group * 2 + f, lane);
-                y[f][p] = BTile::read(Bt + p * PLANE, wn, group * 2 + f, lane);
-            }
+            for (int f = 0; f < 2; f++)
 #pragma unroll
-        for (int f = 0; f < 2; f++) {
-            if constexpr (SPLIT) {
-                acc[f] = mfma_step<T>(x[f][1], y[f][0], acc[f]);
-                acc[f] = mfma_step<T>(x[f][0], y[f][1], acc[f]);
-            }
-            acc[f] = mfma_step<T>(x[f][0], y[f][0], acc[f]);
+                for (int p = 0; p < PLANES; p++) {
+                    x[u][f][p] = ATile::read(A + p * PLANE, wm, group * 2 + f, lane);
+                    y[u][f][p] = BTile::read(Bt + p * PLANE, wn, group * 2 + f, lane);
+                }
         }
-        from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++) issue();
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; u++)
+#pragma unroll
+            for (int f = 0; f < 2; f++) {
+                if constexpr (SPLIT) {
+                    acc[f] = mfma_step<T>(x[u][f][1], y[u][f][0], acc[f]);
+                    acc[f] = mfma_step<T>(x[u][f][0], y[u][f][1], acc[f]);
+                }
+                acc[f] = mfma_step<T>(x[u][f][0], y[u][f][0], acc[f]);
+            }
+        from = from + AT_ONCE * STAGE == ST * STAGE ? 0 : from + AT_ONCE * STAGE;
     }
     tile_wait<0>();
     float* sum = reinterpret_cast<float*>(lds);
@@ -1106,6 +1112,18 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
     //    overlap (the whole: 4096 x 8192 2.62 ms for 2.98, 8192 x 8192 11.0 for 12.4; 4 x 1024 x 4096 0.575 for 0.541), 128, 64
     const uint64_t s256 = (uint64_t)triangle(tiles(a.m, 256)) * batch, s192 = (uint64_t)triangle(tiles(a.m, 192)) * batch, s128 = (uint64_t)triangle(tiles(a.m, 128)) * batch, x256 = (uint64_t)tiles(a.m, 256) * tiles(a.n, 256) * batch, x128 = (uint64_t)tiles(a.m, 128) * tiles(a.n, 128) * batch;
     auto rounds = [&](uint64_t t) { return (t + cus - 1) / cus; };
+    // tiles of 64: where a workgroup has its CU to itself, six stages and two of them at a time (1024 x 1024: 120 us for 126; 768 x 3000, where two
+    // share one, 204 for 184); not SPLIT, whose stages are twice the size (777 x 1001: 201 for 174)
+    auto small = [&](auto kind, uint32_t grid) {
+        constexpr int K = decltype(kind)::value;
+        if constexpr (!SPLIT) {
+            if ((uint64_t)grid * batch <= cus) {
+                ortho_small<SPLIT, K, true><<<dim3(grid, batch), 512, 0, s>>>(a);
+                return;
+            }
+        }
+        ortho_small<SPLIT, K, false><<<dim3(grid, batch), 512, 0, s>>>(a);
+    };
     auto sym = [&](auto kind) {
         constexpr int K = decltype(kind)::value;
         const uint32_t inner = K == ORTHO_GRAM ? a.n : a.m;
@@ -1118,11 +1136,9 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
         }
         if (s128 < cus && s128 >= cus / 2 && inner >= 4096) ortho_tile<SPLIT, 2, 2, 2, 2, 2, SPLIT ? 2 : 4, 4, K><<<dim3(triangle(tiles(a.m, 128)), batch), 512, 0, s>>>(a);
         else if (s128 >= cus) ortho_tile<SPLIT, 2, 1, 2, 4, 1, 4, 2, K><<<dim3(triangle(tiles(a.m, 128)), batch), 512, 0, s>>>(a);
-        else if (K == ORTHO_GRAM && a.cuts > 1) {
-            ortho_small<SPLIT, K><<<dim3(triangle(tiles(a.m, 64)) * a.cuts, batch), 512, 0, s>>>(a);
-            ortho_join<SPLIT><<<dim3(triangle(tiles(a.m, 64)), batch), 512, 0, s>>>(a);
-        } else {
-            ortho_small<SPLIT, K><<<dim3(triangle(tiles(a.m, 64)), batch), 512, 0, s>>>(a);
+        else {
+            small(kind, triangle(tiles(a.m, 64)) * (K == ORTHO_GRAM ? a.cuts : 1));
+            if (K == ORTHO_GRAM && a.cuts > 1) ortho_join<SPLIT><<<dim3(triangle(tiles(a.m, 64)), batch), 512, 0, s>>>(a);
         }
     };
     auto step = [&](auto kind) {
@@ -1134,7 +1150,7 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
             }
         }
         if (x128 >= cus) ortho_tile<SPLIT, 2, 1, 2, 4, 1, 4, 2, K><<<dim3(tiles(a.m, 128) * tiles(a.n, 128), batch), 512, 0, s>>>(a);
-        else ortho_small<SPLIT, K><<<dim3(tiles(a.m, 64) * tiles(a.n, 64), batch), 512, 0, s>>>(a);
+        else small(kind, tiles(a.m, 64) * tiles(a.n, 64));
     };
     for (uint32_t i = 0; i < p->steps; i++) {
         sym(std::integral_constant<int, ORTHO_GRAM>{});
