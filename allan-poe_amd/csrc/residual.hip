@@ -20,26 +20,37 @@ struct ResArgs {
     apoe_gated_residual_args p;
     float* part;     // [blocks][2][dim]
     uint32_t blocks;
+    bool aligned; // the vectors begin at multiples of 16 bytes
 };
 
 // Values (c G + t) V .. of a row, c = 0, 1, ..: 16 bytes a load with V > 1.
 template <typename T, int V, int G> struct RowOf {
     typedef T tv __attribute__((ext_vector_type(V)));
     static constexpr int C = RES_E / V;
-    __device__ static void load(float* v, const void* p, uint64_t row, uint64_t stride, uint32_t dim, int t) {
+    // as it comes, and as numbers
+    __device__ static void fetch(tv* raw, const void* p, uint64_t row, uint64_t stride, uint32_t dim, int t) {
         const T* at = (const T*)p + row * stride;
 #pragma unroll
         for (int c = 0; c < C; c++) {
             const uint32_t d = (c * G + t) * V;
+            raw[c] = tv{};
             if constexpr (V == 1) {
-                v[c] = d < dim ? (float)at[d] : 0.f;
+                if (d < dim) raw[c][0] = at[d];
             } else {
-                tv x = {};
-                if (d < dim) x = *reinterpret_cast<const tv*>(at + d);
-#pragma unroll
-                for (int k = 0; k < V; k++) v[c * V + k] = (float)x[k];
+                if (d < dim) raw[c] = *reinterpret_cast<const tv*>(at + d);
             }
         }
+    }
+    __device__ static void widen(float* v, const tv* raw) {
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int k = 0; k < V; k++) v[c * V + k] = (float)raw[c][k];
+    }
+    __device__ static void load(float* v, const void* p, uint64_t row, uint64_t stride, uint32_t dim, int t) {
+        tv raw[C];
+        fetch(raw, p, row, stride, dim, t);
+        widen(v, raw);
     }
     __device__ static void store(void* p, uint64_t row, uint64_t stride, uint32_t dim, int t, const float* v) {
         T* at = (T*)p + row * stride;
@@ -58,7 +69,23 @@ template <typename T, int V, int G> struct RowOf {
         }
     }
     // a vector of floats (ones without one)
-    __device__ static void vec(float* v, const float* p, uint32_t dim, int t) {
+    __device__ static void vec(float* v, const float* p, uint32_t dim, int t, bool aligned) {
+        if constexpr (V > 1) {
+            if (p && aligned) {
+                typedef float f4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+                for (int c = 0; c < C; c++) {
+                    const uint32_t d = (c * G + t) * V;
+#pragma unroll
+                    for (int q = 0; q < V / 4; q++) {
+                        const f4 x = d < dim ? *reinterpret_cast<const f4*>(p + d + 4 * q) : f4{};
+#pragma unroll
+                        for (int k = 0; k < 4; k++) v[c * V + 4 * q + k] = x[k];
+                    }
+                }
+                return;
+            }
+        }
 #pragma unroll
         for (int c = 0; c < C; c++)
 #pragma unroll
@@ -102,12 +129,25 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
     const apoe_gated_residual_args& p = a.p;
     const int t = threadIdx.x % G;
     const float inv = 1.f / (float)p.dim;
+    const bool element = p.gate_kind == APOE_GATE_ELEMENT;
+    // a row is asked for before the one in front of it is worked on, the first before the vectors
+    typename R::tv xr[R::C], hr[R::C], gr[R::C];
+    auto ask = [&](uint64_t row) {
+        if (row >= p.rows) return;
+        R::fetch(xr, p.x, row, p.x_stride, p.dim, t);
+        if (!p.h) return;
+        R::fetch(hr, p.h, row, p.h_stride, p.dim, t);
+        if (element) R::fetch(gr, p.gate, row, p.gate_stride, p.dim, t);
+    };
+    const uint64_t step = (uint64_t)gridDim.x * GROUPS;
+    uint64_t row = (uint64_t)blockIdx.x * GROUPS + threadIdx.x / G;
+    ask(row);
     float sw[RES_E], wn[RES_E];
-    R::vec(sw, p.scale, p.dim, t);
-    R::vec(wn, p.w_next, p.dim, t);
+    R::vec(sw, p.scale, p.dim, t, a.aligned);
+    R::vec(wn, p.w_next, p.dim, t, a.aligned);
     {
         float w[RES_E];
-        R::vec(w, p.w_post, p.dim, t);
+        R::vec(w, p.w_post, p.dim, t, a.aligned);
 #pragma unroll
         for (int k = 0; k < RES_E; k++) sw[k] *= w[k];
         if (p.gate_kind == APOE_GATE_CHANNEL) {
@@ -116,13 +156,15 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
             for (int k = 0; k < RES_E; k++) sw[k] *= sigmoid(w[k]);
         }
     }
-    for (uint64_t row = (uint64_t)blockIdx.x * GROUPS + threadIdx.x / G; row < p.rows; row += (uint64_t)gridDim.x * GROUPS) {
-        float y[RES_E];
-        R::load(y, p.x, row, p.x_stride, p.dim, t);
+    for (; row < p.rows; row += step) {
+        float y[RES_E], h[RES_E], g[RES_E];
+        R::widen(y, xr);
         if (p.h) {
-            float h[RES_E], g[RES_E];
-            R::load(h, p.h, row, p.h_stride, p.dim, t);
-            if (p.gate_kind == APOE_GATE_ELEMENT) R::load(g, p.gate, row, p.gate_stride, p.dim, t);
+            R::widen(h, hr);
+            if (element) R::widen(g, gr);
+        }
+        ask(row + step);
+        if (p.h) {
             float s[1] = {0.f};
 #pragma unroll
             for (int k = 0; k < RES_E; k++) s[0] = __builtin_fmaf(h[k], h[k], s[0]);
@@ -131,7 +173,7 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
 #pragma unroll
             for (int k = 0; k < RES_E; k++) {
                 float b = h[k] * rh * sw[k];
-                if (p.gate_kind == APOE_GATE_ELEMENT) b *= sigmoid(g[k]);
+                if (element) b *= sigmoid(g[k]);
                 y[k] += b;
             }
             if (p.y) R::store(p.y, row, p.y_stride, p.dim, t, y);
@@ -159,11 +201,11 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
     const float inv = 1.f / (float)p.dim;
     const bool channel = p.gate_kind == APOE_GATE_CHANNEL, element = p.gate_kind == APOE_GATE_ELEMENT;
     float sw[RES_E], wn[RES_E], oc[RES_E], Q[RES_E] = {}, Rn[RES_E] = {};
-    R::vec(sw, p.scale, p.dim, t);
-    R::vec(wn, p.w_next, p.dim, t);
+    R::vec(sw, p.scale, p.dim, t, a.aligned);
+    R::vec(wn, p.w_next, p.dim, t, a.aligned);
     {
         float w[RES_E];
-        R::vec(w, p.w_post, p.dim, t);
+        R::vec(w, p.w_post, p.dim, t, a.aligned);
         if (channel) R::load(oc, p.gate, 0, 0, p.dim, t);
 #pragma unroll
         for (int k = 0; k < RES_E; k++) {
@@ -296,7 +338,7 @@ template <typename T> __global__ __launch_bounds__(1024) void residual_vectors(R
 }
 
 template <typename T, int V> static int run_residual(apoe_ctx* ctx, const apoe_gated_residual_args* p, bool grad) {
-    ResArgs a{*p, nullptr, 0};
+    ResArgs a{*p, nullptr, 0, (((uintptr_t)p->scale | (uintptr_t)p->w_post | (uintptr_t)p->w_next) & 15) == 0};
     hipStream_t s = ctx->stream;
     const uint32_t cus = (uint32_t)ctx->num_cus;
     auto go = [&](auto size) -> int {
