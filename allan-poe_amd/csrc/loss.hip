@@ -1513,6 +1513,12 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     using No = std::false_type;
     // One pass, for what needs no G: everything without grad x, and for float the loss and grad q beside it too.
     const bool one_pass = !gx || PLANES == 2;
+    const bool unjoined = !(gq && one_pass) && a.groups <= LOSS_CHUNKS; // few enough for one wave as they are
+    if (unjoined) {
+        a.chunk_ref = a.ref;
+        a.chunk_sum = a.sum;
+        a.chunks = a.groups;
+    }
     if (one_pass) {
         for (uint32_t i = 0; i < pieces; i++) {
             const uint32_t groups = set_piece(i);
@@ -1522,7 +1528,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
                 grad_q(Yes{}, groups, (int)(i & 1), i == 0);
             } else {
                 tiles(Sums{});
-                join_piece(i, groups, No{});
+                if (!unjoined) join_piece(i, groups, No{});
             }
         }
         if (gq) finish(Yes{}, Yes{}, (int)((pieces - 1) & 1));
@@ -1532,12 +1538,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
             const uint32_t groups = set_piece(i);
             if (pieces == 1) tiles(Exp{});
             else tiles(Sums{});
-            if (a.groups > LOSS_CHUNKS) join_piece(i, groups, No{});
-        }
-        if (a.groups <= LOSS_CHUNKS) { // few enough for one wave as they are
-            a.chunk_ref = a.ref;
-            a.chunk_sum = a.sum;
-            a.chunks = a.groups;
+            if (!unjoined) join_piece(i, groups, No{});
         }
     }
     if (gx) {
