@@ -24,6 +24,7 @@ constexpr uint32_t LOSS_GROUP = 128;               // rows that share a referenc
 // Of exponentials (or of G) that exist at a time. Each piece reads and writes the queries' partial sums once more: 1024 queries x 1 M
 // rows take 5.17 ms with pieces of 256 MiB, 4.82 ms with 1 GiB.
 constexpr size_t LOSS_PIECE_BYTES = 1u << 30;
+constexpr uint32_t LOSS_MAX_COLUMNS = APOE_LOSS_MAX_DIM;
 constexpr uint32_t LOSS_CHUNKS = 64;               // parts that the join of the sums is split into, at most
 
 // What the tiles are made of: the type itself, or for float two fp16 planes, a value (times a power of two) rounded and what that
@@ -87,8 +88,7 @@ struct LossArgs {
     uint32_t tile_row0, tile_r_pitch, tile_q_pitch, tile_dim; // the first row at tile_rows; bytes; columns with the pad
     uint64_t tile_r_low, tile_q_low, block_low;
     const char* grad_tile_q;    // q as grad x takes it; (float) the planes lie tile_q_low bytes apart
-    float *row_exp, *q_exp;     // planes: exponents of each 32 rows [n / 32]; of q (one)
-    float* q_max;               // [Q_PARTS] largest values of parts of q
+    float *row_exp, *q_exp;     // planes: exponents of each 32 rows [n / 32] and of each query
     float *chunk_ref, *chunk_sum; // [LOSS_CHUNKS][qp]
     float2* lse_w;              // [qp]: lse in base 2, weight W (to be multiplied with exp(s - lse))
     float *coef, *total;        // [qp]: |weight| (|W| + sum |w|); W
@@ -158,7 +158,6 @@ template <typename W> __device__ inline f32x16 multiply(const i32x4* x, const i3
 template <typename W> constexpr int PRODUCTS = W::PLANES * (W::PLANES + 1) / 2;
 
 // ---- planes of float matrices ----
-constexpr int Q_PARTS = 256;
 // The power of two that brings `top` to 2^14 .. 2^15.
 __device__ inline int plane_exp(float top) {
     int e = 0;
@@ -168,14 +167,6 @@ __device__ inline int plane_exp(float top) {
 __device__ inline float finite_abs(float v) {
     v = fabsf(v);
     return v <= 3.402823466e38f ? v : 0.f; // not a number: zero
-}
-__device__ inline float block_max(float v, float* buf) { // of 256 threads
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return fmaxf(fmaxf(buf[0], buf[1]), fmaxf(buf[2], buf[3]));
 }
 template <typename S, int P> __device__ inline void put_planes(char* at, uint64_t low, f32x4 x, int k) {
     typedef S s4 __attribute__((ext_vector_type(4)));
@@ -191,12 +182,45 @@ template <typename S, int P> __device__ inline void put_planes(char* at, uint64_
     for (int p = 0; p < P; p++) *reinterpret_cast<s4*>(at + p * low) = planes[p];
 }
 
+// A query, by one wave, with an exponent of its own.
+__device__ inline void split_query(const LossArgs& a, uint32_t qi) {
+    constexpr int HELD = LOSS_MAX_COLUMNS / 256;
+    const int lane = threadIdx.x & 63;
+    f32x4 x[HELD];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        const uint32_t d = (i * 64 + lane) * 4;
+        x[i] = d < a.dim ? *reinterpret_cast<const f32x4*>((const char*)a.q + (uint64_t)qi * a.q_pitch + d * 4) : f32x4{};
+    }
+#pragma unroll
+    for (int i = 0; i < HELD; i++) top = fmaxf(fmaxf(fmaxf(top, finite_abs(x[i][0])), fmaxf(finite_abs(x[i][1]), finite_abs(x[i][2]))), finite_abs(x[i][3]));
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const int k = plane_exp(top);
+    if (lane == 0) a.q_exp[qi] = (float)k;
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        const uint32_t d = (i * 64 + lane) * 4;
+        if (d >= a.tile_dim) continue;
+        const uint64_t at = (uint64_t)qi * a.tile_q_pitch + d * 2;
+        put_planes<_Float16, 2>((char*)a.tile_q + at, a.tile_q_low, x[i], k);
+        if (a.grad_x) put_planes<__bf16, 3>((char*)a.grad_tile_q + at, a.tile_q_low, x[i], 0);
+    }
+}
+
+// Workgroups from row_groups on: eight queries each. The others:
 // 32 rows, which share an exponent: up to 1024 columns they are held in registers between their largest value and the planes (read
 // twice, 100 000 rows took 250 us). Rows that are left out are zeros, and 32 of them have an exponent that no others have.
 constexpr int EMPTY_EXP = 1000;
-__global__ __launch_bounds__(512) void loss_split_rows(LossArgs a) {
+__global__ __launch_bounds__(512) void loss_split(LossArgs a, uint32_t row_groups) {
     constexpr int HELD = 16;
     __shared__ float buf[8];
+    if (blockIdx.x >= row_groups) {
+        const uint32_t qi = (blockIdx.x - row_groups) * 8 + (threadIdx.x >> 6);
+        if (qi < a.nq) split_query(a, qi);
+        return;
+    }
     const uint32_t row0 = a.row0 + blockIdx.x * 32, d4 = a.tile_dim / 4, total = 32 * d4;
     uint32_t on = 0;
     if (row0 < a.n) {
@@ -238,29 +262,6 @@ __global__ __launch_bounds__(512) void loss_split_rows(LossArgs a) {
         if (at < total) put(at, held[i]);
     }
     for (uint32_t at = HELD * 512 + threadIdx.x; at < total; at += 512) put(at, fetch(at));
-}
-__global__ __launch_bounds__(256) void loss_max_q(LossArgs a) {
-    __shared__ float buf[4];
-    float top = 0.f;
-    for (uint32_t r = blockIdx.x; r < a.nq; r += Q_PARTS)
-        for (uint32_t d = threadIdx.x * 4; d < a.dim; d += 1024) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>((const char*)a.q + (uint64_t)r * a.q_pitch + d * 4);
-            top = fmaxf(fmaxf(fmaxf(top, finite_abs(x[0])), fmaxf(finite_abs(x[1]), finite_abs(x[2]))), finite_abs(x[3]));
-        }
-    top = block_max(top, buf);
-    if (threadIdx.x == 0) a.q_max[blockIdx.x] = top;
-}
-__global__ __launch_bounds__(256) void loss_split_q(LossArgs a) {
-    __shared__ float buf[4];
-    const int k = plane_exp(block_max(a.q_max[threadIdx.x], buf));
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.q_exp[0] = (float)k;
-    for (uint32_t d = threadIdx.x * 4; d < a.tile_dim; d += 1024) {
-        f32x4 x = {};
-        if (d < a.dim) x = *reinterpret_cast<const f32x4*>((const char*)a.q + (uint64_t)blockIdx.x * a.q_pitch + d * 4);
-        const uint64_t at = (uint64_t)blockIdx.x * a.tile_q_pitch + d * 2;
-        put_planes<_Float16, 2>((char*)a.tile_q + at, a.tile_q_low, x, k);
-        if (a.grad_x) put_planes<__bf16, 3>((char*)a.grad_tile_q + at, a.tile_q_low, x, 0);
-    }
 }
 
 template <typename T, int NT, int WM, int WN, int SF, int ST, int MODE>
@@ -337,23 +338,16 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
     // epilogue: one query a lane (and its other half), 128 rows a wave
     const int h = lane >> 5;
     const uint32_t wrow = row + wm * LOSS_GROUP;
-    float c[4], down[4], row_exp = 0.f; // of each 32 rows: from sums to logits in base 2; what brings their exponentials to the group's exponent
+    float c[4], down[4], e[4] = {}, row_exp = 0.f; // of each 32 rows: from sums to logits in base 2; what brings their exponentials to the group's exponent
     if constexpr (P == 2) {
-        float e[4];
 #pragma unroll
         for (int m = 0; m < 4; m++) e[m] = a.row_exp[wrow / 32 + m];
         row_exp = fminf(fminf(e[0], e[1]), fminf(e[2], e[3]));
+    }
 #pragma unroll
-        for (int m = 0; m < 4; m++) {
-            c[m] = ldexpf(a.scale * LOG2E, -(int)(e[m] + a.q_exp[0]));
-            down[m] = __builtin_amdgcn_exp2f(row_exp - e[m]);
-        }
-    } else {
-#pragma unroll
-        for (int m = 0; m < 4; m++) {
-            c[m] = a.scale * LOG2E;
-            down[m] = 1.f;
-        }
+    for (int m = 0; m < 4; m++) {
+        c[m] = a.scale * LOG2E;
+        down[m] = P == 2 ? __builtin_amdgcn_exp2f(row_exp - e[m]) : 1.f;
     }
     uint32_t words[4];
 #pragma unroll
@@ -362,6 +356,11 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         const uint32_t qi = query + (wn * NT + t) * 32 + (lane & 31);
+        if constexpr (P == 2) {
+            const float own = qi < a.nq ? a.q_exp[qi] : 0.f;
+#pragma unroll
+            for (int m = 0; m < 4; m++) c[m] = ldexpf(a.scale * LOG2E, -(int)(e[m] + own));
+        }
         if (!all) {
 #pragma unroll
             for (int m = 0; m < 4; m++) {
@@ -1420,7 +1419,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.tile_r_low = PLANES == 2 ? piece * a.tile_dim * 2 : 0;
     a.tile_q_low = PLANES == 2 ? (uint64_t)a.qp * a.tile_dim * 2 : 0;
     const size_t o_rows = take(2 * a.tile_r_low), o_q = take(2 * a.tile_q_low), o_gq = take(gx ? 3 * a.tile_q_low : 0), o_bref = take(PLANES == 2 && gq ? (size_t)a.groups * a.qp * 4 : 0);
-    const size_t o_rexp = take((size_t)a.groups * 16), o_qexp = take(4), o_qmax = take(Q_PARTS * 4);
+    const size_t o_rexp = take((size_t)a.groups * 16), o_qexp = take((size_t)a.qp * 4);
     const size_t o_part = take(gq && !direct ? (size_t)splits * a.qp * a.dim * 4 : 0);
     const size_t o_pr0 = take((size_t)splits * a.qp * 4), o_pr1 = take((size_t)splits * a.qp * 4);
     char* ws = nullptr;
@@ -1440,7 +1439,6 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.total = (float*)(ws + o_total);
     a.row_exp = (float*)(ws + o_rexp);
     a.q_exp = (float*)(ws + o_qexp);
-    a.q_max = (float*)(ws + o_qmax);
     a.block_ref = PLANES == 2 ? (float*)(ws + o_bref) : a.ref;
     a.tile_rows = PLANES == 2 ? ws + o_rows : (const char*)a.rows;
     a.tile_q = PLANES == 2 ? ws + o_q : (const char*)a.q;
@@ -1448,11 +1446,6 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.tile_r_pitch = PLANES == 2 ? a.tile_dim * 2 : a.r_pitch;
     a.tile_q_pitch = PLANES == 2 ? a.tile_dim * 2 : a.q_pitch;
     hipStream_t s = ctx->stream;
-    if constexpr (PLANES == 2) {
-        loss_max_q<<<Q_PARTS, 256, 0, s>>>(a);
-        loss_split_q<<<a.nq, 256, 0, s>>>(a);
-    }
-
     uint32_t split_piece = ~0u;
     auto set_piece = [&](uint32_t i) {
         a.row0 = (uint32_t)(i * piece);
@@ -1461,7 +1454,8 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         a.row_blocks = rows / 32;
         if constexpr (PLANES == 2) {
             a.tile_row0 = a.row0;
-            if (i != split_piece) loss_split_rows<<<rows / 32, 512, 0, s>>>(a); // unless the planes are of this piece already
+            // unless the planes are of this piece already; the queries' once
+            if (i != split_piece) loss_split<<<rows / 32 + (split_piece == ~0u ? (a.nq + 7) / 8 : 0), 512, 0, s>>>(a, rows / 32);
             split_piece = i;
         }
         return rows / LOSS_GROUP;
