@@ -1465,8 +1465,8 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         const dim3 grid(a.row_tiles * a.q_tiles);
         if constexpr (PLANES == 2) {
             if (form == T256) loss_tile<T, 2, 2, 4, 2, 2, M><<<grid, 512, 0, s>>>(a);
-            else if (form == T128) loss_tile<T, 1, 1, 4, 2, 3, M><<<grid, 256, 0, s>>>(a);
-            else loss_tile<T, 1, 1, 2, 2, 3, M><<<grid, 128, 0, s>>>(a);
+            else if (form == T128) loss_tile<T, 1, 1, 4, 4, 2, M><<<grid, 256, 0, s>>>(a);
+            else loss_tile<T, 1, 1, 2, 4, 3, M><<<grid, 128, 0, s>>>(a);
         } else {
             if (form == T256) loss_tile<T, 2, 2, 4, 4, 2, M><<<grid, 512, 0, s>>>(a);
             else if (form == T256_128) loss_tile<T, 1, 2, 4, 4, 3, M><<<grid, 512, 0, s>>>(a);
