@@ -656,14 +656,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void loss_grad_q(LossArgs a, 
     __shared__ __align__(1024) char lds[ST * STAGE];
     __shared__ float factor[2][BM];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / (WM * WN), wm = wave % (WM * WN) / WN, wn = wave % WN;
-    const uint32_t per_split = a.q_tiles * n_tiles;
-    uint32_t split = blockIdx.x / per_split, rest = blockIdx.x % per_split;
-    if (a.splits % 8 == 0) { // the workgroups of one split, which read the same rows, on one XCD
-        const uint32_t i = blockIdx.x >> 3;
-        split = (i / per_split) * 8 + (blockIdx.x & 7);
-        rest = i % per_split;
-    }
-    if constexpr (DIRECT) rest = xcd_run(blockIdx.x, gridDim.x); // and the column tiles of one tile of queries, which read the same blocks
+    // the workgroups of one split, which read the same rows, on one XCD, and of those with one tile of queries the same blocks
+    const uint32_t per_split = a.q_tiles * n_tiles, id = xcd_run(blockIdx.x, gridDim.x), split = id / per_split, rest = id % per_split;
     const uint32_t query = rest / n_tiles * BM, col = rest % n_tiles * BN;
     const uint32_t g0 = min(split * groups_per_split, piece_groups), g1 = min(g0 + groups_per_split, piece_groups);
     const uint32_t group0 = a.row0 / LOSS_GROUP;
@@ -1390,15 +1384,15 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.groups = rows_up / LOSS_GROUP;
     const uint32_t chunks_per_piece = std::min<uint32_t>(std::max<uint32_t>(1, LOSS_CHUNKS / pieces), (uint32_t)((piece / LOSS_GROUP + 31) / 32));
     a.chunks = chunks_per_piece * pieces;
-    // grad q: tiles of 256 x 256, of 128 or 64 x 256 (float: 128 or 64 x 128); enough splits of the rows to fill the GPU (twice
-    // over where a CU holds two workgroups)
+    // grad q: tiles of 256 x 256, of 128 or 64 x 256 (float: 128 or 64 x 128); enough splits of the rows to give each CU one. The smaller
+    // tiles with two groups of waves (16 bits, 1000 x 4000: 53 us in all; with one group, two workgroups a CU and twice the splits, whose
+    // sums are written and read again, 60; 128 x 1 M 900 for 975)
     const uint32_t qm = a.nq <= 64 ? 64 : form == T256 && PLANES == 1 ? 256 : 128, qn = PLANES == 2 ? 128 : 256;
     const uint32_t gq_q_tiles = (a.qp + qm - 1) / qm, gq_n_tiles = (a.dim + qn - 1) / qn;
     const uint32_t piece_groups = (uint32_t)(piece / LOSS_GROUP);
     // With G whole in one piece, tiles of 128 x 128 that fill the GPU need no splits: 4096 x 4096 takes 15 us less.
     const bool direct = PLANES == 1 && gq && gx && pieces == 1 && (uint64_t)((a.qp + 127) / 128) * ((a.dim + 127) / 128) >= cus * 9 / 10;
-    uint32_t splits = std::min(LOSS_SPLITS, std::max<uint32_t>(1, (qm == 256 || PLANES == 2 ? 1 : 2) * cus / (gq_q_tiles * gq_n_tiles)));
-    if (splits >= 8) splits = splits / 8 * 8;
+    uint32_t splits = std::min(LOSS_SPLITS, std::max<uint32_t>(1, cus / (gq_q_tiles * gq_n_tiles)));
     splits = std::min(splits, piece_groups);
     const uint32_t per_split = (piece_groups + splits - 1) / splits;
     splits = (piece_groups + per_split - 1) / per_split;
@@ -1484,9 +1478,9 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
             if (qm == 64) loss_grad_q<T, 2, 1, 1, 4, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
             else loss_grad_q<T, 2, 2, 2, 2, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
         } else {
-            if (qm == 64) loss_grad_q<T, 2, 2, 1, 4, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
+            if (qm == 64) loss_grad_q<T, 2, 2, 1, 4, 6, E, false, 2><<<grid, 512, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
             else if (qm == 256) loss_grad_q<T, 4, 2, 2, 4, 4, E><<<grid, 512, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
-            else loss_grad_q<T, 2, 4, 2, 2, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
+            else loss_grad_q<T, 2, 4, 2, 2, 6, E, false, 2><<<grid, 512, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
         }
         a.q_tiles = keep;
     };
