@@ -1386,7 +1386,8 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.chunks = chunks_per_piece * pieces;
     // grad q: tiles of 256 x 256, of 128 or 64 x 256 (float: 128 or 64 x 128); enough splits of the rows to give each CU one. The smaller
     // tiles with two groups of waves (16 bits, 1000 x 4000: 53 us in all; with one group, two workgroups a CU and twice the splits, whose
-    // sums are written and read again, 60; 128 x 1 M 900 for 975)
+    // sums are written and read again, 60; 128 x 1 M 900 for 975; float 1024 x 20 000 357 for 368, but not up to 64 queries, which wait for
+    // memory: 20 x 1 M 3.51 ms for 3.35)
     const uint32_t qm = a.nq <= 64 ? 64 : form == T256 && PLANES == 1 ? 256 : 128, qn = PLANES == 2 ? 128 : 256;
     const uint32_t gq_q_tiles = (a.qp + qm - 1) / qm, gq_n_tiles = (a.dim + qn - 1) / qn;
     const uint32_t piece_groups = (uint32_t)(piece / LOSS_GROUP);
@@ -1476,7 +1477,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         const dim3 grid(gq_q_tiles * gq_n_tiles * splits);
         if constexpr (PLANES == 2) {
             if (qm == 64) loss_grad_q<T, 2, 1, 1, 4, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
-            else loss_grad_q<T, 2, 2, 2, 2, 3, E><<<grid, 256, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
+            else loss_grad_q<T, 2, 2, 2, 2, 4, E, false, 2><<<grid, 512, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
         } else {
             if (qm == 64) loss_grad_q<T, 2, 2, 1, 4, 6, E, false, 2><<<grid, 512, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
             else if (qm == 256) loss_grad_q<T, 4, 2, 2, 4, 4, E><<<grid, 512, 0, s>>>(a, gq_n_tiles, per_split, groups, turn, first);
