@@ -947,7 +947,7 @@ constexpr uint32_t LOSS_SPLITS = 512; // of the rows under one partial sum of gr
 // One workgroup a query: lse, loss, and the query's gradient from its splits. EXP: the splits are sums of exponentials relative
 // to their references without the targets, whose terms are added here; otherwise they are sums of scaled G. A thread holds four
 // columns (and their next 4 THREADS); where a row has fewer than 4 THREADS columns the threads share the splits.
-template <typename T, bool GRAD, bool EXP, int THREADS> __global__ __launch_bounds__(THREADS) void loss_finish(LossArgs a, int turn) {
+template <typename T, bool GRAD, bool EXP, int THREADS> __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 4) void loss_finish(LossArgs a, int turn) {
     constexpr int C = APOE_LOSS_MAX_DIM / (THREADS * 4);
     typedef T t4 __attribute__((ext_vector_type(4)));
     __shared__ float buf[THREADS / 64], lse_of, factor[GRAD ? LOSS_SPLITS : 1];
@@ -957,14 +957,30 @@ template <typename T, bool GRAD, bool EXP, int THREADS> __global__ __launch_boun
     uint32_t lanes = THREADS;
     while (lanes * 2 >= a.dim && lanes > 64) lanes /= 2; // threads along a row
     const uint32_t groups = THREADS / lanes, g = tid / lanes, d0 = tid % lanes * 4;
+    constexpr int EARLY = GRAD && EXP ? 4 : 1; // sums of the splits that are asked for before their factors are known
+    f32x4 early[EARLY];
+    if constexpr (GRAD && EXP) {
+#pragma unroll
+        for (int i = 0; i < EARLY; i++) {
+            const uint32_t s = g + i * groups;
+            early[i] = s < a.splits && d0 < a.dim ? *reinterpret_cast<const f32x4*>(a.part + ((size_t)s * a.qp + qi) * a.dim + d0) : f32x4{};
+        }
+    }
     auto add_splits = [&]() {
 #pragma unroll
         for (int k = 0; k < C; k++) {
             const uint32_t d = d0 + k * THREADS * 4;
             if (d >= a.dim || (k && groups > 1)) continue;
             const float* p = a.part + (size_t)qi * a.dim + d;
+            if (EXP && k == 0) {
+#pragma unroll
+                for (int i = 0; i < EARLY; i++) {
+                    const uint32_t s = g + i * groups;
+                    if (s < a.splits) acc[0] += factor[s] * early[i];
+                }
+            }
 #pragma unroll 4
-            for (uint32_t s = g; s < a.splits; s += groups) {
+            for (uint32_t s = g + (EXP && k == 0 ? EARLY * groups : 0); s < a.splits; s += groups) {
                 const f32x4 x = *reinterpret_cast<const f32x4*>(p + (size_t)s * a.qp * a.dim);
                 acc[k] += EXP ? factor[s] * x : x;
             }
