@@ -14,6 +14,9 @@
 //     over memory: 38 us for 2048 x 30 522, forming the logits again 150 us); otherwise the logits are formed again once lse is known.
 // The targets' own terms are not left to the rounded blocks: their places are zeroed (or rewritten) and W p_t - w_t, which
 // nearly cancels for a query that is served well, is formed in 32 bits.
+// Exponentials (or G) in 16 bits are what the 16-bit products take; a second part of each would double the gradients' products. Against a
+// gradient formed in 32 bits and rounded once the error is 1.2 times as large for many queries (4096 x 4096 bf16: 0.0021 for 0.0017), and
+// 1.5 to 1.8 times for the rows' gradients of a few queries, where one rounded weight of a target is most of a row (0.0030 for 0.0017).
 #include "apoe_internal.h"
 #include "apoe_tile.h"
 
