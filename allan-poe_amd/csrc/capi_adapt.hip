@@ -8,7 +8,7 @@ using namespace apoe;
 
 namespace {
 
-constexpr uint32_t ORTHO_MAX_SIDE = 65536; // 128 rows of a working matrix stay within a 31-bit offset
+constexpr uint32_t ORTHO_MAX_SIDE = 65536; // 256 rows of a working matrix stay well within a 31-bit offset
 
 size_t size_of(uint32_t dtype) { return dtype == APOE_F32 ? 4 : 2; }
 

@@ -1073,11 +1073,12 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
     // X X^T on tiles of 64 that leave CUs idle: its inner side is cut, and what the cuts give is joined by a launch of its own. 1024 values
     // a cut at least, no more workgroups than CUs (the whole, fp16: 128 x 4096 103 us for 141, 128 x 16 384 136 for 382, 512 x 4096 142 for
     // 173; twice the CUs: 4 x 512 x 4096 263 for 245).
-    const uint32_t g64 = triangle(tiles(a.m, 64)) * batch, stages = a.np / 64;
-    a.cuts = std::max(1u, std::min(cus / g64, stages / 16));
+    const uint64_t g64 = (uint64_t)triangle(tiles(a.m, 64)) * batch;
+    const uint32_t stages = a.np / 64;
+    a.cuts = std::max(1u, std::min((uint32_t)(cus / g64), stages / 16));
     a.cut_stages = (stages + a.cuts - 1) / a.cuts;
     a.cuts = (stages + a.cut_stages - 1) / a.cut_stages;
-    const size_t o_cut = take(a.cuts > 1 ? (size_t)g64 * a.cuts * 64 * 64 * 4 : 0);
+    const size_t o_cut = take(a.cuts > 1 ? g64 * a.cuts * 64 * 64 * 4 : 0);
     const size_t o_h = take(2 * a.h_low * 2), o_h2 = take(2 * a.h_low * 2), o_gram = take(PLANES * a.g_low * 2), o_poly = take(PLANES * a.g_low * 2);
     char* ws = nullptr;
     APOE_TRY(ctx->adapt_workspace(bytes, &ws));
