@@ -619,6 +619,8 @@ def orthogonalize(ctx, x, out=None, steps=5, coefs=COEFS, alpha=1.0, beta=0.0, p
     for t, name, row, mat in ((x, "x", "in_stride", "in_batch_stride"), (out, "out", "out_stride", "out_batch_stride")):
         setattr(a, row, _matrix(ctx, t if t.dim() == 2 else t[0], name))
         if t.dim() == 3 and t.shape[0] > 1:
+            if t.stride(0) == 0:  # a matrix that is repeated: to the library zero would say that matrices follow one another
+                raise ApoeError(f"the matrices of {name} overlap")
             setattr(a, mat, t.stride(0))
     a.in_, a.out, a.steps = x.data_ptr(), out.data_ptr(), steps
     a.a, a.b, a.c = coefs
