@@ -356,7 +356,7 @@ template <typename T, int V> static int run_residual(apoe_ctx* ctx, const apoe_g
             APOE_TRY(ctx->adapt_workspace((size_t)a.blocks * 2 * p->dim * 4, &ws));
             a.part = (float*)ws;
         }
-        residual_backward<T, V, G><<<a.blocks, THREADS, 0, s>>>(a);
+        if (a.blocks) residual_backward<T, V, G><<<a.blocks, THREADS, 0, s>>>(a); // no rows: the vectors' gradients alone, which are zeros
         if (vectors) residual_vectors<T><<<(p->dim + 15) / 16, 1024, 0, s>>>(a);
         return APOE_OK;
     };
