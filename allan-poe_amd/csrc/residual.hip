@@ -122,6 +122,16 @@ template <int G, int N> __device__ inline void group_sum(float* v, float (*buf)[
 
 __device__ inline float sigmoid(float g) { return 1.f / (1.f + expf(-g)); }
 
+// A gate as the gradient holds it: sigmoid(g) or 1 - sigmoid(g), whichever is smaller, the latter with its sign bit set. Both come from it with
+// full accuracy (1 - sigmoid(g) as a difference of floats has 13 bits left at g = 8 and none from 17 on), in one register a value.
+constexpr float GATE_OPEN = -0.f;
+__device__ inline float gate_of(float g) {
+    const float t = expf(-fabsf(g)), least = t * __builtin_amdgcn_rcpf(1.f + t); // a reciprocal of 1 .. 2, right to a unit of the last place
+    return g >= 0.f ? -least : least;
+}
+__device__ inline float gate_open(float v) { return __builtin_signbit(v) ? 1.f + v : v; }
+__device__ inline float gate_rest(float v) { return __builtin_signbit(v) ? -v : 1.f - v; }
+
 // GATE: what multiplies the block, in `open` (ones, sigmoid of the row's gate, or of the channel's, which the caller holds).
 template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 256) void residual_forward(ResArgs a) {
     using R = RowOf<T, V, G>;
@@ -211,7 +221,7 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
 #pragma unroll
         for (int k = 0; k < RES_E; k++) {
             sw[k] *= w[k];
-            oc[k] = channel ? sigmoid(oc[k]) : 1.f;
+            oc[k] = channel ? gate_of(oc[k]) : GATE_OPEN;
         }
     }
     for (uint64_t row = (uint64_t)blockIdx.x * GROUPS + group; row < p.rows; row += (uint64_t)gridDim.x * GROUPS) {
@@ -227,9 +237,9 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
             rh = rsqrtf(__builtin_fmaf(s[0], inv, p.eps));
 #pragma unroll
             for (int k = 0; k < RES_E; k++) {
-                o[k] = element ? sigmoid(o[k]) : oc[k];
+                o[k] = element ? gate_of(o[k]) : oc[k];
                 h[k] *= rh;
-                y[k] = __builtin_fmaf(h[k] * sw[k], o[k], y[k]);
+                y[k] = __builtin_fmaf(h[k] * sw[k], gate_open(o[k]), y[k]);
             }
         }
         if (p.grad_u) {
@@ -258,14 +268,14 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
             float s[1] = {0.f};
 #pragma unroll
             for (int k = 0; k < RES_E; k++) {
-                gy[k] *= o[k]; // from here on with the gate
+                gy[k] *= gate_open(o[k]); // from here on with the gate
                 Q[k] = __builtin_fmaf(gy[k], h[k], Q[k]);
                 s[0] = __builtin_fmaf(gy[k] * sw[k], h[k], s[0]);
             }
             if (element && p.grad_gate) {
                 float gg[RES_E];
 #pragma unroll
-                for (int k = 0; k < RES_E; k++) gg[k] = gy[k] * sw[k] * h[k] * (1.f - o[k]);
+                for (int k = 0; k < RES_E; k++) gg[k] = gy[k] * sw[k] * h[k] * gate_rest(o[k]);
                 R::store(p.grad_gate, row, p.grad_gate_stride, p.dim, t, gg);
             }
             if (p.grad_h) {
@@ -335,7 +345,7 @@ template <typename T> __global__ __launch_bounds__(1024) void residual_vectors(R
     if (p.grad_scale) p.grad_scale[d] = Q * w;
     if (p.grad_w_post) p.grad_w_post[d] = Q * s;
     if (p.grad_w_next) p.grad_w_next[d] = R;
-    if (p.gate_kind == APOE_GATE_CHANNEL && p.grad_gate) ((T*)p.grad_gate)[d] = (T)(Q * s * w * (1.f - sigmoid((float)((const T*)p.gate)[d])));
+    if (p.gate_kind == APOE_GATE_CHANNEL && p.grad_gate) ((T*)p.grad_gate)[d] = (T)(Q * s * w * sigmoid(-(float)((const T*)p.gate)[d]));
 }
 
 template <typename T, int V> static int run_residual(apoe_ctx* ctx, const apoe_gated_residual_args* p, bool grad) {

@@ -1,9 +1,31 @@
-"""The gated residual where its parts are nearly nothing (needs the GPU): calls without rows."""
+"""The gated residual where its parts are nearly nothing (needs the GPU): gates that are all but open, calls without rows."""
 import ctypes as C
 
 import pytest
 
+from test_gpu_gated_residual import close, formula, make
+
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", ["element", "channel"])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("d", [40, 1024])
+def test_gates_that_are_all_but_open(gpu_ctx, dtype, kind, d):
+    """What is left of a gate at 10 to 14 is 1 - sigmoid = 1e-6 to 5e-5, and its gradient is as right as any other's. The incoming gradients
+    are large, so that the gradient of a channel's gate is above one, the size that its tolerance is relative to."""
+    import apoe
+    a, grads = make(60, d, dtype, d, kind)
+    a["gate"] = a["gate"].abs() * 0.5 + 10.0
+    for k in grads:
+        grads[k] = grads[k] * 2.0 ** 10
+    if dtype == "float32":
+        for k in grads:
+            grads[k] = grads[k] * 2.0 ** 8
+    want = formula(a, grads)
+    got = apoe.gated_residual_grad(gpu_ctx, **a, **grads)
+    for k in got:
+        close(got[k], want[k], dtype, 60, k, want["terms"])
 
 
 @pytest.mark.parametrize("kind", ["none", "channel"])
