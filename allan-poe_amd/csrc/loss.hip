@@ -214,7 +214,8 @@ __device__ inline void split_query(const LossArgs& a, uint32_t qi) {
 
 // float to planes, bound by memory: 100 000 rows of 1024 in 115 us (820 MB, 7.1 TB/s). Workgroups from row_groups on: eight queries each. The others:
 // 32 rows, which share an exponent: up to 1024 columns they are held in registers between their largest value and the planes (read
-// twice, 100 000 rows took 250 us). Rows that are left out are zeros, and 32 of them have an exponent that no others have.
+// twice, 100 000 rows took 250 us). Rows that are left out are zeros, and 32 zeros, left out or live, have an exponent that no others have: with an
+// ordinary one they would count as larger than the rows beside them, whose exponentials are brought to the group's smallest exponent.
 constexpr int EMPTY_EXP = 1000;
 __global__ __launch_bounds__(512) void loss_split(LossArgs a, uint32_t row_groups) {
     constexpr int HELD = 16;
@@ -254,7 +255,7 @@ __global__ __launch_bounds__(512) void loss_split(LossArgs a, uint32_t row_group
 #pragma unroll
     for (int w = 0; w < 8; w++) top = fmaxf(top, buf[w]);
     const int k = plane_exp(top);
-    if (threadIdx.x == 0) a.row_exp[row0 / 32] = (float)(on ? k : EMPTY_EXP);
+    if (threadIdx.x == 0) a.row_exp[row0 / 32] = (float)(top > 0.f ? k : EMPTY_EXP);
     auto put = [&](uint32_t at, f32x4 x) {
         const uint32_t r = at / d4, d = at % d4 * 4;
         put_planes<_Float16, 2>((char*)a.tile_rows + (uint64_t)(row0 + r - a.tile_row0) * a.tile_r_pitch + d * 2, a.tile_r_low, x, k);
