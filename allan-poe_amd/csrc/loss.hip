@@ -85,13 +85,13 @@ struct LossArgs {
     uint32_t row0, row_tiles, q_tiles, row_blocks; // first row, tiles of either side, blocks of 32 rows (the pitch of `blocks`)
     // workspace
     float *ref, *sum;           // [n / LOSS_GROUP][qp]
-    float* block_ref;           // the same for the blocks: `ref` itself, or with planes less the smallest exponent of the group's rows
+    float* block_ref;           // the same for the blocks: `ref` itself, or with planes of the exponentials times the rows' powers of two
     // the tiles' operands: rows and q themselves, or (float) planes of this piece's rows and of q, whose low parts lie *_low bytes behind
     const char *tile_rows, *tile_q;
     uint32_t tile_row0, tile_r_pitch, tile_q_pitch, tile_dim; // the first row at tile_rows; bytes; columns with the pad
     uint64_t tile_r_low, tile_q_low, block_low;
     const char* grad_tile_q;    // q as grad x takes it; (float) the planes lie tile_q_low bytes apart
-    float *row_exp, *q_exp;     // planes: exponents of each 32 rows [n / 32] and of each query
+    float *row_exp, *q_exp;     // planes: exponents of each row and of each query
     float *chunk_ref, *chunk_sum; // [LOSS_CHUNKS][qp]
     float2* lse_w;              // [qp]: lse in base 2, weight W (to be multiplied with exp(s - lse))
     float *coef, *total;        // [qp]: |weight| (|W| + sum |w|); W
@@ -185,87 +185,76 @@ template <typename S, int P> __device__ inline void put_planes(char* at, uint64_
     for (int p = 0; p < P; p++) *reinterpret_cast<s4*>(at + p * low) = planes[p];
 }
 
-// A query, by one wave, with an exponent of its own.
-__device__ inline void split_query(const LossArgs& a, uint32_t qi) {
-    constexpr int HELD = LOSS_MAX_COLUMNS / 256;
-    const int lane = threadIdx.x & 63;
+// Rows of a matrix that a wave holds between their largest value and the planes, HELD times 256 columns at most.
+template <int HELD> struct HeldRow {
     f32x4 x[HELD];
-    float top = 0.f;
+    __device__ void fetch(const void* row, uint32_t dim, bool on, int lane) {
 #pragma unroll
-    for (int i = 0; i < HELD; i++) {
-        const uint32_t d = (i * 64 + lane) * 4;
-        x[i] = d < a.dim ? *reinterpret_cast<const f32x4*>((const char*)a.q + (uint64_t)qi * a.q_pitch + d * 4) : f32x4{};
+        for (int i = 0; i < HELD; i++) {
+            const uint32_t d = (i * 64 + lane) * 4;
+            x[i] = on && d < dim ? *reinterpret_cast<const f32x4*>((const char*)row + d * 4) : f32x4{};
+        }
     }
+    __device__ float top() const { // the largest magnitude, the same for all lanes
+        float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < HELD; i++) top = fmaxf(fmaxf(fmaxf(top, finite_abs(x[i][0])), fmaxf(finite_abs(x[i][1]), finite_abs(x[i][2]))), finite_abs(x[i][3]));
+        for (int i = 0; i < HELD; i++) top = fmaxf(fmaxf(fmaxf(top, finite_abs(x[i][0])), fmaxf(finite_abs(x[i][1]), finite_abs(x[i][2]))), finite_abs(x[i][3]));
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    const int k = plane_exp(top);
-    if (lane == 0) a.q_exp[qi] = (float)k;
-#pragma unroll
-    for (int i = 0; i < HELD; i++) {
-        const uint32_t d = (i * 64 + lane) * 4;
-        if (d >= a.tile_dim) continue;
-        const uint64_t at = (uint64_t)qi * a.tile_q_pitch + d * 2;
-        put_planes<_Float16, 2>((char*)a.tile_q + at, a.tile_q_low, x[i], k);
-        if (a.grad_x) put_planes<__bf16, 3>((char*)a.grad_tile_q + at, a.tile_q_low, x[i], 0);
+        for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+        return top;
     }
-}
+    template <typename S, int P> __device__ void put(char* row, uint64_t low, uint32_t tile_dim, int k, int lane) const {
+#pragma unroll
+        for (int i = 0; i < HELD; i++) {
+            const uint32_t d = (i * 64 + lane) * 4;
+            if (d < tile_dim) put_planes<S, P>(row + d * 2, low, x[i], k);
+        }
+    }
+};
 
-// float to planes, bound by memory: 100 000 rows of 1024 in 115 us (820 MB, 7.1 TB/s). Workgroups from row_groups on: eight queries each. The others:
-// 32 rows, which share an exponent: up to 1024 columns they are held in registers between their largest value and the planes (read
-// twice, 100 000 rows took 250 us). Rows that are left out are zeros, and 32 zeros, left out or live, have an exponent that no others have: with an
-// ordinary one they would count as larger than the rows beside them, whose exponentials are brought to the group's smallest exponent.
+// float to planes, each row and each query with an exponent of its own, bound by memory: 99 991 rows of 1024, 0.7 of
+// them live, in 116 us (697 MB, 6.0 TB/s).
+// Workgroups from row_groups on: eight queries each, the others 32 rows, four a wave. A row of zeros, left out or live, has an exponent that no other
+// has: with an ordinary one it would count as larger than the rows beside it (loss_tile).
 constexpr int EMPTY_EXP = 1000;
-__global__ __launch_bounds__(512) void loss_split(LossArgs a, uint32_t row_groups) {
-    constexpr int HELD = 16;
-    __shared__ float buf[8];
+template <int HELD> __global__ __launch_bounds__(512) void loss_split(LossArgs a, uint32_t row_groups) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (blockIdx.x >= row_groups) {
-        const uint32_t qi = (blockIdx.x - row_groups) * 8 + (threadIdx.x >> 6);
-        if (qi < a.nq) split_query(a, qi);
+        const uint32_t qi = (blockIdx.x - row_groups) * 8 + wave;
+        if (qi >= a.nq) return;
+        HeldRow<HELD> q;
+        q.fetch((const char*)a.q + (uint64_t)qi * a.q_pitch, a.dim, true, lane);
+        const int k = plane_exp(q.top());
+        if (lane == 0) a.q_exp[qi] = (float)k;
+        const uint64_t at = (uint64_t)qi * a.tile_q_pitch;
+        q.template put<_Float16, 2>((char*)a.tile_q + at, a.tile_q_low, a.tile_dim, k, lane);
+        if (a.grad_x) q.template put<__bf16, 3>((char*)a.grad_tile_q + at, a.tile_q_low, a.tile_dim, 0, lane);
         return;
     }
-    const uint32_t row0 = a.row0 + blockIdx.x * 32, d4 = a.tile_dim / 4, total = 32 * d4;
+    const uint32_t row0 = a.row0 + blockIdx.x * 32;
     uint32_t on = 0;
     if (row0 < a.n) {
         on = a.live ? a.live[row0 >> 5] : ~0u;
         if (a.n - row0 < 32) on &= (1u << (a.n - row0)) - 1u;
     }
-    auto fetch = [&](uint32_t at) {
-        const uint32_t r = at / d4, d = at % d4 * 4;
-        f32x4 x = {};
-        if (((on >> r) & 1) && d < a.dim) x = *reinterpret_cast<const f32x4*>((const char*)a.rows + (uint64_t)(row0 + r) * a.r_pitch + d * 4);
-        return x;
-    };
-    auto largest = [](f32x4 x) { return fmaxf(fmaxf(finite_abs(x[0]), finite_abs(x[1])), fmaxf(finite_abs(x[2]), finite_abs(x[3]))); };
-    f32x4 held[HELD];
-    float top = 0.f;
+    constexpr int AT_ONCE = HELD <= 4 ? 4 : 1; // rows that are on their way together
+    HeldRow<HELD> x[AT_ONCE];
 #pragma unroll
-    for (int i = 0; i < HELD; i++) {
-        const uint32_t at = i * 512 + threadIdx.x;
-        held[i] = at < total ? fetch(at) : f32x4{};
+    for (int r0 = 0; r0 < 4; r0 += AT_ONCE) {
+#pragma unroll
+        for (int r = 0; r < AT_ONCE; r++) {
+            const uint32_t row = wave * 4 + r0 + r;
+            x[r].fetch((const char*)a.rows + (uint64_t)(row0 + row) * a.r_pitch, a.dim, (on >> row) & 1, lane);
+        }
+#pragma unroll
+        for (int r = 0; r < AT_ONCE; r++) {
+            const uint32_t row = wave * 4 + r0 + r;
+            const float top = x[r].top();
+            const int k = plane_exp(top);
+            if (lane == 0) a.row_exp[row0 + row] = (float)(top > 0.f ? k : EMPTY_EXP);
+            x[r].template put<_Float16, 2>((char*)a.tile_rows + (uint64_t)(row0 + row - a.tile_row0) * a.tile_r_pitch, a.tile_r_low, a.tile_dim, k, lane);
+        }
     }
-#pragma unroll
-    for (int i = 0; i < HELD; i++) top = fmaxf(top, largest(held[i]));
-    for (uint32_t at = HELD * 512 + threadIdx.x; at < total; at += 512) top = fmaxf(top, largest(fetch(at)));
-#pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; w++) top = fmaxf(top, buf[w]);
-    const int k = plane_exp(top);
-    if (threadIdx.x == 0) a.row_exp[row0 / 32] = (float)(top > 0.f ? k : EMPTY_EXP);
-    auto put = [&](uint32_t at, f32x4 x) {
-        const uint32_t r = at / d4, d = at % d4 * 4;
-        put_planes<_Float16, 2>((char*)a.tile_rows + (uint64_t)(row0 + r - a.tile_row0) * a.tile_r_pitch + d * 2, a.tile_r_low, x, k);
-    };
-#pragma unroll
-    for (int i = 0; i < HELD; i++) {
-        const uint32_t at = i * 512 + threadIdx.x;
-        if (at < total) put(at, held[i]);
-    }
-    for (uint32_t at = HELD * 512 + threadIdx.x; at < total; at += 512) put(at, fetch(at));
 }
 
 // Rows x queries, rows on the M side: 128 rows a wave (a group), so that a query's maximum and sum over them need one exchange between a
@@ -280,6 +269,7 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
     using ATile = RowTile<S, BM, SF, NW>;
     using BTile = RowTile<S, BN, SF, NW>;
     constexpr int PLANE = ATile::BYTES + BTile::BYTES, STAGE = P * PLANE, PER = P * (ATile::LOADS + BTile::LOADS);
+    constexpr bool SCALED = P == 2 && MODE == TILE_EXP; // the exponentials take the rows' exponents
     __shared__ __align__(1024) char lds[ST * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
     // consecutive workgroups go to the eight XCDs in turn: those of one XCD share a tile of rows, one after the other
@@ -347,16 +337,26 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
     // epilogue: one query a lane (and its other half), 128 rows a wave
     const int h = lane >> 5;
     const uint32_t wrow = row + wm * LOSS_GROUP;
-    float c[4], down[4], e[4] = {}, row_exp = 0.f; // of each 32 rows: from sums to logits in base 2; what brings their exponentials to the group's exponent
+    // planes: what brings a row's sums to the exponent of the largest of the group's rows, as a lane has the rows: a factor, or (SCALED) its logarithm
+    f32x4 down[P == 2 ? 4 : 1][4];
+    float least = 0.f; // that row's exponent
     if constexpr (P == 2) {
+        least = INFINITY;
 #pragma unroll
-        for (int m = 0; m < 4; m++) e[m] = a.row_exp[wrow / 32 + m];
-        row_exp = fminf(fminf(e[0], e[1]), fminf(e[2], e[3]));
-    }
+        for (int m = 0; m < 4; m++)
 #pragma unroll
-    for (int m = 0; m < 4; m++) {
-        c[m] = a.scale * LOG2E;
-        down[m] = P == 2 ? __builtin_amdgcn_exp2f(row_exp - e[m]) : 1.f;
+            for (int k = 0; k < 4; k++) {
+                down[m][k] = *reinterpret_cast<const f32x4*>(a.row_exp + wrow + m * 32 + 8 * k + 4 * h);
+                least = fminf(fminf(fminf(least, down[m][k][0]), fminf(down[m][k][1], down[m][k][2])), down[m][k][3]);
+            }
+        least = fminf(least, __shfl_xor(least, 32));
+#pragma unroll
+        for (int m = 0; m < 4; m++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float l = least - down[m][i >> 2][i & 3];
+                down[m][i >> 2][i & 3] = SCALED ? l : __builtin_amdgcn_exp2f(l);
+            }
     }
     uint32_t words[4];
 #pragma unroll
@@ -365,10 +365,16 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         const uint32_t qi = query + (wn * NT + t) * 32 + (lane & 31);
+        float c = a.scale * LOG2E; // from sums to logits in base 2
         if constexpr (P == 2) {
-            const float own = qi < a.nq ? a.q_exp[qi] : 0.f;
+            c = ldexpf(c, -(int)(least + (qi < a.nq ? a.q_exp[qi] : 0.f)));
 #pragma unroll
-            for (int m = 0; m < 4; m++) c[m] = ldexpf(a.scale * LOG2E, -(int)(e[m] + own));
+            for (int m = 0; m < 4; m++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float d = down[m][i >> 2][i & 3];
+                    acc[m][t][i] = SCALED ? ldexpf(acc[m][t][i], (int)d) : acc[m][t][i] * d;
+                }
         }
         if (!all) {
 #pragma unroll
@@ -390,32 +396,39 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
                 for (int i = 0; i < 16; i++) {
                     const float z = acc[m][t][i];
                     // a query that counts nothing, and a row that is left out, give zero whatever the logit is
-                    p[i] = g == 0.f || z == -INFINITY ? 0.f : g * __builtin_amdgcn_exp2f(__builtin_fmaf(z, c[m], -lw.x));
+                    p[i] = g == 0.f || z == -INFINITY ? 0.f : g * __builtin_amdgcn_exp2f(__builtin_fmaf(z, c, -lw.x));
                 }
 #pragma unroll
                 for (int k = 0; k < BLOCK_PARTS; k++) put_block<GradTiles<T>>(out + m * BLOCK_BYTES + k * 1024 + block_slot(lane & 31, h, k) * 16, a.block_low, p + k * 8);
             }
         } else {
-            float top = -INFINITY;
+            float top = -INFINITY, block_top = -INFINITY;
 #pragma unroll
-            for (int m = 0; m < 4; m++) {
-                float most = -INFINITY;
+            for (int m = 0; m < 4; m++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) most = fmaxf(most, acc[m][t][i]);
-                if (most != -INFINITY) top = fmaxf(top, most * c[m]); // -inf: all left out (and c may be zero)
-            }
+                for (int i = 0; i < 16; i++) {
+                    top = fmaxf(top, acc[m][t][i]);
+                    if constexpr (SCALED) block_top = fmaxf(block_top, __builtin_fmaf(acc[m][t][i], c, down[m][i >> 2][i & 3]));
+                }
             top = fmaxf(top, __shfl_xor(top, 32));
+            if (top != -INFINITY) top *= c; // -inf: all left out (and c may be zero)
             const float ref = top == -INFINITY ? -INFINITY : ceilf(top) - HEADROOM<T>;
             const float less = top == -INFINITY ? 0.f : -ref;
+            float block_ref = ref, block_less = less;
+            if constexpr (SCALED) {
+                block_top = fmaxf(block_top, __shfl_xor(block_top, 32));
+                block_ref = top == -INFINITY ? -INFINITY : ceilf(block_top) - HEADROOM<T>;
+                block_less = top == -INFINITY ? 0.f : -block_ref;
+            }
             float sum = 0.f;
 #pragma unroll
             for (int m = 0; m < 4; m++) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const float z = acc[m][t][i];
-                    p[i] = z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(z, c[m], less));
+                    p[i] = z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(z, c, less));
                     sum += p[i];
-                    if (P == 2 && MODE == TILE_EXP) p[i] *= down[m];
+                    if constexpr (SCALED) p[i] = z == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(__builtin_fmaf(z, c, block_less + down[m][i >> 2][i & 3]));
                 }
                 if constexpr (MODE == TILE_EXP) {
 #pragma unroll
@@ -427,7 +440,7 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
                 const size_t at = (size_t)(wrow / LOSS_GROUP) * a.qp + qi;
                 a.ref[at] = ref;
                 a.sum[at] = sum;
-                if (P == 2 && MODE == TILE_EXP) a.block_ref[at] = ref - row_exp;
+                if constexpr (SCALED) a.block_ref[at] = block_ref - least;
             }
         }
     }
@@ -1441,7 +1454,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.tile_r_low = PLANES == 2 ? piece * a.tile_dim * 2 : 0;
     a.tile_q_low = PLANES == 2 ? (uint64_t)a.qp * a.tile_dim * 2 : 0;
     const size_t o_rows = take(2 * a.tile_r_low), o_q = take(2 * a.tile_q_low), o_gq = take(gx ? 3 * a.tile_q_low : 0), o_bref = take(PLANES == 2 && gq ? (size_t)a.groups * a.qp * 4 : 0);
-    const size_t o_rexp = take((size_t)a.groups * 16), o_qexp = take((size_t)a.qp * 4);
+    const size_t o_rexp = take((size_t)a.groups * LOSS_GROUP * 4), o_qexp = take((size_t)a.qp * 4);
     const size_t o_part = take(gq && !direct ? (size_t)splits * a.qp * a.dim * 4 : 0);
     const size_t o_pr0 = take((size_t)splits * a.qp * 4), o_pr1 = take((size_t)splits * a.qp * 4);
     char* ws = nullptr;
@@ -1477,7 +1490,11 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         if constexpr (PLANES == 2) {
             a.tile_row0 = a.row0;
             // unless the planes are of this piece already; the queries' once
-            if (i != split_piece) loss_split<<<rows / 32 + (split_piece == ~0u ? (a.nq + 7) / 8 : 0), 512, 0, s>>>(a, rows / 32);
+            if (i != split_piece) {
+                const uint32_t grid = rows / 32 + (split_piece == ~0u ? (a.nq + 7) / 8 : 0);
+                if (a.dim <= 1024) loss_split<4><<<grid, 512, 0, s>>>(a, rows / 32);
+                else loss_split<LOSS_MAX_COLUMNS / 256><<<grid, 512, 0, s>>>(a, rows / 32);
+            }
             split_piece = i;
         }
         return rows / LOSS_GROUP;
