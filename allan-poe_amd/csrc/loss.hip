@@ -90,12 +90,15 @@ struct LossArgs {
     const char *tile_rows, *tile_q;
     uint32_t tile_row0, tile_r_pitch, tile_q_pitch, tile_dim; // the first row at tile_rows; bytes; columns with the pad
     uint64_t tile_r_low, tile_q_low, block_low;
-    const char* grad_tile_q;    // q as grad x takes it; (float) the planes lie tile_q_low bytes apart
+    const char* grad_tile_q;    // q as grad x takes it, over the queries' powers of two (fp16), or in planes tile_q_low bytes apart (float)
+    uint32_t grad_tile_q_pitch; // bytes
     float *row_exp, *q_exp;     // planes: exponents of each row and of each query
     float *chunk_ref, *chunk_sum; // [LOSS_CHUNKS][qp]
     float2* lse_w;              // [qp]: lse in base 2, weight W (to be multiplied with exp(s - lse))
     float *coef, *total;        // [qp]: |weight| (|W| + sum |w|); W
     uint32_t *top_coef, *q_on;  // the largest of them, as bits; those that are not zero, as a bit mask
+    float* q_size;              // [qp], for fp16: each query's largest value over its power of two (grad_scale)
+    uint32_t* top_size;         // the largest of them, as bits
     char* blocks;
     float* part;                // [splits][qp][dim]
     float* part_ref[2];         // [splits][qp]
@@ -112,10 +115,20 @@ template <typename T> constexpr float HEADROOM = __is_same(T, __bf16) ? 0.f : 14
 
 enum { TILE_SUMS = 0, TILE_EXP = 1, TILE_GRAD = 2 };
 
-// Power of two that brings the largest coefficient near 2^13: G fits fp16 with room below.
-__device__ inline float grad_scale_of(const uint32_t* top) {
-    const float t = __uint_as_float(*top);
+// Power of two that brings a query's coefficients near 2^13 in G. fp16, whose numbers would not reach from the largest of all queries to what a light
+// one leaves at each row, takes one a query: it is taken out again where the query's own gradient is written, and for the rows' gradients
+// put into the query, times a power of two that is the same for all (scale_of_sizes). The others take that of the largest of all.
+template <typename T> constexpr bool OWN_SCALE = __is_same(T, _Float16);
+template <typename T> __device__ inline float grad_scale(const LossArgs& a, uint32_t qi) {
+    const float t = OWN_SCALE<T> ? a.coef[qi] : __uint_as_float(*a.top_coef);
     return t > 0.f && t < 1e30f && t > 1e-30f ? exp2f(13.f - ceilf(log2f(t))) : 1.f;
+}
+// Exponent that brings the largest of q_size to 2^13 .. 2^14.
+__device__ inline int scale_of_sizes(const LossArgs& a) {
+    const float t = __uint_as_float(*a.top_size);
+    int e = 14;
+    if (t > 0.f) (void)frexpf(t, &e);
+    return 14 - e;
 }
 
 // A value as a sum of P values of type S.
@@ -389,7 +402,7 @@ __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossAr
         char* out = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((wrow - a.row0) >> 5)) * BLOCK_BYTES;
         if constexpr (MODE == TILE_GRAD) {
             const float2 lw = a.lse_w[qi];
-            const float g = lw.y * grad_scale_of(a.top_coef);
+            const float g = lw.y * grad_scale<T>(a, qi);
 #pragma unroll
             for (int m = 0; m < 4; m++) {
 #pragma unroll
@@ -507,12 +520,25 @@ __device__ inline float join_chunks(const LossArgs& a, uint32_t qi, int lane) {
 }
 
 // What the second pass needs of a query, one wave each: lse, and weight W.
-__global__ __launch_bounds__(64) void loss_coefs(LossArgs a) {
+template <typename T> __global__ __launch_bounds__(64) void loss_coefs(LossArgs a) {
     const uint32_t qi = blockIdx.x;
     const int lane = threadIdx.x;
     if (qi >= a.nq) {
-        if (lane == 0) a.lse_w[qi] = make_float2(0.f, 0.f);
+        if (lane == 0) {
+            a.lse_w[qi] = make_float2(0.f, 0.f);
+            a.coef[qi] = 0.f;
+        }
         return;
+    }
+    float size = 0.f;
+    if constexpr (OWN_SCALE<T>) {
+        for (uint32_t d = lane * 8; d < a.dim; d += 512) {
+            const f16x8 x = *reinterpret_cast<const f16x8*>((const char*)a.q + (uint64_t)qi * a.q_pitch + d * 2);
+#pragma unroll
+            for (int k = 0; k < 8; k++) size = fmaxf(size, finite_abs((float)x[k]));
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) size = fmaxf(size, __shfl_xor(size, d));
     }
     const float lse = join_chunks(a, qi, lane);
     const uint32_t e0 = a.t_off[qi], e1 = a.t_off[qi + 1];
@@ -532,27 +558,49 @@ __global__ __launch_bounds__(64) void loss_coefs(LossArgs a) {
         a.lse_w[qi] = make_float2(lse, c * W);
         a.coef[qi] = fabsf(c) * (fabsf(W) + A);
         a.total[qi] = W;
+        if constexpr (OWN_SCALE<T>) a.q_size[qi] = a.coef[qi] != 0.f ? size / grad_scale<T>(a, qi) : 0.f;
     }
 }
 
-// The largest coefficient, and which queries count something (what the others hold is not multiplied), as bits: one workgroup.
-__global__ __launch_bounds__(1024) void loss_queries(LossArgs a) {
-    __shared__ uint32_t top[16];
-    uint32_t most = 0; // of floats that are not negative, as bits
+// The largest coefficient (fp16: the largest size as well), and which queries count something (what the others hold is not multiplied), as bits: one workgroup.
+template <typename T> __global__ __launch_bounds__(1024) void loss_queries(LossArgs a) {
+    constexpr int N = OWN_SCALE<T> ? 2 : 1;
+    __shared__ uint32_t top[N][16];
+    uint32_t most[N] = {}; // of floats that are not negative, as bits
     for (uint32_t q0 = 0; q0 < a.qp; q0 += 1024) {
         const uint32_t qi = q0 + threadIdx.x;
         const uint32_t c = qi < a.nq ? __float_as_uint(a.coef[qi]) : 0;
-        most = max(most, c);
+        most[0] = max(most[0], c);
+        if constexpr (N == 2) most[1] = max(most[1], qi < a.nq ? __float_as_uint(a.q_size[qi]) : 0);
         const unsigned long long b = __ballot(c != 0);
         if ((threadIdx.x & 31) == 0 && qi < a.qp) a.q_on[qi >> 5] = (uint32_t)(b >> (threadIdx.x & 32));
     }
 #pragma unroll
-    for (int d = 32; d; d >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
-    if ((threadIdx.x & 63) == 0) top[threadIdx.x >> 6] = most;
+    for (int n = 0; n < N; n++) {
+#pragma unroll
+        for (int d = 32; d; d >>= 1) most[n] = max(most[n], (uint32_t)__shfl_xor((int)most[n], d));
+        if ((threadIdx.x & 63) == 0) top[n][threadIdx.x >> 6] = most[n];
+    }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int k = 1; k < 16; k++) most = max(most, top[k]);
-        *a.top_coef = most;
+    if (threadIdx.x < N) {
+        uint32_t all = 0;
+        for (int k = 0; k < 16; k++) all = max(all, top[threadIdx.x][k]);
+        (threadIdx.x ? a.top_size : a.top_coef)[0] = all;
+    }
+}
+
+// fp16: the queries as the rows' gradients take them, one wave each. Those that count nothing are not read there.
+__global__ __launch_bounds__(256) void loss_scale_queries(LossArgs a) {
+    const uint32_t qi = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (qi >= a.nq || a.coef[qi] == 0.f) return;
+    int own;
+    (void)frexpf(grad_scale<_Float16>(a, qi), &own); // 2^(own - 1)
+    const int k = scale_of_sizes(a) + 1 - own;
+    for (uint32_t d = (threadIdx.x & 63) * 8; d < a.dim; d += 512) {
+        f16x8 x = *reinterpret_cast<const f16x8*>((const char*)a.q + (uint64_t)qi * a.q_pitch + d * 2);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (_Float16)ldexpf((float)x[i], k);
+        *reinterpret_cast<f16x8*>((char*)a.grad_tile_q + (uint64_t)qi * a.grad_tile_q_pitch + d * 2) = x;
     }
 }
 
@@ -569,7 +617,7 @@ template <typename T> __global__ __launch_bounds__(256) void loss_normalise(Loss
         const uint32_t qi = qb * 32 + (uint32_t)((int)(lane & 31) ^ ((int)(lane >> 5) * 4) ^ (k * 8)); // a slot is its own inverse within a half
         const float ref = a.ref[(size_t)(a.row0 / LOSS_GROUP + g) * a.qp + qi];
         const float2 lw = a.lse_w[qi];
-        const float c = lw.y * grad_scale_of(a.top_coef);
+        const float c = lw.y * grad_scale<T>(a, qi);
         f[k] = c == 0.f || ref == -INFINITY ? 0.f : c * __builtin_amdgcn_exp2f(ref - lw.x);
     }
     typedef T t8 __attribute__((ext_vector_type(8)));
@@ -602,7 +650,7 @@ template <typename T, bool ALL> __global__ __launch_bounds__(64) void loss_targe
     const int lane = threadIdx.x;
     const uint32_t e0 = a.t_off[qi], e1 = a.t_off[qi + 1];
     const float2 lw = a.lse_w[qi];
-    const float gs = grad_scale_of(a.top_coef), cw = a.weight ? a.weight[qi] : 1.f;
+    const float gs = grad_scale<T>(a, qi), cw = a.weight ? a.weight[qi] : 1.f;
     float at = 0.f;
     for (uint32_t e = e0; e < e1; e++) {
         const uint32_t t = a.t_idx[e];
@@ -803,7 +851,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void loss_grad_q(LossArgs a, 
         __syncthreads();
     }
     const int h = lane >> 5;
-    const float back = DIRECT ? a.scale / grad_scale_of(a.top_coef) : 1.f;
+    const float all_back = DIRECT && !OWN_SCALE<T> ? a.scale / grad_scale<T>(a, 0) : 1.f;
 #pragma unroll
     for (int m = 0; m < MT; m++) {
         if (KG == 2 && m / (MT / 2) != kg) continue;
@@ -814,6 +862,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void loss_grad_q(LossArgs a, 
             if constexpr (DIRECT) {
                 const bool on = (a.q_on[(query + r) >> 5] >> (r & 31)) & 1;
                 T* to = reinterpret_cast<T*>((char*)a.grad_q + (uint64_t)(query + r) * a.gq_pitch);
+                const float back = OWN_SCALE<T> ? a.scale / grad_scale<T>(a, query + r) : all_back;
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     const uint32_t d = col + (wn * NT + t) * 32 + (lane & 31);
@@ -864,7 +913,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void loss_grad_x(LossArgs a, 
     const uint64_t astep = (uint64_t)a.row_blocks * BLOCK_BYTES;
     BTile tb[P];
 #pragma unroll
-    for (int p = 0; p < P; p++) tb[p].init(reinterpret_cast<const S*>(a.grad_tile_q + p * a.tile_q_low) + col, a.tile_q_pitch, (int)min((uint32_t)BN, a.tile_dim - col), wave, lane);
+    for (int p = 0; p < P; p++) tb[p].init(reinterpret_cast<const S*>(a.grad_tile_q + p * a.tile_q_low) + col, a.grad_tile_q_pitch, (int)min((uint32_t)BN, a.tile_dim - col), wave, lane);
     const UniformWords q_on = (UniformWords)a.q_on;
     const int stages = (int)((a.nq + 31) / 32);
     const uint32_t base = lds_address(lds);
@@ -932,7 +981,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void loss_grad_x(LossArgs a, 
         static_assert(BM * BN * 4 <= ST * STAGE, "the sums fit the stages");
         exchange_halves<MT, NT, WM * WN>(acc, lds, kg, wave % (WM * WN), lane);
     }
-    const float back = a.scale / grad_scale_of(a.top_coef);
+    const float back = OWN_SCALE<T> ? ldexpf(a.scale, -scale_of_sizes(a)) : a.scale / grad_scale<T>(a, 0);
     const int h = lane >> 5;
 #pragma unroll
     for (int m = 0; m < MT; m++) {
@@ -1044,7 +1093,7 @@ template <typename T, bool GRAD, bool EXP, int THREADS> __global__ __launch_boun
             if (g) acc[0] = f32x4{};
         }
         if constexpr (!EXP) {
-            const float gs = 1.f / grad_scale_of(a.top_coef);
+            const float gs = 1.f / grad_scale<T>(a, qi);
 #pragma unroll
             for (int k = 0; k < C; k++) acc[k] *= gs;
         }
@@ -1448,12 +1497,12 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     };
     const size_t o_ref = take((size_t)a.groups * a.qp * 4), o_sum = take((size_t)a.groups * a.qp * 4);
     const size_t o_cr = take((size_t)a.chunks * a.qp * 4), o_cs = take((size_t)a.chunks * a.qp * 4);
-    const size_t o_lw = take((size_t)a.qp * 8), o_top = take(4), o_on = take(a.qp / 8), o_coef = take((size_t)a.qp * 4), o_total = take((size_t)a.qp * 4);
+    const size_t o_lw = take((size_t)a.qp * 8), o_top = take(8), o_size = take(OWN_SCALE<T> ? (size_t)a.qp * 4 : 0), o_on = take(a.qp / 8), o_coef = take((size_t)a.qp * 4), o_total = take((size_t)a.qp * 4);
     a.block_low = (size_t)a.qp * piece * 2;
     const size_t o_blocks = take(gx ? GradTiles<T>::PLANES * a.block_low : gq ? PLANES * a.block_low : 0);
     a.tile_r_low = PLANES == 2 ? piece * a.tile_dim * 2 : 0;
     a.tile_q_low = PLANES == 2 ? (uint64_t)a.qp * a.tile_dim * 2 : 0;
-    const size_t o_rows = take(2 * a.tile_r_low), o_q = take(2 * a.tile_q_low), o_gq = take(gx ? 3 * a.tile_q_low : 0), o_bref = take(PLANES == 2 && gq ? (size_t)a.groups * a.qp * 4 : 0);
+    const size_t o_rows = take(2 * a.tile_r_low), o_q = take(2 * a.tile_q_low), o_gq = take(!gx ? 0 : PLANES == 2 ? 3 * a.tile_q_low : OWN_SCALE<T> ? (size_t)a.qp * a.dim * 2 : 0), o_bref = take(PLANES == 2 && gq ? (size_t)a.groups * a.qp * 4 : 0);
     const size_t o_rexp = take((size_t)a.groups * LOSS_GROUP * 4), o_qexp = take((size_t)a.qp * 4);
     const size_t o_part = take(gq && !direct ? (size_t)splits * a.qp * a.dim * 4 : 0);
     const size_t o_pr0 = take((size_t)splits * a.qp * 4), o_pr1 = take((size_t)splits * a.qp * 4);
@@ -1465,6 +1514,8 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.chunk_sum = (float*)(ws + o_cs);
     a.lse_w = (float2*)(ws + o_lw);
     a.top_coef = (uint32_t*)(ws + o_top);
+    a.top_size = a.top_coef + 1;
+    a.q_size = (float*)(ws + o_size);
     a.blocks = ws + o_blocks;
     a.part = (float*)(ws + o_part);
     a.part_ref[0] = (float*)(ws + o_pr0);
@@ -1477,9 +1528,10 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.block_ref = PLANES == 2 ? (float*)(ws + o_bref) : a.ref;
     a.tile_rows = PLANES == 2 ? ws + o_rows : (const char*)a.rows;
     a.tile_q = PLANES == 2 ? ws + o_q : (const char*)a.q;
-    a.grad_tile_q = PLANES == 2 ? ws + o_gq : a.tile_q;
+    a.grad_tile_q = PLANES == 2 || OWN_SCALE<T> ? ws + o_gq : a.tile_q;
     a.tile_r_pitch = PLANES == 2 ? a.tile_dim * 2 : a.r_pitch;
     a.tile_q_pitch = PLANES == 2 ? a.tile_dim * 2 : a.q_pitch;
+    a.grad_tile_q_pitch = OWN_SCALE<T> ? a.dim * 2 : a.tile_q_pitch;
     hipStream_t s = ctx->stream;
     uint32_t split_piece = ~0u;
     auto set_piece = [&](uint32_t i) {
@@ -1575,8 +1627,9 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
         }
     }
     if (gx) {
-        loss_coefs<<<a.qp, 64, 0, s>>>(a);
-        loss_queries<<<1, 1024, 0, s>>>(a);
+        loss_coefs<T><<<a.qp, 64, 0, s>>>(a);
+        loss_queries<T><<<1, 1024, 0, s>>>(a);
+        if constexpr (OWN_SCALE<T>) loss_scale_queries<<<(a.nq + 3) / 4, 256, 0, s>>>(a);
         // grad x: tiles of 256 rows x 256 columns, or of 128 x 128 where those do not fill the GPU, and for float
         const bool x_wide = PLANES == 1 && (uint64_t)((piece + 255) / 256) * ((a.dim + 255) / 256) >= cus;
         const uint32_t xm = x_wide ? 256 : 128, x_tiles = (a.dim + xm - 1) / xm;

@@ -1,9 +1,9 @@
-"""The softmax loss on inputs of very uneven sizes (needs the GPU): rows of zeros between others, rows far larger than their
-neighbours. Against the formula in 64 bits; tolerances as in test_gpu_softmax_loss.py, unless a test derives its own."""
+"""The softmax loss on inputs of very uneven sizes (needs the GPU): rows of zeros between others, rows far larger than their neighbours,
+queries whose weights are far apart. Against the formula in 64 bits; tolerances as in test_gpu_softmax_loss.py, unless a test derives its own."""
 import numpy as np
 import pytest
 
-from test_gpu_softmax_loss import check, make, oracle
+from test_gpu_softmax_loss import U, check, make, oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +72,63 @@ def test_a_large_row_costs_its_neighbours_nothing(gpu_ctx, size, grad_rows):
     a["rows"] = x.cuda()
     assert float((a["queries"] @ v.cuda()).min()) > 0.2  # every query's logit of those rows is far below the others'
     close_by_row(gpu_ctx, a, grad_rows)
+
+
+@pytest.mark.parametrize("m", [70, 300])
+@pytest.mark.parametrize("apart", [2.0 ** 8, 2.0 ** 22])
+@pytest.mark.parametrize("grad_queries", [True, False])
+def test_weights_far_apart(gpu_ctx, m, apart, grad_queries):
+    """float16, both gradients, one query that weighs 2^22 times what the others do and finds its row, so that it leaves nothing elsewhere. Tolerances:
+    a query's weight is taken as 2^11 to 2^12 (with its targets' beside it 2^13), so what is lost among the subnormal numbers, 2^-25 for each row, is
+    2^-36 of it; the products take queries times their weights, the largest value as 2^13 to 2^14: 2^-38 of it is lost."""
+    import apoe
+    import torch
+    g = torch.Generator().manual_seed(m)
+    n, d, scale = 20_000, 64, 4.0
+    v = torch.randn(d, generator=g)
+    x = torch.randn(n, d, generator=g) / d ** 0.5 + v / v.norm()  # around one direction, so that the rows' mean is no small part
+    x /= x.norm(dim=1, keepdim=True)
+    idx = torch.randint(0, n, (m,), generator=g)
+    q = torch.randn(m, d, generator=g) / d ** 0.5
+    q[0] = 40 * (x[idx[0]] - v / v.norm())
+    weight = torch.full((m,), 2.0 ** 14 / apart)
+    weight[0] = 2.0 ** 14
+    a = dict(queries=q.half().cuda(), rows=x.half().cuda(), t_off=torch.arange(m + 1, dtype=torch.int32).cuda(), t_idx=idx.int().cuda(), t_val=None,
+             scale=scale, live=None, weight=weight.cuda())
+    got = apoe.softmax_loss(gpu_ctx, **a, grad_queries=grad_queries, grad_rows=True)
+    q, x, cw = (a[k].cpu().double().numpy() for k in ("queries", "rows", "weight"))
+    z = scale * q @ x.T
+    z -= z.max(1, keepdims=True)
+    p = np.exp(z) / np.exp(z).sum(1, keepdims=True)
+    c = (cw * scale)[:, None]
+    w = np.zeros((m, n))
+    w[np.arange(m), idx.numpy()] = 1
+    G, mass, u = c * (p - w), c * (p + w), U["float16"]
+    logit = scale * (d + 4) * 2.0 ** -24 * (np.abs(q) @ np.abs(x).T).max(1, keepdims=True)
+    noise = (2 * u + 4 * logit + 2.0 ** -20 + (n + m) * 2.0 ** -24) * mass + 2.0 ** -36 * c
+    if grad_queries:
+        want = G @ x
+        tol = noise @ np.abs(x) + u * np.abs(want) + 2.0 ** -24
+        err = np.abs(got["grad_queries"].double().cpu().numpy() - want)
+        assert (err <= tol).all(), float((err / tol).max())
+    want = G.T @ q
+    top = (c * np.abs(q).max(1, keepdims=True)).max()
+    tol = noise.T @ np.abs(q) + 2.0 ** -38 * top * (mass / c).sum(0)[:, None] + u * np.abs(want) + 2.0 ** -24
+    err = np.abs(got["grad_rows"].double().cpu().numpy() - want)
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+def test_the_queries_gradient_is_as_good_beside_the_rows(gpu_ctx):
+    """float16, weights 2^20 apart: grad_queries with grad_rows against grad_queries alone, each against 64 bits, query by query."""
+    import apoe
+    import torch
+    a = make(80, 5000, 64, "float16", seed=3, targets=2, scale=1.0)
+    a["weight"] = torch.where(torch.arange(80) % 2 == 0, 2.0 ** 12, 2.0 ** -8).cuda()
+    want = oracle(a)[0]["grad_queries"]
+    some = np.abs(want).max(1) > 0
+    err = {}
+    for rows in (False, True):
+        got = apoe.softmax_loss(gpu_ctx, **a, grad_queries=True, grad_rows=rows)["grad_queries"].double().cpu().numpy()
+        err[rows] = (np.linalg.norm(got - want, axis=1)[some] / np.linalg.norm(want, axis=1)[some])
+    # a second rounding of the coefficients, 2^-11 each, beside the result's: sqrt(3 / 2) and what is left to chance
+    assert (err[True] <= 1.5 * err[False] + 2.0 ** -11 / 3 ** 0.5).all(), float((err[True] / err[False]).max())
