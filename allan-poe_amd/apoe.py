@@ -596,7 +596,8 @@ def softmax_loss(ctx, queries, rows, t_off, t_idx, t_val=None, scale=1.0, weight
 
 def orthogonalize(ctx, x, out=None, steps=5, coefs=COEFS, alpha=1.0, beta=0.0, products=None):
     """out = alpha NS(x) + beta out for a matrix or a batch of matrices: the Newton-Schulz steps that bring x's singular values to
-    about one. products: "f16" (1e-4 to 6e-4 of the result; a short side of up to 64 is exact to 1e-6 either way) or "f32"; by default "f16" where out is bfloat16."""
+    about one. products: "f16" (1e-4 to 6e-4 of the result; a short side of up to 64 is exact to 1e-6 either way) or "f32"; by default "f16" where out is bfloat16.
+    Coefficients under which an entry of X, A or (off its diagonal) b A + c A A passes 15 give a result that is not finite."""
     if x.dim() not in (2, 3):
         raise ApoeError(f"x must be a matrix or a batch of matrices, not {tuple(x.shape)}")
     in_dtype = _dtype(x, "x")

@@ -8,7 +8,7 @@
 // as two fp16 matrices, its rounded value and what that left (22 bits together; kept in fp32 beside an fp16 copy, the errors below are
 // the same in two digits, and the traffic of B X half as much again: 4 x 1024 x 4096 625 us for 595), and the products take fp16
 // copies of X (the high part), A and B, all times 2^12: X and A are about one at most, their small values stay clear of the subnormal
-// numbers; B's diagonal, which is its largest part when all singular values are alike, stays in 32 bits and scales X's rows outside
+// numbers (an entry of 16 would be infinite, in any of the three, and so would be the result); B's diagonal, which is its largest part when all singular values are alike, stays in 32 bits and scales X's rows outside
 // the product. That leaves 1e-4 to 6e-4 (fp16 rounds its result by 2e-4, bf16 by 17e-4), less the longer the sides are, over which
 // the roundings average.
 // SPLIT, for results in 32 bits, for fp16 ones and (ortho_narrow) for short sides, where nothing averages: X in fp32, every operand two fp16 matrices,

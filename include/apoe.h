@@ -357,8 +357,9 @@ typedef struct {
 
 /*
  * Newton-Schulz: X = in / |in| (Frobenius; a zero matrix stays zero), then `steps` times X = a X + (b A + c A A) X with A = X X^T,
- * on the short side, which drives the singular values towards one. Coefficients under which an entry of X passes 15 are beyond it
- * (the result is then not finite). Any sizes and alignments of rows are taken.
+ * on the short side, which drives the singular values towards one. The products hold entries of X, of A and, off its diagonal, of b A + c A A
+ * up to 15: coefficients under which one passes that (as A does once a singular value of X passes 4) are beyond it, and the
+ * result is then not finite. Any sizes and alignments of rows are taken.
  */
 int apoe_orthogonalize(apoe_ctx* ctx, const apoe_orthogonalize_args* args);
 

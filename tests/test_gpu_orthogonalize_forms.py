@@ -56,3 +56,23 @@ def test_added_into_what_is_there(gpu_ctx, batch, rows, cols, pad, out, products
     want = 0.5 * r - old
     u = {"float16": 2.0 ** -11, "bfloat16": 2.0 ** -8, "float32": 2.0 ** -24}[out]
     assert got is w and norm(w.double() - want) < 0.5 * limit("float32", products) * norm(r) + 2 * u * norm(want)
+
+
+@pytest.mark.parametrize("products", ["f16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(40, 200), (100, 200), (700, 900)])
+def test_coefficients_that_pass_the_products_range_give_no_number(gpu_ctx, rows, cols, products):
+    """X grows past a norm of 4, or b A passes 15 off its diagonal: nothing finite comes out that could be taken for a result. Within the
+    range, large coefficients are as good as others."""
+    import torch
+    import apoe
+    g = torch.Generator().manual_seed(1)
+    # one direction, half of whose entries differ in sign: A's entries are 1 / rows, or 1 / 2 between two rows that are all there is
+    x = torch.zeros(rows, cols)
+    x[3], x[7] = torch.ones(cols), torch.ones(cols)
+    x = x.cuda()
+    assert not bool(apoe.orthogonalize(gpu_ctx, x, coefs=(8.0, 0.0, 0.0), products=products).isfinite().all())
+    assert not bool(apoe.orthogonalize(gpu_ctx, x, steps=1, coefs=(1.0, -40.0, 0.0), products=products).isfinite().all())
+    y = (x.cpu() + 0.1 * torch.randn(rows, cols, generator=g)).cuda()
+    got = apoe.orthogonalize(gpu_ctx, y, steps=1, coefs=(1.0, -28.0, 27.0), products=products)
+    want = reference(y, 1, (1.0, -28.0, 27.0))
+    assert norm(got.double() - want) / norm(want) < 28 * limit("float32", products)
