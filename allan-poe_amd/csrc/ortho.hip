@@ -1106,8 +1106,10 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
     //  symmetric products from half as many tiles of 256 as CUs on: 256, or 192 on twelve waves where the rounds over the CUs times a
     //    tile's size (and a seventh, which the smaller one is slower by) are less (4096 x 4096: 253 tiles of 192 for 136 of 256, X X^T 84 us
     //    for 106, the whole 1.53 ms for 1.80; 4608: 300 for 171, 2.86 ms for 2.62)
-    //  128: from as many tiles as CUs on; for X X^T from half as many, where the rows are long (4 x 1024 x 4096: 40 us; 64: 53), there
-    //    with the waves in two groups that take half of a stage each: larger pieces a wave, fewer reads (45 us in the run of the whole, 51)
+    //  128: from as many tiles as CUs on; from half as many where the inner side is long enough, there with the waves in two groups that take
+    //    half of a stage each: larger pieces a wave, fewer reads (X X^T of 4 x 1024 x 4096: 45 us in the run of the whole, 51 with one group, 53 on
+    //    tiles of 64). From 512 on (the whole, with them and on tiles of 64: 25 x 300 x 400 165 us for 153, 14 x 500 x 600 192 for 206, 5 x 900 x 1300
+    //    284 for 328, 2500 x 2500 546 for 714; SPLIT 281 for 268, 370 for 392, 590 for 649, 1282 for 1584)
     //  64: below (1024 x 1024: X X^T 9 us; 128: 12)
     //  B X: 256 where those fill the GPU and the inner side is long enough to hide the end of a tile, whose traffic the next one does not
     //    overlap (the whole: 4096 x 8192 2.62 ms for 2.98, 8192 x 8192 11.0 for 12.4; 4 x 1024 x 4096 0.575 for 0.541), 128, 64
@@ -1135,7 +1137,7 @@ template <bool SPLIT> static int run_ortho(apoe_ctx* ctx, const apoe_orthogonali
                 return;
             }
         }
-        if (s128 < cus && s128 >= cus / 2 && inner >= 4096) ortho_tile<SPLIT, 2, 2, 2, 2, 2, SPLIT ? 2 : 4, 4, K><<<dim3(triangle(tiles(a.m, 128)), batch), 512, 0, s>>>(a);
+        if (s128 < cus && s128 >= cus / 2 && inner >= 512) ortho_tile<SPLIT, 2, 2, 2, 2, 2, SPLIT ? 2 : 4, 4, K><<<dim3(triangle(tiles(a.m, 128)), batch), 512, 0, s>>>(a);
         else if (s128 >= cus) ortho_tile<SPLIT, 2, 1, 2, 4, 1, 4, 2, K><<<dim3(triangle(tiles(a.m, 128)), batch), 512, 0, s>>>(a);
         else {
             small(kind, triangle(tiles(a.m, 64)) * (K == ORTHO_GRAM ? a.cuts : 1));

@@ -40,6 +40,18 @@ def test_products_of_22_bits_on_large_tiles(gpu_ctx, batch, rows, cols, pad, dty
         assert norm(got[i].double() - want) / norm(want) < limit(dtype, "f32"), i
 
 
+# symmetric products on 128 x 128 tiles in two groups of waves, both of them or X X^T alone (A A of a shorter side on tiles of 64)
+@pytest.mark.parametrize("products", ["f16", "f32"])
+@pytest.mark.parametrize("batch,rows,cols,pad", [(14, 513, 600, 0), (5, 900, 1300, 1), (5, 1301, 897, 0), (1, 2500, 2500, 1), (25, 300, 530, 0), (25, 300, 400, 0), (4, 1024, 1024, 0)])
+def test_tiles_in_two_groups(gpu_ctx, batch, rows, cols, pad, products):
+    import apoe
+    x = matrix(rows, cols, "float32", 6, batch=batch, pad=pad)
+    got = apoe.orthogonalize(gpu_ctx, x, products=products)
+    for i in {0, batch // 2, batch - 1}:
+        want = reference(x[i])
+        assert norm(got[i].double() - want) / norm(want) < limit("float32", products), i
+
+
 @pytest.mark.parametrize("products", ["f16", "f32"])
 @pytest.mark.parametrize("out", ["float16", "bfloat16", "float32"])
 @pytest.mark.parametrize("batch,rows,cols,pad", [(1, 2100, 2104, 0), (1, 2105, 2100, 1), (1, 900, 903, 1), (1, 300, 4100, 0)])
