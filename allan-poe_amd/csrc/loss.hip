@@ -1441,8 +1441,11 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.grad_x = p->grad_rows;
     if (a.nq <= FEW_QUERIES<T> && a.dim <= FEW_MAX_DIM && !gx) return run_few<T>(ctx, a, gq);
     // Tiles of rows x queries (times at 1024 columns, fp16, with the exponentials written):
-    //   256 x 256  where they fill the GPU and the queries they pad beyond what 128 would cost less than they gain (1024 x 65 536: 130 us,
-    //              256 x 128: 150; float, 1024 x 100 000: 610 us, 896 on 128 x 128: 700)
+    //   256 x 256  where they fill the GPU and the queries they pad beyond what 128 would cost less than they gain (1024 x 65 536: 130 us, 256 x 128:
+    //              150), up to an eighth: 1100 x 100 000 without gradient 244 us for 259 with 1.11 times the queries, 777 205 for 199 with 1.14 times.
+    //              float without gradient up to 1.3 times: 600 x 100 000 (1.2 times) 555 us for 578 on 128 x 128, 384 (1.33) 460 for 429; with one,
+    //              whose product is padded alike, an eighth too: 1100 x 60 000 1.17 ms for 1.20, 896 x 50 000 (1.14) 822 us for 797, 600 650 for 589,
+    //              with both 1310 for 1244
     //   256 x 128  where those fill it (128 x 131 072: 56 us; 128 x 128: 66)
     //   128 x 128  for fewer rows (1024 x 4000: 16.5 us; 256 x 128: 20)
     //   128 x 64   up to 64 queries (64 x 30 000: 15.5 us; 128 x 128: 17), 512 x 32 for up to 32 where those fill it (32 x 131 072: 44 us; 48)
@@ -1453,7 +1456,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     auto count = [&](uint32_t rows, uint32_t queries) { return (uint64_t)((a.n + rows - 1) / rows) * ((a.nq + queries - 1) / queries); };
     if (PLANES == 1 && a.nq <= 32 && count(512, 32) >= cus) form = T512_32;
     else if (a.nq <= 64) form = T128_64;
-    else if (count(256, 256) >= cus && up(a.nq, 256) * 40 < up(a.nq, 128) * (PLANES == 2 ? 52 : 45)) form = T256;
+    else if (count(256, 256) >= cus && up(a.nq, 256) * 40 < up(a.nq, 128) * (PLANES == 2 && !gq && !gx ? 52 : 45)) form = T256;
     else if (PLANES == 1 && count(256, 128) >= cus) form = T256_128;
     else form = T128;
     const uint32_t bm = form == T512_32 ? 512 : form == T128 || form == T128_64 ? 128 : 256;
