@@ -14,9 +14,10 @@
 //     over memory: 38 us for 2048 x 30 522, forming the logits again 150 us); otherwise the logits are formed again once lse is known.
 // The targets' own terms are not left to the rounded blocks: their places are zeroed (or rewritten) and W p_t - w_t, which
 // nearly cancels for a query that is served well, is formed in 32 bits.
-// Exponentials (or G) in 16 bits are what the 16-bit products take; a second part of each would double the gradients' products. Against a
-// gradient formed in 32 bits and rounded once the error is 1.2 times as large for many queries (4096 x 4096 bf16: 0.0021 for 0.0017), and
-// 1.5 to 1.8 times for the rows' gradients of a few queries, where one rounded weight of a target is most of a row (0.0030 for 0.0017).
+// Exponentials (or G) in 16 bits are what the 16-bit products take; a second part of each would double the gradients' products. What it costs, against a
+// gradient formed in 32 bits and rounded once: nothing in the queries' gradient (0.00166 and 0.00166 at 4096 x 4096 bf16), where the other rows' roundings
+// average, the second one of G (its exponentials were rounded before) too, and what the targets' would do is added in 32 bits (loss_targets); in the
+// rows' gradients, where a rounded target is most of a row, 1.25 times at 4096 x 4096 (0.00206 for 0.00166) and 1.5 times for 100 queries of 4000 rows.
 #include "apoe_internal.h"
 #include "apoe_tile.h"
 
@@ -101,6 +102,7 @@ struct LossArgs {
     uint32_t* top_size;         // the largest of them, as bits
     char* blocks;
     float* part;                // [splits][qp][dim]
+    float* fix;                 // [qp][dim], with G: the targets' terms that rounding took out of G; behind the last split
     float* part_ref[2];         // [splits][qp]
     float *loss, *lse;
     void *grad_q, *grad_x;
@@ -634,24 +636,20 @@ template <typename T> __global__ __launch_bounds__(256) void loss_normalise(Loss
     }
 }
 
-template <typename T> __device__ inline float dot16(const char* x, const char* y) { // of 16 bytes each
-    typedef T tv __attribute__((ext_vector_type(16 / sizeof(T))));
-    const tv u = *reinterpret_cast<const tv*>(x), v = *reinterpret_cast<const tv*>(y);
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16 / (int)sizeof(T); i++) s = __builtin_fmaf((float)u[i], (float)v[i], s);
-    return s;
-}
-
 // Second pass: the targets' places in this piece's G, formed in 32 bits; one wave a query. ALL: the piece holds all rows and no
-// kernel behind this one adds anything, so it writes the loss.
-template <typename T, bool ALL> __global__ __launch_bounds__(64) void loss_targets(LossArgs a) {
+// kernel behind this one adds anything, so it writes the loss. FIX: what the places' rounding leaves of a query's targets, which are most of its
+// gradient, times their rows: the queries' gradient adds it up beside the product (4096 x 4096 bf16, off by 0.00166 for 0.00210; the result's
+// own rounding is 0.00166). The rows' gradients would need it by row, and go without.
+template <typename T, bool ALL, bool FIX, int COLUMNS> __global__ __launch_bounds__(64) void loss_targets(LossArgs a, int first_piece) {
+    constexpr int V = 16 / (int)sizeof(T), C = COLUMNS / (64 * V);
+    typedef T tv __attribute__((ext_vector_type(V)));
     const uint32_t qi = blockIdx.x, end = min(a.row0 + a.row_blocks * 32, a.n);
     const int lane = threadIdx.x;
     const uint32_t e0 = a.t_off[qi], e1 = a.t_off[qi + 1];
     const float2 lw = a.lse_w[qi];
     const float gs = grad_scale<T>(a, qi), cw = a.weight ? a.weight[qi] : 1.f;
-    float at = 0.f;
+    const char* q = (const char*)a.q + (uint64_t)qi * a.q_pitch;
+    float at = 0.f, fix[FIX ? C : 1][V] = {};
     for (uint32_t e = e0; e < e1; e++) {
         const uint32_t t = a.t_idx[e];
         if (t < a.row0 || t >= end || !is_live(a, t)) continue;
@@ -666,19 +664,49 @@ template <typename T, bool ALL> __global__ __launch_bounds__(64) void loss_targe
         if (__any(!first)) continue;
         float dot = 0.f;
         const char* x = (const char*)a.rows + (uint64_t)t * a.r_pitch;
-        const char* q = (const char*)a.q + (uint64_t)qi * a.q_pitch;
-        for (uint32_t b = lane * 16; b < a.dim * sizeof(T); b += 1024) dot += dot16<T>(q + b, x + b);
+        tv held[C];
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const uint32_t d = (c * 64 + lane) * V;
+            if (d >= a.dim) continue;
+            held[c] = *reinterpret_cast<const tv*>(x + d * sizeof(T));
+            const tv u = *reinterpret_cast<const tv*>(q + d * sizeof(T));
+#pragma unroll
+            for (int v = 0; v < V; v++) dot = __builtin_fmaf((float)u[v], (float)held[c][v], dot);
+        }
 #pragma unroll
         for (int d = 32; d; d >>= 1) {
             dot += __shfl_xor(dot, d);
             w += __shfl_xor(w, d);
         }
         if (w != 0.f) at = __builtin_fmaf(w, dot * a.scale, at);
+        const float p = exp2f(__builtin_fmaf(dot, a.scale * LOG2E, -lw.x));
+        const float g = cw == 0.f ? 0.f : gs * (lw.y * p - cw * w);
         if (lane == 0) {
-            const float p = exp2f(__builtin_fmaf(dot, a.scale * LOG2E, -lw.x));
-            const float g = cw == 0.f ? 0.f : gs * (lw.y * p - cw * w);
             char* block = a.blocks + ((size_t)(qi >> 5) * a.row_blocks + ((t - a.row0) >> 5)) * BLOCK_BYTES;
             put_value<GradTiles<T>>(block + block_place(qi & 31, (t - a.row0) & 31), a.block_low, g);
+        }
+        if constexpr (FIX) {
+            const float left = g - (float)(T)g;
+#pragma unroll
+            for (int c = 0; c < C; c++)
+                if ((uint32_t)(c * 64 + lane) * V < a.dim) {
+#pragma unroll
+                    for (int v = 0; v < V; v++) fix[c][v] = __builtin_fmaf(left, (float)held[c][v], fix[c][v]);
+                }
+        }
+    }
+    if constexpr (FIX) {
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const uint32_t d = (c * 64 + lane) * V;
+            if (d >= a.dim) continue;
+            f32x4* to = reinterpret_cast<f32x4*>(a.fix + (size_t)qi * a.dim + d);
+#pragma unroll
+            for (int k = 0; k < V / 4; k++) {
+                const f32x4 v = {fix[c][4 * k], fix[c][4 * k + 1], fix[c][4 * k + 2], fix[c][4 * k + 3]};
+                to[k] = first_piece ? v : to[k] + v;
+            }
         }
     }
     if (ALL && lane == 0) {
@@ -833,6 +861,20 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void loss_grad_q(LossArgs a, 
         interleave<P * (MT + 2 * NT), PRODUCTS<Tiles<T>> * MT * NT, SF>();
         from = from + KG * STAGE == ST * STAGE ? 0 : from + KG * STAGE;
     }
+    float fix[DIRECT ? MT / KG : 1][16][NT]; // asked for together, before the last loads are waited for (4096 x 4096: 51 us; one by one beside the stores 57, without it 50)
+    if constexpr (DIRECT) {
+#pragma unroll
+        for (int m = 0; m < MT / KG; m++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const uint32_t qi = query + (wm * MT + kg * (MT / KG) + m) * 32 + result_row(i, lane >> 5);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    const uint32_t d = col + (wn * NT + t) * 32 + (lane & 31);
+                    fix[m][i][t] = qi < a.nq && d < a.dim ? a.fix[(size_t)qi * a.dim + d] : 0.f;
+                }
+            }
+    }
     tile_wait<0>();
     if constexpr (KG == 2) {
         static_assert(BM * BN * 4 <= ST * STAGE, "the sums fit the stages");
@@ -866,7 +908,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void loss_grad_q(LossArgs a, 
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     const uint32_t d = col + (wn * NT + t) * 32 + (lane & 31);
-                    if (d < a.dim) to[d] = (T)(on ? acc[m][t][i] * back : 0.f);
+                    if (d < a.dim) to[d] = (T)(on ? (acc[m][t][i] + fix[m % (MT / KG)][i][t]) * back : 0.f);
                 }
                 continue;
             }
@@ -1507,7 +1549,8 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.tile_q_low = PLANES == 2 ? (uint64_t)a.qp * a.tile_dim * 2 : 0;
     const size_t o_rows = take(2 * a.tile_r_low), o_q = take(2 * a.tile_q_low), o_gq = take(!gx ? 0 : PLANES == 2 ? 3 * a.tile_q_low : OWN_SCALE<T> ? (size_t)a.qp * a.dim * 2 : 0), o_bref = take(PLANES == 2 && gq ? (size_t)a.groups * a.qp * 4 : 0);
     const size_t o_rexp = take((size_t)a.groups * LOSS_GROUP * 4), o_qexp = take((size_t)a.qp * 4);
-    const size_t o_part = take(gq && !direct ? (size_t)splits * a.qp * a.dim * 4 : 0);
+    const size_t part_bytes = gq && !direct ? (size_t)splits * a.qp * a.dim * 4 : 0;
+    const size_t o_part = take(part_bytes + (PLANES == 1 && gq && gx ? (size_t)a.qp * a.dim * 4 : 0));
     const size_t o_pr0 = take((size_t)splits * a.qp * 4), o_pr1 = take((size_t)splits * a.qp * 4);
     char* ws = nullptr;
     APOE_TRY(ctx->adapt_workspace(bytes, &ws));
@@ -1521,6 +1564,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.q_size = (float*)(ws + o_size);
     a.blocks = ws + o_blocks;
     a.part = (float*)(ws + o_part);
+    a.fix = (float*)(ws + o_part + part_bytes);
     a.part_ref[0] = (float*)(ws + o_pr0);
     a.part_ref[1] = (float*)(ws + o_pr1);
     a.q_on = (uint32_t*)(ws + o_on);
@@ -1645,8 +1689,16 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
             } else {
                 tiles(Grad{});
             }
-            if (whole) loss_targets<T, true><<<a.nq, 64, 0, s>>>(a);
-            else loss_targets<T, false><<<a.nq, 64, 0, s>>>(a);
+            const bool fix = PLANES == 1 && gq;
+            auto targets = [&](auto columns) { // up to how many a wave holds
+                constexpr int N = decltype(columns)::value;
+                if (whole && fix) loss_targets<T, true, PLANES == 1, N><<<a.nq, 64, 0, s>>>(a, i == 0);
+                else if (whole) loss_targets<T, true, false, N><<<a.nq, 64, 0, s>>>(a, i == 0);
+                else if (fix) loss_targets<T, false, PLANES == 1, N><<<a.nq, 64, 0, s>>>(a, i == 0);
+                else loss_targets<T, false, false, N><<<a.nq, 64, 0, s>>>(a, i == 0);
+            };
+            if (a.dim <= 1024) targets(std::integral_constant<int, 1024>{});
+            else targets(std::integral_constant<int, (int)LOSS_MAX_COLUMNS>{});
             const dim3 grid((a.row_blocks * 32 + xm - 1) / xm * x_tiles);
             if constexpr (PLANES == 1) {
                 if (direct) {
@@ -1666,8 +1718,12 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
             }
         }
         if (!one_pass && !whole) {
-            if (gq) finish(Yes{}, No{}, 0);
-            else finish(No{}, No{}, 0);
+            if (gq) {
+                a.splits++; // and `fix`
+                finish(Yes{}, No{}, 0);
+            } else {
+                finish(No{}, No{}, 0);
+            }
         }
     }
     APOE_HIP(hipGetLastError());

@@ -132,3 +132,37 @@ def test_the_queries_gradient_is_as_good_beside_the_rows(gpu_ctx):
         err[rows] = (np.linalg.norm(got - want, axis=1)[some] / np.linalg.norm(want, axis=1)[some])
     # a second rounding of the coefficients, 2^-11 each, beside the result's: sqrt(3 / 2) and what is left to chance
     assert (err[True] <= 1.5 * err[False] + 2.0 ** -11 / 3 ** 0.5).all(), float((err[True] / err[False]).max())
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("m,n,d", [(80, 3000, 64), (300, 5000, 1024), (4000, 500, 1024), (300, 700, 2056)])
+def test_the_targets_of_a_query_are_not_rounded_in_its_gradient(gpu_ctx, m, n, d, dtype):
+    """With grad_rows too, where the coefficients of both products are in the rows' type: what grad_queries is off by beside its own rounding is by the
+    coefficients of the other rows, two roundings of u each, independent: at most four times u sqrt(sum p^2) of a query's weight, and the logits' part."""
+    import apoe
+    import torch
+    a = make(m, n, d, dtype, seed=m, targets=3, scale=10.0)
+    a["weight"] = torch.full((m,), 1.0, device="cuda")
+    got = apoe.softmax_loss(gpu_ctx, **a, grad_queries=True, grad_rows=True)["grad_queries"].double().cpu().numpy()
+    want = oracle(a)[0]["grad_queries"]
+    once = torch.from_numpy(want).to(getattr(torch, dtype)).double().numpy()
+    q, x = (a[k].cpu().double().numpy() for k in ("queries", "rows"))
+    z = a["scale"] * q @ x.T
+    p = np.exp(z - z.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    off = a["t_off"].cpu().numpy()
+    w, idx = np.zeros((m, n)), a["t_idx"].cpu().numpy()
+    for i in range(m):
+        for e in range(off[i], off[i + 1]):
+            w[i, idx[e]] += float(a["t_val"][e])
+    W = w.sum(1)
+    logit = a["scale"] * (d + 4) * 2.0 ** -24 * (np.abs(q) @ np.abs(x).T).max(1)
+    others = 4 * U[dtype] * np.sqrt((p ** 2).sum(1)) + 4 * logit + 2.0 ** -20
+    length = np.linalg.norm(x, axis=1).max()
+    some = W > 0
+    err, own = np.linalg.norm(got - want, axis=1), np.linalg.norm(once - want, axis=1)
+    # own rounding: the value that is rounded is another, so its error is another draw of d values: 1.5 times covers it from 64 columns on
+    tol = 1.5 * own + a["scale"] * W * others * length
+    assert (err[some] <= tol[some]).all(), float((err[some] / tol[some]).max())
+    target = a["scale"] * np.sqrt((w ** 2).sum(1)) * U[dtype] / 12 ** 0.5  # what the targets' rounding alone would come to
+    assert float(np.mean(err[some])) < float(np.mean(np.sqrt(own ** 2 + (0.5 * target) ** 2)[some]) + np.mean((a["scale"] * W * (others / 4 + 2 * logit))[some]))
