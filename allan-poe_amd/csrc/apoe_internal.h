@@ -19,6 +19,7 @@ void set_error(const char* fmt, ...);
     do {                                                                                            \
         hipError_t e_ = (call);                                                                     \
         if (e_ != hipSuccess) {                                                                     \
+            (void)hipGetLastError(); /* told here: not once more by the check of the next launch */ \
             apoe::set_error("%s failed: %s (%s:%d)", #call, hipGetErrorString(e_), __FILE__, __LINE__); \
             return APOE_ERR_HIP;                                                                    \
         }                                                                                           \
