@@ -11,7 +11,7 @@
 //   grad q (for 16 bits: alone): one pass. A piece's exponentials (relative to their own references) are multiplied with the piece's rows at
 //     once; what the references lack to the common one goes into the exponents of the fragments on their way to the product.
 //   grad x: the normalised G is needed. Where one piece holds everything its 16-bit exponentials are brought to G in place (a pass
-//     over memory: 38 us for 2048 x 30 522, forming the logits again 150 us); otherwise the logits are formed again once lse is known.
+//     over memory: 38 us for 2048 x 30 522, forming the logits again 130 us); otherwise the logits are formed again once lse is known.
 // The targets' own terms are not left to the rounded blocks: their places are zeroed (or rewritten) and W p_t - w_t, which
 // nearly cancels for a query that is served well, is formed in 32 bits.
 // Exponentials (or G) in 16 bits are what the 16-bit products take; a second part of each would double the gradients' products. What it costs, against a
@@ -274,8 +274,9 @@ template <int HELD> __global__ __launch_bounds__(512) void loss_split(LossArgs a
 
 // Rows x queries, rows on the M side: 128 rows a wave (a group), so that a query's maximum and sum over them need one exchange between a
 // lane and its other half. SUMS: references and sums. EXP: the exponentials too, as blocks. GRAD: with lse known, G as blocks.
-// Bound by the matrix units and the power that they draw: 256 x 256 tiles reach 1040 TFLOP/s at 1024 queries x 65 536 fp16 rows of 1024 (zeros
-// in place of data 1240, a library product of 1024 x 131 072 x 1024 1005), float (three products each) 1190 at 1024 x 100 000. Eight waves of
+// Bound by the matrix units and the clock that they leave: 256 x 256 tiles reach 1040 TFLOP/s at 1024 queries x 65 536 fp16 rows of 1024 (zeros
+// in place of data 1240, a library product of 1024 x 131 072 x 1024 1005), float (three products each) 1190 at 1024 x 100 000; over a million rows 990,
+// with the matrix units busy in 47 % of the cycles, the clock at 1.9 GHz of 2.4 and 2.5 TB/s of memory traffic. Eight waves of
 // 128 x 64: two a SIMD (four waves of 128 x 128: 800); reads of the next fragment between the products of this one (974 without).
 template <typename T, int NT, int WM, int WN, int SF, int ST, int MODE>
 __global__ __launch_bounds__(64 * WM * WN, NT > 2 ? 1 : 2) void loss_tile(LossArgs a) {
@@ -739,7 +740,7 @@ template <typename T> __device__ inline i32x4 scale_down(i32x4 v, float less) {
 // grad q: a split's rows x its queries' blocks. M side: queries (blocks), N side: columns of the rows. EXP: fragments are brought
 // to the largest reference of the split, and a split's sum to the largest so far.
 // DIRECT: the only split of the only piece, whose sum is the gradient.
-// 256 x 256 tiles, 1024 queries x 524 000 fp16 rows of 1024: 1.25 ms, 880 TFLOP/s (the exponents' sums beside the products); 2048 x 30 522 bf16, G: 131 us, 980.
+// 256 x 256 tiles, 1024 queries x 500 000 fp16 rows of 1024: 1.30 ms, 810 TFLOP/s (the exponents' sums beside the products); 2048 x 30 522 bf16, G: 115 us, 1115.
 // KG: groups of waves that take every KG-th stage, where one workgroup has a CU to itself: two waves a SIMD, each with a whole wave's
 // piece of the tile (4096 x 4096 x 1024, direct: 47 us; one group 53, the same on eight waves of half the piece 52; grad x 42, 48.6).
 template <typename T, int MT, int NT, int WM, int WN, int ST, bool EXP, bool DIRECT = false, int KG = 1>
@@ -927,7 +928,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void loss_grad_q(LossArgs a, 
 }
 
 // grad x of a piece: rows (blocks read transposed) x queries. Each row's gradient is whole here: all queries are in.
-// 256 x 256 tiles, 2048 queries x 30 522 bf16 rows of 1024: 148 us, 865 TFLOP/s; 128 x 128, 4096 x 4096: 42 us (KG as above), 820.
+// 256 x 256 tiles, 2048 queries x 30 522 bf16 rows of 1024: 130 us, 990 TFLOP/s; 128 x 128, 4096 x 4096: 42 us (KG as above), 820.
 template <typename T, int MT, int NT, int WM, int WN, int ST, int KG = 1>
 __global__ __launch_bounds__(64 * WM * WN * KG, 2) void loss_grad_x(LossArgs a, uint32_t n_tiles) {
     using S = typename GradTiles<T>::S;

@@ -7,9 +7,11 @@
 // over rows in strides of the grid, so that the vectors s, w, w' stay in registers. The gradients of s, w and a channel gate
 // are all multiples of one sum over rows, Q = sum gy sigmoid(g) h / rms(h), and that of w' is R = sum gu y / rms(y): each group
 // adds up its rows, a workgroup its groups, a second kernel the workgroups, in a fixed order.
-// Measured: 65 536 bf16 rows of 1024 with an element gate, forward 131 us for 671 MB (5.1 TB/s; 152 when a row was asked for only once the one
-// in front of it was done), gradient 235 us for 1.07 GB (4.6 TB/s; a copy of 2 GiB runs at 4.86); 10 007 float rows, channel gate: 34 and
-// 41 us (164 and 205 MB); the vectors' sums 5 us; 64 rows 5 us.
+// Measured: 65 536 bf16 rows of 1024 with an element gate, forward 129 us for 671 MB (5.2 TB/s; 152 when a row was asked for only once the one
+// in front of it was done), gradient 205 us for 1.07 GB (5.2 TB/s; a copy of 2 GiB runs at 4.86); 10 007 float rows, channel gate: 33 and
+// 39 us (164 and 205 MB); the vectors' sums 5 us; 64 rows 5 us. Rows of up to 256 columns are held by 16 threads, in more registers: the gradient runs
+// one wave a SIMD, with no loads on their way meanwhile (262 144 bf16 rows of 256: forward 126 us, 5.3 TB/s; gradient 324 us, 3.3 TB/s; of 128
+// columns, which leave half of a thread's values empty, 374 us for both, 1.8 TB/s).
 #include "apoe_internal.h"
 
 namespace apoe {

@@ -320,10 +320,12 @@ typedef struct {
     const void* rows;           /* [n_rows][dim]; NULL: the half-precision rows of `corpus` */
     const apoe_corpus* corpus;  /* with rows == NULL: apoe_corpus_make_half_rows has run, dtype is APOE_F16 */
     uint64_t q_stride, rows_stride, grad_q_stride, grad_rows_stride; /* multiples of 8 (APOE_F32: 4), at most 2^18 */
-    const uint32_t *t_off, *t_idx; /* CSR: the rows that are relevant to each query (entries at or above n_rows count nothing); t_off
-                                      may be NULL without gradients (lse alone) */
+    const uint32_t *t_off, *t_idx; /* CSR: the rows that are relevant to each query (entries at or above n_rows count nothing). t_off has
+                                      n_queries + 1 numbers that do not fall, t_idx (and t_val) t_off[n_queries]: they are on the
+                                      GPU, so this is not checked. t_off may be NULL without gradients (lse alone) */
     const float* t_val;         /* their weights; NULL: equal shares that sum to one */
-    const uint32_t* live;       /* bit i % 32 of word i / 32: row i takes part (NULL: all do). What other rows hold is not looked at */
+    const uint32_t* live;       /* bit i % 32 of word i / 32, (n_rows + 31) / 32 words: row i takes part (NULL: all do). What other rows hold
+                                   is not looked at */
     const float* weight;        /* [n_queries] of the queries in the sum that is differentiated; NULL: 1. With APOE_F16 it is also the
                                    place for a loss scale: gradients below 6e-5 lose bits in that type */
     float scale;                /* of the inner products (one over the temperature), positive */
@@ -335,9 +337,9 @@ typedef struct {
  * Softmax cross entropy of every query over the live rows, and the gradient of sum_i weight_i loss_i:
  *   s_ij = scale <q_i, x_j>, lse_i = log sum_j exp(s_ij), W_i = sum_t w_it, loss_i = W_i lse_i - sum_t w_it s_it.
  * Without live rows lse is -inf; without live targets loss and gradient are zero, whatever the query holds; a dead row's
- * gradient is zero. The logits are never in memory as a whole: the workspace holds at most 1 GiB of exponentials at a time (one
- * tile's rows at least), 8 bytes for every 128 logits, partial sums of grad_q, and for APOE_F32 at most 1 GiB of rows in the form
- * that the products take.
+ * gradient is zero. Without queries nothing is written, and grad_rows is refused. The logits are never in memory as a whole: the workspace holds at most 1 GiB of exponentials at a time (one
+ * tile's rows at least), 8 bytes for every 128 logits, partial sums of grad_q, for APOE_F16 with grad_rows the queries once
+ * more, and for APOE_F32 at most 1 GiB of rows in the form that the products take.
  */
 int apoe_softmax_loss(apoe_ctx* ctx, const apoe_softmax_loss_args* args);
 
