@@ -17,7 +17,7 @@
 // Exponentials (or G) in 16 bits are what the 16-bit products take; a second part of each would double the gradients' products. What it costs, against a
 // gradient formed in 32 bits and rounded once: nothing in the queries' gradient (0.00166 and 0.00166 at 4096 x 4096 bf16), where the other rows' roundings
 // average, the second one of G (its exponentials were rounded before) too, and what the targets' would do is added in 32 bits (loss_targets); in the
-// rows' gradients, where a rounded target is most of a row, 1.25 times at 4096 x 4096 (0.00206 for 0.00166) and 1.5 times for 100 queries of 4000 rows.
+// rows' gradients, where a rounded target is most of a row, 1.25 times at 4096 x 4096 (0.00206 for 0.00166), 1.5 times for 100 queries of 4000 rows.
 #include "apoe_internal.h"
 #include "apoe_tile.h"
 
@@ -100,6 +100,7 @@ struct LossArgs {
     uint32_t *top_coef, *q_on;  // the largest of them, as bits; those that are not zero, as a bit mask
     float* q_size;              // [qp], for fp16: each query's largest value over its power of two (grad_scale)
     uint32_t* top_size;         // the largest of them, as bits
+    float *peak, *part_of_two;  // [qp]: the largest |weight w| of a query's targets; what brings the largest of all to a power of two (grad_scale)
     char* blocks;
     float* part;                // [splits][qp][dim]
     float* fix;                 // [qp][dim], with G: the targets' terms that rounding took out of G; behind the last split
@@ -117,14 +118,17 @@ template <typename T> constexpr float HEADROOM = __is_same(T, __bf16) ? 0.f : 14
 
 enum { TILE_SUMS = 0, TILE_EXP = 1, TILE_GRAD = 2 };
 
-// Power of two that brings a query's coefficients near 2^13 in G. fp16, whose numbers would not reach from the largest of all queries to what a light
-// one leaves at each row, takes one a query: it is taken out again where the query's own gradient is written, and for the rows' gradients
-// put into the query, times a power of two that is the same for all (scale_of_sizes). The others take that of the largest of all.
+// What a query's coefficients are taken times in G: near 2^13 at most. First a power of two: fp16, whose numbers would not reach from the largest of
+// all queries to what a light one leaves at each row, takes one a query: it is taken out again where the query's own gradient is written, and for the
+// rows' gradients put into the query, times a power of two that is the same for all (scale_of_sizes); the others take that of the largest of all. Then a
+// factor of a half to one, the same for all, under which the heaviest target's weight is a power of two: with equal weights, the usual case, a
+// rounded target loses what its row's probability is and not also the weight's own bits, which are the same for all targets and would not average.
 template <typename T> constexpr bool OWN_SCALE = __is_same(T, _Float16);
-template <typename T> __device__ inline float grad_scale(const LossArgs& a, uint32_t qi) {
+template <typename T> __device__ inline float grad_power(const LossArgs& a, uint32_t qi) {
     const float t = OWN_SCALE<T> ? a.coef[qi] : __uint_as_float(*a.top_coef);
     return t > 0.f && t < 1e30f && t > 1e-30f ? exp2f(13.f - ceilf(log2f(t))) : 1.f;
 }
+template <typename T> __device__ inline float grad_scale(const LossArgs& a, uint32_t qi) { return grad_power<T>(a, qi) * *a.part_of_two; }
 // Exponent that brings the largest of q_size to 2^13 .. 2^14.
 __device__ inline int scale_of_sizes(const LossArgs& a) {
     const float t = __uint_as_float(*a.top_size);
@@ -545,36 +549,40 @@ template <typename T> __global__ __launch_bounds__(64) void loss_coefs(LossArgs 
     }
     const float lse = join_chunks(a, qi, lane);
     const uint32_t e0 = a.t_off[qi], e1 = a.t_off[qi + 1];
-    float W = 0.f, A = 0.f;
+    float W = 0.f, A = 0.f, M = 0.f;
     for (uint32_t e = e0 + lane; e < e1; e += 64) {
         const float w = is_live(a, a.t_idx[e]) ? target_weight(a, e, e0, e1) : 0.f;
         W += w;
         A += fabsf(w);
+        M = fmaxf(M, fabsf(w));
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) {
         W += __shfl_xor(W, d);
         A += __shfl_xor(A, d);
+        M = fmaxf(M, __shfl_xor(M, d));
     }
     if (lane == 0) {
         const float c = a.weight ? a.weight[qi] : 1.f;
         a.lse_w[qi] = make_float2(lse, c * W);
         a.coef[qi] = fabsf(c) * (fabsf(W) + A);
         a.total[qi] = W;
-        if constexpr (OWN_SCALE<T>) a.q_size[qi] = a.coef[qi] != 0.f ? size / grad_scale<T>(a, qi) : 0.f;
+        if constexpr (OWN_SCALE<T>) a.q_size[qi] = a.coef[qi] != 0.f ? size / grad_power<T>(a, qi) : 0.f;
+        a.peak[qi] = fabsf(c) * M;
     }
 }
 
-// The largest coefficient (fp16: the largest size as well), and which queries count something (what the others hold is not multiplied), as bits: one workgroup.
+// The largest coefficient, target and (fp16) size, and which queries count something (what the others hold is not multiplied), as bits: one workgroup.
 template <typename T> __global__ __launch_bounds__(1024) void loss_queries(LossArgs a) {
-    constexpr int N = OWN_SCALE<T> ? 2 : 1;
+    constexpr int N = OWN_SCALE<T> ? 3 : 2;
     __shared__ uint32_t top[N][16];
     uint32_t most[N] = {}; // of floats that are not negative, as bits
     for (uint32_t q0 = 0; q0 < a.qp; q0 += 1024) {
         const uint32_t qi = q0 + threadIdx.x;
         const uint32_t c = qi < a.nq ? __float_as_uint(a.coef[qi]) : 0;
         most[0] = max(most[0], c);
-        if constexpr (N == 2) most[1] = max(most[1], qi < a.nq ? __float_as_uint(a.q_size[qi]) : 0);
+        most[1] = max(most[1], qi < a.nq ? __float_as_uint(a.peak[qi]) : 0);
+        if constexpr (N == 3) most[2] = max(most[2], qi < a.nq ? __float_as_uint(a.q_size[qi]) : 0);
         const unsigned long long b = __ballot(c != 0);
         if ((threadIdx.x & 31) == 0 && qi < a.qp) a.q_on[qi >> 5] = (uint32_t)(b >> (threadIdx.x & 32));
     }
@@ -588,7 +596,13 @@ template <typename T> __global__ __launch_bounds__(1024) void loss_queries(LossA
     if (threadIdx.x < N) {
         uint32_t all = 0;
         for (int k = 0; k < 16; k++) all = max(all, top[threadIdx.x][k]);
-        (threadIdx.x ? a.top_size : a.top_coef)[0] = all;
+        if (threadIdx.x == 0) *a.top_coef = all;
+        if (threadIdx.x == 1) {
+            const float peak = __uint_as_float(all);
+            int e;
+            *a.part_of_two = peak > 0.f && peak < 1e30f ? 0.5f / frexpf(peak, &e) : 1.f;
+        }
+        if (threadIdx.x == 2) *a.top_size = all;
     }
 }
 
@@ -597,7 +611,7 @@ __global__ __launch_bounds__(256) void loss_scale_queries(LossArgs a) {
     const uint32_t qi = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (qi >= a.nq || a.coef[qi] == 0.f) return;
     int own;
-    (void)frexpf(grad_scale<_Float16>(a, qi), &own); // 2^(own - 1)
+    (void)frexpf(grad_power<_Float16>(a, qi), &own); // 2^(own - 1)
     const int k = scale_of_sizes(a) + 1 - own;
     for (uint32_t d = (threadIdx.x & 63) * 8; d < a.dim; d += 512) {
         f16x8 x = *reinterpret_cast<const f16x8*>((const char*)a.q + (uint64_t)qi * a.q_pitch + d * 2);
@@ -1024,7 +1038,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void loss_grad_x(LossArgs a, 
         static_assert(BM * BN * 4 <= ST * STAGE, "the sums fit the stages");
         exchange_halves<MT, NT, WM * WN>(acc, lds, kg, wave % (WM * WN), lane);
     }
-    const float back = OWN_SCALE<T> ? ldexpf(a.scale, -scale_of_sizes(a)) : a.scale / grad_scale<T>(a, 0);
+    const float back = OWN_SCALE<T> ? ldexpf(a.scale, -scale_of_sizes(a)) / *a.part_of_two : a.scale / grad_scale<T>(a, 0);
     const int h = lane >> 5;
 #pragma unroll
     for (int m = 0; m < MT; m++) {
@@ -1543,7 +1557,7 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     };
     const size_t o_ref = take((size_t)a.groups * a.qp * 4), o_sum = take((size_t)a.groups * a.qp * 4);
     const size_t o_cr = take((size_t)a.chunks * a.qp * 4), o_cs = take((size_t)a.chunks * a.qp * 4);
-    const size_t o_lw = take((size_t)a.qp * 8), o_top = take(8), o_size = take(OWN_SCALE<T> ? (size_t)a.qp * 4 : 0), o_on = take(a.qp / 8), o_coef = take((size_t)a.qp * 4), o_total = take((size_t)a.qp * 4);
+    const size_t o_lw = take((size_t)a.qp * 8), o_top = take(12), o_peak = take((size_t)a.qp * 4), o_size = take(OWN_SCALE<T> ? (size_t)a.qp * 4 : 0), o_on = take(a.qp / 8), o_coef = take((size_t)a.qp * 4), o_total = take((size_t)a.qp * 4);
     a.block_low = (size_t)a.qp * piece * 2;
     const size_t o_blocks = take(gx ? GradTiles<T>::PLANES * a.block_low : gq ? PLANES * a.block_low : 0);
     a.tile_r_low = PLANES == 2 ? piece * a.tile_dim * 2 : 0;
@@ -1562,6 +1576,8 @@ template <typename T> static int run_loss(apoe_ctx* ctx, const apoe_softmax_loss
     a.lse_w = (float2*)(ws + o_lw);
     a.top_coef = (uint32_t*)(ws + o_top);
     a.top_size = a.top_coef + 1;
+    a.part_of_two = (float*)(a.top_coef + 2);
+    a.peak = (float*)(ws + o_peak);
     a.q_size = (float*)(ws + o_size);
     a.blocks = ws + o_blocks;
     a.part = (float*)(ws + o_part);

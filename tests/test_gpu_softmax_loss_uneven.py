@@ -166,3 +166,23 @@ def test_the_targets_of_a_query_are_not_rounded_in_its_gradient(gpu_ctx, m, n, d
     assert (err[some] <= tol[some]).all(), float((err[some] / tol[some]).max())
     target = a["scale"] * np.sqrt((w ** 2).sum(1)) * U[dtype] / 12 ** 0.5  # what the targets' rounding alone would come to
     assert float(np.mean(err[some])) < float(np.mean(np.sqrt(own ** 2 + (0.5 * target) ** 2)[some]) + np.mean((a["scale"] * W * (others / 4 + 2 * logit))[some]))
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("odd", [1.0, 0.75, 1.0 + 2.0 ** -9, 1.0 - 2.0 ** -9 / 3, 1.0 + 2.0 ** -12])
+def test_equal_weights_do_not_turn_all_targets_the_same_way(gpu_ctx, dtype, odd):
+    """Every query weighs the same and names one row; the logits are near zero, so that a row's gradient is its targets' but for 1 / n. The targets' coefficients
+    are rounded in the rows' type, all to the same number: along the gradient itself, where the result's roundings average, it has the right length
+    whatever the weight's bits are. Off by 2 / n (the probability that rounding takes from one, up to half a unit there) and u / sqrt(values) three times."""
+    import apoe
+    import torch
+    m, n, d = 300, 6000, 256
+    a = make(m, n, d, dtype, seed=5, targets=1, scale=0.25)
+    a["t_off"] = torch.arange(m + 1, dtype=torch.int32, device="cuda")
+    a["t_idx"] = torch.randint(0, n, (m,), generator=torch.Generator().manual_seed(1)).int().cuda()
+    a["t_val"] = None
+    a["weight"] = torch.full((m,), 64.0 * odd, device="cuda")
+    got = apoe.softmax_loss(gpu_ctx, **a, grad_queries=False, grad_rows=True)["grad_rows"].double().cpu().numpy()
+    want = oracle(a)[0]["grad_rows"]
+    length = float((got * want).sum() / (want * want).sum())
+    assert abs(length - 1) < 2 / n + 3 * U[dtype] / (m * d) ** 0.5 + 2.0 ** -20, length - 1
