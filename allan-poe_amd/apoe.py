@@ -4,8 +4,9 @@ Arrays may be numpy arrays (host) or torch tensors (host or the context's GPU); 
 library copies as needed. There is no CPU fallback: if the HIP library is missing or a
 call fails, an exception is raised.
 
-The operators that fit a query adapter (`softmax_loss`, `orthogonalize`, `gated_residual`) take torch tensors on the context's
-GPU, write torch tensors and return without waiting; their work is ordered with torch's current stream.
+The operators that fit a query adapter (`softmax_loss`, `orthogonalize`, `gated_residual`) and those that its layers are built and trained
+from (`embed`, `layer_norm`, `linear`, `AdamW`) take torch tensors on the context's GPU, write torch tensors and return without waiting; their
+work is ordered with torch's current stream.
 """
 import ctypes as C
 import os
@@ -65,6 +66,39 @@ class GatedResidualArgs(C.Structure):
                 ("grad_scale", C.c_void_p), ("grad_w_post", C.c_void_p), ("grad_w_next", C.c_void_p)]
 
 
+class EmbedArgs(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("n_rows", C.c_uint32), ("n_table", C.c_uint32), ("n_entries", C.c_uint32), ("dim", C.c_uint32),
+                ("table", C.c_void_p), ("idx", C.c_void_p), ("off", C.c_void_p), ("val", C.c_void_p), ("scale", C.c_float), ("base", C.c_void_p), ("out", C.c_void_p),
+                ("table_stride", C.c_uint64), ("base_stride", C.c_uint64), ("out_stride", C.c_uint64),
+                ("grad", C.c_void_p), ("grad_table", C.c_void_p), ("grad_val", C.c_void_p), ("grad_stride", C.c_uint64), ("grad_table_stride", C.c_uint64),
+                ("accumulate", C.c_uint32)]
+
+
+class LayerNormArgs(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("rows", C.c_uint32), ("dim", C.c_uint32), ("x", C.c_void_p), ("w", C.c_void_p), ("b", C.c_void_p), ("eps", C.c_float),
+                ("y", C.c_void_p), ("x_stride", C.c_uint64), ("y_stride", C.c_uint64),
+                ("grad_y_stride", C.c_uint64), ("grad_skip_stride", C.c_uint64), ("grad_x_stride", C.c_uint64),
+                ("grad_y", C.c_void_p), ("grad_skip", C.c_void_p), ("grad_x", C.c_void_p), ("grad_w", C.c_void_p), ("grad_b", C.c_void_p)]
+
+
+class LinearArgs(C.Structure):
+    _fields_ = [("dtype", C.c_uint32), ("rows", C.c_uint32), ("cols_in", C.c_uint32), ("cols_out", C.c_uint32), ("act", C.c_uint32),
+                ("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("y", C.c_void_p), ("pre", C.c_void_p),
+                ("x_stride", C.c_uint64), ("w_stride", C.c_uint64), ("residual_stride", C.c_uint64), ("y_stride", C.c_uint64), ("pre_stride", C.c_uint64),
+                ("grad_y", C.c_void_p), ("grad_x", C.c_void_p), ("grad_w", C.c_void_p), ("grad_bias", C.c_void_p),
+                ("grad_y_stride", C.c_uint64), ("grad_x_stride", C.c_uint64), ("grad_w_stride", C.c_uint64)]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("m", C.c_void_p), ("v", C.c_void_p), ("m_scale", C.c_void_p), ("v_scale", C.c_void_p), ("copy", C.c_void_p),
+                ("copy_dtype", C.c_uint32), ("n", C.c_uint64), ("decay", C.c_double)]
+
+
+class AdamwStepArgs(C.Structure):
+    _fields_ = [("grads", C.c_void_p), ("grad_dtypes", C.c_void_p), ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("grad_scale", C.c_double), ("step", C.c_uint32), ("step_dev", C.c_void_p), ("lr_dev", C.c_void_p)]
+
+
 EXPORTS = [
     "apoe_last_error_string", "apoe_ctx_create", "apoe_ctx_destroy", "apoe_ctx_synchronize", "apoe_corpus_create", "apoe_corpus_create_without",
     "apoe_corpus_destroy", "apoe_corpus_info", "apoe_corpus_bytes", "apoe_corpus_pair_bytes", "apoe_corpus_make_half_rows", "apoe_queries_create", "apoe_queries_destroy",
@@ -74,6 +108,8 @@ EXPORTS = [
     "apoe_knn_elapsed_ms", "apoe_knn_counters", "apoe_knn_read_counters", "apoe_graph_create", "apoe_graph_destroy", "apoe_graph_info", "apoe_graph_download",
     "apoe_search", "apoe_search_noalloc",
     "apoe_ctx_create_on_stream", "apoe_ctx_stream", "apoe_softmax_loss", "apoe_orthogonalize", "apoe_gated_residual", "apoe_gated_residual_grad",
+    "apoe_embed", "apoe_embed_grad", "apoe_layer_norm", "apoe_layer_norm_grad", "apoe_linear", "apoe_linear_grad",
+    "apoe_adamw_create", "apoe_adamw_destroy", "apoe_adamw_step", "apoe_adamw_moments",
 ]
 
 
@@ -99,7 +135,7 @@ def lib():
         _lib.apoe_knn_elapsed_ms.restype = C.c_float
         _lib.apoe_knn_elapsed_ms.argtypes = [C.c_void_p]
         for name in ("apoe_ctx_destroy", "apoe_corpus_destroy", "apoe_queries_destroy", "apoe_kg_destroy",
-                     "apoe_knn_destroy", "apoe_graph_destroy"):
+                     "apoe_knn_destroy", "apoe_graph_destroy", "apoe_adamw_destroy"):
             getattr(_lib, name).restype = None
             getattr(_lib, name).argtypes = [C.c_void_p]
     return _lib
@@ -534,9 +570,16 @@ def _call(ctx, function, args):
     if _raw_stream(ctx.device) == ctx.stream:
         _check(function(ctx.h, C.byref(args)))
         return
+    _ordered(ctx, lambda: function(ctx.h, C.byref(args)))
+
+
+def _ordered(ctx, call):
+    if _raw_stream(ctx.device) == ctx.stream:
+        _check(call())
+        return
     theirs, ours = _torch.cuda.current_stream(ctx.device), ctx.torch_stream()
     ours.wait_stream(theirs)
-    status = function(ctx.h, C.byref(args))
+    status = call()
     theirs.wait_stream(ours)
     _check(status)
 
@@ -692,3 +735,306 @@ def gated_residual_grad(ctx, x, h=None, gate=None, scale=None, w_post=None, w_ne
         setattr(a, name, t.data_ptr())
     _call(ctx, lib().apoe_gated_residual_grad, a)
     return out
+
+
+# ---- layers of an adapter or an encoder, and their training ----
+
+def _wanted(ctx, asked, name, shape, like):
+    """The tensor that a gradient goes to: the caller's own (checked), or a new one where True is asked for. None: not wanted."""
+    if asked is False or asked is None:
+        return None
+    if asked is True:
+        return _torch.empty(shape, dtype=like.dtype, device=like.device)
+    _matrix(ctx, asked, name, _torch.Size(shape), like.dtype)
+    return asked
+
+
+def _embed_args(ctx, table, idx, off, val, scale):
+    a = EmbedArgs()
+    a.dtype = _dtype(table, "table")
+    a.table_stride = _matrix(ctx, table, "table")
+    (a.n_table, a.dim), a.table = table.shape, table.data_ptr()
+    a.idx = _vector(ctx, idx, "idx", None, _INTS)
+    a.n_entries = a.n_rows = idx.shape[0]
+    if off is not None:
+        a.off = _vector(ctx, off, "off", None, _INTS)
+        a.n_rows = off.shape[0] - 1
+        if off.shape[0] == 0:
+            raise ApoeError("off must have one number more than there are rows")
+    if val is not None:
+        a.val = _vector(ctx, val, "val", idx.shape[0], _FLOATS)
+    a.scale = scale
+    return a
+
+
+def embed(ctx, table, idx, off=None, val=None, scale=1.0, base=None, out=None):
+    """out[i] = base[i] + scale * the sum of val[e] * table[idx[e]] over the entries e of row i: off [m + 1], idx and val are the CSR of the
+    rows' terms and weights (ones without val); without off entry i is row i's. Entries at or above the table's length count nothing. table, base and
+    out have one type; out may be base itself."""
+    a = _embed_args(ctx, table, idx, off, val, scale)
+    shape = _torch.Size((a.n_rows, a.dim))
+    if base is not None:
+        a.base_stride, a.base = _matrix(ctx, base, "base", shape, table.dtype), base.data_ptr()
+    if out is None:
+        out = _torch.empty(shape, dtype=table.dtype, device=table.device)
+    a.out_stride, a.out = _matrix(ctx, out, "out", shape, table.dtype), out.data_ptr()
+    if out.numel() == 0:
+        return out
+    _call(ctx, lib().apoe_embed, a)
+    return out
+
+
+def embed_grad(ctx, table, grad, idx, off=None, val=None, scale=1.0, grad_table=True, grad_val=False, accumulate=False):
+    """Gradients of embed from that of out (which is base's own): a dict of grad_table (True, or a matrix like the table to write to, with
+    accumulate to add to) and grad_val [entries]."""
+    a = _embed_args(ctx, table, idx, off, val, scale)
+    a.grad_stride, a.grad = _matrix(ctx, grad, "grad", _torch.Size((a.n_rows, a.dim)), table.dtype), grad.data_ptr()
+    if accumulate and (grad_table is True or grad_table is False or grad_table is None):
+        raise ApoeError("accumulate needs the grad_table that is added to")
+    out = {}
+    g = _wanted(ctx, grad_table, "grad_table", table.shape, table)
+    if g is not None:
+        a.grad_table_stride, a.grad_table, a.accumulate = _matrix(ctx, g, "grad_table"), g.data_ptr(), bool(accumulate)
+        out["grad_table"] = g
+    if grad_val:
+        out["grad_val"] = _torch.empty(idx.shape[0], dtype=_torch.float32, device=table.device)
+        a.grad_val = out["grad_val"].data_ptr()
+    if not out:
+        raise ApoeError("neither grad_table nor grad_val")
+    if all(t.numel() == 0 for t in out.values()):
+        return out
+    if table.numel() == 0:  # no row that an entry could name
+        out["grad_val"].zero_()
+        return out
+    if idx.numel() == 0 and a.grad_table is None:
+        return out
+    _call(ctx, lib().apoe_embed_grad, a)
+    return out
+
+
+def _norm_args(ctx, x, w, b, eps):
+    a = LayerNormArgs()
+    a.dtype = _dtype(x, "x")
+    a.x_stride = _matrix(ctx, x, "x")
+    (a.rows, a.dim), a.eps, a.x = x.shape, eps, x.data_ptr()
+    for t, name in ((w, "w"), (b, "b")):
+        if t is not None:
+            setattr(a, name, _vector(ctx, t, name, a.dim, _FLOATS))
+    return a
+
+
+def layer_norm(ctx, x, w=None, b=None, eps=1e-5, out=None):
+    """w * (x - mean(x)) / sqrt(var(x) + eps) + b for every row of x [m, d]; w and b are float32. out may be x itself."""
+    a = _norm_args(ctx, x, w, b, eps)
+    if out is None:
+        out = _torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    a.y_stride, a.y = _matrix(ctx, out, "out", x.shape, x.dtype), out.data_ptr()
+    if x.numel() == 0:
+        return out
+    _call(ctx, lib().apoe_layer_norm, a)
+    return out
+
+
+def layer_norm_grad(ctx, x, w=None, b=None, eps=1e-5, grad_y=None, grad_skip=None):
+    """Gradients of layer_norm: a dict of grad_x (grad_skip, what x's gradient has by another way, is added to it), and of grad_w, grad_b for
+    the vectors that are not None."""
+    a = _norm_args(ctx, x, w, b, eps)
+    if grad_y is None:
+        raise ApoeError("grad_y is None")
+    for t, name in ((grad_y, "grad_y"), (grad_skip, "grad_skip")):
+        if t is not None:
+            setattr(a, name + "_stride", _matrix(ctx, t, name, x.shape, x.dtype))
+            setattr(a, name, t.data_ptr())
+    out = dict(grad_x=_torch.empty(x.shape, dtype=x.dtype, device=x.device))
+    for t, name in ((w, "grad_w"), (b, "grad_b")):
+        if t is not None:
+            out[name] = _torch.empty(a.dim, dtype=_torch.float32, device=x.device)
+    if x.numel() == 0:
+        for t in out.values():
+            t.zero_()
+        return out
+    for name, t in out.items():
+        setattr(a, name, t.data_ptr())
+    _call(ctx, lib().apoe_layer_norm_grad, a)
+    return out
+
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+def _linear_args(ctx, x, w, act):
+    a = LinearArgs()
+    a.dtype = _dtype(x, "x")
+    a.x_stride = _matrix(ctx, x, "x")
+    a.w_stride = _matrix(ctx, w, "w", dtype=x.dtype)
+    if w.shape[1] != x.shape[1]:
+        raise ApoeError(f"w must have x's {x.shape[1]} columns, not {w.shape[1]}")
+    a.rows, a.cols_in = x.shape
+    a.cols_out, a.x, a.w = w.shape[0], x.data_ptr(), w.data_ptr()
+    if act not in ACTIVATIONS:
+        raise ApoeError(f"act must be one of {', '.join(ACTIVATIONS)}, not {act!r}")
+    if 0 in w.shape:
+        raise ApoeError("w is empty")
+    a.act = ACTIVATIONS[act]
+    return a
+
+
+def linear(ctx, x, w, bias=None, act="none", residual=None, want_pre=False, out=None):
+    """(y, pre): y = act(pre) + residual with pre = x w^T + bias, for x [m, k], w [n, k], bias [n] float32, residual [m, n]; act: "none", "relu",
+    "gelu" or "silu". pre, which linear_grad needs where there is an activation, is None unless it is wanted."""
+    a = _linear_args(ctx, x, w, act)
+    shape = _torch.Size((a.rows, a.cols_out))
+    if bias is not None:
+        a.bias = _vector(ctx, bias, "bias", a.cols_out, _FLOATS)
+    if residual is not None:
+        a.residual_stride, a.residual = _matrix(ctx, residual, "residual", shape, x.dtype), residual.data_ptr()
+    if out is None:
+        out = _torch.empty(shape, dtype=x.dtype, device=x.device)
+    a.y_stride, a.y = _matrix(ctx, out, "out", shape, x.dtype), out.data_ptr()
+    pre = _torch.empty(shape, dtype=x.dtype, device=x.device) if want_pre else None
+    if pre is not None:
+        a.pre = pre.data_ptr()
+    if x.shape[0] == 0:
+        return out, pre
+    _call(ctx, lib().apoe_linear, a)
+    return out, pre
+
+
+def linear_grad(ctx, x, w, grad_y, act="none", pre=None, grad_x=True, grad_w=True, grad_bias=True):
+    """Gradients of linear from that of y (which is residual's own): a dict of grad_x, grad_w (True, or a matrix to write to) and grad_bias
+    (float32). pre: what linear gave, where there is an activation."""
+    a = _linear_args(ctx, x, w, act)
+    shape = _torch.Size((a.rows, a.cols_out))
+    a.grad_y_stride, a.grad_y = _matrix(ctx, grad_y, "grad_y", shape, x.dtype), grad_y.data_ptr()
+    if a.act:
+        if pre is None:
+            raise ApoeError("the gradient of an activation needs pre")
+        a.pre_stride, a.pre = _matrix(ctx, pre, "pre", shape, x.dtype), pre.data_ptr()
+    out = {}
+    for asked, name, t in ((grad_x, "grad_x", x), (grad_w, "grad_w", w)):
+        g = _wanted(ctx, asked, name, t.shape, t)
+        if g is not None:
+            setattr(a, name + "_stride", _matrix(ctx, g, name))
+            setattr(a, name, g.data_ptr())
+            out[name] = g
+    if grad_bias:
+        out["grad_bias"] = _torch.empty(a.cols_out, dtype=_torch.float32, device=x.device)
+        a.grad_bias = out["grad_bias"].data_ptr()
+    if not out:
+        raise ApoeError("nothing to compute")
+    if x.shape[0] == 0:
+        for t in out.values():
+            t.zero_()
+        return out
+    _call(ctx, lib().apoe_linear_grad, a)
+    return out
+
+
+class AdamW:
+    """AdamW over a list of float32 parameters (any shapes, contiguous; stepped in place).
+
+    copies: for each parameter a float16 or bfloat16 tensor of its shape (or None) that gets the stepped values, rounded. bits: of the moments, 32 or 8
+    (8: a code a value and a scale for every 256; rounded up or down by chance, which `seed` chooses). weight_decay: one number, or one for each
+    parameter. state: what `state()` of an earlier object gave, used in place; by default the moments are zeros and no step has been taken.
+
+    The moments of all parameters lie in one array each, parameter i from offsets[i] on (a multiple of 256)."""
+
+    BLOCK = 256
+
+    def __init__(self, ctx, params, copies=None, bits=32, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, seed=0, state=None):
+        self.h = C.c_void_p()
+        if _torch is None:
+            _load_torch()
+        self.ctx, self.bits, self.betas, self.eps, self.seed = ctx, bits, betas, eps, seed
+        self.params = list(params)
+        self.copies = [None] * len(self.params) if copies is None else list(copies)
+        decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(self.params)
+        if bits not in (8, 32):
+            raise ApoeError(f"moments have 8 or 32 bits, not {bits}")
+        if len(self.copies) != len(self.params) or len(decay) != len(self.params):
+            raise ApoeError("copies and weight_decay need one entry for each parameter")
+        blocks, self.offsets = 0, []
+        for p, c in zip(self.params, self.copies):
+            self._checked(p, "a parameter", _FLOATS)
+            if c is not None:
+                self._checked(c, "a copy", (_torch.float16, _torch.bfloat16), p.shape)
+            self.offsets.append(blocks * self.BLOCK)
+            blocks += -(-p.numel() // self.BLOCK)
+        n, dev = blocks * self.BLOCK, f"cuda:{ctx.device}"
+        types = dict(m=_torch.float32, v=_torch.float32) if bits == 32 else dict(m=_torch.int8, v=_torch.uint8, m_scale=_torch.float32, v_scale=_torch.float32)
+        if state is None:
+            state = {k: _torch.zeros(blocks if k.endswith("scale") else n, dtype=t, device=dev) for k, t in types.items()}
+        for k, t in types.items():
+            if k not in state:
+                raise ApoeError(f"state has no {k}")
+            _vector(ctx, state[k], k, blocks if k.endswith("scale") else n, (t,))
+        self._moments = {k: state[k] for k in types}
+        self.t = int(state.get("t", 0))
+        tensors = (AdamwTensor * len(self.params))()
+        for a, p, c, d, at in zip(tensors, self.params, self.copies, decay, self.offsets):
+            a.p, a.n, a.decay = p.data_ptr(), p.numel(), d
+            for k, t in self._moments.items():
+                setattr(a, k, t.data_ptr() + (at // self.BLOCK if k.endswith("scale") else at) * t.element_size())
+            if c is not None:
+                a.copy, a.copy_dtype = c.data_ptr(), _DTYPES[c.dtype]
+        _check(lib().apoe_adamw_create(ctx.h, C.c_uint32(len(self.params)), tensors, C.c_uint32(bits), C.c_uint32(seed & 0xFFFFFFFF), C.byref(self.h)))
+        self._grads, self._types = (C.c_void_p * len(self.params))(), (C.c_uint32 * len(self.params))()
+        self._sizes = [p.numel() for p in self.params]
+
+    def _checked(self, t, name, dtypes, shape=None):
+        _on_gpu(self.ctx, t, name)
+        if t.dtype not in dtypes or not t.is_contiguous() or (shape is not None and t.shape != shape):
+            raise ApoeError(f"{name} must be a contiguous tensor of {' or '.join(str(d) for d in dtypes)}{'' if shape is None else f' of shape {tuple(shape)}'}")
+
+    def step(self, grads, lr, grad_scale=1.0, t=None):
+        """One step with the parameters' gradients (None: that parameter and its moments stay as they are), which count times grad_scale. lr may be a
+        float32 tensor of one number on the GPU, and t, the number of the step, an int32 one: a captured step reads both when it
+        is replayed (the program counts t up; without it the object counts)."""
+        if len(grads) != len(self.params):
+            raise ApoeError(f"{len(grads)} gradients for {len(self.params)} parameters")
+        a = AdamwStepArgs()
+        for i, g in enumerate(grads):
+            if g is None:
+                self._grads[i] = None
+                continue
+            if g.get_device() != self.ctx.device or g.numel() != self._sizes[i] or not g.is_contiguous():
+                raise ApoeError(f"gradient {i} must be a contiguous tensor of {self._sizes[i]} values on GPU {self.ctx.device}, the context's")
+            self._types[i] = _dtype(g, "a gradient")
+            self._grads[i] = g.data_ptr()
+        a.grads, a.grad_dtypes = C.addressof(self._grads), C.addressof(self._types)
+        if isinstance(lr, _torch.Tensor):
+            a.lr_dev = _vector(self.ctx, lr.reshape(-1), "lr", 1, _FLOATS)
+        else:
+            a.lr = lr
+        a.beta1, a.beta2 = self.betas
+        a.eps, a.grad_scale, a.step = self.eps, grad_scale, self.t + 1
+        if t is not None:
+            a.step_dev = _vector(self.ctx, t.reshape(-1), "t", 1, _INTS)
+        _ordered(self.ctx, lambda: lib().apoe_adamw_step(self.h, C.byref(a)))
+        if t is None:
+            self.t += 1
+
+    def moments(self):
+        """(m, v) as float32, laid out like the moments themselves: those themselves where they have 32 bits."""
+        m = self._moments
+        if self.bits == 32:
+            return m["m"], m["v"]
+        out = [_torch.empty(t.shape, dtype=_torch.float32, device=t.device) for t in (m["m"], m["v"])]
+        pointers = [C.c_void_p(t.data_ptr()) for t in (m["m"], m["m_scale"], m["v"], m["v_scale"], *out)]
+        _ordered(self.ctx, lambda: lib().apoe_adamw_moments(self.ctx.h, C.c_uint64(m["m"].numel()), *pointers))
+        return tuple(out)
+
+    def state(self):
+        """What another object over the same parameters goes on from (the arrays themselves, not copies)."""
+        return dict(self._moments, t=self.t)
+
+    def close(self):
+        if self.h:
+            lib().apoe_adamw_destroy(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

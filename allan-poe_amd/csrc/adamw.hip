@@ -1,0 +1,329 @@
+// One AdamW step over many parameters, moments in 32 bits or in 8:
+//   m' = m + (1 - b1)(g - m), v' = v + (1 - b2)(g g - v), p' = p - lr (decay p + (m' / (1 - b1^t)) / (sqrt(v' / (1 - b2^t)) + eps)).
+//
+// Bound by memory: p, m, v read and written, g read, a 16-bit copy written: 28 to 30 bytes a value, in 8 bits 14 to 16. The list of parameters
+// travels in the kernel's arguments, so that there is nothing to copy to the GPU and a call can be captured; a workgroup finds its parameter
+// by the number of its piece. A wave works on 256 values at a time, a block of the 8-bit moments.
+// 8 bits: m = s c |c| / 127^2, v = s c^4 / 255^4, s the block's largest. Squares and fourth powers put the codes close together where values are
+// small: the smallest v is 4e9 times below the largest (a root that steps divide by: 65 025 times). An average that moves by a
+// thousandth a step would stand still if it were rounded to the nearest code, so it goes up or down by chance, with the probability that keeps
+// its mean in m and in v. What is above a code is a difference of two close numbers, and the comparison with the chance decides a
+// code: both in 64 bits, at the same rate as 32 on this GPU's vector units.
+#include <algorithm>
+#include <cmath>
+
+#include "apoe_internal.h"
+
+namespace apoe {
+
+constexpr uint32_t ADAM_LIST = 44;       // parameters of a launch: what the kernel's arguments have room for
+constexpr uint32_t ADAM_PIECE = 4096;    // values of a workgroup
+constexpr uint32_t BLOCK = APOE_ADAMW_BLOCK;
+
+using f32x4a = float __attribute__((ext_vector_type(4)));
+using u32x2a = uint32_t __attribute__((ext_vector_type(2)));
+
+struct AdamTensor {
+    float* p;
+    const void* g;
+    void *m, *v;
+    float *ms, *vs;
+    void* copy;
+    uint64_t n;
+    float decay;
+    uint32_t index;       // in the caller's list
+    uint32_t first;       // its first piece
+    uint8_t g_type, copy_type, whole; // whole: four values a load
+};
+
+struct AdamArgs {
+    AdamTensor t[ADAM_LIST];
+    uint32_t count, pieces, seed, step;
+    const uint32_t* step_dev;
+    const float* lr_dev;
+    double b1, b2, grad_scale;
+    float lr, eps, c1, c2; // c: one over 1 - b^t
+};
+static_assert(sizeof(AdamArgs) <= 4096, "the arguments of a kernel");
+
+__device__ __host__ inline uint32_t mix(uint32_t h) { // the finishing rounds of a 32-bit hash (Appleby's fmix32): shifts and odd multipliers
+    h = (h ^ (h >> 16)) * 0x85ebca6bu;
+    h = (h ^ (h >> 13)) * 0xc2b2ae35u;
+    return h ^ (h >> 16);
+}
+
+__device__ __host__ inline double power(double b, uint32_t t) {
+    double r = 1.;
+    for (; t; t >>= 1, b *= b)
+        if (t & 1) r *= b;
+    return r;
+}
+
+// A moment's step in 64 bits, every operation rounded by itself: a tenth of the way between two floats lies half way between two others often enough
+// that the largest of a block, which is rounded to a float, must not hang on how the operations are joined.
+__device__ inline double moved(double m, double target, double share) {
+#pragma clang fp contract(off)
+    const double way = target - m;
+    const double part = share * way;
+    return m + part;
+}
+__device__ inline double value_of_m(float scale, int c) {
+#pragma clang fp contract(off)
+    const double r = (double)(c * abs(c)) * (1. / (127. * 127.));
+    return (double)scale * r;
+}
+__device__ inline double value_of_v(float scale, uint32_t c) {
+#pragma clang fp contract(off)
+    const double r = (double)(c * c * c * c) * (1. / (255. * 255. * 255. * 255.)); // below 2^32
+    return (double)scale * r;
+}
+
+// Values k of a lane: four in a row, or (parameters that begin anywhere, a block's rest) 64 apart.
+__device__ inline uint32_t place(bool whole, int lane, int k) { return whole ? (uint32_t)lane * 4 + k : (uint32_t)k * 64 + lane; }
+
+__device__ inline void load_grad(float* g, const AdamTensor& t, uint64_t at, bool whole, int lane, uint32_t left) {
+    if (whole) {
+        const uint64_t e = at + lane * 4;
+        if (t.g_type == APOE_F32) {
+            const f32x4a x = *reinterpret_cast<const f32x4a*>((const float*)t.g + e);
+#pragma unroll
+            for (int k = 0; k < 4; k++) g[k] = x[k];
+        } else {
+            const u32x2a x = *reinterpret_cast<const u32x2a*>((const uint16_t*)t.g + e);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint16_t h = (uint16_t)(x[k >> 1] >> (16 * (k & 1)));
+                g[k] = t.g_type == APOE_F16 ? (float)__builtin_bit_cast(_Float16, h) : __builtin_bit_cast(float, (uint32_t)h << 16);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t i = place(false, lane, k);
+        g[k] = 0.f;
+        if (i >= left) continue;
+        if (t.g_type == APOE_F32) g[k] = ((const float*)t.g)[at + i];
+        else if (t.g_type == APOE_F16) g[k] = (float)((const _Float16*)t.g)[at + i];
+        else g[k] = (float)((const __bf16*)t.g)[at + i];
+    }
+}
+
+template <typename T> __device__ inline void load4(T* x, const T* from, uint64_t at, bool whole, int lane, uint32_t left) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    if (whole) {
+        const t4 v = *reinterpret_cast<const t4*>(from + at + lane * 4);
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = v[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t i = place(false, lane, k);
+            x[k] = i < left ? from[at + i] : (T)0;
+        }
+    }
+}
+
+template <typename T> __device__ inline void store4(T* to, const T* x, uint64_t at, bool whole, int lane, uint32_t left) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    if (whole) {
+        t4 v;
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = x[k];
+        *reinterpret_cast<t4*>(to + at + lane * 4) = v;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t i = place(false, lane, k);
+            if (i < left) to[at + i] = x[k];
+        }
+    }
+}
+
+// The largest of the wave's numbers, as the bits of floats that are not negative: a NaN is larger than all.
+__device__ inline float wave_largest(float v) {
+    uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) b = max(b, (uint32_t)__shfl_xor((int)b, d));
+    return __uint_as_float(b);
+}
+
+// The code of x >= 0 in a block whose largest is `top`: x = top (code / STEPS)^POWER, up where `chance` is below the share of the way from the code
+// beneath to the one above. inv: STEPS^POWER / top. A largest that is not finite leaves zero: the block's values are its scale's.
+template <int POWER, int STEPS> __device__ inline int code_of(double x, double inv, uint32_t chance) {
+    constexpr double MOST = POWER == 2 ? (double)STEPS * STEPS : (double)STEPS * STEPS * STEPS * STEPS;
+    const double w = fmin(x * inv, MOST);
+    const float root = POWER == 2 ? sqrtf((float)w) : sqrtf(sqrtf((float)w));
+    double k = (double)floorf(root);
+    auto raised = [](double c) { return POWER == 2 ? c * c : c * c * (c * c); };
+    if (raised(k) > w) k -= 1.;
+    if (raised(k + 1.) <= w) k += 1.;
+    const double low = raised(k), gap = raised(k + 1.) - low;
+    const double u = ((double)chance + 0.5) * 0x1p-32;
+    return min((int)k + (u * gap < w - low ? 1 : 0), STEPS);
+}
+
+template <int BITS> __global__ __launch_bounds__(256) void adamw_step(AdamArgs a) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t which = 0;
+    for (uint32_t lo = 0, hi = a.count; hi - lo > 1;) { // the last parameter whose first piece is at or before this one
+        const uint32_t mid = (lo + hi) / 2;
+        if (a.t[mid].first <= blockIdx.x) lo = mid;
+        else hi = mid;
+        which = lo;
+    }
+    const AdamTensor& t = a.t[which];
+    const uint64_t begin = (uint64_t)(blockIdx.x - t.first) * ADAM_PIECE, end = min(begin + ADAM_PIECE, t.n);
+    float c1 = a.c1, c2 = a.c2, lr = a.lr;
+    uint32_t step = a.step;
+    if (a.step_dev) {
+        step = *a.step_dev;
+        c1 = (float)(1. / (1. - power(a.b1, step)));
+        c2 = (float)(1. / (1. - power(a.b2, step)));
+    }
+    if (a.lr_dev) lr = *a.lr_dev;
+    const uint32_t key = mix(mix(mix(a.seed) ^ step) ^ t.index);
+    for (uint64_t at = begin + wave * BLOCK; at < end; at += 4 * BLOCK) {
+        const uint32_t left = (uint32_t)min((uint64_t)BLOCK, t.n - at);
+        const bool whole = t.whole && left == BLOCK;
+        float p[4], g[4], m[4], v[4];
+        load4(p, t.p, at, whole, lane, left);
+        load_grad(g, t, at, whole, lane, left);
+        if constexpr (BITS == 32) {
+            load4(m, (const float*)t.m, at, whole, lane, left);
+            load4(v, (const float*)t.v, at, whole, lane, left);
+            const float d1 = (float)(1. - a.b1), d2 = (float)(1. - a.b2), gs = (float)a.grad_scale;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float x = g[k] * gs;
+                m[k] = __builtin_fmaf(d1, x - m[k], m[k]);
+                v[k] = __builtin_fmaf(d2, __builtin_fmaf(x, x, -v[k]), v[k]);
+            }
+            store4((float*)t.m, m, at, whole, lane, left);
+            store4((float*)t.v, v, at, whole, lane, left);
+        } else {
+            const uint64_t block = at / BLOCK;
+            int8_t cm[4];
+            uint8_t cv[4];
+            load4(cm, (const int8_t*)t.m, at, whole, lane, left);
+            load4(cv, (const uint8_t*)t.v, at, whole, lane, left);
+            const float sm = t.ms[block], sv = t.vs[block];
+            double md[4], vd[4];
+            float mt = 0.f, vt = 0.f; // the largest, by magnitude; a value beyond the parameter's end is zero
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const bool in = place(whole, lane, k) < left;
+                const double x = (double)g[k] * a.grad_scale;
+                md[k] = in ? moved(value_of_m(sm, cm[k]), x, 1. - a.b1) : 0.;
+                vd[k] = in ? moved(value_of_v(sv, cv[k]), x * x, 1. - a.b2) : 0.;
+                m[k] = (float)md[k];
+                v[k] = (float)vd[k];
+                mt = __uint_as_float(max(__float_as_uint(mt), __float_as_uint(m[k]) & 0x7fffffffu));
+                vt = __uint_as_float(max(__float_as_uint(vt), __float_as_uint(v[k]) & 0x7fffffffu));
+            }
+            mt = wave_largest(mt);
+            vt = wave_largest(vt);
+            const double im = mt > 0.f ? 127. * 127. / (double)mt : 0., iv = vt > 0.f ? 255. * 255. * 255. * 255. / (double)vt : 0.;
+            const uint32_t bk = mix(mix(key ^ (uint32_t)block) ^ (uint32_t)(block >> 32));
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t i = place(whole, lane, k);
+                const int c = code_of<2, 127>(fabs(md[k]), im, mix(bk + 2 * i)), r = code_of<4, 255>(vd[k], iv, mix(bk + 2 * i + 1));
+                cm[k] = (int8_t)(md[k] < 0. ? -c : c);
+                cv[k] = (uint8_t)(vd[k] > 0. ? max(r, 1) : 0);
+            }
+            store4((int8_t*)t.m, cm, at, whole, lane, left);
+            store4((uint8_t*)t.v, cv, at, whole, lane, left);
+            if (lane == 0) {
+                t.ms[block] = mt;
+                t.vs[block] = vt;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) p[k] = __builtin_fmaf(-lr, __builtin_fmaf(t.decay, p[k], m[k] * c1 / (sqrtf(v[k] * c2) + a.eps)), p[k]);
+        store4(t.p, p, at, whole, lane, left);
+        if (t.copy) {
+            if (t.copy_type == APOE_F16) {
+                _Float16 h[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) h[k] = (_Float16)p[k];
+                store4((_Float16*)t.copy, h, at, whole, lane, left);
+            } else {
+                __bf16 h[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) h[k] = (__bf16)p[k];
+                store4((__bf16*)t.copy, h, at, whole, lane, left);
+            }
+        }
+    }
+}
+
+// Four values a thread from a block's beginning on.
+__global__ __launch_bounds__(256) void adamw_read(uint64_t n, const int8_t* m, const float* ms, const uint8_t* v, const float* vs, float* m_out, float* v_out, bool whole) {
+    const int lane = threadIdx.x & 63;
+    for (uint64_t at = ((uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * BLOCK; at < n; at += (uint64_t)gridDim.x * 4 * BLOCK) {
+        const uint32_t left = (uint32_t)min((uint64_t)BLOCK, n - at);
+        const bool w = whole && left == BLOCK;
+        int8_t cm[4];
+        uint8_t cv[4];
+        load4(cm, m, at, w, lane, left);
+        load4(cv, v, at, w, lane, left);
+        const float sm = ms[at / BLOCK], sv = vs[at / BLOCK];
+        float x[4], y[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            x[k] = (float)value_of_m(sm, cm[k]);
+            y[k] = (float)value_of_v(sv, cv[k]);
+        }
+        store4(m_out, x, at, w, lane, left);
+        store4(v_out, y, at, w, lane, left);
+    }
+}
+
+int launch_adamw(apoe_adamw* opt, const apoe_adamw_step_args* p) {
+    AdamArgs a{};
+    a.seed = opt->seed;
+    a.step = p->step;
+    a.step_dev = p->step_dev;
+    a.lr_dev = p->lr_dev;
+    a.b1 = p->beta1;
+    a.b2 = p->beta2;
+    a.grad_scale = p->grad_scale;
+    a.lr = (float)p->lr;
+    a.eps = (float)p->eps;
+    if (!p->step_dev) {
+        a.c1 = (float)(1. / (1. - power(a.b1, a.step)));
+        a.c2 = (float)(1. / (1. - power(a.b2, a.step)));
+    }
+    auto go = [&]() -> int {
+        if (a.pieces == 0) return APOE_OK;
+        if (opt->bits == 32) adamw_step<32><<<a.pieces, 256, 0, opt->ctx->stream>>>(a);
+        else adamw_step<8><<<a.pieces, 256, 0, opt->ctx->stream>>>(a);
+        a.count = a.pieces = 0;
+        APOE_HIP(hipGetLastError());
+        return APOE_OK;
+    };
+    for (size_t i = 0; i < opt->tensors.size(); i++) {
+        const apoe_adamw_tensor& t = opt->tensors[i];
+        if (!p->grads[i] || t.n == 0) continue;
+        const uint32_t pieces = (uint32_t)((t.n + ADAM_PIECE - 1) / ADAM_PIECE);
+        if (a.count == ADAM_LIST || a.pieces + (uint64_t)pieces > (1u << 23)) APOE_TRY(go());
+        const uintptr_t g = (uintptr_t)p->grads[i], c = (uintptr_t)t.copy;
+        const bool narrow = p->grad_dtypes[i] != APOE_F32;
+        bool whole = ((uintptr_t)t.p & 15) == 0 && (g & (narrow ? 7 : 15)) == 0 && (c & 7) == 0;
+        whole &= (((uintptr_t)t.m | (uintptr_t)t.v) & (opt->bits == 32 ? 15 : 3)) == 0;
+        a.t[a.count++] = AdamTensor{t.p, p->grads[i], t.m, t.v, t.m_scale, t.v_scale, t.copy, t.n, (float)t.decay, (uint32_t)i, a.pieces, (uint8_t)p->grad_dtypes[i],
+                                    (uint8_t)t.copy_dtype, (uint8_t)whole};
+        a.pieces += pieces;
+    }
+    return go();
+}
+
+int launch_adamw_moments(apoe_ctx* ctx, uint64_t n, const int8_t* m, const float* m_scale, const uint8_t* v, const float* v_scale, float* m_out, float* v_out) {
+    const bool whole = ((((uintptr_t)m | (uintptr_t)v) & 3) | (((uintptr_t)m_out | (uintptr_t)v_out) & 15)) == 0;
+    adamw_read<<<(uint32_t)std::min<uint64_t>((n + 1023) / 1024, 1u << 16), 256, 0, ctx->stream>>>(n, m, m_scale, v, v_scale, m_out, v_out, whole);
+    APOE_HIP(hipGetLastError());
+    return APOE_OK;
+}
+
+} // namespace apoe

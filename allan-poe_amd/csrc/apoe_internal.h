@@ -111,10 +111,34 @@ struct apoe_ctx {
         *out = search_ws.p;
         return APOE_OK;
     }
+    // Graphs that were captured from this context hold the address of the workspace as it was: one that has been captured is kept when a larger
+    // one takes its place (each at least twice as large, so that there are few), and none is made while a capture runs.
+    static constexpr int MOST_KEPT = 40;
+    void* kept_ws[MOST_KEPT] = {};
+    int n_kept = 0;
+    bool ws_captured = false;
     int adapt_workspace(size_t bytes, char** out) {
-        if (adapt_ws.n < bytes) APOE_TRY(adapt_ws.alloc(bytes));
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        if (stream && hipStreamIsCapturing(stream, &capture) != hipSuccess) (void)hipGetLastError();
+        const bool capturing = capture != hipStreamCaptureStatusNone;
+        if (adapt_ws.n < bytes) {
+            APOE_REQUIRE_STATE(!capturing, "the workspace would have to grow to %zu bytes during a capture: make the call once before", bytes);
+            if (ws_captured) {
+                APOE_REQUIRE_STATE(n_kept < MOST_KEPT, "too many workspaces in captured graphs");
+                bytes = bytes < 2 * adapt_ws.n ? 2 * adapt_ws.n : bytes;
+                kept_ws[n_kept++] = adapt_ws.p;
+                adapt_ws.p = nullptr;
+                adapt_ws.n = 0;
+                ws_captured = false;
+            }
+            APOE_TRY(adapt_ws.alloc(bytes));
+        }
+        ws_captured |= capturing;
         *out = adapt_ws.p;
         return APOE_OK;
+    }
+    void release_kept() {
+        while (n_kept) (void)hipFree(kept_ws[--n_kept]);
     }
 };
 
@@ -188,6 +212,12 @@ struct apoe_knn {
     apoe::DevBuf<uint32_t> open; // prune: what a node leaves to another form [n], how many are left to either, and which [n]
 };
 
+struct apoe_adamw {
+    apoe_ctx* ctx = nullptr;
+    uint32_t bits = 32, seed = 0;
+    std::vector<apoe_adamw_tensor> tensors;
+};
+
 namespace apoe {
 
 // Copies between caller memory (host or device) and library device memory.
@@ -225,6 +255,11 @@ int launch_final_graph(apoe_knn* g, uint32_t* rows_dev);
 int launch_softmax_loss(apoe_ctx* ctx, const apoe_softmax_loss_args* args); // strides filled in
 int launch_orthogonalize(apoe_ctx* ctx, const apoe_orthogonalize_args* args);
 int launch_gated_residual(apoe_ctx* ctx, const apoe_gated_residual_args* args, bool grad);
+int launch_layer_norm(apoe_ctx* ctx, const apoe_layer_norm_args* args, bool grad);
+int launch_embed(apoe_ctx* ctx, const apoe_embed_args* args, bool grad);
+int launch_linear(apoe_ctx* ctx, const apoe_linear_args* args, bool grad);
+int launch_adamw(apoe_adamw* opt, const apoe_adamw_step_args* args);
+int launch_adamw_moments(apoe_ctx* ctx, uint64_t n, const int8_t* m, const float* m_scale, const uint8_t* v, const float* v_scale, float* m_out, float* v_out);
 
 // Times `fn` (which enqueues work on ctx->stream) with HIP events; blocks until done.
 template <typename F>

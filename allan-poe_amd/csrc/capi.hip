@@ -201,6 +201,7 @@ int apoe_ctx_create_on_stream(int device, void* stream, apoe_ctx** out) { return
 void apoe_ctx_destroy(apoe_ctx* ctx) {
     if (!ctx) return;
     if (ctx->stream || !ctx->own_stream) (void)hipStreamSynchronize(ctx->stream);
+    ctx->release_kept();
     if (ctx->ev0) (void)hipEventDestroy(ctx->ev0);
     if (ctx->ev1) (void)hipEventDestroy(ctx->ev1);
     for (int b = 0; b < 2; b++) {

@@ -1,0 +1,522 @@
+// A linear layer and its gradient:
+//   z = x w^T + b, y = act(z) + residual;   gz = gy act'(z), gx = gz w, gw = gz^T x, gb = sum of gz's rows.
+//
+// Three products of one kernel: an operand's inner dimension goes along its rows (x, w, and gz for gx) or down them (w for gx, both for gw; read
+// transposed from LDS). 16-bit matrices are taken as they lie; float ones as three bfloat16 planes that hold their 24 bits exactly, six products
+// of which (those above 2^-24) are added up: as accurate value by value as float products, whatever the exponents are, at 1381 / 6 = 230
+// TFLOP/s where the float matrix units have 154. What is done to a result (bias, activation, residual, rounding) is done behind the last stage,
+// through LDS, 16 bytes a thread. Where tiles are too few for the GPU the inner dimension is cut and a second launch adds the cuts up, in order.
+// Up to 64 rows a kernel of its own streams w once (the serving form).
+#include <algorithm>
+
+#include "apoe_internal.h"
+#include "apoe_tile.h"
+
+namespace apoe {
+
+struct LinOut { // what becomes of a product's sums
+    void* out;
+    const float* bias;      // by columns
+    const void* residual;
+    void* pre;
+    uint64_t out_stride, residual_stride, pre_stride;
+    uint32_t m, n, act;
+    bool whole;             // every row begins at a multiple of 16 bytes, and so does the bias
+};
+
+struct LinTile {
+    const void *a, *b;      // 16-bit values, or planes of such
+    uint64_t a_low, b_low;  // from plane to plane
+    uint32_t a_pitch, b_pitch; // bytes
+    uint32_t k, nt;         // inner side, tiles along a row of tiles
+    uint32_t cuts, cut_stages;
+    float* part;            // [cuts][m][np]
+    uint32_t np;
+    LinOut o;
+};
+
+// Phi(-u), the normal distribution's tail, for u >= 0, and its density there: exp(-u u / 2) times a polynomial in 1 / (1 + c u), fitted to
+// erfc's scaled form (relative error 6e-8; with the rounding of the exponent (4 + u u) 2^-24).
+__device__ inline float normal_tail(float u, float& density) {
+    const float e = __builtin_amdgcn_exp2f(-0.72134752f * (u * u)), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.28284271f, u, 1.f));
+    density = 0.39894228f * e;
+    float s = 0.0201337803f;
+    s = __builtin_fmaf(s, t, -0.0677357092f);
+    s = __builtin_fmaf(s, t, 0.0369214416f);
+    s = __builtin_fmaf(s, t, 0.0498643406f);
+    s = __builtin_fmaf(s, t, 0.0357544832f);
+    s = __builtin_fmaf(s, t, 0.0984813645f);
+    s = __builtin_fmaf(s, t, 0.100479335f);
+    s = __builtin_fmaf(s, t, 0.113287851f);
+    s = __builtin_fmaf(s, t, 0.112813152f);
+    return s * t * e;
+}
+
+__device__ inline float activate(float z, uint32_t act) {
+    if (act == APOE_ACT_RELU) return z < 0.f ? 0.f : z;
+    if (act == APOE_ACT_GELU) {
+        float d;
+        const float q = normal_tail(fabsf(z), d);
+        return z * (z > 0.f ? 1.f - q : q);
+    }
+    if (act == APOE_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * z));
+    return z;
+}
+
+__device__ inline float slope(float z, uint32_t act) {
+    if (act == APOE_ACT_RELU) return z > 0.f ? 1.f : 0.f;
+    if (act == APOE_ACT_GELU) {
+        float d;
+        const float q = normal_tail(fabsf(z), d);
+        return __builtin_fmaf(z, d, z > 0.f ? 1.f - q : q);
+    }
+    if (act == APOE_ACT_SILU) { // o (1 + z (1 - o))
+        const float o = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * z)), rest = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(1.44269504f * z));
+        return o * __builtin_fmaf(z, rest, 1.f);
+    }
+    return 1.f;
+}
+
+// Eight values of a row as numbers, `left` of them there (whole: eight, from a multiple of 16 bytes).
+template <typename T> __device__ inline void take8(float* v, const void* p, uint64_t at, bool whole, uint32_t left) {
+    const T* from = (const T*)p + at;
+    if (whole) {
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(from), y = *reinterpret_cast<const f32x4*>(from + 4);
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = k < 4 ? x[k] : y[k - 4];
+        } else {
+            typedef T t8 __attribute__((ext_vector_type(8)));
+            const t8 x = *reinterpret_cast<const t8*>(from);
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = (float)x[k];
+        }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = (uint32_t)k < left ? (float)from[k] : 0.f;
+}
+template <typename T> __device__ inline void give8(void* p, uint64_t at, const float* v, bool whole, uint32_t left) {
+    T* to = (T*)p + at;
+    if (whole) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4*>(to + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
+            typedef T t8 __attribute__((ext_vector_type(8)));
+            t8 x;
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = (T)v[k];
+            *reinterpret_cast<t8*>(to) = x;
+        }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+        if ((uint32_t)k < left) to[k] = (T)v[k];
+}
+
+// Eight sums of row i from column j on. T: the type of the results.
+template <typename T> __device__ inline void finish8(const LinOut& o, uint32_t i, uint32_t j, float* v) {
+    const bool whole = o.whole && j + 8 <= o.n;
+    const uint32_t left = o.n - j;
+    if (o.bias) {
+        float b[8];
+        take8<float>(b, o.bias, j, whole, left);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] += b[k];
+    }
+    if (o.pre) give8<T>(o.pre, i * o.pre_stride + j, v, whole, left);
+    if (o.act != APOE_ACT_NONE) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = activate(v[k], o.act);
+    }
+    if (o.residual) {
+        float r[8];
+        take8<T>(r, o.residual, i * o.residual_stride + j, whole, left);
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] += r[k];
+    }
+    give8<T>(o.out, i * o.out_stride + j, v, whole, left);
+}
+
+// S: the operands' type, P planes of it; T: the results'. ACOL, BCOL: the inner dimension goes down the rows.
+template <typename S, typename T, int P, bool ACOL, bool BCOL, int MT, int NT, int WM, int WN, int KG, int SF, int ST>
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_tile(LinTile a) {
+    constexpr int NW = WM * WN * KG, FS = SF / KG, BM = WM * MT * 32, BN = WN * NT * 32;
+    using ATile = std::conditional_t<ACOL, ColTile<S, BM, SF, NW, ORDER_ROWS>, RowTile<S, BM, SF, NW>>;
+    using BTile = std::conditional_t<BCOL, ColTile<S, BN, SF, NW, ORDER_ROWS>, RowTile<S, BN, SF, NW>>;
+    constexpr int PLANE = ATile::BYTES + BTile::BYTES, STAGE = P * PLANE, PER = P * (ATile::LOADS + BTile::LOADS), KE = ATile::KE;
+    __shared__ __align__(1024) char lds[ST * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / (WM * WN), wm = wave % (WM * WN) / WN, wn = wave % WN;
+    const uint32_t m = a.o.m, n = a.o.n;
+    const uint32_t id = xcd_run(blockIdx.x, gridDim.x), tile = id / a.cuts, cut = id % a.cuts;
+    const uint32_t row = tile / a.nt * BM, col = tile % a.nt * BN;
+    const uint32_t s0 = cut * a.cut_stages, stages = min(a.cut_stages, (a.k + KE - 1) / KE - s0);
+    const int mrows = (int)min((uint32_t)BM, m - row), ncols = (int)min((uint32_t)BN, n - col);
+    ATile ta[P];
+    BTile tb[P];
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+        const char* pa = (const char*)a.a + p * a.a_low * sizeof(S);
+        const char* pb = (const char*)a.b + p * a.b_low * sizeof(S);
+        if constexpr (ACOL) ta[p].init((const S*)(pa + (uint64_t)s0 * KE * a.a_pitch) + row, a.a_pitch, (mrows + 7) / 8 * 8, wave, lane);
+        else ta[p].init((const S*)(pa + (uint64_t)row * a.a_pitch) + (uint64_t)s0 * KE, a.a_pitch, mrows, wave, lane);
+        if constexpr (BCOL) tb[p].init((const S*)(pb + (uint64_t)s0 * KE * a.b_pitch) + col, a.b_pitch, (ncols + 7) / 8 * 8, wave, lane);
+        else tb[p].init((const S*)(pb + (uint64_t)col * a.b_pitch) + (uint64_t)s0 * KE, a.b_pitch, ncols, wave, lane);
+    }
+    const uint32_t base = lds_address(lds);
+    int left = (int)min(stages * KE, a.k - s0 * KE); // of the inner side; a row's values are followed by zeros up to a multiple of eight
+    uint32_t into = 0;
+    auto issue = [&]() {
+        const auto one = [&](auto& t, uint32_t at, auto down) {
+            if constexpr (decltype(down)::value) {
+                using Mask = typename std::remove_reference_t<decltype(t)>::Mask;
+                t.load(at, left >= KE ? t.ALL : left > 0 ? (Mask)(((Mask)1 << left) - 1) : (Mask)0, wave, lane);
+            } else {
+                t.load(at, (left + 7) / 8 * 16, wave);
+            }
+            t.next();
+        };
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            one(ta[p], base + into + p * PLANE, std::integral_constant<bool, ACOL>{});
+            one(tb[p], base + into + p * PLANE + ATile::BYTES, std::integral_constant<bool, BCOL>{});
+        }
+        left -= KE;
+        into = into + STAGE == ST * STAGE ? 0 : into + STAGE;
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; s++) issue();
+    f32x16 acc[MT][NT] = {};
+    uint32_t from = 0;
+    for (uint32_t s = 0; s < stages; s++) {
+        tile_wait<(ST - 2) * PER>();
+        const char* A = lds + from;
+        const char* B = A + ATile::BYTES;
+        i32x4 x[2][P][MT], y[2][P][NT];
+        auto read = [&](int f) {
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+#pragma unroll
+                for (int i = 0; i < MT; i++) x[f & 1][p][i] = ATile::read(A + p * PLANE, wm * MT + i, kg * FS + f, lane);
+#pragma unroll
+                for (int t = 0; t < NT; t++) y[f & 1][p][t] = BTile::read(B + p * PLANE, wn * NT + t, kg * FS + f, lane);
+            }
+        };
+        read(0);
+        issue();
+#pragma unroll
+        for (int f = 0; f < FS; f++) {
+            if (f + 1 < FS) read(f + 1);
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int total = P - 1; total >= 0; total--) // the smaller products first
+#pragma unroll
+                        for (int p = 0; p <= total; p++) acc[i][t] = mfma_step<S>(x[f & 1][p][i], y[f & 1][total - p][t], acc[i][t]);
+        }
+        interleave<P * ((ACOL ? 2 : 1) * MT + (BCOL ? 2 : 1) * NT), P * (P + 1) / 2 * MT * NT, FS>();
+        from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
+    }
+    tile_wait<0>();
+    if constexpr (KG == 2) {
+        static_assert(BM * BN * 4 <= ST * STAGE, "the sums fit the stages");
+        exchange_halves<MT, NT, WM * WN>(acc, lds, kg, wave % (WM * WN), lane);
+        __syncthreads();
+    }
+    // one block of 32 rows a wave at a time through LDS: then a thread has eight values of a row
+    constexpr int PITCH = BN + 4, ROWS = WM * 32, ITEMS = ROWS * BN / 8 / (64 * NW);
+    static_assert(ROWS * PITCH * 4 <= ST * STAGE && ROWS * BN % (512 * NW) == 0, "the sums fit the stages");
+    float* sum = reinterpret_cast<float*>(lds);
+    const int half = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        if (KG == 1 || i / (MT / KG) == kg) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) sum[(wm * 32 + result_row(k, half)) * PITCH + (wn * NT + t) * 32 + (lane & 31)] = acc[i][t][k];
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int item = 0; item < ITEMS; item++) {
+            const uint32_t at = item * 64 * NW + threadIdx.x, r = at / (BN / 8), c = at % (BN / 8) * 8;
+            const uint32_t gi = row + (r / 32 * MT + i) * 32 + r % 32, gj = col + c;
+            if (gi >= m || gj >= n) continue;
+            const f32x4 v0 = *reinterpret_cast<const f32x4*>(sum + r * PITCH + c), v1 = *reinterpret_cast<const f32x4*>(sum + r * PITCH + c + 4);
+            if (a.cuts > 1) {
+                float* to = a.part + ((uint64_t)cut * m + gi) * a.np + gj;
+                *reinterpret_cast<f32x4*>(to) = v0;
+                *reinterpret_cast<f32x4*>(to + 4) = v1;
+            } else {
+                float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                finish8<T>(a.o, gi, gj, v);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// The cuts' sums, eight columns a thread.
+template <typename T> __global__ __launch_bounds__(256) void linear_join(LinTile a) {
+    const uint32_t per = a.np / 8;
+    const uint64_t total = (uint64_t)a.o.m * per;
+    for (uint64_t at = (uint64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (uint64_t)gridDim.x * 256) {
+        const uint32_t i = (uint32_t)(at / per), j = (uint32_t)(at % per) * 8;
+        f32x4 s0 = {}, s1 = {};
+#pragma unroll 4
+        for (uint32_t c = 0; c < a.cuts; c++) {
+            const float* from = a.part + ((uint64_t)c * a.o.m + i) * a.np + j;
+            s0 += *reinterpret_cast<const f32x4*>(from);
+            s1 += *reinterpret_cast<const f32x4*>(from + 4);
+        }
+        float v[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
+        finish8<T>(a.o, i, j, v);
+    }
+}
+
+// ---- operands in the products' form, gz, and the columns' sums ----
+
+struct LinPack {
+    const void *src, *pre;  // pre: multiply by the activation's slope there
+    uint64_t src_stride, pre_stride;
+    void* dst;              // [rows][pitch] a plane, zeros behind a row's end; NULL: sums alone
+    uint64_t low;           // values from plane to plane
+    uint32_t rows, cols, pitch, act;
+    float* part;            // [strips][cols] sums of columns, or NULL
+    bool whole;
+};
+
+// A thread has eight columns and every fourth row of a strip: grid (columns / 512, strips).
+template <typename T> __global__ __launch_bounds__(256) void linear_pack(LinPack a) {
+    constexpr bool SPLIT = sizeof(T) == 4;
+    __shared__ float sums[4][512];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = blockIdx.x * 512 + lane * 8;
+    float s[8] = {};
+    if (j < a.pitch) {
+        const bool whole = a.whole && j + 8 <= a.cols;
+        const uint32_t left = j < a.cols ? a.cols - j : 0;
+#pragma unroll 2
+        for (uint64_t i = (uint64_t)blockIdx.y * 4 + wave; i < a.rows; i += gridDim.y * 4ull) {
+            float v[8];
+            take8<T>(v, a.src, i * a.src_stride + j, whole, left);
+            if (a.pre) {
+                float z[8];
+                take8<T>(z, a.pre, i * a.pre_stride + j, whole, left);
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] *= slope(z[k], a.act);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) s[k] += v[k];
+            if (!a.dst) continue;
+            if constexpr (SPLIT) { // a plane holds what the ones before it left, rounded to 8 bits: the third one holds the rest exactly
+#pragma unroll
+                for (int p = 0; p < 3; p++) {
+                    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+                    b8 w;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        __bf16 top = (__bf16)v[k];
+                        if (p == 0 && __builtin_isinf((float)top)) top = (__bf16)__uint_as_float(__float_as_uint(v[k]) & 0xffff0000u); // just below the largest float
+                        w[k] = top;
+                        v[k] -= (float)top;
+                    }
+                    *reinterpret_cast<b8*>((__bf16*)a.dst + p * a.low + i * a.pitch + j) = w;
+                }
+            } else {
+                give8<T>(a.dst, i * a.pitch + j, v, true, 8);
+            }
+        }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int k = 0; k < 8; k++) sums[wave][lane * 8 + k] = s[k];
+    __syncthreads();
+    for (uint32_t c = threadIdx.x; c < 512; c += 256)
+        if (blockIdx.x * 512 + c < a.cols) a.part[(uint64_t)blockIdx.y * a.cols + blockIdx.x * 512 + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+}
+
+// Columns' sums over the strips: 16 columns a workgroup, 64 threads each.
+__global__ __launch_bounds__(1024) void linear_bias(const float* part, uint32_t strips, uint32_t cols, float* out) {
+    __shared__ float q[64][17];
+    const uint32_t c = threadIdx.x & 15, l = threadIdx.x >> 4, d = blockIdx.x * 16 + c;
+    float s = 0.f;
+    if (d < cols)
+#pragma unroll 4
+        for (uint32_t b = l; b < strips; b += 64) s += part[(uint64_t)b * cols + d];
+    q[l][c] = s;
+    for (uint32_t k = 32; k; k >>= 1) {
+        __syncthreads();
+        if (l < k) q[l][c] += q[l + k][c];
+    }
+    if (l == 0 && d < cols) out[d] = q[0][c];
+}
+
+// ---- host ----
+
+struct LinOperand { // as the products take it
+    const void* p;
+    uint64_t low;
+    uint32_t pitch; // bytes
+};
+
+constexpr uint32_t LIN_STRIPS = 256; // of rows under one partial sum of the bias' gradient, at most
+
+// Whether a matrix can be taken where it lies.
+static bool as_it_is(const void* p, uint64_t stride, uint32_t cols, bool split) {
+    return !split && cols % 8 == 0 && stride % 8 == 0 && stride <= (1u << 21) && ((uintptr_t)p & 15) == 0;
+}
+
+struct LinPlan {
+    uint64_t bytes = 0;
+    uint64_t take(uint64_t b) {
+        const uint64_t at = bytes;
+        bytes += (b + 1023) / 1024 * 1024;
+        return at;
+    }
+};
+
+static uint32_t pitch_of(uint32_t cols) { return (cols + 7) / 8 * 8; }
+
+template <typename T> static uint64_t packed_bytes(uint64_t rows, uint32_t cols) { return rows * pitch_of(cols) * 2 * (sizeof(T) == 4 ? 3 : 1); }
+
+template <typename T>
+static void pack(apoe_ctx* ctx, const void* src, uint64_t stride, uint32_t rows, uint32_t cols, void* dst, const void* pre, uint64_t pre_stride, uint32_t act, float* part, uint32_t* strips) {
+    LinPack a{src, pre, stride, pre_stride, dst, (uint64_t)rows * pitch_of(cols), rows, cols, pitch_of(cols), act, part, false};
+    constexpr uint32_t V = 16 / sizeof(T);
+    a.whole = ((uintptr_t)src & 15) == 0 && stride % V == 0 && (!pre || (((uintptr_t)pre & 15) == 0 && pre_stride % V == 0));
+    const uint32_t across = (a.pitch + 511) / 512;
+    const uint32_t down = std::max(1u, std::min({(rows + 3) / 4, LIN_STRIPS, std::max(1u, (uint32_t)ctx->num_cus * 8 / across)}));
+    if (strips) *strips = down;
+    linear_pack<T><<<dim3(across, down), 256, 0, ctx->stream>>>(a);
+}
+
+struct LinShape {
+    uint32_t bm, bn, kind, cuts, cut_stages, ke;
+};
+
+template <typename S, typename T, int P, bool ACOL, bool BCOL> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t n, uint32_t k) {
+    const uint32_t cus = (uint32_t)ctx->num_cus;
+    auto tiles = [&](uint32_t bm, uint32_t bn) { return (uint64_t)((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
+    LinShape s{};
+    if (P == 1 && tiles(256, 256) >= cus * 4 / 5) s = LinShape{256, 256, 0, 1, 0, 64};
+    else if (tiles(128, 128) >= cus * 4 / 5) s = LinShape{128, 128, 1, 1, 0, P == 1 ? 64u : 32u};
+    else s = LinShape{64, 64, 2, 1, 0, P == 1 ? 64u : 32u};
+    const uint32_t stages = (k + s.ke - 1) / s.ke;
+    const uint64_t t = tiles(s.bm, s.bn);
+    const uint32_t least = 512 / s.ke;
+    s.cuts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(cus / t, stages / least));
+    s.cut_stages = std::max(1u, (stages + s.cuts - 1) / s.cuts);
+    s.cuts = std::max(1u, (stages + s.cut_stages - 1) / s.cut_stages);
+    return s;
+}
+
+static uint64_t cut_bytes(const LinShape& s, uint32_t m, uint32_t n) { return s.cuts > 1 ? (uint64_t)s.cuts * m * pitch_of(n) * 4 : 0; }
+
+template <typename S, typename T, int P, bool ACOL, bool BCOL>
+static void product(apoe_ctx* ctx, const LinShape& s, LinOperand a, LinOperand b, uint32_t k, float* part, const LinOut& o) {
+    LinTile t{a.p, b.p, a.low, b.low, a.pitch, b.pitch, k, (o.n + s.bn - 1) / s.bn, s.cuts, s.cut_stages, part, pitch_of(o.n), o};
+    const uint32_t grid = (uint32_t)((uint64_t)((o.m + s.bm - 1) / s.bm) * t.nt * s.cuts);
+    hipStream_t st = ctx->stream;
+    if constexpr (P == 1) {
+        if (s.kind == 0) linear_tile<S, T, P, ACOL, BCOL, 4, 2, 2, 4, 1, 4, 2><<<grid, 512, 0, st>>>(t);
+        else if (s.kind == 1) linear_tile<S, T, P, ACOL, BCOL, 2, 1, 2, 4, 1, 4, 2><<<grid, 512, 0, st>>>(t);
+        else linear_tile<S, T, P, ACOL, BCOL, 1, 1, 2, 2, 1, 4, 4><<<grid, 256, 0, st>>>(t);
+    } else {
+        if (s.kind == 1) linear_tile<S, T, P, ACOL, BCOL, 2, 2, 2, 2, 2, 2, 3><<<grid, 512, 0, st>>>(t);
+        else linear_tile<S, T, P, ACOL, BCOL, 1, 1, 2, 2, 1, 2, 3><<<grid, 256, 0, st>>>(t);
+    }
+    if (s.cuts > 1) linear_join<T><<<(uint32_t)std::min<uint64_t>(((uint64_t)o.m * (t.np / 8) + 255) / 256, 1u << 16), 256, 0, st>>>(t);
+}
+
+template <typename T> static bool whole_out(const void* p, uint64_t stride) { return ((uintptr_t)p & 15) == 0 && stride % (16 / sizeof(T)) == 0; }
+
+template <typename T> struct LinTypes {
+    using S = T;
+    static constexpr int P = 1;
+};
+template <> struct LinTypes<float> {
+    using S = __bf16;
+    static constexpr int P = 3;
+};
+
+template <typename T> static int run_linear(apoe_ctx* ctx, const apoe_linear_args* p) {
+    using S = typename LinTypes<T>::S;
+    constexpr int P = LinTypes<T>::P;
+    const uint32_t m = p->rows, n = p->cols_out, k = p->cols_in;
+    const bool x_is = as_it_is(p->x, p->x_stride, k, P > 1), w_is = as_it_is(p->w, p->w_stride, k, P > 1);
+    const LinShape s = choose<S, T, P, false, false>(ctx, m, n, k);
+    LinPlan plan;
+    const uint64_t o_x = plan.take(x_is ? 0 : packed_bytes<T>(m, k)), o_w = plan.take(w_is ? 0 : packed_bytes<T>(n, k)), o_part = plan.take(cut_bytes(s, m, n));
+    char* ws = nullptr;
+    if (plan.bytes) APOE_TRY(ctx->adapt_workspace(plan.bytes, &ws));
+    LinOperand x{p->x, 0, (uint32_t)(p->x_stride * sizeof(S))}, w{p->w, 0, (uint32_t)(p->w_stride * sizeof(S))};
+    if (!x_is) {
+        x = LinOperand{ws + o_x, (uint64_t)m * pitch_of(k), pitch_of(k) * (uint32_t)sizeof(S)};
+        pack<T>(ctx, p->x, p->x_stride, m, k, ws + o_x, nullptr, 0, 0, nullptr, nullptr);
+    }
+    if (!w_is) {
+        w = LinOperand{ws + o_w, (uint64_t)n * pitch_of(k), pitch_of(k) * (uint32_t)sizeof(S)};
+        pack<T>(ctx, p->w, p->w_stride, n, k, ws + o_w, nullptr, 0, 0, nullptr, nullptr);
+    }
+    LinOut o{p->y, p->bias, p->residual, p->pre, p->y_stride, p->residual_stride, p->pre_stride, m, n, p->act, false};
+    o.whole = whole_out<T>(p->y, p->y_stride) && whole_out<T>(p->residual, p->residual_stride) && whole_out<T>(p->pre, p->pre_stride) && ((uintptr_t)p->bias & 15) == 0;
+    product<S, T, P, false, false>(ctx, s, x, w, k, (float*)(ws + o_part), o);
+    APOE_HIP(hipGetLastError());
+    return APOE_OK;
+}
+
+template <typename T> static int run_linear_grad(apoe_ctx* ctx, const apoe_linear_args* p) {
+    using S = typename LinTypes<T>::S;
+    constexpr int P = LinTypes<T>::P;
+    const uint32_t m = p->rows, n = p->cols_out, k = p->cols_in;
+    const bool act = p->act != APOE_ACT_NONE, products = p->grad_x || p->grad_w;
+    const bool g_is = !act && as_it_is(p->grad_y, p->grad_y_stride, n, P > 1), x_is = !p->grad_w || as_it_is(p->x, p->x_stride, k, P > 1), w_is = !p->grad_x || as_it_is(p->w, p->w_stride, k, P > 1);
+    const bool pack_g = products && !g_is;
+    LinShape sx{}, sw{};
+    if (p->grad_x) sx = choose<S, T, P, false, true>(ctx, m, k, n);
+    if (p->grad_w) sw = choose<S, T, P, true, true>(ctx, n, k, m);
+    LinPlan plan;
+    const uint64_t o_g = plan.take(pack_g ? packed_bytes<T>(m, n) : 0), o_x = plan.take(x_is ? 0 : packed_bytes<T>(m, k)), o_w = plan.take(w_is ? 0 : packed_bytes<T>(n, k));
+    const uint64_t o_part = plan.take(std::max({p->grad_x ? cut_bytes(sx, m, k) : 0, p->grad_w ? cut_bytes(sw, n, k) : 0, p->grad_bias ? (uint64_t)LIN_STRIPS * n * 4 : 0}));
+    char* ws = nullptr;
+    if (plan.bytes) APOE_TRY(ctx->adapt_workspace(plan.bytes, &ws));
+    LinOperand g{p->grad_y, 0, (uint32_t)(p->grad_y_stride * sizeof(S))}, x{p->x, 0, (uint32_t)(p->x_stride * sizeof(S))}, w{p->w, 0, (uint32_t)(p->w_stride * sizeof(S))};
+    if (pack_g || p->grad_bias) {
+        uint32_t strips = 0;
+        pack<T>(ctx, p->grad_y, p->grad_y_stride, m, n, pack_g ? ws + o_g : nullptr, act ? p->pre : nullptr, p->pre_stride, p->act, p->grad_bias ? (float*)(ws + o_part) : nullptr, &strips);
+        if (p->grad_bias) linear_bias<<<(n + 15) / 16, 1024, 0, ctx->stream>>>((const float*)(ws + o_part), strips, n, p->grad_bias);
+        if (pack_g) g = LinOperand{ws + o_g, (uint64_t)m * pitch_of(n), pitch_of(n) * (uint32_t)sizeof(S)};
+    }
+    if (!x_is) {
+        x = LinOperand{ws + o_x, (uint64_t)m * pitch_of(k), pitch_of(k) * (uint32_t)sizeof(S)};
+        pack<T>(ctx, p->x, p->x_stride, m, k, ws + o_x, nullptr, 0, 0, nullptr, nullptr);
+    }
+    if (!w_is) {
+        w = LinOperand{ws + o_w, (uint64_t)n * pitch_of(k), pitch_of(k) * (uint32_t)sizeof(S)};
+        pack<T>(ctx, p->w, p->w_stride, n, k, ws + o_w, nullptr, 0, 0, nullptr, nullptr);
+    }
+    if (p->grad_x && m) {
+        LinOut o{p->grad_x, nullptr, nullptr, nullptr, p->grad_x_stride, 0, 0, m, k, APOE_ACT_NONE, whole_out<T>(p->grad_x, p->grad_x_stride)};
+        product<S, T, P, false, true>(ctx, sx, g, w, n, (float*)(ws + o_part), o);
+    }
+    if (p->grad_w) {
+        LinOut o{p->grad_w, nullptr, nullptr, nullptr, p->grad_w_stride, 0, 0, n, k, APOE_ACT_NONE, whole_out<T>(p->grad_w, p->grad_w_stride)};
+        product<S, T, P, true, true>(ctx, sw, g, x, m, (float*)(ws + o_part), o);
+    }
+    APOE_HIP(hipGetLastError());
+    return APOE_OK;
+}
+
+int launch_linear(apoe_ctx* ctx, const apoe_linear_args* p, bool grad) {
+    switch (p->dtype) {
+    case APOE_F32: return grad ? run_linear_grad<float>(ctx, p) : run_linear<float>(ctx, p);
+    case APOE_F16: return grad ? run_linear_grad<_Float16>(ctx, p) : run_linear<_Float16>(ctx, p);
+    default: return grad ? run_linear_grad<__bf16>(ctx, p) : run_linear<__bf16>(ctx, p);
+    }
+}
+
+} // namespace apoe

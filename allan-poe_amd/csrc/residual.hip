@@ -13,10 +13,11 @@
 // one wave a SIMD, with no loads on their way meanwhile (262 144 bf16 rows of 256: forward 126 us, 5.3 TB/s; gradient 324 us, 3.3 TB/s; of 128
 // columns, which leave half of a thread's values empty, 374 us for both, 1.8 TB/s).
 #include "apoe_internal.h"
+#include "apoe_rows.h"
 
 namespace apoe {
 
-constexpr int RES_E = 16;            // values of a row that a thread holds
+constexpr int RES_E = ROW_E;         // values of a row that a thread holds
 constexpr uint32_t RES_BLOCKS = 512; // workgroups of the gradient, at most: rows of the partial sums
 
 struct ResArgs {
@@ -25,102 +26,6 @@ struct ResArgs {
     uint32_t blocks;
     bool aligned; // the vectors begin at multiples of 16 bytes
 };
-
-// Values (c G + t) V .. of a row, c = 0, 1, ..: 16 bytes a load with V > 1.
-template <typename T, int V, int G> struct RowOf {
-    typedef T tv __attribute__((ext_vector_type(V)));
-    static constexpr int C = RES_E / V;
-    // as it comes, and as numbers
-    __device__ static void fetch(tv* raw, const void* p, uint64_t row, uint64_t stride, uint32_t dim, int t) {
-        const T* at = (const T*)p + row * stride;
-#pragma unroll
-        for (int c = 0; c < C; c++) {
-            const uint32_t d = (c * G + t) * V;
-            raw[c] = tv{};
-            if constexpr (V == 1) {
-                if (d < dim) raw[c][0] = at[d];
-            } else {
-                if (d < dim) raw[c] = *reinterpret_cast<const tv*>(at + d);
-            }
-        }
-    }
-    __device__ static void widen(float* v, const tv* raw) {
-#pragma unroll
-        for (int c = 0; c < C; c++)
-#pragma unroll
-            for (int k = 0; k < V; k++) v[c * V + k] = (float)raw[c][k];
-    }
-    __device__ static void load(float* v, const void* p, uint64_t row, uint64_t stride, uint32_t dim, int t) {
-        tv raw[C];
-        fetch(raw, p, row, stride, dim, t);
-        widen(v, raw);
-    }
-    __device__ static void store(void* p, uint64_t row, uint64_t stride, uint32_t dim, int t, const float* v) {
-        T* at = (T*)p + row * stride;
-#pragma unroll
-        for (int c = 0; c < C; c++) {
-            const uint32_t d = (c * G + t) * V;
-            if (d >= dim) continue;
-            if constexpr (V == 1) {
-                at[d] = (T)v[c];
-            } else {
-                tv x;
-#pragma unroll
-                for (int k = 0; k < V; k++) x[k] = (T)v[c * V + k];
-                *reinterpret_cast<tv*>(at + d) = x;
-            }
-        }
-    }
-    // a vector of floats (ones without one)
-    __device__ static void vec(float* v, const float* p, uint32_t dim, int t, bool aligned) {
-        if constexpr (V > 1) {
-            if (p && aligned) {
-                typedef float f4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-                for (int c = 0; c < C; c++) {
-                    const uint32_t d = (c * G + t) * V;
-#pragma unroll
-                    for (int q = 0; q < V / 4; q++) {
-                        const f4 x = d < dim ? *reinterpret_cast<const f4*>(p + d + 4 * q) : f4{};
-#pragma unroll
-                        for (int k = 0; k < 4; k++) v[c * V + 4 * q + k] = x[k];
-                    }
-                }
-                return;
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < C; c++)
-#pragma unroll
-            for (int k = 0; k < V; k++) {
-                const uint32_t d = (c * G + t) * V + k;
-                v[c * V + k] = d < dim ? (p ? p[d] : 1.f) : 0.f;
-            }
-    }
-};
-
-// N sums over the threads of a group, the same for all of them.
-template <int G, int N> __device__ inline void group_sum(float* v, float (*buf)[8]) {
-#pragma unroll
-    for (int d = G < 64 ? G / 2 : 32; d; d >>= 1)
-#pragma unroll
-        for (int n = 0; n < N; n++) v[n] += __shfl_xor(v[n], d);
-    if constexpr (G > 64) { // one row a workgroup
-        const int w = threadIdx.x >> 6;
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0)
-#pragma unroll
-            for (int n = 0; n < N; n++) buf[n][w] = v[n];
-        __syncthreads();
-#pragma unroll
-        for (int n = 0; n < N; n++) {
-            float s = buf[n][0];
-#pragma unroll
-            for (int k = 1; k < G / 64; k++) s += buf[n][k];
-            v[n] = s;
-        }
-    }
-}
 
 __device__ inline float sigmoid(float g) { return 1.f / (1.f + expf(-g)); }
 
@@ -372,12 +277,7 @@ template <typename T, int V> static int run_residual(apoe_ctx* ctx, const apoe_g
         if (vectors) residual_vectors<T><<<(p->dim + 15) / 16, 1024, 0, s>>>(a);
         return APOE_OK;
     };
-    int st;
-    if (p->dim <= 16 * RES_E) st = go(std::integral_constant<int, 16>{});
-    else if (p->dim <= 64 * RES_E) st = go(std::integral_constant<int, 64>{});
-    else if (p->dim <= 256 * RES_E) st = go(std::integral_constant<int, 256>{});
-    else st = go(std::integral_constant<int, 512>{});
-    APOE_TRY(st);
+    APOE_TRY(with_group(p->dim, go));
     APOE_HIP(hipGetLastError());
     return APOE_OK;
 }

@@ -44,6 +44,7 @@ typedef struct apoe_queries apoe_queries;
 typedef struct apoe_kg apoe_kg;
 typedef struct apoe_graph apoe_graph;
 typedef struct apoe_knn apoe_knn;
+typedef struct apoe_adamw apoe_adamw;
 
 const char* apoe_last_error_string(void);
 
@@ -393,6 +394,134 @@ typedef struct {
  */
 int apoe_gated_residual(apoe_ctx* ctx, const apoe_gated_residual_args* args);
 int apoe_gated_residual_grad(apoe_ctx* ctx, const apoe_gated_residual_args* args);
+
+/*
+ * What an adapter with layers of its own, or a small encoder in front of the index, is built and trained from beside these: rows of a table
+ * summed up (terms of the learned-sparse path, tokens), layer norm, matrix products with what is done to their results, and the step of
+ * all parameters. The rules above hold: the context's stream, device pointers, strides from row to row (0: dense), workspace that the context
+ * keeps. Rows may begin at any multiple of their type's size; such as begin at multiples of 16 bytes are read 16 bytes at a time.
+ */
+#define APOE_EMBED_MAX_DIM 8192u
+#define APOE_NORM_MAX_DIM 8192u
+#define APOE_LINEAR_MAX_SIDE 65536u /* columns of x and of y */
+
+typedef struct {
+    uint32_t dtype;                 /* of table, base, out, grad and grad_table; sums and weights are float */
+    uint32_t n_rows, n_table, n_entries, dim; /* n_table < 2^30, n_entries < 2^27; off == NULL: n_entries == n_rows */
+    const void* table;              /* [n_table][dim]; the gradient needs it for grad_val alone */
+    const uint32_t* idx;            /* [n_entries]: an entry at or above n_table counts nothing, and its grad_val is zero */
+    const uint32_t* off;            /* [n_rows + 1]: CSR, numbers from 0 to n_entries that do not fall (on the GPU: not checked, but nothing
+                                       beyond n_entries is read); NULL: entry i is row i's */
+    const float* val;               /* [n_entries]; NULL: ones */
+    float scale;
+    const void* base;               /* [n_rows][dim], may be NULL */
+    void* out;                      /* [n_rows][dim], may be `base` itself when the strides are equal */
+    uint64_t table_stride, base_stride, out_stride;
+    /* the gradient */
+    const void* grad;               /* [n_rows][dim], of out */
+    void* grad_table;               /* [n_table][dim], may be NULL */
+    float* grad_val;                /* [n_entries], may be NULL */
+    uint64_t grad_stride, grad_table_stride;
+    uint32_t accumulate;            /* grad_table += instead of =; rows that no entry names are then not touched */
+} apoe_embed_args;
+
+/*
+ * out_i = base_i + scale sum_e val_e table[idx_e] over the entries of row i; grad_table[r] = scale sum_{e: idx_e = r} val_e grad[row of e],
+ * grad_val_e = scale <table[idx_e], grad[row of e]>. (The gradient of base is grad.) Entries are sorted by the row that they name, and
+ * each sum is in the entries' order, or parts of it: the same call gives the same bits. Workspace of the gradient: 32 bytes an entry, and 8 dim bytes for
+ * every 32 entries.
+ */
+int apoe_embed(apoe_ctx* ctx, const apoe_embed_args* args);
+int apoe_embed_grad(apoe_ctx* ctx, const apoe_embed_args* args);
+
+typedef struct {
+    uint32_t dtype;          /* of x, y and their gradients; vectors are float */
+    uint32_t rows, dim;      /* dim at most APOE_NORM_MAX_DIM; rows == 0 is fine */
+    const void* x;
+    const float *w, *b;      /* [dim]; NULL: ones, zeros */
+    float eps;
+    void* y;                 /* may be x itself when the strides are equal */
+    uint64_t x_stride, y_stride;
+    /* the gradient: what comes in (grad_skip, the gradient that x has by another way, may be NULL) and what goes out (each may be NULL) */
+    uint64_t grad_y_stride, grad_skip_stride, grad_x_stride;
+    const void *grad_y, *grad_skip;
+    void* grad_x;            /* may be grad_y or grad_skip itself when the strides are equal */
+    float *grad_w, *grad_b;
+} apoe_layer_norm_args;
+
+/*
+ * y = w (x - mean x) / sqrt(var x + eps) + b, row by row, with the variance of the row's values about their mean. The gradient is formed
+ * from x alone: nothing is kept from the forward call. grad_x = grad_skip + what comes through the norm.
+ */
+int apoe_layer_norm(apoe_ctx* ctx, const apoe_layer_norm_args* args);
+int apoe_layer_norm_grad(apoe_ctx* ctx, const apoe_layer_norm_args* args);
+
+#define APOE_ACT_NONE 0u
+#define APOE_ACT_RELU 1u
+#define APOE_ACT_GELU 2u /* z Phi(z), with the normal distribution's Phi itself */
+#define APOE_ACT_SILU 3u /* z / (1 + exp(-z)) */
+
+typedef struct {
+    uint32_t dtype;              /* of every matrix; the bias and its gradient are float */
+    uint32_t rows, cols_in, cols_out; /* columns at least 1 and at most APOE_LINEAR_MAX_SIDE, rows < 2^30; rows == 0 is fine */
+    uint32_t act;
+    const void *x, *w;           /* [rows][cols_in], [cols_out][cols_in] */
+    const float* bias;           /* [cols_out] or NULL */
+    const void* residual;        /* [rows][cols_out] or NULL */
+    void *y, *pre;               /* [rows][cols_out]; pre may be NULL: z as the gradient needs it */
+    uint64_t x_stride, w_stride, residual_stride, y_stride, pre_stride;
+    /* the gradient: from x, w, grad_y and (with an activation) pre; each output may be NULL */
+    const void* grad_y;
+    void *grad_x, *grad_w;       /* like x and w */
+    float* grad_bias;
+    uint64_t grad_y_stride, grad_x_stride, grad_w_stride;
+} apoe_linear_args;
+
+/*
+ * z = x w^T + bias, y = act(z) + residual; with gz = grad_y act'(pre): grad_x = gz w, grad_w = gz^T x, grad_bias = sum of gz's rows. (The
+ * gradient of residual is grad_y.) Sums are 32 bits and rounded once. float matrices are multiplied as three bfloat16 parts each, 24 bits, six
+ * products; a value that is infinite gives NaN there. gz is rounded to the matrices' type for the two products (with an activation; float: to 24 bits), not for
+ * grad_bias. Workspace: gz; partial sums of up to 128 MiB where rows and columns are too few to fill the GPU; float matrices
+ * (and such whose rows are not multiples of 16 bytes) in the form that the products take, 6 (2) bytes a value.
+ */
+int apoe_linear(apoe_ctx* ctx, const apoe_linear_args* args);
+int apoe_linear_grad(apoe_ctx* ctx, const apoe_linear_args* args);
+
+#define APOE_ADAMW_BLOCK 256u /* values of a parameter that share the scale of their 8-bit moments */
+
+typedef struct {
+    float* p;                    /* [n], any n */
+    void *m, *v;                 /* bits 32: float [n]; bits 8: int8_t [n] and uint8_t [n] */
+    float *m_scale, *v_scale;    /* bits 8: [(n + 255) / 256], the largest |m| and v of each block; bits 32: NULL */
+    void* copy;                  /* p once more, rounded to copy_dtype (APOE_F16, APOE_BF16), or NULL */
+    uint32_t copy_dtype;
+    uint64_t n;
+    double decay;
+} apoe_adamw_tensor;
+
+typedef struct {
+    const void* const* grads;    /* one for each parameter (NULL: it is left as it is), contiguous; the list itself is host memory */
+    const uint32_t* grad_dtypes; /* of each; host memory */
+    double lr, beta1, beta2, eps, grad_scale; /* gradients count times grad_scale */
+    uint32_t step;               /* 1, 2, ..: the number of this step */
+    const uint32_t* step_dev;    /* the same on the GPU, read there (NULL: `step`), for a captured step */
+    const float* lr_dev;         /* likewise */
+} apoe_adamw_step_args;
+
+/*
+ * AdamW over many parameters at once (the arrays that `tensors` points to stay the caller's and must outlive the handle; the list itself is
+ * copied). With g = grad_scale grad, t the step:
+ *   m = m + (1 - beta1) (g - m), v = v + (1 - beta2) (g g - v), p = p - lr (decay p + (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps)).
+ * bits 8: m = m_scale c |c| / 127^2 and v = v_scale c^4 / 255^4 for a code c, finer for small values; a new moment goes to one of the two codes beside it
+ * by chance, so that its mean is kept and small changes are not lost (a v above zero keeps a code above zero). The chances come from
+ * seed, step, parameter and place: the same call gives the same bits. p is stepped with the moments before they are rounded. A moment that is not finite
+ * makes its block's scale so.
+ */
+int apoe_adamw_create(apoe_ctx* ctx, uint32_t count, const apoe_adamw_tensor* tensors, uint32_t bits, uint32_t seed, apoe_adamw** out);
+void apoe_adamw_destroy(apoe_adamw* opt);
+int apoe_adamw_step(apoe_adamw* opt, const apoe_adamw_step_args* args);
+/* The values that 8-bit moments stand for: n of them from a block's beginning on. */
+int apoe_adamw_moments(apoe_ctx* ctx, uint64_t n, const int8_t* m, const float* m_scale, const uint8_t* v, const float* v_scale, float* m_out, float* v_out);
 
 #ifdef __cplusplus
 }
