@@ -11,6 +11,7 @@
 // code: both in 64 bits, at the same rate as 32 on this GPU's vector units.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "apoe_internal.h"
 
@@ -140,27 +141,45 @@ template <typename T> __device__ inline void store4(T* to, const T* x, uint64_t 
     }
 }
 
-// The largest of the wave's numbers, as the bits of floats that are not negative: a NaN is larger than all.
-__device__ inline float wave_largest(float v) {
-    uint32_t b = __float_as_uint(v) & 0x7fffffffu;
-#pragma unroll
-    for (int d = 32; d; d >>= 1) b = max(b, (uint32_t)__shfl_xor((int)b, d));
-    return __uint_as_float(b);
+// The largest of the wave's numbers by magnitude, the same for all lanes: as bits of floats without their signs, so that a NaN is larger than all. Rows of
+// sixteen lanes by moves between lanes, the four rows in scalar registers.
+__device__ inline float wave_largest(uint32_t b) {
+    const auto with = [&](auto control) { b = max(b, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b, decltype(control)::value, 0xf, 0xf, true)); };
+    with(std::integral_constant<int, 0xB1>{});  // lane xor 1
+    with(std::integral_constant<int, 0x4E>{});  // lane xor 2
+    with(std::integral_constant<int, 0x141>{}); // mirrored in eight
+    with(std::integral_constant<int, 0x140>{}); // mirrored in sixteen
+    const uint32_t r0 = __builtin_amdgcn_readlane((int)b, 0), r1 = __builtin_amdgcn_readlane((int)b, 16), r2 = __builtin_amdgcn_readlane((int)b, 32), r3 = __builtin_amdgcn_readlane((int)b, 48);
+    return __uint_as_float(max(max(r0, r1), max(r2, r3)));
 }
 
-// The code of x >= 0 in a block whose largest is `top`: x = top (code / STEPS)^POWER, up where `chance` is below the share of the way from the code
-// beneath to the one above. inv: STEPS^POWER / top. A largest that is not finite leaves zero: the block's values are its scale's.
+// most / top, off by a unit of the last place at most; zero where top is zero or not finite.
+__device__ inline double share_of(double most, float top) {
+    if (!(top > 0.f && top < INFINITY)) return 0.;
+    const double t = (double)top;
+    double r = __builtin_amdgcn_rcp(t);
+    r = __builtin_fma(__builtin_fma(-t, r, 1.), r, r);
+    r = __builtin_fma(__builtin_fma(-t, r, 1.), r, r);
+    return most * r;
+}
+
+// The code of x >= 0 in a block whose largest is top: x = top (code / STEPS)^POWER, up where `chance` is below the share of the way from the code
+// beneath to the one above; inv: STEPS^POWER / top. The root is only an estimate: where it takes the code next to the right one, x lies
+// so close to that code that the share (below zero, or above one) leads to it all the same. A top that is not finite gives zero: the
+// block's values are its scale's.
 template <int POWER, int STEPS> __device__ inline int code_of(double x, double inv, uint32_t chance) {
-    constexpr double MOST = POWER == 2 ? (double)STEPS * STEPS : (double)STEPS * STEPS * STEPS * STEPS;
-    const double w = fmin(x * inv, MOST);
-    const float root = POWER == 2 ? sqrtf((float)w) : sqrtf(sqrtf((float)w));
-    double k = (double)floorf(root);
-    auto raised = [](double c) { return POWER == 2 ? c * c : c * c * (c * c); };
-    if (raised(k) > w) k -= 1.;
-    if (raised(k + 1.) <= w) k += 1.;
-    const double low = raised(k), gap = raised(k + 1.) - low;
-    const double u = ((double)chance + 0.5) * 0x1p-32;
-    return min((int)k + (u * gap < w - low ? 1 : 0), STEPS);
+    const double w = x * inv;
+    const float r = __builtin_amdgcn_sqrtf((float)w), k = floorf(POWER == 2 ? r : __builtin_amdgcn_sqrtf(r)), square = k * k;
+    double above, gap; // what w is above its code, and the way to the next one: both from numbers that floats hold exactly
+    if constexpr (POWER == 2) {
+        above = w - (double)square;
+        gap = (double)__builtin_fmaf(2.f, k, 1.f);
+    } else {
+        above = __builtin_fma(-(double)square, (double)square, w);
+        gap = (double)__builtin_fmaf(2.f, k, 1.f) * (double)__builtin_fmaf(2.f, square + k, 1.f);
+    }
+    const double u = __builtin_fma((double)chance, 0x1p-32, 0x1p-33);
+    return min((int)k + (u * gap < above ? 1 : 0), STEPS);
 }
 
 template <int BITS> __global__ __launch_bounds__(256) void adamw_step(AdamArgs a) {
@@ -209,7 +228,7 @@ template <int BITS> __global__ __launch_bounds__(256) void adamw_step(AdamArgs a
             load4(cv, (const uint8_t*)t.v, at, whole, lane, left);
             const float sm = t.ms[block], sv = t.vs[block];
             double md[4], vd[4];
-            float mt = 0.f, vt = 0.f; // the largest, by magnitude; a value beyond the parameter's end is zero
+            uint32_t mb = 0, vb = 0; // the largest, by magnitude; a value beyond the parameter's end is zero
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const bool in = place(whole, lane, k) < left;
@@ -218,12 +237,11 @@ template <int BITS> __global__ __launch_bounds__(256) void adamw_step(AdamArgs a
                 vd[k] = in ? moved(value_of_v(sv, cv[k]), x * x, 1. - a.b2) : 0.;
                 m[k] = (float)md[k];
                 v[k] = (float)vd[k];
-                mt = __uint_as_float(max(__float_as_uint(mt), __float_as_uint(m[k]) & 0x7fffffffu));
-                vt = __uint_as_float(max(__float_as_uint(vt), __float_as_uint(v[k]) & 0x7fffffffu));
+                mb = max(mb, __float_as_uint(m[k]) & 0x7fffffffu);
+                vb = max(vb, __float_as_uint(v[k]) & 0x7fffffffu);
             }
-            mt = wave_largest(mt);
-            vt = wave_largest(vt);
-            const double im = mt > 0.f ? 127. * 127. / (double)mt : 0., iv = vt > 0.f ? 255. * 255. * 255. * 255. / (double)vt : 0.;
+            const float mt = wave_largest(mb), vt = wave_largest(vb);
+            const double im = share_of(127. * 127., mt), iv = share_of(255. * 255. * 255. * 255., vt);
             const uint32_t bk = mix(mix(key ^ (uint32_t)block) ^ (uint32_t)(block >> 32));
 #pragma unroll
             for (int k = 0; k < 4; k++) {

@@ -15,10 +15,13 @@
 
 namespace apoe {
 
-constexpr uint32_t EMBED_BLOCK = 32;     // entries that one group adds up
-constexpr uint32_t SORT_TILE = 4096;     // entries that a workgroup of the sort ranks at a time
+constexpr uint32_t EMBED_BLOCK = 32;     // entries that one group adds up, at most (and the lanes that hold their names)
+constexpr uint32_t SORT_TILE = 1024;     // entries that a workgroup of the sort ranks at a time
+constexpr uint32_t SORT_ONE = 4096;      // entries that one workgroup sorts by itself
 constexpr uint32_t SORT_TILES = 1024;    // workgroups of the sort, at most
 constexpr uint32_t NO_ROW = 0xffffffffu;
+
+using f32x4e = float __attribute__((ext_vector_type(4)));
 
 struct Entry { // sorted: the row of the table, the row of g, and the weight
     uint32_t key, row;
@@ -33,23 +36,23 @@ struct EmbedArgs {
     uint32_t* counts;  // [tiles][256]
     uint32_t tile_entries, tiles;
     float* part;       // [blocks][2][part_pitch]: what a block's first and last row have in it, where they go on in other blocks
-    uint32_t blocks, part_pitch;
+    uint32_t block, blocks, part_pitch; // block: entries of one
 };
 
-// WIDE: a workgroup of 1024 threads a row, whose groups take its entries in turn; otherwise a group a row.
-template <typename T, int V, int G, bool WIDE> __global__ __launch_bounds__(WIDE ? 1024 : (G > 256 ? G : 256)) void embed_rows(apoe_embed_args p) {
+// S groups share a row's entries, in turn, and are the workgroup's threads; with S = 1 a workgroup has as many rows as groups.
+template <typename T, int V, int G, int S> __global__ __launch_bounds__(S > 1 ? S * G : (G > 256 ? G : 256)) void embed_rows(apoe_embed_args p) {
     using R = RowOf<T, V, G>;
-    constexpr int THREADS = WIDE ? 1024 : (G > 256 ? G : 256), GROUPS = THREADS / G, S = WIDE ? GROUPS : 1, U = 4;
-    __shared__ float sums[WIDE ? GROUPS * G * ROW_E : 1];
+    constexpr int THREADS = S > 1 ? S * G : (G > 256 ? G : 256), GROUPS = S > 1 ? 1 : THREADS / G, U = 4;
+    __shared__ float sums[S > 1 ? S * G * ROW_E : 1];
     const int t = threadIdx.x % G, group = threadIdx.x / G;
-    for (uint64_t row = WIDE ? blockIdx.x : (uint64_t)blockIdx.x * GROUPS + group; row < p.n_rows; row += WIDE ? gridDim.x : (uint64_t)gridDim.x * GROUPS) {
+    for (uint64_t row = (uint64_t)blockIdx.x * GROUPS + (S > 1 ? 0 : group); row < p.n_rows; row += (uint64_t)gridDim.x * GROUPS) {
         uint32_t begin = (uint32_t)row, end = (uint32_t)row + 1;
         if (p.off) {
             end = min(p.off[row + 1], p.n_entries);
             begin = min(p.off[row], end);
         }
         float acc[ROW_E] = {};
-        for (uint64_t e = (uint64_t)begin + (WIDE ? group : 0); e < end; e += S * U) {
+        for (uint64_t e = (uint64_t)begin + (S > 1 ? group : 0); e < end; e += S * U) {
             typename R::tv raw[U][R::C];
             float w[U];
             uint32_t id[U];
@@ -77,7 +80,7 @@ template <typename T, int V, int G, bool WIDE> __global__ __launch_bounds__(WIDE
                 for (int k = 0; k < ROW_E; k++) acc[k] = __builtin_fmaf(w[u], x[k], acc[k]);
             }
         }
-        if constexpr (WIDE) {
+        if constexpr (S > 1) {
             __syncthreads();
 #pragma unroll
             for (int c = 0; c < R::C; c++)
@@ -87,7 +90,7 @@ template <typename T, int V, int G, bool WIDE> __global__ __launch_bounds__(WIDE
             for (uint32_t d = threadIdx.x; d < p.dim; d += THREADS) {
                 float s = sums[d];
 #pragma unroll
-                for (int g = 1; g < GROUPS; g++) s += sums[g * G * ROW_E + d];
+                for (int g = 1; g < S; g++) s += sums[g * G * ROW_E + d];
                 s *= p.scale;
                 if (p.base) s += (float)((const T*)p.base)[row * p.base_stride + d];
                 ((T*)p.out)[row * p.out_stride + d] = (T)s;
@@ -166,7 +169,49 @@ __global__ __launch_bounds__(256) void embed_count(EmbedArgs a, const uint2* fro
     a.counts[blockIdx.x * 256 + threadIdx.x] = n[threadIdx.x];
 }
 
-// Every entry goes behind those with a smaller digit, and behind the earlier ones with the same. TO: the last pass, which looks up rows and weights.
+// Ranks of a wave's items among those of the same digit before them, round by round; `seen` counts the wave's items of each digit.
+template <int ROUNDS> __device__ inline void rank_in_wave(const uint2* item, const bool* in, uint32_t* rank, volatile uint32_t* seen, uint32_t shift, uint32_t mask, int lane) {
+    for (int k = lane; k < 256; k += 64) seen[k] = 0;
+#pragma unroll
+    for (int r = 0; r < ROUNDS; r++) {
+        const uint32_t digit = (item[r].x >> shift) & mask;
+        uint64_t same = __ballot(in[r]);
+#pragma unroll
+        for (int b = 0; b < 8; b++) {
+            const uint64_t set = __ballot((digit >> b) & 1);
+            same &= (digit >> b) & 1 ? set : ~set;
+        }
+        const uint64_t below = same & ((1ull << lane) - 1);
+        rank[r] = in[r] ? seen[digit] + (uint32_t)__popcll(below) : 0;
+        if (in[r] && below == 0) seen[digit] = rank[r] + (uint32_t)__popcll(same); // one lane a digit; a wave's LDS accesses keep their order
+    }
+}
+
+// Sums of all smaller digits' counts, for 256 threads of a larger workgroup or all of them.
+__device__ inline void scan256(uint32_t* total, int tid) {
+    for (int d = 1; d < 256; d <<= 1) {
+        const uint32_t v = tid < 256 && tid >= d ? total[tid - d] : 0;
+        __syncthreads();
+        if (tid < 256) total[tid] += v;
+        __syncthreads();
+    }
+}
+
+__device__ inline Entry entry_of(const EmbedArgs& a, uint2 item) {
+    uint32_t row = item.y;
+    if (a.p.off) { // the last row that begins at or before the entry
+        uint32_t lo = 0, hi = a.p.n_rows;
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            if (a.p.off[mid] <= item.y) lo = mid;
+            else hi = mid;
+        }
+        row = a.p.n_rows && a.p.off[lo] <= item.y && item.y < a.p.off[lo + 1] ? lo : NO_ROW;
+    }
+    return Entry{item.x, row, a.p.val ? a.p.val[item.y] : 1.f, 0};
+}
+
+// Every entry goes behind those with a smaller digit, and behind the earlier ones with the same. LAST: the last pass, which looks up rows and weights.
 template <bool LAST> __global__ __launch_bounds__(256) void embed_place(EmbedArgs a, const uint2* from, uint2* to, uint32_t shift, uint32_t mask) {
     constexpr int WAVES = 4, ROUNDS = SORT_TILE / (64 * WAVES);
     __shared__ uint32_t next[256], total[256];
@@ -181,38 +226,20 @@ template <bool LAST> __global__ __launch_bounds__(256) void embed_place(EmbedArg
     }
     total[tid] = all;
     __syncthreads();
-    for (int d = 1; d < 256; d <<= 1) {
-        const uint32_t v = tid >= d ? total[tid - d] : 0;
-        __syncthreads();
-        total[tid] += v;
-        __syncthreads();
-    }
+    scan256(total, tid);
     next[tid] = total[tid] - all + before;
     const uint64_t begin = (uint64_t)blockIdx.x * a.tile_entries, end = min(begin + a.tile_entries, (uint64_t)a.p.n_entries);
     for (uint64_t tile = begin; tile < end; tile += SORT_TILE) {
-        volatile uint32_t* mine = seen[wave];
-        for (int k = lane; k < 256; k += 64) mine[k] = 0;
         uint2 item[ROUNDS];
         uint32_t rank[ROUNDS];
+        bool in[ROUNDS];
 #pragma unroll
         for (int r = 0; r < ROUNDS; r++) {
             const uint64_t e = tile + wave * (64 * ROUNDS) + r * 64 + lane;
-            item[r] = e < end ? pair_of(a, from, e) : uint2{0, 0};
+            in[r] = e < end;
+            item[r] = in[r] ? pair_of(a, from, e) : uint2{0, 0};
         }
-#pragma unroll
-        for (int r = 0; r < ROUNDS; r++) {
-            const bool in = tile + wave * (64 * ROUNDS) + r * 64 + lane < end;
-            const uint32_t digit = (item[r].x >> shift) & mask;
-            uint64_t same = __ballot(in);
-#pragma unroll
-            for (int b = 0; b < 8; b++) {
-                const uint64_t set = __ballot((digit >> b) & 1);
-                same &= (digit >> b) & 1 ? set : ~set;
-            }
-            const uint64_t below = same & ((1ull << lane) - 1);
-            rank[r] = in ? mine[digit] + (uint32_t)__popcll(below) : 0;
-            if (in && below == 0) mine[digit] = rank[r] + (uint32_t)__popcll(same); // one lane a digit; a wave's LDS accesses keep their order
-        }
+        rank_in_wave<ROUNDS>(item, in, rank, seen[wave], shift, mask, lane);
         __syncthreads();
         uint32_t at = next[tid];
         for (int w = 0; w < WAVES; w++) {
@@ -224,25 +251,60 @@ template <bool LAST> __global__ __launch_bounds__(256) void embed_place(EmbedArg
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < ROUNDS; r++) {
-            if (tile + wave * (64 * ROUNDS) + r * 64 + lane >= end) continue;
-            const uint32_t place = seen[wave][(item[r].x >> shift) & mask] + rank[r], e = item[r].y;
-            if constexpr (LAST) {
-                uint32_t row = e;
-                if (a.p.off) { // the last row that begins at or before the entry
-                    uint32_t lo = 0, hi = a.p.n_rows;
-                    while (hi - lo > 1) {
-                        const uint32_t mid = lo + (hi - lo) / 2;
-                        if (a.p.off[mid] <= e) lo = mid;
-                        else hi = mid;
-                    }
-                    row = a.p.n_rows && a.p.off[lo] <= e && e < a.p.off[lo + 1] ? lo : NO_ROW;
-                }
-                a.sorted[place] = Entry{item[r].x, row, a.p.val ? a.p.val[e] : 1.f, 0};
-            } else {
-                to[place] = item[r];
-            }
+            if (!in[r]) continue;
+            const uint32_t place = seen[wave][(item[r].x >> shift) & mask] + rank[r];
+            if constexpr (LAST) a.sorted[place] = entry_of(a, item[r]);
+            else to[place] = item[r];
         }
         __syncthreads(); // the next tile clears the counts
+    }
+}
+
+// Few entries: every pass in one workgroup's LDS.
+__global__ __launch_bounds__(1024) void embed_sort(EmbedArgs a, uint32_t passes, uint32_t width) {
+    constexpr int WAVES = 16, ROUNDS = SORT_ONE / (64 * WAVES);
+    __shared__ uint2 items[SORT_ONE];
+    __shared__ uint32_t total[256];
+    __shared__ uint32_t seen[WAVES][256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t n = a.p.n_entries, mask = (1u << width) - 1;
+    uint2 item[ROUNDS];
+    uint32_t rank[ROUNDS];
+    bool in[ROUNDS];
+    for (uint32_t pass = 0; pass < passes; pass++) {
+        const uint32_t shift = pass * width;
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++) {
+            const uint32_t e = wave * (64 * ROUNDS) + r * 64 + lane;
+            in[r] = e < n;
+            item[r] = in[r] ? (pass ? items[e] : pair_of(a, nullptr, e)) : uint2{0, 0};
+        }
+        rank_in_wave<ROUNDS>(item, in, rank, seen[wave], shift, mask, lane);
+        __syncthreads();
+        uint32_t all = 0;
+        if (tid < 256) {
+            for (int w = 0; w < WAVES; w++) all += seen[w][tid];
+            total[tid] = all;
+        }
+        __syncthreads();
+        scan256(total, tid);
+        if (tid < 256) {
+            uint32_t at = total[tid] - all;
+            for (int w = 0; w < WAVES; w++) {
+                const uint32_t k = seen[w][tid];
+                seen[w][tid] = at;
+                at += k;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++) {
+            if (!in[r]) continue;
+            const uint32_t place = seen[wave][(item[r].x >> shift) & mask] + rank[r];
+            if (pass + 1 == passes) a.sorted[place] = entry_of(a, item[r]);
+            else items[place] = item[r];
+        }
+        __syncthreads();
     }
 }
 
@@ -275,7 +337,7 @@ template <typename T, int V, int G> __device__ inline void put_table_row(const a
 // The first workgroups: a group a block of entries. The others: zeros for the rows that no entry names, 64 of the table a workgroup.
 template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 256) void embed_table(EmbedArgs a, uint32_t entry_groups) {
     using R = RowOf<T, V, G>;
-    constexpr int THREADS = G > 256 ? G : 256, GROUPS = THREADS / G, U = 4;
+    constexpr int THREADS = G > 256 ? G : 256, GROUPS = THREADS / G, U = sizeof(T) == 4 ? 2 : 4;
     const apoe_embed_args& p = a.p;
     const int t = threadIdx.x % G, group = threadIdx.x / G;
     if (blockIdx.x >= entry_groups) {
@@ -300,14 +362,18 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
     }
     const uint32_t block = blockIdx.x * GROUPS + group;
     if (block >= a.blocks) return;
-    const uint32_t begin = block * EMBED_BLOCK, end = min(begin + EMBED_BLOCK, p.n_entries);
-    uint32_t key = a.sorted[begin].key;
-    bool goes_on = begin > 0 && a.sorted[begin - 1].key == key; // the row began in an earlier block
+    const uint32_t begin = block * a.block, n = min(a.block, p.n_entries - begin);
+    constexpr int WIDTH = G < 64 ? G : 64; // every lane holds one entry of the block
+    const int l = threadIdx.x % WIDTH;
+    const Entry mine = a.sorted[begin + min((uint32_t)l, n - 1)];
+    const uint32_t in_front = begin ? a.sorted[begin - 1].key : NO_ROW, behind = begin + n < p.n_entries ? a.sorted[begin + n].key : NO_ROW;
+    const auto key_of = [&](uint32_t e) { return (uint32_t)__shfl((int)mine.key, (int)e, WIDTH); };
+    uint32_t key = key_of(0);
+    bool goes_on = in_front == key; // the row began in an earlier block
     float acc[ROW_E] = {};
     auto leave = [&](bool last) {
         if (key >= p.n_table) return;
-        const bool open = last && end < p.n_entries && a.sorted[end].key == key;
-        if (!goes_on && !open) {
+        if (!goes_on && !(last && behind == key)) {
             put_table_row<T, V, G>(p, key, t, acc);
             return;
         }
@@ -317,39 +383,54 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
 #pragma unroll
             for (int k = 0; k < V; k++) {
                 const uint32_t d = (c * G + t) * V + k;
-                if (d < p.dim) out[d] = acc[c * V + k];
+                if (d < a.part_pitch) out[d] = acc[c * V + k]; // zeros behind the row's end
             }
     };
-    for (uint32_t e = begin; e < end; e += U) {
-        Entry item[U];
-        typename R::tv raw[U][R::C];
-#pragma unroll
-        for (int u = 0; u < U; u++) item[u] = a.sorted[min(e + u, end - 1)];
+    typename R::tv raw[2][U][R::C]; // the next entries' rows are asked for before these are added up
+    float w[2][U];
+    auto ask = [&](uint32_t e, auto side) {
+        constexpr int Q = decltype(side)::value;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            if (item[u].row < p.n_rows && item[u].key < p.n_table) {
-                R::fetch(raw[u], p.grad, item[u].row, p.grad_stride, p.dim, t);
+            const int at = (int)min(e + u, n - 1);
+            const uint32_t row = (uint32_t)__shfl((int)mine.row, at, WIDTH), k = key_of(at);
+            w[Q][u] = __shfl(mine.val, at, WIDTH);
+            if (e + u < n && row < p.n_rows && k < p.n_table) {
+                R::fetch(raw[Q][u], p.grad, row, p.grad_stride, p.dim, t);
             } else {
-                item[u].val = 0.f;
+                w[Q][u] = 0.f;
 #pragma unroll
-                for (int c = 0; c < R::C; c++) raw[u][c] = typename R::tv{};
+                for (int c = 0; c < R::C; c++) raw[Q][u][c] = typename R::tv{};
             }
         }
+    };
+    auto add = [&](uint32_t e, auto side) {
+        constexpr int Q = decltype(side)::value;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            if (e + u >= end) break;
-            if (item[u].key != key) {
+            if (e + u >= n) break;
+            const uint32_t k0 = key_of(e + u);
+            if (k0 != key) {
                 leave(false);
-                key = item[u].key;
+                key = k0;
                 goes_on = false;
 #pragma unroll
                 for (int k = 0; k < ROW_E; k++) acc[k] = 0.f;
             }
             float x[ROW_E];
-            R::widen(x, raw[u]);
+            R::widen(x, raw[Q][u]);
 #pragma unroll
-            for (int k = 0; k < ROW_E; k++) acc[k] = __builtin_fmaf(item[u].val, x[k], acc[k]);
+            for (int k = 0; k < ROW_E; k++) acc[k] = __builtin_fmaf(w[Q][u], x[k], acc[k]);
         }
+    };
+    const std::integral_constant<int, 0> even;
+    const std::integral_constant<int, 1> odd;
+    ask(0, even);
+    for (uint32_t e = 0; e < n; e += 2 * U) {
+        if (e + U < n) ask(e + U, odd);
+        add(e, even);
+        if (e + 2 * U < n) ask(e + 2 * U, even);
+        if (e + U < n) add(e + U, odd);
     }
     leave(true);
 }
@@ -358,32 +439,53 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
 // everywhere) are added up by the workgroup's waves together.
 template <typename T> __global__ __launch_bounds__(1024) void embed_join(EmbedArgs a) {
     constexpr uint32_t WAVES = 16, LONG = 16;
-    __shared__ uint32_t later[WAVES];
-    __shared__ float sums[WAVES][257];
+    __shared__ uint32_t later[WAVES], later_key[WAVES];
+    __shared__ __align__(16) float sums[WAVES][256];
     const apoe_embed_args& p = a.p;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t block = blockIdx.x * WAVES + wave, d0 = blockIdx.y * 256;
     uint32_t parts = 0, key = 0; // blocks after this one that have a part of the row
     auto look = [&](uint32_t b) {
         parts = 0;
-        const uint64_t end = (uint64_t)(b + 1) * EMBED_BLOCK;
+        const uint64_t end = (uint64_t)(b + 1) * a.block;
         if (b >= a.blocks || end >= p.n_entries) return;
+        const uint32_t begin = b * a.block;
         key = a.sorted[end - 1].key;
-        const uint32_t begin = b * EMBED_BLOCK;
-        if (key >= p.n_table || a.sorted[end].key != key) return;
-        if (a.sorted[begin].key == key && begin > 0 && a.sorted[begin - 1].key == key) return; // it began earlier
-        parts = (first_at_least(a.sorted, (uint32_t)end, p.n_entries, key + 1) - 1) / EMBED_BLOCK - b;
-    };
-    auto add = [&](uint32_t b, uint32_t first, uint32_t step, float* s) { // parts `first`, `first` + step, .. of the row that begins in block b
-#pragma unroll 4
-        for (uint32_t k = first; k <= parts; k += step) {
-            const float* from = a.part + ((size_t)(b + k) * 2 + (k ? 0 : 1)) * a.part_pitch + d0;
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const uint32_t d = c * 64 + lane;
-                if (d0 + d < p.dim) s[c] += from[d];
-            }
+        const uint32_t next = a.sorted[end].key, first = a.sorted[begin].key, in_front = begin ? a.sorted[begin - 1].key : NO_ROW;
+        if (key >= p.n_table || next != key) return;
+        if (first == key && in_front == key) return; // it began earlier
+        // the last block that has a part: the wave's lanes look at 64 places at once, in strides that grow until one is beyond, then shrink
+        uint64_t has = b + 1, stride = 1;
+        const auto reach = [&]() {
+            const uint64_t c = has + stride * (lane + 1); // block c has a part where the row's name is its first one
+            const uint64_t yes = __ballot(c < a.blocks && a.sorted[c * a.block].key == key);
+            has += stride * __popcll(yes);
+            return yes == ~0ull;
+        };
+        while (reach()) stride *= 64;
+        while (stride > 1) {
+            stride /= 64;
+            reach();
         }
+        parts = (uint32_t)(has - b);
+    };
+    // Parts `first`, `first` + step, .. of the row that begins in block b, four columns a lane: eight rows are asked for at once, beyond the last one
+    // that one again, which is not counted (a load under a condition would be waited for before the next is sent).
+    auto add = [&](uint32_t b, uint32_t first, uint32_t step) {
+        const uint32_t last = __builtin_amdgcn_readfirstlane(parts);
+        const float* column = a.part + min(d0 + lane * 4, a.part_pitch - 4);
+        f32x4e s = {};
+        for (uint32_t k = first; k <= last; k += 8 * step) {
+            f32x4e x[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const uint32_t q = min(k + u * step, last);
+                x[u] = *reinterpret_cast<const f32x4e*>(column + ((size_t)(b + q) * 2 + (q ? 0 : 1)) * a.part_pitch);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) s += k + u * step <= last ? x[u] : f32x4e{};
+        }
+        return s;
     };
     auto put = [&](uint32_t d, float s) {
         if (d >= p.dim) return;
@@ -392,22 +494,23 @@ template <typename T> __global__ __launch_bounds__(1024) void embed_join(EmbedAr
         *at = (T)(p.accumulate ? s + (float)*at : s);
     };
     look(block);
-    if (lane == 0) later[wave] = parts > LONG;
+    if (lane == 0) {
+        later[wave] = parts > LONG ? parts : 0;
+        later_key[wave] = key;
+    }
     if (parts && parts <= LONG) {
-        float s[4] = {};
-        add(block, 0, 1, s);
+        const f32x4e s = add(block, 0, 1);
 #pragma unroll
-        for (int c = 0; c < 4; c++) put(d0 + c * 64 + lane, s[c]);
+        for (int c = 0; c < 4; c++) put(d0 + lane * 4 + c, s[c]);
     }
     __syncthreads();
     for (uint32_t w = 0; w < WAVES; w++) {
-        if (!later[w]) continue;
-        look(blockIdx.x * WAVES + w);
-        float s[4] = {};
-        add(blockIdx.x * WAVES + w, wave, WAVES, s);
+        parts = later[w];
+        if (!parts) continue;
+        key = later_key[w];
+        const f32x4e s = add(blockIdx.x * WAVES + w, wave, WAVES);
         __syncthreads();
-#pragma unroll
-        for (int c = 0; c < 4; c++) sums[wave][c * 64 + lane] = s[c];
+        *reinterpret_cast<f32x4e*>(&sums[wave][lane * 4]) = s;
         __syncthreads();
         if (threadIdx.x < 256) {
             float v = 0.f;
@@ -419,17 +522,23 @@ template <typename T> __global__ __launch_bounds__(1024) void embed_join(EmbedAr
 
 template <typename T, int V> static int run_embed(apoe_ctx* ctx, const apoe_embed_args* p) {
     hipStream_t s = ctx->stream;
-    const uint32_t cus = (uint32_t)ctx->num_cus;
-    // a workgroup a row where groups of a row each would leave most of the GPU idle and there are entries to share
-    const bool wide = p->n_rows <= cus * 4 && (uint64_t)p->n_entries >= (uint64_t)p->n_rows * 8;
+    // Few rows with many entries each: groups share a row, so that the GPU has some 16 waves a CU to wait for memory with, and each at least two entries.
     return with_group(p->dim, [&](auto size) -> int {
-        constexpr int G = decltype(size)::value, THREADS = G > 256 ? G : 256;
-        if (wide) {
-            embed_rows<T, V, G, true><<<p->n_rows, 1024, 0, s>>>(*p);
-        } else {
-            const uint64_t need = ((uint64_t)p->n_rows + THREADS / G - 1) / (THREADS / G);
-            embed_rows<T, V, G, false><<<(uint32_t)std::min<uint64_t>(need, 1u << 20), THREADS, 0, s>>>(*p);
+        constexpr int G = decltype(size)::value, THREADS = G > 256 ? G : 256, MOST = 1024 / G < 16 ? 1024 / G : 16;
+        const uint64_t waves = (uint64_t)p->n_rows * (G > 64 ? G / 64 : 1), room = (uint64_t)ctx->num_cus * 16;
+        const auto shared_by = [&](uint64_t groups) { return p->n_entries >= (uint64_t)p->n_rows * groups * 2 && waves * groups <= room * 4; };
+        if (shared_by(MOST)) {
+            embed_rows<T, V, G, MOST><<<p->n_rows, MOST * G, 0, s>>>(*p);
+            return APOE_OK;
         }
+        if constexpr (MOST > 4) {
+            if (shared_by(4)) {
+                embed_rows<T, V, G, 4><<<p->n_rows, 4 * G, 0, s>>>(*p);
+                return APOE_OK;
+            }
+        }
+        const uint64_t need = ((uint64_t)p->n_rows + THREADS / G - 1) / (THREADS / G);
+        embed_rows<T, V, G, 1><<<(uint32_t)std::min<uint64_t>(need, 1u << 20), THREADS, 0, s>>>(*p);
         return APOE_OK;
     });
 }
@@ -453,7 +562,11 @@ template <typename T, int V> static int run_embed_grad(apoe_ctx* ctx, const apoe
     const uint64_t n = p->n_entries;
     a.tile_entries = (uint32_t)(((n + SORT_TILES - 1) / SORT_TILES + SORT_TILE - 1) / SORT_TILE * SORT_TILE);
     a.tiles = n ? (uint32_t)((n + a.tile_entries - 1) / a.tile_entries) : 0;
-    a.blocks = (uint32_t)((n + EMBED_BLOCK - 1) / EMBED_BLOCK);
+    // Some 8 waves a CU, of 8 to 32 entries each (16: groups of 16 lanes): smaller blocks fill the GPU, larger ones cut fewer rows (launch that walks and
+    // launch that joins, us: 31 080 float entries of 1024 columns, blocks of 8 30 + 37, 16 31 + 24, 32 45 + 23; 65 536 bf16 ones, 16 62 + 39, 32 57 + 25).
+    const uint32_t most = p->dim <= 16 * ROW_E ? 16 : EMBED_BLOCK;
+    a.block = (uint32_t)std::min<uint64_t>(most, std::max<uint64_t>(8, (n / ((uint64_t)ctx->num_cus * 8) + 2) / 4 * 4));
+    a.blocks = (uint32_t)((n + a.block - 1) / a.block);
     a.part_pitch = (p->dim + 3) / 4 * 4;
     const size_t records = n * sizeof(Entry), pairs = n * sizeof(uint2), counts = (size_t)a.tiles * 256 * 4;
     char* ws = nullptr;
@@ -466,7 +579,9 @@ template <typename T, int V> static int run_embed_grad(apoe_ctx* ctx, const apoe
     uint32_t bits = 1;
     while (bits < 32 && (p->n_table >> bits)) bits++; // keys go to n_table
     const uint32_t passes = (bits + 7) / 8, width = (bits + passes - 1) / passes;
-    if (n) {
+    if (n && n <= SORT_ONE) {
+        embed_sort<<<1, 1024, 0, s>>>(a, passes, width);
+    } else if (n) {
         const uint2* from = nullptr;
         for (uint32_t pass = 0; pass < passes; pass++) {
             const uint32_t shift = pass * width, mask = (1u << width) - 1;

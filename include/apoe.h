@@ -429,7 +429,7 @@ typedef struct {
  * out_i = base_i + scale sum_e val_e table[idx_e] over the entries of row i; grad_table[r] = scale sum_{e: idx_e = r} val_e grad[row of e],
  * grad_val_e = scale <table[idx_e], grad[row of e]>. (The gradient of base is grad.) Entries are sorted by the row that they name, and
  * each sum is in the entries' order, or parts of it: the same call gives the same bits. Workspace of the gradient: 32 bytes an entry, and 8 dim bytes for
- * every 32 entries.
+ * every 8 to 32 entries (32 from 65 000 on; 16 up to 256 columns).
  */
 int apoe_embed(apoe_ctx* ctx, const apoe_embed_args* args);
 int apoe_embed_grad(apoe_ctx* ctx, const apoe_embed_args* args);
