@@ -558,8 +558,10 @@ def _matrix(ctx, t, name, shape=None, dtype=None):
 
 
 def _vector(ctx, t, name, n, dtypes):
-    _on_gpu(ctx, t, name)
-    if t.dtype not in dtypes or t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
+    shape = t.shape
+    if t.get_device() != ctx.device:
+        raise ApoeError(f"{name} must be on GPU {ctx.device}, the context's")
+    if t.dtype not in dtypes or len(shape) != 1 or (n is not None and shape[0] != n) or not t.is_contiguous():
         raise ApoeError(f"{name} must be a contiguous vector of {' or '.join(str(d) for d in dtypes)}{'' if n is None else f' of length {n}'}")
     return t.data_ptr()
 
@@ -755,15 +757,15 @@ def _embed_args(ctx, table, idx, off, val, scale):
     a.table_stride = _matrix(ctx, table, "table")
     (a.n_table, a.dim), a.table = table.shape, table.data_ptr()
     a.idx = _vector(ctx, idx, "idx", None, _INTS)
-    a.n_entries = a.n_rows = idx.shape[0]
+    entries = idx.shape[0]
+    a.n_entries, a.n_rows, a.scale = entries, entries, scale
     if off is not None:
         a.off = _vector(ctx, off, "off", None, _INTS)
         a.n_rows = off.shape[0] - 1
         if off.shape[0] == 0:
             raise ApoeError("off must have one number more than there are rows")
     if val is not None:
-        a.val = _vector(ctx, val, "val", idx.shape[0], _FLOATS)
-    a.scale = scale
+        a.val = _vector(ctx, val, "val", entries, _FLOATS)
     return a
 
 
@@ -772,13 +774,15 @@ def embed(ctx, table, idx, off=None, val=None, scale=1.0, base=None, out=None):
     rows' terms and weights (ones without val); without off entry i is row i's. Entries at or above the table's length count nothing. table, base and
     out have one type; out may be base itself."""
     a = _embed_args(ctx, table, idx, off, val, scale)
-    shape = _torch.Size((a.n_rows, a.dim))
+    shape = (a.n_rows, a.dim)
     if base is not None:
         a.base_stride, a.base = _matrix(ctx, base, "base", shape, table.dtype), base.data_ptr()
     if out is None:
-        out = _torch.empty(shape, dtype=table.dtype, device=table.device)
-    a.out_stride, a.out = _matrix(ctx, out, "out", shape, table.dtype), out.data_ptr()
-    if out.numel() == 0:
+        out = table.new_empty(shape)
+    else:
+        a.out_stride = _matrix(ctx, out, "out", shape, table.dtype)
+    a.out = out.data_ptr()
+    if a.n_rows == 0 or a.dim == 0:
         return out
     _call(ctx, lib().apoe_embed, a)
     return out
@@ -816,10 +820,12 @@ def _norm_args(ctx, x, w, b, eps):
     a = LayerNormArgs()
     a.dtype = _dtype(x, "x")
     a.x_stride = _matrix(ctx, x, "x")
-    (a.rows, a.dim), a.eps, a.x = x.shape, eps, x.data_ptr()
-    for t, name in ((w, "w"), (b, "b")):
-        if t is not None:
-            setattr(a, name, _vector(ctx, t, name, a.dim, _FLOATS))
+    (a.rows, d), a.eps, a.x = x.shape, eps, x.data_ptr()
+    a.dim = d
+    if w is not None:
+        a.w = _vector(ctx, w, "w", d, _FLOATS)
+    if b is not None:
+        a.b = _vector(ctx, b, "b", d, _FLOATS)
     return a
 
 
@@ -827,9 +833,11 @@ def layer_norm(ctx, x, w=None, b=None, eps=1e-5, out=None):
     """w * (x - mean(x)) / sqrt(var(x) + eps) + b for every row of x [m, d]; w and b are float32. out may be x itself."""
     a = _norm_args(ctx, x, w, b, eps)
     if out is None:
-        out = _torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a.y_stride, a.y = _matrix(ctx, out, "out", x.shape, x.dtype), out.data_ptr()
-    if x.numel() == 0:
+        out = x.new_empty(x.shape)
+    else:
+        a.y_stride = _matrix(ctx, out, "out", x.shape, x.dtype)
+    a.y = out.data_ptr()
+    if a.rows == 0 or a.dim == 0:
         return out
     _call(ctx, lib().apoe_layer_norm, a)
     return out
@@ -867,15 +875,15 @@ def _linear_args(ctx, x, w, act):
     a.dtype = _dtype(x, "x")
     a.x_stride = _matrix(ctx, x, "x")
     a.w_stride = _matrix(ctx, w, "w", dtype=x.dtype)
-    if w.shape[1] != x.shape[1]:
-        raise ApoeError(f"w must have x's {x.shape[1]} columns, not {w.shape[1]}")
-    a.rows, a.cols_in = x.shape
-    a.cols_out, a.x, a.w = w.shape[0], x.data_ptr(), w.data_ptr()
-    if act not in ACTIVATIONS:
-        raise ApoeError(f"act must be one of {', '.join(ACTIVATIONS)}, not {act!r}")
-    if 0 in w.shape:
+    (m, k), (n, same) = x.shape, w.shape
+    if same != k:
+        raise ApoeError(f"w must have x's {k} columns, not {same}")
+    if n == 0 or k == 0:
         raise ApoeError("w is empty")
-    a.act = ACTIVATIONS[act]
+    a.act = ACTIVATIONS.get(act, -1)
+    if a.act > 3:
+        raise ApoeError(f"act must be one of {', '.join(ACTIVATIONS)}, not {act!r}")
+    a.rows, a.cols_in, a.cols_out, a.x, a.w = m, k, n, x.data_ptr(), w.data_ptr()
     return a
 
 
@@ -883,18 +891,22 @@ def linear(ctx, x, w, bias=None, act="none", residual=None, want_pre=False, out=
     """(y, pre): y = act(pre) + residual with pre = x w^T + bias, for x [m, k], w [n, k], bias [n] float32, residual [m, n]; act: "none", "relu",
     "gelu" or "silu". pre, which linear_grad needs where there is an activation, is None unless it is wanted."""
     a = _linear_args(ctx, x, w, act)
-    shape = _torch.Size((a.rows, a.cols_out))
+    n = a.cols_out
+    shape = (a.rows, n)
     if bias is not None:
-        a.bias = _vector(ctx, bias, "bias", a.cols_out, _FLOATS)
+        a.bias = _vector(ctx, bias, "bias", n, _FLOATS)
     if residual is not None:
         a.residual_stride, a.residual = _matrix(ctx, residual, "residual", shape, x.dtype), residual.data_ptr()
     if out is None:
-        out = _torch.empty(shape, dtype=x.dtype, device=x.device)
-    a.y_stride, a.y = _matrix(ctx, out, "out", shape, x.dtype), out.data_ptr()
-    pre = _torch.empty(shape, dtype=x.dtype, device=x.device) if want_pre else None
-    if pre is not None:
+        out = x.new_empty(shape)
+    else:
+        a.y_stride = _matrix(ctx, out, "out", shape, x.dtype)
+    a.y = out.data_ptr()
+    pre = None
+    if want_pre:
+        pre = x.new_empty(shape)
         a.pre = pre.data_ptr()
-    if x.shape[0] == 0:
+    if shape[0] == 0:
         return out, pre
     _call(ctx, lib().apoe_linear, a)
     return out, pre

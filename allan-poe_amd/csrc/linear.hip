@@ -8,6 +8,7 @@
 // through LDS, 16 bytes a thread. Where tiles are too few for the GPU the inner dimension is cut and a second launch adds the cuts up, in order.
 // Up to 64 rows a kernel of its own streams w once (the serving form).
 #include <algorithm>
+#include <cmath>
 
 #include "apoe_internal.h"
 #include "apoe_tile.h"
@@ -52,29 +53,49 @@ __device__ inline float normal_tail(float u, float& density) {
     return s * t * e;
 }
 
-__device__ inline float activate(float z, uint32_t act) {
-    if (act == APOE_ACT_RELU) return z < 0.f ? 0.f : z;
-    if (act == APOE_ACT_GELU) {
-        float d;
-        const float q = normal_tail(fabsf(z), d);
-        return z * (z > 0.f ? 1.f - q : q);
+__device__ inline float relu(float z) { return z < 0.f ? 0.f : z; }
+__device__ inline float gelu(float z) {
+    float d;
+    const float q = normal_tail(fabsf(z), d);
+    return z * (z > 0.f ? 1.f - q : q);
+}
+__device__ inline float silu(float z) { return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * z)); }
+
+__device__ inline float activate1(float z, uint32_t act) { return act == APOE_ACT_RELU ? relu(z) : act == APOE_ACT_GELU ? gelu(z) : act == APOE_ACT_SILU ? silu(z) : z; }
+
+// Eight values under one decision, so that the roots of one do not wait for another's.
+__device__ inline void activate8(float* z, uint32_t act) {
+    if (act == APOE_ACT_RELU) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) z[k] = relu(z[k]);
+    } else if (act == APOE_ACT_GELU) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) z[k] = gelu(z[k]);
+    } else if (act == APOE_ACT_SILU) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) z[k] = silu(z[k]);
     }
-    if (act == APOE_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * z));
-    return z;
 }
 
-__device__ inline float slope(float z, uint32_t act) {
-    if (act == APOE_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-    if (act == APOE_ACT_GELU) {
-        float d;
-        const float q = normal_tail(fabsf(z), d);
-        return __builtin_fmaf(z, d, z > 0.f ? 1.f - q : q);
+// v times the activation's slope at z.
+__device__ inline void slope8(float* v, const float* z, uint32_t act) {
+    if (act == APOE_ACT_RELU) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] *= z[k] > 0.f ? 1.f : 0.f;
+    } else if (act == APOE_ACT_GELU) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            float d;
+            const float q = normal_tail(fabsf(z[k]), d);
+            v[k] *= __builtin_fmaf(z[k], d, z[k] > 0.f ? 1.f - q : q);
+        }
+    } else if (act == APOE_ACT_SILU) { // o (1 + z (1 - o))
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float e = __builtin_amdgcn_exp2f(-1.44269504f * z[k]), o = __builtin_amdgcn_rcpf(1.f + e), rest = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(1.44269504f * z[k]));
+            v[k] *= o * __builtin_fmaf(z[k], rest, 1.f);
+        }
     }
-    if (act == APOE_ACT_SILU) { // o (1 + z (1 - o))
-        const float o = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504f * z)), rest = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(1.44269504f * z));
-        return o * __builtin_fmaf(z, rest, 1.f);
-    }
-    return 1.f;
 }
 
 // Eight values of a row as numbers, `left` of them there (whole: eight, from a multiple of 16 bytes).
@@ -127,10 +148,7 @@ template <typename T> __device__ inline void finish8(const LinOut& o, uint32_t i
         for (int k = 0; k < 8; k++) v[k] += b[k];
     }
     if (o.pre) give8<T>(o.pre, i * o.pre_stride + j, v, whole, left);
-    if (o.act != APOE_ACT_NONE) {
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = activate(v[k], o.act);
-    }
+    activate8(v, o.act);
     if (o.residual) {
         float r[8];
         take8<T>(r, o.residual, i * o.residual_stride + j, whole, left);
@@ -140,9 +158,55 @@ template <typename T> __device__ inline void finish8(const LinOut& o, uint32_t i
     give8<T>(o.out, i * o.out_stride + j, v, whole, left);
 }
 
+// One.
+template <typename T> __device__ inline void finish1(const LinOut& o, uint32_t i, uint32_t j, float z) {
+    if (o.bias) z += o.bias[j];
+    if (o.pre) ((T*)o.pre)[i * o.pre_stride + j] = (T)z;
+    z = activate1(z, o.act);
+    if (o.residual) z += (float)((const T*)o.residual)[i * o.residual_stride + j];
+    ((T*)o.out)[i * o.out_stride + j] = (T)z;
+}
+
+// What the waves hold goes out: one block of 32 rows a wave at a time through LDS, then a thread has eight values of a row. Waits between are for LDS alone: the
+// stores of the block before are on their way meanwhile.
+template <typename T, int MT, int NT, int WM, int WN, int KG, int BYTES>
+__device__ inline void tile_out(const LinTile& a, f32x16 (&acc)[MT][NT], char* lds, uint32_t row, uint32_t col, uint32_t cut, int kg, int wm, int wn, int lane) {
+    constexpr int NW = WM * WN * KG, BN = WN * NT * 32, PITCH = BN + 4, ROWS = WM * 32, ITEMS = ROWS * BN / 8 / (64 * NW);
+    static_assert(ROWS * PITCH * 4 <= BYTES && ROWS * BN % (512 * NW) == 0, "the sums fit the stages");
+    const uint32_t m = a.o.m, n = a.o.n;
+    float* sum = reinterpret_cast<float*>(lds);
+    const int half = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        if (KG == 1 || i / (MT / KG) == kg) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int k = 0; k < 16; k++) sum[(wm * 32 + result_row(k, half)) * PITCH + (wn * NT + t) * 32 + (lane & 31)] = acc[i][t][k];
+        }
+        tile_wait<63>();
+#pragma unroll 1
+        for (int item = 0; item < ITEMS; item++) {
+            const uint32_t at = item * 64 * NW + threadIdx.x, r = at / (BN / 8), c = at % (BN / 8) * 8;
+            const uint32_t gi = row + (r / 32 * MT + i) * 32 + r % 32, gj = col + c;
+            if (gi >= m || gj >= n) continue;
+            const f32x4 v0 = *reinterpret_cast<const f32x4*>(sum + r * PITCH + c), v1 = *reinterpret_cast<const f32x4*>(sum + r * PITCH + c + 4);
+            if (a.cuts > 1) {
+                float* to = a.part + ((uint64_t)cut * m + gi) * a.np + gj;
+                *reinterpret_cast<f32x4*>(to) = v0;
+                *reinterpret_cast<f32x4*>(to + 4) = v1;
+            } else {
+                float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                finish8<T>(a.o, gi, gj, v);
+            }
+        }
+        if (i + 1 < MT) tile_wait<63>();
+    }
+}
+
 // S: the operands' type, P planes of it; T: the results'. ACOL, BCOL: the inner dimension goes down the rows.
 template <typename S, typename T, int P, bool ACOL, bool BCOL, int MT, int NT, int WM, int WN, int KG, int SF, int ST>
-__global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_tile(LinTile a) {
+__global__ __launch_bounds__(64 * WM * WN * KG, WM * WN * KG == 4 && P == 3 ? 1 : 2) void linear_tile(LinTile a) {
     constexpr int NW = WM * WN * KG, FS = SF / KG, BM = WM * MT * 32, BN = WN * NT * 32;
     using ATile = std::conditional_t<ACOL, ColTile<S, BM, SF, NW, ORDER_ROWS>, RowTile<S, BM, SF, NW>>;
     using BTile = std::conditional_t<BCOL, ColTile<S, BN, SF, NW, ORDER_ROWS>, RowTile<S, BN, SF, NW>>;
@@ -227,37 +291,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_tile(LinTile a) {
         exchange_halves<MT, NT, WM * WN>(acc, lds, kg, wave % (WM * WN), lane);
         __syncthreads();
     }
-    // one block of 32 rows a wave at a time through LDS: then a thread has eight values of a row
-    constexpr int PITCH = BN + 4, ROWS = WM * 32, ITEMS = ROWS * BN / 8 / (64 * NW);
-    static_assert(ROWS * PITCH * 4 <= ST * STAGE && ROWS * BN % (512 * NW) == 0, "the sums fit the stages");
-    float* sum = reinterpret_cast<float*>(lds);
-    const int half = lane >> 5;
-#pragma unroll
-    for (int i = 0; i < MT; i++) {
-        if (KG == 1 || i / (MT / KG) == kg) {
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int k = 0; k < 16; k++) sum[(wm * 32 + result_row(k, half)) * PITCH + (wn * NT + t) * 32 + (lane & 31)] = acc[i][t][k];
-        }
-        __syncthreads();
-#pragma unroll 1
-        for (int item = 0; item < ITEMS; item++) {
-            const uint32_t at = item * 64 * NW + threadIdx.x, r = at / (BN / 8), c = at % (BN / 8) * 8;
-            const uint32_t gi = row + (r / 32 * MT + i) * 32 + r % 32, gj = col + c;
-            if (gi >= m || gj >= n) continue;
-            const f32x4 v0 = *reinterpret_cast<const f32x4*>(sum + r * PITCH + c), v1 = *reinterpret_cast<const f32x4*>(sum + r * PITCH + c + 4);
-            if (a.cuts > 1) {
-                float* to = a.part + ((uint64_t)cut * m + gi) * a.np + gj;
-                *reinterpret_cast<f32x4*>(to) = v0;
-                *reinterpret_cast<f32x4*>(to + 4) = v1;
-            } else {
-                float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-                finish8<T>(a.o, gi, gj, v);
-            }
-        }
-        __syncthreads();
-    }
+    tile_out<T, MT, NT, WM, WN, KG, ST * STAGE>(a, acc, lds, row, col, cut, kg, wm, wn, lane);
 }
 
 // The cuts' sums, eight columns a thread.
@@ -278,6 +312,67 @@ template <typename T> __global__ __launch_bounds__(256) void linear_join(LinTile
     }
 }
 
+// ---- up to 64 rows ----
+
+struct LinFew {
+    const void *x, *w;
+    uint64_t x_stride, w_stride;
+    uint32_t k;
+    LinOut o;
+};
+
+// Bound by the one reading of w (and for small layers by its latency): a workgroup has 16 of w's rows, its NW waves share the inner side, 128 indices at a time, all of
+// whose loads are on their way at once; x comes from the L2. MB blocks of 16 rows of x; 16 x 16 matrix instructions, float matrices on the float ones.
+// The waves' sums meet in LDS, one result a thread. 16 x 1024 -> 4096 fp16: 5 us (64 x 64 tiles in two cuts and their sum 9).
+template <typename T, int MB, int NW> __global__ __launch_bounds__(64 * NW) void linear_few(LinFew a) {
+    constexpr int E = 16 / sizeof(T), STEP = 4 * E, U = 128 / STEP; // values a lane loads; inner indices of a load; loads of a turn
+    typedef T tv __attribute__((ext_vector_type(E)));
+    __shared__ float sums[NW][MB * 256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, r = lane & 15;
+    const uint32_t m = a.o.m, n = a.o.n, col = blockIdx.x * 16;
+    const T* wr = (const T*)a.w + (uint64_t)min(col + r, n - 1) * a.w_stride; // rows beyond the end: the last one again, whose results go nowhere
+    const T* xr[MB];
+#pragma unroll
+    for (int b = 0; b < MB; b++) xr[b] = (const T*)a.x + (uint64_t)min((uint32_t)(b * 16 + r), m - 1) * a.x_stride;
+    f32x4 acc[MB] = {};
+    for (uint32_t k0 = wave * 128; k0 < a.k; k0 += NW * 128) {
+        tv wv[U], xv[MB][U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t k = k0 + u * STEP + q * E;
+            wv[u] = k < a.k ? *reinterpret_cast<const tv*>(wr + k) : tv{};
+#pragma unroll
+            for (int b = 0; b < MB; b++) xv[b][u] = k < a.k ? *reinterpret_cast<const tv*>(xr[b] + k) : tv{};
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int b = 0; b < MB; b++) {
+                if constexpr (std::is_same_v<T, float>) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) acc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[b][u][j], wv[u][j], acc[b], 0, 0, 0);
+                } else if constexpr (std::is_same_v<T, _Float16>) {
+                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xv[b][u], wv[u], acc[b], 0, 0, 0);
+                } else {
+                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv[b][u], wv[u], acc[b], 0, 0, 0);
+                }
+            }
+    }
+#pragma unroll
+    for (int b = 0; b < MB; b++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) sums[wave][b * 256 + (4 * q + i) * 16 + r] = acc[b][i];
+    __syncthreads();
+    for (uint32_t v = threadIdx.x; v < MB * 256; v += 64 * NW) {
+        const uint32_t i = v / 16, j = col + v % 16;
+        if (i >= m || j >= n) continue;
+        float z[8] = {};
+#pragma unroll
+        for (int w = 0; w < NW; w++) z[0] += sums[w][v];
+        finish1<T>(a.o, i, j, z[0]);
+    }
+}
+
 // ---- operands in the products' form, gz, and the columns' sums ----
 
 struct LinPack {
@@ -288,26 +383,33 @@ struct LinPack {
     uint32_t rows, cols, pitch, act;
     float* part;            // [strips][cols] sums of columns, or NULL
     bool whole;
+    uint32_t across, strips, first; // workgroups: 512 columns each, strips of rows; the first one's number
+};
+struct LinPacks {
+    LinPack one[3];
+    uint32_t count, groups;
 };
 
-// A thread has eight columns and every fourth row of a strip: grid (columns / 512, strips).
-template <typename T> __global__ __launch_bounds__(256) void linear_pack(LinPack a) {
+// A thread has eight columns and every fourth row of a strip; one launch for all matrices that a call needs in another form.
+template <typename T> __global__ __launch_bounds__(256) void linear_pack(LinPacks all) {
     constexpr bool SPLIT = sizeof(T) == 4;
     __shared__ float sums[4][512];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = blockIdx.x * 512 + lane * 8;
+    const uint32_t which = all.count > 2 && blockIdx.x >= all.one[2].first ? 2 : all.count > 1 && blockIdx.x >= all.one[1].first ? 1 : 0;
+    const LinPack& a = all.one[which];
+    const uint32_t group = blockIdx.x - a.first, strip = group / a.across, bx = group % a.across;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = bx * 512 + lane * 8;
     float s[8] = {};
     if (j < a.pitch) {
         const bool whole = a.whole && j + 8 <= a.cols;
         const uint32_t left = j < a.cols ? a.cols - j : 0;
 #pragma unroll 2
-        for (uint64_t i = (uint64_t)blockIdx.y * 4 + wave; i < a.rows; i += gridDim.y * 4ull) {
+        for (uint64_t i = (uint64_t)strip * 4 + wave; i < a.rows; i += a.strips * 4ull) {
             float v[8];
             take8<T>(v, a.src, i * a.src_stride + j, whole, left);
             if (a.pre) {
                 float z[8];
                 take8<T>(z, a.pre, i * a.pre_stride + j, whole, left);
-#pragma unroll
-                for (int k = 0; k < 8; k++) v[k] *= slope(z[k], a.act);
+                slope8(v, z, a.act);
             }
 #pragma unroll
             for (int k = 0; k < 8; k++) s[k] += v[k];
@@ -336,7 +438,7 @@ template <typename T> __global__ __launch_bounds__(256) void linear_pack(LinPack
     for (int k = 0; k < 8; k++) sums[wave][lane * 8 + k] = s[k];
     __syncthreads();
     for (uint32_t c = threadIdx.x; c < 512; c += 256)
-        if (blockIdx.x * 512 + c < a.cols) a.part[(uint64_t)blockIdx.y * a.cols + blockIdx.x * 512 + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+        if (bx * 512 + c < a.cols) a.part[(uint64_t)strip * a.cols + bx * 512 + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
 }
 
 // Columns' sums over the strips: 16 columns a workgroup, 64 threads each.
@@ -384,34 +486,69 @@ static uint32_t pitch_of(uint32_t cols) { return (cols + 7) / 8 * 8; }
 template <typename T> static uint64_t packed_bytes(uint64_t rows, uint32_t cols) { return rows * pitch_of(cols) * 2 * (sizeof(T) == 4 ? 3 : 1); }
 
 template <typename T>
-static void pack(apoe_ctx* ctx, const void* src, uint64_t stride, uint32_t rows, uint32_t cols, void* dst, const void* pre, uint64_t pre_stride, uint32_t act, float* part, uint32_t* strips) {
-    LinPack a{src, pre, stride, pre_stride, dst, (uint64_t)rows * pitch_of(cols), rows, cols, pitch_of(cols), act, part, false};
-    constexpr uint32_t V = 16 / sizeof(T);
-    a.whole = ((uintptr_t)src & 15) == 0 && stride % V == 0 && (!pre || (((uintptr_t)pre & 15) == 0 && pre_stride % V == 0));
-    const uint32_t across = (a.pitch + 511) / 512;
-    const uint32_t down = std::max(1u, std::min({(rows + 3) / 4, LIN_STRIPS, std::max(1u, (uint32_t)ctx->num_cus * 8 / across)}));
-    if (strips) *strips = down;
-    linear_pack<T><<<dim3(across, down), 256, 0, ctx->stream>>>(a);
+static LinPack& add_pack(apoe_ctx* ctx, LinPacks& all, const void* src, uint64_t stride, uint32_t rows, uint32_t cols, void* dst) {
+    LinPack& a = all.one[all.count++];
+    a = LinPack{src, nullptr, stride, 0, dst, (uint64_t)rows * pitch_of(cols), rows, cols, pitch_of(cols), 0, nullptr, false, 0, 0, 0};
+    a.whole = ((uintptr_t)src & 15) == 0 && stride % (16 / sizeof(T)) == 0;
+    a.across = (a.pitch + 511) / 512;
+    a.strips = std::max(1u, std::min({(rows + 3) / 4, LIN_STRIPS, std::max(1u, (uint32_t)ctx->num_cus * 8 / a.across)}));
+    return a;
+}
+
+template <typename T> static void pack(apoe_ctx* ctx, LinPacks& all) {
+    for (uint32_t i = 0; i < all.count; i++) {
+        all.one[i].first = all.groups;
+        all.groups += all.one[i].across * all.one[i].strips;
+    }
+    if (all.groups) linear_pack<T><<<all.groups, 256, 0, ctx->stream>>>(all);
 }
 
 struct LinShape {
-    uint32_t bm, bn, kind, cuts, cut_stages, ke;
+    uint32_t bm, bn, kind, cuts, cut_stages;
 };
 
-template <typename S, typename T, int P, bool ACOL, bool BCOL> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t n, uint32_t k) {
-    const uint32_t cus = (uint32_t)ctx->num_cus;
-    auto tiles = [&](uint32_t bm, uint32_t bn) { return (uint64_t)((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
-    LinShape s{};
-    if (P == 1 && tiles(256, 256) >= cus * 4 / 5) s = LinShape{256, 256, 0, 1, 0, 64};
-    else if (tiles(128, 128) >= cus * 4 / 5) s = LinShape{128, 128, 1, 1, 0, P == 1 ? 64u : 32u};
-    else s = LinShape{64, 64, 2, 1, 0, P == 1 ? 64u : 32u};
-    const uint32_t stages = (k + s.ke - 1) / s.ke;
-    const uint64_t t = tiles(s.bm, s.bn);
-    const uint32_t least = 512 / s.ke;
-    s.cuts = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(cus / t, stages / least));
-    s.cut_stages = std::max(1u, (stages + s.cuts - 1) / s.cuts);
-    s.cuts = std::max(1u, (stages + s.cut_stages - 1) / s.cut_stages);
-    return s;
+// Tiles and cuts, by what a product of each kind takes (us, fitted to fp16 and bf16 products of 256 to 8192 a side: a fixed part and one for each
+// inner index, for every round of tiles over the CUs; `two`: pairs of workgroups share a CU, and a CU with one alone takes `alone`). Where few large tiles
+// would leave CUs idle, smaller ones or parts of the inner side win, for which a launch adds the parts up:
+//   256 x 256 8192 x 4096 x 1024 74 (256 x 128: 89); 256 x 128 8192 x 1024 x 4096 69 (256 x 256 in two cuts 84, 128 x 128 76); 128 x 128 with two groups
+//   of waves 4096 x 1024 x 8192 75 (one group, in two cuts 82, 256 x 256 in four 82); 64 x 64 2048 x 1024 x 1024 9.4 (128 x 128 13), 512 x 512 x 4096
+//   17.5, in four cuts 12.
+struct LinKind {
+    uint32_t bm, bn, ke;
+    bool two;
+    float fixed, inner, alone_fixed, alone_inner;
+};
+constexpr LinKind LIN_KINDS[] = {{256, 256, 64, false, 9.f, .0243f, 0.f, 0.f}, {256, 128, 64, false, 6.5f, .0142f, 0.f, 0.f}, {128, 128, 64, true, 5.4f, .0165f, .4f, .0115f},
+                                 {128, 128, 64, false, 3.f, .0082f, 0.f, 0.f}, {64, 64, 64, true, 1.f, .0055f, 1.f, .0033f}};
+constexpr LinKind LIN_KINDS_SPLIT[] = {{128, 128, 32, false, 8.f, .0421f, 0.f, 0.f}, {64, 64, 64, false, 1.5f, .0165f, 0.f, 0.f}};
+
+template <int P> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t n, uint32_t k) {
+    const uint64_t cus = (uint64_t)ctx->num_cus;
+    LinShape best{};
+    float least = INFINITY;
+    const auto look = [&](const LinKind& kind, uint32_t number) {
+        const uint64_t tiles = (uint64_t)((m + kind.bm - 1) / kind.bm) * ((n + kind.bn - 1) / kind.bn);
+        const uint32_t stages = (k + kind.ke - 1) / kind.ke;
+        for (uint32_t cuts = 1; cuts <= 16 && (cuts == 1 || (stages / cuts >= 4 && tiles * cuts <= 2 * cus)); cuts++) {
+            const uint32_t each = std::max(1u, (stages + cuts - 1) / cuts);
+            const uint64_t groups = tiles * cuts, at_once = kind.two ? 2 * cus : cus;
+            const bool alone = kind.two && groups <= cus;
+            const float inner = (float)(each * kind.ke);
+            float t = 3.f + (float)((groups + at_once - 1) / at_once) * (alone ? kind.alone_fixed + kind.alone_inner * inner : kind.fixed + kind.inner * inner);
+            if (cuts > 1) t += 3.f + (float)(cuts + 1) * (float)m * (float)n * 1e-6f; // 4 bytes at 4 TB/s
+            if (t < least) {
+                least = t;
+                best = LinShape{kind.bm, kind.bn, number, std::max(1u, (stages + each - 1) / each), each};
+            }
+        }
+    };
+    uint32_t number = 0;
+    if constexpr (P == 1) {
+        for (const LinKind& kind : LIN_KINDS) look(kind, number++);
+    } else {
+        for (const LinKind& kind : LIN_KINDS_SPLIT) look(kind, number++);
+    }
+    return best;
 }
 
 static uint64_t cut_bytes(const LinShape& s, uint32_t m, uint32_t n) { return s.cuts > 1 ? (uint64_t)s.cuts * m * pitch_of(n) * 4 : 0; }
@@ -423,11 +560,13 @@ static void product(apoe_ctx* ctx, const LinShape& s, LinOperand a, LinOperand b
     hipStream_t st = ctx->stream;
     if constexpr (P == 1) {
         if (s.kind == 0) linear_tile<S, T, P, ACOL, BCOL, 4, 2, 2, 4, 1, 4, 2><<<grid, 512, 0, st>>>(t);
-        else if (s.kind == 1) linear_tile<S, T, P, ACOL, BCOL, 2, 1, 2, 4, 1, 4, 2><<<grid, 512, 0, st>>>(t);
+        else if (s.kind == 1) linear_tile<S, T, P, ACOL, BCOL, 2, 2, 4, 2, 1, 4, 3><<<grid, 512, 0, st>>>(t);
+        else if (s.kind == 2) linear_tile<S, T, P, ACOL, BCOL, 2, 2, 2, 2, 1, 4, 2><<<grid, 256, 0, st>>>(t);
+        else if (s.kind == 3) linear_tile<S, T, P, ACOL, BCOL, 2, 2, 2, 2, 2, 4, 4><<<grid, 512, 0, st>>>(t);
         else linear_tile<S, T, P, ACOL, BCOL, 1, 1, 2, 2, 1, 4, 4><<<grid, 256, 0, st>>>(t);
     } else {
-        if (s.kind == 1) linear_tile<S, T, P, ACOL, BCOL, 2, 2, 2, 2, 2, 2, 3><<<grid, 512, 0, st>>>(t);
-        else linear_tile<S, T, P, ACOL, BCOL, 1, 1, 2, 2, 1, 2, 3><<<grid, 256, 0, st>>>(t);
+        if (s.kind == 0) linear_tile<S, T, P, ACOL, BCOL, 2, 2, 2, 2, 2, 2, 3><<<grid, 512, 0, st>>>(t);
+        else linear_tile<S, T, P, ACOL, BCOL, 1, 1, 2, 2, 1, 4, 3><<<grid, 256, 0, st>>>(t);
     }
     if (s.cuts > 1) linear_join<T><<<(uint32_t)std::min<uint64_t>(((uint64_t)o.m * (t.np / 8) + 255) / 256, 1u << 16), 256, 0, st>>>(t);
 }
@@ -443,25 +582,43 @@ template <> struct LinTypes<float> {
     static constexpr int P = 3;
 };
 
+template <typename T, int MB> static void few(apoe_ctx* ctx, const LinFew& a) {
+    const uint32_t grid = (a.o.n + 15) / 16;
+    // sixteen waves where each has two turns of the inner side at least
+    if (a.k >= 4096) linear_few<T, MB, 16><<<grid, 1024, 0, ctx->stream>>>(a);
+    else linear_few<T, MB, 8><<<grid, 512, 0, ctx->stream>>>(a);
+}
+
 template <typename T> static int run_linear(apoe_ctx* ctx, const apoe_linear_args* p) {
     using S = typename LinTypes<T>::S;
     constexpr int P = LinTypes<T>::P;
     const uint32_t m = p->rows, n = p->cols_out, k = p->cols_in;
+    constexpr uint32_t E = 16 / sizeof(T);
+    if (m <= 64 && k % E == 0 && whole_out<T>(p->x, p->x_stride) && whole_out<T>(p->w, p->w_stride)) {
+        const LinFew a{p->x, p->w, p->x_stride, p->w_stride, k, LinOut{p->y, p->bias, p->residual, p->pre, p->y_stride, p->residual_stride, p->pre_stride, m, n, p->act, false}};
+        if (m <= 16) few<T, 1>(ctx, a);
+        else if (m <= 32) few<T, 2>(ctx, a);
+        else few<T, 4>(ctx, a);
+        APOE_HIP(hipGetLastError());
+        return APOE_OK;
+    }
     const bool x_is = as_it_is(p->x, p->x_stride, k, P > 1), w_is = as_it_is(p->w, p->w_stride, k, P > 1);
-    const LinShape s = choose<S, T, P, false, false>(ctx, m, n, k);
+    const LinShape s = choose<P>(ctx, m, n, k);
     LinPlan plan;
     const uint64_t o_x = plan.take(x_is ? 0 : packed_bytes<T>(m, k)), o_w = plan.take(w_is ? 0 : packed_bytes<T>(n, k)), o_part = plan.take(cut_bytes(s, m, n));
     char* ws = nullptr;
     if (plan.bytes) APOE_TRY(ctx->adapt_workspace(plan.bytes, &ws));
     LinOperand x{p->x, 0, (uint32_t)(p->x_stride * sizeof(S))}, w{p->w, 0, (uint32_t)(p->w_stride * sizeof(S))};
+    LinPacks packs{};
     if (!x_is) {
         x = LinOperand{ws + o_x, (uint64_t)m * pitch_of(k), pitch_of(k) * (uint32_t)sizeof(S)};
-        pack<T>(ctx, p->x, p->x_stride, m, k, ws + o_x, nullptr, 0, 0, nullptr, nullptr);
+        add_pack<T>(ctx, packs, p->x, p->x_stride, m, k, ws + o_x);
     }
     if (!w_is) {
         w = LinOperand{ws + o_w, (uint64_t)n * pitch_of(k), pitch_of(k) * (uint32_t)sizeof(S)};
-        pack<T>(ctx, p->w, p->w_stride, n, k, ws + o_w, nullptr, 0, 0, nullptr, nullptr);
+        add_pack<T>(ctx, packs, p->w, p->w_stride, n, k, ws + o_w);
     }
+    pack<T>(ctx, packs);
     LinOut o{p->y, p->bias, p->residual, p->pre, p->y_stride, p->residual_stride, p->pre_stride, m, n, p->act, false};
     o.whole = whole_out<T>(p->y, p->y_stride) && whole_out<T>(p->residual, p->residual_stride) && whole_out<T>(p->pre, p->pre_stride) && ((uintptr_t)p->bias & 15) == 0;
     product<S, T, P, false, false>(ctx, s, x, w, k, (float*)(ws + o_part), o);
@@ -477,28 +634,38 @@ template <typename T> static int run_linear_grad(apoe_ctx* ctx, const apoe_linea
     const bool g_is = !act && as_it_is(p->grad_y, p->grad_y_stride, n, P > 1), x_is = !p->grad_w || as_it_is(p->x, p->x_stride, k, P > 1), w_is = !p->grad_x || as_it_is(p->w, p->w_stride, k, P > 1);
     const bool pack_g = products && !g_is;
     LinShape sx{}, sw{};
-    if (p->grad_x) sx = choose<S, T, P, false, true>(ctx, m, k, n);
-    if (p->grad_w) sw = choose<S, T, P, true, true>(ctx, n, k, m);
+    if (p->grad_x) sx = choose<P>(ctx, m, k, n);
+    if (p->grad_w) sw = choose<P>(ctx, n, k, m);
     LinPlan plan;
     const uint64_t o_g = plan.take(pack_g ? packed_bytes<T>(m, n) : 0), o_x = plan.take(x_is ? 0 : packed_bytes<T>(m, k)), o_w = plan.take(w_is ? 0 : packed_bytes<T>(n, k));
     const uint64_t o_part = plan.take(std::max({p->grad_x ? cut_bytes(sx, m, k) : 0, p->grad_w ? cut_bytes(sw, n, k) : 0, p->grad_bias ? (uint64_t)LIN_STRIPS * n * 4 : 0}));
     char* ws = nullptr;
     if (plan.bytes) APOE_TRY(ctx->adapt_workspace(plan.bytes, &ws));
     LinOperand g{p->grad_y, 0, (uint32_t)(p->grad_y_stride * sizeof(S))}, x{p->x, 0, (uint32_t)(p->x_stride * sizeof(S))}, w{p->w, 0, (uint32_t)(p->w_stride * sizeof(S))};
+    LinPacks packs{};
+    uint32_t strips = 0;
     if (pack_g || p->grad_bias) {
-        uint32_t strips = 0;
-        pack<T>(ctx, p->grad_y, p->grad_y_stride, m, n, pack_g ? ws + o_g : nullptr, act ? p->pre : nullptr, p->pre_stride, p->act, p->grad_bias ? (float*)(ws + o_part) : nullptr, &strips);
-        if (p->grad_bias) linear_bias<<<(n + 15) / 16, 1024, 0, ctx->stream>>>((const float*)(ws + o_part), strips, n, p->grad_bias);
+        LinPack& a = add_pack<T>(ctx, packs, p->grad_y, p->grad_y_stride, m, n, pack_g ? ws + o_g : nullptr);
+        if (act) {
+            a.pre = p->pre;
+            a.pre_stride = p->pre_stride;
+            a.act = p->act;
+            a.whole &= ((uintptr_t)p->pre & 15) == 0 && p->pre_stride % (16 / sizeof(T)) == 0;
+        }
+        if (p->grad_bias) a.part = (float*)(ws + o_part);
+        strips = a.strips;
         if (pack_g) g = LinOperand{ws + o_g, (uint64_t)m * pitch_of(n), pitch_of(n) * (uint32_t)sizeof(S)};
     }
     if (!x_is) {
         x = LinOperand{ws + o_x, (uint64_t)m * pitch_of(k), pitch_of(k) * (uint32_t)sizeof(S)};
-        pack<T>(ctx, p->x, p->x_stride, m, k, ws + o_x, nullptr, 0, 0, nullptr, nullptr);
+        add_pack<T>(ctx, packs, p->x, p->x_stride, m, k, ws + o_x);
     }
     if (!w_is) {
         w = LinOperand{ws + o_w, (uint64_t)n * pitch_of(k), pitch_of(k) * (uint32_t)sizeof(S)};
-        pack<T>(ctx, p->w, p->w_stride, n, k, ws + o_w, nullptr, 0, 0, nullptr, nullptr);
+        add_pack<T>(ctx, packs, p->w, p->w_stride, n, k, ws + o_w);
     }
+    pack<T>(ctx, packs);
+    if (p->grad_bias) linear_bias<<<(n + 15) / 16, 1024, 0, ctx->stream>>>((const float*)(ws + o_part), strips, n, p->grad_bias);
     if (p->grad_x && m) {
         LinOut o{p->grad_x, nullptr, nullptr, nullptr, p->grad_x_stride, 0, 0, m, k, APOE_ACT_NONE, whole_out<T>(p->grad_x, p->grad_x_stride)};
         product<S, T, P, false, true>(ctx, sx, g, w, n, (float*)(ws + o_part), o);
