@@ -11,9 +11,11 @@ namespace apoe {
 
 constexpr int ROW_E = 16; // values of a row that a thread holds
 
-// Values (c G + t) V .. of a row, c = 0, 1, ..: 16 bytes a load with V > 1.
-template <typename T, int V, int G> struct RowOf {
+// Values (c G + t) V .. of a row, c = 0, 1, ..: 16 bytes a load with V > 1. WHOLE: rows begin at multiples of 16 bytes and have a multiple of V values;
+// otherwise they begin at any value, and a row's last few are read and written one by one.
+template <typename T, int V, int G, bool WHOLE = true> struct RowOf {
     typedef T tv __attribute__((ext_vector_type(V)));
+    typedef tv tu __attribute__((aligned(WHOLE ? sizeof(tv) : sizeof(T))));
     static constexpr int C = ROW_E / V;
     // as it comes, and as numbers
     __device__ static void fetch(tv* raw, const void* p, uint64_t row, uint64_t stride, uint32_t dim, int t) {
@@ -24,8 +26,16 @@ template <typename T, int V, int G> struct RowOf {
             raw[c] = tv{};
             if constexpr (V == 1) {
                 if (d < dim) raw[c][0] = at[d];
-            } else {
+            } else if constexpr (WHOLE) {
                 if (d < dim) raw[c] = *reinterpret_cast<const tv*>(at + d);
+            } else {
+                if (d + V <= dim) {
+                    raw[c] = *reinterpret_cast<const tu*>(at + d);
+                } else if (d < dim) {
+#pragma unroll
+                    for (int k = 0; k < V - 1; k++)
+                        if (d + k < dim) raw[c][k] = at[d + k];
+                }
             }
         }
     }
@@ -52,13 +62,21 @@ template <typename T, int V, int G> struct RowOf {
                 tv x;
 #pragma unroll
                 for (int k = 0; k < V; k++) x[k] = (T)v[c * V + k];
-                *reinterpret_cast<tv*>(at + d) = x;
+                if constexpr (WHOLE) {
+                    *reinterpret_cast<tv*>(at + d) = x;
+                } else if (d + V <= dim) {
+                    *reinterpret_cast<tu*>(at + d) = x;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < V - 1; k++)
+                        if (d + k < dim) at[d + k] = x[k];
+                }
             }
         }
     }
     // a vector of floats (ones without one)
     __device__ static void vec(float* v, const float* p, uint32_t dim, int t, bool aligned) {
-        if constexpr (V > 1) {
+        if constexpr (V > 1 && WHOLE) {
             if (p && aligned) {
                 typedef float f4 __attribute__((ext_vector_type(4)));
 #pragma unroll

@@ -40,8 +40,8 @@ struct EmbedArgs {
 };
 
 // S groups share a row's entries, in turn, and are the workgroup's threads; with S = 1 a workgroup has as many rows as groups.
-template <typename T, int V, int G, int S> __global__ __launch_bounds__(S > 1 ? S * G : (G > 256 ? G : 256)) void embed_rows(apoe_embed_args p) {
-    using R = RowOf<T, V, G>;
+template <typename T, int V, int G, bool WHOLE, int S> __global__ __launch_bounds__(S > 1 ? S * G : (G > 256 ? G : 256)) void embed_rows(apoe_embed_args p) {
+    using R = RowOf<T, V, G, WHOLE>;
     constexpr int THREADS = S > 1 ? S * G : (G > 256 ? G : 256), GROUPS = S > 1 ? 1 : THREADS / G, U = 4;
     __shared__ float sums[S > 1 ? S * G * ROW_E : 1];
     const int t = threadIdx.x % G, group = threadIdx.x / G;
@@ -106,8 +106,8 @@ template <typename T, int V, int G, int S> __global__ __launch_bounds__(S > 1 ? 
 }
 
 // One number an entry: the entries of a row in turn by blockIdx.y.
-template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 256) void embed_weights(apoe_embed_args p) {
-    using R = RowOf<T, V, G>;
+template <typename T, int V, int G, bool WHOLE> __global__ __launch_bounds__(G > 256 ? G : 256) void embed_weights(apoe_embed_args p) {
+    using R = RowOf<T, V, G, WHOLE>;
     constexpr int GROUPS = (G > 256 ? G : 256) / G, U = 4;
     __shared__ float buf[U][8];
     const int t = threadIdx.x % G;
@@ -320,8 +320,8 @@ __device__ inline uint32_t first_at_least(const Entry* sorted, uint32_t lo, uint
     return lo;
 }
 
-template <typename T, int V, int G> __device__ inline void put_table_row(const apoe_embed_args& p, uint32_t key, int t, const float* sum) {
-    using R = RowOf<T, V, G>;
+template <typename T, int V, int G, bool WHOLE> __device__ inline void put_table_row(const apoe_embed_args& p, uint32_t key, int t, const float* sum) {
+    using R = RowOf<T, V, G, WHOLE>;
     float v[ROW_E];
     if (p.accumulate) {
         R::load(v, p.grad_table, key, p.grad_table_stride, p.dim, t);
@@ -335,8 +335,8 @@ template <typename T, int V, int G> __device__ inline void put_table_row(const a
 }
 
 // The first workgroups: a group a block of entries. The others: zeros for the rows that no entry names, 64 of the table a workgroup.
-template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 256) void embed_table(EmbedArgs a, uint32_t entry_groups) {
-    using R = RowOf<T, V, G>;
+template <typename T, int V, int G, bool WHOLE> __global__ __launch_bounds__(G > 256 ? G : 256) void embed_table(EmbedArgs a, uint32_t entry_groups) {
+    using R = RowOf<T, V, G, WHOLE>;
     constexpr int THREADS = G > 256 ? G : 256, GROUPS = THREADS / G, U = sizeof(T) == 4 ? 2 : 4;
     const apoe_embed_args& p = a.p;
     const int t = threadIdx.x % G, group = threadIdx.x / G;
@@ -374,7 +374,7 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
     auto leave = [&](bool last) {
         if (key >= p.n_table) return;
         if (!goes_on && !(last && behind == key)) {
-            put_table_row<T, V, G>(p, key, t, acc);
+            put_table_row<T, V, G, WHOLE>(p, key, t, acc);
             return;
         }
         float* out = a.part + ((size_t)block * 2 + (goes_on ? 0 : 1)) * a.part_pitch;
@@ -520,7 +520,7 @@ template <typename T> __global__ __launch_bounds__(1024) void embed_join(EmbedAr
     }
 }
 
-template <typename T, int V> static int run_embed(apoe_ctx* ctx, const apoe_embed_args* p) {
+template <typename T, int V, bool WHOLE> static int run_embed(apoe_ctx* ctx, const apoe_embed_args* p) {
     hipStream_t s = ctx->stream;
     // Few rows with many entries each: groups share a row, so that the GPU has some 16 waves a CU to wait for memory with, and each at least two entries.
     return with_group(p->dim, [&](auto size) -> int {
@@ -528,22 +528,22 @@ template <typename T, int V> static int run_embed(apoe_ctx* ctx, const apoe_embe
         const uint64_t waves = (uint64_t)p->n_rows * (G > 64 ? G / 64 : 1), room = (uint64_t)ctx->num_cus * 16;
         const auto shared_by = [&](uint64_t groups) { return p->n_entries >= (uint64_t)p->n_rows * groups * 2 && waves * groups <= room * 4; };
         if (shared_by(MOST)) {
-            embed_rows<T, V, G, MOST><<<p->n_rows, MOST * G, 0, s>>>(*p);
+            embed_rows<T, V, G, WHOLE, MOST><<<p->n_rows, MOST * G, 0, s>>>(*p);
             return APOE_OK;
         }
         if constexpr (MOST > 4) {
             if (shared_by(4)) {
-                embed_rows<T, V, G, 4><<<p->n_rows, 4 * G, 0, s>>>(*p);
+                embed_rows<T, V, G, WHOLE, 4><<<p->n_rows, 4 * G, 0, s>>>(*p);
                 return APOE_OK;
             }
         }
         const uint64_t need = ((uint64_t)p->n_rows + THREADS / G - 1) / (THREADS / G);
-        embed_rows<T, V, G, 1><<<(uint32_t)std::min<uint64_t>(need, 1u << 20), THREADS, 0, s>>>(*p);
+        embed_rows<T, V, G, WHOLE, 1><<<(uint32_t)std::min<uint64_t>(need, 1u << 20), THREADS, 0, s>>>(*p);
         return APOE_OK;
     });
 }
 
-template <typename T, int V> static int run_embed_grad(apoe_ctx* ctx, const apoe_embed_args* p) {
+template <typename T, int V, bool WHOLE> static int run_embed_grad(apoe_ctx* ctx, const apoe_embed_args* p) {
     hipStream_t s = ctx->stream;
     if (p->grad_val && p->n_rows && p->n_entries) {
         APOE_TRY(with_group(p->dim, [&](auto size) -> int {
@@ -551,7 +551,7 @@ template <typename T, int V> static int run_embed_grad(apoe_ctx* ctx, const apoe
             const uint64_t need = ((uint64_t)p->n_rows + THREADS / G - 1) / (THREADS / G);
             // few rows: their entries in turn by up to 16 workgroups
             const uint32_t share = (uint32_t)std::min<uint64_t>(16, std::max<uint64_t>(1, std::min<uint64_t>((uint64_t)ctx->num_cus * 8 / need, p->n_entries / (p->n_rows * 4ull))));
-            embed_weights<T, V, G><<<dim3((uint32_t)std::min<uint64_t>(need, 1u << 20), share), THREADS, 0, s>>>(*p);
+            embed_weights<T, V, G, WHOLE><<<dim3((uint32_t)std::min<uint64_t>(need, 1u << 20), share), THREADS, 0, s>>>(*p);
             return APOE_OK;
         }));
     }
@@ -594,7 +594,7 @@ template <typename T, int V> static int run_embed_grad(apoe_ctx* ctx, const apoe
     APOE_TRY(with_group(p->dim, [&](auto size) -> int {
         constexpr int G = decltype(size)::value, THREADS = G > 256 ? G : 256;
         const uint32_t entry_groups = (a.blocks + THREADS / G - 1) / (THREADS / G), zero_groups = p->accumulate ? 0 : std::min((p->n_table + 63) / 64, 1u << 20);
-        embed_table<T, V, G><<<entry_groups + zero_groups, THREADS, 0, s>>>(a, entry_groups);
+        embed_table<T, V, G, WHOLE><<<entry_groups + zero_groups, THREADS, 0, s>>>(a, entry_groups);
         return APOE_OK;
     }));
     if (a.blocks > 1) embed_join<T><<<dim3((a.blocks + 15) / 16, (p->dim + 255) / 256), 1024, 0, s>>>(a);
@@ -603,11 +603,11 @@ template <typename T, int V> static int run_embed_grad(apoe_ctx* ctx, const apoe
 
 template <typename T> static int run_aligned(apoe_ctx* ctx, const apoe_embed_args* p, bool grad) {
     constexpr int V = 16 / (int)sizeof(T);
-    bool whole = p->dim % V == 0; // 16 bytes a load where every row begins at a multiple of that
+    bool whole = p->dim % V == 0;
     for (const void* q : {p->table, p->base, (const void*)p->out, p->grad, (const void*)p->grad_table}) whole &= ((uintptr_t)q & 15) == 0;
     for (uint64_t q : {p->table_stride, p->base_stride, p->out_stride, p->grad_stride, p->grad_table_stride}) whole &= q % V == 0;
-    if (grad) APOE_TRY(whole ? (run_embed_grad<T, V>(ctx, p)) : (run_embed_grad<T, 1>(ctx, p)));
-    else APOE_TRY(whole ? (run_embed<T, V>(ctx, p)) : (run_embed<T, 1>(ctx, p)));
+    if (grad) APOE_TRY(whole ? (run_embed_grad<T, V, true>(ctx, p)) : (run_embed_grad<T, V, false>(ctx, p)));
+    else APOE_TRY(whole ? (run_embed<T, V, true>(ctx, p)) : (run_embed<T, V, false>(ctx, p)));
     APOE_HIP(hipGetLastError());
     return APOE_OK;
 }

@@ -22,7 +22,6 @@ struct LinOut { // what becomes of a product's sums
     void* pre;
     uint64_t out_stride, residual_stride, pre_stride;
     uint32_t m, n, act;
-    bool whole;             // every row begins at a multiple of 16 bytes, and so does the bias
 };
 
 struct LinTile {
@@ -98,37 +97,36 @@ __device__ inline void slope8(float* v, const float* z, uint32_t act) {
     }
 }
 
-// Eight values of a row as numbers, `left` of them there (whole: eight, from a multiple of 16 bytes).
-template <typename T> __device__ inline void take8(float* v, const void* p, uint64_t at, bool whole, uint32_t left) {
+// Eight values of a row as numbers, `left` of them there. They begin at any value: the vector loads and stores ask for no more alignment than its type's.
+template <typename T> __device__ inline void take8(float* v, const void* p, uint64_t at, uint32_t left) {
     const T* from = (const T*)p + at;
-    if (whole) {
-        if constexpr (sizeof(T) == 4) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(from), y = *reinterpret_cast<const f32x4*>(from + 4);
+    if (left >= 8) {
+        typedef T tv __attribute__((ext_vector_type(16 / sizeof(T))));
+        typedef tv tu __attribute__((aligned(sizeof(T))));
+        constexpr int E = 16 / sizeof(T);
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = k < 4 ? x[k] : y[k - 4];
-        } else {
-            typedef T t8 __attribute__((ext_vector_type(8)));
-            const t8 x = *reinterpret_cast<const t8*>(from);
+        for (int c = 0; c < 8 / E; c++) {
+            const tv x = *reinterpret_cast<const tu*>(from + c * E);
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = (float)x[k];
+            for (int k = 0; k < E; k++) v[c * E + k] = (float)x[k];
         }
         return;
     }
 #pragma unroll
     for (int k = 0; k < 8; k++) v[k] = (uint32_t)k < left ? (float)from[k] : 0.f;
 }
-template <typename T> __device__ inline void give8(void* p, uint64_t at, const float* v, bool whole, uint32_t left) {
+template <typename T> __device__ inline void give8(void* p, uint64_t at, const float* v, uint32_t left) {
     T* to = (T*)p + at;
-    if (whole) {
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<f32x4*>(to + 4) = f32x4{v[4], v[5], v[6], v[7]};
-        } else {
-            typedef T t8 __attribute__((ext_vector_type(8)));
-            t8 x;
+    if (left >= 8) {
+        typedef T tv __attribute__((ext_vector_type(16 / sizeof(T))));
+        typedef tv tu __attribute__((aligned(sizeof(T))));
+        constexpr int E = 16 / sizeof(T);
 #pragma unroll
-            for (int k = 0; k < 8; k++) x[k] = (T)v[k];
-            *reinterpret_cast<t8*>(to) = x;
+        for (int c = 0; c < 8 / E; c++) {
+            tv x;
+#pragma unroll
+            for (int k = 0; k < E; k++) x[k] = (T)v[c * E + k];
+            *reinterpret_cast<tu*>(to + c * E) = x;
         }
         return;
     }
@@ -139,23 +137,22 @@ template <typename T> __device__ inline void give8(void* p, uint64_t at, const f
 
 // Eight sums of row i from column j on. T: the type of the results.
 template <typename T> __device__ inline void finish8(const LinOut& o, uint32_t i, uint32_t j, float* v) {
-    const bool whole = o.whole && j + 8 <= o.n;
     const uint32_t left = o.n - j;
     if (o.bias) {
         float b[8];
-        take8<float>(b, o.bias, j, whole, left);
+        take8<float>(b, o.bias, j, left);
 #pragma unroll
         for (int k = 0; k < 8; k++) v[k] += b[k];
     }
-    if (o.pre) give8<T>(o.pre, i * o.pre_stride + j, v, whole, left);
+    if (o.pre) give8<T>(o.pre, i * o.pre_stride + j, v, left);
     activate8(v, o.act);
     if (o.residual) {
         float r[8];
-        take8<T>(r, o.residual, i * o.residual_stride + j, whole, left);
+        take8<T>(r, o.residual, i * o.residual_stride + j, left);
 #pragma unroll
         for (int k = 0; k < 8; k++) v[k] += r[k];
     }
-    give8<T>(o.out, i * o.out_stride + j, v, whole, left);
+    give8<T>(o.out, i * o.out_stride + j, v, left);
 }
 
 // One.
@@ -382,7 +379,6 @@ struct LinPack {
     uint64_t low;           // values from plane to plane
     uint32_t rows, cols, pitch, act;
     float* part;            // [strips][cols] sums of columns, or NULL
-    bool whole;
     uint32_t across, strips, first; // workgroups: 512 columns each, strips of rows; the first one's number
 };
 struct LinPacks {
@@ -400,15 +396,14 @@ template <typename T> __global__ __launch_bounds__(256) void linear_pack(LinPack
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = bx * 512 + lane * 8;
     float s[8] = {};
     if (j < a.pitch) {
-        const bool whole = a.whole && j + 8 <= a.cols;
-        const uint32_t left = j < a.cols ? a.cols - j : 0;
+        const uint32_t left = a.cols - j;
 #pragma unroll 2
         for (uint64_t i = (uint64_t)strip * 4 + wave; i < a.rows; i += a.strips * 4ull) {
             float v[8];
-            take8<T>(v, a.src, i * a.src_stride + j, whole, left);
+            take8<T>(v, a.src, i * a.src_stride + j, left);
             if (a.pre) {
                 float z[8];
-                take8<T>(z, a.pre, i * a.pre_stride + j, whole, left);
+                take8<T>(z, a.pre, i * a.pre_stride + j, left);
                 slope8(v, z, a.act);
             }
 #pragma unroll
@@ -429,7 +424,7 @@ template <typename T> __global__ __launch_bounds__(256) void linear_pack(LinPack
                     *reinterpret_cast<b8*>((__bf16*)a.dst + p * a.low + i * a.pitch + j) = w;
                 }
             } else {
-                give8<T>(a.dst, i * a.pitch + j, v, true, 8);
+                give8<T>(a.dst, i * a.pitch + j, v, 8);
             }
         }
     }
@@ -488,8 +483,7 @@ template <typename T> static uint64_t packed_bytes(uint64_t rows, uint32_t cols)
 template <typename T>
 static LinPack& add_pack(apoe_ctx* ctx, LinPacks& all, const void* src, uint64_t stride, uint32_t rows, uint32_t cols, void* dst) {
     LinPack& a = all.one[all.count++];
-    a = LinPack{src, nullptr, stride, 0, dst, (uint64_t)rows * pitch_of(cols), rows, cols, pitch_of(cols), 0, nullptr, false, 0, 0, 0};
-    a.whole = ((uintptr_t)src & 15) == 0 && stride % (16 / sizeof(T)) == 0;
+    a = LinPack{src, nullptr, stride, 0, dst, (uint64_t)rows * pitch_of(cols), rows, cols, pitch_of(cols), 0, nullptr, 0, 0, 0};
     a.across = (a.pitch + 511) / 512;
     a.strips = std::max(1u, std::min({(rows + 3) / 4, LIN_STRIPS, std::max(1u, (uint32_t)ctx->num_cus * 8 / a.across)}));
     return a;
@@ -571,7 +565,7 @@ static void product(apoe_ctx* ctx, const LinShape& s, LinOperand a, LinOperand b
     if (s.cuts > 1) linear_join<T><<<(uint32_t)std::min<uint64_t>(((uint64_t)o.m * (t.np / 8) + 255) / 256, 1u << 16), 256, 0, st>>>(t);
 }
 
-template <typename T> static bool whole_out(const void* p, uint64_t stride) { return ((uintptr_t)p & 15) == 0 && stride % (16 / sizeof(T)) == 0; }
+template <typename T> static bool whole_rows(const void* p, uint64_t stride) { return ((uintptr_t)p & 15) == 0 && stride % (16 / sizeof(T)) == 0; }
 
 template <typename T> struct LinTypes {
     using S = T;
@@ -594,8 +588,8 @@ template <typename T> static int run_linear(apoe_ctx* ctx, const apoe_linear_arg
     constexpr int P = LinTypes<T>::P;
     const uint32_t m = p->rows, n = p->cols_out, k = p->cols_in;
     constexpr uint32_t E = 16 / sizeof(T);
-    if (m <= 64 && k % E == 0 && whole_out<T>(p->x, p->x_stride) && whole_out<T>(p->w, p->w_stride)) {
-        const LinFew a{p->x, p->w, p->x_stride, p->w_stride, k, LinOut{p->y, p->bias, p->residual, p->pre, p->y_stride, p->residual_stride, p->pre_stride, m, n, p->act, false}};
+    if (m <= 64 && k % E == 0 && whole_rows<T>(p->x, p->x_stride) && whole_rows<T>(p->w, p->w_stride)) {
+        const LinFew a{p->x, p->w, p->x_stride, p->w_stride, k, LinOut{p->y, p->bias, p->residual, p->pre, p->y_stride, p->residual_stride, p->pre_stride, m, n, p->act}};
         if (m <= 16) few<T, 1>(ctx, a);
         else if (m <= 32) few<T, 2>(ctx, a);
         else few<T, 4>(ctx, a);
@@ -619,8 +613,7 @@ template <typename T> static int run_linear(apoe_ctx* ctx, const apoe_linear_arg
         add_pack<T>(ctx, packs, p->w, p->w_stride, n, k, ws + o_w);
     }
     pack<T>(ctx, packs);
-    LinOut o{p->y, p->bias, p->residual, p->pre, p->y_stride, p->residual_stride, p->pre_stride, m, n, p->act, false};
-    o.whole = whole_out<T>(p->y, p->y_stride) && whole_out<T>(p->residual, p->residual_stride) && whole_out<T>(p->pre, p->pre_stride) && ((uintptr_t)p->bias & 15) == 0;
+    LinOut o{p->y, p->bias, p->residual, p->pre, p->y_stride, p->residual_stride, p->pre_stride, m, n, p->act};
     product<S, T, P, false, false>(ctx, s, x, w, k, (float*)(ws + o_part), o);
     APOE_HIP(hipGetLastError());
     return APOE_OK;
@@ -650,7 +643,6 @@ template <typename T> static int run_linear_grad(apoe_ctx* ctx, const apoe_linea
             a.pre = p->pre;
             a.pre_stride = p->pre_stride;
             a.act = p->act;
-            a.whole &= ((uintptr_t)p->pre & 15) == 0 && p->pre_stride % (16 / sizeof(T)) == 0;
         }
         if (p->grad_bias) a.part = (float*)(ws + o_part);
         strips = a.strips;
@@ -667,11 +659,11 @@ template <typename T> static int run_linear_grad(apoe_ctx* ctx, const apoe_linea
     pack<T>(ctx, packs);
     if (p->grad_bias) linear_bias<<<(n + 15) / 16, 1024, 0, ctx->stream>>>((const float*)(ws + o_part), strips, n, p->grad_bias);
     if (p->grad_x && m) {
-        LinOut o{p->grad_x, nullptr, nullptr, nullptr, p->grad_x_stride, 0, 0, m, k, APOE_ACT_NONE, whole_out<T>(p->grad_x, p->grad_x_stride)};
+        LinOut o{p->grad_x, nullptr, nullptr, nullptr, p->grad_x_stride, 0, 0, m, k, APOE_ACT_NONE};
         product<S, T, P, false, true>(ctx, sx, g, w, n, (float*)(ws + o_part), o);
     }
     if (p->grad_w) {
-        LinOut o{p->grad_w, nullptr, nullptr, nullptr, p->grad_w_stride, 0, 0, n, k, APOE_ACT_NONE, whole_out<T>(p->grad_w, p->grad_w_stride)};
+        LinOut o{p->grad_w, nullptr, nullptr, nullptr, p->grad_w_stride, 0, 0, n, k, APOE_ACT_NONE};
         product<S, T, P, true, true>(ctx, sw, g, x, m, (float*)(ws + o_part), o);
     }
     APOE_HIP(hipGetLastError());

@@ -24,7 +24,7 @@ struct NormArgs {
 };
 
 // v less its mean (zeros beyond the row), and one over its deviation.
-template <typename R, int V, int G> __device__ inline float normalise(float* v, uint32_t dim, float inv, float eps, int t, float (*buf)[8]) {
+template <typename R, int V, int G, bool WHOLE> __device__ inline float normalise(float* v, uint32_t dim, float inv, float eps, int t, float (*buf)[8]) {
     float s[1] = {0.f};
 #pragma unroll
     for (int k = 0; k < ROW_E; k++) s[0] += v[k];
@@ -33,11 +33,11 @@ template <typename R, int V, int G> __device__ inline float normalise(float* v, 
     s[0] = 0.f;
 #pragma unroll
     for (int c = 0; c < R::C; c++) {
-        const bool in = (uint32_t)(c * G + t) * V < dim;
+        const uint32_t d = (c * G + t) * V;
 #pragma unroll
         for (int k = 0; k < V; k++) {
             float& x = v[c * V + k];
-            x = in ? x - mean : 0.f;
+            x = d + (WHOLE ? 0 : k) < dim ? x - mean : 0.f;
             s[0] = __builtin_fmaf(x, x, s[0]);
         }
     }
@@ -45,8 +45,8 @@ template <typename R, int V, int G> __device__ inline float normalise(float* v, 
     return 1.f / sqrtf(__builtin_fmaf(s[0], inv, eps));
 }
 
-template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 256) void norm_forward(NormArgs a) {
-    using R = RowOf<T, V, G>;
+template <typename T, int V, int G, bool WHOLE> __global__ __launch_bounds__(G > 256 ? G : 256) void norm_forward(NormArgs a) {
+    using R = RowOf<T, V, G, WHOLE>;
     constexpr int GROUPS = (G > 256 ? G : 256) / G;
     __shared__ float buf[2][8];
     const apoe_layer_norm_args& p = a.p;
@@ -68,15 +68,15 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
         float v[ROW_E];
         R::widen(v, xr);
         if (row + step < p.rows) R::fetch(xr, p.x, row + step, p.x_stride, p.dim, t);
-        const float r = normalise<R, V, G>(v, p.dim, inv, p.eps, t, buf);
+        const float r = normalise<R, V, G, WHOLE>(v, p.dim, inv, p.eps, t, buf);
 #pragma unroll
         for (int k = 0; k < ROW_E; k++) v[k] = __builtin_fmaf(v[k] * r, w[k], b[k]);
         R::store(p.y, row, p.y_stride, p.dim, t, v);
     }
 }
 
-template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 256) void norm_backward(NormArgs a) {
-    using R = RowOf<T, V, G>;
+template <typename T, int V, int G, bool WHOLE> __global__ __launch_bounds__(G > 256 ? G : 256) void norm_backward(NormArgs a) {
+    using R = RowOf<T, V, G, WHOLE>;
     constexpr int THREADS = G > 256 ? G : 256, GROUPS = THREADS / G;
     __shared__ float buf[2][8];
     __shared__ float sums[GROUPS > 1 ? THREADS * ROW_E : 1];
@@ -103,7 +103,7 @@ template <typename T, int V, int G> __global__ __launch_bounds__(G > 256 ? G : 2
 #pragma unroll
         for (int c = 0; c < R::C; c++) skip[c] = sr[c];
         ask(row + step);
-        const float r = normalise<R, V, G>(v, p.dim, inv, p.eps, t, buf);
+        const float r = normalise<R, V, G, WHOLE>(v, p.dim, inv, p.eps, t, buf);
         float s[2] = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < ROW_E; k++) {
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(1024) void norm_vectors(NormArgs a) {
     if (l == 0 && d < dim) out[d] = q[0][c];
 }
 
-template <typename T, int V> static int run_norm(apoe_ctx* ctx, const apoe_layer_norm_args* p, bool grad) {
+template <typename T, int V, bool WHOLE> static int run_norm(apoe_ctx* ctx, const apoe_layer_norm_args* p, bool grad) {
     NormArgs a{*p, nullptr, 0, (((uintptr_t)p->w | (uintptr_t)p->b) & 15) == 0};
     hipStream_t s = ctx->stream;
     const uint32_t cus = (uint32_t)ctx->num_cus;
@@ -181,7 +181,7 @@ template <typename T, int V> static int run_norm(apoe_ctx* ctx, const apoe_layer
         constexpr int G = decltype(size)::value, THREADS = G > 256 ? G : 256;
         const uint32_t need = (uint32_t)(((uint64_t)p->rows + THREADS / G - 1) / (THREADS / G));
         if (!grad) {
-            norm_forward<T, V, G><<<std::min(need, cus * 8), THREADS, 0, s>>>(a);
+            norm_forward<T, V, G, WHOLE><<<std::min(need, cus * 8), THREADS, 0, s>>>(a);
             return APOE_OK;
         }
         a.blocks = std::min(need, NORM_BLOCKS);
@@ -191,7 +191,7 @@ template <typename T, int V> static int run_norm(apoe_ctx* ctx, const apoe_layer
             APOE_TRY(ctx->adapt_workspace((size_t)a.blocks * 2 * p->dim * 4, &ws));
             a.part = (float*)ws;
         }
-        if (a.blocks) norm_backward<T, V, G><<<a.blocks, THREADS, 0, s>>>(a); // no rows: the vectors' gradients alone, which are zeros
+        if (a.blocks) norm_backward<T, V, G, WHOLE><<<a.blocks, THREADS, 0, s>>>(a); // no rows: the vectors' gradients alone, which are zeros
         if (vectors) norm_vectors<<<dim3((p->dim + 15) / 16, 2), 1024, 0, s>>>(a);
         return APOE_OK;
     }));
@@ -201,10 +201,10 @@ template <typename T, int V> static int run_norm(apoe_ctx* ctx, const apoe_layer
 
 template <typename T> static int run_aligned(apoe_ctx* ctx, const apoe_layer_norm_args* p, bool grad) {
     constexpr int V = 16 / (int)sizeof(T);
-    bool whole = p->dim % V == 0; // 16 bytes a load where every row begins at a multiple of that
+    bool whole = p->dim % V == 0;
     for (const void* q : {p->x, (const void*)p->y, p->grad_y, p->grad_skip, (const void*)p->grad_x}) whole &= ((uintptr_t)q & 15) == 0;
     for (uint64_t q : {p->x_stride, p->y_stride, p->grad_y_stride, p->grad_skip_stride, p->grad_x_stride}) whole &= q % V == 0;
-    return whole ? run_norm<T, V>(ctx, p, grad) : run_norm<T, 1>(ctx, p, grad);
+    return whole ? run_norm<T, V, true>(ctx, p, grad) : run_norm<T, V, false>(ctx, p, grad);
 }
 
 int launch_layer_norm(apoe_ctx* ctx, const apoe_layer_norm_args* p, bool grad) {

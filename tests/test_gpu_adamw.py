@@ -229,6 +229,21 @@ def test_zero_gradients_and_moments(gpu_ctx):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
+def test_without_eps(gpu_ctx, bits):
+    """A first step without eps goes by lr against the sign, whatever the gradient's size: v of the smallest, 1e-17, is 1e-37, where floats have all their bits
+    (a step: eight roundings)."""
+    import torch
+    import apoe
+    g = torch.tensor([1e-17, -1e-17, 1e-10, 1.0, -1e4], device="cuda")
+    p = torch.zeros(5, device="cuda")
+    if bits == 8:  # a block each: one that shares a block with far larger ones has a code of one, but the step is taken before that
+        g, p = g.repeat_interleave(256), p.repeat_interleave(256)
+    opt = apoe.AdamW(gpu_ctx, [p], bits=bits, eps=0.0, weight_decay=0.0)
+    opt.step([g], 0.5)
+    assert bool(((p + 0.5 * g.sign()).abs() <= 10 * E * 0.5).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
 def test_captured(bits):
     """A captured step reads its number and rate when it is replayed."""
     import torch
