@@ -28,7 +28,8 @@ struct LinTile {
     const void *a, *b;      // 16-bit values, or planes of such
     uint64_t a_low, b_low;  // from plane to plane
     uint32_t a_pitch, b_pitch; // bytes
-    uint32_t k, nt;         // inner side, tiles along a row of tiles
+    uint32_t k, mt, nt;     // inner side, tiles down and along
+    uint32_t band;          // rows of tiles that are walked through together, column by column
     uint32_t cuts, cut_stages;
     float* part;            // [cuts][m][np]
     uint32_t np;
@@ -212,7 +213,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG, WM * WN * KG == 4 && P == 3 ? 1 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / (WM * WN), wm = wave % (WM * WN) / WN, wn = wave % WN;
     const uint32_t m = a.o.m, n = a.o.n;
     const uint32_t id = xcd_run(blockIdx.x, gridDim.x), tile = id / a.cuts, cut = id % a.cuts;
-    const uint32_t row = tile / a.nt * BM, col = tile % a.nt * BN;
+    // an XCD's run of tiles is about as high as it is wide: it reads the fewest rows of both sides into its L2
+    const uint32_t band = tile / (a.band * a.nt), in_band = tile % (a.band * a.nt), high = min(a.band, a.mt - band * a.band);
+    const uint32_t row = (band * a.band + in_band % high) * BM, col = in_band / high * BN;
     const uint32_t s0 = cut * a.cut_stages, stages = min(a.cut_stages, (a.k + KE - 1) / KE - s0);
     const int mrows = (int)min((uint32_t)BM, m - row), ncols = (int)min((uint32_t)BN, n - col);
     ATile ta[P];
@@ -549,8 +552,11 @@ static uint64_t cut_bytes(const LinShape& s, uint32_t m, uint32_t n) { return s.
 
 template <typename S, typename T, int P, bool ACOL, bool BCOL>
 static void product(apoe_ctx* ctx, const LinShape& s, LinOperand a, LinOperand b, uint32_t k, float* part, const LinOut& o) {
-    LinTile t{a.p, b.p, a.low, b.low, a.pitch, b.pitch, k, (o.n + s.bn - 1) / s.bn, s.cuts, s.cut_stages, part, pitch_of(o.n), o};
-    const uint32_t grid = (uint32_t)((uint64_t)((o.m + s.bm - 1) / s.bm) * t.nt * s.cuts);
+    const uint32_t mt = (o.m + s.bm - 1) / s.bm, nt = (o.n + s.bn - 1) / s.bn;
+    uint32_t band = 1; // a power of two, so that runs end where bands do (8192 x 8192 x 4096: 444 us, row by row 482; 8192 x 1024 x 4096 67, 75)
+    while (band * 2 <= mt && (uint64_t)band * band * 32 <= (uint64_t)mt * nt) band *= 2;
+    LinTile t{a.p, b.p, a.low, b.low, a.pitch, b.pitch, k, mt, nt, band, s.cuts, s.cut_stages, part, pitch_of(o.n), o};
+    const uint32_t grid = (uint32_t)((uint64_t)mt * nt * s.cuts);
     hipStream_t st = ctx->stream;
     if constexpr (P == 1) {
         if (s.kind == 0) linear_tile<S, T, P, ACOL, BCOL, 4, 2, 2, 4, 1, 4, 2><<<grid, 512, 0, st>>>(t);
