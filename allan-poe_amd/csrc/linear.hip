@@ -515,7 +515,7 @@ struct LinKind {
     bool two;
     float fixed, inner, alone_fixed, alone_inner;
 };
-constexpr LinKind LIN_KINDS[] = {{256, 256, 64, false, 9.f, .0243f, 0.f, 0.f}, {256, 128, 64, false, 6.5f, .0142f, 0.f, 0.f}, {128, 128, 64, true, 5.4f, .0165f, .4f, .0115f},
+constexpr LinKind LIN_KINDS[] = {{256, 256, 64, false, 9.f, .0243f, 0.f, 0.f}, {256, 128, 64, false, 6.5f, .0142f, 0.f, 0.f}, {128, 128, 64, true, 5.4f, .0165f, 2.5f, .0103f},
                                  {128, 128, 64, false, 3.f, .0082f, 0.f, 0.f}, {64, 64, 64, true, 1.f, .0055f, 1.f, .0033f}};
 constexpr LinKind LIN_KINDS_SPLIT[] = {{128, 128, 32, false, 8.f, .0421f, 0.f, 0.f}, {64, 64, 64, false, 1.5f, .0165f, 0.f, 0.f}};
 

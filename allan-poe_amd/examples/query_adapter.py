@@ -1,6 +1,6 @@
 """Fits a query adapter to a stored index: the encoder of the queries has changed, the documents and their graph stay.
 
-    python allan-poe_amd/examples/query_adapter.py [--docs 20000] [--train 32768] [--steps 300] [--batch 512]
+    python allan-poe_amd/examples/query_adapter.py [--docs 20000] [--train 32768] [--steps 300] [--batch 512] [--block mlp]
 
 The corpus is the synthetic one whose dense rows have neighbours. The "new encoder" gives vectors that lean away from the
 documents' space (a fixed rotation mixed in), so a search with them misses most of what is relevant. What is known is a set of
@@ -11,6 +11,13 @@ judgements, rows that are relevant to each training query. The adapter is one re
 and it learns from the softmax cross entropy of q over every document: `apoe.gated_residual` (and its gradient) is the frame,
 `apoe.softmax_loss` the loss over the corpus' half-precision rows, and the matrix W takes steps that `apoe.orthogonalize` makes
 from its momentum. Nothing of the index is built again; the same graph is searched before and after. Prints one line of JSON.
+
+With --block mlp the adapter is a layer of the kind that encoders have, and reads the query's learned-sparse terms too:
+
+    e = x + s sum_t val_t E[t],  n = layer_norm(e),  y = e + W2 gelu(W1 n + b1) + b2,  q = y / |y|
+
+through `apoe.embed`, `apoe.layer_norm` and `apoe.linear` and their gradients; all of it, the table of the terms among it, takes its steps from
+`apoe.AdamW` (--bits 8: with moments in 8 bits), which writes the half-precision copies that the next step multiplies with.
 """
 import argparse
 import json
@@ -74,6 +81,73 @@ class QueryAdapter:
         return out["loss"]
 
 
+class MlpAdapter:
+    """The layer's parameters (float32 masters and copies in `dtype` that the products take), its map and one training step. `terms` is the CSR
+    of the queries' learned-sparse terms: offsets, term ids, weights."""
+
+    LOSS_SCALE = 1024.0  # gradients travel as float16
+    SCALE = 0.1          # of the terms' sum
+
+    def __init__(self, ctx, dim=DIM, hidden=2 * DIM, vocab=S.VOCAB, dtype=torch.float16, bits=32, seed=0):
+        g = torch.Generator().manual_seed(seed)
+        dev = f"cuda:{ctx.device}"
+        self.ctx, self.dtype = ctx, dtype
+        rand = lambda *shape: torch.randn(*shape, generator=g).to(dev)  # noqa: E731
+        self.params = dict(E=torch.zeros(vocab, dim, device=dev), w=torch.ones(dim, device=dev), b=torch.zeros(dim, device=dev), W1=rand(hidden, dim) / dim ** 0.5,
+                           b1=torch.zeros(hidden, device=dev), W2=0.02 * rand(dim, hidden) / hidden ** 0.5, b2=torch.zeros(dim, device=dev))
+        matrices = ("E", "W1", "W2")
+        self.copies = {k: self.params[k].to(dtype) for k in matrices}
+        self.unit = torch.full((dim,), 1 / dim ** 0.5, device=dev)
+        in_type = {k: v for k, v in self.copies.items() if dtype != torch.float32}  # float32: the products take the masters themselves
+        self.opt = apoe.AdamW(ctx, list(self.params.values()), copies=[in_type.get(k) for k in self.params], bits=bits,
+                              weight_decay=[0.01 if k in matrices else 0.0 for k in self.params], seed=seed)
+
+    def _matrix(self, name):
+        return self.params[name] if self.dtype == torch.float32 else self.copies[name]
+
+    def _layer(self, x, terms):
+        off, idx, val = terms
+        e = apoe.embed(self.ctx, self._matrix("E"), idx, off, val, scale=self.SCALE, base=x)
+        n = apoe.layer_norm(self.ctx, e, self.params["w"], self.params["b"])
+        h, pre = apoe.linear(self.ctx, n, self._matrix("W1"), self.params["b1"], act="gelu", want_pre=True)
+        y, _ = apoe.linear(self.ctx, h, self._matrix("W2"), self.params["b2"], residual=e)
+        return e, n, h, pre, y
+
+    def __call__(self, x, terms):
+        """Adapted queries of unit length [m, dim]."""
+        return apoe.gated_residual(self.ctx, self._layer(x, terms)[-1], w_next=self.unit, eps=1e-12)[1]
+
+    def gradients(self, x, terms, rows, t_off, t_idx, temperature):
+        """(losses [m], gradients of LOSS_SCALE times their mean by every parameter)."""
+        e, n, h, pre, y = self._layer(x, terms)
+        off, idx, val = terms
+        q = apoe.gated_residual(self.ctx, y, w_next=self.unit, eps=1e-12)[1]
+        weight = torch.full((x.shape[0],), self.LOSS_SCALE / x.shape[0], device=x.device)
+        out = apoe.softmax_loss(self.ctx, q, rows, t_off, t_idx, scale=1 / temperature, weight=weight, grad_queries=True)
+        gy = apoe.gated_residual_grad(self.ctx, y, w_next=self.unit, eps=1e-12, grad_u=out["grad_queries"])["grad_x"]
+        two = apoe.linear_grad(self.ctx, h, self._matrix("W2"), gy)
+        one = apoe.linear_grad(self.ctx, n, self._matrix("W1"), two["grad_x"], act="gelu", pre=pre)
+        norm = apoe.layer_norm_grad(self.ctx, e, self.params["w"], self.params["b"], grad_y=one["grad_x"], grad_skip=gy)  # y = e + ..: past the layer
+        table = apoe.embed_grad(self.ctx, self._matrix("E"), norm["grad_x"], idx, off, val, scale=self.SCALE)["grad_table"]
+        return out["loss"], dict(E=table, w=norm["grad_w"], b=norm["grad_b"], W1=one["grad_w"], b1=one["grad_bias"], W2=two["grad_w"], b2=two["grad_bias"])
+
+    def step(self, x, terms, rows, t_off, t_idx, temperature, lr):
+        loss, grads = self.gradients(x, terms, rows, t_off, t_idx, temperature)
+        self.opt.step([grads[k] for k in self.params], lr, grad_scale=1 / self.LOSS_SCALE)
+        return loss
+
+
+def rows_of(csr, at):
+    """The CSR of the rows `at`."""
+    off, idx, val = csr
+    off = off.long()
+    count = off[at + 1] - off[at]
+    new = torch.zeros(len(at) + 1, dtype=torch.long, device=idx.device)
+    new[1:] = count.cumsum(0)
+    entries = torch.arange(int(new[-1]), device=idx.device) + torch.repeat_interleave(off[at] - new[:-1], count)
+    return new.to(torch.int32), idx[entries], val[entries]
+
+
 def judgements(queries, dense, k):
     """CSR of the k rows closest to each query (what people or logs would say)."""
     idx = (queries @ dense.T).topk(k, dim=1).indices.to(torch.int32)
@@ -97,10 +171,15 @@ def main(argv=None):
     p.add_argument("--held-out", type=int, default=512)
     p.add_argument("--steps", type=int, default=300)
     p.add_argument("--batch", type=int, default=512)
-    p.add_argument("--lr", type=float, default=0.05)
+    p.add_argument("--block", choices=("gated", "mlp"), default="gated")
+    p.add_argument("--bits", type=int, choices=(8, 32), default=32, help="of the moments of --block mlp")
+    p.add_argument("--lr", type=float, default=None, help="0.05, with --block mlp 0.001")
     p.add_argument("--temperature", type=float, default=0.05)
     p.add_argument("--cands", type=int, default=128)
     args = p.parse_args(argv)
+    mlp = args.block == "mlp"
+    if args.lr is None:
+        args.lr = 0.001 if mlp else 0.05
     dev = "cuda:0"
     ctx = apoe.Context(0, stream=torch.cuda.current_stream())
     rows = S.latent_corpus(args.docs, device=dev)
@@ -108,7 +187,8 @@ def main(argv=None):
     corpus.make_half_rows()
     graph, build_ms = apoe.build_graph(ctx, corpus, K=64, iters=10, degree=32, join=1)
 
-    old = S.latent_queries(args.train + args.held_out, device=dev)[0]   # what the old encoder said
+    said = S.latent_queries(args.train + args.held_out, device=dev)
+    old, csr = said[0], (said[1].to(torch.int32), said[2].to(torch.int32), said[3])  # what the old encoder said, and the queries' terms
     g = torch.Generator().manual_seed(1)
     turn = torch.linalg.qr(torch.randn(DIM, DIM, generator=g)).Q.to(dev)
     new = old + 1.5 * old @ turn                                        # what the new one says
@@ -118,7 +198,7 @@ def main(argv=None):
     wanted = judgements(old[args.train:], rows[0], 10)[1].view(-1, 10)
 
     before = recall(ctx, corpus, graph, held, sparse, wanted, args.cands)
-    adapter = QueryAdapter(ctx)
+    adapter = MlpAdapter(ctx, bits=args.bits) if mlp else QueryAdapter(ctx)
     losses = []
     torch.cuda.synchronize()
     start = time.perf_counter()
@@ -127,14 +207,18 @@ def main(argv=None):
         idx = t_idx.view(-1, 3)[at].reshape(-1)
         off = torch.arange(0, 3 * args.batch + 1, 3, dtype=torch.int32, device=dev)
         warm = min(1.0, 4.0 * (args.steps - step) / args.steps)         # the last quarter's steps shrink
-        losses.append(adapter.step(new[at], corpus, off, idx, args.temperature, args.lr * warm).mean())
+        if mlp:
+            losses.append(adapter.step(new[at], rows_of(csr, at), corpus, off, idx, args.temperature, args.lr * warm).mean())
+        else:
+            losses.append(adapter.step(new[at], corpus, off, idx, args.temperature, args.lr * warm).mean())
     torch.cuda.synchronize()
     took = time.perf_counter() - start
-    after = recall(ctx, corpus, graph, adapter(held), sparse, wanted, args.cands)
+    mapped = adapter(held, rows_of(csr, torch.arange(args.train, args.train + args.held_out, device=dev))) if mlp else adapter(held)
+    after = recall(ctx, corpus, graph, mapped, sparse, wanted, args.cands)
     limit = recall(ctx, corpus, graph, old[args.train:], sparse, wanted, args.cands)
     for part in (graph, corpus, ctx):
         part.close()
-    return dict(docs=args.docs, build_ms=round(build_ms, 1), steps=args.steps, batch=args.batch, ms_per_step=round(1e3 * took / args.steps, 3),
+    return dict(block=args.block, docs=args.docs, build_ms=round(build_ms, 1), steps=args.steps, batch=args.batch, ms_per_step=round(1e3 * took / args.steps, 3),
                 loss_first=round(float(losses[0]), 3), loss_last=round(float(torch.stack(losses[-10:]).mean()), 3),
                 recall_at_10_before=round(before, 4), recall_at_10_after=round(after, 4), recall_at_10_old_encoder=round(limit, 4))
 
