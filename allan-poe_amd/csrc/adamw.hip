@@ -23,6 +23,7 @@ constexpr uint32_t BLOCK = APOE_ADAMW_BLOCK;
 
 using f32x4a = float __attribute__((ext_vector_type(4)));
 using u32x2a = uint32_t __attribute__((ext_vector_type(2)));
+using u32x4a = uint32_t __attribute__((ext_vector_type(4)));
 
 struct AdamTensor {
     float* p;
@@ -81,34 +82,6 @@ __device__ inline double value_of_v(float scale, uint32_t c) {
 
 // Values k of a lane: four in a row, or (parameters that begin anywhere, a block's rest) 64 apart.
 __device__ inline uint32_t place(bool whole, int lane, int k) { return whole ? (uint32_t)lane * 4 + k : (uint32_t)k * 64 + lane; }
-
-__device__ inline void load_grad(float* g, const AdamTensor& t, uint64_t at, bool whole, int lane, uint32_t left) {
-    if (whole) {
-        const uint64_t e = at + lane * 4;
-        if (t.g_type == APOE_F32) {
-            const f32x4a x = *reinterpret_cast<const f32x4a*>((const float*)t.g + e);
-#pragma unroll
-            for (int k = 0; k < 4; k++) g[k] = x[k];
-        } else {
-            const u32x2a x = *reinterpret_cast<const u32x2a*>((const uint16_t*)t.g + e);
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const uint16_t h = (uint16_t)(x[k >> 1] >> (16 * (k & 1)));
-                g[k] = t.g_type == APOE_F16 ? (float)__builtin_bit_cast(_Float16, h) : __builtin_bit_cast(float, (uint32_t)h << 16);
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        const uint32_t i = place(false, lane, k);
-        g[k] = 0.f;
-        if (i >= left) continue;
-        if (t.g_type == APOE_F32) g[k] = ((const float*)t.g)[at + i];
-        else if (t.g_type == APOE_F16) g[k] = (float)((const _Float16*)t.g)[at + i];
-        else g[k] = (float)((const __bf16*)t.g)[at + i];
-    }
-}
 
 template <typename T> __device__ inline void load4(T* x, const T* from, uint64_t at, bool whole, int lane, uint32_t left) {
     typedef T t4 __attribute__((ext_vector_type(4)));
@@ -182,7 +155,63 @@ template <int POWER, int STEPS> __device__ inline int code_of(double x, double i
     return min((int)k + (u * gap < above ? 1 : 0), STEPS);
 }
 
-// NEAR: root and reciprocal to a unit of the last place.
+// What a lane needs of a block, as it comes: nothing here waits for a load.
+template <int BITS> struct AdamRaw {
+    f32x4a p, m, v;
+    u32x4a g;        // floats, or two 16-bit values a word
+    uint32_t cm, cv; // four codes
+    float sm, sv;
+    __device__ void fetch(const AdamTensor& t, uint64_t at, int lane) {
+        const uint32_t left = (uint32_t)min((uint64_t)BLOCK, t.n - at);
+        if (t.whole && left == BLOCK) {
+            const uint64_t e = at + lane * 4;
+            p = *reinterpret_cast<const f32x4a*>(t.p + e);
+            if (t.g_type == APOE_F32) {
+                g = *reinterpret_cast<const u32x4a*>((const float*)t.g + e);
+            } else {
+                const u32x2a x = *reinterpret_cast<const u32x2a*>((const uint16_t*)t.g + e);
+                g[0] = x[0];
+                g[1] = x[1];
+            }
+            if constexpr (BITS == 32) {
+                m = *reinterpret_cast<const f32x4a*>((const float*)t.m + e);
+                v = *reinterpret_cast<const f32x4a*>((const float*)t.v + e);
+            } else {
+                cm = *reinterpret_cast<const uint32_t*>((const int8_t*)t.m + e);
+                cv = *reinterpret_cast<const uint32_t*>((const uint8_t*)t.v + e);
+            }
+        } else {
+            g = u32x4a{};
+            cm = cv = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t i = place(false, lane, k);
+                const bool in = i < left;
+                p[k] = in ? t.p[at + i] : 0.f;
+                if (t.g_type == APOE_F32) g[k] = in ? ((const uint32_t*)t.g)[at + i] : 0u;
+                else g[k >> 1] |= (in ? (uint32_t)((const uint16_t*)t.g)[at + i] : 0u) << (16 * (k & 1));
+                if constexpr (BITS == 32) {
+                    m[k] = in ? ((const float*)t.m)[at + i] : 0.f;
+                    v[k] = in ? ((const float*)t.v)[at + i] : 0.f;
+                } else {
+                    cm |= (in ? (uint32_t)((const uint8_t*)t.m)[at + i] : 0u) << (8 * k);
+                    cv |= (in ? (uint32_t)((const uint8_t*)t.v)[at + i] : 0u) << (8 * k);
+                }
+            }
+        }
+        if constexpr (BITS == 8) {
+            sm = t.ms[at / BLOCK];
+            sv = t.vs[at / BLOCK];
+        }
+    }
+    __device__ float grad(int k, uint32_t type) const {
+        if (type == APOE_F32) return __uint_as_float(g[k]);
+        const uint16_t h = (uint16_t)(g[k >> 1] >> (16 * (k & 1)));
+        return type == APOE_F16 ? (float)__builtin_bit_cast(_Float16, h) : __uint_as_float((uint32_t)h << 16);
+    }
+};
+
+// NEAR: root and reciprocal to a unit of the last place. A block is asked for before the one in front of it is worked on.
 template <int BITS, bool NEAR> __global__ __launch_bounds__(256) void adamw_step(AdamArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t which = 0;
@@ -194,6 +223,9 @@ template <int BITS, bool NEAR> __global__ __launch_bounds__(256) void adamw_step
     }
     const AdamTensor& t = a.t[which];
     const uint64_t begin = (uint64_t)(blockIdx.x - t.first) * ADAM_PIECE, end = min(begin + ADAM_PIECE, t.n);
+    uint64_t at = begin + wave * BLOCK;
+    AdamRaw<BITS> next;
+    if (at < end) next.fetch(t, at, lane);
     float c1 = a.c1, c2 = a.c2, lr = a.lr;
     uint32_t step = a.step;
     if (a.step_dev) {
@@ -203,39 +235,33 @@ template <int BITS, bool NEAR> __global__ __launch_bounds__(256) void adamw_step
     }
     if (a.lr_dev) lr = *a.lr_dev;
     const uint32_t key = mix(mix(mix(a.seed) ^ step) ^ t.index);
-    for (uint64_t at = begin + wave * BLOCK; at < end; at += 4 * BLOCK) {
+    const uint32_t g_type = t.g_type;
+    for (; at < end; at += 4 * BLOCK) {
         const uint32_t left = (uint32_t)min((uint64_t)BLOCK, t.n - at);
         const bool whole = t.whole && left == BLOCK;
-        float p[4], g[4], m[4], v[4];
-        load4(p, t.p, at, whole, lane, left);
-        load_grad(g, t, at, whole, lane, left);
+        const AdamRaw<BITS> now = next;
+        if (at + 4 * BLOCK < end) next.fetch(t, at + 4 * BLOCK, lane);
+        float p[4], m[4], v[4];
         if constexpr (BITS == 32) {
-            load4(m, (const float*)t.m, at, whole, lane, left);
-            load4(v, (const float*)t.v, at, whole, lane, left);
             const float d1 = (float)(1. - a.b1), d2 = (float)(1. - a.b2), gs = (float)a.grad_scale;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const float x = g[k] * gs;
-                m[k] = __builtin_fmaf(d1, x - m[k], m[k]);
-                v[k] = __builtin_fmaf(d2, __builtin_fmaf(x, x, -v[k]), v[k]);
+                const float x = now.grad(k, g_type) * gs;
+                m[k] = __builtin_fmaf(d1, x - now.m[k], now.m[k]);
+                v[k] = __builtin_fmaf(d2, __builtin_fmaf(x, x, -now.v[k]), now.v[k]);
             }
             store4((float*)t.m, m, at, whole, lane, left);
             store4((float*)t.v, v, at, whole, lane, left);
         } else {
             const uint64_t block = at / BLOCK;
-            int8_t cm[4];
-            uint8_t cv[4];
-            load4(cm, (const int8_t*)t.m, at, whole, lane, left);
-            load4(cv, (const uint8_t*)t.v, at, whole, lane, left);
-            const float sm = t.ms[block], sv = t.vs[block];
             double md[4], vd[4];
             uint32_t mb = 0, vb = 0; // the largest, by magnitude; a value beyond the parameter's end is zero
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const bool in = place(whole, lane, k) < left;
-                const double x = (double)g[k] * a.grad_scale;
-                md[k] = in ? moved(value_of_m(sm, cm[k]), x, 1. - a.b1) : 0.;
-                vd[k] = in ? moved(value_of_v(sv, cv[k]), x * x, 1. - a.b2) : 0.;
+                const bool in = whole || place(false, lane, k) < left;
+                const double x = (double)now.grad(k, g_type) * a.grad_scale;
+                md[k] = in ? moved(value_of_m(now.sm, (int8_t)(now.cm >> (8 * k))), x, 1. - a.b1) : 0.;
+                vd[k] = in ? moved(value_of_v(now.sv, (uint8_t)(now.cv >> (8 * k))), x * x, 1. - a.b2) : 0.;
                 m[k] = (float)md[k];
                 v[k] = (float)vd[k];
                 mb = max(mb, __float_as_uint(m[k]) & 0x7fffffffu);
@@ -244,6 +270,8 @@ template <int BITS, bool NEAR> __global__ __launch_bounds__(256) void adamw_step
             const float mt = wave_largest(mb), vt = wave_largest(vb);
             const double im = share_of(127. * 127., mt), iv = share_of(255. * 255. * 255. * 255., vt);
             const uint32_t bk = mix(mix(key ^ (uint32_t)block) ^ (uint32_t)(block >> 32));
+            int8_t cm[4];
+            uint8_t cv[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const uint32_t i = place(whole, lane, k);
@@ -259,10 +287,10 @@ template <int BITS, bool NEAR> __global__ __launch_bounds__(256) void adamw_step
             }
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < 4; k++) {
             m[k] = NEAR ? m[k] * c1 * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[k] * c2) + a.eps) : m[k] * c1 / (sqrtf(v[k] * c2) + a.eps);
-#pragma unroll
-        for (int k = 0; k < 4; k++) p[k] = __builtin_fmaf(-lr, __builtin_fmaf(t.decay, p[k], m[k]), p[k]);
+            p[k] = __builtin_fmaf(-lr, __builtin_fmaf(t.decay, now.p[k], m[k]), now.p[k]);
+        }
         store4(t.p, p, at, whole, lane, left);
         if (t.copy) {
             if (t.copy_type == APOE_F16) {
