@@ -1002,6 +1002,8 @@ class AdamW:
         """One step with the parameters' gradients (None: that parameter and its moments stay as they are), which count times grad_scale. lr may be a
         float32 tensor of one number on the GPU, and t, the number of the step, an int32 one: a captured step reads both when it
         is replayed (the program counts t up; without it the object counts)."""
+        if not (self.h and self.ctx.h):
+            raise ApoeError("the object or its context has been closed")
         if len(grads) != len(self.params):
             raise ApoeError(f"{len(grads)} gradients for {len(self.params)} parameters")
         a = AdamwStepArgs()

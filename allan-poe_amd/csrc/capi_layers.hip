@@ -183,7 +183,7 @@ int fill_adamw(apoe_adamw* opt, uint32_t count, const apoe_adamw_tensor* tensors
     apoe_ctx* ctx = opt->ctx;
     opt->tensors.assign(tensors, tensors + count);
     for (apoe_adamw_tensor& t : opt->tensors) {
-        APOE_REQUIRE(t.n < (1ull << 40), "a parameter of %llu values is beyond 2^40", (unsigned long long)t.n);
+        APOE_REQUIRE(t.n < (1ull << 35), "a parameter of %llu values is beyond 2^35", (unsigned long long)t.n);
         APOE_REQUIRE(std::isfinite(t.decay), "decay must be finite");
         if (t.n == 0) continue;
         APOE_REQUIRE(t.p && t.m && t.v, "p/m/v is null");

@@ -526,6 +526,7 @@ template <int P> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t n, u
     const auto look = [&](const LinKind& kind, uint32_t number) {
         const uint64_t tiles = (uint64_t)((m + kind.bm - 1) / kind.bm) * ((n + kind.bn - 1) / kind.bn);
         const uint32_t stages = (k + kind.ke - 1) / kind.ke;
+        if (number && tiles > (1u << 22)) return; // more than a launch takes
         for (uint32_t cuts = 1; cuts <= 16 && (cuts == 1 || (stages / cuts >= 4 && tiles * cuts <= 2 * cus)); cuts++) {
             const uint32_t each = std::max(1u, (stages + cuts - 1) / cuts);
             const uint64_t groups = tiles * cuts, at_once = kind.two ? 2 * cus : cus;

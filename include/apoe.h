@@ -451,7 +451,8 @@ typedef struct {
 
 /*
  * y = w (x - mean x) / sqrt(var x + eps) + b, row by row, with the variance of the row's values about their mean. The gradient is formed
- * from x alone: nothing is kept from the forward call. grad_x = grad_skip + what comes through the norm.
+ * from x alone: nothing is kept from the forward call. grad_x = grad_skip + what comes through the norm. Squares and sums of a row are
+ * floats: its values are to stay below 1e19.
  */
 int apoe_layer_norm(apoe_ctx* ctx, const apoe_layer_norm_args* args);
 int apoe_layer_norm_grad(apoe_ctx* ctx, const apoe_layer_norm_args* args);
@@ -490,7 +491,7 @@ int apoe_linear_grad(apoe_ctx* ctx, const apoe_linear_args* args);
 #define APOE_ADAMW_BLOCK 256u /* values of a parameter that share the scale of their 8-bit moments */
 
 typedef struct {
-    float* p;                    /* [n], any n */
+    float* p;                    /* [n], n below 2^35 */
     void *m, *v;                 /* bits 32: float [n]; bits 8: int8_t [n] and uint8_t [n] */
     float *m_scale, *v_scale;    /* bits 8: [(n + 255) / 256], the largest |m| and v of each block; bits 32: NULL */
     void* copy;                  /* p once more, rounded to copy_dtype (APOE_F16, APOE_BF16), or NULL */

@@ -276,3 +276,28 @@ def test_captured(bits):
     assert not bool((params[0] == start[0]).all())
     del graph
     ctx.close()
+
+
+def test_closed(gpu_ctx):
+    import torch
+    import apoe
+    p = torch.zeros(10, device="cuda")
+    ctx = apoe.Context(0)
+    a, b = apoe.AdamW(ctx, [p]), apoe.AdamW(ctx, [p])
+    a.close()
+    for opt in (a, b):
+        if opt is b:
+            ctx.close()
+        with pytest.raises(apoe.ApoeError, match="closed"):
+            opt.step([p], LR)
+
+
+def test_arrays_that_share_memory_are_refused(gpu_ctx):
+    import torch
+    import apoe
+    store = torch.zeros(2000, device="cuda")
+    half = torch.zeros(1000, dtype=torch.float16, device="cuda")
+    for params, copies in (([store[:600], store[500:]], None), ([store[:600]] * 2, None), ([store[:1000], store[1000:]], [half, half]), ([store], [store.view(torch.float16)[:2000]])):
+        with pytest.raises(apoe.ApoeError, match="share memory"):
+            apoe.AdamW(gpu_ctx, params, copies=copies)
+    apoe.AdamW(gpu_ctx, [store[:600], store[600:]])

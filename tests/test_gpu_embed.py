@@ -229,3 +229,43 @@ def test_queries_of_the_index_as_they_are_stored(gpu_ctx, small_world):
     table = matrix(g, int(s_idx.max()) + 1, 128, "float16")
     want, tol = formula(table, s_idx, s_off, s_val, 0.1, "float16")
     close(apoe.embed(gpu_ctx, table, s_idx, s_off, s_val, 0.1), want["out"], tol["out"])
+
+
+@pytest.mark.parametrize("n,n_table", [((1 << 20) + 4321, 1000), (70_000, (1 << 25) + 5)])
+def test_many_entries_and_many_rows(gpu_ctx, n, n_table):
+    """More entries than the sort's workgroups rank at a time, and names of 26 bits (four passes): numbers small enough that every sum is exact."""
+    import torch
+    import apoe
+    g = torch.Generator(device="cuda").manual_seed(9)
+    idx = torch.randint(0, n_table, (n,), generator=g, device="cuda")
+    idx[: n // 3] %= 40
+    grad = torch.randint(-3, 4, (n, 8), generator=g, device="cuda").to(torch.float32)
+    table = torch.zeros(n_table, 8, device="cuda")
+    want = torch.zeros(n_table, 8, device="cuda").index_add_(0, idx, grad)  # whole numbers below 2^24, in any order
+    got = apoe.embed_grad(gpu_ctx, table, grad, idx.to(torch.int32))["grad_table"]
+    assert bool((got == want).all())
+
+
+def test_matrices_past_four_gigabytes(gpu_ctx):
+    import torch
+    import apoe
+    g = torch.Generator().manual_seed(10)
+    n, t, d, gap = 300, 40, 136, (1 << 31) // 39 + 5
+
+    def far(m, gap):
+        store = torch.empty((m.shape[0] - 1) * gap + m.shape[1], dtype=m.dtype, device="cuda")
+        v = store.as_strided(m.shape, (gap, 1))
+        v.copy_(m)
+        assert m.shape[0] * gap * m.element_size() > 1 << 32
+        return v
+    table, grad, base = matrix(g, t, d, "float16"), matrix(g, n, d, "float16"), matrix(g, n, d, "float16")
+    off, idx, val = entries(g, [4] * n, t)
+    wide = far(table, gap)
+    near = apoe.embed(gpu_ctx, table, idx, off, val, base=base)
+    away = far(torch.zeros_like(base), (1 << 31) // 299 + 3)
+    assert bool((apoe.embed(gpu_ctx, wide, idx, off, val, base=far(base, (1 << 31) // 299 + 1), out=away) == near).all())
+    near = apoe.embed_grad(gpu_ctx, table, grad, idx, off, val, grad_val=True)
+    wide_grad = far(torch.zeros_like(table), gap + 2)
+    got = apoe.embed_grad(gpu_ctx, wide, far(grad, (1 << 31) // 299 + 7), idx, off, val, grad_table=wide_grad, grad_val=True)
+    for k in near:
+        assert bool(((got[k] - near[k]).abs() <= 2.0 ** -10 * near[k].abs() + 2.0 ** -24).all()), k  # rows that begin elsewhere are added up by other threads

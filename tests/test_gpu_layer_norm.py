@@ -192,3 +192,19 @@ def test_captured():
         for k in want:
             assert bool((got[k] == want[k]).all()), k
     ctx.close()
+
+
+def test_matrices_past_four_gigabytes(gpu_ctx):
+    import torch
+    import apoe
+    g = torch.Generator().manual_seed(12)
+    n, d, gap = 5000, 200, 1 << 19
+    x, gy = matrix(g, n, d, "float16"), matrix(g, n, d, "float16")
+    w, b = vectors(g, d)
+    store = torch.empty((n - 1) * gap + d, dtype=torch.float16, device="cuda")
+    far = store.as_strided((n, d), (gap, 1))
+    far.copy_(x)
+    assert bool((apoe.layer_norm(gpu_ctx, far, w, b) == apoe.layer_norm(gpu_ctx, x, w, b)).all())
+    near, away = (apoe.layer_norm_grad(gpu_ctx, t, w, b, grad_y=gy) for t in (x, far))
+    for k in near:
+        assert bool((near[k] == away[k]).all()), k
