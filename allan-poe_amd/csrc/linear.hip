@@ -2,9 +2,9 @@
 //   z = x w^T + b, y = act(z) + residual;   gz = gy act'(z), gx = gz w, gw = gz^T x, gb = sum of gz's rows.
 //
 // Three products of one kernel: an operand's inner dimension goes along its rows (x, w, and gz for gx) or down them (w for gx, both for gw; read
-// transposed from LDS). 16-bit matrices are taken as they lie; float ones as three bfloat16 planes that hold their 24 bits exactly, six products
-// of which (those above 2^-24) are added up: as accurate value by value as float products, whatever the exponents are, at 1381 / 6 = 230
-// TFLOP/s where the float matrix units have 154. What is done to a result (bias, activation, residual, rounding) is done behind the last stage,
+// transposed from LDS). Float matrices go through the bfloat16 units: a wave takes each value of its operands apart into three parts of eight bits as it comes from LDS, and of
+// the nine products the six that count are added up: as accurate value by value as float products, whatever the exponents are, at a sixth of
+// 1400 TFLOP/s where the float matrix units have 154. What is done to a result (bias, activation, residual, rounding) is done behind the last stage,
 // through LDS, 16 bytes a thread. Where tiles are too few for the GPU the inner dimension is cut and a second launch adds the cuts up, in order.
 // Up to 64 rows a kernel of its own streams w once (the serving form).
 #include <algorithm>
@@ -25,8 +25,7 @@ struct LinOut { // what becomes of a product's sums
 };
 
 struct LinTile {
-    const void *a, *b;      // 16-bit values, or planes of such
-    uint64_t a_low, b_low;  // from plane to plane
+    const void *a, *b;
     uint32_t a_pitch, b_pitch; // bytes
     uint32_t k, mt, nt;     // inner side, tiles down and along
     uint32_t band;          // rows of tiles that are walked through together, column by column
@@ -165,29 +164,40 @@ template <typename T> __device__ inline void finish1(const LinOut& o, uint32_t i
     ((T*)o.out)[i * o.out_stride + j] = (T)z;
 }
 
+// (ADD: groups of waves hold parts of every sum; otherwise each group has whole ones of its share of the blocks.)
 // What the waves hold goes out: one block of 32 rows a wave at a time through LDS, then a thread has eight values of a row. Waits between are for LDS alone: the
 // stores of the block before are on their way meanwhile.
-template <typename T, int MT, int NT, int WM, int WN, int KG, int BYTES>
+template <typename T, int MT, int NT, int WM, int WN, int KG, int BYTES, bool ADD = false>
 __device__ inline void tile_out(const LinTile& a, f32x16 (&acc)[MT][NT], char* lds, uint32_t row, uint32_t col, uint32_t cut, int kg, int wm, int wn, int lane) {
-    constexpr int NW = WM * WN * KG, BN = WN * NT * 32, PITCH = BN + 4, ROWS = WM * 32, ITEMS = ROWS * BN / 8 / (64 * NW);
-    static_assert(ROWS * PITCH * 4 <= BYTES && ROWS * BN % (512 * NW) == 0, "the sums fit the stages");
+    constexpr int NW = WM * WN * KG, BN = WN * NT * 32, PITCH = BN + 4, ROWS = WM * 32, ITEMS = (ROWS * BN / 8 + 64 * NW - 1) / (64 * NW);
+    static_assert(ROWS * PITCH * 4 <= BYTES, "the sums fit the stages");
     const uint32_t m = a.o.m, n = a.o.n;
     float* sum = reinterpret_cast<float*>(lds);
     const int half = lane >> 5;
 #pragma unroll
     for (int i = 0; i < MT; i++) {
-        if (KG == 1 || i / (MT / KG) == kg) {
+        const auto each = [&](auto&& use) {
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int k = 0; k < 16; k++) sum[(wm * 32 + result_row(k, half)) * PITCH + (wn * NT + t) * 32 + (lane & 31)] = acc[i][t][k];
+                for (int k = 0; k < 16; k++) use(sum[(wm * 32 + result_row(k, half)) * PITCH + (wn * NT + t) * 32 + (lane & 31)], acc[i][t][k]);
+        };
+        if constexpr (ADD) {
+#pragma unroll
+            for (int g = KG - 1; g > 0; g--) {
+                if (kg == g) each([&](float& at, float v) { at = g == KG - 1 ? v : at + v; });
+                tile_wait<63>();
+            }
+            if (kg == 0) each([](float& at, float v) { at += v; });
+        } else if (KG == 1 || i / (MT / KG) == kg) {
+            each([](float& at, float v) { at = v; });
         }
         tile_wait<63>();
 #pragma unroll 1
         for (int item = 0; item < ITEMS; item++) {
             const uint32_t at = item * 64 * NW + threadIdx.x, r = at / (BN / 8), c = at % (BN / 8) * 8;
             const uint32_t gi = row + (r / 32 * MT + i) * 32 + r % 32, gj = col + c;
-            if (gi >= m || gj >= n) continue;
+            if (r >= ROWS || gi >= m || gj >= n) continue;
             const f32x4 v0 = *reinterpret_cast<const f32x4*>(sum + r * PITCH + c), v1 = *reinterpret_cast<const f32x4*>(sum + r * PITCH + c + 4);
             if (a.cuts > 1) {
                 float* to = a.part + ((uint64_t)cut * m + gi) * a.np + gj;
@@ -202,13 +212,13 @@ __device__ inline void tile_out(const LinTile& a, f32x16 (&acc)[MT][NT], char* l
     }
 }
 
-// S: the operands' type, P planes of it; T: the results'. ACOL, BCOL: the inner dimension goes down the rows.
-template <typename S, typename T, int P, bool ACOL, bool BCOL, int MT, int NT, int WM, int WN, int KG, int SF, int ST>
-__global__ __launch_bounds__(64 * WM * WN * KG, WM * WN * KG == 4 && P == 3 ? 1 : 2) void linear_tile(LinTile a) {
+// 16-bit matrices. ACOL, BCOL: the inner dimension goes down the rows.
+template <typename T, bool ACOL, bool BCOL, int MT, int NT, int WM, int WN, int KG, int SF, int ST>
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_tile(LinTile a) {
     constexpr int NW = WM * WN * KG, FS = SF / KG, BM = WM * MT * 32, BN = WN * NT * 32;
-    using ATile = std::conditional_t<ACOL, ColTile<S, BM, SF, NW, ORDER_ROWS>, RowTile<S, BM, SF, NW>>;
-    using BTile = std::conditional_t<BCOL, ColTile<S, BN, SF, NW, ORDER_ROWS>, RowTile<S, BN, SF, NW>>;
-    constexpr int PLANE = ATile::BYTES + BTile::BYTES, STAGE = P * PLANE, PER = P * (ATile::LOADS + BTile::LOADS), KE = ATile::KE;
+    using ATile = std::conditional_t<ACOL, ColTile<T, BM, SF, NW, ORDER_ROWS>, RowTile<T, BM, SF, NW>>;
+    using BTile = std::conditional_t<BCOL, ColTile<T, BN, SF, NW, ORDER_ROWS>, RowTile<T, BN, SF, NW>>;
+    constexpr int STAGE = ATile::BYTES + BTile::BYTES, PER = ATile::LOADS + BTile::LOADS, KE = ATile::KE;
     __shared__ __align__(1024) char lds[ST * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / (WM * WN), wm = wave % (WM * WN) / WN, wn = wave % WN;
     const uint32_t m = a.o.m, n = a.o.n;
@@ -218,17 +228,13 @@ __global__ __launch_bounds__(64 * WM * WN * KG, WM * WN * KG == 4 && P == 3 ? 1 
     const uint32_t row = (band * a.band + in_band % high) * BM, col = in_band / high * BN;
     const uint32_t s0 = cut * a.cut_stages, stages = min(a.cut_stages, (a.k + KE - 1) / KE - s0);
     const int mrows = (int)min((uint32_t)BM, m - row), ncols = (int)min((uint32_t)BN, n - col);
-    ATile ta[P];
-    BTile tb[P];
-#pragma unroll
-    for (int p = 0; p < P; p++) {
-        const char* pa = (const char*)a.a + p * a.a_low * sizeof(S);
-        const char* pb = (const char*)a.b + p * a.b_low * sizeof(S);
-        if constexpr (ACOL) ta[p].init((const S*)(pa + (uint64_t)s0 * KE * a.a_pitch) + row, a.a_pitch, (mrows + 7) / 8 * 8, wave, lane);
-        else ta[p].init((const S*)(pa + (uint64_t)row * a.a_pitch) + (uint64_t)s0 * KE, a.a_pitch, mrows, wave, lane);
-        if constexpr (BCOL) tb[p].init((const S*)(pb + (uint64_t)s0 * KE * a.b_pitch) + col, a.b_pitch, (ncols + 7) / 8 * 8, wave, lane);
-        else tb[p].init((const S*)(pb + (uint64_t)col * a.b_pitch) + (uint64_t)s0 * KE, a.b_pitch, ncols, wave, lane);
-    }
+    ATile ta;
+    BTile tb;
+    const char *pa = (const char*)a.a, *pb = (const char*)a.b;
+    if constexpr (ACOL) ta.init((const T*)(pa + (uint64_t)s0 * KE * a.a_pitch) + row, a.a_pitch, (mrows + 7) / 8 * 8, wave, lane);
+    else ta.init((const T*)(pa + (uint64_t)row * a.a_pitch) + (uint64_t)s0 * KE, a.a_pitch, mrows, wave, lane);
+    if constexpr (BCOL) tb.init((const T*)(pb + (uint64_t)s0 * KE * a.b_pitch) + col, a.b_pitch, (ncols + 7) / 8 * 8, wave, lane);
+    else tb.init((const T*)(pb + (uint64_t)col * a.b_pitch) + (uint64_t)s0 * KE, a.b_pitch, ncols, wave, lane);
     const uint32_t base = lds_address(lds);
     int left = (int)min(stages * KE, a.k - s0 * KE); // of the inner side; a row's values are followed by zeros up to a multiple of eight
     uint32_t into = 0;
@@ -242,11 +248,8 @@ __global__ __launch_bounds__(64 * WM * WN * KG, WM * WN * KG == 4 && P == 3 ? 1 
             }
             t.next();
         };
-#pragma unroll
-        for (int p = 0; p < P; p++) {
-            one(ta[p], base + into + p * PLANE, std::integral_constant<bool, ACOL>{});
-            one(tb[p], base + into + p * PLANE + ATile::BYTES, std::integral_constant<bool, BCOL>{});
-        }
+        one(ta, base + into, std::integral_constant<bool, ACOL>{});
+        one(tb, base + into + ATile::BYTES, std::integral_constant<bool, BCOL>{});
         left -= KE;
         into = into + STAGE == ST * STAGE ? 0 : into + STAGE;
     };
@@ -258,15 +261,12 @@ __global__ __launch_bounds__(64 * WM * WN * KG, WM * WN * KG == 4 && P == 3 ? 1 
         tile_wait<(ST - 2) * PER>();
         const char* A = lds + from;
         const char* B = A + ATile::BYTES;
-        i32x4 x[2][P][MT], y[2][P][NT];
+        i32x4 x[2][MT], y[2][NT];
         auto read = [&](int f) {
 #pragma unroll
-            for (int p = 0; p < P; p++) {
+            for (int i = 0; i < MT; i++) x[f & 1][i] = ATile::read(A, wm * MT + i, kg * FS + f, lane);
 #pragma unroll
-                for (int i = 0; i < MT; i++) x[f & 1][p][i] = ATile::read(A + p * PLANE, wm * MT + i, kg * FS + f, lane);
-#pragma unroll
-                for (int t = 0; t < NT; t++) y[f & 1][p][t] = BTile::read(B + p * PLANE, wn * NT + t, kg * FS + f, lane);
-            }
+            for (int t = 0; t < NT; t++) y[f & 1][t] = BTile::read(B, wn * NT + t, kg * FS + f, lane);
         };
         read(0);
         issue();
@@ -276,13 +276,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG, WM * WN * KG == 4 && P == 3 ? 1 
 #pragma unroll
             for (int i = 0; i < MT; i++)
 #pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int total = P - 1; total >= 0; total--) // the smaller products first
-#pragma unroll
-                        for (int p = 0; p <= total; p++) acc[i][t] = mfma_step<S>(x[f & 1][p][i], y[f & 1][total - p][t], acc[i][t]);
+                for (int t = 0; t < NT; t++) acc[i][t] = mfma_step<T>(x[f & 1][i], y[f & 1][t], acc[i][t]);
         }
-        interleave<P * ((ACOL ? 2 : 1) * MT + (BCOL ? 2 : 1) * NT), P * (P + 1) / 2 * MT * NT, FS>();
+        interleave<(ACOL ? 2 : 1) * MT + (BCOL ? 2 : 1) * NT, MT * NT, FS>();
         from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
     }
     tile_wait<0>();
@@ -292,6 +288,167 @@ __global__ __launch_bounds__(64 * WM * WN * KG, WM * WN * KG == 4 && P == 3 ? 1 
         __syncthreads();
     }
     tile_out<T, MT, NT, WM, WN, KG, ST * STAGE>(a, acc, lds, row, col, cut, kg, wm, wn, lane);
+}
+
+// ---- float matrices ----
+
+// Eight floats as three parts of eight bits that add up to them exactly: the leading bits as they are, then what each part leaves, rounded to the next.
+struct Parts {
+    bf16x8 p[3];
+};
+__device__ inline Parts split8(f32x4 lo, f32x4 hi) {
+    Parts s;
+    i32x4 top;
+    float rest[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const float v = k < 4 ? lo[k] : hi[k - 4];
+        rest[k] = v - __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t a = __float_as_uint(k < 2 ? lo[2 * k] : hi[2 * k - 4]), b = __float_as_uint(k < 2 ? lo[2 * k + 1] : hi[2 * k - 3]);
+        top[k] = (int)__builtin_amdgcn_perm(b, a, 0x07060302u); // the upper halves
+    }
+    s.p[0] = __builtin_bit_cast(bf16x8, top);
+#pragma unroll
+    for (int k = 0; k < 8; k++) s.p[1][k] = (__bf16)rest[k];
+#pragma unroll
+    for (int k = 0; k < 8; k++) s.p[2][k] = (__bf16)(rest[k] - (float)s.p[1][k]);
+    return s;
+}
+
+// What a lane gets of sixteen inner indices is 4 h + 0..3 and 8 + 4 h + 0..3 for its half h: the same on both sides. Rows begin at multiples of 16 bytes, and a row's
+// values are followed by zeros up to one.
+template <int ROWS, int NW, int KE> struct RowTile32 { // inner index along the rows; a row's 16-byte pieces lie at places that its number turns
+    static constexpr int BYTES = ROWS * KE * 4, LOADS = BYTES / (1024 * NW);
+    static_assert(BYTES % (1024 * NW) == 0, "whole loads");
+    uint32_t offset[LOADS], at[LOADS]; // at: byte in a row's stage
+    uint64_t base;
+    __device__ static int turn(int row) { return KE == 64 ? row & 15 : (row >> 1) & 7; }
+    __device__ void init(const float* row0, uint32_t pitch_bytes, int rows, int wave, int lane) {
+        base = uniform64((uint64_t)row0);
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int l = ((i * NW + wave) * 64 + lane) * 4, row = l / KE, k = l % KE;
+            at[i] = (uint32_t)(((k / 4) ^ turn(row)) * 16);
+            offset[i] = row < rows ? (uint32_t)row * pitch_bytes + at[i] : TILE_MASKED;
+        }
+    }
+    __device__ void load(uint32_t lds, int left, int wave, int) const { // left: inner indices from here on
+        const i32x4 buffer = buffer_of(base);
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const uint32_t from = left >= KE || (int)at[i] < left * 4 ? offset[i] : TILE_MASKED;
+            load_to_lds16(buffer, from, lds + (i * NW + wave) * 1024);
+        }
+    }
+    __device__ void next() { base += KE * 4; }
+    __device__ static f32x4 read(const char* lds, int rb, int e, int lane) { // eight inner indices, four a half
+        const int row = lane & 31;
+        return *reinterpret_cast<const f32x4*>(lds + (rb * 32 + row) * KE * 4 + (((2 * e + (lane >> 5)) ^ turn(row)) * 16));
+    }
+};
+template <int COLS, int NW, int KE> struct ColTile32 { // inner index down the rows
+    static constexpr int BYTES = COLS * KE * 4, LOADS = BYTES / (1024 * NW);
+    static_assert(BYTES % (1024 * NW) == 0, "whole loads");
+    uint32_t offset[LOADS];
+    uint64_t base, step;
+    __device__ static int row_of(int i, int wave, int lane) { return ((i * NW + wave) * 64 + lane) * 4 / COLS; }
+    __device__ void init(const float* at, uint32_t pitch_bytes, int cols, int wave, int lane) {
+        base = uniform64((uint64_t)at);
+        step = (uint64_t)KE * pitch_bytes;
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const int col = ((i * NW + wave) * 64 + lane) * 4 % COLS;
+            offset[i] = col < cols ? (uint32_t)row_of(i, wave, lane) * pitch_bytes + col * 4 : TILE_MASKED;
+        }
+    }
+    __device__ void load(uint32_t lds, int left, int wave, int lane) const {
+        const i32x4 buffer = buffer_of(base);
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const uint32_t from = left >= KE || row_of(i, wave, lane) < left ? offset[i] : TILE_MASKED;
+            load_to_lds16(buffer, from, lds + (i * NW + wave) * 1024);
+        }
+    }
+    __device__ void next() { base += step; }
+    __device__ static f32x4 read(const char* lds, int cb, int e, int lane) {
+        const float* p = reinterpret_cast<const float*>(lds) + (8 * e + 4 * (lane >> 5)) * COLS + cb * 32 + (lane & 31);
+        return f32x4{p[0], p[COLS], p[2 * COLS], p[3 * COLS]};
+    }
+};
+
+template <bool ACOL, bool BCOL, int MT, int NT, int WM, int WN, int KG, int KE, int ST>
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_tile32(LinTile a) {
+    constexpr int NW = WM * WN * KG, BM = WM * MT * 32, BN = WN * NT * 32, FS = KE / 16 / KG;
+    using ATile = std::conditional_t<ACOL, ColTile32<BM, NW, KE>, RowTile32<BM, NW, KE>>;
+    using BTile = std::conditional_t<BCOL, ColTile32<BN, NW, KE>, RowTile32<BN, NW, KE>>;
+    constexpr int STAGE = ATile::BYTES + BTile::BYTES, PER = ATile::LOADS + BTile::LOADS;
+    __shared__ __align__(1024) char lds[ST * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / (WM * WN), wm = wave % (WM * WN) / WN, wn = wave % WN;
+    const uint32_t m = a.o.m, n = a.o.n;
+    const uint32_t id = xcd_run(blockIdx.x, gridDim.x), tile = id / a.cuts, cut = id % a.cuts;
+    const uint32_t band = tile / (a.band * a.nt), in_band = tile % (a.band * a.nt), high = min(a.band, a.mt - band * a.band);
+    const uint32_t row = (band * a.band + in_band % high) * BM, col = in_band / high * BN;
+    const uint32_t s0 = cut * a.cut_stages, stages = min(a.cut_stages, (a.k + KE - 1) / KE - s0);
+    const int mrows = (int)min((uint32_t)BM, m - row), ncols = (int)min((uint32_t)BN, n - col);
+    ATile ta;
+    BTile tb;
+    if constexpr (ACOL) ta.init((const float*)((const char*)a.a + (uint64_t)s0 * KE * a.a_pitch) + row, a.a_pitch, (mrows + 3) / 4 * 4, wave, lane);
+    else ta.init((const float*)((const char*)a.a + (uint64_t)row * a.a_pitch) + (uint64_t)s0 * KE, a.a_pitch, mrows, wave, lane);
+    if constexpr (BCOL) tb.init((const float*)((const char*)a.b + (uint64_t)s0 * KE * a.b_pitch) + col, a.b_pitch, (ncols + 3) / 4 * 4, wave, lane);
+    else tb.init((const float*)((const char*)a.b + (uint64_t)col * a.b_pitch) + (uint64_t)s0 * KE, a.b_pitch, ncols, wave, lane);
+    const uint32_t base = lds_address(lds);
+    int left = (int)min(stages * KE, a.k - s0 * KE);
+    uint32_t into = 0;
+    auto issue = [&]() {
+        ta.load(base + into, left, wave, lane);
+        tb.load(base + into + ATile::BYTES, left, wave, lane);
+        ta.next();
+        tb.next();
+        left -= KE;
+        into = into + STAGE == ST * STAGE ? 0 : into + STAGE;
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; s++) issue();
+    f32x16 acc[MT][NT] = {};
+    uint32_t from = 0;
+    for (uint32_t s = 0; s < stages; s++) {
+        tile_wait<(ST - 2) * PER>();
+        const char* A = lds + from;
+        const char* B = A + ATile::BYTES;
+        f32x4 x[FS][MT][2], y[FS][NT][2];
+#pragma unroll
+        for (int f = 0; f < FS; f++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+#pragma unroll
+                for (int i = 0; i < MT; i++) x[f][i][e] = ATile::read(A, wm * MT + i, 2 * (kg * FS + f) + e, lane);
+#pragma unroll
+                for (int t = 0; t < NT; t++) y[f][t][e] = BTile::read(B, wn * NT + t, 2 * (kg * FS + f) + e, lane);
+            }
+        issue();
+#pragma unroll
+        for (int f = 0; f < FS; f++) {
+            Parts sx[MT], sy[NT];
+#pragma unroll
+            for (int i = 0; i < MT; i++) sx[i] = split8(x[f][i][0], x[f][i][1]);
+#pragma unroll
+            for (int t = 0; t < NT; t++) sy[t] = split8(y[f][t][0], y[f][t][1]);
+#pragma unroll
+            for (int total = 2; total >= 0; total--) // the smaller products first
+#pragma unroll
+                for (int p = 0; p <= total; p++)
+#pragma unroll
+                    for (int i = 0; i < MT; i++)
+#pragma unroll
+                        for (int t = 0; t < NT; t++) acc[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(sx[i].p[p], sy[t].p[total - p], acc[i][t], 0, 0, 0);
+        }
+        from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
+    }
+    tile_wait<0>();
+    tile_out<float, MT, NT, WM, WN, KG, ST * STAGE, (KG > 1)>(a, acc, lds, row, col, cut, kg, wm, wn, lane);
 }
 
 // The cuts' sums, eight columns a thread.
@@ -378,8 +535,7 @@ template <typename T, int MB, int NW> __global__ __launch_bounds__(64 * NW) void
 struct LinPack {
     const void *src, *pre;  // pre: multiply by the activation's slope there
     uint64_t src_stride, pre_stride;
-    void* dst;              // [rows][pitch] a plane, zeros behind a row's end; NULL: sums alone
-    uint64_t low;           // values from plane to plane
+    void* dst;              // [rows][pitch], zeros behind a row's end; NULL: sums alone
     uint32_t rows, cols, pitch, act;
     float* part;            // [strips][cols] sums of columns, or NULL
     uint32_t across, strips, first; // workgroups: 512 columns each, strips of rows; the first one's number
@@ -391,7 +547,6 @@ struct LinPacks {
 
 // A thread has eight columns and every fourth row of a strip; one launch for all matrices that a call needs in another form.
 template <typename T> __global__ __launch_bounds__(256) void linear_pack(LinPacks all) {
-    constexpr bool SPLIT = sizeof(T) == 4;
     __shared__ float sums[4][512];
     const uint32_t which = all.count > 2 && blockIdx.x >= all.one[2].first ? 2 : all.count > 1 && blockIdx.x >= all.one[1].first ? 1 : 0;
     const LinPack& a = all.one[which];
@@ -412,23 +567,7 @@ template <typename T> __global__ __launch_bounds__(256) void linear_pack(LinPack
 #pragma unroll
             for (int k = 0; k < 8; k++) s[k] += v[k];
             if (!a.dst) continue;
-            if constexpr (SPLIT) { // a plane holds what the ones before it left, rounded to 8 bits: the third one holds the rest exactly
-#pragma unroll
-                for (int p = 0; p < 3; p++) {
-                    typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-                    b8 w;
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        __bf16 top = (__bf16)v[k];
-                        if (p == 0 && __builtin_isinf((float)top)) top = (__bf16)__uint_as_float(__float_as_uint(v[k]) & 0xffff0000u); // just below the largest float
-                        w[k] = top;
-                        v[k] -= (float)top;
-                    }
-                    *reinterpret_cast<b8*>((__bf16*)a.dst + p * a.low + i * a.pitch + j) = w;
-                }
-            } else {
-                give8<T>(a.dst, i * a.pitch + j, v, 8);
-            }
+            give8<T>(a.dst, i * a.pitch + j, v, 8);
         }
     }
     if (!a.part) return;
@@ -459,15 +598,15 @@ __global__ __launch_bounds__(1024) void linear_bias(const float* part, uint32_t 
 
 struct LinOperand { // as the products take it
     const void* p;
-    uint64_t low;
     uint32_t pitch; // bytes
 };
 
 constexpr uint32_t LIN_STRIPS = 256; // of rows under one partial sum of the bias' gradient, at most
 
-// Whether a matrix can be taken where it lies.
-static bool as_it_is(const void* p, uint64_t stride, uint32_t cols, bool split) {
-    return !split && cols % 8 == 0 && stride % 8 == 0 && stride <= (1u << 21) && ((uintptr_t)p & 15) == 0;
+// Whether a matrix can be taken where it lies: 16 bytes a load, offsets of 256 rows in 31 bits.
+template <typename T> static bool as_it_is(const void* p, uint64_t stride, uint32_t cols) {
+    constexpr uint32_t E = 16 / sizeof(T);
+    return cols % E == 0 && stride % E == 0 && stride * sizeof(T) <= (1u << 22) && ((uintptr_t)p & 15) == 0;
 }
 
 struct LinPlan {
@@ -481,12 +620,12 @@ struct LinPlan {
 
 static uint32_t pitch_of(uint32_t cols) { return (cols + 7) / 8 * 8; }
 
-template <typename T> static uint64_t packed_bytes(uint64_t rows, uint32_t cols) { return rows * pitch_of(cols) * 2 * (sizeof(T) == 4 ? 3 : 1); }
+template <typename T> static uint64_t packed_bytes(uint64_t rows, uint32_t cols) { return rows * pitch_of(cols) * sizeof(T); }
 
 template <typename T>
 static LinPack& add_pack(apoe_ctx* ctx, LinPacks& all, const void* src, uint64_t stride, uint32_t rows, uint32_t cols, void* dst) {
     LinPack& a = all.one[all.count++];
-    a = LinPack{src, nullptr, stride, 0, dst, (uint64_t)rows * pitch_of(cols), rows, cols, pitch_of(cols), 0, nullptr, 0, 0, 0};
+    a = LinPack{src, nullptr, stride, 0, dst, rows, cols, pitch_of(cols), 0, nullptr, 0, 0, 0};
     a.across = (a.pitch + 511) / 512;
     a.strips = std::max(1u, std::min({(rows + 3) / 4, LIN_STRIPS, std::max(1u, (uint32_t)ctx->num_cus * 8 / a.across)}));
     return a;
@@ -517,9 +656,9 @@ struct LinKind {
 };
 constexpr LinKind LIN_KINDS[] = {{256, 256, 64, false, 9.f, .0243f, 0.f, 0.f}, {256, 128, 64, false, 6.5f, .0142f, 0.f, 0.f}, {128, 128, 64, true, 5.4f, .0165f, 2.5f, .0103f},
                                  {128, 128, 64, false, 3.f, .0082f, 0.f, 0.f}, {64, 64, 64, true, 1.f, .0055f, 1.f, .0033f}};
-constexpr LinKind LIN_KINDS_SPLIT[] = {{128, 128, 32, false, 8.f, .0421f, 0.f, 0.f}, {64, 64, 64, false, 1.5f, .0165f, 0.f, 0.f}};
+constexpr LinKind LIN_KINDS_FLOAT[] = {{256, 256, 32, false, 12.f, .157f, 0.f, 0.f}, {128, 128, 32, false, 6.5f, .044f, 0.f, 0.f}, {64, 64, 64, false, 2.f, .0155f, 0.f, 0.f}};
 
-template <int P> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t n, uint32_t k) {
+template <typename T> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t n, uint32_t k) {
     const uint64_t cus = (uint64_t)ctx->num_cus;
     LinShape best{};
     float least = INFINITY;
@@ -541,47 +680,39 @@ template <int P> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t n, u
         }
     };
     uint32_t number = 0;
-    if constexpr (P == 1) {
+    if constexpr (sizeof(T) == 2) {
         for (const LinKind& kind : LIN_KINDS) look(kind, number++);
     } else {
-        for (const LinKind& kind : LIN_KINDS_SPLIT) look(kind, number++);
+        for (const LinKind& kind : LIN_KINDS_FLOAT) look(kind, number++);
     }
     return best;
 }
 
 static uint64_t cut_bytes(const LinShape& s, uint32_t m, uint32_t n) { return s.cuts > 1 ? (uint64_t)s.cuts * m * pitch_of(n) * 4 : 0; }
 
-template <typename S, typename T, int P, bool ACOL, bool BCOL>
+template <typename T, bool ACOL, bool BCOL>
 static void product(apoe_ctx* ctx, const LinShape& s, LinOperand a, LinOperand b, uint32_t k, float* part, const LinOut& o) {
     const uint32_t mt = (o.m + s.bm - 1) / s.bm, nt = (o.n + s.bn - 1) / s.bn;
     uint32_t band = 1; // a power of two, so that runs end where bands do (8192 x 8192 x 4096: 444 us, row by row 482; 8192 x 1024 x 4096 67, 75)
     while (band * 2 <= mt && (uint64_t)band * band * 32 <= (uint64_t)mt * nt) band *= 2;
-    LinTile t{a.p, b.p, a.low, b.low, a.pitch, b.pitch, k, mt, nt, band, s.cuts, s.cut_stages, part, pitch_of(o.n), o};
+    LinTile t{a.p, b.p, a.pitch, b.pitch, k, mt, nt, band, s.cuts, s.cut_stages, part, pitch_of(o.n), o};
     const uint32_t grid = (uint32_t)((uint64_t)mt * nt * s.cuts);
     hipStream_t st = ctx->stream;
-    if constexpr (P == 1) {
-        if (s.kind == 0) linear_tile<S, T, P, ACOL, BCOL, 4, 2, 2, 4, 1, 4, 2><<<grid, 512, 0, st>>>(t);
-        else if (s.kind == 1) linear_tile<S, T, P, ACOL, BCOL, 2, 2, 4, 2, 1, 4, 3><<<grid, 512, 0, st>>>(t);
-        else if (s.kind == 2) linear_tile<S, T, P, ACOL, BCOL, 2, 2, 2, 2, 1, 4, 2><<<grid, 256, 0, st>>>(t);
-        else if (s.kind == 3) linear_tile<S, T, P, ACOL, BCOL, 2, 2, 2, 2, 2, 4, 4><<<grid, 512, 0, st>>>(t);
-        else linear_tile<S, T, P, ACOL, BCOL, 1, 1, 2, 2, 1, 4, 4><<<grid, 256, 0, st>>>(t);
+    if constexpr (sizeof(T) == 2) {
+        if (s.kind == 0) linear_tile<T, ACOL, BCOL, 4, 2, 2, 4, 1, 4, 2><<<grid, 512, 0, st>>>(t);
+        else if (s.kind == 1) linear_tile<T, ACOL, BCOL, 2, 2, 4, 2, 1, 4, 3><<<grid, 512, 0, st>>>(t);
+        else if (s.kind == 2) linear_tile<T, ACOL, BCOL, 2, 2, 2, 2, 1, 4, 2><<<grid, 256, 0, st>>>(t);
+        else if (s.kind == 3) linear_tile<T, ACOL, BCOL, 2, 2, 2, 2, 2, 4, 4><<<grid, 512, 0, st>>>(t);
+        else linear_tile<T, ACOL, BCOL, 1, 1, 2, 2, 1, 4, 4><<<grid, 256, 0, st>>>(t);
     } else {
-        if (s.kind == 0) linear_tile<S, T, P, ACOL, BCOL, 2, 2, 2, 2, 2, 2, 3><<<grid, 512, 0, st>>>(t);
-        else linear_tile<S, T, P, ACOL, BCOL, 1, 1, 2, 2, 1, 4, 3><<<grid, 256, 0, st>>>(t);
+        if (s.kind == 0) linear_tile32<ACOL, BCOL, 4, 2, 2, 4, 1, 32, 2><<<grid, 512, 0, st>>>(t);
+        else if (s.kind == 1) linear_tile32<ACOL, BCOL, 2, 2, 2, 2, 2, 32, 4><<<grid, 512, 0, st>>>(t);
+        else linear_tile32<ACOL, BCOL, 2, 1, 1, 2, 4, 64, 4><<<grid, 512, 0, st>>>(t);
     }
     if (s.cuts > 1) linear_join<T><<<(uint32_t)std::min<uint64_t>(((uint64_t)o.m * (t.np / 8) + 255) / 256, 1u << 16), 256, 0, st>>>(t);
 }
 
 template <typename T> static bool whole_rows(const void* p, uint64_t stride) { return ((uintptr_t)p & 15) == 0 && stride % (16 / sizeof(T)) == 0; }
-
-template <typename T> struct LinTypes {
-    using S = T;
-    static constexpr int P = 1;
-};
-template <> struct LinTypes<float> {
-    using S = __bf16;
-    static constexpr int P = 3;
-};
 
 template <typename T, int MB> static void few(apoe_ctx* ctx, const LinFew& a) {
     const uint32_t grid = (a.o.n + 15) / 16;
@@ -591,8 +722,6 @@ template <typename T, int MB> static void few(apoe_ctx* ctx, const LinFew& a) {
 }
 
 template <typename T> static int run_linear(apoe_ctx* ctx, const apoe_linear_args* p) {
-    using S = typename LinTypes<T>::S;
-    constexpr int P = LinTypes<T>::P;
     const uint32_t m = p->rows, n = p->cols_out, k = p->cols_in;
     constexpr uint32_t E = 16 / sizeof(T);
     if (m <= 64 && k % E == 0 && whole_rows<T>(p->x, p->x_stride) && whole_rows<T>(p->w, p->w_stride)) {
@@ -603,45 +732,43 @@ template <typename T> static int run_linear(apoe_ctx* ctx, const apoe_linear_arg
         APOE_HIP(hipGetLastError());
         return APOE_OK;
     }
-    const bool x_is = as_it_is(p->x, p->x_stride, k, P > 1), w_is = as_it_is(p->w, p->w_stride, k, P > 1);
-    const LinShape s = choose<P>(ctx, m, n, k);
+    const bool x_is = as_it_is<T>(p->x, p->x_stride, k), w_is = as_it_is<T>(p->w, p->w_stride, k);
+    const LinShape s = choose<T>(ctx, m, n, k);
     LinPlan plan;
     const uint64_t o_x = plan.take(x_is ? 0 : packed_bytes<T>(m, k)), o_w = plan.take(w_is ? 0 : packed_bytes<T>(n, k)), o_part = plan.take(cut_bytes(s, m, n));
     char* ws = nullptr;
     if (plan.bytes) APOE_TRY(ctx->adapt_workspace(plan.bytes, &ws));
-    LinOperand x{p->x, 0, (uint32_t)(p->x_stride * sizeof(S))}, w{p->w, 0, (uint32_t)(p->w_stride * sizeof(S))};
+    LinOperand x{p->x, (uint32_t)(p->x_stride * sizeof(T))}, w{p->w, (uint32_t)(p->w_stride * sizeof(T))};
     LinPacks packs{};
     if (!x_is) {
-        x = LinOperand{ws + o_x, (uint64_t)m * pitch_of(k), pitch_of(k) * (uint32_t)sizeof(S)};
+        x = LinOperand{ws + o_x, pitch_of(k) * (uint32_t)sizeof(T)};
         add_pack<T>(ctx, packs, p->x, p->x_stride, m, k, ws + o_x);
     }
     if (!w_is) {
-        w = LinOperand{ws + o_w, (uint64_t)n * pitch_of(k), pitch_of(k) * (uint32_t)sizeof(S)};
+        w = LinOperand{ws + o_w, pitch_of(k) * (uint32_t)sizeof(T)};
         add_pack<T>(ctx, packs, p->w, p->w_stride, n, k, ws + o_w);
     }
     pack<T>(ctx, packs);
     LinOut o{p->y, p->bias, p->residual, p->pre, p->y_stride, p->residual_stride, p->pre_stride, m, n, p->act};
-    product<S, T, P, false, false>(ctx, s, x, w, k, (float*)(ws + o_part), o);
+    product<T, false, false>(ctx, s, x, w, k, (float*)(ws + o_part), o);
     APOE_HIP(hipGetLastError());
     return APOE_OK;
 }
 
 template <typename T> static int run_linear_grad(apoe_ctx* ctx, const apoe_linear_args* p) {
-    using S = typename LinTypes<T>::S;
-    constexpr int P = LinTypes<T>::P;
     const uint32_t m = p->rows, n = p->cols_out, k = p->cols_in;
     const bool act = p->act != APOE_ACT_NONE, products = p->grad_x || p->grad_w;
-    const bool g_is = !act && as_it_is(p->grad_y, p->grad_y_stride, n, P > 1), x_is = !p->grad_w || as_it_is(p->x, p->x_stride, k, P > 1), w_is = !p->grad_x || as_it_is(p->w, p->w_stride, k, P > 1);
+    const bool g_is = !act && as_it_is<T>(p->grad_y, p->grad_y_stride, n), x_is = !p->grad_w || as_it_is<T>(p->x, p->x_stride, k), w_is = !p->grad_x || as_it_is<T>(p->w, p->w_stride, k);
     const bool pack_g = products && !g_is;
     LinShape sx{}, sw{};
-    if (p->grad_x) sx = choose<P>(ctx, m, k, n);
-    if (p->grad_w) sw = choose<P>(ctx, n, k, m);
+    if (p->grad_x) sx = choose<T>(ctx, m, k, n);
+    if (p->grad_w) sw = choose<T>(ctx, n, k, m);
     LinPlan plan;
     const uint64_t o_g = plan.take(pack_g ? packed_bytes<T>(m, n) : 0), o_x = plan.take(x_is ? 0 : packed_bytes<T>(m, k)), o_w = plan.take(w_is ? 0 : packed_bytes<T>(n, k));
     const uint64_t o_part = plan.take(std::max({p->grad_x ? cut_bytes(sx, m, k) : 0, p->grad_w ? cut_bytes(sw, n, k) : 0, p->grad_bias ? (uint64_t)LIN_STRIPS * n * 4 : 0}));
     char* ws = nullptr;
     if (plan.bytes) APOE_TRY(ctx->adapt_workspace(plan.bytes, &ws));
-    LinOperand g{p->grad_y, 0, (uint32_t)(p->grad_y_stride * sizeof(S))}, x{p->x, 0, (uint32_t)(p->x_stride * sizeof(S))}, w{p->w, 0, (uint32_t)(p->w_stride * sizeof(S))};
+    LinOperand g{p->grad_y, (uint32_t)(p->grad_y_stride * sizeof(T))}, x{p->x, (uint32_t)(p->x_stride * sizeof(T))}, w{p->w, (uint32_t)(p->w_stride * sizeof(T))};
     LinPacks packs{};
     uint32_t strips = 0;
     if (pack_g || p->grad_bias) {
@@ -653,25 +780,25 @@ template <typename T> static int run_linear_grad(apoe_ctx* ctx, const apoe_linea
         }
         if (p->grad_bias) a.part = (float*)(ws + o_part);
         strips = a.strips;
-        if (pack_g) g = LinOperand{ws + o_g, (uint64_t)m * pitch_of(n), pitch_of(n) * (uint32_t)sizeof(S)};
+        if (pack_g) g = LinOperand{ws + o_g, pitch_of(n) * (uint32_t)sizeof(T)};
     }
     if (!x_is) {
-        x = LinOperand{ws + o_x, (uint64_t)m * pitch_of(k), pitch_of(k) * (uint32_t)sizeof(S)};
+        x = LinOperand{ws + o_x, pitch_of(k) * (uint32_t)sizeof(T)};
         add_pack<T>(ctx, packs, p->x, p->x_stride, m, k, ws + o_x);
     }
     if (!w_is) {
-        w = LinOperand{ws + o_w, (uint64_t)n * pitch_of(k), pitch_of(k) * (uint32_t)sizeof(S)};
+        w = LinOperand{ws + o_w, pitch_of(k) * (uint32_t)sizeof(T)};
         add_pack<T>(ctx, packs, p->w, p->w_stride, n, k, ws + o_w);
     }
     pack<T>(ctx, packs);
     if (p->grad_bias) linear_bias<<<(n + 15) / 16, 1024, 0, ctx->stream>>>((const float*)(ws + o_part), strips, n, p->grad_bias);
     if (p->grad_x && m) {
         LinOut o{p->grad_x, nullptr, nullptr, nullptr, p->grad_x_stride, 0, 0, m, k, APOE_ACT_NONE};
-        product<S, T, P, false, true>(ctx, sx, g, w, n, (float*)(ws + o_part), o);
+        product<T, false, true>(ctx, sx, g, w, n, (float*)(ws + o_part), o);
     }
     if (p->grad_w) {
         LinOut o{p->grad_w, nullptr, nullptr, nullptr, p->grad_w_stride, 0, 0, n, k, APOE_ACT_NONE};
-        product<S, T, P, true, true>(ctx, sw, g, x, m, (float*)(ws + o_part), o);
+        product<T, true, true>(ctx, sw, g, x, m, (float*)(ws + o_part), o);
     }
     APOE_HIP(hipGetLastError());
     return APOE_OK;

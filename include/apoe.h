@@ -480,10 +480,10 @@ typedef struct {
 
 /*
  * z = x w^T + bias, y = act(z) + residual; with gz = grad_y act'(pre): grad_x = gz w, grad_w = gz^T x, grad_bias = sum of gz's rows. (The
- * gradient of residual is grad_y.) Sums are 32 bits and rounded once. float matrices are multiplied as three bfloat16 parts each, 24 bits, six
- * products; a value that is infinite gives NaN there. gz is rounded to the matrices' type for the two products (with an activation; float: to 24 bits), not for
- * grad_bias. Workspace: gz; partial sums of up to 128 MiB where rows and columns are too few to fill the GPU; float matrices
- * (and such whose rows are not multiples of 16 bytes) in the form that the products take, 6 (2) bytes a value.
+ * gradient of residual is grad_y; y may be residual itself when the strides are equal.) Sums are 32 bits and rounded once. float matrices are
+ * multiplied as three parts of eight bits each, six products: off by 2^-22 of each product of two values at most; a value that is infinite gives NaN there. gz of
+ * 16-bit matrices with an activation is rounded for the two products, not for grad_bias. Workspace: gz, partial sums of up to 128 MiB
+ * where rows and columns are too few to fill the GPU, and copies of matrices whose rows are not whole multiples of 16 bytes or lie further than 4 MiB apart.
  */
 int apoe_linear(apoe_ctx* ctx, const apoe_linear_args* args);
 int apoe_linear_grad(apoe_ctx* ctx, const apoe_linear_args* args);
