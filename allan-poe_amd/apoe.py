@@ -832,8 +832,8 @@ def _norm_args(ctx, x, w, b, eps):
 def layer_norm(ctx, x, w=None, b=None, eps=1e-5, out=None):
     """w * (x - mean(x)) / sqrt(var(x) + eps) + b for every row of x [m, d]; w and b are float32. out may be x itself."""
     a = _norm_args(ctx, x, w, b, eps)
-    if out is None:
-        out = x.new_empty(x.shape)
+    if out is None:  # (like x where that is dense: half a microsecond less)
+        out = _torch.empty_like(x) if a.x_stride == a.dim else x.new_empty(x.shape)
     else:
         a.y_stride = _matrix(ctx, out, "out", x.shape, x.dtype)
     a.y = out.data_ptr()

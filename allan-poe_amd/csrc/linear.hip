@@ -6,7 +6,7 @@
 // the nine products the six that count are added up: as accurate value by value as float products, whatever the exponents are, at a sixth of
 // 1400 TFLOP/s where the float matrix units have 154. What is done to a result (bias, activation, residual, rounding) is done behind the last stage,
 // through LDS, 16 bytes a thread. Where tiles are too few for the GPU the inner dimension is cut and a second launch adds the cuts up, in order.
-// Up to 64 rows a kernel of its own streams w once (the serving form).
+// Up to 16 rows a kernel of its own streams w once (the serving form).
 #include <algorithm>
 #include <cmath>
 
@@ -469,7 +469,7 @@ template <typename T> __global__ __launch_bounds__(256) void linear_join(LinTile
     }
 }
 
-// ---- up to 64 rows ----
+// ---- up to 16 rows ----
 
 struct LinFew {
     const void *x, *w;
@@ -479,55 +479,46 @@ struct LinFew {
 };
 
 // Bound by the one reading of w (and for small layers by its latency): a workgroup has 16 of w's rows, its NW waves share the inner side, 128 indices at a time, all of
-// whose loads are on their way at once; x comes from the L2. MB blocks of 16 rows of x; 16 x 16 matrix instructions, float matrices on the float ones.
-// The waves' sums meet in LDS, one result a thread. 16 x 1024 -> 4096 fp16: 5 us (64 x 64 tiles in two cuts and their sum 9).
-template <typename T, int MB, int NW> __global__ __launch_bounds__(64 * NW) void linear_few(LinFew a) {
+// whose loads are on their way at once; x comes from the L2. 16 x 16 matrix instructions, float matrices on the float ones. The waves' sums meet in LDS, one
+// result a thread. 16 x 1024 -> 4096 fp16: 4.5 us (64 x 64 tiles in two cuts and their sum 9).
+template <typename T, int NW> __global__ __launch_bounds__(64 * NW) void linear_few(LinFew a) {
     constexpr int E = 16 / sizeof(T), STEP = 4 * E, U = 128 / STEP; // values a lane loads; inner indices of a load; loads of a turn
     typedef T tv __attribute__((ext_vector_type(E)));
-    __shared__ float sums[NW][MB * 256];
+    __shared__ float sums[NW][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, r = lane & 15;
     const uint32_t m = a.o.m, n = a.o.n, col = blockIdx.x * 16;
-    const T* wr = (const T*)a.w + (uint64_t)min(col + r, n - 1) * a.w_stride; // rows beyond the end: the last one again, whose results go nowhere
-    const T* xr[MB];
-#pragma unroll
-    for (int b = 0; b < MB; b++) xr[b] = (const T*)a.x + (uint64_t)min((uint32_t)(b * 16 + r), m - 1) * a.x_stride;
-    f32x4 acc[MB] = {};
+    const T* xr = (const T*)a.x + (uint64_t)min((uint32_t)r, m - 1) * a.x_stride; // rows beyond the end: the last one again, whose results go nowhere
+    const T* wr = (const T*)a.w + (uint64_t)min(col + r, n - 1) * a.w_stride;
+    f32x4 acc = {};
     for (uint32_t k0 = wave * 128; k0 < a.k; k0 += NW * 128) {
-        tv wv[U], xv[MB][U];
+        tv xv[U], wv[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const uint32_t k = k0 + u * STEP + q * E;
+            xv[u] = k < a.k ? *reinterpret_cast<const tv*>(xr + k) : tv{};
             wv[u] = k < a.k ? *reinterpret_cast<const tv*>(wr + k) : tv{};
-#pragma unroll
-            for (int b = 0; b < MB; b++) xv[b][u] = k < a.k ? *reinterpret_cast<const tv*>(xr[b] + k) : tv{};
         }
 #pragma unroll
-        for (int u = 0; u < U; u++)
+        for (int u = 0; u < U; u++) {
+            if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
-            for (int b = 0; b < MB; b++) {
-                if constexpr (std::is_same_v<T, float>) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) acc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[b][u][j], wv[u][j], acc[b], 0, 0, 0);
-                } else if constexpr (std::is_same_v<T, _Float16>) {
-                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xv[b][u], wv[u], acc[b], 0, 0, 0);
-                } else {
-                    acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv[b][u], wv[u], acc[b], 0, 0, 0);
-                }
+                for (int j = 0; j < 4; j++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[u][j], wv[u][j], acc, 0, 0, 0);
+            } else if constexpr (std::is_same_v<T, _Float16>) {
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(xv[u], wv[u], acc, 0, 0, 0);
+            } else {
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xv[u], wv[u], acc, 0, 0, 0);
             }
+        }
     }
 #pragma unroll
-    for (int b = 0; b < MB; b++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) sums[wave][b * 256 + (4 * q + i) * 16 + r] = acc[b][i];
+    for (int i = 0; i < 4; i++) sums[wave][(4 * q + i) * 16 + r] = acc[i];
     __syncthreads();
-    for (uint32_t v = threadIdx.x; v < MB * 256; v += 64 * NW) {
-        const uint32_t i = v / 16, j = col + v % 16;
-        if (i >= m || j >= n) continue;
-        float z[8] = {};
+    const uint32_t i = threadIdx.x / 16, j = col + threadIdx.x % 16;
+    if (i >= m || j >= n) return;
+    float z = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; w++) z[0] += sums[w][v];
-        finish1<T>(a.o, i, j, z[0]);
-    }
+    for (int w = 0; w < NW; w++) z += sums[w][threadIdx.x];
+    finish1<T>(a.o, i, j, z);
 }
 
 // ---- operands in the products' form, gz, and the columns' sums ----
@@ -714,21 +705,16 @@ static void product(apoe_ctx* ctx, const LinShape& s, LinOperand a, LinOperand b
 
 template <typename T> static bool whole_rows(const void* p, uint64_t stride) { return ((uintptr_t)p & 15) == 0 && stride % (16 / sizeof(T)) == 0; }
 
-template <typename T, int MB> static void few(apoe_ctx* ctx, const LinFew& a) {
-    const uint32_t grid = (a.o.n + 15) / 16;
-    // sixteen waves where each has two turns of the inner side at least
-    if (a.k >= 4096) linear_few<T, MB, 16><<<grid, 1024, 0, ctx->stream>>>(a);
-    else linear_few<T, MB, 8><<<grid, 512, 0, ctx->stream>>>(a);
-}
-
 template <typename T> static int run_linear(apoe_ctx* ctx, const apoe_linear_args* p) {
     const uint32_t m = p->rows, n = p->cols_out, k = p->cols_in;
     constexpr uint32_t E = 16 / sizeof(T);
-    if (m <= 64 && k % E == 0 && whole_rows<T>(p->x, p->x_stride) && whole_rows<T>(p->w, p->w_stride)) {
+    // Few rows and a w that is soon read (us of a call, tiles of 64 x 64 in brackets: 16 rows of fp16, 1024 x 1024 6.8 (7.4), 4096 -> 1024 9.0 (9.9), 4096 x 4096 9.4 (11),
+    // 4096 -> 16 384 39 (31), one row 26 (31); float, 1024 x 1024 6.5 (9.8), 2048 x 2048 10 (12), 4096 -> 1024 18 (12)); more rows: tiles (32 of 4096 x 4096 13.5 (11)).
+    const bool soon = k <= (sizeof(T) == 2 ? 4096 : 2048) && ((uint64_t)n * k <= 1u << 25 || m <= 4);
+    if (m <= 16 && soon && k % E == 0 && whole_rows<T>(p->x, p->x_stride) && whole_rows<T>(p->w, p->w_stride)) {
         const LinFew a{p->x, p->w, p->x_stride, p->w_stride, k, LinOut{p->y, p->bias, p->residual, p->pre, p->y_stride, p->residual_stride, p->pre_stride, m, n, p->act}};
-        if (m <= 16) few<T, 1>(ctx, a);
-        else if (m <= 32) few<T, 2>(ctx, a);
-        else few<T, 4>(ctx, a);
+        if (k >= 4096) linear_few<T, 16><<<(n + 15) / 16, 1024, 0, ctx->stream>>>(a); // two turns of the inner side for each wave
+        else linear_few<T, 8><<<(n + 15) / 16, 512, 0, ctx->stream>>>(a);
         APOE_HIP(hipGetLastError());
         return APOE_OK;
     }

@@ -106,6 +106,13 @@ def test_sizes_and_types(gpu_ctx, m, n, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 17, 4096), (16, 4100, 1032), (4, 33, 264), (16, 64, 4096), (17, 64, 4096), (3, 20, 8192)])
+def test_few_rows(gpu_ctx, m, n, k, dtype):
+    for act in ("none", "gelu"):
+        check(gpu_ctx, m, n, k, dtype, act, m + k, pad=8, grad=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("act", ACTS)
 def test_activations(gpu_ctx, act, dtype):
     check(gpu_ctx, 200, 136, 96, dtype, act, 1)
