@@ -9,6 +9,9 @@
 // thousandth a step would stand still if it were rounded to the nearest code, so it goes up or down by chance, with the probability that keeps
 // its mean in m and in v. What is above a code is a difference of two close numbers, and the comparison with the chance decides a
 // code: both in 64 bits, at the same rate as 32 on this GPU's vector units.
+// Measured: 132 M values in twelve layers and a table, 32 bits 711 us for 3.7 GB (5.2 TB/s); 8 bits 536 us for 2.1 GB (4.0 TB/s): 125 vector instructions a value, which
+// keep the units busy in 78 % of the cycles (deciding the codes in 32 bits with 64 as a fallback took 719); reading the moments back 295 us for
+// 1.3 GB. 8.4 M values in 32 bits 50 us (4.7 TB/s).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -347,8 +350,8 @@ int launch_adamw(apoe_adamw* opt, const apoe_adamw_step_args* p) {
     }
     auto go = [&]() -> int {
         if (a.pieces == 0) return APOE_OK;
-        // In 8 bits the kernel's operations are what it waits for: root and reciprocal to a unit of the last place (132 M values 568 us, with a rounded
-        // root and quotient 670). Their instructions take numbers below 2^-126 for zero: beside an eps of 2^-36 and more, such a root counts nothing.
+        // In 8 bits the kernel's operations are what it waits for: root and reciprocal to a unit of the last place (132 M values then took 568 us, with a
+        // rounded root and quotient 670). Their instructions take numbers below 2^-126 for zero: beside an eps of 2^-36 and more, such a root counts nothing.
         const bool near = p->eps >= 0x1p-36;
         const auto run = [&](auto kernel) { kernel<<<a.pieces, 256, 0, opt->ctx->stream>>>(a); };
         if (opt->bits == 32) run(near ? adamw_step<32, true> : adamw_step<32, false>);

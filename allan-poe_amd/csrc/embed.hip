@@ -8,6 +8,9 @@
 // are added up in never changes), then walks over them in blocks of 32: a row whose entries lie in one block is written directly, of one that
 // crosses blocks each block leaves its part, and a last launch adds the parts up in order. So a token that is a tenth of all entries costs what
 // its rows' bytes cost, and no atomic changes a bit between two calls.
+// Measured: 65 536 bf16 tokens of 1024 columns, table of 30 522 rows: forward 41 us (134 MB written, 62 read at least: 4.8 TB/s), gradient 90: sort 25 (four launches),
+// walk 56 (212 MB: 3.8 TB/s; rows in order 47), join 8; every entry the same row: join 43. 777 float queries of 40 terms: forward 26, weights 22 (127 MB each
+// through the L2 and what lies behind), sort 30, walk 31, join 10. 32 fp16 queries of 40 terms 7 us.
 #include <algorithm>
 
 #include "apoe_internal.h"
@@ -198,7 +201,7 @@ __device__ inline void scan256(uint32_t* total, int tid) {
 }
 
 // Each item's row, the last one that begins at or before it, and weight, to its place. The searches of all rounds go step by step together: a step waits for one
-// load, not for ROUNDS (four of 428 rows: 13 us in turn, 8 together).
+// load, not for ROUNDS (17 120 entries of 428 rows, the whole launch: 13.3 us in turn, 11.3 together).
 template <int ROUNDS> __device__ inline void put_entries(const EmbedArgs& a, const uint2* item, const bool* in, const uint32_t* place) {
     uint32_t row[ROUNDS];
     float val[ROUNDS];
