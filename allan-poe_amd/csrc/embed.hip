@@ -153,6 +153,12 @@ template <typename T, int V, int G, bool WHOLE> __global__ __launch_bounds__(G >
                 if (t == u && e + u < end) p.grad_val[e + u] = on[u] ? s[u] * p.scale : 0.f;
         }
     }
+    if (p.off) { // entries in front of the first row and behind the last one
+        const uint32_t last = min(p.off[p.n_rows], p.n_entries), first = min(p.off[0], last);
+        const uint64_t at = ((uint64_t)blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x, step = (uint64_t)gridDim.x * gridDim.y * blockDim.x;
+        for (uint64_t e = at; e < first; e += step) p.grad_val[e] = 0.f;
+        for (uint64_t e = last + at; e < p.n_entries; e += step) p.grad_val[e] = 0.f;
+    }
 }
 
 // ---- the sort ----

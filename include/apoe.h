@@ -400,6 +400,8 @@ int apoe_gated_residual_grad(apoe_ctx* ctx, const apoe_gated_residual_args* args
  * summed up (terms of the learned-sparse path, tokens), layer norm, matrix products with what is done to their results, and the step of
  * all parameters. The rules above hold: the context's stream, device pointers, strides from row to row (0: dense), workspace that the context
  * keeps. Rows may begin at any multiple of their type's size; such as begin at multiples of 16 bytes are read 16 bytes at a time.
+ * A captured graph uses the context's workspace as it was then, which is kept as long as the context: all of a context's calls and graphs run one
+ * after the other, and the context outlives its graphs.
  */
 #define APOE_EMBED_MAX_DIM 8192u
 #define APOE_NORM_MAX_DIM 8192u
@@ -410,8 +412,9 @@ typedef struct {
     uint32_t n_rows, n_table, n_entries, dim; /* n_table < 2^30, n_entries < 2^27; off == NULL: n_entries == n_rows */
     const void* table;              /* [n_table][dim]; the gradient needs it for grad_val alone */
     const uint32_t* idx;            /* [n_entries]: an entry at or above n_table counts nothing, and its grad_val is zero */
-    const uint32_t* off;            /* [n_rows + 1]: CSR, numbers from 0 to n_entries that do not fall (on the GPU: not checked, but nothing
-                                       beyond n_entries is read); NULL: entry i is row i's */
+    const uint32_t* off;            /* [n_rows + 1]: CSR, numbers that do not fall (on the GPU: not checked, but nothing beyond n_entries is
+                                       read); entries in front of off[0] or from off[n_rows] on are no row's, and their grad_val is zero
+                                       (entries and no row at all: refused); NULL: entry i is row i's */
     const float* val;               /* [n_entries]; NULL: ones */
     float scale;
     const void* base;               /* [n_rows][dim], may be NULL */
@@ -479,11 +482,13 @@ typedef struct {
 } apoe_linear_args;
 
 /*
- * z = x w^T + bias, y = act(z) + residual; with gz = grad_y act'(pre): grad_x = gz w, grad_w = gz^T x, grad_bias = sum of gz's rows. (The
- * gradient of residual is grad_y; y may be residual itself when the strides are equal.) Sums are 32 bits and rounded once. float matrices are
- * multiplied as three parts of eight bits each, six products: off by 2^-22 of each product of two values at most; a value that is infinite gives NaN there. gz of
- * 16-bit matrices with an activation is rounded for the two products, not for grad_bias. Workspace: gz, partial sums of up to 128 MiB
- * where rows and columns are too few to fill the GPU, and copies of matrices whose rows are not whole multiples of 16 bytes or lie further than 4 MiB apart.
+ * z = x w^T + bias, y = act(z) + residual; with gz = grad_y act'(pre) (APOE_ACT_RELU: zero where pre is not above zero, whatever grad_y is there):
+ * grad_x = gz w, grad_w = gz^T x, grad_bias = sum of gz's rows. (The gradient of residual is grad_y; y may be residual itself when the strides are
+ * equal.) Sums are 32 bits and rounded once. float matrices are multiplied as three parts of eight bits each, six products: off by 2^-22 of each
+ * product of two values at most, and a value below 2^-111, whose last part is below the parts' smallest number, by 2^-133 of the other; a value that is
+ * infinite gives NaN there. gz of 16-bit matrices with an activation is rounded for the two products, not for grad_bias. Workspace: gz, partial sums
+ * of up to 128 MiB where rows and columns are too few to fill the GPU, and copies of matrices whose rows are not whole multiples of 16 bytes or lie
+ * further than 4 MiB apart.
  */
 int apoe_linear(apoe_ctx* ctx, const apoe_linear_args* args);
 int apoe_linear_grad(apoe_ctx* ctx, const apoe_linear_args* args);

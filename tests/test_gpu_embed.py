@@ -269,3 +269,42 @@ def test_matrices_past_four_gigabytes(gpu_ctx):
     got = apoe.embed_grad(gpu_ctx, wide, far(grad, (1 << 31) // 299 + 7), idx, off, val, grad_table=wide_grad, grad_val=True)
     for k in near:
         assert bool(((got[k] - near[k]).abs() <= 2.0 ** -10 * near[k].abs() + 2.0 ** -24).all()), k  # rows that begin elsewhere are added up by other threads
+
+
+@pytest.mark.parametrize("n", [50, 9000])
+def test_rows_that_do_not_cover_all_entries(gpu_ctx, n):
+    """A part of a batch's rows with all of its entries: those in front of the first row and behind the last one are no row's, and their weights' gradients are
+    zeros; the rest is as if the entries had been cut too."""
+    import torch
+    import apoe
+    g = torch.Generator().manual_seed(21)
+    off = torch.arange(0, n + 1, 5, dtype=torch.int32).cuda()
+    idx, val = torch.randint(0, 300, (n,), generator=g, dtype=torch.int32).cuda(), torch.randn(n, generator=g).cuda()
+    table = matrix(g, 300, 40, "float32")
+    rows = len(off) - 1
+    for first, last in ((2, rows - 3), (0, 4), (rows - 1, rows), (rows, rows), (3, 3)):
+        part = off[first:last + 1].contiguous()
+        grad = matrix(g, last - first, 40, "float32")
+        if first == last:  # entries and no row at all
+            for call in (lambda: apoe.embed_grad(gpu_ctx, table, grad, idx, part, val, grad_val=True), lambda: apoe.embed_grad(gpu_ctx, table, grad, idx, part, val)):
+                with pytest.raises(apoe.ApoeError, match="without rows"):
+                    call()
+            continue
+        begin, end = int(part[0]), int(part[-1])
+        alone = part - begin
+        # what the result's memory held before: not zeros
+        fill = torch.full((n,), 7.0, device="cuda")
+        del fill
+        got = apoe.embed_grad(gpu_ctx, table, grad, idx, part, val, grad_val=True)
+        want = apoe.embed_grad(gpu_ctx, table, grad, idx[begin:end], alone, val[begin:end], grad_val=True)
+        # how many threads share a row hangs on the number of entries: two orders of five additions
+        a, b = apoe.embed(gpu_ctx, table, idx, part, val), apoe.embed(gpu_ctx, table, idx[begin:end], alone, val[begin:end])
+        terms = apoe.embed(gpu_ctx, table.abs(), idx[begin:end], alone, val[begin:end].abs())
+        close(a, b.double(), 2 * (5 + 4) * E * 1.01 * terms.double())
+        assert bool((got["grad_val"][begin:end] == want["grad_val"]).all())
+        assert not bool(got["grad_val"][:begin].any()) and not bool(got["grad_val"][end:].any())
+        # the sums' parts are cut at other places: two orders of at most n additions
+        size = torch.zeros(300, 40, device="cuda", dtype=torch.float64)
+        row_of = torch.repeat_interleave(torch.arange(last - first, device="cuda"), (alone[1:] - alone[:-1]).long())
+        size.index_add_(0, idx[begin:end].long(), (val[begin:end, None] * grad[row_of]).abs().double())
+        close(got["grad_table"], want["grad_table"].double(), 2 * (end - begin + 4) * E * size)
