@@ -324,3 +324,32 @@ def test_strides_past_four_gigabytes(gpu_ctx):
         for k in a:
             assert bool((a[k] == b[k]).all()), k
         del store, x
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_relu_lets_nothing_back_where_nothing_went_out(gpu_ctx, dtype):
+    """An infinity or a NaN in grad_y where pre is zero or below leaves all gradients as a zero there does."""
+    import torch
+    import apoe
+    g = torch.Generator().manual_seed(12)
+    x, w, gy = matrix(g, 70, 40, dtype), matrix(g, 24, 40, dtype), matrix(g, 70, 24, dtype)
+    pre = apoe.linear(gpu_ctx, x, w, act="relu", want_pre=True)[1]
+    pre[3, 5], pre[40, 23], pre[69, 0] = -1.0, 0.0, -0.0
+    gy[3, 5] = gy[40, 23] = gy[69, 0] = 0.0
+    want = apoe.linear_grad(gpu_ctx, x, w, gy, act="relu", pre=pre)
+    gy[3, 5], gy[40, 23], gy[69, 0] = float("inf"), float("nan"), float("-inf")
+    got = apoe.linear_grad(gpu_ctx, x, w, gy, act="relu", pre=pre)
+    for k in want:
+        assert bool(torch.isfinite(want[k]).all()) and bool((got[k] == want[k]).all()), k
+
+
+def test_small_values_with_large_ones_in_float32(gpu_ctx):
+    """Values from 2^-126 to 2^-100 times values around 2^110: the parts of small ones end at 2^-133, which each is off by at most."""
+    import torch
+    import apoe
+    g = torch.Generator().manual_seed(13)
+    m, n, k = 90, 70, 200
+    x = (torch.randn(m, k, generator=g).sign() * 2 ** (26 * torch.rand(m, k, generator=g, dtype=torch.float64) - 126)).float().cuda()
+    w = (torch.randn(n, k, generator=g) * 2.0 ** 110).cuda()
+    val, tol = formula(x, w, None, "none", None, "float32")
+    close(apoe.linear(gpu_ctx, x, w)[0], val["y"], tol["y"] + 2.0 ** -133 * w.double().abs().sum(1)[None, :])
