@@ -10,7 +10,7 @@
 // its rows' bytes cost, and no atomic changes a bit between two calls.
 // Measured: 65 536 bf16 tokens of 1024 columns, table of 30 522 rows: forward 41 us (134 MB written, 62 read at least: 4.8 TB/s), gradient 90: sort 25 (four launches),
 // walk 56 (212 MB: 3.8 TB/s; rows in order 47), join 8; every entry the same row: join 43. 777 float queries of 40 terms: forward 26, weights 22 (127 MB each
-// through the L2 and what lies behind), sort 30, walk 31, join 10. 32 fp16 queries of 40 terms 7 us.
+// through the L2 and what lies behind), sort 24, walk 31, join 10. 32 fp16 queries of 40 terms 7 us.
 #include <algorithm>
 
 #include "apoe_internal.h"
@@ -22,6 +22,7 @@ constexpr uint32_t EMBED_BLOCK = 32;     // entries that one group adds up, at m
 constexpr uint32_t SORT_TILE = 1024;     // entries that a workgroup of the sort ranks at a time
 constexpr uint32_t SORT_ONE = 4096;      // entries that one workgroup sorts by itself
 constexpr uint32_t SORT_TILES = 1024;    // workgroups of the sort, at most
+constexpr uint32_t ROW_STARTS = 2048;    // places where rows begin that a workgroup of the sort keeps in LDS
 constexpr uint32_t NO_ROW = 0xffffffffu;
 
 using f32x4e = float __attribute__((ext_vector_type(4)));
@@ -173,7 +174,15 @@ __global__ __launch_bounds__(256) void embed_count(EmbedArgs a, const uint2* fro
     n[threadIdx.x] = 0;
     __syncthreads();
     const uint64_t begin = (uint64_t)blockIdx.x * a.tile_entries, end = min(begin + a.tile_entries, (uint64_t)a.p.n_entries);
-    for (uint64_t e = begin + threadIdx.x; e < end; e += 256) atomicAdd(&n[(pair_of(a, from, e).x >> shift) & mask], 1u); // whole numbers: in any order
+    constexpr int U = SORT_TILE / 256;
+    for (uint64_t e = begin + threadIdx.x; e < end + threadIdx.x; e += SORT_TILE) {
+        uint32_t key[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) key[u] = pair_of(a, from, min(e + u * 256, end - 1)).x;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (e + u * 256 < end) atomicAdd(&n[(key[u] >> shift) & mask], 1u); // whole numbers: in any order
+    }
     __syncthreads();
     a.counts[blockIdx.x * 256 + threadIdx.x] = n[threadIdx.x];
 }
@@ -206,9 +215,26 @@ __device__ inline void scan256(uint32_t* total, int tid) {
     }
 }
 
+// Where rows begin, every 2^shift-th of them: what a search of them starts with. Searched in LDS, where a step waits for no memory (31 080
+// entries of 777 rows, the whole launch: 13.0 us with every step in memory, 8.2 so).
+__device__ inline uint32_t starts_shift(uint32_t n_rows) {
+    uint32_t s = 0;
+    while ((n_rows >> s) >= ROW_STARTS) s++;
+    return s;
+}
+template <int THREADS> __device__ inline void fill_starts(const EmbedArgs& a, uint32_t* starts, int tid) {
+    if (!a.p.off) return;
+    const uint32_t shift = starts_shift(a.p.n_rows);
+#pragma unroll
+    for (uint32_t k = 0; k < ROW_STARTS / THREADS; k++) {
+        const uint32_t i = k * THREADS + tid;
+        starts[i] = a.p.off[min(i << shift, a.p.n_rows - 1)];
+    }
+}
+
 // Each item's row, the last one that begins at or before it, and weight, to its place. The searches of all rounds go step by step together: a step waits for one
-// load, not for ROUNDS (17 120 entries of 428 rows, the whole launch: 13.3 us in turn, 11.3 together).
-template <int ROUNDS> __device__ inline void put_entries(const EmbedArgs& a, const uint2* item, const bool* in, const uint32_t* place) {
+// load, not for ROUNDS.
+template <int ROUNDS> __device__ inline void put_entries(const EmbedArgs& a, const uint2* item, const bool* in, const uint32_t* place, const uint32_t* starts) {
     uint32_t row[ROUNDS];
     float val[ROUNDS];
 #pragma unroll
@@ -217,10 +243,18 @@ template <int ROUNDS> __device__ inline void put_entries(const EmbedArgs& a, con
         val[r] = in[r] && a.p.val ? a.p.val[item[r].y] : 1.f;
     }
     if (a.p.off) {
-        const uint32_t n = a.p.n_rows;
+        const uint32_t n = a.p.n_rows, shift = starts_shift(n), last = (n - 1) >> shift;
 #pragma unroll
         for (int r = 0; r < ROUNDS; r++) row[r] = 0;
-        for (uint32_t step = n > 1 ? 1u << (31 - __builtin_clz(n - 1)) : 0; step; step >>= 1)
+        for (uint32_t step = ROW_STARTS / 2; step; step >>= 1)
+#pragma unroll
+            for (int r = 0; r < ROUNDS; r++) {
+                const uint32_t to = min(row[r] + step, last);
+                if (starts[to] <= item[r].y) row[r] = to;
+            }
+#pragma unroll
+        for (int r = 0; r < ROUNDS; r++) row[r] <<= shift;
+        for (uint32_t step = (1u << shift) >> 1; step; step >>= 1)
 #pragma unroll
             for (int r = 0; r < ROUNDS; r++) {
                 const uint32_t to = min(row[r] + step, n - 1); // off[to] of the last row says where that begins
@@ -228,7 +262,7 @@ template <int ROUNDS> __device__ inline void put_entries(const EmbedArgs& a, con
             }
 #pragma unroll
         for (int r = 0; r < ROUNDS; r++)
-            if (!(n && a.p.off[row[r]] <= item[r].y && item[r].y < a.p.off[row[r] + 1])) row[r] = NO_ROW;
+            if (!(a.p.off[row[r]] <= item[r].y && item[r].y < a.p.off[row[r] + 1])) row[r] = NO_ROW;
     }
 #pragma unroll
     for (int r = 0; r < ROUNDS; r++)
@@ -240,13 +274,20 @@ template <bool LAST> __global__ __launch_bounds__(256) void embed_place(EmbedArg
     constexpr int WAVES = 4, ROUNDS = SORT_TILE / (64 * WAVES);
     __shared__ uint32_t next[256], total[256];
     __shared__ uint32_t seen[WAVES][256]; // per wave: entries of a digit so far, then where its first one goes
+    __shared__ uint32_t starts[LAST ? ROW_STARTS : 1];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if constexpr (LAST) fill_starts<256>(a, starts, tid);
     uint32_t all = 0, before = 0;
-#pragma unroll 8
-    for (uint32_t t = 0; t < a.tiles; t++) {
-        const uint32_t n = a.counts[t * 256 + tid];
-        all += n;
-        before += t < blockIdx.x ? n : 0;
+    for (uint32_t t0 = 0; t0 < a.tiles; t0 += 16) { // sixteen loads at once, beyond the last tile that one again
+        uint32_t n[16];
+#pragma unroll
+        for (uint32_t u = 0; u < 16; u++) n[u] = a.counts[min(t0 + u, a.tiles - 1) * 256 + tid];
+#pragma unroll
+        for (uint32_t u = 0; u < 16; u++) {
+            const uint32_t c = t0 + u < a.tiles ? n[u] : 0;
+            all += c;
+            before += t0 + u < blockIdx.x ? c : 0;
+        }
     }
     total[tid] = all;
     __syncthreads();
@@ -279,7 +320,7 @@ template <bool LAST> __global__ __launch_bounds__(256) void embed_place(EmbedArg
             if constexpr (!LAST)
                 if (in[r]) to[rank[r]] = item[r];
         }
-        if constexpr (LAST) put_entries<ROUNDS>(a, item, in, rank);
+        if constexpr (LAST) put_entries<ROUNDS>(a, item, in, rank, starts);
         __syncthreads(); // the next tile clears the counts
     }
 }
@@ -290,8 +331,10 @@ __global__ __launch_bounds__(1024) void embed_sort(EmbedArgs a, uint32_t passes,
     __shared__ uint2 items[SORT_ONE];
     __shared__ uint32_t total[256];
     __shared__ uint32_t seen[WAVES][256];
+    __shared__ uint32_t starts[ROW_STARTS];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t n = a.p.n_entries, mask = (1u << width) - 1;
+    fill_starts<1024>(a, starts, tid); // (every pass has barriers between this and its use)
     uint2 item[ROUNDS];
     uint32_t rank[ROUNDS];
     bool in[ROUNDS];
@@ -327,7 +370,7 @@ __global__ __launch_bounds__(1024) void embed_sort(EmbedArgs a, uint32_t passes,
             rank[r] += seen[wave][(item[r].x >> shift) & mask];
             if (in[r] && !last) items[rank[r]] = item[r];
         }
-        if (last) put_entries<ROUNDS>(a, item, in, rank);
+        if (last) put_entries<ROUNDS>(a, item, in, rank, starts);
         __syncthreads();
     }
 }

@@ -579,8 +579,13 @@ __global__ __launch_bounds__(1024) void linear_bias(const float* part, uint32_t 
     const uint32_t c = threadIdx.x & 15, l = threadIdx.x >> 4, d = blockIdx.x * 16 + c;
     float s = 0.f;
     if (d < cols)
-#pragma unroll 4
-        for (uint32_t b = l; b < strips; b += 64) s += part[(uint64_t)b * cols + d];
+        for (uint32_t b0 = l; b0 < strips; b0 += 256) { // four loads at once, beyond the last strip that one again
+            float v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) v[u] = part[(uint64_t)min(b0 + u * 64, strips - 1) * cols + d];
+#pragma unroll
+            for (int u = 0; u < 4; u++) s += b0 + u * 64 < strips ? v[u] : 0.f;
+        }
     q[l][c] = s;
     for (uint32_t k = 32; k; k >>= 1) {
         __syncthreads();

@@ -166,8 +166,13 @@ __global__ __launch_bounds__(1024) void norm_vectors(NormArgs a) {
     if (!out) return;
     float s = 0.f;
     if (d < dim)
-#pragma unroll 4
-        for (uint32_t b = l; b < a.blocks; b += 64) s += a.part[((size_t)b * 2 + blockIdx.y) * dim + d];
+        for (uint32_t b0 = l; b0 < a.blocks; b0 += 512) { // eight loads at once, beyond the last row that one again
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) v[u] = a.part[((size_t)min(b0 + u * 64, a.blocks - 1) * 2 + blockIdx.y) * dim + d];
+#pragma unroll
+            for (int u = 0; u < 8; u++) s += b0 + u * 64 < a.blocks ? v[u] : 0.f;
+        }
     q[l][c] = s;
     for (uint32_t n = 32; n; n >>= 1) {
         __syncthreads();
