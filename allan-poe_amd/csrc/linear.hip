@@ -28,6 +28,12 @@ struct LinOut { // what becomes of a product's sums
     uint32_t m, n, act;
 };
 
+struct LinBias { // the bias' gradient, which workgroups behind the tiles' add up from the strips' sums
+    const float* part; // [strips][cols]
+    float* out;
+    uint32_t strips, cols;
+};
+
 struct LinTile {
     const void *a, *b;
     uint32_t a_pitch, b_pitch; // bytes
@@ -36,7 +42,9 @@ struct LinTile {
     uint32_t cuts, cut_stages;
     float* part;            // [cuts][m][np]
     uint32_t np;
+    uint32_t groups;        // of the product; workgroups behind them: the bias' gradient
     LinOut o;
+    LinBias bias;
 };
 
 // Phi(-u), the normal distribution's tail, for u >= 0, and its density there: exp(-u u / 2) times a polynomial in 1 / (1 + c u), fitted to
@@ -216,6 +224,28 @@ __device__ inline void tile_out(const LinTile& a, f32x16 (&acc)[MT][NT], char* l
     }
 }
 
+// Columns' sums over the strips: THREADS / 16 columns a workgroup, sixteen threads each, the same order whatever THREADS is.
+template <int THREADS> __device__ inline void bias_sums(const LinBias& a, uint32_t group, float* lds) {
+    constexpr uint32_t WIDE = THREADS / 16;
+    const uint32_t c = threadIdx.x % WIDE, l = threadIdx.x / WIDE, d = group * WIDE + c;
+    float s = 0.f;
+    if (d < a.cols)
+        for (uint32_t b0 = l; b0 < a.strips; b0 += 128) { // eight loads at once, beyond the last strip that one again
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) v[u] = a.part[(uint64_t)min(b0 + u * 16, a.strips - 1) * a.cols + d];
+#pragma unroll
+            for (int u = 0; u < 8; u++) s += b0 + u * 16 < a.strips ? v[u] : 0.f;
+        }
+    float* q = lds + l * (WIDE + 1) + c;
+    *q = s;
+    for (uint32_t k = 8; k; k >>= 1) {
+        __syncthreads();
+        if (l < k) *q += q[k * (WIDE + 1)];
+    }
+    if (l == 0 && d < a.cols) a.out[d] = *q;
+}
+
 // 16-bit matrices. ACOL, BCOL: the inner dimension goes down the rows.
 template <typename T, bool ACOL, bool BCOL, int MT, int NT, int WM, int WN, int KG, int SF, int ST>
 __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_tile(LinTile a) {
@@ -226,7 +256,11 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_tile(LinTile a) {
     __shared__ __align__(1024) char lds[ST * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / (WM * WN), wm = wave % (WM * WN) / WN, wn = wave % WN;
     const uint32_t m = a.o.m, n = a.o.n;
-    const uint32_t id = xcd_run(blockIdx.x, gridDim.x), tile = id / a.cuts, cut = id % a.cuts;
+    if (blockIdx.x >= a.groups) {
+        bias_sums<64 * NW>(a.bias, blockIdx.x - a.groups, reinterpret_cast<float*>(lds));
+        return;
+    }
+    const uint32_t id = xcd_run(blockIdx.x, a.groups), tile = id / a.cuts, cut = id % a.cuts;
     // an XCD's run of tiles is about as high as it is wide: it reads the fewest rows of both sides into its L2
     const uint32_t band = tile / (a.band * a.nt), in_band = tile % (a.band * a.nt), high = min(a.band, a.mt - band * a.band);
     const uint32_t row = (band * a.band + in_band % high) * BM, col = in_band / high * BN;
@@ -392,7 +426,11 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_tile32(LinTile a)
     __shared__ __align__(1024) char lds[ST * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / (WM * WN), wm = wave % (WM * WN) / WN, wn = wave % WN;
     const uint32_t m = a.o.m, n = a.o.n;
-    const uint32_t id = xcd_run(blockIdx.x, gridDim.x), tile = id / a.cuts, cut = id % a.cuts;
+    if (blockIdx.x >= a.groups) {
+        bias_sums<64 * NW>(a.bias, blockIdx.x - a.groups, reinterpret_cast<float*>(lds));
+        return;
+    }
+    const uint32_t id = xcd_run(blockIdx.x, a.groups), tile = id / a.cuts, cut = id % a.cuts;
     const uint32_t band = tile / (a.band * a.nt), in_band = tile % (a.band * a.nt), high = min(a.band, a.mt - band * a.band);
     const uint32_t row = (band * a.band + in_band % high) * BM, col = in_band / high * BN;
     const uint32_t s0 = cut * a.cut_stages, stages = min(a.cut_stages, (a.k + KE - 1) / KE - s0);
@@ -573,25 +611,9 @@ template <typename T> __global__ __launch_bounds__(256) void linear_pack(LinPack
         if (bx * 512 + c < a.cols) a.part[(uint64_t)strip * a.cols + bx * 512 + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
 }
 
-// Columns' sums over the strips: 16 columns a workgroup, 64 threads each.
-__global__ __launch_bounds__(1024) void linear_bias(const float* part, uint32_t strips, uint32_t cols, float* out) {
-    __shared__ float q[64][17];
-    const uint32_t c = threadIdx.x & 15, l = threadIdx.x >> 4, d = blockIdx.x * 16 + c;
-    float s = 0.f;
-    if (d < cols)
-        for (uint32_t b0 = l; b0 < strips; b0 += 256) { // four loads at once, beyond the last strip that one again
-            float v[4];
-#pragma unroll
-            for (int u = 0; u < 4; u++) v[u] = part[(uint64_t)min(b0 + u * 64, strips - 1) * cols + d];
-#pragma unroll
-            for (int u = 0; u < 4; u++) s += b0 + u * 64 < strips ? v[u] : 0.f;
-        }
-    q[l][c] = s;
-    for (uint32_t k = 32; k; k >>= 1) {
-        __syncthreads();
-        if (l < k) q[l][c] += q[l + k][c];
-    }
-    if (l == 0 && d < cols) out[d] = q[0][c];
+__global__ __launch_bounds__(512) void linear_bias(LinBias a) {
+    __shared__ float lds[16 * 33];
+    bias_sums<512>(a, blockIdx.x, lds);
 }
 
 // ---- host ----
@@ -691,23 +713,23 @@ template <typename T> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t
 static uint64_t cut_bytes(const LinShape& s, uint32_t m, uint32_t n) { return s.cuts > 1 ? (uint64_t)s.cuts * m * pitch_of(n) * 4 : 0; }
 
 template <typename T, bool ACOL, bool BCOL>
-static void product(apoe_ctx* ctx, const LinShape& s, LinOperand a, LinOperand b, uint32_t k, float* part, const LinOut& o) {
+static void product(apoe_ctx* ctx, const LinShape& s, LinOperand a, LinOperand b, uint32_t k, float* part, const LinOut& o, const LinBias& bias = {}) {
     const uint32_t mt = (o.m + s.bm - 1) / s.bm, nt = (o.n + s.bn - 1) / s.bn;
     uint32_t band = 1; // a power of two, so that runs end where bands do (8192 x 8192 x 4096: 444 us, row by row 482; 8192 x 1024 x 4096 67, 75)
     while (band * 2 <= mt && (uint64_t)band * band * 32 <= (uint64_t)mt * nt) band *= 2;
-    LinTile t{a.p, b.p, a.pitch, b.pitch, k, mt, nt, band, s.cuts, s.cut_stages, part, pitch_of(o.n), o};
-    const uint32_t grid = (uint32_t)((uint64_t)mt * nt * s.cuts);
+    LinTile t{a.p, b.p, a.pitch, b.pitch, k, mt, nt, band, s.cuts, s.cut_stages, part, pitch_of(o.n), (uint32_t)((uint64_t)mt * nt * s.cuts), o, bias};
+    const auto grid = [&](uint32_t threads) { return t.groups + (bias.out ? (bias.cols + threads / 16 - 1) / (threads / 16) : 0); };
     hipStream_t st = ctx->stream;
     if constexpr (sizeof(T) == 2) {
-        if (s.kind == 0) linear_tile<T, ACOL, BCOL, 4, 2, 2, 4, 1, 4, 2><<<grid, 512, 0, st>>>(t);
-        else if (s.kind == 1) linear_tile<T, ACOL, BCOL, 2, 2, 4, 2, 1, 4, 3><<<grid, 512, 0, st>>>(t);
-        else if (s.kind == 2) linear_tile<T, ACOL, BCOL, 2, 2, 2, 2, 1, 4, 2><<<grid, 256, 0, st>>>(t);
-        else if (s.kind == 3) linear_tile<T, ACOL, BCOL, 2, 2, 2, 2, 2, 4, 4><<<grid, 512, 0, st>>>(t);
-        else linear_tile<T, ACOL, BCOL, 1, 1, 2, 2, 1, 4, 4><<<grid, 256, 0, st>>>(t);
+        if (s.kind == 0) linear_tile<T, ACOL, BCOL, 4, 2, 2, 4, 1, 4, 2><<<grid(512), 512, 0, st>>>(t);
+        else if (s.kind == 1) linear_tile<T, ACOL, BCOL, 2, 2, 4, 2, 1, 4, 3><<<grid(512), 512, 0, st>>>(t);
+        else if (s.kind == 2) linear_tile<T, ACOL, BCOL, 2, 2, 2, 2, 1, 4, 2><<<grid(256), 256, 0, st>>>(t);
+        else if (s.kind == 3) linear_tile<T, ACOL, BCOL, 2, 2, 2, 2, 2, 4, 4><<<grid(512), 512, 0, st>>>(t);
+        else linear_tile<T, ACOL, BCOL, 1, 1, 2, 2, 1, 4, 4><<<grid(256), 256, 0, st>>>(t);
     } else {
-        if (s.kind == 0) linear_tile32<ACOL, BCOL, 4, 2, 2, 4, 1, 32, 2><<<grid, 512, 0, st>>>(t);
-        else if (s.kind == 1) linear_tile32<ACOL, BCOL, 2, 2, 2, 2, 2, 32, 4><<<grid, 512, 0, st>>>(t);
-        else linear_tile32<ACOL, BCOL, 2, 1, 1, 2, 4, 64, 4><<<grid, 512, 0, st>>>(t);
+        if (s.kind == 0) linear_tile32<ACOL, BCOL, 4, 2, 2, 4, 1, 32, 2><<<grid(512), 512, 0, st>>>(t);
+        else if (s.kind == 1) linear_tile32<ACOL, BCOL, 2, 2, 2, 2, 2, 32, 4><<<grid(512), 512, 0, st>>>(t);
+        else linear_tile32<ACOL, BCOL, 2, 1, 1, 2, 4, 64, 4><<<grid(512), 512, 0, st>>>(t);
     }
     if (s.cuts > 1) linear_join<T><<<(uint32_t)std::min<uint64_t>(((uint64_t)o.m * (t.np / 8) + 255) / 256, 1u << 16), 256, 0, st>>>(t);
 }
@@ -760,12 +782,13 @@ template <typename T> static int run_linear_grad(apoe_ctx* ctx, const apoe_linea
     if (p->grad_w) sw = choose<T>(ctx, n, k, m);
     LinPlan plan;
     const uint64_t o_g = plan.take(pack_g ? packed_bytes<T>(m, n) : 0), o_x = plan.take(x_is ? 0 : packed_bytes<T>(m, k)), o_w = plan.take(w_is ? 0 : packed_bytes<T>(n, k));
-    const uint64_t o_part = plan.take(std::max({p->grad_x ? cut_bytes(sx, m, k) : 0, p->grad_w ? cut_bytes(sw, n, k) : 0, p->grad_bias ? (uint64_t)LIN_STRIPS * n * 4 : 0}));
+    const uint64_t o_part = plan.take(std::max(p->grad_x ? cut_bytes(sx, m, k) : 0, p->grad_w ? cut_bytes(sw, n, k) : 0));
+    const uint64_t o_bias = plan.take(p->grad_bias ? (uint64_t)LIN_STRIPS * n * 4 : 0);
     char* ws = nullptr;
     if (plan.bytes) APOE_TRY(ctx->adapt_workspace(plan.bytes, &ws));
     LinOperand g{p->grad_y, (uint32_t)(p->grad_y_stride * sizeof(T))}, x{p->x, (uint32_t)(p->x_stride * sizeof(T))}, w{p->w, (uint32_t)(p->w_stride * sizeof(T))};
     LinPacks packs{};
-    uint32_t strips = 0;
+    LinBias bias{};
     if (pack_g || p->grad_bias) {
         LinPack& a = add_pack<T>(ctx, packs, p->grad_y, p->grad_y_stride, m, n, pack_g ? ws + o_g : nullptr);
         if (act) {
@@ -773,8 +796,10 @@ template <typename T> static int run_linear_grad(apoe_ctx* ctx, const apoe_linea
             a.pre_stride = p->pre_stride;
             a.act = p->act;
         }
-        if (p->grad_bias) a.part = (float*)(ws + o_part);
-        strips = a.strips;
+        if (p->grad_bias) {
+            a.part = (float*)(ws + o_bias);
+            bias = LinBias{a.part, p->grad_bias, a.strips, n};
+        }
         if (pack_g) g = LinOperand{ws + o_g, pitch_of(n) * (uint32_t)sizeof(T)};
     }
     if (!x_is) {
@@ -786,15 +811,15 @@ template <typename T> static int run_linear_grad(apoe_ctx* ctx, const apoe_linea
         add_pack<T>(ctx, packs, p->w, p->w_stride, n, k, ws + o_w);
     }
     pack<T>(ctx, packs);
-    if (p->grad_bias) linear_bias<<<(n + 15) / 16, 1024, 0, ctx->stream>>>((const float*)(ws + o_part), strips, n, p->grad_bias);
     if (p->grad_x && m) {
         LinOut o{p->grad_x, nullptr, nullptr, nullptr, p->grad_x_stride, 0, 0, m, k, APOE_ACT_NONE};
-        product<T, false, true>(ctx, sx, g, w, n, (float*)(ws + o_part), o);
+        product<T, false, true>(ctx, sx, g, w, n, (float*)(ws + o_part), o, p->grad_w ? LinBias{} : bias);
     }
     if (p->grad_w) {
         LinOut o{p->grad_w, nullptr, nullptr, nullptr, p->grad_w_stride, 0, 0, n, k, APOE_ACT_NONE};
-        product<T, true, true>(ctx, sw, g, x, m, (float*)(ws + o_part), o);
+        product<T, true, true>(ctx, sw, g, x, m, (float*)(ws + o_part), o, bias);
     }
+    if (p->grad_bias && !p->grad_w && !(p->grad_x && m)) linear_bias<<<(n + 31) / 32, 512, 0, ctx->stream>>>(bias);
     APOE_HIP(hipGetLastError());
     return APOE_OK;
 }
