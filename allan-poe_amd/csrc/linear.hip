@@ -387,6 +387,30 @@ template <int ROWS, int NW, int KE> struct RowTile32 { // inner index along the 
         return *reinterpret_cast<const f32x4*>(lds + (rb * 32 + row) * KE * 4 + (((2 * e + (lane >> 5)) ^ turn(row)) * 16));
     }
 };
+// The same for rows that begin at any value: a float a load. What a lane asks for in load i follows from load 0.
+template <int ROWS, int NW, int KE> struct RowTile32One : RowTile32<ROWS, NW, KE> {
+    using Whole = RowTile32<ROWS, NW, KE>;
+    static constexpr int LOADS = Whole::BYTES / (256 * NW), STEP = 64 * NW / KE; // STEP: rows from one load to the next
+    static_assert(NW == 8 && (KE == 32 || KE == 64), "a row's turn is that of load 0, with 64 inner indices turned by 8 more in every second load");
+    uint32_t first, place, step; // bytes: of the lane's row, in a row's stage, from one load to the next
+    int rows;                    // that are there, from load 0's on
+    __device__ void init(const float* row0, uint32_t pitch_bytes, int count, int wave, int lane) {
+        this->base = uniform64((uint64_t)row0);
+        const int l = wave * 64 + lane, row = l / KE, k = l % KE;
+        place = (uint32_t)(((k / 4) ^ Whole::turn(row)) * 16 + k % 4 * 4);
+        first = (uint32_t)row * pitch_bytes;
+        step = STEP * pitch_bytes;
+        rows = count - row;
+    }
+    __device__ void load(uint32_t lds, int left, int wave, int) const {
+        const i32x4 buffer = buffer_of(this->base);
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+            const uint32_t to = place ^ (KE == 64 && i & 1 ? 8 * 16 : 0);
+            load_to_lds4(buffer, i * STEP < rows && (int)to < left * 4 ? first + i * step + to : TILE_MASKED, lds + (i * NW + wave) * 256);
+        }
+    }
+};
 template <int COLS, int NW, int KE> struct ColTile32 { // inner index down the rows
     static constexpr int BYTES = COLS * KE * 4, LOADS = BYTES / (1024 * NW);
     static_assert(BYTES % (1024 * NW) == 0, "whole loads");
@@ -417,11 +441,12 @@ template <int COLS, int NW, int KE> struct ColTile32 { // inner index down the r
     }
 };
 
-template <bool ACOL, bool BCOL, int MT, int NT, int WM, int WN, int KG, int KE, int ST>
+// ONE: rows that begin at any value, on both sides.
+template <bool ACOL, bool BCOL, bool ONE, int MT, int NT, int WM, int WN, int KG, int KE, int ST>
 __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_tile32(LinTile a) {
     constexpr int NW = WM * WN * KG, BM = WM * MT * 32, BN = WN * NT * 32, FS = KE / 16 / KG;
-    using ATile = std::conditional_t<ACOL, ColTile32<BM, NW, KE>, RowTile32<BM, NW, KE>>;
-    using BTile = std::conditional_t<BCOL, ColTile32<BN, NW, KE>, RowTile32<BN, NW, KE>>;
+    using ATile = std::conditional_t<ACOL, ColTile32<BM, NW, KE>, std::conditional_t<ONE, RowTile32One<BM, NW, KE>, RowTile32<BM, NW, KE>>>;
+    using BTile = std::conditional_t<BCOL, ColTile32<BN, NW, KE>, std::conditional_t<ONE, RowTile32One<BN, NW, KE>, RowTile32<BN, NW, KE>>>;
     constexpr int STAGE = ATile::BYTES + BTile::BYTES, PER = ATile::LOADS + BTile::LOADS;
     __shared__ __align__(1024) char lds[ST * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave / (WM * WN), wm = wave % (WM * WN) / WN, wn = wave % WN;
@@ -625,10 +650,11 @@ struct LinOperand { // as the products take it
 
 constexpr uint32_t LIN_STRIPS = 256; // of rows under one partial sum of the bias' gradient, at most
 
-// Whether a matrix can be taken where it lies: 16 bytes a load, offsets of 256 rows in 31 bits.
+// Whether a matrix can be taken where it lies: offsets of 256 rows in 31 bits, and 16 bytes a load.
+template <typename T> static bool near_rows(uint64_t stride) { return stride * sizeof(T) <= (1u << 22); }
 template <typename T> static bool as_it_is(const void* p, uint64_t stride, uint32_t cols) {
     constexpr uint32_t E = 16 / sizeof(T);
-    return cols % E == 0 && stride % E == 0 && stride * sizeof(T) <= (1u << 22) && ((uintptr_t)p & 15) == 0;
+    return cols % E == 0 && stride % E == 0 && near_rows<T>(stride) && ((uintptr_t)p & 15) == 0;
 }
 
 struct LinPlan {
@@ -663,6 +689,7 @@ template <typename T> static void pack(apoe_ctx* ctx, LinPacks& all) {
 
 struct LinShape {
     uint32_t bm, bn, kind, cuts, cut_stages;
+    float us;
 };
 
 // Tiles and cuts, by what a product of each kind takes (us, fitted to fp16 and bf16 products of 256 to 8192 a side: a fixed part and one for each
@@ -697,7 +724,7 @@ template <typename T> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t
             if (cuts > 1) t += 3.f + (float)(cuts + 1) * (float)m * (float)n * 1e-6f; // 4 bytes at 4 TB/s
             if (t < least) {
                 least = t;
-                best = LinShape{kind.bm, kind.bn, number, std::max(1u, (stages + each - 1) / each), each};
+                best = LinShape{kind.bm, kind.bn, number, std::max(1u, (stages + each - 1) / each), each, t};
             }
         }
     };
@@ -712,7 +739,7 @@ template <typename T> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t
 
 static uint64_t cut_bytes(const LinShape& s, uint32_t m, uint32_t n) { return s.cuts > 1 ? (uint64_t)s.cuts * m * pitch_of(n) * 4 : 0; }
 
-template <typename T, bool ACOL, bool BCOL>
+template <typename T, bool ACOL, bool BCOL, bool ONE = false>
 static void product(apoe_ctx* ctx, const LinShape& s, LinOperand a, LinOperand b, uint32_t k, float* part, const LinOut& o, const LinBias& bias = {}) {
     const uint32_t mt = (o.m + s.bm - 1) / s.bm, nt = (o.n + s.bn - 1) / s.bn;
     uint32_t band = 1; // a power of two, so that runs end where bands do (8192 x 8192 x 4096: 444 us, row by row 482; 8192 x 1024 x 4096 67, 75)
@@ -727,9 +754,9 @@ static void product(apoe_ctx* ctx, const LinShape& s, LinOperand a, LinOperand b
         else if (s.kind == 3) linear_tile<T, ACOL, BCOL, 2, 2, 2, 2, 2, 4, 4><<<grid(512), 512, 0, st>>>(t);
         else linear_tile<T, ACOL, BCOL, 1, 1, 2, 2, 1, 4, 4><<<grid(256), 256, 0, st>>>(t);
     } else {
-        if (s.kind == 0) linear_tile32<ACOL, BCOL, 4, 2, 2, 4, 1, 32, 2><<<grid(512), 512, 0, st>>>(t);
-        else if (s.kind == 1) linear_tile32<ACOL, BCOL, 2, 2, 2, 2, 2, 32, 4><<<grid(512), 512, 0, st>>>(t);
-        else linear_tile32<ACOL, BCOL, 2, 1, 1, 2, 4, 64, 4><<<grid(512), 512, 0, st>>>(t);
+        if (s.kind == 0) linear_tile32<ACOL, BCOL, ONE, 4, 2, 2, 4, 1, 32, 2><<<grid(512), 512, 0, st>>>(t);
+        else if (s.kind == 1) linear_tile32<ACOL, BCOL, ONE, 2, 2, 2, 2, 2, 32, 4><<<grid(512), 512, 0, st>>>(t);
+        else linear_tile32<ACOL, BCOL, ONE, 2, 1, 1, 2, 4, 64, 4><<<grid(512), 512, 0, st>>>(t);
     }
     if (s.cuts > 1) linear_join<T><<<(uint32_t)std::min<uint64_t>(((uint64_t)o.m * (t.np / 8) + 255) / 256, 1u << 16), 256, 0, st>>>(t);
 }
@@ -749,8 +776,16 @@ template <typename T> static int run_linear(apoe_ctx* ctx, const apoe_linear_arg
         APOE_HIP(hipGetLastError());
         return APOE_OK;
     }
-    const bool x_is = as_it_is<T>(p->x, p->x_stride, k), w_is = as_it_is<T>(p->w, p->w_stride, k);
+    bool x_is = as_it_is<T>(p->x, p->x_stride, k), w_is = as_it_is<T>(p->w, p->w_stride, k);
     const LinShape s = choose<T>(ctx, m, n, k);
+    // Floats that begin anywhere: taken a float a load where that costs the product (a seventh more) less than laying them out anew costs, 5 us and the bytes
+    // (777 x 1001 x 999 26 us, laid out anew 31; 8191 x 4095 x 1001 388, 424; 4096 x 4095 x 4097 is laid out, 950, a float a load 978).
+    bool one = false;
+    if constexpr (sizeof(T) == 4) {
+        const float anew = 5.f + ((x_is ? 0.f : (float)m) + (w_is ? 0.f : (float)n)) * (float)k * 8.f / 4e6f;
+        one = !(x_is && w_is) && near_rows<T>(p->x_stride) && near_rows<T>(p->w_stride) && .15f * s.us < anew;
+        if (one) x_is = w_is = true;
+    }
     LinPlan plan;
     const uint64_t o_x = plan.take(x_is ? 0 : packed_bytes<T>(m, k)), o_w = plan.take(w_is ? 0 : packed_bytes<T>(n, k)), o_part = plan.take(cut_bytes(s, m, n));
     char* ws = nullptr;
@@ -767,7 +802,10 @@ template <typename T> static int run_linear(apoe_ctx* ctx, const apoe_linear_arg
     }
     pack<T>(ctx, packs);
     LinOut o{p->y, p->bias, p->residual, p->pre, p->y_stride, p->residual_stride, p->pre_stride, m, n, p->act};
-    product<T, false, false>(ctx, s, x, w, k, (float*)(ws + o_part), o);
+    if constexpr (sizeof(T) == 4) {
+        if (one) product<T, false, false, true>(ctx, s, x, w, k, (float*)(ws + o_part), o);
+    }
+    if (!one) product<T, false, false>(ctx, s, x, w, k, (float*)(ws + o_part), o);
     APOE_HIP(hipGetLastError());
     return APOE_OK;
 }
