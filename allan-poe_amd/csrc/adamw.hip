@@ -139,24 +139,38 @@ __device__ inline double share_of(double most, float top) {
     return most * r;
 }
 
-// The code of x >= 0 in a block whose largest is top: x = top (code / STEPS)^POWER, up where `chance` is below the share of the way from the code
-// beneath to the one above; inv: STEPS^POWER / top. The root is only an estimate: where it takes the code next to the right one, x lies
-// so close to that code that the share (below zero, or above one) leads to it all the same. A top that is not finite gives zero: the
-// block's values are its scale's.
-template <int POWER, int STEPS> __device__ inline int code_of(double x, double inv, uint32_t chance) {
-    const double w = x * inv;
-    const float r = __builtin_amdgcn_sqrtf((float)w), k = floorf(POWER == 2 ? r : __builtin_amdgcn_sqrtf(r)), square = k * k;
-    double above, gap; // what w is above its code, and the way to the next one: both from numbers that floats hold exactly
-    if constexpr (POWER == 2) {
-        above = w - (double)square;
-        gap = (double)__builtin_fmaf(2.f, k, 1.f);
-    } else {
-        above = __builtin_fma(-(double)square, (double)square, w);
-        gap = (double)__builtin_fmaf(2.f, k, 1.f) * (double)__builtin_fmaf(2.f, square + k, 1.f);
+// The code of w = STEPS^POWER x / top >= 0: k, the last one at or below w, or k + 1 where `chance` is below the share of the way between them that w has gone. k comes from
+// a root in 32 bits that is taken a little too large: it is the right one or, seldom, the next, with w below it; whoever calls looks for that. The block's largest
+// counts as on its way to the last code: rounded to a float it can be larger than it was. A top that is not finite gives zero: the block's values are its scale's.
+template <int POWER, int STEPS> struct Code {
+    float k;
+    double above; // of w, above k
+    __device__ void reach(double w) {
+        const float square = k * k; // a whole number that a float holds, as is all of the gap
+        if constexpr (POWER == 2) above = w - (double)square;
+        else above = __builtin_fma(-(double)square, (double)square, w);
     }
-    const double u = __builtin_fma((double)chance, 0x1p-32, 0x1p-33);
-    return min((int)k + (u * gap < above ? 1 : 0), STEPS);
-}
+    __device__ void guess(double w) {
+        float r = __builtin_amdgcn_sqrtf((float)w);
+        if constexpr (POWER == 4) r = __builtin_amdgcn_sqrtf(r);
+        k = floorf(__builtin_fmaf(r, 0x1p-21f, r));
+        k = k >= (float)STEPS ? (float)(STEPS - 1) : k;
+        reach(w);
+    }
+    __device__ void correct(double w) {
+        if (above < 0.) {
+            k -= 1.f;
+            reach(w);
+        }
+    }
+    __device__ uint32_t sign() const { return (uint32_t)(__builtin_bit_cast(uint64_t, above) >> 32); }
+    __device__ int take(uint32_t chance) const {
+        double gap = (double)__builtin_fmaf(2.f, k, 1.f);
+        if constexpr (POWER == 4) gap *= (double)__builtin_fmaf(2.f, __builtin_fmaf(k, k, k), 1.f);
+        const double u = __builtin_fma((double)chance, 0x1p-32, 0x1p-33);
+        return (int)k + (u * gap < above ? 1 : 0);
+    }
+};
 
 // What a lane needs of a block, as it comes: nothing here waits for a load.
 template <int BITS> struct AdamRaw {
@@ -275,10 +289,26 @@ template <int BITS, bool NEAR> __global__ __launch_bounds__(256) void adamw_step
             const uint32_t bk = mix(mix(key ^ (uint32_t)block) ^ (uint32_t)(block >> 32));
             int8_t cm[4];
             uint8_t cv[4];
+            Code<2, 127> xm[4];
+            Code<4, 255> xv[4];
+            uint32_t below = 0; // whether a guess is above its number: one in some 20 000, so that a wave seldom has any
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                xm[k].guess(fabs(md[k]) * im);
+                xv[k].guess(vd[k] * iv);
+                below |= xm[k].sign() | xv[k].sign();
+            }
+            if (__builtin_expect(__ballot((int32_t)below < 0) != 0, 0)) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    xm[k].correct(fabs(md[k]) * im);
+                    xv[k].correct(vd[k] * iv);
+                }
+            }
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const uint32_t i = place(whole, lane, k);
-                const int c = code_of<2, 127>(fabs(md[k]), im, mix(bk + 2 * i)), r = code_of<4, 255>(vd[k], iv, mix(bk + 2 * i + 1));
+                const int c = xm[k].take(mix(bk + 2 * i)), r = xv[k].take(mix(bk + 2 * i + 1));
                 cm[k] = (int8_t)(md[k] < 0. ? -c : c);
                 cv[k] = (uint8_t)(vd[k] > 0. ? max(r, 1) : 0);
             }

@@ -301,3 +301,47 @@ def test_arrays_that_share_memory_are_refused(gpu_ctx):
         with pytest.raises(apoe.ApoeError, match="share memory"):
             apoe.AdamW(gpu_ctx, params, copies=copies)
     apoe.AdamW(gpu_ctx, [store[:600], store[600:]])
+
+
+def test_codes_next_to_a_step_of_the_list(gpu_ctx):
+    """Chances next to one, for numbers just below a code (or a block's largest, rounded up to a float): they go to the code beneath where the chance is above the
+    share, however near both are to one. Of 2^24 values those with such a chance are taken, each with the first or the second moment at a step's end."""
+    import torch
+    import apoe
+    n, seed = 1 << 24, 5
+    lists = ((torch.arange(128).double() / 127) ** 2, (torch.arange(256).double() / 255) ** 4)
+    g = torch.Generator().manual_seed(3)
+    grads = torch.zeros(n)
+    blocks = []
+    chance = [chances(seed, 1, 0, n, which) for which in (0, 1)]
+    for which in (0, 1):
+        places = (chance[which] > 1 - 4e-6).nonzero().flatten().tolist()
+        assert len(places) > 30
+        for at in places:
+            block = at // 256
+            if block in blocks:
+                continue
+            blocks.append(block)
+            if len(blocks) % 2:  # alone in its block: its largest
+                grads[at] = torch.randn(1, generator=g)[0]
+                continue
+            grads[block * 256 + (at + 1) % 256] = top = float(torch.rand(1, generator=g) + 0.5)
+            k = int(torch.randint(20, len(lists[which]) - 1, (1,), generator=g))
+            x = top * float(lists[which][k]) ** (1.0 if which == 0 else 0.5)
+            grads[at] = torch.nextafter(torch.tensor(x), torch.tensor(0.0))
+    at = (torch.tensor(blocks)[:, None] * 256 + torch.arange(256)).flatten()
+    x = grads[at].double()
+    _, m, v, _ = step64(0.0, x, torch.zeros_like(x), torch.zeros_like(x), 1, 0.0, 1.0)
+    opt = apoe.AdamW(gpu_ctx, [torch.zeros(n, device="cuda")], bits=8, betas=BETAS, eps=EPS, seed=seed)
+    opt.step([grads.cuda()], LR)
+    state = {k: t.cpu() for k, t in opt.state().items() if k != "t"}
+    below = 0
+    for name, value, list_, which in (("m", m.abs(), lists[0], 0), ("v", v, lists[1], 1)):
+        code, top, near = coded(value, list_, chance[which][at], which == 1)
+        got = state[name][at].long().abs()
+        assert bool((state[name + "_scale"][torch.tensor(blocks)] == top).all())
+        bad = (got != code) & (near > 1e-9)
+        assert not bool(bad.any()), (name, int(bad.sum()), got[bad].tolist(), code[bad].tolist(), near[bad].tolist())
+        t = top.double().repeat_interleave(256)
+        below += int(((value > 0) & (chance[which][at] > 1 - 4e-6) & (list_[code] * t < value)).sum())
+    assert below > 5  # numbers that stay beneath the next code, against nearly all chances
