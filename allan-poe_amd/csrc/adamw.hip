@@ -9,9 +9,9 @@
 // thousandth a step would stand still if it were rounded to the nearest code, so it goes up or down by chance, with the probability that keeps
 // its mean in m and in v. What is above a code is a difference of two close numbers, and the comparison with the chance decides a
 // code: both in 64 bits, at the same rate as 32 on this GPU's vector units.
-// Measured: 132 M values in twelve layers and a table, 32 bits 711 us for 3.7 GB (5.2 TB/s); 8 bits 536 us for 2.1 GB (4.0 TB/s): 125 vector instructions a value, which
-// keep the units busy in 78 % of the cycles (deciding the codes in 32 bits with 64 as a fallback took 719); reading the moments back 295 us for
-// 1.3 GB. 8.4 M values in 32 bits 50 us (4.7 TB/s).
+// Measured: 132 M values in twelve layers and a table, 32 bits 711 us for 3.7 GB (5.2 TB/s); 8 bits 571 us for 2.1 GB (3.7 TB/s): 140 vector instructions a value, which
+// keep the units busy in nine cycles of ten (guesses that may be off at a code's very end 536; deciding the codes in 32 bits with 64 as a fallback 719); reading
+// the moments back 297 us for 1.3 GB. 8.4 M values in 32 bits 50 us (4.7 TB/s).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -145,30 +145,28 @@ __device__ inline double share_of(double most, float top) {
 template <int POWER, int STEPS> struct Code {
     float k;
     double above; // of w, above k
-    __device__ void reach(double w) {
-        const float square = k * k; // a whole number that a float holds, as is all of the gap
-        if constexpr (POWER == 2) above = w - (double)square;
-        else above = __builtin_fma(-(double)square, (double)square, w);
+    __device__ double gap() const { // from k to the next: of numbers that floats hold, as k k is
+        const double g = (double)__builtin_fmaf(2.f, k, 1.f);
+        return POWER == 2 ? g : g * (double)__builtin_fmaf(2.f, __builtin_fmaf(k, k, k), 1.f);
     }
     __device__ void guess(double w) {
         float r = __builtin_amdgcn_sqrtf((float)w);
         if constexpr (POWER == 4) r = __builtin_amdgcn_sqrtf(r);
         k = floorf(__builtin_fmaf(r, 0x1p-21f, r));
         k = k >= (float)STEPS ? (float)(STEPS - 1) : k;
-        reach(w);
+        const double square = (double)(k * k);
+        above = POWER == 2 ? w - square : __builtin_fma(-square, square, w);
     }
-    __device__ void correct(double w) {
+    __device__ void correct() {
         if (above < 0.) {
             k -= 1.f;
-            reach(w);
+            above += gap();
         }
     }
     __device__ uint32_t sign() const { return (uint32_t)(__builtin_bit_cast(uint64_t, above) >> 32); }
     __device__ int take(uint32_t chance) const {
-        double gap = (double)__builtin_fmaf(2.f, k, 1.f);
-        if constexpr (POWER == 4) gap *= (double)__builtin_fmaf(2.f, __builtin_fmaf(k, k, k), 1.f);
         const double u = __builtin_fma((double)chance, 0x1p-32, 0x1p-33);
-        return (int)k + (u * gap < above ? 1 : 0);
+        return (int)k + (u * gap() < above ? 1 : 0);
     }
 };
 
@@ -289,29 +287,23 @@ template <int BITS, bool NEAR> __global__ __launch_bounds__(256) void adamw_step
             const uint32_t bk = mix(mix(key ^ (uint32_t)block) ^ (uint32_t)(block >> 32));
             int8_t cm[4];
             uint8_t cv[4];
-            Code<2, 127> xm[4];
-            Code<4, 255> xv[4];
-            uint32_t below = 0; // whether a guess is above its number: one in some 20 000, so that a wave seldom has any
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                xm[k].guess(fabs(md[k]) * im);
-                xv[k].guess(vd[k] * iv);
-                below |= xm[k].sign() | xv[k].sign();
-            }
-            if (__builtin_expect(__ballot((int32_t)below < 0) != 0, 0)) {
+            const auto codes = [&](auto code, const double* x, double inv, uint32_t which, auto&& put) { // the codes of four numbers without their signs
+                decltype(code) c[4];
+                uint32_t below = 0; // whether a guess is above its number: one in some 20 000, so that a wave seldom has any
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    xm[k].correct(fabs(md[k]) * im);
-                    xv[k].correct(vd[k] * iv);
+                    c[k].guess(fabs(x[k]) * inv);
+                    below |= c[k].sign();
                 }
-            }
+                if (__builtin_expect(__ballot((int32_t)below < 0) != 0, 0)) {
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const uint32_t i = place(whole, lane, k);
-                const int c = xm[k].take(mix(bk + 2 * i)), r = xv[k].take(mix(bk + 2 * i + 1));
-                cm[k] = (int8_t)(md[k] < 0. ? -c : c);
-                cv[k] = (uint8_t)(vd[k] > 0. ? max(r, 1) : 0);
-            }
+                    for (int k = 0; k < 4; k++) c[k].correct();
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) put(k, c[k].take(mix(bk + 2 * place(whole, lane, k) + which)));
+            };
+            codes(Code<2, 127>{}, md, im, 0, [&](int k, int c) { cm[k] = (int8_t)(md[k] < 0. ? -c : c); });
+            codes(Code<4, 255>{}, vd, iv, 1, [&](int k, int c) { cv[k] = (uint8_t)(vd[k] > 0. ? max(c, 1) : 0); });
             store4((int8_t*)t.m, cm, at, whole, lane, left);
             store4((uint8_t*)t.v, cv, at, whole, lane, left);
             if (lane == 0) {
