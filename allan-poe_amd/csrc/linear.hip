@@ -3,8 +3,8 @@
 //
 // Three products of one kernel: an operand's inner dimension goes along its rows (x, w, and gz for gx) or down them (w for gx, both for gw; read
 // transposed from LDS). Float matrices go through the bfloat16 units: a wave takes each value of its operands apart into three parts of eight bits as it comes from LDS, and of
-// the nine products the six that count are added up: as accurate value by value as float products, whatever the exponents are, at a sixth of
-// 1400 TFLOP/s where the float matrix units have 154. What is done to a result (bias, activation, residual, rounding) is done behind the last stage,
+// the nine products the six that count are added up: as accurate value by value as float products, for values of any size from 2^-111 on (the
+// last part of smaller ones ends at 2^-133), at a sixth of 1400 TFLOP/s where the float matrix units have 154. What is done to a result (bias, activation, residual, rounding) is done behind the last stage,
 // through LDS, 16 bytes a thread. Where tiles are too few for the GPU the inner dimension is cut and a second launch adds the cuts up, in order.
 // Up to 16 rows a kernel of its own streams w once (the serving form).
 // Measured (a library product of 8192 x 8192 x 8192 in bf16 runs at 1470 TFLOP/s, of 8192 x 4096 x 1024 at 1160): 8192 x 4096 x 1024 bf16 73 us (940 TFLOP/s), with GELU and
