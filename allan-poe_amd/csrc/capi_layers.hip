@@ -26,6 +26,9 @@ int check_pointer(const apoe_ctx* ctx, const void* p, size_t align, const char* 
     if ((s) == 0) (s) = (cols); \
     APOE_REQUIRE((s) >= (cols), "rows overlap: stride %llu for %u columns", (unsigned long long)(s), (cols))
 
+// What is written while `q` is still read, or written by others. (Matrices may share a buffer, side by side: only the same beginning is refused.)
+#define APOE_APART(p, q) APOE_REQUIRE(!(p) || (const void*)(p) != (const void*)(q), #p " and " #q " are the same memory")
+
 int embed(apoe_ctx* ctx, const apoe_embed_args* args, bool grad) {
     APOE_REQUIRE(ctx && args, "ctx/args is null");
     apoe_embed_args a = *args;
@@ -66,6 +69,10 @@ int embed(apoe_ctx* ctx, const apoe_embed_args* args, bool grad) {
     APOE_POINTER(a.grad, e, "grad");
     APOE_POINTER(a.grad_table, e, "grad_table");
     APOE_POINTER(a.grad_val, 4, "grad_val");
+    APOE_APART(a.out, a.table);
+    APOE_APART(a.grad_table, a.grad);
+    APOE_APART(a.grad_table, a.table);
+    if (grad) APOE_APART(a.grad_val, a.val);
     APOE_HIP(hipSetDevice(ctx->device));
     return launch_embed(ctx, &a, grad);
 }
@@ -143,10 +150,21 @@ int linear(apoe_ctx* ctx, const apoe_linear_args* args, bool grad) {
         APOE_POINTER(a.grad_x, e, "grad_x");
         APOE_POINTER(a.grad_w, e, "grad_w");
         APOE_POINTER(a.grad_bias, 4, "grad_bias");
+        for (const void* in : {a.grad_y, a.act == APOE_ACT_NONE ? nullptr : (const void*)a.pre, a.x, a.w}) {
+            APOE_APART(a.grad_x, in);
+            APOE_APART(a.grad_w, in);
+        }
+        APOE_APART(a.grad_x, a.grad_w);
     } else {
         APOE_POINTER(a.bias, 4, "bias");
         APOE_POINTER(a.residual, e, "residual");
         APOE_POINTER(a.y, e, "y");
+        for (const void* in : {a.x, a.w}) {
+            APOE_APART(a.y, in);
+            APOE_APART(a.pre, in);
+        }
+        APOE_APART(a.y, a.pre);
+        APOE_APART(a.pre, a.residual);
     }
     APOE_HIP(hipSetDevice(ctx->device));
     return launch_linear(ctx, &a, grad);
