@@ -5,7 +5,8 @@
 // transposed from LDS). Float matrices go through the bfloat16 units: a wave takes each value of its operands apart into three parts of eight bits as it comes from LDS, and of
 // the nine products the six that count are added up: as accurate value by value as float products, for values of any size from 2^-111 on (the
 // last part of smaller ones ends at 2^-133), at a sixth of 1400 TFLOP/s where the float matrix units have 154. What is done to a result (bias, activation, residual, rounding) is done behind the last stage,
-// through LDS, 16 bytes a thread. Where tiles are too few for the GPU the inner dimension is cut and a second launch adds the cuts up, in order.
+// through LDS, 16 bytes a thread. gz of 16-bit matrices with GELU or SiLU has more bits than their type: it is multiplied as two parts, which costs its two products
+// twice their operations (rounded to one, gx and gw would be off by 1.4 times their own rounding). Where tiles are too few for the GPU the inner dimension is cut and a second launch adds the cuts up, in order.
 // Up to 16 rows a kernel of its own streams w once (the serving form).
 // Measured (a library product of 8192 x 8192 x 8192 in bf16 runs at 1470 TFLOP/s, of 8192 x 4096 x 1024 at 1160): 8192 x 4096 x 1024 bf16 73 us (940 TFLOP/s), with GELU and
 // both outputs 99, whose operations cost what the products wait for; 8192 x 1024 x 4096 68 (1010); 4096 x 1024 x 8192, both sides transposed, 76 (900); 8192 x 4096 x
@@ -45,6 +46,17 @@ struct LinTile {
     uint32_t groups;        // of the product; workgroups behind them: the bias' gradient
     LinOut o;
     LinBias bias;
+    uint64_t second;        // bytes from a to its second part (0: it has one)
+    bool a_down, b_down;    // the inner dimension goes down the rows
+};
+
+// gz of 16-bit matrices with GELU or SiLU, which its type does not hold, as two parts: its rounding, and the rounding of what that leaves. (What ReLU lets back is a value of grad_y.) float16
+// holds halves, so that no slope above one makes an infinity, and the second part times 2^11, so that it does not fall below the smallest numbers.
+template <typename T> struct Two {
+    static constexpr float HALF = 1.f, DOWN = 1.f;
+};
+template <> struct Two<_Float16> {
+    static constexpr float HALF = 0.5f, DOWN = 0x1p-11f;
 };
 
 // Phi(-u), the normal distribution's tail, for u >= 0, and its density there: exp(-u u / 2) times a polynomial in 1 / (1 + c u), fitted to
@@ -176,10 +188,34 @@ template <typename T> __device__ inline void finish1(const LinOut& o, uint32_t i
     ((T*)o.out)[i * o.out_stride + j] = (T)z;
 }
 
+__device__ inline bool is_finite(float v) { return fabsf(v) < INFINITY; }
+
+// Sum (i, j) once more, one product after the other: of an a in two parts, whose second is zero beside an infinity (zero times infinity would be NaN). Sums that are not finite come here.
+template <typename T> __device__ inline float sum_again(const LinTile& a, uint32_t i, uint32_t j) {
+    const char* pa = (const char*)a.a + (a.a_down ? i * sizeof(T) : (uint64_t)i * a.a_pitch);
+    const char* pb = (const char*)a.b + (a.b_down ? j * sizeof(T) : (uint64_t)j * a.b_pitch);
+    const uint64_t sa = a.a_down ? a.a_pitch : sizeof(T), sb = a.b_down ? a.b_pitch : sizeof(T);
+    float s = 0.f;
+    for (uint64_t k = 0; k < a.k && s == s; k++) {
+        const float hi = (float)*(const T*)(pa + k * sa), lo = (float)*(const T*)(pa + k * sa + a.second);
+        s = __builtin_fmaf(__builtin_fmaf(lo, Two<T>::DOWN, hi) / Two<T>::HALF, (float)*(const T*)(pb + k * sb), s);
+    }
+    return s;
+}
+template <typename T> __device__ inline void make_sums_again(const LinTile& a, uint32_t i, uint32_t j, float* v) {
+    bool all = true;
+#pragma unroll
+    for (int k = 0; k < 8; k++) all &= is_finite(v[k]);
+    if (__builtin_expect(all, 1)) return;
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+        if (!is_finite(v[k]) && j + k < a.o.n) v[k] = sum_again<T>(a, i, j + k);
+}
+
 // (ADD: groups of waves hold parts of every sum; otherwise each group has whole ones of its share of the blocks.)
 // What the waves hold goes out: one block of 32 rows a wave at a time through LDS, then a thread has eight values of a row. Waits between are for LDS alone: the
 // stores of the block before are on their way meanwhile.
-template <typename T, int MT, int NT, int WM, int WN, int KG, int BYTES, bool ADD = false>
+template <typename T, int MT, int NT, int WM, int WN, int KG, int BYTES, bool ADD = false, bool TWO = false>
 __device__ inline void tile_out(const LinTile& a, f32x16 (&acc)[MT][NT], char* lds, uint32_t row, uint32_t col, uint32_t cut, int kg, int wm, int wn, int lane) {
     constexpr int NW = WM * WN * KG, BN = WN * NT * 32, PITCH = BN + 4, ROWS = WM * 32, ITEMS = (ROWS * BN / 8 + 64 * NW - 1) / (64 * NW);
     static_assert(ROWS * PITCH * 4 <= BYTES, "the sums fit the stages");
@@ -217,6 +253,7 @@ __device__ inline void tile_out(const LinTile& a, f32x16 (&acc)[MT][NT], char* l
                 *reinterpret_cast<f32x4*>(to + 4) = v1;
             } else {
                 float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                if constexpr (TWO) make_sums_again<T>(a, gi, gj, v);
                 finish8<T>(a.o, gi, gj, v);
             }
         }
@@ -246,8 +283,8 @@ template <int THREADS> __device__ inline void bias_sums(const LinBias& a, uint32
     if (l == 0 && d < a.cols) a.out[d] = *q;
 }
 
-// 16-bit matrices. ACOL, BCOL: the inner dimension goes down the rows.
-template <typename T, bool ACOL, bool BCOL, int MT, int NT, int WM, int WN, int KG, int SF, int ST>
+// 16-bit matrices. ACOL, BCOL: the inner dimension goes down the rows. TWO: a has two parts; all of the second's products are added up in front of the first's.
+template <typename T, bool ACOL, bool BCOL, bool TWO, int MT, int NT, int WM, int WN, int KG, int SF, int ST>
 __device__ inline void one_tile(const LinTile& a, uint32_t block, char* lds) {
     constexpr int NW = WM * WN * KG, FS = SF / KG, BM = WM * MT * 32, BN = WN * NT * 32;
     using ATile = std::conditional_t<ACOL, ColTile<T, BM, SF, NW, ORDER_ROWS>, RowTile<T, BM, SF, NW>>;
@@ -267,14 +304,17 @@ __device__ inline void one_tile(const LinTile& a, uint32_t block, char* lds) {
     const int mrows = (int)min((uint32_t)BM, m - row), ncols = (int)min((uint32_t)BN, n - col);
     ATile ta;
     BTile tb;
-    const char *pa = (const char*)a.a, *pb = (const char*)a.b;
+    const char *pa = (const char*)a.a + (TWO ? a.second : 0), *pb = (const char*)a.b;
     if constexpr (ACOL) ta.init((const T*)(pa + (uint64_t)s0 * KE * a.a_pitch) + row, a.a_pitch, (mrows + 7) / 8 * 8, wave, lane);
     else ta.init((const T*)(pa + (uint64_t)row * a.a_pitch) + (uint64_t)s0 * KE, a.a_pitch, mrows, wave, lane);
     if constexpr (BCOL) tb.init((const T*)(pb + (uint64_t)s0 * KE * a.b_pitch) + col, a.b_pitch, (ncols + 7) / 8 * 8, wave, lane);
     else tb.init((const T*)(pb + (uint64_t)col * a.b_pitch) + (uint64_t)s0 * KE, a.b_pitch, ncols, wave, lane);
     const uint32_t base = lds_address(lds);
-    int left = (int)min(stages * KE, a.k - s0 * KE); // of the inner side; a row's values are followed by zeros up to a multiple of eight
+    const int inner = (int)min(stages * KE, a.k - s0 * KE); // a row's values are followed by zeros up to a multiple of eight
+    int left = inner;
     uint32_t into = 0;
+    const uint64_t first_a = uniform64(ta.base - a.second), first_b = tb.base;
+    int more = 1;
     auto issue = [&]() {
         const auto one = [&](auto& t, uint32_t at, auto down) {
             if constexpr (decltype(down)::value) {
@@ -288,55 +328,74 @@ __device__ inline void one_tile(const LinTile& a, uint32_t block, char* lds) {
         one(ta, base + into, std::integral_constant<bool, ACOL>{});
         one(tb, base + into + ATile::BYTES, std::integral_constant<bool, BCOL>{});
         left -= KE;
+        if constexpr (TWO) { // (selections: a branch would end the block whose order is given below)
+            const bool turn = left < more; // more: 1, then a number that left never is below
+            ta.base = turn ? first_a : ta.base;
+            tb.base = turn ? first_b : tb.base;
+            left = turn ? inner : left;
+            more = turn ? INT32_MIN : more;
+        }
         into = into + STAGE == ST * STAGE ? 0 : into + STAGE;
     };
 #pragma unroll
     for (int s = 0; s < ST - 1; s++) issue();
     f32x16 acc[MT][NT] = {};
     uint32_t from = 0;
-    for (uint32_t s = 0; s < stages; s++) {
-        tile_wait<(ST - 2) * PER>();
-        const char* A = lds + from;
-        const char* B = A + ATile::BYTES;
-        i32x4 x[2][MT], y[2][NT];
-        auto read = [&](int f) {
-#pragma unroll
-            for (int i = 0; i < MT; i++) x[f & 1][i] = ATile::read(A, wm * MT + i, kg * FS + f, lane);
-#pragma unroll
-            for (int t = 0; t < NT; t++) y[f & 1][t] = BTile::read(B, wn * NT + t, kg * FS + f, lane);
-        };
-        read(0);
-        issue();
-#pragma unroll
-        for (int f = 0; f < FS; f++) {
-            if (f + 1 < FS) read(f + 1);
+    const auto scale = [&](float by) {
+        if constexpr (Two<T>::HALF != 1.f)
 #pragma unroll
             for (int i = 0; i < MT; i++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) acc[i][t] = mfma_step<T>(x[f & 1][i], y[f & 1][t], acc[i][t]);
+                for (int t = 0; t < NT; t++) acc[i][t] *= by;
+    };
+#pragma unroll 1
+    for (int part = 0; part < (TWO ? 2 : 1); part++) {
+        if (part) scale(Two<T>::DOWN);
+        for (uint32_t s = 0; s < stages; s++) {
+            tile_wait<(ST - 2) * PER>();
+            const char* A = lds + from;
+            const char* B = A + ATile::BYTES;
+            i32x4 x[2][MT], y[2][NT];
+            auto read = [&](int f) {
+#pragma unroll
+                for (int i = 0; i < MT; i++) x[f & 1][i] = ATile::read(A, wm * MT + i, kg * FS + f, lane);
+#pragma unroll
+                for (int t = 0; t < NT; t++) y[f & 1][t] = BTile::read(B, wn * NT + t, kg * FS + f, lane);
+            };
+            read(0);
+            issue();
+#pragma unroll
+            for (int f = 0; f < FS; f++) {
+                if (f + 1 < FS) read(f + 1);
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int t = 0; t < NT; t++) acc[i][t] = mfma_step<T>(x[f & 1][i], y[f & 1][t], acc[i][t]);
+            }
+            interleave<(ACOL ? 2 : 1) * MT + (BCOL ? 2 : 1) * NT, MT * NT, FS>();
+            from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
         }
-        interleave<(ACOL ? 2 : 1) * MT + (BCOL ? 2 : 1) * NT, MT * NT, FS>();
-        from = from + STAGE == ST * STAGE ? 0 : from + STAGE;
     }
+    if constexpr (TWO) scale(1.f / Two<T>::HALF);
     tile_wait<0>();
     if constexpr (KG == 2) {
         static_assert(BM * BN * 4 <= ST * STAGE, "the sums fit the stages");
         exchange_halves<MT, NT, WM * WN>(acc, lds, kg, wave % (WM * WN), lane);
         __syncthreads();
     }
-    tile_out<T, MT, NT, WM, WN, KG, ST * STAGE>(a, acc, lds, row, col, cut, kg, wm, wn, lane);
+    tile_out<T, MT, NT, WM, WN, KG, ST * STAGE, false, TWO>(a, acc, lds, row, col, cut, kg, wm, wn, lane);
 }
 
-template <typename T, bool ACOL, bool BCOL, int MT, int NT, int WM, int WN, int KG, int SF, int ST> __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_tile(LinTile a) {
+template <typename T, bool ACOL, bool BCOL, bool TWO, int MT, int NT, int WM, int WN, int KG, int SF, int ST> __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_tile(LinTile a) {
     __shared__ __align__(1024) char lds[ST * (WM * MT + WN * NT) * 32 * SF * 32];
-    one_tile<T, ACOL, BCOL, MT, NT, WM, WN, KG, SF, ST>(a, blockIdx.x, lds);
+    one_tile<T, ACOL, BCOL, TWO, MT, NT, WM, WN, KG, SF, ST>(a, blockIdx.x, lds);
 }
 
 // gx = gz w and gw = gz^T x in one launch (gx may have no workgroups): neither waits for the other's last tiles.
-template <typename T, int MT, int NT, int WM, int WN, int KG, int SF, int ST> __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_grads(LinTile x, LinTile w) {
+template <typename T, bool TWO, int MT, int NT, int WM, int WN, int KG, int SF, int ST> __global__ __launch_bounds__(64 * WM * WN * KG, 2) void linear_grads(LinTile x, LinTile w) {
     __shared__ __align__(1024) char lds[ST * (WM * MT + WN * NT) * 32 * SF * 32];
-    if (blockIdx.x < x.groups) one_tile<T, false, true, MT, NT, WM, WN, KG, SF, ST>(x, blockIdx.x, lds);
-    else one_tile<T, true, true, MT, NT, WM, WN, KG, SF, ST>(w, blockIdx.x - x.groups, lds);
+    if (blockIdx.x < x.groups) one_tile<T, false, true, TWO, MT, NT, WM, WN, KG, SF, ST>(x, blockIdx.x, lds);
+    else one_tile<T, true, true, TWO, MT, NT, WM, WN, KG, SF, ST>(w, blockIdx.x - x.groups, lds);
 }
 
 // ---- float matrices ----
@@ -553,6 +612,7 @@ template <typename T> __global__ __launch_bounds__(256) void linear_join(LinTile
             s1 += *reinterpret_cast<const f32x4*>(from + 4);
         }
         float v[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
+        if (a.second) make_sums_again<T>(a, i, j, v);
         finish8<T>(a.o, i, j, v);
     }
 }
@@ -614,7 +674,7 @@ template <typename T, int NW> __global__ __launch_bounds__(64 * NW) void linear_
 struct LinPack {
     const void *src, *pre;  // pre: multiply by the activation's slope there
     uint64_t src_stride, pre_stride;
-    void* dst;              // [rows][pitch], zeros behind a row's end; NULL: sums alone
+    void *dst, *second;     // [rows][pitch], zeros behind a row's end; NULL: sums alone. second: the second part, or NULL
     uint32_t rows, cols, pitch, act;
     float* part;            // [strips][cols] sums of columns, or NULL
     uint32_t across, strips, first; // workgroups: 512 columns each, strips of rows; the first one's number
@@ -646,6 +706,18 @@ template <typename T> __global__ __launch_bounds__(256) void linear_pack(LinPack
 #pragma unroll
             for (int k = 0; k < 8; k++) s[k] += v[k];
             if (!a.dst) continue;
+            if constexpr (sizeof(T) == 2) {
+                if (a.second) {
+                    float rest[8];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        v[k] *= Two<T>::HALF;
+                        const float r = v[k] - (float)(T)v[k];
+                        rest[k] = is_finite(r) ? r * (1.f / Two<T>::DOWN) : 0.f; // (an infinity is all in its first part)
+                    }
+                    give8<T>(a.second, i * a.pitch + j, rest, 8);
+                }
+            }
             give8<T>(a.dst, i * a.pitch + j, v, 8);
         }
     }
@@ -694,7 +766,7 @@ template <typename T> static uint64_t packed_bytes(uint64_t rows, uint32_t cols)
 template <typename T>
 static LinPack& add_pack(apoe_ctx* ctx, LinPacks& all, const void* src, uint64_t stride, uint32_t rows, uint32_t cols, void* dst) {
     LinPack& a = all.one[all.count++];
-    a = LinPack{src, nullptr, stride, 0, dst, rows, cols, pitch_of(cols), 0, nullptr, 0, 0, 0};
+    a = LinPack{src, nullptr, stride, 0, dst, nullptr, rows, cols, pitch_of(cols), 0, nullptr, 0, 0, 0};
     a.across = (a.pitch + 511) / 512;
     a.strips = std::max(1u, std::min({(rows + 3) / 4, LIN_STRIPS, std::max(1u, (uint32_t)ctx->num_cus * 8 / a.across)}));
     return a;
@@ -728,7 +800,7 @@ constexpr LinKind LIN_KINDS[] = {{256, 256, 64, false, 9.f, .0243f, 0.f, 0.f}, {
                                  {128, 128, 64, false, 3.f, .0082f, 0.f, 0.f}, {64, 64, 64, true, 1.f, .0055f, 1.f, .0033f}};
 constexpr LinKind LIN_KINDS_FLOAT[] = {{256, 256, 32, false, 12.f, .157f, 0.f, 0.f}, {128, 128, 32, false, 6.5f, .044f, 0.f, 0.f}, {64, 64, 64, false, 2.f, .0155f, 0.f, 0.f}};
 
-template <typename T> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t n, uint32_t k) {
+template <typename T> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t n, uint32_t k, uint32_t parts = 1) {
     const uint64_t cus = (uint64_t)ctx->num_cus;
     LinShape best{};
     float least = INFINITY;
@@ -740,7 +812,7 @@ template <typename T> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t
             const uint32_t each = std::max(1u, (stages + cuts - 1) / cuts);
             const uint64_t groups = tiles * cuts, at_once = kind.two ? 2 * cus : cus;
             const bool alone = kind.two && groups <= cus;
-            const float inner = (float)(each * kind.ke);
+            const float inner = (float)(each * kind.ke * parts);
             float t = 3.f + (float)((groups + at_once - 1) / at_once) * (alone ? kind.alone_fixed + kind.alone_inner * inner : kind.fixed + kind.inner * inner);
             if (cuts > 1) t += 3.f + (float)(cuts + 1) * (float)m * (float)n * 1e-6f; // 4 bytes at 4 TB/s
             if (t < least) {
@@ -760,11 +832,12 @@ template <typename T> static LinShape choose(apoe_ctx* ctx, uint32_t m, uint32_t
 
 static uint64_t cut_bytes(const LinShape& s, uint32_t m, uint32_t n) { return s.cuts > 1 ? (uint64_t)s.cuts * m * pitch_of(n) * 4 : 0; }
 
-static LinTile tiles_of(const LinShape& s, LinOperand a, LinOperand b, uint32_t k, float* part, const LinOut& o, const LinBias& bias = {}) {
+static LinTile tiles_of(const LinShape& s, LinOperand a, LinOperand b, uint32_t k, float* part, const LinOut& o, const LinBias& bias = {}, uint64_t second = 0, bool a_down = false,
+                        bool b_down = false) {
     const uint32_t mt = (o.m + s.bm - 1) / s.bm, nt = (o.n + s.bn - 1) / s.bn;
     uint32_t band = 1; // a power of two, so that runs end where bands do (8192 x 8192 x 4096: 444 us, row by row 482; 8192 x 1024 x 4096 67, 75)
     while (band * 2 <= mt && (uint64_t)band * band * 32 <= (uint64_t)mt * nt) band *= 2;
-    return LinTile{a.p, b.p, a.pitch, b.pitch, k, mt, nt, band, s.cuts, s.cut_stages, part, pitch_of(o.n), (uint32_t)((uint64_t)mt * nt * s.cuts), o, bias};
+    return LinTile{a.p, b.p, a.pitch, b.pitch, k, mt, nt, band, s.cuts, s.cut_stages, part, pitch_of(o.n), (uint32_t)((uint64_t)mt * nt * s.cuts), o, bias, second, a_down, b_down};
 }
 
 static uint32_t bias_groups(const LinBias& b, uint32_t threads) { return b.out ? (b.cols + threads / 16 - 1) / (threads / 16) : 0; }
@@ -791,7 +864,10 @@ template <typename T, typename F> static void with_kind(uint32_t kind, F&& go) {
 
 template <typename T, bool BCOL, bool ONE, int... N> static void start(hipStream_t s, uint32_t threads, const LinTile& t, Numbers<N...>) {
     const uint32_t grid = t.groups + bias_groups(t.bias, threads);
-    if constexpr (sizeof(T) == 2) linear_tile<T, false, BCOL, N...><<<grid, threads, 0, s>>>(t);
+    if constexpr (sizeof(T) == 2 && BCOL) {
+        if (t.second) linear_tile<T, false, BCOL, true, N...><<<grid, threads, 0, s>>>(t);
+        else linear_tile<T, false, BCOL, false, N...><<<grid, threads, 0, s>>>(t);
+    } else if constexpr (sizeof(T) == 2) linear_tile<T, false, BCOL, false, N...><<<grid, threads, 0, s>>>(t);
     else linear_tile32<false, BCOL, ONE, N...><<<grid, threads, 0, s>>>(t);
 }
 template <typename T, bool BCOL, bool ONE = false> static void product(apoe_ctx* ctx, uint32_t kind, const LinTile& t) {
@@ -801,8 +877,10 @@ template <typename T, bool BCOL, bool ONE = false> static void product(apoe_ctx*
 
 template <typename T, int... N> static void start_grads(hipStream_t s, uint32_t threads, const LinTile& x, const LinTile& w, Numbers<N...>) {
     const uint32_t grid = x.groups + w.groups + bias_groups(w.bias, threads);
-    if constexpr (sizeof(T) == 2) linear_grads<T, N...><<<grid, threads, 0, s>>>(x, w);
-    else linear_grads32<N...><<<grid, threads, 0, s>>>(x, w);
+    if constexpr (sizeof(T) == 2) {
+        if (w.second) linear_grads<T, true, N...><<<grid, threads, 0, s>>>(x, w);
+        else linear_grads<T, false, N...><<<grid, threads, 0, s>>>(x, w);
+    } else linear_grads32<N...><<<grid, threads, 0, s>>>(x, w);
 }
 template <typename T> static void grad_products(apoe_ctx* ctx, uint32_t kind, const LinTile& x, const LinTile& w) {
     with_kind<T>(kind, [&](uint32_t threads, auto numbers) { start_grads<T>(ctx->stream, threads, x, w, numbers); });
@@ -865,11 +943,13 @@ template <typename T> static int run_linear_grad(apoe_ctx* ctx, const apoe_linea
     const bool act = p->act != APOE_ACT_NONE, products = p->grad_x || p->grad_w;
     const bool g_is = !act && as_it_is<T>(p->grad_y, p->grad_y_stride, n), x_is = !p->grad_w || as_it_is<T>(p->x, p->x_stride, k), w_is = !p->grad_x || as_it_is<T>(p->w, p->w_stride, k);
     const bool pack_g = products && !g_is;
+    const uint32_t parts = sizeof(T) == 2 && (p->act == APOE_ACT_GELU || p->act == APOE_ACT_SILU) ? 2 : 1;
+    const uint64_t second = parts == 2 ? packed_bytes<T>(m, n) : 0;
     LinShape sx{}, sw{};
-    if (p->grad_x) sx = choose<T>(ctx, m, k, n);
-    if (p->grad_w) sw = choose<T>(ctx, n, k, m);
+    if (p->grad_x) sx = choose<T>(ctx, m, k, n, parts);
+    if (p->grad_w) sw = choose<T>(ctx, n, k, m, parts);
     LinPlan plan;
-    const uint64_t o_g = plan.take(pack_g ? packed_bytes<T>(m, n) : 0), o_x = plan.take(x_is ? 0 : packed_bytes<T>(m, k)), o_w = plan.take(w_is ? 0 : packed_bytes<T>(n, k));
+    const uint64_t o_g = plan.take(pack_g ? parts * packed_bytes<T>(m, n) : 0), o_x = plan.take(x_is ? 0 : packed_bytes<T>(m, k)), o_w = plan.take(w_is ? 0 : packed_bytes<T>(n, k));
     // Both products in one launch where they have tiles of one kind: none waits for the other's last tiles (bf16, the whole call: 512 rows of 1024 x 1024 21.4 -> 18.3 us, 2048
     // of them 25.8 -> 23.2, 8192 of 4096 x 4096 479 -> 477; float 4096 rows of 1024 x 1024 116 -> 114). Each has the tiles and cuts that it has alone: the same bits.
     const bool together = p->grad_x && p->grad_w && m && sx.kind == sw.kind;
@@ -887,6 +967,7 @@ template <typename T> static int run_linear_grad(apoe_ctx* ctx, const apoe_linea
             a.pre = p->pre;
             a.pre_stride = p->pre_stride;
             a.act = p->act;
+            if (pack_g && second) a.second = ws + o_g + second;
         }
         if (p->grad_bias) {
             a.part = (float*)(ws + o_bias);
@@ -906,12 +987,12 @@ template <typename T> static int run_linear_grad(apoe_ctx* ctx, const apoe_linea
     LinTile tx{};
     if (p->grad_x && m) {
         const LinOut o{p->grad_x, nullptr, nullptr, nullptr, p->grad_x_stride, 0, 0, m, k, APOE_ACT_NONE};
-        tx = tiles_of(sx, g, w, n, (float*)(ws + o_part), o, p->grad_w ? LinBias{} : bias);
+        tx = tiles_of(sx, g, w, n, (float*)(ws + o_part), o, p->grad_w ? LinBias{} : bias, second, false, true);
         if (!together) product<T, true>(ctx, sx.kind, tx);
     }
     if (p->grad_w) {
         const LinOut o{p->grad_w, nullptr, nullptr, nullptr, p->grad_w_stride, 0, 0, n, k, APOE_ACT_NONE};
-        grad_products<T>(ctx, sw.kind, together ? tx : LinTile{}, tiles_of(sw, g, x, m, (float*)(ws + o_more), o, bias));
+        grad_products<T>(ctx, sw.kind, together ? tx : LinTile{}, tiles_of(sw, g, x, m, (float*)(ws + o_more), o, bias, second, true, true));
     }
     if (p->grad_bias && !p->grad_w && !(p->grad_x && m)) linear_bias<<<(n + 31) / 32, 512, 0, ctx->stream>>>(bias);
     APOE_HIP(hipGetLastError());

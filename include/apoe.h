@@ -487,7 +487,8 @@ typedef struct {
  * grad_x = gz w, grad_w = gz^T x, grad_bias = sum of gz's rows. (The gradient of residual is grad_y; y may be residual itself when the strides are
  * equal.) Sums are 32 bits and rounded once. float matrices are multiplied as three parts of eight bits each, six products: off by 2^-22 of each
  * product of two values at most, and a value below 2^-111, whose last part is below the parts' smallest number, by 2^-133 of the other; a value that is
- * infinite gives NaN there. gz of 16-bit matrices with an activation is rounded for the two products, not for grad_bias. Workspace: gz, partial sums
+ * infinite gives NaN there. gz of 16-bit matrices with GELU or SiLU goes
+ * into the two products as two parts of its type, off by their two roundings' product (bfloat16 2^-16 of it, float16 2^-22). Workspace: gz (once or twice), partial sums
  * of up to 128 MiB a product where rows and columns are too few to fill the GPU, and copies of matrices whose rows are not whole multiples of 16 bytes (of
  * floats only where that is quicker) or lie further than 4 MiB apart.
  */
