@@ -104,7 +104,7 @@ __device__ inline void activate8(float* z, uint32_t act) {
 __device__ inline void slope8(float* v, const float* z, uint32_t act) {
     if (act == APOE_ACT_RELU) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = z[k] <= 0.f ? 0.f : v[k]; // whatever comes in where nothing went out: an infinity too
+        for (int k = 0; k < 8; k++) v[k] = z[k] > 0.f ? v[k] : 0.f; // whatever comes in where nothing went out: an infinity too
     } else if (act == APOE_ACT_GELU) {
 #pragma unroll
         for (int k = 0; k < 8; k++) {
