@@ -28,6 +28,9 @@ int check_pointer(const apoe_ctx* ctx, const void* p, size_t align, const char* 
 
 // What is written while `q` is still read, or written by others. (Matrices may share a buffer, side by side: only the same beginning is refused.)
 #define APOE_APART(p, q) APOE_REQUIRE(!(p) || (const void*)(p) != (const void*)(q), #p " and " #q " are the same memory")
+// What may be `q` itself, row by row.
+#define APOE_IN_PLACE(p, q, rows) \
+    APOE_REQUIRE(!(p) || (const void*)(p) != (const void*)(q) || p##_stride == q##_stride || (rows) <= 1, #p " and " #q " are the same memory with other strides")
 
 int embed(apoe_ctx* ctx, const apoe_embed_args* args, bool grad) {
     APOE_REQUIRE(ctx && args, "ctx/args is null");
@@ -60,6 +63,11 @@ int embed(apoe_ctx* ctx, const apoe_embed_args* args, bool grad) {
         a.grad_table = nullptr;
     }
     APOE_REQUIRE(a.idx || a.n_entries == 0, "idx is null");
+    APOE_APART(a.out, a.table);
+    APOE_IN_PLACE(a.out, a.base, a.n_rows);
+    APOE_APART(a.grad_table, a.grad);
+    APOE_APART(a.grad_table, a.table);
+    if (grad) APOE_APART(a.grad_val, a.val);
     APOE_POINTER(a.table, e, "table");
     APOE_POINTER(a.idx, 4, "idx");
     APOE_POINTER(a.off, 4, "off");
@@ -69,10 +77,6 @@ int embed(apoe_ctx* ctx, const apoe_embed_args* args, bool grad) {
     APOE_POINTER(a.grad, e, "grad");
     APOE_POINTER(a.grad_table, e, "grad_table");
     APOE_POINTER(a.grad_val, 4, "grad_val");
-    APOE_APART(a.out, a.table);
-    APOE_APART(a.grad_table, a.grad);
-    APOE_APART(a.grad_table, a.table);
-    if (grad) APOE_APART(a.grad_val, a.val);
     APOE_HIP(hipSetDevice(ctx->device));
     return launch_embed(ctx, &a, grad);
 }
@@ -99,6 +103,10 @@ int layer_norm(apoe_ctx* ctx, const apoe_layer_norm_args* args, bool grad) {
     }
     if (a.rows == 0 && !(grad && (a.grad_w || a.grad_b))) return APOE_OK;
     APOE_REQUIRE(a.x || a.rows == 0, "x is null");
+    APOE_IN_PLACE(a.y, a.x, a.rows);
+    APOE_IN_PLACE(a.grad_x, a.x, a.rows);
+    APOE_IN_PLACE(a.grad_x, a.grad_y, a.rows);
+    APOE_IN_PLACE(a.grad_x, a.grad_skip, a.rows);
     const size_t e = size_of(a.dtype);
     APOE_POINTER(a.x, e, "x");
     APOE_POINTER(a.w, 4, "w");
@@ -138,9 +146,21 @@ int linear(apoe_ctx* ctx, const apoe_linear_args* args, bool grad) {
         APOE_REQUIRE(a.rows == 0 || (a.grad_y && (a.x || !a.grad_w)), "grad_y/x is null");
         APOE_REQUIRE(a.rows == 0 || a.w || !a.grad_x, "w is null");
         APOE_REQUIRE(a.rows == 0 || a.act == APOE_ACT_NONE || a.pre, "the gradient of an activation needs pre");
+        for (const void* in : {a.grad_y, a.act == APOE_ACT_NONE ? nullptr : (const void*)a.pre, a.x, a.w}) {
+            APOE_APART(a.grad_x, in);
+            APOE_APART(a.grad_w, in);
+        }
+        APOE_APART(a.grad_x, a.grad_w);
     } else {
         if (a.rows == 0) return APOE_OK;
         APOE_REQUIRE(a.x && a.w && a.y, "x/w/y is null");
+        for (const void* in : {a.x, a.w}) {
+            APOE_APART(a.y, in);
+            APOE_APART(a.pre, in);
+        }
+        APOE_APART(a.y, a.pre);
+        APOE_APART(a.pre, a.residual);
+        APOE_IN_PLACE(a.y, a.residual, a.rows);
     }
     APOE_POINTER(a.x, e, "x");
     APOE_POINTER(a.w, e, "w");
@@ -150,21 +170,10 @@ int linear(apoe_ctx* ctx, const apoe_linear_args* args, bool grad) {
         APOE_POINTER(a.grad_x, e, "grad_x");
         APOE_POINTER(a.grad_w, e, "grad_w");
         APOE_POINTER(a.grad_bias, 4, "grad_bias");
-        for (const void* in : {a.grad_y, a.act == APOE_ACT_NONE ? nullptr : (const void*)a.pre, a.x, a.w}) {
-            APOE_APART(a.grad_x, in);
-            APOE_APART(a.grad_w, in);
-        }
-        APOE_APART(a.grad_x, a.grad_w);
     } else {
         APOE_POINTER(a.bias, 4, "bias");
         APOE_POINTER(a.residual, e, "residual");
         APOE_POINTER(a.y, e, "y");
-        for (const void* in : {a.x, a.w}) {
-            APOE_APART(a.y, in);
-            APOE_APART(a.pre, in);
-        }
-        APOE_APART(a.y, a.pre);
-        APOE_APART(a.pre, a.residual);
     }
     APOE_HIP(hipSetDevice(ctx->device));
     return launch_linear(ctx, &a, grad);
