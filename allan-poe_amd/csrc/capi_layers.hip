@@ -65,9 +65,11 @@ int embed(apoe_ctx* ctx, const apoe_embed_args* args, bool grad) {
     APOE_REQUIRE(a.idx || a.n_entries == 0, "idx is null");
     APOE_APART(a.out, a.table);
     APOE_IN_PLACE(a.out, a.base, a.n_rows);
+    for (const void* in : {(const void*)a.idx, (const void*)a.off, (const void*)a.val}) APOE_APART(a.out, in);
     APOE_APART(a.grad_table, a.grad);
     APOE_APART(a.grad_table, a.table);
-    if (grad) APOE_APART(a.grad_val, a.val);
+    if (grad)
+        for (const void* in : {(const void*)a.idx, (const void*)a.off, (const void*)a.val, a.table, a.grad, (const void*)a.grad_table}) APOE_APART(a.grad_val, in);
     APOE_POINTER(a.table, e, "table");
     APOE_POINTER(a.idx, 4, "idx");
     APOE_POINTER(a.off, 4, "off");
@@ -107,6 +109,12 @@ int layer_norm(apoe_ctx* ctx, const apoe_layer_norm_args* args, bool grad) {
     APOE_IN_PLACE(a.grad_x, a.x, a.rows);
     APOE_IN_PLACE(a.grad_x, a.grad_y, a.rows);
     APOE_IN_PLACE(a.grad_x, a.grad_skip, a.rows);
+    APOE_APART(a.y, a.w);
+    APOE_APART(a.y, a.b);
+    if (grad) { // (grad_w and grad_b are written by a launch behind the one that reads the rows)
+        for (const void* other : {a.w, (const float*)a.grad_w, (const float*)a.grad_b}) APOE_APART(a.grad_x, other);
+        APOE_APART(a.grad_w, a.grad_b);
+    }
     const size_t e = size_of(a.dtype);
     APOE_POINTER(a.x, e, "x");
     APOE_POINTER(a.w, 4, "w");
@@ -149,12 +157,15 @@ int linear(apoe_ctx* ctx, const apoe_linear_args* args, bool grad) {
         for (const void* in : {a.grad_y, a.act == APOE_ACT_NONE ? nullptr : (const void*)a.pre, a.x, a.w}) {
             APOE_APART(a.grad_x, in);
             APOE_APART(a.grad_w, in);
+            APOE_APART(a.grad_bias, in);
         }
         APOE_APART(a.grad_x, a.grad_w);
+        APOE_APART(a.grad_bias, a.grad_x);
+        APOE_APART(a.grad_bias, a.grad_w);
     } else {
         if (a.rows == 0) return APOE_OK;
         APOE_REQUIRE(a.x && a.w && a.y, "x/w/y is null");
-        for (const void* in : {a.x, a.w}) {
+        for (const void* in : {a.x, a.w, (const void*)a.bias}) {
             APOE_APART(a.y, in);
             APOE_APART(a.pre, in);
         }
@@ -294,6 +305,11 @@ int apoe_adamw_moments(apoe_ctx* ctx, uint64_t n, const int8_t* m, const float* 
     if (n == 0) return APOE_OK;
     APOE_REQUIRE(n < (1ull << 40), "%llu values are beyond 2^40", (unsigned long long)n);
     APOE_REQUIRE(m && m_scale && v && v_scale && m_out && v_out, "m/m_scale/v/v_scale/m_out/v_out is null");
+    for (const void* in : {(const void*)m, (const void*)m_scale, (const void*)v, (const void*)v_scale}) {
+        APOE_APART(m_out, in);
+        APOE_APART(v_out, in);
+    }
+    APOE_APART(m_out, v_out);
     APOE_POINTER(m, 1, "m");
     APOE_POINTER(v, 1, "v");
     APOE_POINTER(m_scale, 4, "m_scale");

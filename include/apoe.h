@@ -400,7 +400,7 @@ int apoe_gated_residual_grad(apoe_ctx* ctx, const apoe_gated_residual_args* args
  * summed up (terms of the learned-sparse path, tokens), layer norm, matrix products with what is done to their results, and the step of
  * all parameters. The rules above hold: the context's stream, device pointers, strides from row to row (0: dense), workspace that the context
  * keeps. Rows may begin at any multiple of their type's size; such as begin at multiples of 16 bytes are read 16 bytes at a time.
- * An output that begins where an input does is refused where others would still read it.
+ * An output that begins where an input does is refused where others would still read it, and so are two outputs with one beginning.
  * A captured graph uses the context's workspace as it was then, which is kept as long as the context: all of a context's calls and graphs run one
  * after the other, and the context outlives its graphs.
  */

@@ -53,3 +53,34 @@ def test_what_may_be_in_place(name, same):
     """These go on to the check of the addresses."""
     st, message = status(name, *CALLS[name], same)
     assert st == -1 and "device memory" in message, message
+
+
+@pytest.mark.parametrize("name,same", [
+    ("apoe_layer_norm", dict(y="w")), ("apoe_layer_norm", dict(y="b")), ("apoe_layer_norm_grad", dict(grad_x="w")), ("apoe_layer_norm_grad", dict(grad_w="grad_x")),
+    ("apoe_layer_norm_grad", dict(grad_b="grad_x")), ("apoe_layer_norm_grad", dict(grad_w="grad_b")),
+    ("apoe_embed", dict(out="idx")), ("apoe_embed", dict(out="off")), ("apoe_embed", dict(out="val")),
+    ("apoe_embed_grad", dict(grad_val="idx")), ("apoe_embed_grad", dict(grad_val="off")), ("apoe_embed_grad", dict(grad_val="table")),
+    ("apoe_embed_grad", dict(grad_val="grad")), ("apoe_embed_grad", dict(grad_val="grad_table")),
+    ("apoe_linear", dict(y="bias")), ("apoe_linear", dict(pre="bias")),
+    *(("apoe_linear_grad", dict(grad_bias=k)) for k in ("x", "w", "pre", "grad_y", "grad_x", "grad_w"))])
+def test_vectors_too(name, same):
+    """A vector that others still read, or two outputs at one place."""
+    st, message = status(name, *CALLS[name], same)
+    assert st == -1 and "the same memory" in message, message
+
+
+@pytest.mark.parametrize("name,same", [("apoe_layer_norm_grad", dict(grad_w="w", grad_b="x")), ("apoe_linear_grad", dict(grad_bias="pre", act=0))])
+def test_what_is_not_read_any_more(name, same):
+    """The norm's vectors are added up behind the launch that reads its inputs; without an activation pre is not read."""
+    st, message = status(name, *CALLS[name], same)
+    assert st == -1 and "device memory" in message, message
+
+
+@pytest.mark.parametrize("to", [4, 5])
+@pytest.mark.parametrize("source", [0, 1, 2, 3, 9])
+def test_moments_that_are_read_back(to, source):
+    """Of m, m_scale, v, v_scale and both results, each result at another's address (9: at the other result's)."""
+    lib, p = apoe.lib(), [4096 * (i + 1) for i in range(6)]
+    p[to] = p[9 - to if source == 9 else source]
+    assert lib.apoe_adamw_moments(C.create_string_buffer(b"\xff" * 4096, 4096), C.c_uint64(512), *(C.c_void_p(x) for x in p)) == -1
+    assert "the same memory" in lib.apoe_last_error_string().decode()
