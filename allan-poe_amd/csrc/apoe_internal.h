@@ -216,6 +216,11 @@ struct apoe_adamw {
     apoe_ctx* ctx = nullptr;
     uint32_t bits = 32, seed = 0;
     std::vector<apoe_adamw_tensor> tensors;
+    struct Written { // an array that a step writes
+        uintptr_t begin, end;
+        uint32_t tensor, value; // bytes of a value
+    };
+    std::vector<Written> written; // by address, apart from each other
 };
 
 namespace apoe {

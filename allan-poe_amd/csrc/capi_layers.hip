@@ -191,29 +191,37 @@ int linear(apoe_ctx* ctx, const apoe_linear_args* args, bool grad) {
 }
 
 // No two arrays that a step writes may share memory.
-int check_disjoint(const apoe_adamw* opt) {
-    struct Range {
-        uintptr_t begin, end;
-    };
-    std::vector<Range> ranges;
+int check_disjoint(apoe_adamw* opt) {
+    using Written = apoe_adamw::Written;
+    std::vector<Written>& ranges = opt->written;
     ranges.reserve(opt->tensors.size() * 6);
-    const size_t value = opt->bits / 8;
-    for (const apoe_adamw_tensor& t : opt->tensors) {
+    const uint32_t value = opt->bits / 8;
+    for (uint32_t i = 0; i < opt->tensors.size(); i++) {
+        const apoe_adamw_tensor& t = opt->tensors[i];
         const size_t blocks = (t.n + APOE_ADAMW_BLOCK - 1) / APOE_ADAMW_BLOCK;
-        auto add = [&](const void* p, size_t bytes) {
-            if (p && bytes) ranges.push_back(Range{(uintptr_t)p, (uintptr_t)p + bytes});
+        auto add = [&](const void* p, size_t n, uint32_t size) {
+            if (p && n) ranges.push_back(Written{(uintptr_t)p, (uintptr_t)p + n * size, i, size});
         };
-        add(t.p, t.n * 4);
-        add(t.m, t.n * value);
-        add(t.v, t.n * value);
+        add(t.p, t.n, 4);
+        add(t.m, t.n, value);
+        add(t.v, t.n, value);
         if (opt->bits == 8) {
-            add(t.m_scale, blocks * 4);
-            add(t.v_scale, blocks * 4);
+            add(t.m_scale, blocks, 4);
+            add(t.v_scale, blocks, 4);
         }
-        add(t.copy, t.n * 2);
+        add(t.copy, t.n, 2);
     }
-    std::sort(ranges.begin(), ranges.end(), [](const Range& x, const Range& y) { return x.begin < y.begin; });
+    std::sort(ranges.begin(), ranges.end(), [](const Written& x, const Written& y) { return x.begin < y.begin; });
     for (size_t i = 1; i < ranges.size(); i++) APOE_REQUIRE(ranges[i].begin >= ranges[i - 1].end, "two parameters, moments or copies share memory");
+    return APOE_OK;
+}
+
+// What a step reads must not lie in what it writes, but for a gradient that is an array of its own parameter, value by value.
+int check_apart(const apoe_adamw* opt, const void* p, size_t n, size_t size, uint32_t tensor, const char* name) {
+    const uintptr_t begin = (uintptr_t)p, end = begin + n * size;
+    auto r = std::upper_bound(opt->written.begin(), opt->written.end(), begin, [](uintptr_t at, const apoe_adamw::Written& w) { return at < w.end; });
+    APOE_REQUIRE(r == opt->written.end() || r->begin >= end || (r->tensor == tensor && r->begin == begin && r->end == end && r->value == size),
+                 "%s and what the step writes are the same memory", name);
     return APOE_OK;
 }
 
@@ -291,10 +299,13 @@ int apoe_adamw_step(apoe_adamw* opt, const apoe_adamw_step_args* args) {
     APOE_REQUIRE(a.step >= 1 || a.step_dev, "steps are counted from 1");
     APOE_POINTER(a.step_dev, 4, "step_dev");
     APOE_POINTER(a.lr_dev, 4, "lr_dev");
+    if (a.step_dev) APOE_TRY(check_apart(opt, a.step_dev, 1, 4, UINT32_MAX, "step_dev"));
+    if (a.lr_dev) APOE_TRY(check_apart(opt, a.lr_dev, 1, 4, UINT32_MAX, "lr_dev"));
     for (size_t i = 0; i < opt->tensors.size(); i++) {
         if (!a.grads[i] || opt->tensors[i].n == 0) continue;
         APOE_REQUIRE(a.grad_dtypes[i] <= APOE_BF16, "unknown dtype %u of gradient %zu", a.grad_dtypes[i], i);
         APOE_TRY(check_pointer(ctx, a.grads[i], size_of(a.grad_dtypes[i]), "a gradient"));
+        APOE_TRY(check_apart(opt, a.grads[i], opt->tensors[i].n, size_of(a.grad_dtypes[i]), (uint32_t)i, "a gradient"));
     }
     APOE_HIP(hipSetDevice(ctx->device));
     return launch_adamw(opt, args);

@@ -523,7 +523,8 @@ typedef struct {
  * bits 8: m = m_scale c |c| / 127^2 and v = v_scale c^4 / 255^4 for a code c, finer for small values; a new moment goes to one of the two codes beside it
  * by chance, so that its mean is kept and small changes are not lost (a v above zero keeps a code above zero). The chances come from
  * seed, step, parameter and place: the same call gives the same bits. p is stepped with the moments before they are rounded. A moment that is not finite
- * makes its block's scale so.
+ * makes its block's scale so. Gradients, step_dev and lr_dev that lie in what a step writes are refused, but for a gradient that is an array of its own
+ * parameter with values of the same size.
  */
 int apoe_adamw_create(apoe_ctx* ctx, uint32_t count, const apoe_adamw_tensor* tensors, uint32_t bits, uint32_t seed, apoe_adamw** out);
 void apoe_adamw_destroy(apoe_adamw* opt);
