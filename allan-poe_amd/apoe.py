@@ -96,7 +96,7 @@ class AdamwTensor(C.Structure):
 
 class AdamwStepArgs(C.Structure):
     _fields_ = [("grads", C.c_void_p), ("grad_dtypes", C.c_void_p), ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
-                ("grad_scale", C.c_double), ("step", C.c_uint32), ("step_dev", C.c_void_p), ("lr_dev", C.c_void_p)]
+                ("grad_scale", C.c_double), ("step", C.c_uint32), ("step_dev", C.c_void_p), ("lr_dev", C.c_void_p), ("step_taken", C.c_void_p)]
 
 
 EXPORTS = [
@@ -981,6 +981,7 @@ class AdamW:
                 raise ApoeError(f"state has no {k}")
             _vector(ctx, state[k], k, blocks if k.endswith("scale") else n, (t,))
         self._moments = {k: state[k] for k in types}
+        self._taken, self._on_gpu = _torch.empty(1, dtype=_torch.int32, device=dev), False  # the last step's number, as the GPU took it
         self.t = int(state.get("t", 0))
         tensors = (AdamwTensor * len(self.params))()
         for a, p, c, d, at in zip(tensors, self.params, self.copies, decay, self.offsets):
@@ -998,10 +999,23 @@ class AdamW:
         if t.dtype not in dtypes or not t.is_contiguous() or (shape is not None and t.shape != shape):
             raise ApoeError(f"{name} must be a contiguous tensor of {' or '.join(str(d) for d in dtypes)}{'' if shape is None else f' of shape {tuple(shape)}'}")
 
+    @property
+    def t(self):
+        """The number of steps taken. (After steps whose number is a tensor it is asked of the GPU, which is waited for.)"""
+        if self._on_gpu:
+            _torch.cuda.synchronize(self.ctx.device)
+            return int(self._taken)
+        return self._t
+
+    @t.setter
+    def t(self, t):
+        self._t = t
+        self._taken.fill_(t)
+
     def step(self, grads, lr, grad_scale=1.0, t=None):
         """One step with the parameters' gradients (None: that parameter and its moments stay as they are), which count times grad_scale. lr may be a
         float32 tensor of one number on the GPU, and t, the number of the step, an int32 one: a captured step reads both when it
-        is replayed (the program counts t up; without it the object counts)."""
+        is replayed (the program counts t up; without it the object counts on from the last step that was taken)."""
         if not (self.h and self.ctx.h):
             raise ApoeError("the object or its context has been closed")
         if len(grads) != len(self.params):
@@ -1021,12 +1035,16 @@ class AdamW:
         else:
             a.lr = lr
         a.beta1, a.beta2 = self.betas
-        a.eps, a.grad_scale, a.step = self.eps, grad_scale, self.t + 1
+        a.eps, a.grad_scale, a.step_taken = self.eps, grad_scale, self._taken.data_ptr()
         if t is not None:
             a.step_dev = _vector(self.ctx, t.reshape(-1), "t", 1, _INTS)
+        else:
+            a.step = self.t + 1
         _ordered(self.ctx, lambda: lib().apoe_adamw_step(self.h, C.byref(a)))
         if t is None:
-            self.t += 1
+            self._t = a.step
+        else:
+            self._on_gpu = True  # from now on: a captured step may be replayed at any time
 
     def moments(self):
         """(m, v) as float32, laid out like the moments themselves: those themselves where they have 32 bits."""

@@ -46,6 +46,7 @@ struct AdamArgs {
     uint32_t count, pieces, seed, step;
     const uint32_t* step_dev;
     const float* lr_dev;
+    uint32_t* taken;
     double b1, b2, grad_scale;
     float lr, eps, c1, c2; // c: one over 1 - b^t
 };
@@ -249,6 +250,7 @@ template <int BITS, bool NEAR> __global__ __launch_bounds__(256) void adamw_step
         c2 = (float)(1. / (1. - power(a.b2, step)));
     }
     if (a.lr_dev) lr = *a.lr_dev;
+    if (a.taken && blockIdx.x == 0 && threadIdx.x == 0) *a.taken = step;
     const uint32_t key = mix(mix(mix(a.seed) ^ step) ^ t.index);
     const uint32_t g_type = t.g_type;
     for (; at < end; at += 4 * BLOCK) {
@@ -333,6 +335,9 @@ template <int BITS, bool NEAR> __global__ __launch_bounds__(256) void adamw_step
     }
 }
 
+// A step of no parameter at all.
+__global__ void adamw_count(AdamArgs a) { *a.taken = a.step_dev ? *a.step_dev : a.step; }
+
 // Four values a thread from a block's beginning on.
 __global__ __launch_bounds__(256) void adamw_read(uint64_t n, const int8_t* m, const float* ms, const uint8_t* v, const float* vs, float* m_out, float* v_out, bool whole) {
     const int lane = threadIdx.x & 63;
@@ -361,6 +366,7 @@ int launch_adamw(apoe_adamw* opt, const apoe_adamw_step_args* p) {
     a.step = p->step;
     a.step_dev = p->step_dev;
     a.lr_dev = p->lr_dev;
+    a.taken = p->step_taken;
     a.b1 = p->beta1;
     a.b2 = p->beta2;
     a.grad_scale = p->grad_scale;
@@ -379,6 +385,7 @@ int launch_adamw(apoe_adamw* opt, const apoe_adamw_step_args* p) {
         if (opt->bits == 32) run(near ? adamw_step<32, true> : adamw_step<32, false>);
         else run(near ? adamw_step<8, true> : adamw_step<8, false>);
         a.count = a.pieces = 0;
+        a.taken = nullptr; // (the first launch tells)
         APOE_HIP(hipGetLastError());
         return APOE_OK;
     };
@@ -394,6 +401,11 @@ int launch_adamw(apoe_adamw* opt, const apoe_adamw_step_args* p) {
         a.t[a.count++] = AdamTensor{t.p, p->grads[i], t.m, t.v, t.m_scale, t.v_scale, t.copy, t.n, (float)t.decay, (uint32_t)i, a.pieces, (uint8_t)p->grad_dtypes[i],
                                     (uint8_t)t.copy_dtype, (uint8_t)whole};
         a.pieces += pieces;
+    }
+    if (a.pieces == 0 && a.taken) {
+        adamw_count<<<1, 1, 0, opt->ctx->stream>>>(a);
+        APOE_HIP(hipGetLastError());
+        return APOE_OK;
     }
     return go();
 }

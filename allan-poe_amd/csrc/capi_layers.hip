@@ -299,8 +299,12 @@ int apoe_adamw_step(apoe_adamw* opt, const apoe_adamw_step_args* args) {
     APOE_REQUIRE(a.step >= 1 || a.step_dev, "steps are counted from 1");
     APOE_POINTER(a.step_dev, 4, "step_dev");
     APOE_POINTER(a.lr_dev, 4, "lr_dev");
+    APOE_POINTER(a.step_taken, 4, "step_taken");
+    APOE_APART(a.step_taken, a.lr_dev);
+    APOE_APART(a.step_taken, a.step_dev);
     if (a.step_dev) APOE_TRY(check_apart(opt, a.step_dev, 1, 4, UINT32_MAX, "step_dev"));
     if (a.lr_dev) APOE_TRY(check_apart(opt, a.lr_dev, 1, 4, UINT32_MAX, "lr_dev"));
+    if (a.step_taken) APOE_TRY(check_apart(opt, a.step_taken, 1, 4, UINT32_MAX, "step_taken"));
     for (size_t i = 0; i < opt->tensors.size(); i++) {
         if (!a.grads[i] || opt->tensors[i].n == 0) continue;
         APOE_REQUIRE(a.grad_dtypes[i] <= APOE_BF16, "unknown dtype %u of gradient %zu", a.grad_dtypes[i], i);

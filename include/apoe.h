@@ -514,6 +514,7 @@ typedef struct {
     uint32_t step;               /* 1, 2, ..: the number of this step */
     const uint32_t* step_dev;    /* the same on the GPU, read there (NULL: `step`), for a captured step */
     const float* lr_dev;         /* likewise */
+    uint32_t* step_taken;        /* on the GPU: gets the step's number once it is taken; NULL: nothing */
 } apoe_adamw_step_args;
 
 /*

@@ -47,3 +47,68 @@ def test_gradients_beside_or_in_their_own_parameter(gpu_ctx, bits):
         return out
     for x, y in zip(run(True), run(False)):
         assert bool((x == y).all())
+
+
+@pytest.mark.parametrize("after", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_number_of_captured_steps(bits, after):
+    """Steps whose number is a tensor are counted as the GPU takes them, whether the program counts up before or behind each: an object that goes on from the state, and the
+    object itself without a graph, take the next one."""
+    import torch
+    import apoe
+    g = torch.Generator().manual_seed(4)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    ctx = apoe.Context(0, stream=stream)
+    with torch.cuda.stream(stream):
+        first, grad = torch.randn(1000, generator=g).cuda(), [(0.01 * torch.randn(1000, generator=g)).cuda()]
+        eager, graphed = first.clone(), first.clone()
+        want, opt = (apoe.AdamW(ctx, [p], bits=bits, seed=5) for p in (eager, graphed))
+        for o in (want, opt):
+            o.step(grad, 0.1)
+        t, lr = torch.full((1,), 2 if after else 1, dtype=torch.int32, device="cuda"), torch.full((1,), 0.1, device="cuda")
+    stream.synchronize()
+    assert opt.state()["t"] == 1
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        if not after:
+            t.add_(1)
+        opt.step(grad, lr, t=t)
+        if after:
+            t.add_(1)
+    assert opt.state()["t"] == 1  # captured, not run
+    for k in range(3):
+        with torch.cuda.stream(stream):
+            graph.replay()
+            want.step(grad, 0.1)
+            torch.randn(1000, device="cuda").sum()
+        assert opt.state()["t"] == opt.t == k + 2
+    assert float((eager - graphed).abs().max()) <= 2.0 ** -20  # lr is rounded to a float: 3 steps of 0.1 at most, each off by 2^-24 of it, and the factors' last places
+    with torch.cuda.stream(stream):
+        graphed.copy_(eager)
+        state = {k: (v.clone() if isinstance(v, torch.Tensor) else v) for k, v in want.state().items()}
+        on = apoe.AdamW(ctx, [again := eager.clone()], bits=bits, seed=5, state=dict(state, t=opt.state()["t"]))
+        for k, v in opt.state().items():
+            if k != "t":
+                v.copy_(want.state()[k])
+        for o in (want, opt, on):
+            o.step(grad, 0.1)
+        assert want.t == opt.t == on.t == 5
+    stream.synchronize()
+    assert bool((eager == graphed).all()) and bool((eager == again).all())
+    del graph
+    ctx.close()
+
+
+def test_a_number_without_gradients(gpu_ctx):
+    """A step in which no parameter has a gradient counts, with a tensor as without."""
+    import torch
+    import apoe
+    opt = apoe.AdamW(gpu_ctx, [torch.zeros(8, device="cuda")])
+    opt.step([None], 0.1)
+    assert opt.state()["t"] == 1
+    opt.step([None], 0.1, t=torch.full((1,), 9, dtype=torch.int32, device="cuda"))
+    assert opt.state()["t"] == 9
+    opt.step([None], 0.1)
+    assert opt.state()["t"] == opt.t == 10
+    opt.close()
