@@ -190,26 +190,32 @@ template <typename T> __device__ inline void finish1(const LinOut& o, uint32_t i
 
 __device__ inline bool is_finite(float v) { return fabsf(v) < INFINITY; }
 
-// Sum (i, j) once more, one product after the other: of an a in two parts, whose second is zero beside an infinity (zero times infinity would be NaN). Sums that are not finite come here.
+// Sum (i, j) once more, one product after the other. Sums of parts that are not finite come here: a part that is zero makes NaN of the other side's infinity, floats' parts of an infinity leave
+// NaN, and parts of either sign give infinities of either sign where a product is beyond the largest float. NaN ends it. (Float 4096 x 4096 x 1024 with an infinity in one row 1.1 ms, in every row 30 ms, all NaN as
+// without any.)
 template <typename T> __device__ inline float sum_again(const LinTile& a, uint32_t i, uint32_t j) {
     const char* pa = (const char*)a.a + (a.a_down ? i * sizeof(T) : (uint64_t)i * a.a_pitch);
     const char* pb = (const char*)a.b + (a.b_down ? j * sizeof(T) : (uint64_t)j * a.b_pitch);
     const uint64_t sa = a.a_down ? a.a_pitch : sizeof(T), sb = a.b_down ? a.b_pitch : sizeof(T);
     float s = 0.f;
     for (uint64_t k = 0; k < a.k && s == s; k++) {
-        const float hi = (float)*(const T*)(pa + k * sa), lo = (float)*(const T*)(pa + k * sa + a.second);
-        s = __builtin_fmaf(__builtin_fmaf(lo, Two<T>::DOWN, hi) / Two<T>::HALF, (float)*(const T*)(pb + k * sb), s);
+        float v = (float)*(const T*)(pa + k * sa);
+        if (a.second) v = __builtin_fmaf((float)*(const T*)(pa + k * sa + a.second), Two<T>::DOWN, v) * (1.f / Two<T>::HALF);
+        s = __builtin_fmaf(v, (float)*(const T*)(pb + k * sb), s);
     }
     return s;
 }
 template <typename T> __device__ inline void make_sums_again(const LinTile& a, uint32_t i, uint32_t j, float* v) {
-    bool all = true;
+    uint32_t bad = 0;
 #pragma unroll
-    for (int k = 0; k < 8; k++) all &= is_finite(v[k]);
-    if (__builtin_expect(all, 1)) return;
+    for (int k = 0; k < 8; k++) bad |= is_finite(v[k]) || j + k >= a.o.n ? 0 : 1u << k;
+    while (__builtin_expect(bad, 0)) {
+        const int at = __builtin_ctz(bad);
+        const float s = sum_again<T>(a, i, j + at);
 #pragma unroll
-    for (int k = 0; k < 8; k++)
-        if (!is_finite(v[k]) && j + k < a.o.n) v[k] = sum_again<T>(a, i, j + k);
+        for (int k = 0; k < 8; k++) v[k] = k == at ? s : v[k];
+        bad &= bad - 1;
+    }
 }
 
 // (ADD: groups of waves hold parts of every sum; otherwise each group has whole ones of its share of the blocks.)
@@ -253,7 +259,7 @@ __device__ inline void tile_out(const LinTile& a, f32x16 (&acc)[MT][NT], char* l
                 *reinterpret_cast<f32x4*>(to + 4) = v1;
             } else {
                 float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-                if constexpr (TWO) make_sums_again<T>(a, gi, gj, v);
+                if constexpr (TWO || sizeof(T) == 4) make_sums_again<T>(a, gi, gj, v);
                 finish8<T>(a.o, gi, gj, v);
             }
         }
@@ -304,7 +310,8 @@ __device__ inline void one_tile(const LinTile& a, uint32_t block, char* lds) {
     const int mrows = (int)min((uint32_t)BM, m - row), ncols = (int)min((uint32_t)BN, n - col);
     ATile ta;
     BTile tb;
-    const char *pa = (const char*)a.a + (TWO ? a.second : 0), *pb = (const char*)a.b;
+    const char *pa = (const char*)a.a, *pb = (const char*)a.b;
+    if constexpr (TWO) pa += a.second;
     if constexpr (ACOL) ta.init((const T*)(pa + (uint64_t)s0 * KE * a.a_pitch) + row, a.a_pitch, (mrows + 7) / 8 * 8, wave, lane);
     else ta.init((const T*)(pa + (uint64_t)row * a.a_pitch) + (uint64_t)s0 * KE, a.a_pitch, mrows, wave, lane);
     if constexpr (BCOL) tb.init((const T*)(pb + (uint64_t)s0 * KE * a.b_pitch) + col, a.b_pitch, (ncols + 7) / 8 * 8, wave, lane);
@@ -313,8 +320,12 @@ __device__ inline void one_tile(const LinTile& a, uint32_t block, char* lds) {
     const int inner = (int)min(stages * KE, a.k - s0 * KE); // a row's values are followed by zeros up to a multiple of eight
     int left = inner;
     uint32_t into = 0;
-    const uint64_t first_a = uniform64(ta.base - a.second), first_b = tb.base;
-    int more = 1;
+    [[maybe_unused]] uint64_t first_a = 0, first_b = 0;
+    if constexpr (TWO) {
+        first_a = uniform64(ta.base - a.second);
+        first_b = tb.base;
+    }
+    [[maybe_unused]] int more = 1;
     auto issue = [&]() {
         const auto one = [&](auto& t, uint32_t at, auto down) {
             if constexpr (decltype(down)::value) {
@@ -612,7 +623,7 @@ template <typename T> __global__ __launch_bounds__(256) void linear_join(LinTile
             s1 += *reinterpret_cast<const f32x4*>(from + 4);
         }
         float v[8] = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
-        if (a.second) make_sums_again<T>(a, i, j, v);
+        if (sizeof(T) == 4 || a.second) make_sums_again<T>(a, i, j, v);
         finish8<T>(a.o, i, j, v);
     }
 }
@@ -684,8 +695,9 @@ struct LinPacks {
     uint32_t count, groups;
 };
 
-// A thread has eight columns and every fourth row of a strip; one launch for all matrices that a call needs in another form.
-template <typename T> __global__ __launch_bounds__(256) void linear_pack(LinPacks all) {
+// A thread has eight columns and every fourth row of a strip; one launch for all matrices that a call needs in another form. (TWO: one of them in two parts, which takes registers for a wave
+// less a SIMD; without it the rest goes 4 % slower.)
+template <typename T, bool TWO> __global__ __launch_bounds__(256) void linear_pack(LinPacks all) {
     __shared__ float sums[4][512];
     const uint32_t which = all.count > 2 && blockIdx.x >= all.one[2].first ? 2 : all.count > 1 && blockIdx.x >= all.one[1].first ? 1 : 0;
     const LinPack& a = all.one[which];
@@ -706,7 +718,7 @@ template <typename T> __global__ __launch_bounds__(256) void linear_pack(LinPack
 #pragma unroll
             for (int k = 0; k < 8; k++) s[k] += v[k];
             if (!a.dst) continue;
-            if constexpr (sizeof(T) == 2) {
+            if constexpr (TWO) {
                 if (a.second) {
                     float rest[8];
 #pragma unroll
@@ -777,7 +789,14 @@ template <typename T> static void pack(apoe_ctx* ctx, LinPacks& all) {
         all.one[i].first = all.groups;
         all.groups += all.one[i].across * all.one[i].strips;
     }
-    if (all.groups) linear_pack<T><<<all.groups, 256, 0, ctx->stream>>>(all);
+    if (!all.groups) return;
+    if constexpr (sizeof(T) == 2) {
+        if (all.one[0].second) { // gz is the first
+            linear_pack<T, true><<<all.groups, 256, 0, ctx->stream>>>(all);
+            return;
+        }
+    }
+    linear_pack<T, false><<<all.groups, 256, 0, ctx->stream>>>(all);
 }
 
 struct LinShape {
