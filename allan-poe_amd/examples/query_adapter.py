@@ -85,7 +85,7 @@ class MlpAdapter:
     """The layer's parameters (float32 masters and copies in `dtype` that the products take), its map and one training step. `terms` is the CSR
     of the queries' learned-sparse terms: offsets, term ids, weights."""
 
-    LOSS_SCALE = 1024.0  # gradients travel as float16
+    LOSS_SCALE = 1024.0  # gradients travel as float16; halved when they overflow
     SCALE = 0.1          # of the terms' sum
 
     def __init__(self, ctx, dim=DIM, hidden=2 * DIM, vocab=S.VOCAB, dtype=torch.float16, bits=32, seed=0):
@@ -133,7 +133,10 @@ class MlpAdapter:
 
     def step(self, x, terms, rows, t_off, t_idx, temperature, lr):
         loss, grads = self.gradients(x, terms, rows, t_off, t_idx, temperature)
-        self.opt.step([grads[k] for k in self.params], lr, grad_scale=1 / self.LOSS_SCALE)
+        if torch.stack([torch.isfinite(g).all() for g in grads.values()]).all():
+            self.opt.step([grads[k] for k in self.params], lr, grad_scale=1 / self.LOSS_SCALE)
+        else:  # a moment that is not finite never is again, in 8 bits its whole block
+            self.LOSS_SCALE /= 2
         return loss
 
 
