@@ -487,9 +487,9 @@ typedef struct {
  * grad_x = gz w, grad_w = gz^T x, grad_bias = sum of gz's rows. (The gradient of residual is grad_y; y may be residual itself when the strides are
  * equal.) Sums are 32 bits and rounded once. float matrices are multiplied as three parts of eight bits each, six products: off by 2^-22 of each
  * product of two values at most, and a value below 2^-111, whose last part is below the parts' smallest number, by 2^-133 of the other. gz of 16-bit
- * matrices with GELU or SiLU goes into the two products as two parts of its type, off by their two roundings' product (bfloat16 2^-16 of it, float16 2^-22). A sum
- * of parts that comes out infinite or NaN is formed again, one product after the other, and is then what float products and sums give: infinite where they overflow or an infinity comes in,
- * NaN where infinities meet zeros or each other, whatever the number of rows (a row with an infinity costs a millisecond for every thousand columns of the inner side). Workspace: gz (once or twice), partial sums
+ * matrices with GELU or SiLU goes into the two products as two parts of its type, off by their two roundings' product (bfloat16 2^-16 of it, float16
+ * 2^-22). A sum of parts that comes out NaN is formed again, one product after the other, and is then what float products and sums give: an infinity where they overflow or
+ * one comes in, NaN where it meets a zero or one of the other sign, whatever the number of rows (float 4096 x 4096 x 1024: 0.2 ms, with an infinity in one row 0.4, in every row 29). Workspace: gz (once or twice), partial sums
  * of up to 128 MiB a product where rows and columns are too few to fill the GPU, and copies of matrices whose rows are not whole multiples of 16 bytes (of
  * floats only where that is quicker) or lie further than 4 MiB apart.
  */
