@@ -83,3 +83,17 @@ def test_infinite_operands_beside_two_parts(gpu_ctx, dtype):
         odd = ~torch.isfinite(want)
         assert int(odd.sum()) > 40 and bool((torch.isfinite(have) == ~odd).all()), name
         assert bool((have.isnan() == want.isnan()).all()) and bool((have[odd & ~want.isnan()] == want[odd & ~want.isnan()]).all()), name
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("m,n,k", [(150, 96, 80), (1489, 1477, 299), (60, 72, 5000)])
+def test_parts_of_the_gradient(gpu_ctx, m, n, k, dtype):
+    """Each gradient by itself has the bits that it has with the others."""
+    import torch
+    import apoe
+    g = torch.Generator().manual_seed(6)
+    x, w, gy, pre = matrix(g, m, k, dtype), matrix(g, n, k, dtype), matrix(g, m, n, dtype), matrix(g, m, n, dtype)
+    whole = apoe.linear_grad(gpu_ctx, x, w, gy, act="silu", pre=pre)
+    for name in whole:
+        part = apoe.linear_grad(gpu_ctx, x, w, gy, act="silu", pre=pre, **{key: key == name for key in whole})
+        assert set(part) == {name} and bool((part[name] == whole[name]).all())
