@@ -739,7 +739,7 @@ def gated_residual_grad(ctx, x, h=None, gate=None, scale=None, w_post=None, w_ne
     return out
 
 
-# ---- layers of an adapter or an encoder, and their training ----
+# ---- layers of an adapter, and their training ----
 
 def _wanted(ctx, asked, name, shape, like):
     """The tensor that a gradient goes to: the caller's own (checked), or a new one where True is asked for. None: not wanted."""

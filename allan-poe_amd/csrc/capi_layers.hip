@@ -1,4 +1,4 @@
-// C-ABI entry points of the operators that layers of an adapter or an encoder are built and trained from (include/apoe.h): checks of the
+// C-ABI entry points of the operators that layers of an adapter are built and trained from (include/apoe.h): checks of the
 // arguments, then the launchers. Nothing behind them throws.
 #include <algorithm>
 #include <cmath>

@@ -9,7 +9,7 @@
 // twice their operations (rounded to one, gx and gw would be off by 1.4 times their own rounding). Where tiles are too few for the GPU the inner dimension is cut and a second launch adds the cuts up, in order.
 // Up to 16 rows a kernel of its own streams w once (the serving form).
 // Measured (a library product of 8192 x 8192 x 8192 in bf16 runs at 1470 TFLOP/s, of 8192 x 4096 x 1024 at 1160): 8192 x 4096 x 1024 bf16 73 us (940 TFLOP/s), with GELU and
-// both outputs 99, whose operations cost what the products wait for; 8192 x 1024 x 4096 68 (1010); 4096 x 1024 x 8192, both sides transposed, 76 (900); 8192 x 4096 x
+// both outputs 99, whose operations cost what the products wait for; 8192 x 1024 x 4096 68 (1010), in two parts 131; 4096 x 1024 x 8192, both sides transposed, 76 (900), in two parts 138; 8192 x 4096 x
 // 4096 fp16 237 to 243 (1140), with SiLU 258. The matrix units are busy in 55 % of the cycles at most; stages and ends of tiles are what the rest goes to. Float 4096 x
 // 4096 x 1024 191 us (180 TFLOP/s; the library 153).
 #include <algorithm>

@@ -8,9 +8,9 @@
 // from x, which it reads anyway. Groups walk over rows in strides of the grid, w and b stay in registers, and a row is asked for before the
 // one in front of it is worked on. The vectors' gradients: each group adds up its rows, a workgroup its groups, a second kernel the workgroups, in
 // a fixed order.
-// Measured (a copy of 2 GiB runs at 4.9 TB/s): 65 536 bf16 rows of 1024, forward 49 us for 268 MB (5.4 TB/s), gradient with grad_skip 105 us for 537 MB (5.1), the vectors'
-// sums 5; 10 007 float rows 16 and 24 us (5 TB/s); 262 144 bf16 rows of 256 49 and 119 us; rows of 1001 fp16 values, which begin anywhere: 60 000 of
-// them 75 and 124 us (3.2 and 2.9 TB/s); 64 rows 4 us.
+// Measured (a copy of 2 GiB runs at 4.9 TB/s): 65 536 bf16 rows of 1024, forward 51 us for 268 MB (5.3 TB/s), gradient with grad_skip 106 us for 537 MB (5.1), the vectors'
+// sums 5 to 6; 10 007 float rows 16 and 24 us (5 TB/s); 262 144 bf16 rows of 256 49 and 125 us; rows of 1001 fp16 values, which begin anywhere and end in a value by itself: 60 000 of
+// them 77 and 126 us (3.1 and 2.9 TB/s); 64 rows 4 us.
 #include <algorithm>
 
 #include "apoe_internal.h"

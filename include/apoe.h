@@ -396,7 +396,7 @@ int apoe_gated_residual(apoe_ctx* ctx, const apoe_gated_residual_args* args);
 int apoe_gated_residual_grad(apoe_ctx* ctx, const apoe_gated_residual_args* args);
 
 /*
- * What an adapter with layers of its own, or a small encoder in front of the index, is built and trained from beside these: rows of a table
+ * What an adapter with layers of its own is built and trained from beside these: rows of a table
  * summed up (terms of the learned-sparse path, tokens), layer norm, matrix products with what is done to their results, and the step of
  * all parameters. The rules above hold: the context's stream, device pointers, strides from row to row (0: dense), workspace that the context
  * keeps. Rows may begin at any multiple of their type's size; such as begin at multiples of 16 bytes are read 16 bytes at a time.
@@ -488,9 +488,9 @@ typedef struct {
  * equal.) Sums are 32 bits and rounded once. float matrices are multiplied as three parts of eight bits each, six products: off by 2^-22 of each
  * product of two values at most, and a value below 2^-111, whose last part is below the parts' smallest number, by 2^-133 of the other. gz of 16-bit
  * matrices with GELU or SiLU goes into the two products as two parts of its type, off by their two roundings' product (bfloat16 2^-16 of it, float16
- * 2^-22). A sum of parts that comes out NaN is formed again, one product after the other, and is then what float products and sums give: an infinity where they overflow or
- * one comes in, NaN where it meets a zero or one of the other sign, whatever the number of rows (float 4096 x 4096 x 1024: 0.2 ms, with an infinity in one row 0.4, in every row 29). Workspace: gz (once or twice), partial sums
- * of up to 128 MiB a product where rows and columns are too few to fill the GPU, and copies of matrices whose rows are not whole multiples of 16 bytes (of
+ * 2^-22). A sum of parts that comes out NaN is formed again, one product after the other, and is then what float products and sums give: an infinity
+ * where they overflow or one comes in, NaN where it meets a zero or one of the other sign, whatever the number of rows (float 4096 x 4096 x 1024
+ * 0.2 ms, with an infinity in one row 0.4, in every row 29). Workspace: gz (once or twice), partial sums of up to 128 MiB a product where rows and columns are too few to fill the GPU, and copies of matrices whose rows are not whole multiples of 16 bytes (of
  * floats only where that is quicker) or lie further than 4 MiB apart.
  */
 int apoe_linear(apoe_ctx* ctx, const apoe_linear_args* args);
