@@ -1003,6 +1003,8 @@ class AdamW:
     def t(self):
         """The number of steps taken. (After steps whose number is a tensor it is asked of the GPU, which is waited for.)"""
         if self._on_gpu:
+            if _torch.cuda.is_current_stream_capturing():
+                raise ApoeError("the number of steps taken is the GPU's after steps whose number was a tensor: during a capture give t")
             _torch.cuda.synchronize(self.ctx.device)
             return int(self._taken)
         return self._t

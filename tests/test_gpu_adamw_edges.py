@@ -112,3 +112,30 @@ def test_a_number_without_gradients(gpu_ctx):
     opt.step([None], 0.1)
     assert opt.state()["t"] == opt.t == 10
     opt.close()
+
+
+def test_a_capture_without_a_number_after_one_with(gpu_ctx):
+    """What the GPU counts cannot be asked during a capture: such a step is refused there, and nothing of it is captured."""
+    import torch
+    import apoe
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    ctx = apoe.Context(0, stream=stream)
+    with torch.cuda.stream(stream):
+        p, g = torch.ones(300, device="cuda"), [torch.ones(300, device="cuda")]
+        t, total = torch.full((1,), 1, dtype=torch.int32, device="cuda"), torch.zeros(1, device="cuda")
+        opt = apoe.AdamW(ctx, [p])
+        opt.step(g, 0.1, t=t)
+    stream.synchronize()
+    kept, graph = p.clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(apoe.ApoeError, match="capture"):
+            opt.step(g, 0.1)
+        total.add_(1)
+    for k in range(3):
+        with torch.cuda.stream(stream):
+            graph.replay()
+        stream.synchronize()
+        assert float(total) == k + 1 and bool((p == kept).all()) and opt.t == 1
+    del graph
+    ctx.close()
