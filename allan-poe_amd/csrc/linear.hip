@@ -868,10 +868,11 @@ static uint32_t bias_groups(const LinBias& b, uint32_t threads) { return b.out ?
 template <typename T> static void join(apoe_ctx* ctx, const LinTile& t) {
     if (t.cuts <= 1) return;
     const uint32_t grid = (uint32_t)std::min<uint64_t>(((uint64_t)t.o.m * (t.np / 8) + 255) / 256, 1u << 16);
-    if (sizeof(T) == 4 || t.second) {
+    if constexpr (sizeof(T) == 4) {
         linear_join<T, true><<<grid, 256, 0, ctx->stream>>>(t);
     } else {
-        if constexpr (sizeof(T) == 2) linear_join<T, false><<<grid, 256, 0, ctx->stream>>>(t);
+        if (t.second) linear_join<T, true><<<grid, 256, 0, ctx->stream>>>(t);
+        else linear_join<T, false><<<grid, 256, 0, ctx->stream>>>(t);
     }
 }
 
@@ -893,11 +894,14 @@ template <typename T, typename F> static void with_kind(uint32_t kind, F&& go) {
 
 template <typename T, bool BCOL, bool ONE, int... N> static void start(hipStream_t s, uint32_t threads, const LinTile& t, Numbers<N...>) {
     const uint32_t grid = t.groups + bias_groups(t.bias, threads);
-    if constexpr (sizeof(T) == 2 && BCOL) {
-        if (t.second) linear_tile<T, false, BCOL, true, N...><<<grid, threads, 0, s>>>(t);
-        else linear_tile<T, false, BCOL, false, N...><<<grid, threads, 0, s>>>(t);
-    } else if constexpr (sizeof(T) == 2) linear_tile<T, false, BCOL, false, N...><<<grid, threads, 0, s>>>(t);
-    else linear_tile32<false, BCOL, ONE, N...><<<grid, threads, 0, s>>>(t);
+    if constexpr (sizeof(T) == 4) {
+        linear_tile32<false, BCOL, ONE, N...><<<grid, threads, 0, s>>>(t);
+    } else if constexpr (BCOL) {
+        if (t.second) linear_tile<T, false, true, true, N...><<<grid, threads, 0, s>>>(t);
+        else linear_tile<T, false, true, false, N...><<<grid, threads, 0, s>>>(t);
+    } else {
+        linear_tile<T, false, false, false, N...><<<grid, threads, 0, s>>>(t);
+    }
 }
 template <typename T, bool BCOL, bool ONE = false> static void product(apoe_ctx* ctx, uint32_t kind, const LinTile& t) {
     with_kind<T>(kind, [&](uint32_t threads, auto numbers) { start<T, BCOL, ONE>(ctx->stream, threads, t, numbers); });
@@ -906,10 +910,12 @@ template <typename T, bool BCOL, bool ONE = false> static void product(apoe_ctx*
 
 template <typename T, int... N> static void start_grads(hipStream_t s, uint32_t threads, const LinTile& x, const LinTile& w, Numbers<N...>) {
     const uint32_t grid = x.groups + w.groups + bias_groups(w.bias, threads);
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 4) {
+        linear_grads32<N...><<<grid, threads, 0, s>>>(x, w);
+    } else {
         if (w.second) linear_grads<T, true, N...><<<grid, threads, 0, s>>>(x, w);
         else linear_grads<T, false, N...><<<grid, threads, 0, s>>>(x, w);
-    } else linear_grads32<N...><<<grid, threads, 0, s>>>(x, w);
+    }
 }
 template <typename T> static void grad_products(apoe_ctx* ctx, uint32_t kind, const LinTile& x, const LinTile& w) {
     with_kind<T>(kind, [&](uint32_t threads, auto numbers) { start_grads<T>(ctx->stream, threads, x, w, numbers); });
